@@ -1,0 +1,496 @@
+// Sparse attention over the tiles that a cheap score selects for each query (gfx950).
+//
+// The index holds the elementwise smallest and largest key of every tile, so
+//   score(h, m, t) = sum over the query heads of h and over d of max(q_d low_td, q_d high_td)
+// bounds the sum of a query's scores over the tile's keys. As max(q x, q y) is q+ y + q- x for x <= y, with
+// q+ = max(q, 0) and q- = min(q, 0), the sum over the query heads comes before the product: one dot product of
+// 128 elements for each (query, KV head, tile). A query attends to the `blocks` tiles of the highest scores
+// (equal ones: the first), to every tile after the index and to its chunk, in four launches: scores, choice,
+// attention, and a merge where a query's tiles are split over workgroups.
+#include "dkv_rows.h"
+#include "dkv_select.h"
+
+namespace dkv {
+namespace sparse {
+
+using namespace rows;
+
+constexpr int BLOCK = 64;        // tiles of an index block
+constexpr int BLOCK_PIECES = 16;  // 16-byte pieces of a tile's bounds: elements 8 p of low, then of high
+
+// Index layout: [tile / 64][layer][head][16 pieces][64 tiles][8 bf16], so that lanes which hold a tile each read
+// 1 KB of consecutive bytes, and an index that grows keeps its bytes in place.
+__device__ __forceinline__ int64_t piece_at(int block, int layer, int layers, int h, int heads) {
+  return (((int64_t)block * layers + layer) * heads + h) * BLOCK_PIECES * BLOCK;
+}
+
+constexpr int INDEX_TILES = 16;  // tiles of an index workgroup, four a wave
+
+// The bounds of a tile's keys, dequantized. Lane (row / 4, quarter): 16 elements of every 16th row; then halves of
+// the elements change lanes, so that each lane ends with one element's bounds.
+template <int BITS>
+__device__ __forceinline__ void tile_bounds(const UnitRows& u, int lane, float& low, float& high) {
+  float lo[16], hi[16];
+  KeyPiece<BITS> p[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) load_key<BITS>(u, 16 * j + (lane >> 2), lane & 3, p[j]);
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    lo[e] = INFINITY, hi[e] = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float x = BITS == 16 ? (e & 1 ? bf16_hi(p[j].w[e / 2]) : bf16_lo(p[j].w[e / 2]))
+                                 : code_at<BITS>(p[j].w, e) * p[j].as.y + p[j].as.x;
+      lo[e] = fminf(lo[e], x);
+      hi[e] = fmaxf(hi[e], x);
+    }
+  }
+#pragma unroll
+  for (int half = 8, bit = 32; half >= 1; half >>= 1, bit >>= 1) {
+    const bool upper = lane & bit;
+#pragma unroll
+    for (int e = 0; e < half; ++e) {
+      const float give_lo = upper ? lo[e] : lo[e + half], give_hi = upper ? hi[e] : hi[e + half];
+      const float got_lo = __shfl_xor(give_lo, bit, 64), got_hi = __shfl_xor(give_hi, bit, 64);
+      lo[e] = fminf(upper ? lo[e + half] : lo[e], got_lo);
+      hi[e] = fmaxf(upper ? hi[e + half] : hi[e], got_hi);
+    }
+  }
+  low = lo[0], high = hi[0];
+}
+
+__global__ __launch_bounds__(256) void index_kernel(const uint8_t* arena, const dkv_tile* tiles, int tile0, int tile1,
+                                                    int layers, int heads, u32x4* bounds) {
+  __shared__ u32x4 out[BLOCK_PIECES][INDEX_TILES];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int first = (tile0 / INDEX_TILES + blockIdx.x) * INDEX_TILES;
+  const int layer = blockIdx.y / heads, h = blockIdx.y % heads;
+  dkv_attn_args a{};
+  a.arena = arena, a.layer = layer, a.heads = heads;
+  for (int i = wave; i < INDEX_TILES; i += 4) {
+    const int t = first + i;
+    if (t < tile0 || t >= tile1) continue;
+    const UnitRows u = tile_rows(a, tiles[t], INT32_MAX, h);
+    float low, high;
+    if (u.bits == 4) tile_bounds<4>(u, lane, low, high);
+    else if (u.bits == 8) tile_bounds<8>(u, lane, low, high);
+    else tile_bounds<16>(u, lane, low, high);
+    const int d = 16 * (lane & 3) + 8 * (lane >> 5) + 4 * (lane >> 4 & 1) + 2 * (lane >> 3 & 1) + (lane >> 2 & 1);
+    reinterpret_cast<uint16_t*>(&out[d / 8][i])[d % 8] = (uint16_t)f32_to_bf16_rne(low);
+    reinterpret_cast<uint16_t*>(&out[8 + d / 8][i])[d % 8] = (uint16_t)f32_to_bf16_rne(high);
+  }
+  __syncthreads();
+  const int p = threadIdx.x / INDEX_TILES, i = threadIdx.x % INDEX_TILES, t = first + i;
+  if (t >= tile0 && t < tile1) bounds[piece_at(t / BLOCK, layer, layers, h, heads) + p * BLOCK + t % BLOCK] = out[p][i];
+}
+
+// The history a launch sees: the arguments' or the device step's {past, n_tiles, n_indexed}.
+struct Seen {
+  int past, n_tiles, n_indexed, chosen;  // chosen: tiles a query chooses of the indexed ones
+};
+
+__device__ __forceinline__ Seen seen_of(const dkv_attn_args& a, const dkv_sparse& s) {
+  Seen v{a.past, a.n_tiles, s.n_indexed, 0};
+  if (a.step) v = Seen{a.step[0], a.step[1], a.step[2], 0};
+  v.n_indexed = min(min(v.n_indexed, s.n_indexed), v.n_tiles);
+  v.chosen = min(s.blocks, v.n_indexed);
+  return v;
+}
+
+struct SparsePlan {
+  int row_blocks;          // 16-row blocks of a KV head's query heads
+  int most, splits;        // workgroups of a (query, KV head, row block): the cap, and those launched
+  int max_indexed, max_chosen;  // launch bounds
+  int64_t keys, lists, part_o, part_ml, bytes;  // workspace offsets
+};
+
+// Workgroups of a (query, KV head, row block): a unit a wave while the `most` of the launch give room. Replays apply it
+// to the history they find, so they split it as a call over that history does (their launch may hold more).
+__host__ __device__ inline int split_count(int most, int64_t units) {
+  const int64_t want = (units + 3) / 4;
+  return want < 1 ? 1 : want < most ? (int)want : most;
+}
+__device__ __forceinline__ int splits_of(const dkv_attn_args& a, const Seen& v, int most) {
+  return split_count(most, (int64_t)v.chosen + v.n_tiles - v.n_indexed + (a.nq + TILE - 1) / TILE);
+}
+
+constexpr int SCORE_QUERIES = 16;
+
+// Scores of 64 tiles for 16 queries of a KV head, as sortable keys. Each wave takes 32 of the 128 elements, a lane
+// a tile; their sums meet in LDS in a fixed order. In 64 bits, rounded to 32 at the end: the products of bf16 values
+// are exact there and their sums as good as exact, so equal scores tie and no order of summation chooses a tile.
+__global__ __launch_bounds__(256) void score_kernel(dkv_attn_args a, dkv_sparse s, int max_indexed, uint32_t* keys) {
+  __shared__ double query[SCORE_QUERIES][2 * D];  // q+ then q-, as the pieces' high and low
+  __shared__ double part[4][SCORE_QUERIES][BLOCK];
+  const Seen v = seen_of(a, s);
+  const int block = blockIdx.x, h = blockIdx.y, m0 = blockIdx.z * SCORE_QUERIES;
+  if (v.chosen == v.n_indexed || block * BLOCK >= v.n_indexed) return;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, G = a.q_heads / a.heads;
+  const int queries = min(SCORE_QUERIES, a.nq - m0);
+  for (int i = threadIdx.x; i < queries * D; i += 256) {
+    const int m = i / D, d = i % D;
+    double plus = 0, minus = 0;
+    for (int g = 0; g < G; ++g) {
+      const uint16_t* q = static_cast<const uint16_t*>(a.q) + (h * G + g) * a.q_head_stride + (m0 + m) * a.q_tok_stride;
+      const float x = bf16_lo(q[d]);
+      plus += x > 0.f ? x : 0.f;
+      minus += x > 0.f ? 0.f : x;
+    }
+    query[m][d] = minus;  // meets low
+    query[m][D + d] = plus;
+  }
+  const u32x4* from = static_cast<const u32x4*>(s.bounds) + piece_at(block, a.layer, a.layers, h, a.heads) +
+                      4 * wave * BLOCK + lane;
+  double x[32];
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    const u32x4 w = block * BLOCK + lane < v.n_indexed ? from[p * BLOCK] : u32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[8 * p + 2 * j] = bf16_lo(w[j]), x[8 * p + 2 * j + 1] = bf16_hi(w[j]);
+  }
+  __syncthreads();
+  for (int m = 0; m < queries; ++m) {
+    double sum = 0;
+#pragma unroll
+    for (int e = 0; e < 32; ++e) sum = __builtin_fma(query[m][32 * wave + e], x[e], sum);
+    part[wave][m][lane] = sum;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < queries * BLOCK; i += 256) {
+    const int m = i / BLOCK, t = i % BLOCK;
+    if (block * BLOCK + t < v.n_indexed)
+      keys[((int64_t)h * a.nq + m0 + m) * max_indexed + block * BLOCK + t] =
+          order_key((float)(part[0][m][t] + part[1][m][t] + (part[2][m][t] + part[3][m][t])));
+  }
+}
+
+// The chosen tiles of a (query, KV head), in order.
+__global__ __launch_bounds__(256) void choose_kernel(dkv_attn_args a, dkv_sparse s, int max_indexed, int max_chosen,
+                                                     const uint32_t* keys, int32_t* lists) {
+  __shared__ SelectScratch scratch;
+  __shared__ uint32_t sums[4];
+  const Seen v = seen_of(a, s);
+  if (v.chosen == v.n_indexed) return;  // every tile, or none: no list is read
+  const int64_t pair = (int64_t)blockIdx.y * a.nq + blockIdx.x;
+  keys += pair * max_indexed;
+  lists += pair * max_chosen;
+  int ties;
+  const uint32_t at = kth_largest<256>(scratch, v.n_indexed, v.chosen, ties, [&](int i, uint32_t& x) {
+    x = keys[i];
+    return true;
+  });
+  int listed = 0, tied = 0;
+  for (int i0 = 0; i0 < v.n_indexed; i0 += 256) {
+    const int i = i0 + threadIdx.x;
+    const uint32_t x = i < v.n_indexed ? keys[i] : 0u;
+    int n;
+    const bool tie = i < v.n_indexed && x == at;
+    const int rank = tied + block_rank<256>(tie, sums, n);
+    tied += n;
+    const bool take = i < v.n_indexed && (x > at || (tie && rank < ties));
+    const int place = listed + block_rank<256>(take, sums, n);
+    listed += n;
+    if (take) lists[place] = i;
+  }
+}
+
+// A wave's running softmax over its units for 16 query rows: row c's maximum (base 2), this lane's share of its sum
+// and the lane's 16 output elements.
+struct Running {
+  float m, l;
+  f32x4 o[4];
+};
+
+template <int BITS, int PREC>
+__device__ __forceinline__ void attend_unit(const UnitRows& u, const Op (&q)[2], float scale2, int c, int g, Running& r) {
+  KeyPiece<BITS> kp[4];
+  ValuePiece<BITS> vp;
+#pragma unroll
+  for (int b = 0; b < 4; ++b) load_key<BITS>(u, 16 * b + c, g, kp[b]);
+  load_values<BITS>(u, c, g, vp);
+  f32x4 s[4];
+#pragma unroll
+  for (int b = 0; b < 4; ++b) {
+    Op k[Terms<BITS, PREC>::K][2];
+    key_ops<BITS, PREC>(kp[b], k);
+    s[b] = f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int t = Terms<BITS, PREC>::K - 1; t >= 0; --t) s[b] = mfma(k[t][1], q[1], mfma(k[t][0], q[0], s[b]));
+  }
+  const bool whole = u.low == 0 && u.high == TILE;
+  float top = -INFINITY;
+#pragma unroll
+  for (int b = 0; b < 4; ++b)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = 16 * b + 4 * g + i;
+      s[b][i] = whole || (row >= u.low && row < u.high) ? s[b][i] * scale2 : -INFINITY;
+      top = fmaxf(top, s[b][i]);
+    }
+  top = fmaxf(row_max(top), r.m);
+  const float ref = top == -INFINITY ? 0.f : top;  // nothing visible yet: keep the empty state
+  const float alpha = __builtin_amdgcn_exp2f(r.m - ref);
+  r.m = top;
+  float sum = 0;
+  Op p[2][2];  // [term][step]: p as the sum of two bf16 values, so that only V's own terms limit the product
+#pragma unroll
+  for (int b = 0; b < 4; ++b)
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+      const float p0 = __builtin_amdgcn_exp2f(s[b][i] - ref), p1 = __builtin_amdgcn_exp2f(s[b][i + 1] - ref);
+      sum += p0 + p1;
+      uint32_t t[2];
+      split_pair<2>(p0, p1, t);
+      p[0][b / 2].u[2 * (b % 2) + i / 2] = t[0];
+      p[1][b / 2].u[2 * (b % 2) + i / 2] = t[1];
+    }
+  r.l = r.l * alpha + sum;
+#pragma unroll
+  for (int db = 0; db < 4; ++db) {
+    Op v[Terms<BITS, PREC>::V][2];
+    value_ops<BITS, PREC>(u, vp, g, db, whole, v);
+    f32x4 o = r.o[db] * alpha;
+#pragma unroll
+    for (int t = Terms<BITS, PREC>::V - 1; t >= 0; --t)
+#pragma unroll
+      for (int pt = t ? 0 : 1; pt >= 0; --pt)  // the product of both low terms is below the sums' rounding
+        o = mfma(v[t][1], p[pt][1], mfma(v[t][0], p[pt][0], o));
+    r.o[db] = o;
+  }
+}
+
+__device__ __forceinline__ void store4(void* out, int out_dtype, int64_t at, f32x4 x) {
+  if (out_dtype == 1)
+    *reinterpret_cast<f32x4*>(static_cast<float*>(out) + at) = x;
+  else
+    *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(out) + at) = u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
+}
+
+template <int PREC>
+__global__ __launch_bounds__(256) void attend_kernel(dkv_attn_args a, dkv_sparse s, int row_blocks, int most, int max_chosen,
+                                                     const int32_t* lists, float* part_o, float2* part_ml) {
+  __shared__ float ml[4][16][2];
+  __shared__ f32x4 o[4][16][17];  // [wave][row][element / 4], padded
+  const Seen v = seen_of(a, s);
+  const int splits = splits_of(a, v, most);
+  if ((int)blockIdx.x >= splits) return;
+  const int G = a.q_heads / a.heads, h = blockIdx.y / row_blocks, rb = blockIdx.y % row_blocks, m = blockIdx.z;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+  const int heads_here = min(16, G - 16 * rb);
+  const int64_t pair = (int64_t)h * a.nq + m;
+  Op q[2];
+  query_ops(static_cast<const uint16_t*>(a.q) + (h * G + 16 * rb + min(c, heads_here - 1)) * a.q_head_stride + m * a.q_tok_stride,
+            c < heads_here, g, q);
+  Running r;
+  r.m = -INFINITY, r.l = 0.f;
+  for (int db = 0; db < 4; ++db) r.o[db] = f32x4{0, 0, 0, 0};
+  const int start = chunk_seg_start(a, m), tail = v.n_tiles - v.n_indexed;
+  const int piece0 = start / TILE, units = v.chosen + tail + m / TILE - piece0 + 1;
+  const bool listed = v.chosen < v.n_indexed;
+  const float scale2 = a.scale * LOG2E;
+  for (int i = blockIdx.x * 4 + wave; i < units; i += 4 * splits) {
+    UnitRows u;
+    if (i < v.chosen + tail) {
+      const int t = i >= v.chosen ? v.n_indexed + i - v.chosen : listed ? lists[pair * max_chosen + i] : i;
+      u = tile_rows(a, a.tiles[t], v.past, h);
+    } else {
+      const int piece = piece0 + i - v.chosen - tail;
+      u = chunk_rows(a, piece, h);
+      u.low = max(0, start - piece * TILE);
+      u.high = min(TILE, m + 1 - piece * TILE);
+    }
+    const int bits = __builtin_amdgcn_readfirstlane(u.bits);
+    if (bits == 4) attend_unit<4, PREC>(u, q, scale2, c, g, r);
+    else if (bits == 8) attend_unit<8, PREC>(u, q, scale2, c, g, r);
+    else attend_unit<16, PREC>(u, q, scale2, c, g, r);
+  }
+  r.l = row_sum(r.l);
+  if (g == 0) ml[wave][c][0] = r.m, ml[wave][c][1] = r.l;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[wave][c][4 * g + i] = f32x4{r.o[0][i], r.o[1][i], r.o[2][i], r.o[3][i]};
+  __syncthreads();
+  const int row = threadIdx.x >> 4, e4 = threadIdx.x & 15;  // the four waves' rows, four elements a thread
+  if (row >= heads_here) return;
+  float top = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) top = fmaxf(top, ml[w][row][0]);
+  const float ref = top == -INFINITY ? 0.f : top;
+  float l = 0.f;
+  f32x4 x = {0, 0, 0, 0};
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const float f = __builtin_amdgcn_exp2f(ml[w][row][0] - ref);
+    l += f * ml[w][row][1];
+    x += f * o[w][row][e4];
+  }
+  if (gridDim.x == 1) {
+    store4(a.out, a.out_dtype, m * a.out_tok_stride + (h * G + 16 * rb + row) * a.out_head_stride + 4 * e4, x / l);
+  } else {
+    const int64_t at = (pair * splits + blockIdx.x) * G + 16 * rb + row;
+    *reinterpret_cast<f32x4*>(part_o + at * D + 4 * e4) = x;
+    if (e4 == 0) part_ml[at] = make_float2(top, l);
+  }
+}
+
+// Joins a query's splits: 16 lanes an output row, four elements a lane.
+__global__ __launch_bounds__(256) void merge_kernel(dkv_attn_args a, dkv_sparse s, int most, const float* part_o,
+                                                    const float2* part_ml) {
+  const int G = a.q_heads / a.heads, row = blockIdx.x * 16 + (threadIdx.x >> 4), h = blockIdx.y, m = blockIdx.z;
+  if (row >= G) return;
+  const int splits = splits_of(a, seen_of(a, s), most), e4 = threadIdx.x & 15;
+  const int64_t first = ((int64_t)h * a.nq + m) * splits * G + row;
+  float top = -INFINITY;
+  for (int i = e4; i < splits; i += 16) top = fmaxf(top, part_ml[first + (int64_t)i * G].x);
+#pragma unroll
+  for (int d = 8; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 16));
+  float l = 0.f;
+  f32x4 x = {0, 0, 0, 0};
+#pragma unroll 4
+  for (int i = 0; i < splits; ++i) {
+    const float2 p = part_ml[first + (int64_t)i * G];
+    const float f = __builtin_amdgcn_exp2f(p.x - top);
+    l += f * p.y;
+    x += f * *reinterpret_cast<const f32x4*>(part_o + (first + (int64_t)i * G) * D + 4 * e4);
+  }
+  store4(a.out, a.out_dtype, m * a.out_tok_stride + (h * G + row) * a.out_head_stride + 4 * e4, x / l);
+}
+
+constexpr int WORKGROUPS = 512;  // attention workgroups that a call is split into
+
+static SparsePlan plan_of(const dkv_attn_args& a, const dkv_sparse& s) {
+  SparsePlan p{};
+  const int G = a.q_heads / a.heads;
+  p.row_blocks = (G + 15) / 16;
+  p.max_indexed = s.n_indexed < a.n_tiles ? s.n_indexed : a.n_tiles;
+  p.max_chosen = s.blocks < p.max_indexed ? s.blocks : p.max_indexed;
+  const int64_t pairs = (int64_t)a.heads * a.nq;
+  const int64_t units = p.max_chosen + (a.n_tiles - p.max_indexed) + (a.nq + TILE - 1) / TILE;
+  const int64_t most = WORKGROUPS / (pairs * p.row_blocks);
+  p.most = most < 1 ? 1 : (int)most;
+  p.splits = split_count(p.most, units);
+  auto up = [](int64_t x) { return (x + 255) & ~(int64_t)255; };
+  const int64_t choosing = p.max_chosen < p.max_indexed || a.step;
+  p.keys = 0;
+  p.lists = p.keys + (choosing ? up(4 * pairs * p.max_indexed) : 0);
+  p.part_o = p.lists + (choosing ? up(4 * pairs * p.max_chosen) : 0);
+  const int64_t parts = p.splits > 1 ? pairs * p.splits * G : 0;
+  p.part_ml = p.part_o + up(4 * D * parts);
+  p.bytes = p.part_ml + up(8 * parts);
+  return p;
+}
+
+}  // namespace sparse
+
+// What the sparse-attention and attention-mass calls ask of their arguments; `what` names the call.
+int check_history_args(const dkv_attn_args& a, const char* what) {
+  auto a16 = [](const void* p) { return ((uintptr_t)p & 15) == 0; };
+  if (!a.q || !a.k_new || (a.n_tiles > 0 && (!a.tiles || !a.arena))) {
+    set_error("%s: null pointer argument", what);
+  } else if (a.heads <= 0 || a.q_heads <= 0 || a.q_heads % a.heads || a.nq <= 0 || a.past < 0 || a.n_tiles < 0 || a.layer < 0 ||
+             a.layer >= a.layers || a.heads > 65535 / ((a.q_heads / a.heads + 15) / 16)) {
+    set_error("%s: bad shape (heads %d, q_heads %d, nq %d, past %d, layer %d/%d)", what, a.heads, a.q_heads, a.nq, a.past,
+              a.layer, a.layers);
+  } else if (a.n_segs < 0 || a.n_segs > DKV_MAX_CHUNK_SEGS) {
+    set_error("%s: n_segs %d outside [0, %d]", what, a.n_segs, DKV_MAX_CHUNK_SEGS);
+  } else if (a.precision < 0 || a.precision > 1) {
+    set_error("%s: precision must be 0 (bf16) or 1 (fp32)", what);
+  } else if (!a16(a.q) || !a16(a.k_new) || (a.q_head_stride & 7) || (a.q_tok_stride & 7) || (a.kn_head_stride & 7) ||
+             (a.kn_tok_stride & 7)) {
+    set_error("%s: Q and K must be 16-byte aligned with strides that are multiples of 8 elements", what);
+  } else {
+    if (a.n_segs <= 1) return 0;
+    bool ok = a.seg_bounds[0] == 0 && a.seg_bounds[a.n_segs] == a.nq;
+    for (int s = 0; s < a.n_segs; ++s) ok = ok && a.seg_bounds[s + 1] > a.seg_bounds[s];
+    if (ok) return 0;
+    set_error("%s: segment bounds must increase from 0 to nq", what);
+  }
+  return DKV_EINVAL;
+}
+
+}  // namespace dkv
+
+using namespace dkv;
+using namespace dkv::sparse;
+
+extern "C" {
+
+int64_t dkv_index_bytes(int32_t n_tiles, int32_t layers, int32_t heads) {
+  if (n_tiles < 0 || layers <= 0 || heads <= 0) return 0;
+  return ((int64_t)n_tiles + BLOCK - 1) / BLOCK * layers * heads * BLOCK_PIECES * BLOCK * 16;
+}
+
+int dkv_index(const void* arena, const dkv_tile* tiles, int32_t tile0, int32_t n_tiles, int32_t layers, int32_t heads,
+              void* bounds, void* stream) {
+  clear_error();
+  if (tile0 < 0 || n_tiles < tile0 || layers <= 0 || heads <= 0 || (int64_t)layers * heads > 65535) {
+    set_error("dkv_index: bad range (tiles [%d, %d), layers %d, heads %d)", tile0, n_tiles, layers, heads);
+    return DKV_EINVAL;
+  }
+  if (n_tiles == tile0) return 0;
+  if (!arena || !tiles || !bounds || ((uintptr_t)bounds & 15)) {
+    set_error("dkv_index: null or misaligned pointer argument");
+    return DKV_EINVAL;
+  }
+  const int groups = (n_tiles + INDEX_TILES - 1) / INDEX_TILES - tile0 / INDEX_TILES;
+  hipLaunchKernelGGL(index_kernel, dim3(groups, layers * heads), dim3(256), 0, (hipStream_t)stream,
+                     static_cast<const uint8_t*>(arena), tiles, tile0, n_tiles, layers, heads, static_cast<u32x4*>(bounds));
+  return (int)hipGetLastError();
+}
+
+int64_t dkv_attend_sparse_workspace_bytes(const dkv_attn_args* args, const dkv_sparse* sparse) {
+  if (!args || !sparse || args->heads <= 0 || args->q_heads <= 0 || args->q_heads % args->heads || args->nq <= 0 ||
+      args->n_tiles < 0 || sparse->n_indexed < 0 || sparse->blocks < 0)
+    return 0;
+  return plan_of(*args, *sparse).bytes;
+}
+
+int dkv_attend_sparse(const dkv_attn_args* args, const dkv_sparse* sparse, void* stream) {
+  clear_error();
+  if (!args || !sparse) {
+    set_error("dkv_attend_sparse: null args");
+    return DKV_EINVAL;
+  }
+  const dkv_attn_args& a = *args;
+  const dkv_sparse& s = *sparse;
+  if (int rc = check_history_args(a, "dkv_attend_sparse")) return rc;
+  if (!a.v_new || !a.out || ((uintptr_t)a.v_new & 15) || ((uintptr_t)a.out & 15) || (a.vn_head_stride & 7) ||
+      (a.vn_tok_stride & 7) || (a.out_tok_stride & 3) || (a.out_head_stride & 3) || a.out_dtype < 0 || a.out_dtype > 1) {
+    set_error("dkv_attend_sparse: V and out must be 16-byte aligned, strides multiples of 8 and 4 elements, out bf16 (0) or fp32 (1)");
+    return DKV_EINVAL;
+  }
+  if (s.n_indexed < 0 || s.blocks < 0 || (s.n_indexed > 0 && (!s.bounds || ((uintptr_t)s.bounds & 15)))) {
+    set_error("dkv_attend_sparse: n_indexed %d and blocks %d must not be negative, bounds 16-byte aligned", s.n_indexed, s.blocks);
+    return DKV_EINVAL;
+  }
+  if (a.nq > 65535) {
+    set_error("dkv_attend_sparse: at most 65535 queries a call, got %d", a.nq);
+    return DKV_EINVAL;
+  }
+  const SparsePlan p = plan_of(a, s);
+  if (p.bytes > 0 && (!a.workspace || a.workspace_bytes < p.bytes)) {
+    set_error("dkv_attend_sparse: workspace of %lld bytes needed, %lld given", (long long)p.bytes, (long long)a.workspace_bytes);
+    return DKV_EINVAL;
+  }
+  const hipStream_t st = (hipStream_t)stream;
+  char* ws = static_cast<char*>(a.workspace);
+  uint32_t* keys = reinterpret_cast<uint32_t*>(ws + p.keys);
+  int32_t* lists = reinterpret_cast<int32_t*>(ws + p.lists);
+  float* part_o = reinterpret_cast<float*>(ws + p.part_o);
+  float2* part_ml = reinterpret_cast<float2*>(ws + p.part_ml);
+  if (p.max_chosen > 0 && (p.max_chosen < p.max_indexed || a.step)) {
+    hipLaunchKernelGGL(score_kernel, dim3((p.max_indexed + BLOCK - 1) / BLOCK, a.heads, (a.nq + SCORE_QUERIES - 1) / SCORE_QUERIES),
+                       dim3(256), 0, st, a, s, p.max_indexed, keys);
+    hipLaunchKernelGGL(choose_kernel, dim3(a.nq, a.heads), dim3(256), 0, st, a, s, p.max_indexed, p.max_chosen, keys, lists);
+  }
+  const dim3 grid(p.splits, a.heads * p.row_blocks, a.nq);
+  if (a.precision == 1)
+    hipLaunchKernelGGL(attend_kernel<1>, grid, dim3(256), 0, st, a, s, p.row_blocks, p.most, p.max_chosen, lists, part_o, part_ml);
+  else
+    hipLaunchKernelGGL(attend_kernel<0>, grid, dim3(256), 0, st, a, s, p.row_blocks, p.most, p.max_chosen, lists, part_o, part_ml);
+  if (p.splits > 1)
+    hipLaunchKernelGGL(merge_kernel, dim3((a.q_heads / a.heads + 15) / 16, a.heads, a.nq), dim3(256), 0, st, a, s, p.most,
+                       part_o, part_ml);
+  return (int)hipGetLastError();
+}
+
+}  // extern "C"

@@ -60,6 +60,10 @@ class SegmentIO(ctypes.Structure):
                 ('write_tiles', ctypes.c_int32)]
 
 
+class Sparse(ctypes.Structure):
+    _fields_ = [('bounds', ctypes.c_void_p), ('n_indexed', ctypes.c_int32), ('blocks', ctypes.c_int32)]
+
+
 assert ctypes.sizeof(Tile) == 16
 
 
@@ -146,6 +150,11 @@ SIGNATURES = [
                                     ctypes.c_int64, ctypes.c_int32, ctypes.c_int32, ctypes.c_float, ctypes.c_void_p]),
     ('dkv_silu_mul', ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64,
                                     ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p]),
+    ('dkv_index_bytes', ctypes.c_int64, [ctypes.c_int32, ctypes.c_int32, ctypes.c_int32]),
+    ('dkv_index', ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
+                                 ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p]),
+    ('dkv_attend_sparse_workspace_bytes', ctypes.c_int64, [ctypes.c_void_p, ctypes.POINTER(Sparse)]),
+    ('dkv_attend_sparse', ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(Sparse), ctypes.c_void_p]),
 ]
 
 

@@ -121,6 +121,7 @@ class GPUCache(_CacheBase):
         # attend() calls of path 'auto' take the kernels graph replays take: long chunks run the
         # frame-chunk kernel, as launches with a step pair do (forwards that also run as replays)
         self.as_replayed = False
+        self.sparse_blocks = 0  # tiles a query of attend() chooses of the indexed history (0: attends to all)
         self.online = plan is None
         self.plan = []  # (start, end, bits, row) per segment, as in the reference
         self.segments = []
@@ -152,6 +153,8 @@ class GPUCache(_CacheBase):
         self._workspace = None  # the last call's workspace, up to WORKSPACE_KEPT bytes (_workspace_for)
         self._graph = None  # GraphSteps while launches read their step parameters from the device
         self._fused_args, self._fused_key = None, None  # the argument block _fused_attention() reuses
+        self.n_indexed = 0  # tiles in the index of index()
+        self._bounds = None  # the index (dkv_index), room for whole blocks of tiles; allocated by index()
         for bits, n in planned:
             if n:
                 self._open_segment(self.segments[-1].end if self.segments else 0, n, bits)
@@ -568,7 +571,8 @@ class GPUCache(_CacheBase):
         if len(shape) != 4 or shape[0] != 1 or shape[3] != d or shape[1] % heads:
             raise ValueError('attend expects q [1, q_heads, n, 64] with q_heads a multiple of heads')
         _, q_heads, n, _ = shape
-        if path == 0 and self.as_replayed and q_heads // heads * n > SMALL_ROWS:
+        auto = path == 0
+        if auto and self.as_replayed and q_heads // heads * n > SMALL_ROWS:
             path = PATHS['mfma']
         if k.shape != (1, heads, n, d) or v.shape != k.shape:
             raise ValueError(f'attend expects the chunk k, v of shape [1, {heads}, {n}, {d}]')
@@ -581,6 +585,8 @@ class GPUCache(_CacheBase):
             segments = self.chunk_segments
         if segments is not None and (segments[0] != 0 or segments[-1] != n):
             raise ValueError(f'chunk segments {segments} do not cover the {n}-token chunk')
+        if self.sparse_blocks and auto and not splits:
+            return self.attend_sparse(q, k, v, layer, past, self.sparse_blocks, out_dtype, segments, precision)
         if splits == 0 and q_heads // heads * n > SHORT_ROWS:
             splits = self.chunk_splits
         out_dtype = out_dtype or q.dtype
@@ -618,6 +624,119 @@ class GPUCache(_CacheBase):
             rc = lib.dkv_attend(a, _lib.raw_stream(self.device))
         if rc:
             _lib.check(rc, 'dkv_attend')
+        return out
+
+    # -- sparse attention over long histories (no reference counterpart) -------
+    def _call(self, name, *args):
+        """One C entry point on this cache's device and torch's current stream there."""
+        index = self.arena.get_device()
+        fn = getattr(_lib.load(), name)
+        if torch.cuda.current_device() == index:
+            rc = fn(*args, _lib.raw_stream(index))
+        else:
+            with torch.cuda.device(index):
+                rc = fn(*args, _lib.raw_stream(index))
+        if rc:
+            _lib.check(rc, name)
+
+    def index(self, first=None):
+        """Brings the index of the history up to date: the elementwise smallest and largest key of every
+        filled tile, which attend_sparse() scores. One launch over all layers, which must be level; tiles
+        indexed before are kept (from tile `first` on they are indexed again). Tokens appended later are
+        not in the index until the next call: every query attends to them. Returns the tiles indexed."""
+        if self._graph is not None:
+            raise ValueError('index() cannot run in graph steps')
+        if len(set(self.seen)) != 1:
+            raise ValueError('index: every layer must be at the same length')
+        first = self.n_indexed if first is None else first
+        if not 0 <= first <= self.n_indexed:
+            raise ValueError(f'index: first must be within the {self.n_indexed} tiles indexed so far')
+        n = self._tiles_before(self.seen[0])
+        if n and int(self.tiles_host[n - 1]['token_start']) + int(self.tiles_host[n - 1]['rows']) > self.seen[0]:
+            n -= 1  # a planned tile that still fills up
+        n = max(n, self.n_indexed)
+        need = _lib.load().dkv_index_bytes(n, self.layers, self.heads)
+        if self._bounds is None or self._bounds.numel() < need:
+            old, used = self._bounds, _lib.load().dkv_index_bytes(self.n_indexed, self.layers, self.heads)
+            room = min(n + n // 2, self.tiles.shape[0])
+            with torch.inference_mode(False):
+                self._bounds = torch.empty(_lib.load().dkv_index_bytes(max(room, n), self.layers, self.heads),
+                                           dtype=torch.uint8, device=self.device)
+                if used:
+                    self._bounds[:used].copy_(old[:used])
+        if n > first:
+            self._call('dkv_index', self.arena.data_ptr(), self.tiles.data_ptr(), first, n, self.layers, self.heads,
+                       self._bounds.data_ptr())
+        self.n_indexed = n
+        return n
+
+    def tile_bounds(self):
+        """The index as (smallest, largest) keys, each [n_indexed, layers, heads, 64] bf16 (copies)."""
+        n, L, H, d = self.n_indexed, self.layers, self.heads, self.dim
+        if not n:
+            return tuple(self.arena.new_empty((0, L, H, d), dtype=torch.bfloat16) for _ in range(2))
+        blocks = -(-n // TILE)
+        x = self._bounds[:_lib.load().dkv_index_bytes(n, L, H)].view(torch.bfloat16)
+        x = x.view(blocks, L, H, 2, d // 8, TILE, 8).permute(3, 0, 5, 1, 2, 4, 6).reshape(2, blocks * TILE, L, H, d)
+        return x[0, :n], x[1, :n]
+
+    def _chunk(self, what, q, k, layer, past, segments, precision, v=None):
+        """The checks that the calls over a chunk share; (q, k, v) as the kernels read them, segments and
+        precision as the call uses them."""
+        precision = self.precision if precision is None else precision
+        if precision not in PRECISIONS:
+            raise ValueError(f'precision must be one of {sorted(PRECISIONS)}')
+        H, d = self.heads, self.dim
+        if q.dim() != 4 or q.shape[0] != 1 or q.shape[3] != d or q.shape[1] % H or not q.shape[1]:
+            raise ValueError(f'{what} expects q [1, q_heads, n, {d}] with q_heads a multiple of heads')
+        n = q.shape[2]
+        if k.shape != (1, H, n, d) or (v is not None and v.shape != k.shape):
+            raise ValueError(f'{what} expects the chunk of shape [1, {H}, {n}, {d}]')
+        if not 0 <= layer < self.layers:
+            raise ValueError(f'{what}: layer {layer} of {self.layers}')
+        if past < 0 or past + n > self.capacity or past > self.seen[layer]:
+            raise ValueError(f'{what}: history longer than the cache holds')
+        index = self.arena.get_device()
+        if not self.arena.is_cuda or any(t is not None and t.get_device() != index for t in (q, k, v)):
+            raise ValueError(f'{what} requires CUDA tensors on the device of the cache')
+        if segments is None:
+            segments = self.chunk_segments
+        if segments is not None and (segments[0] != 0 or segments[-1] != n):
+            raise ValueError(f'chunk segments {segments} do not cover the {n}-token chunk')
+        return self._kv_view(q), self._kv_view(k), None if v is None else self._kv_view(v), segments, precision
+
+    def _chunk_args(self, q, k, v, layer, past, out, segments, precision):
+        """attend_args() of a call over a chunk: of the recorded step in graph steps."""
+        make = self if self._graph is None else self._graph
+        if make is self:
+            return self.attend_args(q, k, v, layer, past, out, segments, 0, 0, precision)
+        return make.attend_args(q, k, v, layer, out, segments, 0, 0, precision)
+
+    def attend_sparse(self, q, k, v, layer, past, blocks, out_dtype=None, segments=None, precision=None):
+        """attend() over a part of a long history: each query attends to the `blocks` tiles of the index
+        (index()) whose keys can score highest for it, to every token appended after the index, and to its
+        chunk. A tile's score is the sum over the query heads of a KV head of sum_d max(q_d * smallest_d,
+        q_d * largest_d), an upper bound of the sum of their scores over its keys; the query heads of a KV
+        head choose together, equal scores choose the earlier tile. With blocks >= n_indexed every query
+        attends to everything. The other arguments and the result are attend()'s."""
+        if blocks < 0:
+            raise ValueError(f'attend_sparse: blocks must not be negative, got {blocks}')
+        out_dtype = out_dtype or q.dtype
+        _check_dtype(out_dtype, 'attend_sparse output dtype')
+        q, k, v, segments, precision = self._chunk('attend_sparse', q, k, layer, past, segments, precision, v)
+        n, q_heads = q.shape[2], q.shape[1]
+        out = q.new_empty((1, n, q_heads, self.dim), dtype=out_dtype)
+        if not n:
+            return out
+        a = self._chunk_args(q, k, v, layer, past, out, segments, precision)
+        s = _lib.Sparse(0 if self._bounds is None else self._bounds.data_ptr(), self.n_indexed, blocks)
+        if self._graph is not None:
+            s.n_indexed = self._graph.indexed_bound()
+        need = _lib.load().dkv_attend_sparse_workspace_bytes(ctypes.byref(a), ctypes.byref(s))
+        if need:
+            ws = self._graph.workspace(need) if self._graph is not None else self.arena.new_empty(need)
+            a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+        self._call('dkv_attend_sparse', ctypes.byref(a), ctypes.byref(s))
         return out
 
     def materialize(self, layer, out_dtype=None):
@@ -731,6 +850,7 @@ class GPUCache(_CacheBase):
         self.seen = [0] * self.layers
         self.cursors = [0] * self.layers
         self.pending_bits, self.frame_id = 16, -1
+        self.n_indexed = 0
         if self.online:
             self.segments, self.tile_starts, self.plan = [], [], []
             self.host_counts = {4: 0, 8: 0, 16: 0}
@@ -857,7 +977,7 @@ class GraphSteps:
     """Device-side step parameters of one GPUCache for HIP-graph replays.
 
     One device buffer holds a pack job per layer (dkv_pack_batch reads layer l's job) and the
-    {past, n_tiles} pair every attention launch reads (dkv_attn_args.step). step() does the host
+    {past, n_tiles, n_indexed} that attention launches read (dkv_attn_args.step). step() does the host
     bookkeeping of one chunk and uploads the buffer through a ring of pinned host copies, so the
     host can prepare step i+1 while the GPU still runs step i. The K/V pointers of the jobs are
     those append() saw while the graph was captured (they are fixed for a captured graph): a
@@ -871,7 +991,7 @@ class GraphSteps:
         # the buffers the recorded launches address: step() refuses to run once the cache holds others
         self.arena, self.tiles = cache.arena, cache.tiles
         self.job_bytes = ctypes.sizeof(_lib.PackJob)
-        self.nbytes = cache.layers * self.job_bytes + 8
+        self.nbytes = cache.layers * self.job_bytes + 16
         with torch.inference_mode(False):  # ordinary tensors: step() may run inside or outside inference mode
             self.dev = torch.zeros(self.nbytes, dtype=torch.uint8, device=cache.device)
         self.ring = None  # pinned host copies, allocated by the first upload()
@@ -886,6 +1006,7 @@ class GraphSteps:
         self.tiles_bound = cache.tiles.shape[0]
         self.ws = None  # attention workspace of the recorded launches (grow-only)
         self.retired = []  # smaller workspaces handed out before: graphs captured earlier still address them
+        self.bounds = False  # the index that recorded launches of attend_sparse() read (False: none recorded)
 
     def workspace(self, nbytes):
         """The attention workspace graph launches use, at least `nbytes` bytes. A buffer once handed
@@ -904,6 +1025,18 @@ class GraphSteps:
         if c.arena is not self.arena or c.tiles is not self.tiles:
             raise ValueError('the cache no longer holds the arena and tile table these graph steps recorded '
                              '(it grew or was rebuilt): capture again')
+        if self.bounds is not False and c._bounds is not self.bounds:
+            raise ValueError('the cache no longer holds the index these graph steps recorded: capture again')
+
+    def indexed_bound(self):
+        """Most tiles that the recorded launches can find in the index: what its buffer has room for. The
+        buffer is the recorded one from here on."""
+        c = self.cache
+        self.bounds = c._bounds
+        if c._bounds is None:
+            return 0
+        block = _lib.load().dkv_index_bytes(1, c.layers, c.heads)
+        return min(c._bounds.numel() // block * TILE, self.tiles_bound)
 
     def step(self):
         c, n = self.cache, self.chunk
@@ -931,10 +1064,10 @@ class GraphSteps:
 
     def _view(self, host):
         """(jobs, tail) numpy views of a pinned ring buffer: the per-layer PackJob array, then the
-        {past, n_tiles} int32 pair."""
+        int32 values past, n_tiles, n_indexed."""
         raw = host.numpy()
         split = self.cache.layers * self.job_bytes
-        return raw[:split].view(self.JOB), raw[split:split + 8].view(np.int32)
+        return raw[:split].view(self.JOB), raw[split:split + 16].view(np.int32)
 
     def upload(self):
         """Writes the current step's jobs and bounds to the device buffer (async, stream-ordered)."""
@@ -954,7 +1087,7 @@ class GraphSteps:
             write_job_sources(jobs, self.kv)
             self.slot_kv[self.slot] = self.kv_version
         write_step_jobs(jobs, seg, past, n, write)
-        tail[0], tail[1] = past, c._tiles_before(past)
+        tail[0], tail[1], tail[2] = past, c._tiles_before(past), c.n_indexed
         if all(kv is not None for kv in self.kv):
             _lib.check(_lib.load().dkv_pack_validate(host.data_ptr(), c.layers, c.arena_bytes, c.layers, c.heads),
                        'dkv_pack_validate')

@@ -380,6 +380,38 @@ int dkv_rms_norm_tiled(const void* x, int64_t x_row_stride, const void* weight, 
                        int32_t k, float eps, int32_t layout, void* stream);
 int dkv_linear_prenorm(int32_t rows, int32_t n, int32_t k, int32_t epilogue);
 
+/* Sparse attention: a query attends to a part of a long history. No counterpart
+ * in the reference, whose attention reads every key.
+ *
+ * dkv_index: the elementwise smallest and largest key of the tiles
+ * [tile0, n_tiles) of every layer and head, dequantized and rounded to bf16, into
+ * the index `bounds` (dkv_index_bytes(n_tiles, ...) bytes at least, 16-byte
+ * aligned): element d of a tile's bound (side 0 = smallest, 1 = largest) at
+ *   ((((tile / 64 * layers + layer) * heads + head) * 16 + side * 8 + d / 8) * 64
+ *     + tile % 64) * 8 + d % 8
+ * in bf16 values; an index grows in place. NaN keys are passed over. */
+int64_t dkv_index_bytes(int32_t n_tiles, int32_t layers, int32_t heads);
+int dkv_index(const void* arena, const dkv_tile* tiles, int32_t tile0, int32_t n_tiles,
+              int32_t layers, int32_t heads, void* bounds, void* stream);
+
+/* Which of the history's tiles a query attends to. */
+typedef struct dkv_sparse {
+  const void* bounds; /* the index (may be NULL while n_indexed is 0) */
+  int32_t n_indexed;  /* tiles [0, n_indexed) are in the index; those after it are always attended */
+  int32_t blocks;     /* tiles that a query attends to of the indexed ones */
+} dkv_sparse;
+
+/* dkv_attend over the `blocks` tiles of the index with the largest
+ *   sum over the KV head's query heads and d of max(q_d * smallest_d, q_d * largest_d)
+ * for each query and KV head (rounded to fp32; equal ones: the first tiles; NaN
+ * last), every tile after the index, and the chunk. Of args, path, splits and
+ * tiles_host are not read; a step (HIP graph replays) has three elements,
+ * {past, n_tiles, n_indexed}, which must stay within the arguments' values.
+ * `precision` as in dkv_attend, but p is never rounded below 16 bits. With
+ * blocks >= n_indexed the call is dense attention. At most 65535 queries. */
+int64_t dkv_attend_sparse_workspace_bytes(const dkv_attn_args* args, const dkv_sparse* sparse);
+int dkv_attend_sparse(const dkv_attn_args* args, const dkv_sparse* sparse, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
