@@ -1,0 +1,256 @@
+// Eviction (gfx950): a cache's packed rows, less the tokens of the smallest attention mass, into another arena.
+//
+// The segments between the protected ends become one segment a width. Every layer and KV head keeps its own rows of
+// each width, as many as the host says, so the tile table is known before the kernels run and nothing waits for the
+// device: history rows carry no mask and no position of their own, so a tile may hold other tokens in every head.
+// Three launches: where each token lies, with the new tile table; the choice, a radix search for the smallest
+// kept mass per (layer, head, width); and the move, which is bound by memory (each kept row read and written once).
+#include "dkv_select.h"
+
+namespace dkv {
+namespace evict {
+
+constexpr int THREADS = 1024;  // of a choosing workgroup
+
+__device__ __forceinline__ int class_of(const dkv_evict_args& e, int bits) {
+  for (int c = 0; c < e.n_classes; ++c)
+    if (e.class_bits[c] == bits) return c;
+  return 3;  // no token of this width stays
+}
+
+// The middle's tokens kept before class c, and their tiles.
+__host__ __device__ inline int rows_before(const dkv_evict_args& e, int c) {
+  int n = 0;
+  for (int i = 0; i < c; ++i) n += e.class_keep[i];
+  return n;
+}
+__host__ __device__ inline int tiles_before(const dkv_evict_args& e, int c) {
+  int n = 0;
+  for (int i = 0; i < c; ++i) n += (e.class_keep[i] + TILE - 1) / TILE;
+  return n;
+}
+__host__ __device__ inline int64_t bytes_before(const dkv_evict_args& e, int c) {
+  int64_t n = 0;
+  for (int i = 0; i < c; ++i) n = segment_end(n, e.class_keep[i], e.class_bits[i], e.layers, e.heads);
+  return n;
+}
+
+// place[token - lead_tokens]: the middle token's tile and class, tile * 4 + class.
+__global__ __launch_bounds__(256) void map_kernel(dkv_evict_args e, int32_t* place) {
+  const int i = blockIdx.x * 256 + threadIdx.x, mid_tiles = tiles_before(e, e.n_classes);
+  const int tail_tiles = e.n_tiles - e.end_tile;
+  if (i < e.lead_tiles) {
+    e.out_tiles[i] = e.tiles[i];
+  } else if (i < e.lead_tiles + mid_tiles) {
+    int c = e.n_classes - 1, t = i - e.lead_tiles;
+    while (t < tiles_before(e, c)) --c;
+    t -= tiles_before(e, c);
+    dkv_tile d;
+    d.offset = e.lead_bytes + bytes_before(e, c) + t * slab_bytes(TILE, e.class_bits[c], e.layers, e.heads);
+    d.token_start = e.lead_tokens + rows_before(e, c) + t * TILE;
+    d.rows = (uint16_t)min(TILE, e.class_keep[c] - t * TILE);
+    d.bits = (uint8_t)e.class_bits[c];
+    d.reserved = 0;
+    e.out_tiles[i] = d;
+  } else if (i < e.lead_tiles + mid_tiles + tail_tiles) {
+    dkv_tile d = e.tiles[e.end_tile + i - e.lead_tiles - mid_tiles];
+    d.offset += e.lead_bytes + bytes_before(e, e.n_classes) - e.tail_offset;
+    d.token_start += e.lead_tokens + rows_before(e, e.n_classes) - e.end_token;
+    e.out_tiles[i] = d;
+  }
+  // a wave a tile of the middle
+  const int t = e.lead_tiles + blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (t >= e.end_tile) return;
+  const dkv_tile d = e.tiles[t];
+  const int row = threadIdx.x & 63;
+  if (row < d.rows) place[d.token_start + row - e.lead_tokens] = t * 4 + class_of(e, d.bits);
+}
+
+// blockIdx: (layer * heads + head, class). The class's tokens of the largest masses, in token order; equal masses
+// keep the earlier token. Class 0 also lists the protected ends.
+__global__ __launch_bounds__(THREADS) void choose_kernel(dkv_evict_args e, const int32_t* place) {
+  __shared__ SelectScratch scratch;
+  __shared__ uint32_t sums[THREADS / 64];
+  const int lh = blockIdx.x, c = blockIdx.y, n = e.end_token - e.lead_tokens;
+  const int mid = rows_before(e, e.n_classes), tail = e.tokens - e.end_token;
+  const float* mass = e.mass + lh * e.mass_stride;
+  int32_t* kept = e.kept + (int64_t)lh * (e.lead_tokens + mid + tail);
+  float* out = e.out_mass + lh * e.out_mass_stride;
+  if (c == 0) {
+    for (int i = threadIdx.x; i < e.lead_tokens; i += THREADS) kept[i] = i, out[i] = mass[i];
+    for (int i = threadIdx.x; i < tail; i += THREADS)
+      kept[e.lead_tokens + mid + i] = e.end_token + i, out[e.lead_tokens + mid + i] = mass[e.end_token + i];
+    for (int64_t i = e.lead_tokens + mid + tail + threadIdx.x; i < e.out_mass_stride; i += THREADS) out[i] = 0.f;
+  }
+  if (c >= e.n_classes) return;
+  mass += e.lead_tokens;
+  int ties;
+  const uint32_t at = kth_largest<THREADS>(scratch, n, e.class_keep[c], ties, [&](int i, uint32_t& x) {
+    x = order_key(mass[i]);
+    return (place[i] & 3) == c;
+  });
+  int listed = e.lead_tokens + rows_before(e, c), tied = 0;
+  const int end = listed + e.class_keep[c];
+  for (int i0 = 0; i0 < n; i0 += THREADS) {
+    const int i = i0 + threadIdx.x;
+    const bool here = i < n && (place[i] & 3) == c;
+    const float w = here ? mass[i] : 0.f;
+    const uint32_t x = order_key(w);
+    int count;
+    const bool tie = here && x == at;
+    const int rank = tied + block_rank<THREADS>(tie, sums, count);
+    tied += count;
+    const bool take = here && (x > at || (tie && rank < ties));
+    const int to = listed + block_rank<THREADS>(take, sums, count);
+    listed += count;
+    if (take && to < end) kept[to] = e.lead_tokens + i, out[to] = w;
+  }
+}
+
+// One row's 16-byte pieces: 2, 4 or 8 lanes. The rows of K and V of a (new tile, layer, head) move in one wave: lane
+// r first finds where row r lies, then the lanes of a row take its address from it.
+template <int BITS>
+__device__ __forceinline__ void move_rows(const dkv_evict_args& e, const dkv_tile& d, int layer, int h, const int32_t* kept,
+                                          const int32_t* place, int lane) {
+  constexpr int PIECES = BITS / 2, ROWS = 64 / PIECES, STEPS = TILE / ROWS;  // rows an instruction, instructions a tile
+  const int token = kept[min(lane, d.rows - 1)];
+  const dkv_tile from = e.tiles[place[token - e.lead_tokens] >> 2];
+  const int row = token - from.token_start;
+  const int64_t from_sb = subblock_bytes(from.rows, BITS), to_sb = subblock_bytes(d.rows, BITS);
+  const int64_t block = (int64_t)(layer * 2) * e.heads + h;
+  const uint8_t* src = static_cast<const uint8_t*>(e.arena) + from.offset + block * from_sb;
+  uint8_t* dst = static_cast<uint8_t*>(e.out_arena) + d.offset + block * to_sb;
+  const uint64_t k_row = (uint64_t)(src + (int64_t)row * (8 * BITS)), v_gap = (uint64_t)(e.heads * from_sb);
+  u32x4 x[2][STEPS];
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s) {
+    const int r = min(s * ROWS + lane / PIECES, d.rows - 1);
+    const uint64_t at = (uint64_t)(uint32_t)__shfl((int)k_row, r, 64) | (uint64_t)(uint32_t)__shfl((int)(k_row >> 32), r, 64) << 32;
+    const uint64_t gap = (uint64_t)(uint32_t)__shfl((int)v_gap, r, 64) | (uint64_t)(uint32_t)__shfl((int)(v_gap >> 32), r, 64) << 32;
+    x[0][s] = *reinterpret_cast<const u32x4*>(at + lane % PIECES * 16);
+    x[1][s] = *reinterpret_cast<const u32x4*>(at + gap + lane % PIECES * 16);
+  }
+  float2 as[2];
+  if (BITS < 16) {
+    const uint8_t* meta = src + (int64_t)from.rows * (8 * BITS) + 8 * row;
+    as[0] = *reinterpret_cast<const float2*>(meta);
+    as[1] = *reinterpret_cast<const float2*>(meta + v_gap);
+  }
+  const int64_t to_gap = e.heads * to_sb;
+#pragma unroll
+  for (int kv = 0; kv < 2; ++kv) {
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s)
+      if (s * ROWS + lane / PIECES < d.rows) *reinterpret_cast<u32x4*>(dst + kv * to_gap + (s * 64 + lane) * 16) = x[kv][s];
+    if (BITS < 16 && lane < d.rows)
+      *reinterpret_cast<float2*>(dst + kv * to_gap + (int64_t)d.rows * (8 * BITS) + 8 * lane) = as[kv];
+  }
+}
+
+constexpr int COPY_BYTES = 32768;  // of a copying workgroup
+
+// Workgroups [0, gathers): four (layer, head) of a new tile of the middle, a wave each; the rest copy the ends.
+__global__ __launch_bounds__(256) void move_kernel(dkv_evict_args e, int gathers, const int32_t* place) {
+  const int lhs = e.layers * e.heads, per_tile = (lhs + 3) / 4;
+  if ((int)blockIdx.x < gathers) {
+    const int lh = blockIdx.x % per_tile * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (lh >= lhs) return;
+    const dkv_tile d = e.out_tiles[e.lead_tiles + blockIdx.x / per_tile];
+    const int total = e.lead_tokens + rows_before(e, e.n_classes) + e.tokens - e.end_token;
+    const int32_t* kept = e.kept + (int64_t)lh * total + d.token_start;
+    const int bits = __builtin_amdgcn_readfirstlane((int)d.bits);
+    if (bits == 4) move_rows<4>(e, d, lh / e.heads, lh % e.heads, kept, place, lane);
+    else if (bits == 8) move_rows<8>(e, d, lh / e.heads, lh % e.heads, kept, place, lane);
+    else move_rows<16>(e, d, lh / e.heads, lh % e.heads, kept, place, lane);
+    return;
+  }
+  // 16-byte pieces of the leading tiles, which stay where they were, then of the trailing ones
+  const int64_t pieces = (e.lead_bytes + e.tail_bytes) / 16, lead = e.lead_bytes / 16;
+  const u32x4* from = static_cast<const u32x4*>(e.arena);
+  u32x4* to = static_cast<u32x4*>(e.out_arena);
+  const int64_t tail_from = e.tail_offset / 16 - lead, tail_to = bytes_before(e, e.n_classes) / 16;
+  const int64_t first = (int64_t)(blockIdx.x - gathers) * (COPY_BYTES / 16);
+#pragma unroll
+  for (int i = 0; i < COPY_BYTES / 16 / 256; ++i) {
+    const int64_t p = first + i * 256 + threadIdx.x;
+    if (p < pieces) to[p < lead ? p : p + tail_to] = from[p < lead ? p : p + tail_from];
+  }
+}
+
+static bool fits(const dkv_evict_args& e) {
+  if (e.layers <= 0 || e.heads <= 0 || (int64_t)e.layers * e.heads > INT32_MAX / 4 || e.n_tiles < 0 || e.lead_tiles < 0 ||
+      e.end_tile < e.lead_tiles || e.n_tiles < e.end_tile || e.lead_tokens < 0 || e.end_token < e.lead_tokens ||
+      e.tokens < e.end_token || e.n_classes < 0 || e.n_classes > 3 || e.lead_bytes < 0 || e.tail_offset < e.lead_bytes ||
+      e.tail_bytes < 0 || (e.lead_bytes & 15) || (e.tail_offset & 15) || (e.tail_bytes & 15))
+    return false;
+  int64_t kept = 0;
+  for (int c = 0; c < e.n_classes; ++c) {
+    if ((e.class_bits[c] != 4 && e.class_bits[c] != 8 && e.class_bits[c] != 16) || e.class_keep[c] <= 0) return false;
+    for (int i = 0; i < c; ++i)
+      if (e.class_bits[i] == e.class_bits[c]) return false;
+    kept += e.class_keep[c];
+  }
+  const int64_t total = e.lead_tokens + kept + e.tokens - e.end_token;
+  return kept <= e.end_token - e.lead_tokens && e.mass_stride >= e.tokens && e.out_mass_stride >= total &&
+         e.out_arena_bytes >= e.lead_bytes + bytes_before(e, e.n_classes) + e.tail_bytes &&
+         e.arena_bytes >= e.tail_offset + e.tail_bytes;
+}
+
+}  // namespace evict
+}  // namespace dkv
+
+using namespace dkv;
+
+extern "C" {
+
+int64_t dkv_evict_workspace_bytes(const dkv_evict_args* args) {
+  if (!args || args->end_token <= args->lead_tokens) return 0;
+  return 4 * ((int64_t)args->end_token - args->lead_tokens);
+}
+
+int dkv_evict(const dkv_evict_args* args, void* stream) {
+  clear_error();
+  if (!args) {
+    set_error("dkv_evict: null args");
+    return DKV_EINVAL;
+  }
+  const dkv_evict_args& e = *args;
+  if (!evict::fits(e)) {
+    set_error("dkv_evict: bad ranges (tiles %d | %d | %d, tokens %d | %d | %d, widths %d, or rows or arenas too small)",
+              e.lead_tiles, e.end_tile, e.n_tiles, e.lead_tokens, e.end_token, e.tokens, e.n_classes);
+    return DKV_EINVAL;
+  }
+  if (e.n_tiles == 0) return 0;
+  if (!e.arena || !e.tiles || !e.mass || !e.out_arena || !e.out_tiles || !e.out_mass || !e.kept ||
+      ((uintptr_t)e.arena & 15) || ((uintptr_t)e.out_arena & 15)) {
+    set_error("dkv_evict: null or misaligned pointer argument");
+    return DKV_EINVAL;
+  }
+  const uint8_t *from = static_cast<const uint8_t*>(e.arena), *to = static_cast<const uint8_t*>(e.out_arena);
+  if ((from < to + e.out_arena_bytes && to < from + e.arena_bytes) || e.tiles == e.out_tiles || e.mass == e.out_mass) {
+    set_error("dkv_evict: the new arena, tiles and masses must not be the old ones");
+    return DKV_EINVAL;
+  }
+  if (e.workspace_bytes < dkv_evict_workspace_bytes(args) || (!e.workspace && dkv_evict_workspace_bytes(args))) {
+    set_error("dkv_evict: workspace of %lld bytes needed, %lld given", (long long)dkv_evict_workspace_bytes(args),
+              (long long)e.workspace_bytes);
+    return DKV_EINVAL;
+  }
+  int32_t* place = static_cast<int32_t*>(e.workspace);
+  const int mid_tiles = evict::tiles_before(e, e.n_classes), out_tiles = e.lead_tiles + mid_tiles + e.n_tiles - e.end_tile;
+  const int by_tile = (out_tiles + 255) / 256, by_wave = (e.end_tile - e.lead_tiles + 3) / 4, lhs = e.layers * e.heads;
+  const hipStream_t st = (hipStream_t)stream;
+  hipLaunchKernelGGL(evict::map_kernel, dim3(by_tile > by_wave ? by_tile : by_wave), dim3(256), 0, st, e, place);
+  hipLaunchKernelGGL(evict::choose_kernel, dim3(lhs, e.n_classes ? e.n_classes : 1), dim3(evict::THREADS), 0, st, e, place);
+  const int64_t gathers = (int64_t)mid_tiles * ((lhs + 3) / 4);
+  const int64_t copies = (e.lead_bytes + e.tail_bytes + evict::COPY_BYTES - 1) / evict::COPY_BYTES;
+  if (gathers + copies > INT32_MAX) {
+    set_error("dkv_evict: too many rows for one call");
+    return DKV_EINVAL;
+  }
+  if (gathers + copies)
+    hipLaunchKernelGGL(evict::move_kernel, dim3((unsigned)(gathers + copies)), dim3(256), 0, st, e, (int)gathers, place);
+  return (int)hipGetLastError();
+}
+
+}  // extern "C"

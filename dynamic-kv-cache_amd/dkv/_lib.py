@@ -64,6 +64,20 @@ class Sparse(ctypes.Structure):
     _fields_ = [('bounds', ctypes.c_void_p), ('n_indexed', ctypes.c_int32), ('blocks', ctypes.c_int32)]
 
 
+class EvictArgs(ctypes.Structure):
+    _fields_ = [('arena', ctypes.c_void_p), ('arena_bytes', ctypes.c_int64), ('tiles', ctypes.c_void_p),
+                ('n_tiles', ctypes.c_int32), ('tokens', ctypes.c_int32),
+                ('layers', ctypes.c_int32), ('heads', ctypes.c_int32),
+                ('lead_tiles', ctypes.c_int32), ('lead_tokens', ctypes.c_int32),
+                ('end_tile', ctypes.c_int32), ('end_token', ctypes.c_int32),
+                ('lead_bytes', ctypes.c_int64), ('tail_offset', ctypes.c_int64), ('tail_bytes', ctypes.c_int64),
+                ('n_classes', ctypes.c_int32), ('class_bits', ctypes.c_int32 * 3), ('class_keep', ctypes.c_int32 * 3),
+                ('mass', ctypes.c_void_p), ('mass_stride', ctypes.c_int64),
+                ('out_arena', ctypes.c_void_p), ('out_arena_bytes', ctypes.c_int64), ('out_tiles', ctypes.c_void_p),
+                ('out_mass', ctypes.c_void_p), ('out_mass_stride', ctypes.c_int64), ('kept', ctypes.c_void_p),
+                ('workspace', ctypes.c_void_p), ('workspace_bytes', ctypes.c_int64)]
+
+
 assert ctypes.sizeof(Tile) == 16
 
 
@@ -155,6 +169,11 @@ SIGNATURES = [
                                  ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p]),
     ('dkv_attend_sparse_workspace_bytes', ctypes.c_int64, [ctypes.c_void_p, ctypes.POINTER(Sparse)]),
     ('dkv_attend_sparse', ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(Sparse), ctypes.c_void_p]),
+    ('dkv_attention_mass_workspace_bytes', ctypes.c_int64, [ctypes.c_void_p]),
+    ('dkv_attention_mass', ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32,
+                                          ctypes.c_void_p]),
+    ('dkv_evict_workspace_bytes', ctypes.c_int64, [ctypes.POINTER(EvictArgs)]),
+    ('dkv_evict', ctypes.c_int, [ctypes.POINTER(EvictArgs), ctypes.c_void_p]),
 ]
 
 

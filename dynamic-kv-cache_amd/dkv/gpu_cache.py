@@ -155,6 +155,12 @@ class GPUCache(_CacheBase):
         self._fused_args, self._fused_key = None, None  # the argument block _fused_attention() reuses
         self.n_indexed = 0  # tiles in the index of index()
         self._bounds = None  # the index (dkv_index), room for whole blocks of tiles; allocated by index()
+        self.observing = False  # attend() also counts its attention's mass (observe())
+        self.dropped = 0  # tokens evicted so far: the next token's position is get_seq_length() + dropped
+        self.kept = None  # after an eviction into this cache: the old index of every token, [layers, heads, tokens]
+        self._mass = None  # accumulated attention mass [layers, heads, capacity] fp32; allocated by mass()
+        self._mass_shared = False  # a branch reads its base's until it counts for itself
+        self._branch = False  # made by fork(): its storage is its base's
         for bits, n in planned:
             if n:
                 self._open_segment(self.segments[-1].end if self.segments else 0, n, bits)
@@ -585,6 +591,8 @@ class GPUCache(_CacheBase):
             segments = self.chunk_segments
         if segments is not None and (segments[0] != 0 or segments[-1] != n):
             raise ValueError(f'chunk segments {segments} do not cover the {n}-token chunk')
+        if self.observing:
+            self.observe(q, k, layer, past, segments, precision)
         if self.sparse_blocks and auto and not splits:
             return self.attend_sparse(q, k, v, layer, past, self.sparse_blocks, out_dtype, segments, precision)
         if splits == 0 and q_heads // heads * n > SHORT_ROWS:
@@ -739,6 +747,157 @@ class GPUCache(_CacheBase):
         self._call('dkv_attend_sparse', ctypes.byref(a), ctypes.byref(s))
         return out
 
+    # -- attention mass and eviction by it (no reference counterpart) ----------
+    def attention_mass(self, q, k, layer, past, segments=None, precision=None):
+        """What every token receives of a chunk's softmax: the sum over the queries and the query heads of
+        each KV head of the weights that attend() gives it, [heads, past + n] fp32 (history, then chunk)."""
+        if self._graph is not None:
+            raise ValueError('attention_mass() cannot run in graph steps, whose length is not the host\'s: observe()')
+        q, k, _, segments, precision = self._chunk('attention_mass', q, k, layer, past, segments, precision)
+        n = q.shape[2]
+        out = q.new_empty((self.heads, past + n), dtype=torch.float32)
+        if not n:
+            return out.zero_()
+        self._run_mass(q, k, layer, past, segments, precision, out.data_ptr(), out.stride(0), 0)
+        return out
+
+    def observe(self, q, k, layer, past, segments=None, precision=None):
+        """Adds a chunk's attention mass to the cache's (mass()), which evict() goes by. With `observing` set
+        every attend() does."""
+        q, k, _, segments, precision = self._chunk('observe', q, k, layer, past, segments, precision)
+        mass = self._own_mass()
+        if self._graph is not None:
+            self._graph.mass = mass
+        if q.shape[2]:
+            self._run_mass(q, k, layer, past, segments, precision, mass[layer].data_ptr(), self.capacity, 1)
+
+    def _run_mass(self, q, k, layer, past, segments, precision, out, stride, accumulate):
+        a = self._chunk_args(q, k, k, layer, past, q, segments, precision)  # (no values and no output are read)
+        need = _lib.load().dkv_attention_mass_workspace_bytes(ctypes.byref(a))
+        ws = self._graph.workspace(need) if self._graph is not None else self.arena.new_empty(need)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+        self._call('dkv_attention_mass', ctypes.byref(a), out, stride, accumulate)
+
+    def _own_mass(self):
+        if self._mass is None or self._mass_shared:
+            if self.arena.is_cuda and torch.cuda.is_current_stream_capturing():
+                raise ValueError('allocate the masses before the capture: call mass() once')
+            with torch.inference_mode(False):
+                self._mass = (self._mass.clone() if self._mass is not None else
+                              torch.zeros((self.layers, self.heads, self.capacity), dtype=torch.float32, device=self.device))
+            self._mass_shared = False
+        return self._mass
+
+    def _clear_mass(self):
+        if self._mass is not None:
+            if self._mass_shared:
+                self._mass, self._mass_shared = None, False
+            else:
+                self._mass.zero_()
+
+    def mass(self):
+        """The attention mass accumulated so far, [layers, heads, tokens] fp32: a view that may be written
+        (a branch gets its own). Tokens start at zero."""
+        return self._own_mass()[:, :, :self.seen[0]]
+
+    def _eviction(self, keep, sinks, recent):
+        """(first segment, one past the last, {width: tokens kept}) of an eviction: the segments between the
+        protected ends, and their `keep` less the ends' tokens shared among the widths they have, in
+        proportion to what each holds (largest remainders, the wider one first)."""
+        n, segs = self.seen[0], self.segments
+        a, b = 0, len(segs)
+        while a < b and segs[a].start < sinks:
+            a += 1
+        while b > a and segs[b - 1].end > n - recent:
+            b -= 1
+        if keep >= n:
+            return len(segs), len(segs), {}
+        held = {}
+        for seg in segs[a:b]:
+            held[seg.bits] = held.get(seg.bits, 0) + seg.rows
+        total = sum(held.values())
+        left = keep - (n - total)
+        if left < 0:
+            raise ValueError(f'evict: {n - total} tokens are protected (whole segments), more than the {keep} to keep')
+        share = {w: left * m // total for w, m in held.items()}
+        for w in sorted(held, key=lambda w: (-(left * held[w] % total), -w))[:left - sum(share.values())]:
+            share[w] += 1
+        return a, b, {w: m for w, m in share.items() if m}
+
+    def evict(self, keep, sinks=0, recent=0, into=None):
+        """The `keep` tokens of this cache that matter, as another cache: `into` (an online cache of the same
+        shape, emptied first as by reset(), so its branches end; not a branch itself), or a new one.
+
+        The segments that hold the first `sinks` or the last `recent` tokens stay whole. Of those between,
+        every layer and KV head keeps the tokens of the largest accumulated mass (mass(); equal masses: the
+        earlier token), as one segment a width, in token order; how many of each width follows from what
+        the segments hold. So layers and heads keep different tokens, `into.kept` says which, and the rows
+        are moved as they are packed. This cache, its branches and its graph steps are not touched;
+        graph steps of `into` go on over what it holds now. Nothing waits for the GPU. `into.dropped` counts
+        the tokens evicted so far. The index of the new cache is empty."""
+        if not self.online or self._graph is not None:
+            raise ValueError('evict needs an online cache (no plan) outside graph steps')
+        n = self.seen[0]
+        if len(set(self.seen)) != 1 or (self.segments[-1].end if self.segments else 0) != n:
+            raise ValueError('evict: every layer must be at the same length')
+        if keep < 0 or sinks < 0 or recent < 0:
+            raise ValueError('evict: keep, sinks and recent must not be negative')
+        if self._mass is None:
+            raise ValueError('evict: no attention mass has been counted (observe(), observing or mass())')
+        a, b, share = self._eviction(keep, sinks, recent)
+        if into is None:
+            into = GPUCache(None, self.layers, self.heads, self.dim, self.arena.device, self.dtype, self.backend,
+                            self.block_m, self.block_n, self.capacity, precision=self.precision)
+        if (not isinstance(into, GPUCache) or not into.online or into._graph is not None or into._branch
+                or (into.layers, into.heads, into.dim) != (self.layers, self.heads, self.dim)
+                or into.arena.device != self.arena.device):
+            raise ValueError('evict: into must be an online cache of the same layers and heads on the same device, '
+                             'no branch and outside graph steps')
+        if into.arena is self.arena or into.tiles is self.tiles or into._mass is self._mass:
+            raise ValueError('evict: into must not be this cache or share its storage')
+        lead, trail = self.segments[:a], self.segments[b:]
+        lengths = [s.rows for s in lead] + list(share.values()) + [s.rows for s in trail]
+        bits = [s.bits for s in lead] + list(share) + [s.bits for s in trail]
+        if sum(lengths) > into.capacity or sum(-(-m // TILE) for m in lengths) > into.tiles.shape[0]:
+            raise ValueError('GPU context limit exceeded')
+        mass, into._mass = into._mass, None  # (written below: reset() need not clear it)
+        into.reset()
+        with torch.inference_mode(False):
+            into._mass = torch.empty((into.layers, into.heads, into.capacity), dtype=torch.float32,
+                                     device=into.device) if mass is None else mass
+        kept = self.arena.new_empty((self.layers, self.heads, sum(lengths)), dtype=torch.int32)
+        if lengths:
+            into._open_segments(0, lengths, bits)
+            for new, old in zip(into.segments, lead + [None] * len(share) + trail):
+                if old is not None:
+                    new.frame = old.frame
+            first = self.segments[a] if a < len(self.segments) else None
+            last = self.segments[b] if b < len(self.segments) else None
+            e = _lib.EvictArgs()
+            e.arena, e.arena_bytes, e.tiles = self.arena.data_ptr(), self.arena_bytes, self.tiles.data_ptr()
+            e.n_tiles, e.tokens, e.layers, e.heads = len(self.tile_starts), n, self.layers, self.heads
+            e.lead_tiles, e.lead_tokens = (first.tile0, first.start) if first else (len(self.tile_starts), n)
+            e.end_tile, e.end_token = (last.tile0, last.start) if last else (len(self.tile_starts), n)
+            e.lead_bytes = first.offset if first else self.arena_used
+            e.tail_offset = last.offset if last else self.arena_used
+            e.tail_bytes = self.arena_used - e.tail_offset
+            e.n_classes = len(share)
+            for i, (w, m) in enumerate(share.items()):
+                e.class_bits[i], e.class_keep[i] = w, m
+            e.mass, e.mass_stride = self._mass.data_ptr(), self.capacity
+            e.out_arena, e.out_arena_bytes = into.arena.data_ptr(), into.arena_bytes
+            e.out_tiles, e.out_mass, e.out_mass_stride = into.tiles.data_ptr(), into._mass.data_ptr(), into.capacity
+            e.kept = kept.data_ptr()
+            ws = self.arena.new_empty(_lib.load().dkv_evict_workspace_bytes(ctypes.byref(e)))
+            e.workspace, e.workspace_bytes = ws.data_ptr(), ws.numel()
+            self._call('dkv_evict', ctypes.byref(e))
+        else:
+            into._mass.zero_()
+        into.seen = [sum(lengths)] * into.layers
+        into.kept, into.dropped = kept, self.dropped + n - sum(lengths)
+        into.pending_bits, into.frame_id = self.pending_bits, self.frame_id
+        return into
+
     def materialize(self, layer, out_dtype=None):
         """Dequantized history of one layer: (k, v), each [1, H, seen, 64] (src/gpu_cache.py:106-112)."""
         n = self.seen[layer]
@@ -777,6 +936,8 @@ class GPUCache(_CacheBase):
         other.host_counts = self.host_counts.copy()
         other._workspace = None
         other._graph = None
+        other._mass_shared, other._branch = self._mass is not None, True
+        other.observing = False
         other._fused_args, other._fused_key = None, None
         other.pending_bits = 16
         return other
@@ -850,7 +1011,8 @@ class GPUCache(_CacheBase):
         self.seen = [0] * self.layers
         self.cursors = [0] * self.layers
         self.pending_bits, self.frame_id = 16, -1
-        self.n_indexed = 0
+        self.n_indexed, self.dropped, self.kept = 0, 0, None
+        self._clear_mass()
         if self.online:
             self.segments, self.tile_starts, self.plan = [], [], []
             self.host_counts = {4: 0, 8: 0, 16: 0}
@@ -1006,6 +1168,7 @@ class GraphSteps:
         self.tiles_bound = cache.tiles.shape[0]
         self.ws = None  # attention workspace of the recorded launches (grow-only)
         self.retired = []  # smaller workspaces handed out before: graphs captured earlier still address them
+        self.mass = False  # the masses that recorded launches of observe() add to (False: none recorded)
         self.bounds = False  # the index that recorded launches of attend_sparse() read (False: none recorded)
 
     def workspace(self, nbytes):
@@ -1027,6 +1190,8 @@ class GraphSteps:
                              '(it grew or was rebuilt): capture again')
         if self.bounds is not False and c._bounds is not self.bounds:
             raise ValueError('the cache no longer holds the index these graph steps recorded: capture again')
+        if self.mass is not False and c._mass is not self.mass:
+            raise ValueError('the cache no longer holds the masses these graph steps recorded: capture again')
 
     def indexed_bound(self):
         """Most tiles that the recorded launches can find in the index: what its buffer has room for. The

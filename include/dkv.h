@@ -412,6 +412,53 @@ typedef struct dkv_sparse {
 int64_t dkv_attend_sparse_workspace_bytes(const dkv_attn_args* args, const dkv_sparse* sparse);
 int dkv_attend_sparse(const dkv_attn_args* args, const dkv_sparse* sparse, void* stream);
 
+/* Attention mass: mass[h * mass_head_stride + t] = (accumulate: += ) the sum over
+ * the query heads of KV head h and the chunk's queries of the softmax weight that
+ * dkv_attend gives history token t < past, or chunk token t - past (bf16 rounding
+ * of the keys by `precision`, everything after in fp32). What eviction by
+ * accumulated attention goes by; no counterpart in the reference. v_new, out,
+ * path, splits and tiles_host of args are not read; a step bounds the launch as in
+ * dkv_attend. Masses past past + nq are not written, and sums do not depend on
+ * the order in which workgroups run. */
+int64_t dkv_attention_mass_workspace_bytes(const dkv_attn_args* args);
+int dkv_attention_mass(const dkv_attn_args* args, float* mass, int64_t mass_head_stride,
+                       int32_t accumulate, void* stream);
+
+/* Eviction: the packed rows of one cache, less some tokens, into another arena.
+ * Tiles [0, lead_tiles) (tokens [0, lead_tokens), bytes [0, lead_bytes)) and
+ * [end_tile, n_tiles) (tokens [end_token, tokens), tail_bytes bytes at
+ * tail_offset) are copied whole. Of the tiles between, every layer and KV head
+ * keeps the class_keep[c] tokens at class_bits[c] bits of the largest mass (equal
+ * ones: the first; NaN last), in token order, as one segment a width in the order
+ * of the classes; widths that no class names are dropped. At least class_keep[c]
+ * tokens of that width must be there. The new tiles start at byte 0 of out_arena;
+ * out_tiles and out_mass (zeros after the kept tokens) are written to match, and
+ * kept [layers, heads, new tokens] gets the old index of every new token. */
+typedef struct dkv_evict_args {
+  const void* arena;
+  int64_t arena_bytes;
+  const dkv_tile* tiles;     /* DEVICE table; out_tiles too */
+  int32_t n_tiles, tokens;   /* the history: tiles [0, n_tiles), tokens [0, tokens) */
+  int32_t layers, heads;
+  int32_t lead_tiles, lead_tokens;
+  int32_t end_tile, end_token;
+  int64_t lead_bytes, tail_offset, tail_bytes;
+  int32_t n_classes;         /* 0..3 */
+  int32_t class_bits[3], class_keep[3];
+  const float* mass;         /* [layers * heads] rows of mass_stride */
+  int64_t mass_stride;
+  void* out_arena;           /* must not overlap arena */
+  int64_t out_arena_bytes;
+  dkv_tile* out_tiles;
+  float* out_mass;           /* [layers * heads] rows of out_mass_stride */
+  int64_t out_mass_stride;
+  int32_t* kept;
+  void* workspace;           /* dkv_evict_workspace_bytes */
+  int64_t workspace_bytes;
+} dkv_evict_args;
+int64_t dkv_evict_workspace_bytes(const dkv_evict_args* args);
+int dkv_evict(const dkv_evict_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
