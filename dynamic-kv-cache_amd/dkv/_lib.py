@@ -78,6 +78,12 @@ class EvictArgs(ctypes.Structure):
                 ('workspace', ctypes.c_void_p), ('workspace_bytes', ctypes.c_int64)]
 
 
+class Sampling(ctypes.Structure):
+    _fields_ = [('temperature', ctypes.c_double), ('top_p', ctypes.c_double), ('min_p', ctypes.c_double),
+                ('top_k', ctypes.c_int32), ('temperature_rows', ctypes.c_void_p), ('top_p_rows', ctypes.c_void_p),
+                ('min_p_rows', ctypes.c_void_p), ('top_k_rows', ctypes.c_void_p)]
+
+
 assert ctypes.sizeof(Tile) == 16
 
 
@@ -174,6 +180,9 @@ SIGNATURES = [
                                           ctypes.c_void_p]),
     ('dkv_evict_workspace_bytes', ctypes.c_int64, [ctypes.POINTER(EvictArgs)]),
     ('dkv_evict', ctypes.c_int, [ctypes.POINTER(EvictArgs), ctypes.c_void_p]),
+    ('dkv_sample', ctypes.c_int, [ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32,
+                                  ctypes.c_void_p, ctypes.c_int32, ctypes.POINTER(Sampling), ctypes.c_void_p,
+                                  ctypes.c_void_p]),
 ]
 
 

@@ -17,6 +17,7 @@ residual, gate/up (with post_attention_layernorm) + SiLU*up, down_proj + residua
 Tensors the kernels do not cover (other dtypes, CPU tensors, other shapes)
 take the reference's own torch composition.
 """
+import ctypes
 import functools
 import types
 
@@ -207,6 +208,48 @@ def linear(x, weight, norm=None, eps=1e-6, residual=None, silu_mul=False, weight
     if out_tiled:
         return out
     return out.view(*(x.shape[:-1] if not x_tiled else (rows,)), n_out)
+
+
+def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """Draws a token of each row of logits [..., vocab] (bf16 or fp32) by its random number u [...] in [0, 1)
+    (fp32 or fp64): int64 indices [...], -1 for a row without a token that can be drawn.
+
+    w = exp((logit - max) / temperature). Of the tokens by falling logit (equal ones: the lower index
+    first) the first top_k (0: all), of those the shortest run that holds top_p of their weight, of those
+    the ones with w >= min_p; of the kept tokens the first, by index, up to which their weight exceeds u
+    times its total. Temperature 0 takes the first of the largest logits. Each of the four may be a
+    tensor [...] (fp32, top_k int32) of one value a row: those are not checked (see dkv_sample)."""
+    if not logits.is_cuda or logits.dtype not in (torch.bfloat16, torch.float32) or logits.dim() < 1 or not logits.shape[-1]:
+        raise ValueError('sample expects CUDA logits [..., vocab] in torch.bfloat16 or torch.float32')
+    lead, vocab = logits.shape[:-1], logits.shape[-1]
+    index = logits.get_device()
+    if u.shape != lead or u.get_device() != index or u.dtype not in (torch.float32, torch.float64):
+        raise ValueError(f'sample expects u of shape {tuple(lead)}, torch.float32 or torch.float64, beside the logits')
+    p, keep = _lib.Sampling(1.0, 1.0, 0.0, 0, None, None, None, None), []
+    for name, x, dtype in (('temperature', temperature, torch.float32), ('top_p', top_p, torch.float32),
+                           ('min_p', min_p, torch.float32), ('top_k', top_k, torch.int32)):
+        if isinstance(x, torch.Tensor):
+            if x.shape != lead or x.get_device() != index or x.dtype != dtype:
+                raise ValueError(f'sample expects a {name} tensor of shape {tuple(lead)} and {dtype} beside the logits')
+            x = x.contiguous()
+            keep.append(x)
+            setattr(p, name + '_rows', x.data_ptr())
+        else:
+            setattr(p, name, min(int(x), vocab) if name == 'top_k' else float(x))
+    rows = logits.reshape(-1, vocab)
+    if rows.stride(-1) != 1:
+        rows = rows.contiguous()
+    u = u.contiguous()
+    out = torch.empty(lead, dtype=torch.int64, device=logits.device)
+    args = (rows.data_ptr(), int(logits.dtype == torch.float32), rows.stride(0), rows.shape[0], vocab, u.data_ptr(),
+            int(u.dtype == torch.float64), ctypes.byref(p), out.data_ptr())
+    if torch.cuda.current_device() == index:
+        rc = _lib.load().dkv_sample(*args, _lib.raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = _lib.load().dkv_sample(*args, _lib.raw_stream(index))
+    _lib.check(rc, 'dkv_sample')
+    return out
 
 
 class _LayerPlan:

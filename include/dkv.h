@@ -459,6 +459,31 @@ typedef struct dkv_evict_args {
 int64_t dkv_evict_workspace_bytes(const dkv_evict_args* args);
 int dkv_evict(const dkv_evict_args* args, void* stream);
 
+/* Sampling: out[row] = a token of each row of logits, drawn by the row's random
+ * number u. With w_i = exp((x_i - max) / temperature): of the tokens by falling
+ * logit (equal ones: the lower index first) the first top_k (0: all); of those the
+ * shortest run that holds top_p of their weight; of those the ones with
+ * w_i >= min_p; and of those the first, by index, up to which the weight exceeds
+ * u times their total. Temperature 0: the largest logit, the first of equal ones.
+ * Logits of -infinity and NaN are never drawn; a row of nothing else gives -1. An
+ * infinite logit is drawn before any other. logits: rows of bf16 (dtype 0) or fp32
+ * (1) with a row stride in elements, any alignment of a row that its type has; u:
+ * fp32 (u_dtype 0) or fp64 (1), clamped to [0, 1]. A parameter's *_rows, if not
+ * NULL, gives it for each row (device memory, not checked: a top_p below or above
+ * its range is clamped, a negative top_k is 0, a negative temperature 0). At most
+ * 2^22 tokens. Sums are exact integers: the token does not depend on the order of
+ * any sum. No counterpart in the reference, which scores given answers only. */
+typedef struct dkv_sampling {
+  double temperature, top_p, min_p;
+  int32_t top_k;
+  const float* temperature_rows;
+  const float* top_p_rows;
+  const float* min_p_rows;
+  const int32_t* top_k_rows;
+} dkv_sampling;
+int dkv_sample(const void* logits, int32_t dtype, int64_t row_stride, int32_t rows, int32_t vocab,
+               const void* u, int32_t u_dtype, const dkv_sampling* sampling, int64_t* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
