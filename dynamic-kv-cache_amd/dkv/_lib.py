@@ -182,7 +182,8 @@ SIGNATURES = [
     ('dkv_evict', ctypes.c_int, [ctypes.POINTER(EvictArgs), ctypes.c_void_p]),
     ('dkv_sample', ctypes.c_int, [ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32,
                                   ctypes.c_void_p, ctypes.c_int32, ctypes.POINTER(Sampling), ctypes.c_void_p,
-                                  ctypes.c_void_p]),
+                                  ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]),
+    ('dkv_sample_workspace_bytes', ctypes.c_int64, [ctypes.c_int32, ctypes.c_int32]),
 ]
 
 

@@ -241,8 +241,9 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         rows = rows.contiguous()
     u = u.contiguous()
     out = torch.empty(lead, dtype=torch.int64, device=logits.device)
+    ws = torch.empty(_lib.load().dkv_sample_workspace_bytes(rows.shape[0], vocab), dtype=torch.uint8, device=logits.device)
     args = (rows.data_ptr(), int(logits.dtype == torch.float32), rows.stride(0), rows.shape[0], vocab, u.data_ptr(),
-            int(u.dtype == torch.float64), ctypes.byref(p), out.data_ptr())
+            int(u.dtype == torch.float64), ctypes.byref(p), out.data_ptr(), ws.data_ptr(), ws.numel())
     if torch.cuda.current_device() == index:
         rc = _lib.load().dkv_sample(*args, _lib.raw_stream(index))
     else:

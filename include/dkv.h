@@ -482,7 +482,9 @@ typedef struct dkv_sampling {
   const int32_t* top_k_rows;
 } dkv_sampling;
 int dkv_sample(const void* logits, int32_t dtype, int64_t row_stride, int32_t rows, int32_t vocab,
-               const void* u, int32_t u_dtype, const dkv_sampling* sampling, int64_t* out, void* stream);
+               const void* u, int32_t u_dtype, const dkv_sampling* sampling, int64_t* out,
+               void* workspace, int64_t workspace_bytes, void* stream);
+int64_t dkv_sample_workspace_bytes(int32_t rows, int32_t vocab);
 
 #ifdef __cplusplus
 }

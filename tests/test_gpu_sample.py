@@ -12,7 +12,8 @@ pytestmark = pytest.mark.gpu
 
 
 def drawn(x, u, temperature, top_k, top_p, min_p):
-    """The definition, a row at a time, on the CPU in 64 bits (Python sums are exact: math.fsum)."""
+    """The definition, a row at a time, on the CPU: weights in 64 bits, then whole multiples of 2^-200, so that every
+    sum and comparison is exact."""
     x = [v if v == v else -math.inf for v in x.double().tolist()]
     top = max(x)
     if top == -math.inf:
@@ -20,24 +21,27 @@ def drawn(x, u, temperature, top_k, top_p, min_p):
     if temperature == 0:
         return x.index(top)
     w = [1.0 if v == top else 0.0 if top == math.inf or v == -math.inf else math.exp((v - top) / temperature) for v in x]
+    unit = [int(math.ldexp(v, 200)) for v in w]
     order = sorted(range(len(x)), key=lambda i: (-x[i], i))
     if top_k:
         order = order[:top_k]
     if top_p < 1:
-        total, kept, before = math.fsum(w[i] for i in order), [], 0.0
+        part, whole = top_p.as_integer_ratio()
+        total, kept, before = sum(unit[i] for i in order), [], 0
         for i in order:
-            if kept and not before < top_p * total:
+            if kept and not before * whole < part * total:
                 break
             kept.append(i)
-            before += w[i]
+            before += unit[i]
         order = kept
     order = sorted(i for i in order if w[i] >= min_p)
-    total, before = math.fsum(w[i] for i in order), 0.0
+    part, whole = u.as_integer_ratio()
+    total, before = sum(unit[i] for i in order), 0
     for i in order:
-        before += w[i]
-        if before > u * total:
+        before += unit[i]
+        if before * whole > part * total:
             return i
-    return order[-1]
+    return max(i for i in order if unit[i])
 
 
 def check(cuda, logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
@@ -191,3 +195,33 @@ def test_refusals(cuda):
                       ((x, u, 1.0, torch.ones(3, device=cuda)), 'top_k tensor'), ((x[:, :0], u), 'vocab')]:
         with pytest.raises(ValueError, match=msg):
             sample(*args)
+
+
+def test_temperatures_at_their_ends(cuda):
+    """Exponents past every bin, weights that all round to the largest, and none at all."""
+    x, u = rows_of(4, 3000, torch.float32, 12)
+    for t in (1e-30, 1e-4, 1e-3, 0.01, 60.0, 1e4, 1e30, math.inf):
+        for kw in (dict(), dict(top_k=9), dict(top_p=0.5), dict(top_k=1500, top_p=0.9, min_p=0.01)):
+            check(cuda, x, u, temperature=t, **kw)
+    check(cuda, x + 3e4, u, top_p=0.9)
+    check(cuda, x - 3e4, u, top_p=0.9)
+    check(cuda, x * 1e30, u, top_k=5)
+
+
+def test_masked_stretches(cuda):
+    """Most of the vocabulary at the type's lowest value, or at -infinity, as masks leave it."""
+    for low, dtype in ((torch.finfo(torch.float32).min, torch.float32), (torch.finfo(torch.bfloat16).min, torch.bfloat16),
+                       (-math.inf, torch.float32), (-1e9, torch.float32)):
+        x, u = rows_of(3, 30000, torch.float32, 13)
+        x[:, 300:29000] = low
+        x[1, :29500] = low
+        for kw in (dict(), dict(top_k=50, top_p=0.9), dict(top_p=0.95), dict(min_p=0.1)):
+            check(cuda, x.to(dtype), u, **kw)
+
+
+def test_more_equal_logits_at_a_cut_than_a_list_holds(cuda):
+    x = torch.zeros(3, 40000)
+    x[:, ::4], x[:, 1::4] = 1.0, 2.0
+    u = torch.tensor([0.1, 0.5, 0.95])
+    for kw in (dict(top_k=15000), dict(top_p=0.7), dict(top_k=25000, top_p=0.75), dict(min_p=0.3), dict(min_p=math.exp(-1) * 0.999)):
+        check(cuda, x, u, **kw)
