@@ -20,15 +20,27 @@ namespace sample {
 
 constexpr int THREADS = 1024;
 
+template <class T>  // uint16_t: bf16
 struct Row {
-  const void* logits;
+  const T* logits;
   int vocab, shift;
-  bool bf16;
   float top;           // the largest logit
   double temperature;
 
-  __device__ __forceinline__ float at(int i) const {
-    return bf16 ? bf16_lo(static_cast<const uint16_t*>(logits)[i]) : static_cast<const float*>(logits)[i];
+  __device__ __forceinline__ float at(int i) const { return value(logits[i]); }
+  __device__ __forceinline__ static float value(uint16_t x) { return bf16_lo(x); }
+  __device__ __forceinline__ static float value(float x) { return x; }
+  // Calls f(token, logit) for tokens first + j * STEP below `end`, N loads in flight.
+  template <int N, int STEP, class F>
+  __device__ __forceinline__ void each(int first, int end, F f) const {
+    for (int i = first; i < end; i += N * STEP) {
+      T x[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) x[j] = logits[min(i + j * STEP, end - 1)];
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (i + j * STEP < end) f(i + j * STEP, value(x[j]));
+    }
   }
   // exp((x - max) / temperature): 0 where x is -infinity or NaN, and beside an infinite logit
   __device__ __forceinline__ double weight(float x) const {
@@ -79,7 +91,8 @@ __device__ __forceinline__ uint64_t block_sum(Scratch& s, uint64_t x) {
 }
 
 // The index of the n-th token (n >= 1) with this key, or the last index if there are fewer.
-__device__ __forceinline__ int nth_of_key(Scratch& s, const Row& r, uint32_t key, int64_t n) {
+template <class T>
+__device__ __forceinline__ int nth_of_key(Scratch& s, const Row<T>& r, uint32_t key, int64_t n) {
   int64_t seen = 0;
   if (threadIdx.x == 0) s.found = r.vocab - 1;
   for (int i0 = 0; i0 < r.vocab; i0 += THREADS) {
@@ -105,17 +118,17 @@ struct Args {
   const void* u;
   int64_t row_stride;
   int64_t* out;
-  int vocab, shift, bf16, u_dtype;
+  int vocab, shift, u_dtype;
   int parts, part_len;  // of the vocabulary
   int counting;         // a top_k may be set: weigh_kernel counts, too
   dkv_sampling p;
 };
 
-__device__ __forceinline__ Row row_of(const Args& a, int row) {
-  Row r;
-  r.bf16 = a.bf16, r.vocab = a.vocab, r.shift = a.shift, r.top = 0.f;
-  r.logits = a.bf16 ? (const void*)(static_cast<const uint16_t*>(a.logits) + row * a.row_stride)
-                    : (const void*)(static_cast<const float*>(a.logits) + row * a.row_stride);
+template <class T>
+__device__ __forceinline__ Row<T> row_of(const Args& a, int row) {
+  Row<T> r;
+  r.vocab = a.vocab, r.shift = a.shift, r.top = 0.f;
+  r.logits = static_cast<const T*>(a.logits) + row * a.row_stride;
   r.temperature = a.p.temperature_rows ? (double)a.p.temperature_rows[row] : a.p.temperature;
   return r;
 }
@@ -152,7 +165,8 @@ __device__ __forceinline__ uint64_t target_of(double u, uint64_t total) {
 }
 
 // The whole row by radix searches: right for every row, and slow (every search reads all of it).
-__device__ __noinline__ void search_row(Scratch& s, const Row& r, const Filters& f, int64_t* out) {
+template <class T>
+__device__ __noinline__ void search_row(Scratch& s, const Row<T>& r, const Filters& f, int64_t* out) {
   const int vocab = r.vocab;
   const int64_t top_k = f.top_k;
   const double top_p = f.top_p, min_p = f.min_p;
@@ -237,6 +251,7 @@ constexpr int OCTAVE = 8, BINS = 512;  // bins of an octave of weight; 52 octave
 constexpr int STEPS = 256;             // steps of the table of 2^f
 constexpr int LIST = 4096;             // tokens of a bin that is cut
 constexpr int MAX_PARTS = 64;
+constexpr int AHEAD = 8;  // parts whose bins a thread has in flight
 constexpr int NOTHING = INT32_MIN, BEYOND = INT32_MAX;
 constexpr double FAR = 65536.;         // largest exponent whose weights keep 2^-36 of their value
 
@@ -276,6 +291,7 @@ struct Weigher {
   }
 };
 
+template <class T>
 __global__ __launch_bounds__(WEIGH_THREADS) void weigh_kernel(Args a, Part* parts, uint64_t* masses, uint32_t* counts) {
   __shared__ double table[STEPS];
   __shared__ uint64_t mass[BINS];
@@ -283,17 +299,16 @@ __global__ __launch_bounds__(WEIGH_THREADS) void weigh_kernel(Args a, Part* part
   __shared__ uint32_t best[WEIGH_THREADS / 64];
   __shared__ int at[WEIGH_THREADS / 64];
   const int part = blockIdx.x, row = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const Row r = row_of(a, row);
+  const Row<T> r = row_of<T>(a, row);
   const int from = part * a.part_len, to = min(a.vocab, from + a.part_len);
   for (int i = threadIdx.x; i < STEPS; i += WEIGH_THREADS) table[i] = exp2(i * (1. / STEPS));
   for (int i = threadIdx.x; i < BINS; i += WEIGH_THREADS) mass[i] = 0, count[i] = 0;
   uint32_t top = 0;
   int first = to;
-#pragma unroll 8
-  for (int i = from + threadIdx.x; i < to; i += WEIGH_THREADS) {
-    const uint32_t key = order_key(r.at(i));
+  r.template each<8, WEIGH_THREADS>(from + threadIdx.x, to, [&](int i, float x) {
+    const uint32_t key = order_key(x);
     if (key > top) top = key, first = i;
-  }
+  });
 #pragma unroll
   for (int d = 32; d; d >>= 1) {
     const uint32_t o = (uint32_t)__shfl_xor((int)top, d, 64);
@@ -316,17 +331,15 @@ __global__ __launch_bounds__(WEIGH_THREADS) void weigh_kernel(Args a, Part* part
   if (threadIdx.x == 0) parts[slot] = Part{top, first, exponent, 0};
   if (!(r.temperature > 0.)) return;
   if (exponent != NOTHING && exponent != BEYOND) {
-#pragma unroll 4
-    for (int i = from + threadIdx.x; i < to; i += WEIGH_THREADS) {
-      const float x = r.at(i);
-      if (!(x > -INFINITY)) continue;
+    r.template each<8, WEIGH_THREADS>(from + threadIdx.x, to, [&](int, float x) {
+      if (!(x > -INFINITY)) return;
       int bin;
       const uint64_t w = weigher.weight(x, exponent, bin);
       if (w) {
         atomicAdd(reinterpret_cast<unsigned long long*>(&mass[bin]), (unsigned long long)w);
         if (a.counting) atomicAdd(&count[bin], 1u);
       }
-    }
+    });
   }
   __syncthreads();
   for (int i = threadIdx.x; i < BINS; i += WEIGH_THREADS) {
@@ -346,6 +359,8 @@ struct DrawScratch {
   double table[STEPS];
   uint64_t mass[BINS];  // of all parts, and sums from the top
   uint32_t count[BINS];
+  uint64_t half_mass[BINS];
+  uint32_t half_count[BINS];
   uint64_t sums[THREADS / 64];
   uint64_t part_mass[MAX_PARTS];
   int exponents[MAX_PARTS];
@@ -395,18 +410,18 @@ __device__ __forceinline__ uint32_t first_key(const Weigher& w, double floor8) {
 
 // Lists the row's tokens with keys in [low, high) that `cut` takes, ranked by falling key, then index. Returns how
 // many, or more than LIST if they do not fit.
-__device__ __forceinline__ int rank_tokens(DrawScratch& s, const Row& r, uint32_t low, uint32_t high, const Cut& cut) {
+template <class T>
+__device__ __forceinline__ int rank_tokens(DrawScratch& s, const Row<T>& r, uint32_t low, uint32_t high, const Cut& cut) {
   __syncthreads();
   if (threadIdx.x == 0) s.listed = 0;
   __syncthreads();
-#pragma unroll 8
-  for (int i = threadIdx.x; i < r.vocab; i += THREADS) {
-    const uint32_t key = order_key(r.at(i));
+  r.template each<16, THREADS>(threadIdx.x, r.vocab, [&](int i, float x) {
+    const uint32_t key = order_key(x);
     if (key >= low && key < high && cut.takes(key, i)) {
       const int to = atomicAdd(&s.listed, 1);
       if (to < LIST) s.list[to] = (uint64_t)~key << 32 | (uint32_t)i;
     }
-  }
+  });
   __syncthreads();
   const int n = s.listed;
   if (n > LIST) return n;
@@ -422,20 +437,24 @@ __device__ __forceinline__ int rank_tokens(DrawScratch& s, const Row& r, uint32_
 
 __device__ __forceinline__ uint32_t key_at(const DrawScratch& s, int i) { return ~(uint32_t)(s.ranked[i] >> 32); }
 
+template <class T>
 __global__ __launch_bounds__(THREADS) void draw_kernel(Args a, const Part* parts, const uint64_t* masses, const uint32_t* counts) {
   __shared__ DrawScratch s;
   const int row = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  Row r = row_of(a, row);
+  Row<T> r = row_of<T>(a, row);
   const Filters f = filters_of(a, row);
   parts += (int64_t)row * a.parts, masses += (int64_t)row * a.parts * BINS, counts += (int64_t)row * a.parts * BINS;
-  uint32_t top = 0;
-  int first = 0, exponent = NOTHING;
-  for (int p = 0; p < a.parts; ++p) {
-    const Part x = parts[p];
-    if (x.key > top) top = x.key, first = x.first;
-    exponent = max(exponent, x.exponent);
-    if (threadIdx.x == 0) s.exponents[p] = x.exponent;
+  Part best = lane < a.parts ? parts[lane] : Part{0, 0, NOTHING, 0};  // lane p has part p (MAX_PARTS is a wave)
+  if (wave == 0) s.exponents[lane] = best.exponent;
+#pragma unroll
+  for (int d = 32; d; d >>= 1) {
+    const uint32_t key = (uint32_t)__shfl_xor((int)best.key, d, 64);
+    const int at = __shfl_xor(best.first, d, 64), e = __shfl_xor(best.exponent, d, 64);
+    if (key > best.key || (key == best.key && at < best.first)) best.key = key, best.first = at;
+    best.exponent = max(best.exponent, e);
   }
+  const uint32_t top = best.key;
+  const int first = best.first, exponent = best.exponent;
   int64_t* out = a.out + row;
   if (exponent == NOTHING || !(r.temperature > 0.)) {
     if (threadIdx.x == 0) *out = exponent == NOTHING ? -1 : first;
@@ -447,19 +466,32 @@ __global__ __launch_bounds__(THREADS) void draw_kernel(Args a, const Part* parts
   for (int i = threadIdx.x; i < STEPS; i += THREADS) s.table[i] = exp2(i * (1. / STEPS));
   __syncthreads();
 
+  // octaves from the row's exponent down to a part's (more than any weight has where the part has none)
+  auto apart_of = [&](int p) { return s.exponents[p] == NOTHING ? BINS : (int)min((int64_t)exponent - s.exponents[p], (int64_t)BINS); };
   // the row's bins, running sums from the top
   uint64_t mine = 0;
   uint32_t mine_count = 0;
   const int bins = OCTAVE * a.shift;  // in those below a token weighs nothing
-  if (threadIdx.x < bins)
-    for (int p = 0; p < a.parts; ++p) {
-      const int64_t apart = s.exponents[p] == NOTHING ? a.shift + 1 : (int64_t)exponent - s.exponents[p];
-      const int64_t bin = threadIdx.x - apart * OCTAVE;
-      if (apart <= a.shift && bin >= 0) {
-        mine += masses[(int64_t)p * BINS + bin] >> apart;
-        if (a.counting) mine_count += counts[(int64_t)p * BINS + bin];
-      }
+  for (int p = wave / (BINS / 64); p < MAX_PARTS; p += 2 * AHEAD) {  // half of the threads take the odd parts
+    if (p >= a.parts) break;
+    uint64_t m[AHEAD];
+    uint32_t n[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {  // (loads first, in flight together)
+      const int part = p + 2 * i, bin = threadIdx.x % BINS - OCTAVE * min(apart_of(min(part, a.parts - 1)), BINS);
+      const bool there = part < a.parts && bin >= 0 && threadIdx.x % BINS < bins;
+      const int64_t at = there ? (int64_t)part * BINS + bin : 0;
+      m[i] = masses[at] & (there ? ~0ull : 0ull);
+      n[i] = a.counting && there ? counts[at] : 0u;
     }
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+      mine += m[i] >> min(apart_of(min(p + 2 * i, a.parts - 1)), 63), mine_count += n[i];
+  }
+  if (threadIdx.x >= BINS) s.half_mass[threadIdx.x % BINS] = mine, s.half_count[threadIdx.x % BINS] = mine_count;
+  __syncthreads();
+  if (threadIdx.x < BINS) mine += s.half_mass[threadIdx.x], mine_count += s.half_count[threadIdx.x];
+  else mine = mine_count = 0;
   uint64_t total, ignored;
   mine = block_scan(s, mine, total);
   if (threadIdx.x < BINS) s.mass[threadIdx.x] = mine;
@@ -541,10 +573,12 @@ __global__ __launch_bounds__(THREADS) void draw_kernel(Args a, const Part* parts
   if (threadIdx.x < MAX_PARTS) s.part_mass[threadIdx.x] = 0;
   __syncthreads();
   for (int p = wave; p < a.parts; p += THREADS / 64) {
-    const int64_t apart = s.exponents[p] == NOTHING ? a.shift + 1 : (int64_t)exponent - s.exponents[p];
+    const int apart = apart_of(p);
     if (apart > a.shift) continue;
     uint64_t sum = 0;
-    for (int b = lane; b < min(cut_bin, bins) - apart * OCTAVE; b += 64) sum += masses[(int64_t)p * BINS + b] >> apart;
+#pragma unroll
+    for (int i = 0; i < BINS / 64; ++i)
+      if (const int b = 64 * i + lane; b < min(cut_bin, bins) - apart * OCTAVE) sum += masses[(int64_t)p * BINS + b] >> apart;
     sum = wave_scan(sum);
     if (lane == 63) s.part_mass[p] = sum;
   }
@@ -557,11 +591,11 @@ __global__ __launch_bounds__(THREADS) void draw_kernel(Args a, const Part* parts
         atomicAdd(reinterpret_cast<unsigned long long*>(&s.part_mass[token / a.part_len]), (unsigned long long)weight(key));
     }
   __syncthreads();
-  total = 0;
-  for (int p = 0; p < a.parts; ++p) total += s.part_mass[p];
+  const uint64_t parts_upto = wave_scan(s.part_mass[lane]);  // lane p: the kept weight of parts up to p
+  total = shfl64(parts_upto, 63);
   uint64_t target = target_of(f.u, total);
-  int part = 0;
-  while (part < a.parts - 1 && target >= s.part_mass[part]) target -= s.part_mass[part++];
+  const int part = __ffsll((unsigned long long)__ballot(parts_upto > target)) - 1;
+  target -= shfl64(parts_upto, part) - s.part_mass[part];
 
   // the part, in order: a consecutive run of tokens a thread
   const int from = part * a.part_len, to = min(a.vocab, from + a.part_len), run = (to - from + THREADS - 1) / THREADS;
@@ -591,6 +625,12 @@ static int parts_of(int rows, int vocab) {
   const int64_t most = (vocab + 2047) / 2048, want = (2048 + rows - 1) / rows;
   const int64_t n = most < want ? most : want;
   return n < MAX_PARTS ? (int)n : MAX_PARTS;
+}
+
+template <class T>
+static void launch(const Args& a, int rows, Part* parts, uint64_t* masses, uint32_t* counts, hipStream_t st) {
+  hipLaunchKernelGGL(weigh_kernel<T>, dim3(a.parts, rows), dim3(WEIGH_THREADS), 0, st, a, parts, masses, counts);
+  hipLaunchKernelGGL(draw_kernel<T>, dim3(rows), dim3(THREADS), 0, st, a, parts, masses, counts);
 }
 
 }  // namespace sample
@@ -635,7 +675,7 @@ int dkv_sample(const void* logits, int32_t dtype, int64_t row_stride, int32_t ro
   }
   sample::Args a{};
   a.logits = logits, a.u = u, a.row_stride = row_stride, a.out = out;
-  a.vocab = vocab, a.bf16 = dtype == 0, a.u_dtype = u_dtype, a.p = p;
+  a.vocab = vocab, a.u_dtype = u_dtype, a.p = p;
   a.shift = 62;
   while (a.shift > 50 || ((uint64_t)vocab >> (62 - a.shift)) > 0) --a.shift;  // vocab << shift stays below 2^62
   a.parts = sample::parts_of(rows, vocab), a.part_len = (vocab + a.parts - 1) / a.parts;
@@ -657,10 +697,8 @@ int dkv_sample(const void* logits, int32_t dtype, int64_t row_stride, int32_t ro
     if (p.min_p_rows) b.p.min_p_rows += at;
     if (p.top_k_rows) b.p.top_k_rows += at;
     const int64_t slot = (int64_t)at * a.parts;
-    hipLaunchKernelGGL(sample::weigh_kernel, dim3(a.parts, n), dim3(sample::WEIGH_THREADS), 0, st, b, parts + slot,
-                       masses + slot * sample::BINS, counts + slot * sample::BINS);
-    hipLaunchKernelGGL(sample::draw_kernel, dim3(n), dim3(sample::THREADS), 0, st, b, parts + slot, masses + slot * sample::BINS,
-                       counts + slot * sample::BINS);
+    if (dtype == 0) sample::launch<uint16_t>(b, n, parts + slot, masses + slot * sample::BINS, counts + slot * sample::BINS, st);
+    else sample::launch<float>(b, n, parts + slot, masses + slot * sample::BINS, counts + slot * sample::BINS, st);
   }
   return (int)hipGetLastError();
 }
