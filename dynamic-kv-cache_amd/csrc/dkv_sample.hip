@@ -4,15 +4,20 @@
 // top_k, of those the shortest run that holds top_p of their weight, of those the ones with w >= min_p; then the
 // first token, in the vocabulary's order, up to which the kept weight exceeds u times its total.
 //
-// Two launches. weigh_kernel: many workgroups a row sum the weights of their part of the vocabulary by bins, eight an
-// octave, so that a bin's tokens are consecutive in the order of the logits. draw_kernel, a workgroup a row: finds the
-// bins in which the filters cut, lists and ranks the few tokens of those bins, then finds the part and the token where
-// the kept weight passes the target. Weights are computed in 64 bits and summed as integers (multiples of 2^-SHIFT of
-// a power of two above the largest): such sums are exact and the same in every order, so neither atomics nor the split
-// into parts can move a border between two tokens. SHIFT leaves room for a whole vocabulary's sum (40 for 4 million
-// tokens, 46 for 49280), and what is lighter counts as nothing.
-// What does not fit that (an infinite logit, exponents beyond 65536, more than LIST tokens in a bin that is cut)
-// takes search_row, a radix search over the whole row, in the same launch.
+// Weights are computed in 64 bits and summed as integers, multiples of 2^-SHIFT of a power of two above the largest:
+// such sums are exact and the same in every order, so neither atomics nor the split of a row into parts can move a
+// border between two tokens. SHIFT leaves room for a whole vocabulary's sum (40 for 4 million tokens, 46 for 49280);
+// what is lighter counts as nothing.
+//
+// weigh_kernel: many workgroups a row, each over a part of the vocabulary, sum its weights by bins, eight an octave, so
+// that a bin's tokens are consecutive in the order of the logits. A workgroup alone gets some 30 GB/s from memory that
+// others wrote, so no workgroup reads a whole row again:
+//   - with a top_k up to SMALL_K, weigh_kernel lists what its part can have among the row's first top_k, and
+//     draw_kernel, a workgroup a row, works on these lists alone: two launches;
+//   - else pick_kernel joins a row's bins and finds the first one that a filter cuts, gather_kernel lists that bin's
+//     tokens, and draw_kernel ranks them and finds the part and the token where the kept weight passes the target.
+// What does not fit that (an infinite logit, exponents beyond 65536, more tokens in a list than it holds) takes
+// search_row, a radix search over the whole row, in draw_kernel.
 #include "dkv_select.h"
 
 namespace dkv {
@@ -247,349 +252,602 @@ __device__ __noinline__ void search_row(Scratch& s, const Row<T>& r, const Filte
 
 // ---- bins -------------------------------------------------------------------------------------------------------
 constexpr int WEIGH_THREADS = 256;
-constexpr int OCTAVE = 8, BINS = 512;  // bins of an octave of weight; 52 octaves and more
+constexpr int HELD = 32;               // tokens a thread of weigh_kernel keeps in registers, where a part is that small
+constexpr int OCTAVE = 8, BINS = 512;  // bins of an octave of weight; at most 8 * 50 + 1 are used
 constexpr int STEPS = 256;             // steps of the table of 2^f
 constexpr int LIST = 4096;             // tokens of a bin that is cut
+constexpr int SMALL_K = 256;           // top_k whose tokens are listed by the parts
+constexpr int PART_LIST = 512;         // tokens that a part lists
 constexpr int MAX_PARTS = 64;
-constexpr int AHEAD = 8;  // parts whose bins a thread has in flight
+constexpr int ROWS = 512;              // rows of one set of launches
+constexpr int AHEAD = 8;               // parts whose bins a thread has in flight
 constexpr int NOTHING = INT32_MIN, BEYOND = INT32_MAX;
 constexpr double FAR = 65536.;         // largest exponent whose weights keep 2^-36 of their value
+constexpr double LOG2_E = 1.44269504088896340736, LN_2 = 0.69314718055994530942;
 
 struct Part {
-  uint32_t key;   // its largest logit, and the first index of it
+  float top;     // its largest logit, and at temperature 0 the first index of it
   int first;
-  int exponent;   // its weights are below 2^exponent: the unit of its sums is 2^(exponent - SHIFT)
+  int exponent;  // its weights are below 2^(exponent + 1): the unit of its sums is 2^(exponent - SHIFT)
+  int listed;    // tokens in its list
+};
+
+struct RowState {
+  float top;
+  int exponent, bin;    // the row's exponent; the first bin that a filter cuts (BINS: none)
+  uint32_t low, high;   // keys of that bin
+  int listed;           // of its tokens, in the row's list
+  int search;           // takes search_row
   int pad;
 };
 
-// A logit's base-2 exponent Y = x log2(e) / T as octave + f, and 2^f in [1, 2) as 53 bits: a table of 2^(j / 256) and
-// the exponential's series for the rest (below ln 2 / 256, so its fifth term is below 2^-49).
+struct Work {
+  uint64_t* masses;    // [parts][BINS]
+  uint64_t* part_list;  // [parts][PART_LIST] tokens: ~key << 32 | index
+  uint64_t* sums;      // [rows][BINS] weight from the top bin on
+  uint64_t* lists;     // [rows][LIST] tokens
+  Part* parts;
+  RowState* rows;
+  uint32_t* counts;    // [parts][BINS]
+  uint32_t* count_sums;  // [rows][BINS]
+};
+
+__device__ __forceinline__ bool lists_parts(const Filters& f) { return f.top_k > 0 && f.top_k <= SMALL_K; }
+
+__device__ __forceinline__ uint64_t token_of(uint32_t key, int index) { return (uint64_t)~key << 32 | (uint32_t)index; }
+__device__ __forceinline__ uint32_t key_of(uint64_t token) { return ~(uint32_t)(token >> 32); }
+__device__ __forceinline__ int index_of(uint64_t token) { return (int)(uint32_t)token; }
+
+// Weights relative to 2^exponent. Y = x log2(e) / T is rounded to a multiple k of 1/256 by an addition that leaves k in
+// the sum's low bits; 2^Y is a table's 2^((k mod 256) / 256) times the exponential series of the rest (at most
+// ln 2 / 512, so the fifth term is below 2^-53).
 struct Weigher {
   const double* table;
   double rate;  // log2(e) / T
-  int shift;
-  __device__ __forceinline__ double exponent(float x) const { return (double)x * rate; }
-  // Bin from the top of `exponent` down, 8 an octave, and the weight in units of 2^(exponent - shift), rounded down;
-  // weight 0 where that is nothing. x is finite.
-  __device__ __forceinline__ uint64_t weight(float x, int exponent_, int& bin) const {
-    const double y = exponent(x), octave = floor(y), f = y - octave;
-    const double down = (double)exponent_ - octave;  // at least 1
+  int shift, exponent;
+  float least;  // weights of smaller logits are nothing
+
+  __device__ __forceinline__ Weigher(const double* table_, double temperature, int shift_, int exponent_)
+      : table(table_), rate(LOG2_E / temperature), shift(shift_), exponent(exponent_) {
+    least = fmaxf((float)((exponent - shift - 2) / rate), -3.4028235e38f);
+  }
+  __device__ __forceinline__ static double magic() { return 1.5 * (1ll << 44); }
+  __device__ __forceinline__ int step(float x) const {
+    return (int)(uint32_t)__builtin_bit_cast(uint64_t, (double)x * rate + magic());
+  }
+  // The weight in units of 2^(exponent - shift), rounded down, and its bin from 8 * exponent down.
+  __device__ __forceinline__ uint64_t weight(float x, int& bin) const {
     bin = BINS;
-    if (!(down <= (double)shift)) return 0;
-    const int j = min((int)(f * STEPS), STEPS - 1);
-    const double t = (f - j * (1. / STEPS)) * 0.69314718055994530942;
-    double e = __builtin_fma(t, 1. / 24, 1. / 6);
-    e = __builtin_fma(t, e, .5);
-    e = __builtin_fma(t, e, 1.);
-    const double w = __builtin_fma(t * table[j], e, table[j]);
-    const int d = (int)down;
-    bin = OCTAVE * d - 1 - j / (STEPS / OCTAVE);
-    const uint64_t bits = __builtin_bit_cast(uint64_t, w);
-    // (a series that rounds up to 2 keeps its octave's last value)
-    const uint64_t mantissa = bits >= 0x4000000000000000ull ? (1ull << 53) - 1 : (bits & ((1ull << 52) - 1)) | 1ull << 52;
-    return mantissa >> (52 - shift + d);
+    if (!(x >= least)) return 0;
+    const double y = (double)x * rate, sum = y + magic(), r = y - (sum - magic());
+    const int k = (int)(uint32_t)__builtin_bit_cast(uint64_t, sum), down = exponent - (k >> 8);
+    double e = __builtin_fma(r, LN_2 * LN_2 * LN_2 * LN_2 / 24, LN_2 * LN_2 * LN_2 / 6);
+    e = __builtin_fma(r, e, LN_2 * LN_2 / 2);
+    e = __builtin_fma(r, e, LN_2);
+    const double t = table[k & (STEPS - 1)], w = __builtin_fma(t, r * e, t);
+    if (down > shift) return 0;
+    bin = OCTAVE * exponent - (k >> 5);
+    // w 2^51 as the low bits of a sum with 2^52
+    const uint64_t m = __builtin_bit_cast(uint64_t, __builtin_fma(w, 0x1p51, 0x1p52)) & ((1ull << 52) - 1);
+    return m >> (51 - shift + down);
+  }
+  __device__ __forceinline__ uint64_t weight(float x) const {
+    int bin;
+    return weight(x, bin);
+  }
+  // The smallest key of a bin: the first whose step is 32 * eighth or more, by weight()'s own arithmetic. The border is
+  // half a step below the eighth; a float that near it is at most a few keys off.
+  __device__ __forceinline__ uint32_t first_key(int eighth) const {
+    const float x = (float)((eighth * (1. / OCTAVE) - .5 / STEPS) / rate);
+    uint32_t key = order_key(fminf(fmaxf(x, -3.4028235e38f), 3.4028235e38f));
+    auto reaches = [&](uint32_t k) { return step(logit_of(k)) >> 5 >= eighth; };
+    for (int i = 0; i < 8 && reaches(key - 1); ++i) --key;
+    for (int i = 0; i < 8 && !reaches(key); ++i) ++key;
+    return key;
   }
 };
 
 template <class T>
-__global__ __launch_bounds__(WEIGH_THREADS) void weigh_kernel(Args a, Part* parts, uint64_t* masses, uint32_t* counts) {
+__global__ __launch_bounds__(WEIGH_THREADS) void weigh_kernel(Args a, Work work) {
   __shared__ double table[STEPS];
   __shared__ uint64_t mass[BINS];
   __shared__ uint32_t count[BINS];
-  __shared__ uint32_t best[WEIGH_THREADS / 64];
+  __shared__ float best[WEIGH_THREADS / 64];
   __shared__ int at[WEIGH_THREADS / 64];
+  __shared__ int listed, last_bin;
   const int part = blockIdx.x, row = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const Row<T> r = row_of<T>(a, row);
+  const Filters f = filters_of(a, row);
   const int from = part * a.part_len, to = min(a.vocab, from + a.part_len);
+  const int64_t slot = (int64_t)row * a.parts + part;
+  const bool fits = a.part_len <= HELD * WEIGH_THREADS;
+  float held[HELD];
+  if (fits && from < to) {
+    T x[HELD];
+#pragma unroll
+    for (int j = 0; j < HELD; ++j) x[j] = r.logits[min(from + j * WEIGH_THREADS + (int)threadIdx.x, to - 1)];
+#pragma unroll
+    for (int j = 0; j < HELD; ++j) held[j] = Row<T>::value(x[j]);
+  }
+  auto each = [&](auto g) {  // g(token, logit) for this thread's tokens
+    if (fits) {
+#pragma unroll
+      for (int j = 0; j < HELD; ++j)
+        if (const int i = from + j * WEIGH_THREADS + (int)threadIdx.x; i < to) g(i, held[j]);
+    } else {
+      r.template each<8, WEIGH_THREADS>(from + threadIdx.x, to, g);
+    }
+  };
   for (int i = threadIdx.x; i < STEPS; i += WEIGH_THREADS) table[i] = exp2(i * (1. / STEPS));
   for (int i = threadIdx.x; i < BINS; i += WEIGH_THREADS) mass[i] = 0, count[i] = 0;
-  uint32_t top = 0;
-  int first = to;
-  r.template each<8, WEIGH_THREADS>(from + threadIdx.x, to, [&](int i, float x) {
-    const uint32_t key = order_key(x);
-    if (key > top) top = key, first = i;
+  if (threadIdx.x == 0) listed = 0, last_bin = BINS;
+  float top = -INFINITY;
+  each([&](int, float x) { top = fmaxf(top, x); });  // (passes over NaN)
+#pragma unroll
+  for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+  if (lane == 0) best[wave] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < WEIGH_THREADS / 64; ++w) top = fmaxf(top, best[w]);
+  if (!(r.temperature > 0.)) {
+    int first = to;
+    each([&](int i, float x) {
+      if (x == top) first = min(first, i);
+    });
+#pragma unroll
+    for (int d = 32; d; d >>= 1) first = min(first, __shfl_xor(first, d, 64));
+    if (lane == 0) at[wave] = first;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int w = 0; w < WEIGH_THREADS / 64; ++w) first = min(first, at[w]);
+      work.parts[slot] = Part{top, first, top > -INFINITY ? 0 : NOTHING, 0};
+    }
+    return;
+  }
+  const double y = (double)top * (LOG2_E / r.temperature);
+  // (a part far below the others, of masked tokens say, just adds nothing)
+  const int exponent = !(top > -INFINITY) ? NOTHING : top < INFINITY && y <= FAR ? (int)fmax(floor(y) + 1., -1e9) : BEYOND;
+  const bool far = exponent == NOTHING || exponent == BEYOND || exponent < -FAR - BINS;  // (a row below -FAR is searched)
+  if (threadIdx.x == 0 && (far || !lists_parts(f))) work.parts[slot] = Part{top, 0, exponent, 0};
+  if (far) return;
+  const Weigher weigher(table, r.temperature, a.shift, exponent);
+  const bool lists = lists_parts(f);
+  each([&](int, float x) {
+    int bin;
+    const uint64_t w = weigher.weight(x, bin);
+    if (w) {
+      if (!lists) atomicAdd(reinterpret_cast<unsigned long long*>(&mass[bin]), (unsigned long long)w);
+      if (a.counting) atomicAdd(&count[bin], 1u);
+    }
   });
+  __syncthreads();
+  if (!lists) {
+    for (int i = threadIdx.x; i <= OCTAVE * a.shift; i += WEIGH_THREADS) {
+      work.masses[slot * BINS + i] = mass[i];
+      if (a.counting) work.counts[slot * BINS + i] = count[i];
+    }
+    return;
+  }
+  // tokens down to the bin in which the part's count reaches top_k
+  if (wave == 0) {
+    uint32_t c[BINS / 64], sum = 0;
+#pragma unroll
+    for (int i = 0; i < BINS / 64; ++i) sum += c[i] = count[lane * (BINS / 64) + i];
+    uint32_t upto = sum;
+    for (int d = 1; d < 64; d <<= 1) {
+      const uint32_t o = __shfl_up(upto, d, 64);
+      if (lane >= d) upto += o;
+    }
+    uint32_t before = upto - sum;
+    if (before < f.top_k && f.top_k <= upto) {
+      int i = 0;
+      while (before + c[i] < f.top_k) before += c[i++];
+      last_bin = lane * (BINS / 64) + i;
+    }
+  }
+  __syncthreads();
+  const int last = last_bin;
+  each([&](int i, float x) {
+    int bin;
+    if (x >= weigher.least && OCTAVE * exponent - (weigher.step(x) >> 5) <= last && weigher.weight(x, bin)) {
+      const int to = atomicAdd(&listed, 1);
+      if (to < PART_LIST) work.part_list[slot * PART_LIST + to] = token_of(order_key(x), i);
+    }
+  });
+  __syncthreads();
+  if (threadIdx.x == 0) work.parts[slot] = Part{top, 0, exponent, listed};
+}
+
+struct RowTop {
+  float top;
+  int first, exponent;
+};
+// The row's largest logit, its first index (temperature 0) and exponent, by every wave from its parts: lane p has part p
+// (MAX_PARTS is a wave).
+__device__ __forceinline__ RowTop row_top(const Part& mine) {
+  RowTop t{mine.top, mine.first, mine.exponent};
 #pragma unroll
   for (int d = 32; d; d >>= 1) {
-    const uint32_t o = (uint32_t)__shfl_xor((int)top, d, 64);
-    const int oi = __shfl_xor(first, d, 64);
-    if (o > top || (o == top && oi < first)) top = o, first = oi;
+    const float top = __shfl_xor(t.top, d, 64);
+    const int first = __shfl_xor(t.first, d, 64), exponent = __shfl_xor(t.exponent, d, 64);
+    if (top > t.top || (top == t.top && first < t.first)) t.top = top, t.first = first;
+    t.exponent = max(t.exponent, exponent);
   }
-  if (lane == 0) best[wave] = top, at[wave] = first;
+  return t;
+}
+__device__ __forceinline__ Part part_of(const Args& a, const Part* parts, int lane) {
+  return lane < a.parts ? parts[lane] : Part{-INFINITY, a.vocab, NOTHING, 0};
+}
+// Octaves from the row's exponent down to a part's (more than any weight has where the part has none).
+__device__ __forceinline__ int apart_of(int row_exponent, int exponent) {
+  return exponent == NOTHING ? BINS : (int)min((int64_t)row_exponent - exponent, (int64_t)BINS);
+}
+
+struct BinScratch {
+  uint64_t sums[THREADS / 64];
+  uint64_t before;
+  int bin;
+};
+
+template <int WAVES>
+__device__ __forceinline__ uint64_t block_scan(uint64_t (&sums)[THREADS / 64], uint64_t x, uint64_t& total) {  // inclusive
+  x = wave_scan(x);
   __syncthreads();
-  top = best[0], first = at[0];
+  if ((threadIdx.x & 63) == 63) sums[threadIdx.x >> 6] = x;
+  __syncthreads();
+  uint64_t before = 0;
+  total = 0;
 #pragma unroll
-  for (int w = 1; w < WEIGH_THREADS / 64; ++w)
-    if (best[w] > top || (best[w] == top && at[w] < first)) top = best[w], first = at[w];
-  const Weigher weigher{table, r.temperature > 0. ? 1.44269504088896340736 / r.temperature : 0., a.shift};
-  const float x_top = logit_of(top);
-  const double y_top = weigher.exponent(x_top);
-  const int64_t slot = (int64_t)row * a.parts + part;
-  int exponent = NOTHING;
-  if (top > order_key(-INFINITY))  // (a part far below the others, of masked tokens say, just adds nothing)
-    exponent = x_top < INFINITY && y_top <= FAR ? (int)fmax(floor(y_top) + 1., -1e9) : BEYOND;
-  if (threadIdx.x == 0) parts[slot] = Part{top, first, exponent, 0};
-  if (!(r.temperature > 0.)) return;
-  if (exponent != NOTHING && exponent != BEYOND) {
-    r.template each<8, WEIGH_THREADS>(from + threadIdx.x, to, [&](int, float x) {
-      if (!(x > -INFINITY)) return;
-      int bin;
-      const uint64_t w = weigher.weight(x, exponent, bin);
-      if (w) {
-        atomicAdd(reinterpret_cast<unsigned long long*>(&mass[bin]), (unsigned long long)w);
-        if (a.counting) atomicAdd(&count[bin], 1u);
-      }
-    });
+  for (int w = 0; w < WAVES; ++w) {
+    if (w < (int)(threadIdx.x >> 6)) before += sums[w];
+    total += sums[w];
   }
+  return before + x;
+}
+
+// The first bin in which a running sum from the top, `upto` (inclusive) at thread `bin`, reaches `need`, and the sum
+// before it; BINS if none does.
+__device__ __forceinline__ int bin_of(BinScratch& s, uint64_t upto, uint64_t here, uint64_t need, uint64_t& before) {
   __syncthreads();
-  for (int i = threadIdx.x; i < BINS; i += WEIGH_THREADS) {
-    masses[slot * BINS + i] = mass[i];
-    if (a.counting) counts[slot * BINS + i] = count[i];
+  if (threadIdx.x == 0) s.bin = BINS, s.before = 0;
+  __syncthreads();
+  if (threadIdx.x < BINS && upto >= need && upto - here < need) s.bin = threadIdx.x, s.before = upto - here;
+  __syncthreads();
+  before = s.before;
+  return s.bin;
+}
+
+// The first bin in which min_p cuts.
+__device__ __forceinline__ int min_p_bin(const Weigher& w, float top, double min_p) {
+  if (!(min_p > 0.)) return BINS;
+  const int k = (int)(uint32_t)__builtin_bit_cast(uint64_t, (double)top * w.rate + log2(min_p) + Weigher::magic());
+  const int64_t bin = (int64_t)OCTAVE * w.exponent - (k >> 5);
+  return min_p < 1e-300 || bin >= BINS ? BINS : (int)bin;
+}
+
+// A workgroup a row (BINS threads, a bin each): joins the parts' bins and finds the first that a filter cuts.
+template <class T>
+__global__ __launch_bounds__(BINS) void pick_kernel(Args a, Work work) {
+  __shared__ BinScratch s;
+  __shared__ int apart[MAX_PARTS];
+  const int row = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, bin = threadIdx.x;
+  const Row<T> r = row_of<T>(a, row);
+  const Filters f = filters_of(a, row);
+  if (lists_parts(f) || !(r.temperature > 0.)) return;
+  const Part mine = part_of(a, work.parts + (int64_t)row * a.parts, lane);
+  const RowTop t = row_top(mine);
+  if (t.exponent == NOTHING) return;
+  RowState state{t.top, t.exponent, BINS, 0, 0, 0, t.exponent == BEYOND || t.exponent < -FAR, 0};
+  if (state.search) {
+    if (threadIdx.x == 0) work.rows[row] = state;
+    return;
   }
+  if (wave == 0) apart[lane] = apart_of(t.exponent, mine.exponent);
+  __syncthreads();
+  const uint64_t* masses = work.masses + (int64_t)row * a.parts * BINS;
+  const uint32_t* counts = work.counts + (int64_t)row * a.parts * BINS;
+  uint64_t mass = 0, count = 0;
+  for (int p0 = 0; p0 < a.parts; p0 += AHEAD) {
+    uint64_t m[AHEAD];
+    uint32_t n[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {  // (loads first, in flight together)
+      const int p = min(p0 + i, a.parts - 1), from = bin - OCTAVE * apart[p];
+      const bool there = p0 + i < a.parts && from >= 0 && bin <= OCTAVE * a.shift;
+      const int64_t at = there ? (int64_t)p * BINS + from : 0;
+      m[i] = there ? masses[at] : 0;
+      n[i] = there && a.counting ? counts[at] : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) mass += m[i] >> min(apart[min(p0 + i, a.parts - 1)], 63), count += n[i];
+  }
+  uint64_t total, ignored, before;
+  const uint64_t upto = block_scan<BINS / 64>(s.sums, mass, total);
+  work.sums[(int64_t)row * BINS + bin] = upto;
+  __shared__ double no_table;
+  const Weigher weigher(&no_table, r.temperature, a.shift, t.exponent);
+  int cut = BINS;
+  if (f.top_k > 0 && f.top_k < a.vocab) {
+    const uint64_t count_upto = block_scan<BINS / 64>(s.sums, count, ignored);
+    work.count_sums[(int64_t)row * BINS + bin] = (uint32_t)count_upto;
+    cut = bin_of(s, count_upto, count, (uint64_t)f.top_k, before);
+  }
+  if (cut == BINS) {  // (a rank's cut comes first: what top_p is a share of depends on it)
+    if (f.top_p < 1.) {
+      const uint64_t need = share_of(fmax(f.top_p, 0.), total, true);
+      cut = bin_of(s, upto, mass, need ? need : 1, before);
+    }
+    cut = min(cut, min_p_bin(weigher, t.top, f.min_p));
+  }
+  if (threadIdx.x == 0) {
+    state.bin = cut;
+    if (cut < BINS) {
+      const int eighth = OCTAVE * t.exponent - cut;
+      state.low = max(weigher.first_key(eighth), order_key(-INFINITY) + 1), state.high = weigher.first_key(eighth + 1);
+    }
+    work.rows[row] = state;
+  }
+}
+
+// Lists the tokens of the bin that is cut, in any order.
+template <class T>
+__global__ __launch_bounds__(WEIGH_THREADS) void gather_kernel(Args a, Work work) {
+  const int part = blockIdx.x, row = blockIdx.y;
+  const Row<T> r = row_of<T>(a, row);
+  if (lists_parts(filters_of(a, row)) || !(r.temperature > 0.)) return;
+  const Part p = work.parts[(int64_t)row * a.parts + part];
+  if (p.exponent == NOTHING) return;  // (of a row without any, the state is not set)
+  RowState* state = work.rows + row;
+  const uint32_t low = state->low, high = state->high;
+  if (state->search || state->bin == BINS || order_key(p.top) < low) return;
+  const int from = part * a.part_len, to = min(a.vocab, from + a.part_len);
+  r.template each<16, WEIGH_THREADS>(from + threadIdx.x, to, [&](int i, float x) {
+    const uint32_t key = order_key(x);
+    if (key >= low && key < high) {
+      const int at = atomicAdd(&state->listed, 1);
+      if (at < LIST) work.lists[(int64_t)row * LIST + at] = token_of(key, i);
+    }
+  });
 }
 
 struct DrawScratch {
   union {
     Scratch search;
     struct {
-      uint64_t list[LIST];    // ~key << 32 | index, as found
-      uint64_t ranked[LIST];  // the same by falling key, then index
+      uint64_t list[LIST];    // tokens as found
+      uint64_t ranked[LIST];  // by falling key, then index
     };
   };
   double table[STEPS];
-  uint64_t mass[BINS];  // of all parts, and sums from the top
+  BinScratch bins;
   uint32_t count[BINS];
-  uint64_t half_mass[BINS];
-  uint32_t half_count[BINS];
-  uint64_t sums[THREADS / 64];
   uint64_t part_mass[MAX_PARTS];
-  int exponents[MAX_PARTS];
-  int listed, bin;
-  uint64_t before;
+  int exponents[MAX_PARTS], listed[MAX_PARTS];
+  int ranks[THREADS];
+  int n, keep;
 };
 
-// The first bin up to which `sums` (running, from the top) reaches `need`, and the sum before it; BINS if none does.
-template <class T>
-__device__ __forceinline__ int bin_of(DrawScratch& s, const T* sums, uint64_t need, uint64_t& before) {
-  __syncthreads();
-  if (threadIdx.x == 0) s.bin = BINS;
-  __syncthreads();
-  if (threadIdx.x < BINS) {
-    const uint64_t here = sums[threadIdx.x], above = threadIdx.x ? (uint64_t)sums[threadIdx.x - 1] : 0;
-    if (here >= need && above < need) s.bin = threadIdx.x, s.before = above;
+// ranked = list's n values, rising by order(value) (all different): each counts those before it, several threads a value
+// where there are few.
+template <class Order>
+__device__ __forceinline__ void rank_list(DrawScratch& s, int n, Order order) {
+  int slices = 1;
+  while (slices < 16 && 2 * slices * n <= THREADS) slices *= 2;
+  if (slices == 1) {
+    for (int i = threadIdx.x; i < n; i += THREADS) {
+      const uint64_t x = s.list[i];
+      int rank = 0;
+#pragma unroll 4
+      for (int j = 0; j < n; ++j) rank += order(s.list[j]) < order(x);
+      s.ranked[rank] = x;
+    }
+  } else {
+    s.ranks[threadIdx.x] = 0;
+    __syncthreads();
+    const int i = threadIdx.x % (THREADS / slices), slice = threadIdx.x / (THREADS / slices);
+    if (i < n) {
+      const uint64_t x = s.list[i];
+      int rank = 0;
+#pragma unroll 4
+      for (int j = slice; j < n; j += slices) rank += order(s.list[j]) < order(x);
+      atomicAdd(&s.ranks[i], rank);
+    }
+    __syncthreads();
+    if (threadIdx.x < n) s.ranked[s.ranks[threadIdx.x]] = s.list[threadIdx.x];
   }
   __syncthreads();
-  before = s.before;
-  return s.bin;
 }
 
-__device__ __forceinline__ uint64_t block_scan(DrawScratch& s, uint64_t x, uint64_t& total) {  // inclusive
-  x = wave_scan(x);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 63) s.sums[threadIdx.x >> 6] = x;
-  __syncthreads();
-  uint64_t before = 0;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < THREADS / 64; ++w) {
-    if (w < (int)(threadIdx.x >> 6)) before += s.sums[w];
-    total += s.sums[w];
-  }
-  return before + x;
-}
-
-// The smallest logit's key whose exponent is at least `floor8` eighths (the same arithmetic as weight()'s bin).
-__device__ __forceinline__ uint32_t first_key(const Weigher& w, double floor8) {
-  float x = (float)(floor8 / (8. * w.rate));
-  x = fminf(fmaxf(x, -3.4028235e38f), 3.4028235e38f);
-  uint32_t key = order_key(x);
-  for (int i = 0; i < 8 && floor(8. * w.exponent(logit_of(key - 1))) >= floor8; ++i) --key;
-  for (int i = 0; i < 8 && floor(8. * w.exponent(logit_of(key))) < floor8; ++i) ++key;
-  return key;
-}
-
-// Lists the row's tokens with keys in [low, high) that `cut` takes, ranked by falling key, then index. Returns how
-// many, or more than LIST if they do not fit.
+// Lists and ranks the row's tokens with keys in [low, high) that `cut` takes, reading all of it. Returns how many.
 template <class T>
 __device__ __forceinline__ int rank_tokens(DrawScratch& s, const Row<T>& r, uint32_t low, uint32_t high, const Cut& cut) {
   __syncthreads();
-  if (threadIdx.x == 0) s.listed = 0;
+  if (threadIdx.x == 0) s.n = 0;
   __syncthreads();
   r.template each<16, THREADS>(threadIdx.x, r.vocab, [&](int i, float x) {
     const uint32_t key = order_key(x);
     if (key >= low && key < high && cut.takes(key, i)) {
-      const int to = atomicAdd(&s.listed, 1);
-      if (to < LIST) s.list[to] = (uint64_t)~key << 32 | (uint32_t)i;
+      const int to = atomicAdd(&s.n, 1);
+      if (to < LIST) s.list[to] = token_of(key, i);
     }
   });
   __syncthreads();
-  const int n = s.listed;
-  if (n > LIST) return n;
-  for (int i = threadIdx.x; i < n; i += THREADS) {
-    const uint64_t x = s.list[i];
-    int rank = 0;
-    for (int j = 0; j < n; ++j) rank += s.list[j] < x;
-    s.ranked[rank] = x;
-  }
-  __syncthreads();
+  const int n = s.n;
+  if (n <= LIST) rank_list(s, n, [](uint64_t x) { return x; });
   return n;
 }
 
-__device__ __forceinline__ uint32_t key_at(const DrawScratch& s, int i) { return ~(uint32_t)(s.ranked[i] >> 32); }
+// How many of the n ranked tokens stay: up to the one at which the weight, `sum` before them, reaches `need`, and while
+// w >= min_p.
+template <class T>
+__device__ __forceinline__ int kept_of(DrawScratch& s, const Row<T>& r, const Weigher& weigher, int n, uint64_t sum, uint64_t need,
+                                       double min_p) {
+  __syncthreads();
+  if (threadIdx.x == 0) s.keep = n;
+  __syncthreads();
+  for (int i0 = 0; i0 < n; i0 += THREADS) {
+    const int i = i0 + threadIdx.x;
+    const float x = i < n ? logit_of(key_of(s.ranked[i])) : -INFINITY;
+    uint64_t all;
+    const uint64_t upto = sum + block_scan<THREADS / 64>(s.bins.sums, i < n ? weigher.weight(x) : 0, all);
+    if (i < n && upto >= need) atomicMin(&s.keep, i + 1);
+    if (i < n && min_p > 0. && !(r.weight(x) >= min_p)) atomicMin(&s.keep, i);
+    sum += all;
+  }
+  __syncthreads();
+  return s.keep;
+}
+
+// A row whose parts listed what the first top_k can be among: all of it from the lists.
+template <class T>
+__device__ __forceinline__ bool draw_listed(DrawScratch& s, const Args& a, const Work& work, int row, const Row<T>& r, const Filters& f,
+                                            const Weigher& weigher, int64_t* out) {
+  // how many tokens the bins down to each hold, then the bin in which that reaches top_k
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint64_t* lists = work.part_list + (int64_t)row * a.parts * PART_LIST;
+  for (int i = threadIdx.x; i < BINS; i += THREADS) s.count[i] = 0;
+  if (threadIdx.x == 0) s.n = 0;
+  __syncthreads();
+  auto each = [&](auto g) {  // g(token, bin), a wave a part
+    for (int p = wave; p < a.parts; p += THREADS / 64)
+      for (int i = lane; i < s.listed[p]; i += 64) {
+        const uint64_t token = lists[(int64_t)p * PART_LIST + i];
+        int bin;
+        if (weigher.weight(logit_of(key_of(token)), bin)) g(token, bin);
+      }
+  };
+  each([&](uint64_t, int bin) { atomicAdd(&s.count[bin], 1u); });
+  __syncthreads();
+  uint64_t ignored, before;
+  const uint64_t here = threadIdx.x < BINS ? s.count[threadIdx.x] : 0;
+  const uint64_t upto = block_scan<THREADS / 64>(s.bins.sums, here, ignored);
+  const int last = bin_of(s.bins, upto, here, (uint64_t)f.top_k, before);
+  each([&](uint64_t token, int bin) {
+    if (bin <= last) {
+      const int to = atomicAdd(&s.n, 1);
+      if (to < LIST) s.list[to] = token;
+    }
+  });
+  __syncthreads();
+  int n = s.n;
+  if (n > LIST) return false;
+  rank_list(s, n, [](uint64_t x) { return x; });
+  n = min(n, (int)f.top_k);
+  // (top_k is at most SMALL_K: a token a thread from here on)
+  uint64_t total;
+  const uint64_t w = (int)threadIdx.x < n ? weigher.weight(logit_of(key_of(s.ranked[threadIdx.x]))) : 0;
+  block_scan<THREADS / 64>(s.bins.sums, w, total);
+  uint64_t need = ~0ull;
+  if (f.top_p < 1.) need = share_of(fmax(f.top_p, 0.), total, true);
+  n = kept_of(s, r, weigher, n, 0, need ? need : 1, f.min_p);
+  // by index, then the token at which the weight passes the target
+  if ((int)threadIdx.x < n) s.list[threadIdx.x] = s.ranked[threadIdx.x];
+  __syncthreads();
+  rank_list(s, n, [](uint64_t x) { return (uint32_t)x; });
+  const uint64_t token = (int)threadIdx.x < n ? s.ranked[threadIdx.x] : 0;
+  const uint64_t weight = (int)threadIdx.x < n ? weigher.weight(logit_of(key_of(token))) : 0;
+  const uint64_t sum = block_scan<THREADS / 64>(s.bins.sums, weight, total);
+  const uint64_t target = target_of(f.u, total);
+  if (target < sum && target >= sum - weight) *out = index_of(token);
+  return true;
+}
 
 template <class T>
-__global__ __launch_bounds__(THREADS) void draw_kernel(Args a, const Part* parts, const uint64_t* masses, const uint32_t* counts) {
+__global__ __launch_bounds__(THREADS) void draw_kernel(Args a, Work work) {
   __shared__ DrawScratch s;
   const int row = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   Row<T> r = row_of<T>(a, row);
   const Filters f = filters_of(a, row);
-  parts += (int64_t)row * a.parts, masses += (int64_t)row * a.parts * BINS, counts += (int64_t)row * a.parts * BINS;
-  Part best = lane < a.parts ? parts[lane] : Part{0, 0, NOTHING, 0};  // lane p has part p (MAX_PARTS is a wave)
-  if (wave == 0) s.exponents[lane] = best.exponent;
-#pragma unroll
-  for (int d = 32; d; d >>= 1) {
-    const uint32_t key = (uint32_t)__shfl_xor((int)best.key, d, 64);
-    const int at = __shfl_xor(best.first, d, 64), e = __shfl_xor(best.exponent, d, 64);
-    if (key > best.key || (key == best.key && at < best.first)) best.key = key, best.first = at;
-    best.exponent = max(best.exponent, e);
-  }
-  const uint32_t top = best.key;
-  const int first = best.first, exponent = best.exponent;
+  const Part mine = part_of(a, work.parts + (int64_t)row * a.parts, lane);
+  const RowTop t = row_top(mine);
   int64_t* out = a.out + row;
-  if (exponent == NOTHING || !(r.temperature > 0.)) {
-    if (threadIdx.x == 0) *out = exponent == NOTHING ? -1 : first;
+  if (t.exponent == NOTHING || !(r.temperature > 0.)) {
+    if (threadIdx.x == 0) *out = t.exponent == NOTHING ? -1 : t.first;
     return;
   }
-  r.top = logit_of(top);
-  if (exponent == BEYOND || exponent < -FAR) return search_row(s.search, r, f, out);
-  const Weigher weigher{s.table, 1.44269504088896340736 / r.temperature, a.shift};
+  r.top = t.top;
+  if (t.exponent == BEYOND || t.exponent < -FAR) return search_row(s.search, r, f, out);
+  if (wave == 0) s.exponents[lane] = mine.exponent, s.listed[lane] = mine.listed;
   for (int i = threadIdx.x; i < STEPS; i += THREADS) s.table[i] = exp2(i * (1. / STEPS));
   __syncthreads();
-
-  // octaves from the row's exponent down to a part's (more than any weight has where the part has none)
-  auto apart_of = [&](int p) { return s.exponents[p] == NOTHING ? BINS : (int)min((int64_t)exponent - s.exponents[p], (int64_t)BINS); };
-  // the row's bins, running sums from the top
-  uint64_t mine = 0;
-  uint32_t mine_count = 0;
-  const int bins = OCTAVE * a.shift;  // in those below a token weighs nothing
-  for (int p = wave / (BINS / 64); p < MAX_PARTS; p += 2 * AHEAD) {  // half of the threads take the odd parts
-    if (p >= a.parts) break;
-    uint64_t m[AHEAD];
-    uint32_t n[AHEAD];
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i) {  // (loads first, in flight together)
-      const int part = p + 2 * i, bin = threadIdx.x % BINS - OCTAVE * min(apart_of(min(part, a.parts - 1)), BINS);
-      const bool there = part < a.parts && bin >= 0 && threadIdx.x % BINS < bins;
-      const int64_t at = there ? (int64_t)part * BINS + bin : 0;
-      m[i] = masses[at] & (there ? ~0ull : 0ull);
-      n[i] = a.counting && there ? counts[at] : 0u;
-    }
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i)
-      mine += m[i] >> min(apart_of(min(p + 2 * i, a.parts - 1)), 63), mine_count += n[i];
+  const Weigher weigher(s.table, r.temperature, a.shift, t.exponent);
+  if (lists_parts(f)) {
+    if (__any(mine.listed > PART_LIST) || !draw_listed(s, a, work, row, r, f, weigher, out)) search_row(s.search, r, f, out);
+    return;
   }
-  if (threadIdx.x >= BINS) s.half_mass[threadIdx.x % BINS] = mine, s.half_count[threadIdx.x % BINS] = mine_count;
-  __syncthreads();
-  if (threadIdx.x < BINS) mine += s.half_mass[threadIdx.x], mine_count += s.half_count[threadIdx.x];
-  else mine = mine_count = 0;
-  uint64_t total, ignored;
-  mine = block_scan(s, mine, total);
-  if (threadIdx.x < BINS) s.mass[threadIdx.x] = mine;
-  if (a.counting) {
-    mine = block_scan(s, mine_count, ignored);
-    if (threadIdx.x < BINS) s.count[threadIdx.x] = (uint32_t)mine;
-  }
-  // the keys of a bin: [low, high)
-  auto bin_keys = [&](int bin, uint32_t& low, uint32_t& high) {
-    const double floor8 = (double)OCTAVE * exponent - 1 - bin;
-    low = first_key(weigher, floor8), high = first_key(weigher, floor8 + 1);
-  };
-  auto weight = [&](uint32_t key) {
-    int bin;
-    return weigher.weight(logit_of(key), exponent, bin);
-  };
 
+  const RowState state = work.rows[row];
+  const uint64_t* sums = work.sums + (int64_t)row * BINS;
+  uint64_t total = sums[BINS - 1];
+  const uint64_t upto = threadIdx.x < BINS ? sums[threadIdx.x] : total;
+  const uint64_t here = threadIdx.x < BINS ? upto - (threadIdx.x ? sums[threadIdx.x - 1] : 0) : 0;
   Cut cut{order_key(-INFINITY), -1};  // every finite logit
-  int cut_bin = BINS;                 // the bin that it cuts: those above are whole
-  int listed = 0;                     // tokens of that bin, ranked
-  if (f.top_k > 0 && f.top_k < a.vocab) {
-    uint64_t before;
-    const int bin = bin_of(s, s.count, (uint64_t)f.top_k, before);
-    if (bin < BINS) {
-      uint32_t low, high;
-      bin_keys(bin, low, high);
-      const int n = rank_tokens(s, r, low, high, cut), keep = (int)(f.top_k - (int64_t)before);
-      if (n > LIST) return search_row(s.search, r, f, out);
-      total = bin ? s.mass[bin - 1] : 0;
-      uint64_t sum = 0;
-      for (int i = threadIdx.x; i < keep && i < n; i += THREADS) sum += weight(key_at(s, i));
-      uint64_t more;
-      block_scan(s, sum, more);
-      total += more;
-      const int last = min(keep, n) - 1;
-      cut = Cut{key_at(s, last), (int)(uint32_t)s.ranked[last]}, cut_bin = bin, listed = n;
-    }
-  }
-  if (f.top_p < 1. || f.min_p > 0.) {
-    uint64_t need = ~0ull, before = 0;
-    int p_bin = BINS, m_bin = BINS;
-    if (f.top_p < 1.) {
-      need = share_of(fmax(f.top_p, 0.), total, true);
-      need = need ? need : 1;
-      p_bin = bin_of(s, s.mass, need, before);
-    }
-    if (f.min_p > 0.) {
-      const double at = (double)OCTAVE * exponent - 1 - floor(8. * (weigher.exponent(r.top) + log2(f.min_p)));
-      m_bin = at < BINS ? (int)at : BINS;
-    }
-    const int bin = min(p_bin, m_bin);
-    if (bin < BINS && bin <= cut_bin) {
-      uint32_t low, high;
-      bin_keys(bin, low, high);
-      const int n = rank_tokens(s, r, low, high, cut);
-      if (n > LIST) return search_row(s.search, r, f, out);
-      // the first `keep` of the ranked tokens stay
-      __syncthreads();
-      if (threadIdx.x == 0) s.listed = n;
-      __syncthreads();
-      uint64_t sum = bin ? s.mass[bin - 1] : 0;
-      for (int i0 = 0; i0 < n; i0 += THREADS) {
-        const int i = i0 + threadIdx.x;
-        const uint32_t key = i < n ? key_at(s, i) : 0u;
-        uint64_t here = i < n ? weight(key) : 0, all;
-        const uint64_t upto = sum + block_scan(s, here, all);
-        if (i < n && bin == p_bin && upto >= need) atomicMin(&s.listed, i + 1);
-        if (i < n && bin == m_bin && !(r.weight(logit_of(key)) >= f.min_p)) atomicMin(&s.listed, i);
-        sum += all;
+  int cut_bin = state.bin, n = 0;     // the bin that it cuts, whose n tokens are ranked: the bins above are whole
+  if (cut_bin < BINS) {
+    n = state.listed;
+    if (n > LIST) return search_row(s.search, r, f, out);
+    for (int i = threadIdx.x; i < n; i += THREADS) s.list[i] = work.lists[(int64_t)row * LIST + i];
+    __syncthreads();
+    rank_list(s, n, [](uint64_t x) { return x; });
+    const uint64_t above = cut_bin ? sums[cut_bin - 1] : 0;
+    const bool by_rank = f.top_k > 0 && f.top_k < a.vocab && cut_bin < BINS &&
+                         work.count_sums[(int64_t)row * BINS + cut_bin] >= (uint64_t)f.top_k;
+    int keep;
+    uint64_t need = ~0ull;
+    if (by_rank) {
+      keep = min(n, (int)(f.top_k - (cut_bin ? (int64_t)work.count_sums[(int64_t)row * BINS + cut_bin - 1] : 0)));
+      uint64_t sum = 0, more;
+      for (int i = threadIdx.x; i < keep; i += THREADS) sum += weigher.weight(logit_of(key_of(s.ranked[i])));
+      block_scan<THREADS / 64>(s.bins.sums, sum, more);
+      total = above + more;
+      if (f.top_p < 1. || f.min_p > 0.) {
+        uint64_t before;
+        int bin = BINS;
+        if (f.top_p < 1.) {
+          need = share_of(fmax(f.top_p, 0.), total, true);
+          need = need ? need : 1;
+          bin = bin_of(s.bins, upto, here, need, before);
+        }
+        const int m_bin = min_p_bin(weigher, r.top, f.min_p);
+        if (min(bin, m_bin) < cut_bin) {  // another bin is cut: its tokens are to be found first
+          cut = Cut{key_of(s.ranked[keep - 1]), index_of(s.ranked[keep - 1])};
+          cut_bin = min(bin, m_bin);
+          const int eighth = OCTAVE * t.exponent - cut_bin;
+          n = rank_tokens(s, r, weigher.first_key(eighth), weigher.first_key(eighth + 1), cut);
+          if (n > LIST) return search_row(s.search, r, f, out);
+          keep = n;
+        }
+        keep = kept_of(s, r, weigher, keep, cut_bin ? sums[cut_bin - 1] : 0, need, f.min_p);
       }
-      __syncthreads();
-      const int keep = s.listed;
-      cut = keep ? Cut{key_at(s, keep - 1), (int)(uint32_t)s.ranked[keep - 1]} : Cut{high - 1, -1};
-      cut_bin = bin, listed = n;
+    } else {
+      if (f.top_p < 1.) need = share_of(fmax(f.top_p, 0.), total, true);
+      keep = kept_of(s, r, weigher, n, above, need ? need : 1, f.min_p);
     }
+    cut = keep ? Cut{key_of(s.ranked[keep - 1]), index_of(s.ranked[keep - 1])}
+               : Cut{weigher.first_key(OCTAVE * t.exponent - cut_bin + 1) - 1, -1};
   }
 
-  // the kept weight of every part: whole bins, and what the cut one keeps (its tokens are listed)
+  // the kept weight of every part: whole bins, and what the cut one keeps
+  const uint64_t* masses = work.masses + (int64_t)row * a.parts * BINS;
   if (threadIdx.x < MAX_PARTS) s.part_mass[threadIdx.x] = 0;
   __syncthreads();
   for (int p = wave; p < a.parts; p += THREADS / 64) {
-    const int apart = apart_of(p);
-    if (apart > a.shift) continue;
-    uint64_t sum = 0;
+    const int apart = apart_of(t.exponent, s.exponents[p]), end = min(cut_bin, OCTAVE * a.shift + 1) - OCTAVE * apart;
+    uint64_t m[BINS / 64], sum = 0;
 #pragma unroll
-    for (int i = 0; i < BINS / 64; ++i)
-      if (const int b = 64 * i + lane; b < min(cut_bin, bins) - apart * OCTAVE) sum += masses[(int64_t)p * BINS + b] >> apart;
+    for (int i = 0; i < BINS / 64; ++i) m[i] = 64 * i + lane < end ? masses[(int64_t)p * BINS + 64 * i + lane] : 0;
+#pragma unroll
+    for (int i = 0; i < BINS / 64; ++i) sum += m[i] >> min(apart, 63);
     sum = wave_scan(sum);
     if (lane == 63) s.part_mass[p] = sum;
   }
   __syncthreads();
-  if (cut_bin < BINS)
-    for (int i = threadIdx.x; i < listed; i += THREADS) {
-      const uint32_t key = key_at(s, i);
-      const int token = (int)(uint32_t)s.ranked[i];
-      if (cut.takes(key, token))
-        atomicAdd(reinterpret_cast<unsigned long long*>(&s.part_mass[token / a.part_len]), (unsigned long long)weight(key));
-    }
+  for (int i = threadIdx.x; i < n; i += THREADS) {
+    const uint64_t token = s.ranked[i];
+    if (cut.takes(key_of(token), index_of(token)))
+      atomicAdd(reinterpret_cast<unsigned long long*>(&s.part_mass[index_of(token) / a.part_len]),
+                (unsigned long long)weigher.weight(logit_of(key_of(token))));
+  }
   __syncthreads();
   const uint64_t parts_upto = wave_scan(s.part_mass[lane]);  // lane p: the kept weight of parts up to p
   total = shfl64(parts_upto, 63);
@@ -597,26 +855,30 @@ __global__ __launch_bounds__(THREADS) void draw_kernel(Args a, const Part* parts
   const int part = __ffsll((unsigned long long)__ballot(parts_upto > target)) - 1;
   target -= shfl64(parts_upto, part) - s.part_mass[part];
 
-  // the part, in order: a consecutive run of tokens a thread
-  const int from = part * a.part_len, to = min(a.vocab, from + a.part_len), run = (to - from + THREADS - 1) / THREADS;
-  const int begin = min(to, from + (int)threadIdx.x * run), end = min(to, begin + run);
-  auto kept = [&](int i) -> uint64_t {
-    const uint32_t key = order_key(r.at(i));
-    return cut.takes(key, i) ? weight(key) : 0;
+  // the part, in order: each wave a consecutive run, a lane a token
+  const int from = part * a.part_len, to = min(a.vocab, from + a.part_len);
+  const int run = ((to - from + THREADS / 64 - 1) / (THREADS / 64) + 63) & ~63, begin = min(to, from + wave * run), end = min(to, begin + run);
+  auto kept = [&](int i, float x) -> uint64_t {
+    const uint32_t key = order_key(x);
+    return cut.takes(key, i) ? weigher.weight(x) : 0;
   };
   uint64_t sum = 0, all;
-  for (int i = begin; i < end; ++i) sum += kept(i);
-  uint64_t upto = block_scan(s, sum, all);
+  r.template each<8, 64>(begin + lane, end, [&](int i, float x) { sum += kept(i, x); });
+  const uint64_t wave_upto = shfl64(wave_scan(sum), 63);
+  uint64_t before = block_scan<THREADS / 64>(s.bins.sums, lane == 0 ? wave_upto : 0, all);
+  before = shfl64(before, 63) - wave_upto;
   // (bins' sums were rounded down once, tokens' one by one: their total may be a few units short)
   if (target >= all) target = all - 1;
-  if (all == 0 || target >= upto || target < upto - sum) return;
-  upto -= sum;
-  for (int i = begin; i < end; ++i) {
-    upto += kept(i);
-    if (upto > target) {
-      *out = i;
+  if (target < before || target >= before + wave_upto) return;
+  for (int i0 = begin; i0 < end; i0 += 64) {
+    const int i = i0 + lane;
+    const uint64_t passed = before + wave_scan(i < end ? kept(i, r.at(i)) : 0);
+    const uint64_t over = __ballot(passed > target);
+    if (over) {
+      if (lane == 0) *out = i0 + __ffsll((unsigned long long)over) - 1;
       return;
     }
+    before = shfl64(passed, 63);
   }
 }
 
@@ -627,10 +889,37 @@ static int parts_of(int rows, int vocab) {
   return n < MAX_PARTS ? (int)n : MAX_PARTS;
 }
 
+// Workspace of `rows` rows (at most ROWS at a time), laid out at `at`; returns its bytes.
+static int64_t work_of(int rows, int vocab, void* at, Work* w) {
+  const int64_t n = rows < ROWS ? rows : ROWS, slots = n * parts_of((int)n, vocab);
+  uint8_t* p = static_cast<uint8_t*>(at);
+  int64_t bytes = 0;
+  auto take = [&](int64_t size) {
+    const int64_t here = bytes;
+    bytes += (size + 255) & ~(int64_t)255;
+    return p + here;
+  };
+  Work x;
+  x.masses = reinterpret_cast<uint64_t*>(take(slots * BINS * 8));
+  x.part_list = reinterpret_cast<uint64_t*>(take(slots * PART_LIST * 8));
+  x.sums = reinterpret_cast<uint64_t*>(take(n * BINS * 8));
+  x.lists = reinterpret_cast<uint64_t*>(take(n * LIST * 8));
+  x.parts = reinterpret_cast<Part*>(take(slots * (int64_t)sizeof(Part)));
+  x.rows = reinterpret_cast<RowState*>(take(n * (int64_t)sizeof(RowState)));
+  x.counts = reinterpret_cast<uint32_t*>(take(slots * BINS * 4));
+  x.count_sums = reinterpret_cast<uint32_t*>(take(n * BINS * 4));
+  if (w) *w = x;
+  return bytes;
+}
+
 template <class T>
-static void launch(const Args& a, int rows, Part* parts, uint64_t* masses, uint32_t* counts, hipStream_t st) {
-  hipLaunchKernelGGL(weigh_kernel<T>, dim3(a.parts, rows), dim3(WEIGH_THREADS), 0, st, a, parts, masses, counts);
-  hipLaunchKernelGGL(draw_kernel<T>, dim3(rows), dim3(THREADS), 0, st, a, parts, masses, counts);
+static void launch(const Args& a, int rows, const Work& work, bool all_listed, hipStream_t st) {
+  hipLaunchKernelGGL(weigh_kernel<T>, dim3(a.parts, rows), dim3(WEIGH_THREADS), 0, st, a, work);
+  if (!all_listed) {
+    hipLaunchKernelGGL(pick_kernel<T>, dim3(rows), dim3(BINS), 0, st, a, work);
+    hipLaunchKernelGGL(gather_kernel<T>, dim3(a.parts, rows), dim3(WEIGH_THREADS), 0, st, a, work);
+  }
+  hipLaunchKernelGGL(draw_kernel<T>, dim3(rows), dim3(THREADS), 0, st, a, work);
 }
 
 }  // namespace sample
@@ -642,7 +931,7 @@ extern "C" {
 
 int64_t dkv_sample_workspace_bytes(int32_t rows, int32_t vocab) {
   if (rows <= 0 || vocab <= 0 || vocab > 1 << 22) return 0;
-  return (int64_t)rows * sample::parts_of(rows, vocab) * (sizeof(sample::Part) + sample::BINS * (8 + 4));
+  return sample::work_of(rows, vocab, nullptr, nullptr);
 }
 
 int dkv_sample(const void* logits, int32_t dtype, int64_t row_stride, int32_t rows, int32_t vocab, const void* u, int32_t u_dtype,
@@ -678,16 +967,14 @@ int dkv_sample(const void* logits, int32_t dtype, int64_t row_stride, int32_t ro
   a.vocab = vocab, a.u_dtype = u_dtype, a.p = p;
   a.shift = 62;
   while (a.shift > 50 || ((uint64_t)vocab >> (62 - a.shift)) > 0) --a.shift;  // vocab << shift stays below 2^62
-  a.parts = sample::parts_of(rows, vocab), a.part_len = (vocab + a.parts - 1) / a.parts;
+  a.parts = sample::parts_of(rows < sample::ROWS ? rows : sample::ROWS, vocab);
+  a.part_len = (vocab + a.parts - 1) / a.parts;
   a.counting = p.top_k_rows || (p.top_k > 0 && p.top_k < vocab);
-  const int64_t slots = (int64_t)rows * a.parts;
-  uint64_t* masses = static_cast<uint64_t*>(workspace);
-  sample::Part* parts = reinterpret_cast<sample::Part*>(masses + slots * sample::BINS);
-  uint32_t* counts = reinterpret_cast<uint32_t*>(parts + slots);
-  const hipStream_t st = (hipStream_t)stream;
-  // (the second grid dimension holds 65535 rows)
-  for (int at = 0; at < rows; at += 65535) {
-    const int n = rows - at < 65535 ? rows - at : 65535;
+  sample::Work work;
+  sample::work_of(rows, vocab, workspace, &work);
+  const bool all_listed = !p.top_k_rows && p.top_k > 0 && p.top_k <= sample::SMALL_K;
+  for (int at = 0; at < rows; at += sample::ROWS) {
+    const int n = rows - at < sample::ROWS ? rows - at : sample::ROWS;
     sample::Args b = a;
     b.logits = static_cast<const uint8_t*>(logits) + at * row_stride * (dtype == 0 ? 2 : 4);
     b.u = static_cast<const uint8_t*>(u) + (int64_t)at * (u_dtype ? 8 : 4);
@@ -696,9 +983,8 @@ int dkv_sample(const void* logits, int32_t dtype, int64_t row_stride, int32_t ro
     if (p.top_p_rows) b.p.top_p_rows += at;
     if (p.min_p_rows) b.p.min_p_rows += at;
     if (p.top_k_rows) b.p.top_k_rows += at;
-    const int64_t slot = (int64_t)at * a.parts;
-    if (dtype == 0) sample::launch<uint16_t>(b, n, parts + slot, masses + slot * sample::BINS, counts + slot * sample::BINS, st);
-    else sample::launch<float>(b, n, parts + slot, masses + slot * sample::BINS, counts + slot * sample::BINS, st);
+    if (dtype == 0) sample::launch<uint16_t>(b, n, work, all_listed, (hipStream_t)stream);
+    else sample::launch<float>(b, n, work, all_listed, (hipStream_t)stream);
   }
   return (int)hipGetLastError();
 }
