@@ -23,7 +23,7 @@
 namespace dkv {
 namespace sample {
 
-constexpr int THREADS = 1024;
+constexpr int THREADS = 512;
 
 template <class T>  // uint16_t: bf16
 struct Row {
@@ -255,6 +255,7 @@ constexpr int WEIGH_THREADS = 256;
 constexpr int HELD = 32;               // tokens a thread of weigh_kernel keeps in registers, where a part is that small
 constexpr int OCTAVE = 8, BINS = 512;  // bins of an octave of weight; at most 8 * 50 + 1 are used
 constexpr int STEPS = 256;             // steps of the table of 2^f
+constexpr int SUBS = STEPS / OCTAVE;   // of them in a bin
 constexpr int LIST = 4096;             // tokens of a bin that is cut
 constexpr int SMALL_K = 256;           // top_k whose tokens are listed by the parts
 constexpr int PART_LIST = 512;         // tokens that a part lists
@@ -335,16 +336,18 @@ struct Weigher {
     int bin;
     return weight(x, bin);
   }
-  // The smallest key of a bin: the first whose step is 32 * eighth or more, by weight()'s own arithmetic. The border is
-  // half a step below the eighth; a float that near it is at most a few keys off.
-  __device__ __forceinline__ uint32_t first_key(int eighth) const {
-    const float x = (float)((eighth * (1. / OCTAVE) - .5 / STEPS) / rate);
+  // The smallest key whose step is `first` or more, by weight()'s own arithmetic. The border is half a step below; a
+  // float that near it is at most a few keys off.
+  __device__ __forceinline__ uint32_t first_key(int first) const {
+    const float x = (float)((first - .5) / STEPS / rate);
     uint32_t key = order_key(fminf(fmaxf(x, -3.4028235e38f), 3.4028235e38f));
-    auto reaches = [&](uint32_t k) { return step(logit_of(k)) >> 5 >= eighth; };
+    auto reaches = [&](uint32_t k) { return step(logit_of(k)) >= first; };
     for (int i = 0; i < 8 && reaches(key - 1); ++i) --key;
     for (int i = 0; i < 8 && !reaches(key); ++i) ++key;
     return key;
   }
+  // The smallest step of a bin.
+  __device__ __forceinline__ int bin_step(int bin) const { return SUBS * (OCTAVE * exponent - bin); }
 };
 
 template <class T>
@@ -517,12 +520,12 @@ __device__ __forceinline__ int bin_of(BinScratch& s, uint64_t upto, uint64_t her
   return s.bin;
 }
 
-// The first bin in which min_p cuts.
-__device__ __forceinline__ int min_p_bin(const Weigher& w, float top, double min_p) {
-  if (!(min_p > 0.)) return BINS;
-  const int k = (int)(uint32_t)__builtin_bit_cast(uint64_t, (double)top * w.rate + log2(min_p) + Weigher::magic());
-  const int64_t bin = (int64_t)OCTAVE * w.exponent - (k >> 5);
-  return min_p < 1e-300 || bin >= BINS ? BINS : (int)bin;
+// The bin in which min_p cuts, and the step there.
+__device__ __forceinline__ int min_p_bin(const Weigher& w, float top, double min_p, int& step) {
+  step = INT32_MIN;
+  if (!(min_p > 1e-300)) return BINS;
+  step = (int)(uint32_t)__builtin_bit_cast(uint64_t, (double)top * w.rate + log2(min_p) + Weigher::magic());
+  return (int)min((int64_t)OCTAVE * w.exponent - (step >> 5), (int64_t)BINS);
 }
 
 // A workgroup a row (BINS threads, a bin each): joins the parts' bins and finds the first that a filter cuts.
@@ -577,13 +580,14 @@ __global__ __launch_bounds__(BINS) void pick_kernel(Args a, Work work) {
       const uint64_t need = share_of(fmax(f.top_p, 0.), total, true);
       cut = bin_of(s, upto, mass, need ? need : 1, before);
     }
-    cut = min(cut, min_p_bin(weigher, t.top, f.min_p));
+    int step;
+    cut = min(cut, min_p_bin(weigher, t.top, f.min_p, step));
   }
   if (threadIdx.x == 0) {
     state.bin = cut;
     if (cut < BINS) {
-      const int eighth = OCTAVE * t.exponent - cut;
-      state.low = max(weigher.first_key(eighth), order_key(-INFINITY) + 1), state.high = weigher.first_key(eighth + 1);
+      state.low = max(weigher.first_key(weigher.bin_step(cut)), order_key(-INFINITY) + 1);
+      state.high = weigher.first_key(weigher.bin_step(cut - 1));
     }
     work.rows[row] = state;
   }
@@ -600,67 +604,85 @@ __global__ __launch_bounds__(WEIGH_THREADS) void gather_kernel(Args a, Work work
   RowState* state = work.rows + row;
   const uint32_t low = state->low, high = state->high;
   if (state->search || state->bin == BINS || order_key(p.top) < low) return;
+  __shared__ uint64_t found[LIST];
+  __shared__ int n, first;
+  if (threadIdx.x == 0) n = 0;
+  __syncthreads();
   const int from = part * a.part_len, to = min(a.vocab, from + a.part_len);
   r.template each<16, WEIGH_THREADS>(from + threadIdx.x, to, [&](int i, float x) {
     const uint32_t key = order_key(x);
     if (key >= low && key < high) {
-      const int at = atomicAdd(&state->listed, 1);
-      if (at < LIST) work.lists[(int64_t)row * LIST + at] = token_of(key, i);
+      const int at = atomicAdd(&n, 1);
+      if (at < LIST) found[at] = token_of(key, i);
     }
   });
+  __syncthreads();
+  if (threadIdx.x == 0 && n) first = atomicAdd(&state->listed, n);  // (one of a thousand a row at most: they go one by one)
+  __syncthreads();
+  for (int i = threadIdx.x; i < n && i < LIST && first + i < LIST; i += WEIGH_THREADS) work.lists[(int64_t)row * LIST + first + i] = found[i];
 }
 
 struct DrawScratch {
   union {
     Scratch search;
     struct {
-      uint64_t list[LIST];    // tokens as found
-      uint64_t ranked[LIST];  // by falling key, then index
+      uint64_t list[LIST];  // tokens of a bin
+      uint64_t few[LIST];   // those of them that need ranking: by falling key, then index
     };
   };
   double table[STEPS];
   BinScratch bins;
+  uint64_t sub_mass[SUBS];
+  uint32_t sub_count[SUBS];
   uint32_t count[BINS];
   uint64_t part_mass[MAX_PARTS];
   int exponents[MAX_PARTS], listed[MAX_PARTS];
   int ranks[THREADS];
-  int n, keep;
+  int n, keep, sub;
+  uint64_t sub_before;
+  uint32_t sub_rank;
 };
 
-// ranked = list's n values, rising by order(value) (all different): each counts those before it, several threads a value
+// few's n values in the order of order(value) (all different): each counts those before it, several threads a value
 // where there are few.
 template <class Order>
-__device__ __forceinline__ void rank_list(DrawScratch& s, int n, Order order) {
+__device__ __forceinline__ void rank_few(DrawScratch& s, int n, Order order) {
   int slices = 1;
   while (slices < 16 && 2 * slices * n <= THREADS) slices *= 2;
-  if (slices == 1) {
-    for (int i = threadIdx.x; i < n; i += THREADS) {
-      const uint64_t x = s.list[i];
-      int rank = 0;
-#pragma unroll 4
-      for (int j = 0; j < n; ++j) rank += order(s.list[j]) < order(x);
-      s.ranked[rank] = x;
-    }
-  } else {
-    s.ranks[threadIdx.x] = 0;
-    __syncthreads();
+  uint64_t x[LIST / THREADS];
+  int rank[LIST / THREADS];
+  s.ranks[threadIdx.x] = 0;
+  __syncthreads();
+  if (slices > 1) {
     const int i = threadIdx.x % (THREADS / slices), slice = threadIdx.x / (THREADS / slices);
     if (i < n) {
-      const uint64_t x = s.list[i];
-      int rank = 0;
+      const auto mine = order(s.few[i]);
+      int before = 0;
 #pragma unroll 4
-      for (int j = slice; j < n; j += slices) rank += order(s.list[j]) < order(x);
-      atomicAdd(&s.ranks[i], rank);
+      for (int j = slice; j < n; j += slices) before += order(s.few[j]) < mine;
+      atomicAdd(&s.ranks[i], before);
     }
     __syncthreads();
-    if (threadIdx.x < n) s.ranked[s.ranks[threadIdx.x]] = s.list[threadIdx.x];
   }
+#pragma unroll
+  for (int k = 0; k < LIST / THREADS; ++k) {
+    const int i = k * THREADS + threadIdx.x;
+    if (i >= n) continue;
+    x[k] = s.few[i], rank[k] = slices > 1 ? s.ranks[i] : 0;
+    if (slices == 1)
+#pragma unroll 4
+      for (int j = 0; j < n; ++j) rank[k] += order(s.few[j]) < order(x[k]);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < LIST / THREADS; ++k)
+    if (k * THREADS + (int)threadIdx.x < n) s.few[rank[k]] = x[k];
   __syncthreads();
 }
 
-// Lists and ranks the row's tokens with keys in [low, high) that `cut` takes, reading all of it. Returns how many.
+// Lists the row's tokens with keys in [low, high) that `cut` takes, reading all of it. Returns how many.
 template <class T>
-__device__ __forceinline__ int rank_tokens(DrawScratch& s, const Row<T>& r, uint32_t low, uint32_t high, const Cut& cut) {
+__device__ __forceinline__ int list_tokens(DrawScratch& s, const Row<T>& r, uint32_t low, uint32_t high, const Cut& cut) {
   __syncthreads();
   if (threadIdx.x == 0) s.n = 0;
   __syncthreads();
@@ -672,22 +694,20 @@ __device__ __forceinline__ int rank_tokens(DrawScratch& s, const Row<T>& r, uint
     }
   });
   __syncthreads();
-  const int n = s.n;
-  if (n <= LIST) rank_list(s, n, [](uint64_t x) { return x; });
-  return n;
+  return s.n;
 }
 
-// How many of the n ranked tokens stay: up to the one at which the weight, `sum` before them, reaches `need`, and while
-// w >= min_p.
+// How many of few's n ranked tokens stay: at most `most`, up to the one at which the weight, `sum` before them, reaches
+// `need`, and while w >= min_p.
 template <class T>
-__device__ __forceinline__ int kept_of(DrawScratch& s, const Row<T>& r, const Weigher& weigher, int n, uint64_t sum, uint64_t need,
-                                       double min_p) {
+__device__ __forceinline__ int kept_of(DrawScratch& s, const Row<T>& r, const Weigher& weigher, int n, int64_t most, uint64_t sum,
+                                       uint64_t need, double min_p) {
   __syncthreads();
-  if (threadIdx.x == 0) s.keep = n;
+  if (threadIdx.x == 0) s.keep = (int)min((int64_t)n, most);
   __syncthreads();
   for (int i0 = 0; i0 < n; i0 += THREADS) {
     const int i = i0 + threadIdx.x;
-    const float x = i < n ? logit_of(key_of(s.ranked[i])) : -INFINITY;
+    const float x = i < n ? logit_of(key_of(s.few[i])) : -INFINITY;
     uint64_t all;
     const uint64_t upto = sum + block_scan<THREADS / 64>(s.bins.sums, i < n ? weigher.weight(x) : 0, all);
     if (i < n && upto >= need) atomicMin(&s.keep, i + 1);
@@ -696,6 +716,49 @@ __device__ __forceinline__ int kept_of(DrawScratch& s, const Row<T>& r, const We
   }
   __syncthreads();
   return s.keep;
+}
+
+// Where a filter cuts the bin whose n tokens are listed: after the token at which their weight, `sum` before them,
+// reaches `need`, after `rank` of them, or where w < min_p (min_step: the step of that, if it is in this bin). Only the
+// tokens of one step are ranked.
+template <class T>
+__device__ __forceinline__ Cut cut_bin_at(DrawScratch& s, const Row<T>& r, const Weigher& weigher, int bin, int n, const Cut& within,
+                                          uint64_t sum, uint64_t need, int64_t rank, double min_p, int min_step) {
+  auto sub_of = [&](uint64_t token) { return SUBS - 1 - (weigher.step(logit_of(key_of(token))) & (SUBS - 1)); };
+  auto takes = [&](uint64_t token) { return within.takes(key_of(token), index_of(token)); };
+  __syncthreads();
+  if (threadIdx.x < SUBS) s.sub_mass[threadIdx.x] = 0, s.sub_count[threadIdx.x] = 0;
+  if (threadIdx.x == 0) s.n = 0, s.sub = SUBS;
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += THREADS) {
+    const uint64_t token = s.list[i];
+    if (!takes(token)) continue;
+    const int sub = sub_of(token);
+    atomicAdd(reinterpret_cast<unsigned long long*>(&s.sub_mass[sub]), (unsigned long long)weigher.weight(logit_of(key_of(token))));
+    atomicAdd(&s.sub_count[sub], 1u);
+  }
+  __syncthreads();
+  if (threadIdx.x < 64) {
+    const int lane = threadIdx.x;
+    const uint64_t mass = lane < SUBS ? s.sub_mass[lane] : 0, count = lane < SUBS ? s.sub_count[lane] : 0;
+    const uint64_t upto = sum + wave_scan(mass), ranks = wave_scan(count);
+    const int min_sub = min_step >> 5 == OCTAVE * weigher.exponent - bin ? SUBS - 1 - (min_step & (SUBS - 1)) : SUBS;
+    const uint64_t cuts = __ballot(lane < SUBS && (upto >= need || (int64_t)ranks >= rank || lane == min_sub));
+    if (cuts && lane == __ffsll((unsigned long long)cuts) - 1) s.sub = lane, s.sub_before = upto - mass, s.sub_rank = (uint32_t)(ranks - count);
+  }
+  __syncthreads();
+  const int sub = s.sub;
+  if (sub == SUBS) return Cut{weigher.first_key(weigher.bin_step(bin)) - 1, -1};  // (sums a few units short: all of it)
+  for (int i = threadIdx.x; i < n; i += THREADS) {
+    const uint64_t token = s.list[i];
+    if (takes(token) && sub_of(token) == sub) s.few[atomicAdd(&s.n, 1)] = token;
+  }
+  __syncthreads();
+  const int few = s.n;
+  rank_few(s, few, [](uint64_t x) { return x; });
+  const int keep = kept_of(s, r, weigher, few, rank - s.sub_rank, s.sub_before, need, min_p);
+  if (keep) return Cut{key_of(s.few[keep - 1]), index_of(s.few[keep - 1])};
+  return Cut{few ? key_of(s.few[0]) : weigher.first_key(weigher.bin_step(bin) + SUBS - sub) - 1, -1};
 }
 
 // A row whose parts listed what the first top_k can be among: all of it from the lists.
@@ -725,26 +788,24 @@ __device__ __forceinline__ bool draw_listed(DrawScratch& s, const Args& a, const
   each([&](uint64_t token, int bin) {
     if (bin <= last) {
       const int to = atomicAdd(&s.n, 1);
-      if (to < LIST) s.list[to] = token;
+      if (to < LIST) s.few[to] = token;
     }
   });
   __syncthreads();
   int n = s.n;
   if (n > LIST) return false;
-  rank_list(s, n, [](uint64_t x) { return x; });
+  rank_few(s, n, [](uint64_t x) { return x; });
   n = min(n, (int)f.top_k);
   // (top_k is at most SMALL_K: a token a thread from here on)
   uint64_t total;
-  const uint64_t w = (int)threadIdx.x < n ? weigher.weight(logit_of(key_of(s.ranked[threadIdx.x]))) : 0;
+  const uint64_t w = (int)threadIdx.x < n ? weigher.weight(logit_of(key_of(s.few[threadIdx.x]))) : 0;
   block_scan<THREADS / 64>(s.bins.sums, w, total);
   uint64_t need = ~0ull;
   if (f.top_p < 1.) need = share_of(fmax(f.top_p, 0.), total, true);
-  n = kept_of(s, r, weigher, n, 0, need ? need : 1, f.min_p);
+  n = kept_of(s, r, weigher, n, n, 0, need ? need : 1, f.min_p);
   // by index, then the token at which the weight passes the target
-  if ((int)threadIdx.x < n) s.list[threadIdx.x] = s.ranked[threadIdx.x];
-  __syncthreads();
-  rank_list(s, n, [](uint64_t x) { return (uint32_t)x; });
-  const uint64_t token = (int)threadIdx.x < n ? s.ranked[threadIdx.x] : 0;
+  rank_few(s, n, [](uint64_t x) { return (uint32_t)x; });
+  const uint64_t token = (int)threadIdx.x < n ? s.few[threadIdx.x] : 0;
   const uint64_t weight = (int)threadIdx.x < n ? weigher.weight(logit_of(key_of(token))) : 0;
   const uint64_t sum = block_scan<THREADS / 64>(s.bins.sums, weight, total);
   const uint64_t target = target_of(f.u, total);
@@ -782,49 +843,35 @@ __global__ __launch_bounds__(THREADS) void draw_kernel(Args a, Work work) {
   const uint64_t upto = threadIdx.x < BINS ? sums[threadIdx.x] : total;
   const uint64_t here = threadIdx.x < BINS ? upto - (threadIdx.x ? sums[threadIdx.x - 1] : 0) : 0;
   Cut cut{order_key(-INFINITY), -1};  // every finite logit
-  int cut_bin = state.bin, n = 0;     // the bin that it cuts, whose n tokens are ranked: the bins above are whole
+  int cut_bin = state.bin, n = 0;     // the bin that it cuts, whose n tokens are listed: the bins above are whole
   if (cut_bin < BINS) {
     n = state.listed;
     if (n > LIST) return search_row(s.search, r, f, out);
     for (int i = threadIdx.x; i < n; i += THREADS) s.list[i] = work.lists[(int64_t)row * LIST + i];
-    __syncthreads();
-    rank_list(s, n, [](uint64_t x) { return x; });
-    const uint64_t above = cut_bin ? sums[cut_bin - 1] : 0;
-    const bool by_rank = f.top_k > 0 && f.top_k < a.vocab && cut_bin < BINS &&
-                         work.count_sums[(int64_t)row * BINS + cut_bin] >= (uint64_t)f.top_k;
-    int keep;
-    uint64_t need = ~0ull;
+    const uint32_t* counts = work.count_sums + (int64_t)row * BINS;
+    const bool by_rank = f.top_k > 0 && f.top_k < a.vocab && counts[cut_bin] >= (uint64_t)f.top_k;
     if (by_rank) {
-      keep = min(n, (int)(f.top_k - (cut_bin ? (int64_t)work.count_sums[(int64_t)row * BINS + cut_bin - 1] : 0)));
+      cut = cut_bin_at(s, r, weigher, cut_bin, n, cut, 0, ~0ull, f.top_k - (cut_bin ? (int64_t)counts[cut_bin - 1] : 0), 0., INT32_MIN);
       uint64_t sum = 0, more;
-      for (int i = threadIdx.x; i < keep; i += THREADS) sum += weigher.weight(logit_of(key_of(s.ranked[i])));
+      for (int i = threadIdx.x; i < n; i += THREADS)
+        if (cut.takes(key_of(s.list[i]), index_of(s.list[i]))) sum += weigher.weight(logit_of(key_of(s.list[i])));
       block_scan<THREADS / 64>(s.bins.sums, sum, more);
-      total = above + more;
-      if (f.top_p < 1. || f.min_p > 0.) {
-        uint64_t before;
-        int bin = BINS;
-        if (f.top_p < 1.) {
-          need = share_of(fmax(f.top_p, 0.), total, true);
-          need = need ? need : 1;
-          bin = bin_of(s.bins, upto, here, need, before);
-        }
-        const int m_bin = min_p_bin(weigher, r.top, f.min_p);
-        if (min(bin, m_bin) < cut_bin) {  // another bin is cut: its tokens are to be found first
-          cut = Cut{key_of(s.ranked[keep - 1]), index_of(s.ranked[keep - 1])};
-          cut_bin = min(bin, m_bin);
-          const int eighth = OCTAVE * t.exponent - cut_bin;
-          n = rank_tokens(s, r, weigher.first_key(eighth), weigher.first_key(eighth + 1), cut);
-          if (n > LIST) return search_row(s.search, r, f, out);
-          keep = n;
-        }
-        keep = kept_of(s, r, weigher, keep, cut_bin ? sums[cut_bin - 1] : 0, need, f.min_p);
-      }
-    } else {
-      if (f.top_p < 1.) need = share_of(fmax(f.top_p, 0.), total, true);
-      keep = kept_of(s, r, weigher, n, above, need ? need : 1, f.min_p);
+      total = (cut_bin ? sums[cut_bin - 1] : 0) + more;
     }
-    cut = keep ? Cut{key_of(s.ranked[keep - 1]), index_of(s.ranked[keep - 1])}
-               : Cut{weigher.first_key(OCTAVE * t.exponent - cut_bin + 1) - 1, -1};
+    uint64_t need = ~0ull, before;
+    if (f.top_p < 1.) need = share_of(fmax(f.top_p, 0.), total, true);
+    need = need ? need : 1;
+    int bin = cut_bin, min_step;
+    const int m_bin = min_p_bin(weigher, r.top, f.min_p, min_step);
+    if (by_rank) {
+      bin = min(m_bin, f.top_p < 1. ? bin_of(s.bins, upto, here, need, before) : BINS);
+      if (bin < cut_bin) {  // another bin is cut: its tokens are to be found first
+        n = list_tokens(s, r, weigher.first_key(weigher.bin_step(bin)), weigher.first_key(weigher.bin_step(bin - 1)), cut);
+        if (n > LIST) return search_row(s.search, r, f, out);
+        cut_bin = bin;
+      }
+    }
+    if (bin <= cut_bin) cut = cut_bin_at(s, r, weigher, bin, n, cut, bin ? sums[bin - 1] : 0, need, INT64_MAX, f.min_p, min_step);
   }
 
   // the kept weight of every part: whole bins, and what the cut one keeps
@@ -843,7 +890,7 @@ __global__ __launch_bounds__(THREADS) void draw_kernel(Args a, Work work) {
   }
   __syncthreads();
   for (int i = threadIdx.x; i < n; i += THREADS) {
-    const uint64_t token = s.ranked[i];
+    const uint64_t token = s.list[i];
     if (cut.takes(key_of(token), index_of(token)))
       atomicAdd(reinterpret_cast<unsigned long long*>(&s.part_mass[index_of(token) / a.part_len]),
                 (unsigned long long)weigher.weight(logit_of(key_of(token))));
