@@ -171,7 +171,7 @@ __device__ __forceinline__ uint64_t target_of(double u, uint64_t total) {
 
 // The whole row by radix searches: right for every row, and slow (every search reads all of it).
 template <class T>
-__device__ __noinline__ void search_row(Scratch& s, const Row<T>& r, const Filters& f, int64_t* out) {
+__device__ __forceinline__ void search_row(Scratch& s, const Row<T>& r, const Filters& f, int64_t* out) {
   const int vocab = r.vocab;
   const int64_t top_k = f.top_k;
   const double top_p = f.top_p, min_p = f.min_p;
@@ -813,12 +813,15 @@ __device__ __forceinline__ bool draw_listed(DrawScratch& s, const Args& a, const
   return true;
 }
 
-template <class T>
+// LISTED: rows whose parts listed their tokens, else the others. (Kernels of their own: in one, with search_row called,
+// scalar registers were spilled into vector registers that were spilled themselves, and a value came back wrong.)
+template <class T, bool LISTED>
 __global__ __launch_bounds__(THREADS) void draw_kernel(Args a, Work work) {
   __shared__ DrawScratch s;
   const int row = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   Row<T> r = row_of<T>(a, row);
   const Filters f = filters_of(a, row);
+  if (lists_parts(f) != LISTED) return;
   const Part mine = part_of(a, work.parts + (int64_t)row * a.parts, lane);
   const RowTop t = row_top(mine);
   int64_t* out = a.out + row;
@@ -832,7 +835,7 @@ __global__ __launch_bounds__(THREADS) void draw_kernel(Args a, Work work) {
   for (int i = threadIdx.x; i < STEPS; i += THREADS) s.table[i] = exp2(i * (1. / STEPS));
   __syncthreads();
   const Weigher weigher(s.table, r.temperature, a.shift, t.exponent);
-  if (lists_parts(f)) {
+  if (LISTED) {
     if (__any(mine.listed > PART_LIST) || !draw_listed(s, a, work, row, r, f, weigher, out)) search_row(s.search, r, f, out);
     return;
   }
@@ -960,13 +963,14 @@ static int64_t work_of(int rows, int vocab, void* at, Work* w) {
 }
 
 template <class T>
-static void launch(const Args& a, int rows, const Work& work, bool all_listed, hipStream_t st) {
+static void launch(const Args& a, int rows, const Work& work, bool some_listed, bool all_listed, hipStream_t st) {
   hipLaunchKernelGGL(weigh_kernel<T>, dim3(a.parts, rows), dim3(WEIGH_THREADS), 0, st, a, work);
   if (!all_listed) {
     hipLaunchKernelGGL(pick_kernel<T>, dim3(rows), dim3(BINS), 0, st, a, work);
     hipLaunchKernelGGL(gather_kernel<T>, dim3(a.parts, rows), dim3(WEIGH_THREADS), 0, st, a, work);
+    hipLaunchKernelGGL((draw_kernel<T, false>), dim3(rows), dim3(THREADS), 0, st, a, work);
   }
-  hipLaunchKernelGGL(draw_kernel<T>, dim3(rows), dim3(THREADS), 0, st, a, work);
+  if (some_listed) hipLaunchKernelGGL((draw_kernel<T, true>), dim3(rows), dim3(THREADS), 0, st, a, work);
 }
 
 }  // namespace sample
@@ -1030,8 +1034,8 @@ int dkv_sample(const void* logits, int32_t dtype, int64_t row_stride, int32_t ro
     if (p.top_p_rows) b.p.top_p_rows += at;
     if (p.min_p_rows) b.p.min_p_rows += at;
     if (p.top_k_rows) b.p.top_k_rows += at;
-    if (dtype == 0) sample::launch<uint16_t>(b, n, work, all_listed, (hipStream_t)stream);
-    else sample::launch<float>(b, n, work, all_listed, (hipStream_t)stream);
+    if (dtype == 0) sample::launch<uint16_t>(b, n, work, p.top_k_rows || all_listed, all_listed, (hipStream_t)stream);
+    else sample::launch<float>(b, n, work, p.top_k_rows || all_listed, all_listed, (hipStream_t)stream);
   }
   return (int)hipGetLastError();
 }
