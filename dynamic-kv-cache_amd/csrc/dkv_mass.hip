@@ -1,9 +1,12 @@
 // Attention mass (gfx950): what every token of the history and the chunk receives of the queries' softmax,
 //   mass(h, t) = sum over the query heads of h and the queries m of exp(s_mt - max_m) / sum_m,
-// the weight by which a cache forgets tokens. Two launches over the keys alone: the first gives every query row
-// its maximum and sum over ranges of units (64 keys), the second joins them and sums each key's column over all
-// rows, so that no sum is shared between workgroups and the result does not depend on their order. A workgroup
-// dequantizes a unit's keys once, as MFMA operands in LDS, and its waves take the 16-row query blocks in turn.
+// the weight by which a cache forgets tokens. Two launches over the keys alone: the first gives every query row its
+// maximum and sum over ranges of units (64 keys), the second joins them and sums each key's column over all rows. No
+// sum is shared between workgroups, so the result does not depend on their order; of long chunks the second launch's
+// workgroups take a part of the rows each, and a third adds the parts up.
+//   - up to 64 query rows a KV head (generated tokens): a wave a unit, keys and queries in registers, nothing in LDS;
+//   - more: a workgroup a unit, whose waves unpack 16 keys each into MFMA operands in LDS and take the 16-row query
+//     blocks in turn.
 #include "dkv_rows.h"
 
 namespace dkv {
@@ -11,12 +14,15 @@ namespace mass {
 
 using namespace rows;
 
+constexpr int FEW = 64;           // query rows of a KV head that a wave takes alone
 constexpr int GROUP = 192;        // query rows of a row group: 12 blocks, three a wave
 constexpr int BLOCKS = GROUP / 64;  // 16-row blocks of a wave
 
 struct MassArgs {
-  int splits, row_groups;
+  int splits, row_groups, row_parts;
   float2* part;      // [heads][splits][rows] maximum (base 2) and sum
+  float* columns;    // [row_parts][heads][stride] sums of a part of the rows (row_parts > 1)
+  int64_t columns_stride;
   float* out;        // [heads] rows of out_stride
   int64_t out_stride;
   int accumulate;
@@ -33,61 +39,78 @@ __device__ __forceinline__ History history_of(const dkv_attn_args& a) {
 }
 
 // Splits of the first launch that run for `units` units: replays split the history they find as a call over that
-// history does.
-__host__ __device__ inline int split_count(int most, int units) { return units < most ? units : most; }
+// history does. A workgroup of few rows has four units at a time.
+__host__ __device__ inline int split_count(int most, int units, bool few) {
+  const int want = few ? (units + 3) / 4 : units;
+  return want < most ? want : most;
+}
 
-// A unit's keys as MFMA operands in LDS: [key block][term][half][lane], a wave a key block.
-template <int TERMS>
-struct Keys {
-  Op op[4][TERMS][2][64];
+// A unit, and its first chunk row (negative for history).
+struct Unit64 {
+  UnitRows u;
+  int first;
 };
-
-template <int BITS, int PREC, int TERMS>
-__device__ __forceinline__ void stage_unit(const UnitRows& u, int wave, int lane, Keys<TERMS>& keys) {
-  KeyPiece<BITS> p;
-  load_key<BITS>(u, 16 * wave + (lane & 15), lane >> 4, p);
-  Op op[Terms<BITS, PREC>::K][2];
-  key_ops<BITS, PREC>(p, op);
-#pragma unroll
-  for (int t = 0; t < TERMS; ++t)
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      if (t < Terms<BITS, PREC>::K) keys.op[wave][t][i][lane] = op[t < Terms<BITS, PREC>::K ? t : 0][i];
-      else keys.op[wave][t][i][lane].v = bf16x8{};
-    }
+__device__ __forceinline__ Unit64 unit_of(const dkv_attn_args& a, const History& v, int unit, int h) {
+  if (unit < v.n_tiles) return Unit64{tile_rows(a, a.tiles[unit], v.past, h), -1};
+  return Unit64{chunk_rows(a, unit - v.n_tiles, h), (unit - v.n_tiles) * TILE};
 }
 
-template <int PREC, int TERMS>
-__device__ __forceinline__ UnitRows stage(const dkv_attn_args& a, const History& v, int unit, int h, int wave, int lane,
-                                          Keys<TERMS>& keys) {
-  const UnitRows u = unit < v.n_tiles ? tile_rows(a, a.tiles[unit], v.past, h) : chunk_rows(a, unit - v.n_tiles, h);
-  const int bits = __builtin_amdgcn_readfirstlane(u.bits);
-  if (bits == 4) stage_unit<4, PREC, TERMS>(u, wave, lane, keys);
-  else if (bits == 8) stage_unit<8, PREC, TERMS>(u, wave, lane, keys);
-  else stage_unit<16, PREC, TERMS>(u, wave, lane, keys);
-  return u;
-}
-
-// Scaled scores (base 2) of 16 rows against the unit's keys 16 b + 4 g + i, -inf where a key is not visible: row c is
-// chunk row m, whose segment starts at `start`; first is the unit's first chunk row, or negative for history.
-template <int TERMS>
-__device__ __forceinline__ void score(const Keys<TERMS>& keys, const Op (&q)[2], const UnitRows& u, int first, int m, int start,
-                                      float scale2, int lane, f32x4 (&s)[4]) {
-  const int g = lane >> 4;
-#pragma unroll
-  for (int b = 0; b < 4; ++b) {
-    s[b] = f32x4{0, 0, 0, 0};
-#pragma unroll
-    for (int t = TERMS - 1; t >= 0; --t) s[b] = mfma(keys.op[b][t][1][lane], q[1], mfma(keys.op[b][t][0][lane], q[0], s[b]));
-  }
-  const int low = first < 0 ? 0 : start - first, high = first < 0 ? u.high : min(u.high, m + 1 - first);
+// A row's scores are masked where the unit's key is not visible: keys [low, high) are. Row m's segment starts at `start`.
+__device__ __forceinline__ void mask_scores(const Unit64& x, int m, int start, int g, f32x4 (&s)[4]) {
+  const int low = x.first < 0 ? 0 : start - x.first, high = x.first < 0 ? x.u.high : min(x.u.high, m + 1 - x.first);
+  if (__all(low <= 0 && high >= TILE)) return;
 #pragma unroll
   for (int b = 0; b < 4; ++b)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int row = 16 * b + 4 * g + i;
-      s[b][i] = row >= low && row < high ? s[b][i] * scale2 : -INFINITY;
+      if (row < low || row >= high) s[b][i] = -INFINITY;
     }
+}
+
+// A row's maximum (raw) and sum with 16 scores more. The sum is of exp2(s * scale2 - reference), the reference being the
+// maximum times scale2 as stored, so that both launches round it alike.
+__device__ __forceinline__ void add_scores(const f32x4 (&s)[4], float scale2, float& top, float& sum) {
+  float m = top;
+#pragma unroll
+  for (int b = 0; b < 4; ++b) m = fmaxf(m, fmaxf(fmaxf(s[b][0], s[b][1]), fmaxf(s[b][2], s[b][3])));
+  const float ref = m == -INFINITY ? 0.f : m * scale2;
+  float l = sum * __builtin_amdgcn_exp2f(top * scale2 - ref);
+#pragma unroll
+  for (int b = 0; b < 4; ++b)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) l += __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], scale2, -ref));
+  top = m, sum = l;
+}
+
+// Adds 16 keys' weights of a row (norm: reference and 1 / sum). A masked key gets nothing, also of a row whose sum is not
+// a number.
+__device__ __forceinline__ void add_weights(const f32x4 (&s)[4], float scale2, float2 norm, bool chunk, float (&sum)[4][4]) {
+#pragma unroll
+  for (int b = 0; b < 4; ++b)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], scale2, -norm.x));
+      if (!chunk || s[b][i] != -INFINITY) sum[b][i] = __builtin_fmaf(p, norm.y, sum[b][i]);
+    }
+}
+
+// Maximum and sum of a row over the splits, as its reference and 1 / sum.
+constexpr int AHEAD = 16;  // loads in flight
+__device__ __forceinline__ void join(const float2* part, int from, int to, int64_t stride, float& m, float& l) {
+  for (int s0 = from; s0 < to; s0 += AHEAD) {
+    float2 x[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) x[i] = part[min(s0 + i, to - 1) * stride];
+    float top = m;
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) top = fmaxf(top, x[i].x);
+    const float ref = top == -INFINITY ? 0.f : top;
+    l *= __builtin_amdgcn_exp2f(m - ref);
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) l += s0 + i < to ? x[i].y * __builtin_amdgcn_exp2f(x[i].x - ref) : 0.f;
+    m = top;
+  }
 }
 
 // Query row `row` (query head by query head, q_heads / heads * nq of a KV head).
@@ -96,145 +119,375 @@ __device__ __forceinline__ void query_row(const dkv_attn_args& a, int h, int row
   query_ops(static_cast<const uint16_t*>(a.q) + (h * G + r / a.nq) * a.q_head_stride + r % a.nq * a.q_tok_stride, row < rows, g, q);
 }
 
+// 16 sums a lane, [b][i] of key 16 b + 4 g + i, over the 16 lanes of a group: each lane ends with one key's, which it
+// returns, and that key. Halves change places with the mirrored lane of 16, of 8, of 4 and of 2.
+template <int CONTROL, int HALF>
+__device__ __forceinline__ void fold(float (&x)[16], bool upper) {
+#pragma unroll
+  for (int i = 0; i < HALF; ++i) {
+    const float give = upper ? x[i] : x[i + HALF], keep = upper ? x[i + HALF] : x[i];
+    x[i] = keep + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(give), CONTROL, 0xf, 0xf, true));
+  }
+}
+__device__ __forceinline__ float column_sum(const float (&sum)[4][4], int c, int g, int& key) {
+  float x[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x[i] = sum[i / 4][i % 4];
+  fold<0x140, 8>(x, c & 8);  // row_mirror
+  fold<0x141, 4>(x, c & 4);  // row_half_mirror
+  fold<0x1b, 2>(x, c & 2);   // quad_perm 3 2 1 0
+  fold<0xb1, 1>(x, c & 1);   // quad_perm 1 0 3 2
+  key = 16 * (c >> 2) + 4 * g + (c & 3);
+  return x[0];
+}
+
+// ---- few rows: a wave a unit -----------------------------------------------------------------------------------
+struct RawKeys {
+  KeyPiece p[4];
+  f32x4 as[4][2];
+};
+
+template <int PREC>
+__device__ __forceinline__ void load_unit(const UnitRows& u, int c, int g, RawKeys& k) {
+#pragma unroll
+  for (int b = 0; b < 4; ++b) {
+    if (u.bits == 4) load_key<4>(u, 16 * b + c, g, k.p[b]);
+    else if (u.bits == 8) load_key<8>(u, 16 * b + c, g, k.p[b]);
+    else load_key<16>(u, 16 * b + c, g, k.p[b]);
+  }
+  if (PREC == 1 && u.bits == 4) load_scales<4>(u.k, u.rows, g, k.as);
+  if (PREC == 1 && u.bits == 8) load_scales<8>(u.k, u.rows, g, k.as);
+}
+
+template <int BITS, int PREC, int NB>
+__device__ __forceinline__ void unit_scores(const RawKeys& k, const Op (&q)[NB][2], const float (&q_sum)[NB], f32x4 (&s)[NB][4]) {
+#pragma unroll
+  for (int b = 0; b < 4; ++b) {
+    Op op[2];
+    key_ops<BITS, PREC>(k.p[b], op);
+#pragma unroll
+    for (int n = 0; n < NB; ++n) s[n][b] = mfma(op[1], q[n][1], mfma(op[0], q[n][0], f32x4{0, 0, 0, 0}));
+  }
+  if constexpr (AFFINE<BITS, PREC>)
+#pragma unroll
+    for (int n = 0; n < NB; ++n) affine_scores<BITS>(k.as, q_sum[n], s[n]);
+}
+
+template <int PREC, int NB>
+struct FewRows {
+  Op q[NB][2];
+  float q_sum[NB];
+  int at[NB], start[NB];
+  __device__ __forceinline__ void load(const dkv_attn_args& a, int h, int rows, int c, int g) {
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      query_row(a, h, 16 * n + c, rows, g, q[n]);
+      q_sum[n] = PREC == 1 ? query_sum(q[n]) : 0.f;
+      at[n] = (16 * n + c) % a.nq, start[n] = chunk_seg_start(a, at[n]);
+    }
+  }
+  // use(block, scores) of this wave's units unit, unit + step, ...: the next one's keys load meanwhile
+  template <class Use>
+  __device__ __forceinline__ void each(const dkv_attn_args& a, const History& v, int h, int unit, int step, int c, int g, Use use) {
+    if (unit >= v.units) return;
+    Unit64 x = unit_of(a, v, unit, h);
+    x.u.bits = __builtin_amdgcn_readfirstlane(x.u.bits);
+    RawKeys k;
+    load_unit<PREC>(x.u, c, g, k);
+    for (;;) {
+      const int next = unit + step;
+      Unit64 y = x;
+      RawKeys l;
+      if (next < v.units) {
+        y = unit_of(a, v, next, h);
+        y.u.bits = __builtin_amdgcn_readfirstlane(y.u.bits);
+        load_unit<PREC>(y.u, c, g, l);
+      }
+      f32x4 s[NB][4];
+      if (x.u.bits == 4) unit_scores<4, PREC, NB>(k, q, q_sum, s);
+      else if (x.u.bits == 8) unit_scores<8, PREC, NB>(k, q, q_sum, s);
+      else unit_scores<16, PREC, NB>(k, q, q_sum, s);
+#pragma unroll
+      for (int n = 0; n < NB; ++n) mask_scores(x, at[n], start[n], g, s[n]);
+      use(unit, x, s);
+      if (next >= v.units) return;
+      unit = next, x = y, k = l;
+    }
+  }
+};
+
+template <int PREC, int NB>
+__global__ __launch_bounds__(256) void few_stats_kernel(dkv_attn_args a, MassArgs p) {
+  __shared__ float2 ml[4][16 * NB];
+  const History v = history_of(a);
+  const int splits = split_count(p.splits, v.units, true);
+  if ((int)blockIdx.x >= splits) return;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, h = blockIdx.y;
+  const int rows = a.q_heads / a.heads * a.nq;
+  FewRows<PREC, NB> few;
+  few.load(a, h, rows, c, g);
+  float top[NB], sum[NB];
+#pragma unroll
+  for (int n = 0; n < NB; ++n) top[n] = -INFINITY, sum[n] = 0.f;
+  const float scale2 = a.scale * LOG2E;
+  few.each(a, v, h, 4 * blockIdx.x + wave, 4 * splits, c, g, [&](int, const Unit64&, const f32x4 (&s)[NB][4]) {
+#pragma unroll
+    for (int n = 0; n < NB; ++n) add_scores(s[n], scale2, top[n], sum[n]);
+  });
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {  // the four lanes of a row join theirs
+    const float m = row_max(top[n]), ref = m == -INFINITY ? 0.f : m * scale2;
+    const float l = row_sum(sum[n] * __builtin_amdgcn_exp2f(top[n] * scale2 - ref));
+    if (g == 0) ml[wave][16 * n + c] = make_float2(m * scale2, l);
+  }
+  __syncthreads();
+  if ((int)threadIdx.x < rows) {
+    float m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) m = fmaxf(m, ml[w][threadIdx.x].x);
+    const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) l += ml[w][threadIdx.x].y * __builtin_amdgcn_exp2f(ml[w][threadIdx.x].x - ref);
+    p.part[((int64_t)h * splits + blockIdx.x) * rows + threadIdx.x] = make_float2(m, l);
+  }
+}
+
+template <int PREC, int NB>
+__global__ __launch_bounds__(256) void few_columns_kernel(dkv_attn_args a, MassArgs p) {
+  constexpr int R = 16 * NB, SLICES = 256 / R;  // threads of a row in the join
+  __shared__ float2 ml[SLICES][R], norm[R];
+  const History v = history_of(a);
+  const int h = blockIdx.y, wave = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+  if (4 * (int)blockIdx.x >= v.units) return;
+  const int rows = a.q_heads / a.heads * a.nq, splits = split_count(p.splits, v.units, true);
+  {
+    const int row = threadIdx.x % R, slice = threadIdx.x / R, from = splits * slice / SLICES, to = splits * (slice + 1) / SLICES;
+    float m = -INFINITY, l = 0.f;
+    if (row < rows) join(p.part + (int64_t)h * splits * rows + row, from, to, rows, m, l);
+    ml[slice][row] = make_float2(m, l);
+  }
+  FewRows<PREC, NB> few;
+  few.load(a, h, rows, c, g);
+  __syncthreads();
+  if (threadIdx.x < R) {
+    float m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int i = 0; i < SLICES; ++i) m = fmaxf(m, ml[i][threadIdx.x].x);
+    const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int i = 0; i < SLICES; ++i) l += ml[i][threadIdx.x].y * __builtin_amdgcn_exp2f(ml[i][threadIdx.x].x - ref);
+    norm[threadIdx.x] = (int)threadIdx.x < rows ? make_float2(m, 1.f / l) : make_float2(0.f, 0.f);
+  }
+  __syncthreads();
+  float2 nm[NB];
+#pragma unroll
+  for (int n = 0; n < NB; ++n) nm[n] = norm[16 * n + c];
+  const float scale2 = a.scale * LOG2E;
+  few.each(a, v, h, 4 * blockIdx.x + wave, 4 * gridDim.x, c, g, [&](int unit, const Unit64& x, const f32x4 (&s)[NB][4]) {
+    float sum[4][4] = {};
+#pragma unroll
+    for (int n = 0; n < NB; ++n) add_weights(s[n], scale2, nm[n], x.first >= 0, sum);
+    int key;
+    const float w = column_sum(sum, c, g, key);
+    if (key >= x.u.high) return;
+    float* out = p.out + h * p.out_stride + (x.first < 0 ? a.tiles[unit].token_start : v.past + x.first) + key;
+    *out = p.accumulate ? *out + w : w;
+  });
+}
+
+// ---- many rows: a workgroup a unit -----------------------------------------------------------------------------
+// A unit's keys as MFMA operands, a wave a 16-key block, and their (offset, scale) where scores take them.
+struct Keys {
+  Op op[4][2][64];
+  f32x4 as[32];
+};
+
+template <int PREC>
+__device__ __forceinline__ void load_block(const UnitRows& u, int wave, int lane, KeyPiece& p) {
+  const int row = 16 * wave + (lane & 15), g = lane >> 4;
+  if (u.bits == 4) load_key<4>(u, row, g, p);
+  else if (u.bits == 8) load_key<8>(u, row, g, p);
+  else load_key<16>(u, row, g, p);
+}
+
+template <int PREC>
+__device__ __forceinline__ void stage_block(const UnitRows& u, const KeyPiece& p, int wave, int lane, Keys& keys) {
+  Op op[2];
+  if (u.bits == 4) key_ops<4, PREC>(p, op);
+  else if (u.bits == 8) key_ops<8, PREC>(p, op);
+  else key_ops<16, PREC>(p, op);
+  keys.op[wave][0][lane] = op[0], keys.op[wave][1][lane] = op[1];
+  if (PREC == 1 && lane < 16 && u.bits < 16) reinterpret_cast<float2*>(keys.as)[16 * wave + lane] = p.as;
+}
+
+template <int PREC>
+__device__ __forceinline__ void block_scores(const Keys& keys, int bits, const Op (&q)[2], float q_sum, int lane, f32x4 (&s)[4]) {
+  const int g = lane >> 4;
+#pragma unroll
+  for (int b = 0; b < 4; ++b)
+    s[b] = mfma(keys.op[b][1][lane], q[1], mfma(keys.op[b][0][lane], q[0], f32x4{0, 0, 0, 0}));
+  if (PREC == 1 && bits < 16) {
+    f32x4 as[4][2];
+#pragma unroll
+    for (int b = 0; b < 4; ++b) as[b][0] = keys.as[8 * b + 2 * g], as[b][1] = keys.as[8 * b + 2 * g + 1];
+    if (bits == 4) affine_scores<4>(as, q_sum, s);
+    else affine_scores<8>(as, q_sum, s);
+  }
+}
+
+// (A chunk piece that no row of a block sees has nothing for it.)
+__device__ __forceinline__ bool sees(const Unit64& x, int m, int start) {
+  return x.first < 0 || __any(m >= x.first && start < x.first + TILE);
+}
+
 template <int PREC>
 __global__ __launch_bounds__(256) void stats_kernel(dkv_attn_args a, MassArgs p) {
-  constexpr int TERMS = PREC == 0 ? 1 : 3;
-  __shared__ Keys<TERMS> keys;
+  __shared__ Keys keys;
   const History v = history_of(a);
-  const int splits = split_count(p.splits, v.units);
+  const int splits = split_count(p.splits, v.units, false);
   if ((int)blockIdx.x >= splits) return;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, h = blockIdx.y;
   const int rows = a.q_heads / a.heads * a.nq;
   Op q[BLOCKS][2];
-  float top[BLOCKS], sum[BLOCKS];
+  float top[BLOCKS], sum[BLOCKS], q_sum[BLOCKS];
   int at[BLOCKS], start[BLOCKS];
 #pragma unroll
   for (int k = 0; k < BLOCKS; ++k) {
     const int row = blockIdx.z * GROUP + (4 * k + wave) * 16 + c;
     query_row(a, h, row, rows, g, q[k]);
+    q_sum[k] = PREC == 1 ? query_sum(q[k]) : 0.f;
     at[k] = row % a.nq, start[k] = chunk_seg_start(a, row % a.nq);
     top[k] = -INFINITY, sum[k] = 0.f;
   }
   const float scale2 = a.scale * LOG2E;
   const int from = (int)((int64_t)v.units * blockIdx.x / splits), to = (int)((int64_t)v.units * (blockIdx.x + 1) / splits);
+  Unit64 x = unit_of(a, v, from, h);
+  x.u.bits = __builtin_amdgcn_readfirstlane(x.u.bits);
+  KeyPiece piece;
+  load_block<PREC>(x.u, wave, lane, piece);
   for (int unit = from; unit < to; ++unit) {
     __syncthreads();
-    const UnitRows u = stage<PREC, TERMS>(a, v, unit, h, wave, lane, keys);
+    stage_block<PREC>(x.u, piece, wave, lane, keys);
+    const Unit64 y = x;
+    if (unit + 1 < to) {  // the next unit's keys load while this one's scores are computed
+      x = unit_of(a, v, unit + 1, h);
+      x.u.bits = __builtin_amdgcn_readfirstlane(x.u.bits);
+      load_block<PREC>(x.u, wave, lane, piece);
+    }
     __syncthreads();
-    const int first = unit < v.n_tiles ? -1 : (unit - v.n_tiles) * TILE;
 #pragma unroll
     for (int k = 0; k < BLOCKS; ++k) {
-      // (a block none of whose rows sees a key of this chunk piece has nothing to add)
-      if (first >= 0 && !__any(at[k] >= first && start[k] < first + TILE)) continue;
+      if ((int)blockIdx.z * GROUP + (4 * k + wave) * 16 >= rows || !sees(y, at[k], start[k])) continue;
       f32x4 s[4];
-      score<TERMS>(keys, q[k], u, first, at[k], start[k], scale2, lane, s);
-      float m = top[k];
-#pragma unroll
-      for (int b = 0; b < 4; ++b) m = fmaxf(m, fmaxf(fmaxf(s[b][0], s[b][1]), fmaxf(s[b][2], s[b][3])));
-      const float ref = m == -INFINITY ? 0.f : m;
-      float l = sum[k] * __builtin_amdgcn_exp2f(top[k] - ref);
-#pragma unroll
-      for (int b = 0; b < 4; ++b)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) l += __builtin_amdgcn_exp2f(s[b][i] - ref);
-      top[k] = m, sum[k] = l;
+      block_scores<PREC>(keys, y.u.bits, q[k], q_sum[k], lane, s);
+      mask_scores(y, at[k], start[k], g, s);
+      add_scores(s, scale2, top[k], sum[k]);
     }
   }
 #pragma unroll
   for (int k = 0; k < BLOCKS; ++k) {  // the four lanes of a row join theirs
-    const float m = row_max(top[k]);
-    const float l = row_sum(sum[k] * __builtin_amdgcn_exp2f(top[k] - (m == -INFINITY ? 0.f : m)));
+    const float m = row_max(top[k]), ref = m == -INFINITY ? 0.f : m * scale2;
+    const float l = row_sum(sum[k] * __builtin_amdgcn_exp2f(top[k] * scale2 - ref));
     const int row = blockIdx.z * GROUP + (4 * k + wave) * 16 + c;
-    if (g == 0 && row < rows) p.part[((int64_t)h * splits + blockIdx.x) * rows + row] = make_float2(m, l);
+    if (g == 0 && row < rows) p.part[((int64_t)h * splits + blockIdx.x) * rows + row] = make_float2(m * scale2, l);
   }
 }
 
 template <int PREC>
 __global__ __launch_bounds__(256) void columns_kernel(dkv_attn_args a, MassArgs p) {
-  constexpr int TERMS = PREC == 0 ? 1 : 3;
-  __shared__ Keys<TERMS> keys;
-  __shared__ float2 norm[GROUP];  // maximum and 1 / sum of the row group's rows
+  __shared__ Keys keys;
+  __shared__ float2 norm[GROUP];  // reference and 1 / sum of the row group's rows
   __shared__ float column[4][TILE];
   const History v = history_of(a);
   const int unit = blockIdx.x, h = blockIdx.y;
   if (unit >= v.units) return;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
-  const int rows = a.q_heads / a.heads * a.nq, splits = split_count(p.splits, v.units);
+  const int rows = a.q_heads / a.heads * a.nq, splits = split_count(p.splits, v.units, false);
   const float scale2 = a.scale * LOG2E;
-  const UnitRows u = stage<PREC, TERMS>(a, v, unit, h, wave, lane, keys);
-  const int first = unit < v.n_tiles ? -1 : (unit - v.n_tiles) * TILE;
+  Unit64 x = unit_of(a, v, unit, h);
+  x.u.bits = __builtin_amdgcn_readfirstlane(x.u.bits);
+  KeyPiece piece;
+  load_block<PREC>(x.u, wave, lane, piece);
+  stage_block<PREC>(x.u, piece, wave, lane, keys);
   float total[4][4] = {};
-  for (int group = 0; group < p.row_groups; ++group) {
+  for (int group = blockIdx.z; group < p.row_groups; group += p.row_parts) {
     __syncthreads();
-    for (int i = threadIdx.x; i < GROUP; i += 256) {
-      const int row = group * GROUP + i;
+    if (const int row = group * GROUP + (int)threadIdx.x; threadIdx.x < GROUP) {
       float m = -INFINITY, l = 0.f;
-      if (row < rows) {
-        const float2* part = p.part + (int64_t)h * splits * rows + row;
-        for (int s = 0; s < splits; ++s) m = fmaxf(m, part[(int64_t)s * rows].x);
-        const float ref = m == -INFINITY ? 0.f : m;
-        for (int s = 0; s < splits; ++s) l += part[(int64_t)s * rows].y * __builtin_amdgcn_exp2f(part[(int64_t)s * rows].x - ref);
-      }
-      norm[i] = row < rows ? make_float2(m, 1.f / l) : make_float2(0.f, 0.f);
+      if (row < rows) join(p.part + (int64_t)h * splits * rows + row, 0, splits, rows, m, l);
+      norm[threadIdx.x] = row < rows ? make_float2(m, 1.f / l) : make_float2(0.f, 0.f);
     }
+    Op q[BLOCKS][2];
+#pragma unroll
+    for (int k = 0; k < BLOCKS; ++k) query_row(a, h, group * GROUP + (4 * k + wave) * 16 + c, rows, g, q[k]);
     __syncthreads();
     float sum[4][4] = {};  // this group's share, so that long sums are sums of short ones
 #pragma unroll
     for (int k = 0; k < BLOCKS; ++k) {
-      const int i = (4 * k + wave) * 16 + c, row = group * GROUP + i;
-      if (group * GROUP + (4 * k + wave) * 16 >= rows) break;
-      const int m = row % a.nq, start = chunk_seg_start(a, m);
-      if (first >= 0 && !__any(m >= first && start < first + TILE)) continue;
-      Op q[2];
-      query_row(a, h, row, rows, g, q);
+      const int i = (4 * k + wave) * 16 + c, m = (group * GROUP + i) % a.nq, start = chunk_seg_start(a, m);
+      if (group * GROUP + (4 * k + wave) * 16 >= rows || !sees(x, m, start)) continue;
       f32x4 s[4];
-      score<TERMS>(keys, q, u, first, m, start, scale2, lane, s);
-      const float2 n = norm[i];
-#pragma unroll
-      for (int b = 0; b < 4; ++b)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          // (a masked key gets nothing, also of a row whose sum is not a number)
-          if (first < 0 || s[b][j] != -INFINITY) sum[b][j] += __builtin_amdgcn_exp2f(s[b][j] - n.x) * n.y;
+      block_scores<PREC>(keys, x.u.bits, q[k], PREC == 1 ? query_sum(q[k]) : 0.f, lane, s);
+      mask_scores(x, m, start, g, s);
+      add_weights(s, scale2, norm[i], x.first >= 0, sum);
     }
 #pragma unroll
     for (int b = 0; b < 4; ++b)
 #pragma unroll
       for (int j = 0; j < 4; ++j) total[b][j] += sum[b][j];
   }
-#pragma unroll
-  for (int b = 0; b < 4; ++b)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {  // over the 16 rows of a block
-      float x = total[b][j];
-#pragma unroll
-      for (int d = 8; d; d >>= 1) x += __shfl_xor(x, d, 16);
-      if (c == 0) column[wave][16 * b + 4 * g + j] = x;
-    }
+  int key;
+  const float w = column_sum(total, c, g, key);
+  column[wave][key] = w;
   __syncthreads();
-  const int key = threadIdx.x;
-  if (key >= TILE || key >= u.high) return;
-  const int token = unit < v.n_tiles ? a.tiles[unit].token_start + key : v.past + first + key;
-  const float x = column[0][key] + column[1][key] + (column[2][key] + column[3][key]);
+  key = threadIdx.x;
+  if (key >= TILE || key >= x.u.high) return;
+  const int token = (x.first < 0 ? a.tiles[unit].token_start : v.past + x.first) + key;
+  const float all = column[0][key] + column[1][key] + (column[2][key] + column[3][key]);
+  if (p.row_parts > 1) {
+    p.columns[((int64_t)blockIdx.z * a.heads + h) * p.columns_stride + token] = all;
+  } else {
+    float* out = p.out + h * p.out_stride + token;
+    *out = p.accumulate ? *out + all : all;
+  }
+}
+
+__global__ __launch_bounds__(256) void add_parts_kernel(dkv_attn_args a, MassArgs p) {
+  const int token = blockIdx.x * 256 + threadIdx.x, h = blockIdx.y;
+  if (token >= history_of(a).past + a.nq) return;
+  float x = 0.f;
+  for (int i = 0; i < p.row_parts; ++i) x += p.columns[((int64_t)i * a.heads + h) * p.columns_stride + token];
   float* out = p.out + h * p.out_stride + token;
   *out = p.accumulate ? *out + x : x;
 }
 
-constexpr int WORKGROUPS = 512;  // workgroups of the first launch
-constexpr int MAX_SPLITS = 64;   // and the ranges of units that the second one joins, at most
+constexpr int WORKGROUPS = 1024;  // workgroups of a launch, where there is work for as many
+constexpr int MAX_SPLITS = 32;    // ranges of units that the second launch joins for many rows, at most
+constexpr int MAX_SPLITS_FEW = 128;
+constexpr int MAX_ROW_PARTS = 8;
 
-static MassArgs plan_of(const dkv_attn_args& a) {
-  MassArgs p{};
-  const int64_t rows = (int64_t)(a.q_heads / a.heads) * a.nq;
-  p.row_groups = (int)((rows + GROUP - 1) / GROUP);
-  int64_t most = WORKGROUPS / ((int64_t)a.heads * p.row_groups);
-  most = most < 1 ? 1 : most > MAX_SPLITS ? MAX_SPLITS : most;
-  p.splits = split_count((int)most, a.n_tiles + (a.nq + TILE - 1) / TILE);
-  return p;
-}
+struct MassPlan {
+  MassArgs p;
+  int64_t part_bytes, bytes;
+};
 
-static int64_t bytes_of(const dkv_attn_args& a, const MassArgs& p) {
-  return (int64_t)a.heads * p.splits * (a.q_heads / a.heads) * a.nq * sizeof(float2);
+static MassPlan plan_of(const dkv_attn_args& a) {
+  MassPlan m{};
+  const int64_t rows = (int64_t)(a.q_heads / a.heads) * a.nq, units = (int64_t)a.n_tiles + (a.nq + TILE - 1) / TILE;
+  m.p.row_groups = (int)((rows + GROUP - 1) / GROUP);
+  const bool few = rows <= FEW;
+  int64_t most = WORKGROUPS / ((int64_t)a.heads * m.p.row_groups);
+  const int64_t cap = few ? MAX_SPLITS_FEW : MAX_SPLITS;
+  most = most < 1 ? 1 : most > cap ? cap : most;
+  m.p.splits = split_count((int)most, (int)units, few);
+  // four row groups and more a part: by the chunk alone, so that replays add up what a call does
+  m.p.row_parts = m.p.row_groups / 4;
+  if (m.p.row_parts > MAX_ROW_PARTS) m.p.row_parts = MAX_ROW_PARTS;
+  if (m.p.row_parts < 1) m.p.row_parts = 1;
+  m.p.columns_stride = ((int64_t)a.past + a.nq + 63) & ~63;
+  m.part_bytes = ((int64_t)a.heads * m.p.splits * rows * sizeof(float2) + 255) & ~(int64_t)255;
+  m.bytes = m.part_bytes + (m.p.row_parts > 1 ? m.p.row_parts * a.heads * m.p.columns_stride * 4 : 0);
+  return m;
 }
 
 }  // namespace mass
@@ -250,7 +503,7 @@ extern "C" {
 
 int64_t dkv_attention_mass_workspace_bytes(const dkv_attn_args* args) {
   if (!args || args->heads <= 0 || args->q_heads <= 0 || args->q_heads % args->heads || args->nq <= 0 || args->n_tiles < 0) return 0;
-  return bytes_of(*args, mass::plan_of(*args));
+  return mass::plan_of(*args).bytes;
 }
 
 int dkv_attention_mass(const dkv_attn_args* args, float* mass, int64_t mass_head_stride, int32_t accumulate, void* stream) {
@@ -261,8 +514,10 @@ int dkv_attention_mass(const dkv_attn_args* args, float* mass, int64_t mass_head
   }
   const dkv_attn_args& a = *args;
   if (int rc = check_history_args(a, "dkv_attention_mass")) return rc;
-  MassArgs p = mass::plan_of(a);
-  if (p.row_groups > 65535 || (int64_t)(a.q_heads / a.heads) * a.nq > INT32_MAX - GROUP) {
+  const MassPlan plan = mass::plan_of(a);
+  MassArgs p = plan.p;
+  const int64_t rows = (int64_t)(a.q_heads / a.heads) * a.nq;
+  if (p.row_groups > 65535 || rows > INT32_MAX - GROUP) {
     set_error("dkv_attention_mass: at most %d query rows a KV head", 65535 * GROUP);
     return DKV_EINVAL;
   }
@@ -270,22 +525,31 @@ int dkv_attention_mass(const dkv_attn_args* args, float* mass, int64_t mass_head
     set_error("dkv_attention_mass: rows of %lld masses cannot hold %d tokens", (long long)mass_head_stride, a.past + a.nq);
     return DKV_EINVAL;
   }
-  const int64_t need = bytes_of(a, p);
-  if (!a.workspace || a.workspace_bytes < need) {
-    set_error("dkv_attention_mass: workspace of %lld bytes needed, %lld given", (long long)need, (long long)a.workspace_bytes);
+  if (!a.workspace || a.workspace_bytes < plan.bytes) {
+    set_error("dkv_attention_mass: workspace of %lld bytes needed, %lld given", (long long)plan.bytes, (long long)a.workspace_bytes);
     return DKV_EINVAL;
   }
   p.part = static_cast<float2*>(a.workspace);
+  p.columns = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + plan.part_bytes);
   p.out = mass, p.out_stride = mass_head_stride, p.accumulate = accumulate;
-  const dim3 first(p.splits, a.heads, p.row_groups), second(a.n_tiles + (a.nq + TILE - 1) / TILE, a.heads);
   const hipStream_t st = (hipStream_t)stream;
-  if (a.precision == 1) {
-    hipLaunchKernelGGL(stats_kernel<1>, first, dim3(256), 0, st, a, p);
-    hipLaunchKernelGGL(columns_kernel<1>, second, dim3(256), 0, st, a, p);
-  } else {
-    hipLaunchKernelGGL(stats_kernel<0>, first, dim3(256), 0, st, a, p);
-    hipLaunchKernelGGL(columns_kernel<0>, second, dim3(256), 0, st, a, p);
+  const int units = a.n_tiles + (a.nq + TILE - 1) / TILE;
+  if (rows <= FEW) {
+    const auto stats = a.precision == 1 ? (rows <= 16 ? few_stats_kernel<1, 1> : few_stats_kernel<1, 4>)
+                                        : (rows <= 16 ? few_stats_kernel<0, 1> : few_stats_kernel<0, 4>);
+    const auto columns = a.precision == 1 ? (rows <= 16 ? few_columns_kernel<1, 1> : few_columns_kernel<1, 4>)
+                                          : (rows <= 16 ? few_columns_kernel<0, 1> : few_columns_kernel<0, 4>);
+    const int by_unit = (units + 3) / 4, most = 2 * WORKGROUPS / a.heads;
+    hipLaunchKernelGGL(stats, dim3(p.splits, a.heads), dim3(256), 0, st, a, p);
+    hipLaunchKernelGGL(columns, dim3(by_unit < most ? by_unit : most < 1 ? 1 : most, a.heads), dim3(256), 0, st, a, p);
+    return (int)hipGetLastError();
   }
+  const auto stats = a.precision == 1 ? stats_kernel<1> : stats_kernel<0>;
+  const auto columns = a.precision == 1 ? columns_kernel<1> : columns_kernel<0>;
+  hipLaunchKernelGGL(stats, dim3(p.splits, a.heads, p.row_groups), dim3(256), 0, st, a, p);
+  hipLaunchKernelGGL(columns, dim3(units, a.heads, p.row_parts), dim3(256), 0, st, a, p);
+  if (p.row_parts > 1)
+    hipLaunchKernelGGL(add_parts_kernel, dim3((a.past + a.nq + 255) / 256, a.heads), dim3(256), 0, st, a, p);
   return (int)hipGetLastError();
 }
 

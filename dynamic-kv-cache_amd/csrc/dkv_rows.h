@@ -75,7 +75,7 @@ __device__ __forceinline__ float code_at(const uint32_t* w, int e) {
   return (float)((w[e >> 3] >> (4 * (e & 7))) & 0xfu);
 }
 
-// x as the sum of TERMS bf16 values: two keep 2^-17 of a value, three all 24 bits of it.
+// x as the sum of TERMS bf16 values: two keep all but 2^-17 of a value, three all but 2^-25.
 template <int TERMS>
 __device__ __forceinline__ void split_pair(float x0, float x1, uint32_t (&out)[TERMS]) {
 #pragma unroll
@@ -88,22 +88,30 @@ __device__ __forceinline__ void split_pair(float x0, float x1, uint32_t (&out)[T
   }
 }
 
-// bf16 terms of a key: codes at precision 1 need three (their scores are sums of products with the whole
-// fp32 value), at precision 0 the rounded value is what attention multiplies, and 16-bit rows are bf16.
+// At precision 0 a key or value is its fp32 value rounded to bf16, which is what attention multiplies. At precision 1 a
+// packed row is taken as it is stored, scale * (code - centre) + (offset + scale * centre): the centred codes are exact
+// in bf16, so one MFMA gives their products without a value being unpacked, and scale and offset come after (keys) or go
+// into the weights (values). 16-bit rows are bf16 at both.
 template <int BITS, int PREC>
-struct Terms {
-  static constexpr int K = BITS == 16 || PREC == 0 ? 1 : 3;
-  static constexpr int V = BITS == 16 || PREC == 0 ? 1 : 2;
-};
-
+constexpr bool AFFINE = PREC == 1 && BITS < 16;
 template <int BITS>
-struct KeyPiece {  // 16 elements of a key and its (offset, scale)
-  uint32_t w[BITS / 2];
+constexpr float CENTRE = BITS == 4 ? 8.f : 128.f;
+
+// Codes e and e + 1 (or the elements of a 16-bit row) as a bf16 pair, unpacked as PREC asks.
+template <int BITS, int PREC>
+__device__ __forceinline__ uint32_t unpack_pair(float c0, float c1, float scale0, float offset0, float scale1, float offset1) {
+  if (AFFINE<BITS, PREC>) return pack_bf16(c0 - CENTRE<BITS>, c1 - CENTRE<BITS>);
+  return pack_bf16(c0 * scale0 + offset0, c1 * scale1 + offset1);
+}
+
+// 16 elements of a key and its (offset, scale), as loaded.
+struct KeyPiece {
+  uint32_t w[8];
   float2 as;
 };
 
 template <int BITS>
-__device__ __forceinline__ void load_key(const UnitRows& u, int row, int g, KeyPiece<BITS>& p) {
+__device__ __forceinline__ void load_key(const UnitRows& u, int row, int g, KeyPiece& p) {
   const int r = row < u.rows ? row : 0;
   const uint8_t* at = u.k + r * u.k_stride + g * 2 * BITS;
   if (BITS == 4) {
@@ -120,22 +128,40 @@ __device__ __forceinline__ void load_key(const UnitRows& u, int row, int g, KeyP
   if (BITS < 16) p.as = *reinterpret_cast<const float2*>(u.k + (int64_t)u.rows * (8 * BITS) + 8 * r);
 }
 
-// The operands of a key: op[term][half], elements 16 g + 8 half + [0, 8). Each value is code * scale + offset
-// with the product and the sum rounded, as every kernel here unpacks it.
+// The operands of a key: elements 16 g + 8 half + [0, 8).
 template <int BITS, int PREC>
-__device__ __forceinline__ void key_ops(const KeyPiece<BITS>& p, Op (&op)[Terms<BITS, PREC>::K][2]) {
-  constexpr int T = Terms<BITS, PREC>::K;
+__device__ __forceinline__ void key_ops(const KeyPiece& p, Op (&op)[2]) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    if (BITS == 16) {
-      op[0][j / 4].u[j % 4] = p.w[j];
-    } else {
-      uint32_t t[T];
-      split_pair<T>(code_at<BITS>(p.w, 2 * j) * p.as.y + p.as.x, code_at<BITS>(p.w, 2 * j + 1) * p.as.y + p.as.x, t);
+  for (int j = 0; j < 8; ++j)
+    op[j / 4].u[j % 4] = BITS == 16 ? p.w[j]
+                                    : unpack_pair<BITS, PREC>(code_at<BITS>(p.w, 2 * j), code_at<BITS>(p.w, 2 * j + 1), p.as.y,
+                                                              p.as.x, p.as.y, p.as.x);
+}
+
+// (offset + scale * centre, scale) of the lane's rows 16 b + 4 g + i of a packed tile: as[b][i / 2][2 (i % 2) + ...].
+// Two rows' pairs in one load: a pair whose first row the tile has lies within the sub-block, whose size is rounded up
+// to 16 bytes.
+template <int BITS>
+__device__ __forceinline__ void load_scales(const uint8_t* base, int rows, int g, f32x4 (&as)[4][2]) {
 #pragma unroll
-      for (int k = 0; k < T; ++k) op[k][j / 4].u[j % 4] = t[k];
+  for (int b = 0; b < 4; ++b)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int row = 16 * b + 4 * g + 2 * i;
+      as[b][i] = *reinterpret_cast<const f32x4*>(base + (int64_t)rows * (8 * BITS) + 8 * (row < rows ? row : 0));
     }
-  }
+}
+
+// Products of a query row with a unit's centred codes as scores: scale * product + offset' * (sum of the query).
+template <int BITS>
+__device__ __forceinline__ void affine_scores(const f32x4 (&as)[4][2], float query_sum, f32x4 (&s)[4]) {
+#pragma unroll
+  for (int b = 0; b < 4; ++b)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float offset = as[b][i / 2][2 * (i % 2)], scale = as[b][i / 2][2 * (i % 2) + 1];
+      s[b][i] = __builtin_fmaf(scale, s[b][i], __builtin_fmaf(scale, CENTRE<BITS>, offset) * query_sum);
+    }
 }
 
 // A query row's operands (elements 16 g + [0, 8) and [8, 16)); zeros where there is no row.
@@ -148,10 +174,21 @@ __device__ __forceinline__ void query_ops(const uint16_t* row, bool there, int g
   }
 }
 
+// The sum of a query row's elements, in the four lanes that hold it.
+__device__ __forceinline__ float row_sum(float x);
+__device__ __forceinline__ float query_sum(const Op (&q)[2]) {
+  float x = 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x += bf16_lo(q[i].u[j]) + bf16_hi(q[i].u[j]);
+  return row_sum(x);
+}
+
+// Elements [4 c, 4 c + 4) of the lane's 16 keys 16 b + 4 g + i of V, as loaded.
 template <int BITS>
-struct ValuePiece {  // elements [4 c, 4 c + 4) of the lane's 16 keys 16 b + 4 g + i, and their (offset, scale)
+struct ValuePiece {
   uint32_t w[4][4][BITS == 16 ? 2 : 1];
-  f32x4 as[4][2];
 };
 
 template <int BITS>
@@ -171,40 +208,31 @@ __device__ __forceinline__ void load_values(const UnitRows& u, int c, int g, Val
         p.w[b][i][0] = x[0];
         p.w[b][i][1 % (BITS == 16 ? 2 : 1)] = x[1];
       }
-      // two rows' pairs in one load: a pair whose first row the tile has lies within the sub-block, whose
-      // size is rounded up to 16 bytes
-      if (BITS < 16 && i % 2 == 0)
-        p.as[b][i / 2] = *reinterpret_cast<const f32x4*>(u.v + (int64_t)u.rows * (8 * BITS) + 8 * r);
     }
 }
 
-// The operands of output block db: op[term][step], keys 16 (2 step + j / 4) + 4 g + j % 4. Rows that are
-// not visible give zeros, so that what they hold (NaN or infinity in a masked row) meets no p of zero.
+// The operands of output block db: keys 16 (2 step + j / 4) + 4 g + j % 4. Rows that are not visible give zeros, so that
+// what they hold (NaN or infinity in a masked row) meets no p of zero.
 template <int BITS, int PREC>
-__device__ __forceinline__ void value_ops(const UnitRows& u, const ValuePiece<BITS>& p, int g, int db, bool whole,
-                                          Op (&op)[Terms<BITS, PREC>::V][2]) {
-  constexpr int T = Terms<BITS, PREC>::V;
+__device__ __forceinline__ void value_ops(const UnitRows& u, const ValuePiece<BITS>& p, const f32x4 (&as)[4][2], int g, int db,
+                                          bool whole, Op (&op)[2]) {
 #pragma unroll
   for (int b = 0; b < 4; ++b)
 #pragma unroll
     for (int i = 0; i < 4; i += 2) {
-      uint32_t t[T];
+      uint32_t t;
       if (BITS == 16) {
         const uint32_t x0 = p.w[b][i][(db >> 1) % (BITS == 16 ? 2 : 1)], x1 = p.w[b][i + 1][(db >> 1) % (BITS == 16 ? 2 : 1)];
-        t[0] = db & 1 ? (x0 >> 16) | (x1 & 0xffff0000u) : (x0 & 0xffffu) | (x1 << 16);
+        t = db & 1 ? (x0 >> 16) | (x1 & 0xffff0000u) : (x0 & 0xffffu) | (x1 << 16);
       } else {
-        const f32x4 as = p.as[b][i / 2];
-        split_pair<T>(code_at<BITS>(p.w[b][i], db) * as[1] + as[0], code_at<BITS>(p.w[b][i + 1], db) * as[3] + as[2], t);
+        const f32x4 m = as[b][i / 2];
+        t = unpack_pair<BITS, PREC>(code_at<BITS>(p.w[b][i], db), code_at<BITS>(p.w[b][i + 1], db), m[1], m[0], m[3], m[2]);
       }
       if (!whole) {
         const int row = 16 * b + 4 * g + i;
-        const uint32_t keep = (row >= u.low && row < u.high ? 0xffffu : 0u) |
-                              (row + 1 >= u.low && row + 1 < u.high ? 0xffff0000u : 0u);
-#pragma unroll
-        for (int k = 0; k < T; ++k) t[k] &= keep;
+        t &= (row >= u.low && row < u.high ? 0xffffu : 0u) | (row + 1 >= u.low && row + 1 < u.high ? 0xffff0000u : 0u);
       }
-#pragma unroll
-      for (int k = 0; k < T; ++k) op[k][b / 2].u[2 * (b % 2) + i / 2] = t[k];
+      op[b / 2].u[2 * (b % 2) + i / 2] = t;
     }
 }
 

@@ -31,7 +31,7 @@ constexpr int INDEX_TILES = 16;  // tiles of an index workgroup, four a wave
 template <int BITS>
 __device__ __forceinline__ void tile_bounds(const UnitRows& u, int lane, float& low, float& high) {
   float lo[16], hi[16];
-  KeyPiece<BITS> p[4];
+  KeyPiece p[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) load_key<BITS>(u, 16 * j + (lane >> 2), lane & 3, p[j]);
 #pragma unroll
@@ -194,29 +194,33 @@ __global__ __launch_bounds__(256) void choose_kernel(dkv_attn_args a, dkv_sparse
   }
 }
 
-// A wave's running softmax over its units for 16 query rows: row c's maximum (base 2), this lane's share of its sum
-// and the lane's 16 output elements.
+// A wave's running softmax over its units for 16 query rows: row c's maximum (base 2), this lane's share of its sum, of
+// the packed rows' offsets in the output (precision 1), and the lane's 16 output elements.
 struct Running {
-  float m, l;
+  float m, l, offset;
   f32x4 o[4];
 };
 
-template <int BITS, int PREC>
-__device__ __forceinline__ void attend_unit(const UnitRows& u, const Op (&q)[2], float scale2, int c, int g, Running& r) {
-  KeyPiece<BITS> kp[4];
+// p enters its product as the sum of TERMS bf16 values, so that only the values' own rounding limits a bf16 (two) or fp32
+// (three) output. At precision 1 a packed row's scale goes into p, and its offset is summed beside.
+template <int BITS, int PREC, int TERMS>
+__device__ __forceinline__ void attend_unit(const UnitRows& u, const Op (&q)[2], float q_sum, float scale2, int c, int g, Running& r) {
+  KeyPiece kp[4];
   ValuePiece<BITS> vp;
+  f32x4 k_as[4][2], v_as[4][2];
 #pragma unroll
   for (int b = 0; b < 4; ++b) load_key<BITS>(u, 16 * b + c, g, kp[b]);
+  if (AFFINE<BITS, PREC>) load_scales<BITS>(u.k, u.rows, g, k_as);
   load_values<BITS>(u, c, g, vp);
+  if (BITS < 16) load_scales<BITS>(u.v, u.rows, g, v_as);
   f32x4 s[4];
 #pragma unroll
   for (int b = 0; b < 4; ++b) {
-    Op k[Terms<BITS, PREC>::K][2];
+    Op k[2];
     key_ops<BITS, PREC>(kp[b], k);
-    s[b] = f32x4{0, 0, 0, 0};
-#pragma unroll
-    for (int t = Terms<BITS, PREC>::K - 1; t >= 0; --t) s[b] = mfma(k[t][1], q[1], mfma(k[t][0], q[0], s[b]));
+    s[b] = mfma(k[1], q[1], mfma(k[0], q[0], f32x4{0, 0, 0, 0}));
   }
+  if constexpr (AFFINE<BITS, PREC>) affine_scores<BITS>(k_as, q_sum, s);
   const bool whole = u.low == 0 && u.high == TILE;
   float top = -INFINITY;
 #pragma unroll
@@ -224,37 +228,45 @@ __device__ __forceinline__ void attend_unit(const UnitRows& u, const Op (&q)[2],
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int row = 16 * b + 4 * g + i;
-      s[b][i] = whole || (row >= u.low && row < u.high) ? s[b][i] * scale2 : -INFINITY;
+      if (!whole && !(row >= u.low && row < u.high)) {
+        s[b][i] = -INFINITY;
+        if (AFFINE<BITS, PREC>) v_as[b][i / 2][2 * (i % 2)] = v_as[b][i / 2][2 * (i % 2) + 1] = 0.f;
+      }
+      s[b][i] *= scale2;
       top = fmaxf(top, s[b][i]);
     }
   top = fmaxf(row_max(top), r.m);
   const float ref = top == -INFINITY ? 0.f : top;  // nothing visible yet: keep the empty state
   const float alpha = __builtin_amdgcn_exp2f(r.m - ref);
   r.m = top;
-  float sum = 0;
-  Op p[2][2];  // [term][step]: p as the sum of two bf16 values, so that only V's own terms limit the product
+  float sum = 0, offset = 0;
+  Op p[TERMS][2];
 #pragma unroll
   for (int b = 0; b < 4; ++b)
 #pragma unroll
     for (int i = 0; i < 4; i += 2) {
-      const float p0 = __builtin_amdgcn_exp2f(s[b][i] - ref), p1 = __builtin_amdgcn_exp2f(s[b][i + 1] - ref);
+      float p0 = __builtin_amdgcn_exp2f(s[b][i] - ref), p1 = __builtin_amdgcn_exp2f(s[b][i + 1] - ref);
       sum += p0 + p1;
-      uint32_t t[2];
-      split_pair<2>(p0, p1, t);
-      p[0][b / 2].u[2 * (b % 2) + i / 2] = t[0];
-      p[1][b / 2].u[2 * (b % 2) + i / 2] = t[1];
+      if constexpr (AFFINE<BITS, PREC>) {
+        const f32x4 m = v_as[b][i / 2];
+        offset = __builtin_fmaf(p0, __builtin_fmaf(m[1], CENTRE<BITS>, m[0]), offset);
+        offset = __builtin_fmaf(p1, __builtin_fmaf(m[3], CENTRE<BITS>, m[2]), offset);
+        p0 *= m[1], p1 *= m[3];
+      }
+      uint32_t t[TERMS];
+      split_pair<TERMS>(p0, p1, t);
+#pragma unroll
+      for (int k = 0; k < TERMS; ++k) p[k][b / 2].u[2 * (b % 2) + i / 2] = t[k];
     }
   r.l = r.l * alpha + sum;
+  if (PREC == 1) r.offset = r.offset * alpha + offset;
 #pragma unroll
   for (int db = 0; db < 4; ++db) {
-    Op v[Terms<BITS, PREC>::V][2];
-    value_ops<BITS, PREC>(u, vp, g, db, whole, v);
+    Op v[2];
+    value_ops<BITS, PREC>(u, vp, v_as, g, db, whole, v);
     f32x4 o = r.o[db] * alpha;
 #pragma unroll
-    for (int t = Terms<BITS, PREC>::V - 1; t >= 0; --t)
-#pragma unroll
-      for (int pt = t ? 0 : 1; pt >= 0; --pt)  // the product of both low terms is below the sums' rounding
-        o = mfma(v[t][1], p[pt][1], mfma(v[t][0], p[pt][0], o));
+    for (int t = TERMS - 1; t >= 0; --t) o = mfma(v[1], p[t][1], mfma(v[0], p[t][0], o));
     r.o[db] = o;
   }
 }
@@ -266,7 +278,7 @@ __device__ __forceinline__ void store4(void* out, int out_dtype, int64_t at, f32
     *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(out) + at) = u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
 }
 
-template <int PREC>
+template <int PREC, int TERMS>
 __global__ __launch_bounds__(256) void attend_kernel(dkv_attn_args a, dkv_sparse s, int row_blocks, int most, int max_chosen,
                                                      const int32_t* lists, float* part_o, float2* part_ml) {
   __shared__ float ml[4][16][2];
@@ -282,7 +294,8 @@ __global__ __launch_bounds__(256) void attend_kernel(dkv_attn_args a, dkv_sparse
   query_ops(static_cast<const uint16_t*>(a.q) + (h * G + 16 * rb + min(c, heads_here - 1)) * a.q_head_stride + m * a.q_tok_stride,
             c < heads_here, g, q);
   Running r;
-  r.m = -INFINITY, r.l = 0.f;
+  r.m = -INFINITY, r.l = r.offset = 0.f;
+  const float q_sum = query_sum(q);
   for (int db = 0; db < 4; ++db) r.o[db] = f32x4{0, 0, 0, 0};
   const int start = chunk_seg_start(a, m), tail = v.n_tiles - v.n_indexed;
   const int piece0 = start / TILE, units = v.chosen + tail + m / TILE - piece0 + 1;
@@ -300,14 +313,15 @@ __global__ __launch_bounds__(256) void attend_kernel(dkv_attn_args a, dkv_sparse
       u.high = min(TILE, m + 1 - piece * TILE);
     }
     const int bits = __builtin_amdgcn_readfirstlane(u.bits);
-    if (bits == 4) attend_unit<4, PREC>(u, q, scale2, c, g, r);
-    else if (bits == 8) attend_unit<8, PREC>(u, q, scale2, c, g, r);
-    else attend_unit<16, PREC>(u, q, scale2, c, g, r);
+    if (bits == 4) attend_unit<4, PREC, TERMS>(u, q, q_sum, scale2, c, g, r);
+    else if (bits == 8) attend_unit<8, PREC, TERMS>(u, q, q_sum, scale2, c, g, r);
+    else attend_unit<16, PREC, TERMS>(u, q, q_sum, scale2, c, g, r);
   }
   r.l = row_sum(r.l);
+  r.offset = PREC == 1 ? row_sum(r.offset) : 0.f;
   if (g == 0) ml[wave][c][0] = r.m, ml[wave][c][1] = r.l;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) o[wave][c][4 * g + i] = f32x4{r.o[0][i], r.o[1][i], r.o[2][i], r.o[3][i]};
+  for (int i = 0; i < 4; ++i) o[wave][c][4 * g + i] = f32x4{r.o[0][i], r.o[1][i], r.o[2][i], r.o[3][i]} + r.offset;
   __syncthreads();
   const int row = threadIdx.x >> 4, e4 = threadIdx.x & 15;  // the four waves' rows, four elements a thread
   if (row >= heads_here) return;
@@ -483,10 +497,9 @@ int dkv_attend_sparse(const dkv_attn_args* args, const dkv_sparse* sparse, void*
     hipLaunchKernelGGL(choose_kernel, dim3(a.nq, a.heads), dim3(256), 0, st, a, s, p.max_indexed, p.max_chosen, keys, lists);
   }
   const dim3 grid(p.splits, a.heads * p.row_blocks, a.nq);
-  if (a.precision == 1)
-    hipLaunchKernelGGL(attend_kernel<1>, grid, dim3(256), 0, st, a, s, p.row_blocks, p.most, p.max_chosen, lists, part_o, part_ml);
-  else
-    hipLaunchKernelGGL(attend_kernel<0>, grid, dim3(256), 0, st, a, s, p.row_blocks, p.most, p.max_chosen, lists, part_o, part_ml);
+  const auto attend = a.precision == 1 ? (a.out_dtype == 1 ? attend_kernel<1, 3> : attend_kernel<1, 2>)
+                                       : (a.out_dtype == 1 ? attend_kernel<0, 3> : attend_kernel<0, 2>);
+  hipLaunchKernelGGL(attend, grid, dim3(256), 0, st, a, s, p.row_blocks, p.most, p.max_chosen, lists, part_o, part_ml);
   if (p.splits > 1)
     hipLaunchKernelGGL(merge_kernel, dim3((a.q_heads / a.heads + 15) / 16, a.heads, a.nq), dim3(256), 0, st, a, s, p.most,
                        part_o, part_ml);
