@@ -3,8 +3,9 @@
 // The segments between the protected ends become one segment a width. Every layer and KV head keeps its own rows of
 // each width, as many as the host says, so the tile table is known before the kernels run and nothing waits for the
 // device: history rows carry no mask and no position of their own, so a tile may hold other tokens in every head.
-// Three launches: where each token lies, with the new tile table; the choice, a radix search for the smallest
-// kept mass per (layer, head, width); and the move, which is bound by memory (each kept row read and written once).
+// Three launches: where each token lies and which tokens each width has, with the new tile table; the choice, a radix
+// search for the smallest kept mass per (layer, head, width); and the move, which is bound by memory (each kept row
+// read and written once).
 #include "dkv_select.h"
 
 namespace dkv {
@@ -35,9 +36,29 @@ __host__ __device__ inline int64_t bytes_before(const dkv_evict_args& e, int c) 
   return n;
 }
 
-// place[token - lead_tokens]: the middle token's tile and class, tile * 4 + class.
-__global__ __launch_bounds__(256) void map_kernel(dkv_evict_args e, int32_t* place) {
-  const int i = blockIdx.x * 256 + threadIdx.x, mid_tiles = tiles_before(e, e.n_classes);
+// The middle's tokens: place[token - lead_tokens] is its tile, and order lists a class's tokens after another's.
+struct Work {
+  int32_t* place;
+  int32_t* order;
+};
+__host__ __device__ inline int held_before(const dkv_evict_args& e, int c) {
+  int n = 0;
+  for (int i = 0; i < c; ++i) n += e.class_held[i];
+  return n;
+}
+
+constexpr int MAP_TILES = 128;  // of the middle, a workgroup
+
+// Rows of each class, in 21 bits each.
+__device__ __forceinline__ uint64_t rows_by_class(const dkv_evict_args& e, const dkv_tile& t) {
+  const int c = class_of(e, t.bits);
+  return c < 3 ? (uint64_t)t.rows << (21 * c) : 0;
+}
+
+__global__ __launch_bounds__(THREADS) void map_kernel(dkv_evict_args e, Work w) {
+  __shared__ int before[3], at[MAP_TILES], start[MAP_TILES], rows[MAP_TILES];
+  __shared__ uint64_t half;
+  const int i = blockIdx.x * THREADS + threadIdx.x, mid_tiles = tiles_before(e, e.n_classes);
   const int tail_tiles = e.n_tiles - e.end_tile;
   if (i < e.lead_tiles) {
     e.out_tiles[i] = e.tiles[i];
@@ -58,20 +79,57 @@ __global__ __launch_bounds__(256) void map_kernel(dkv_evict_args e, int32_t* pla
     d.token_start += e.lead_tokens + rows_before(e, e.n_classes) - e.end_token;
     e.out_tiles[i] = d;
   }
-  // a wave a tile of the middle
-  const int t = e.lead_tiles + blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (t >= e.end_tile) return;
-  const dkv_tile d = e.tiles[t];
-  const int row = threadIdx.x & 63;
-  if (row < d.rows) place[d.token_start + row - e.lead_tokens] = t * 4 + class_of(e, d.bits);
+  const int first = e.lead_tiles + blockIdx.x * MAP_TILES, last = min(e.end_tile, first + MAP_TILES);
+  if (first >= last) return;
+  // rows of each class in the middle's tiles before these
+  if (threadIdx.x < 3) before[threadIdx.x] = 0;
+  __syncthreads();
+  int mine[3] = {0, 0, 0};
+  for (int t = e.lead_tiles + threadIdx.x; t < first; t += THREADS) {
+    const dkv_tile d = e.tiles[t];
+    const int c = class_of(e, d.bits);
+#pragma unroll
+    for (int j = 0; j < 3; ++j) mine[j] += c == j ? d.rows : 0;
+  }
+#pragma unroll
+  for (int j = 0; j < 3; ++j)
+    if (mine[j]) atomicAdd(&before[j], mine[j]);
+  // and in these, before each: two waves scan them
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, t = first + threadIdx.x;
+  dkv_tile d = {};
+  uint64_t upto = 0;
+  if (wave < MAP_TILES / 64) {
+    if (t < last) d = e.tiles[t];
+    upto = t < last ? rows_by_class(e, d) : 0;
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) {
+      const uint64_t o = (uint64_t)(uint32_t)__shfl_up((int)upto, k, 64) | (uint64_t)(uint32_t)__shfl_up((int)(upto >> 32), k, 64) << 32;
+      if (lane >= k) upto += o;
+    }
+    if (threadIdx.x == 63) half = upto;
+  }
+  __syncthreads();
+  if (wave < MAP_TILES / 64 && t < last) {
+    start[threadIdx.x] = d.token_start - e.lead_tokens, rows[threadIdx.x] = d.rows;
+    if (wave == 1) upto += half;
+    const int c = class_of(e, d.bits);
+    at[threadIdx.x] = c < 3 ? held_before(e, c) + before[c] + (int)(upto >> (21 * c) & ((1 << 21) - 1)) - d.rows : -1;
+  }
+  __syncthreads();
+  for (int k = wave; k < last - first; k += THREADS / 64) {
+    if (lane >= rows[k]) continue;
+    const int token = start[k] + lane;
+    w.place[token] = first + k;
+    if (at[k] >= 0) w.order[at[k] + lane] = token;
+  }
 }
 
 // blockIdx: (layer * heads + head, class). The class's tokens of the largest masses, in token order; equal masses
-// keep the earlier token. Class 0 also lists the protected ends.
-__global__ __launch_bounds__(THREADS) void choose_kernel(dkv_evict_args e, const int32_t* place) {
-  __shared__ SelectScratch scratch;
-  __shared__ uint32_t sums[THREADS / 64];
-  const int lh = blockIdx.x, c = blockIdx.y, n = e.end_token - e.lead_tokens;
+// keep the earlier token. Class 0 also lists the protected ends. Up to N * THREADS keys stay in registers.
+template <int N>
+__global__ __launch_bounds__(THREADS) void choose_kernel(dkv_evict_args e, Work w) {
+  __shared__ SelectScratch<THREADS, 11> scratch;
+  const int lh = blockIdx.x, c = blockIdx.y;
   const int mid = rows_before(e, e.n_classes), tail = e.tokens - e.end_token;
   const float* mass = e.mass + lh * e.mass_stride;
   int32_t* kept = e.kept + (int64_t)lh * (e.lead_tokens + mid + tail);
@@ -84,26 +142,26 @@ __global__ __launch_bounds__(THREADS) void choose_kernel(dkv_evict_args e, const
   }
   if (c >= e.n_classes) return;
   mass += e.lead_tokens;
-  int ties;
-  const uint32_t at = kth_largest<THREADS>(scratch, n, e.class_keep[c], ties, [&](int i, uint32_t& x) {
-    x = order_key(mass[i]);
-    return (place[i] & 3) == c;
+  const int32_t* order = w.order + held_before(e, c);
+  auto key = [&](int i) { return max(order_key(mass[order[i]]), 1u); };  // (1: not a number, below every number)
+  const int first = e.lead_tokens + rows_before(e, c), keep = e.class_keep[c];
+  Elements<THREADS, N, decltype(key)>(e.class_held[c], key).largest(scratch, (uint32_t)keep, [&](int to, int i) {
+    kept[first + to] = i;
   });
-  int listed = e.lead_tokens + rows_before(e, c), tied = 0;
-  const int end = listed + e.class_keep[c];
-  for (int i0 = 0; i0 < n; i0 += THREADS) {
-    const int i = i0 + threadIdx.x;
-    const bool here = i < n && (place[i] & 3) == c;
-    const float w = here ? mass[i] : 0.f;
-    const uint32_t x = order_key(w);
-    int count;
-    const bool tie = here && x == at;
-    const int rank = tied + block_rank<THREADS>(tie, sums, count);
-    tied += count;
-    const bool take = here && (x > at || (tie && rank < ties));
-    const int to = listed + block_rank<THREADS>(take, sums, count);
-    listed += count;
-    if (take && to < end) kept[to] = e.lead_tokens + i, out[to] = w;
+  __syncthreads();
+  constexpr int AHEAD = 8;  // loads in flight
+  for (int i0 = threadIdx.x; i0 < keep; i0 += AHEAD * THREADS) {
+    int token[AHEAD];
+    float m[AHEAD];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) token[j] = kept[first + min(i0 + j * THREADS, keep - 1)];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) token[j] = order[token[j]];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) m[j] = mass[token[j]];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j)
+      if (const int i = i0 + j * THREADS; i < keep) kept[first + i] = e.lead_tokens + token[j], out[first + i] = m[j];
   }
 }
 
@@ -114,7 +172,7 @@ __device__ __forceinline__ void move_rows(const dkv_evict_args& e, const dkv_til
                                           const int32_t* place, int lane) {
   constexpr int PIECES = BITS / 2, ROWS = 64 / PIECES, STEPS = TILE / ROWS;  // rows an instruction, instructions a tile
   const int token = kept[min(lane, d.rows - 1)];
-  const dkv_tile from = e.tiles[place[token - e.lead_tokens] >> 2];
+  const dkv_tile from = e.tiles[place[token - e.lead_tokens]];
   const int row = token - from.token_start;
   const int64_t from_sb = subblock_bytes(from.rows, BITS), to_sb = subblock_bytes(d.rows, BITS);
   const int64_t block = (int64_t)(layer * 2) * e.heads + h;
@@ -183,15 +241,16 @@ static bool fits(const dkv_evict_args& e) {
       e.tokens < e.end_token || e.n_classes < 0 || e.n_classes > 3 || e.lead_bytes < 0 || e.tail_offset < e.lead_bytes ||
       e.tail_bytes < 0 || (e.lead_bytes & 15) || (e.tail_offset & 15) || (e.tail_bytes & 15))
     return false;
-  int64_t kept = 0;
+  int64_t kept = 0, held = 0;
   for (int c = 0; c < e.n_classes; ++c) {
     if ((e.class_bits[c] != 4 && e.class_bits[c] != 8 && e.class_bits[c] != 16) || e.class_keep[c] <= 0) return false;
     for (int i = 0; i < c; ++i)
       if (e.class_bits[i] == e.class_bits[c]) return false;
-    kept += e.class_keep[c];
+    kept += e.class_keep[c], held += e.class_held[c];
+    if (e.class_held[c] < e.class_keep[c]) return false;
   }
   const int64_t total = e.lead_tokens + kept + e.tokens - e.end_token;
-  return kept <= e.end_token - e.lead_tokens && e.mass_stride >= e.tokens && e.out_mass_stride >= total &&
+  return held <= e.end_token - e.lead_tokens && e.mass_stride >= e.tokens && e.out_mass_stride >= total &&
          e.out_arena_bytes >= e.lead_bytes + bytes_before(e, e.n_classes) + e.tail_bytes &&
          e.arena_bytes >= e.tail_offset + e.tail_bytes;
 }
@@ -205,7 +264,7 @@ extern "C" {
 
 int64_t dkv_evict_workspace_bytes(const dkv_evict_args* args) {
   if (!args || args->end_token <= args->lead_tokens) return 0;
-  return 4 * ((int64_t)args->end_token - args->lead_tokens);
+  return 8 * ((int64_t)args->end_token - args->lead_tokens);
 }
 
 int dkv_evict(const dkv_evict_args* args, void* stream) {
@@ -236,12 +295,19 @@ int dkv_evict(const dkv_evict_args* args, void* stream) {
               (long long)e.workspace_bytes);
     return DKV_EINVAL;
   }
-  int32_t* place = static_cast<int32_t*>(e.workspace);
+  const evict::Work w{static_cast<int32_t*>(e.workspace), static_cast<int32_t*>(e.workspace) + (e.end_token - e.lead_tokens)};
   const int mid_tiles = evict::tiles_before(e, e.n_classes), out_tiles = e.lead_tiles + mid_tiles + e.n_tiles - e.end_tile;
-  const int by_tile = (out_tiles + 255) / 256, by_wave = (e.end_tile - e.lead_tiles + 3) / 4, lhs = e.layers * e.heads;
+  const int by_tile = (out_tiles + evict::THREADS - 1) / evict::THREADS, lhs = e.layers * e.heads;
+  const int by_range = (e.end_tile - e.lead_tiles + evict::MAP_TILES - 1) / evict::MAP_TILES;
   const hipStream_t st = (hipStream_t)stream;
-  hipLaunchKernelGGL(evict::map_kernel, dim3(by_tile > by_wave ? by_tile : by_wave), dim3(256), 0, st, e, place);
-  hipLaunchKernelGGL(evict::choose_kernel, dim3(lhs, e.n_classes ? e.n_classes : 1), dim3(evict::THREADS), 0, st, e, place);
+  hipLaunchKernelGGL(evict::map_kernel, dim3(by_tile > by_range ? by_tile : by_range), dim3(evict::THREADS), 0, st, e, w);
+  int n = 0;
+  for (int c = 0; c < e.n_classes; ++c) n = e.class_held[c] > n ? e.class_held[c] : n;
+  const auto choose = n <= 4 * evict::THREADS    ? evict::choose_kernel<4>
+                      : n <= 12 * evict::THREADS ? evict::choose_kernel<12>
+                      : n <= 32 * evict::THREADS ? evict::choose_kernel<32>
+                                                 : evict::choose_kernel<0>;
+  hipLaunchKernelGGL(choose, dim3(lhs, e.n_classes ? e.n_classes : 1), dim3(evict::THREADS), 0, st, e, w);
   const int64_t gathers = (int64_t)mid_tiles * ((lhs + 3) / 4);
   const int64_t copies = (e.lead_bytes + e.tail_bytes + evict::COPY_BYTES - 1) / evict::COPY_BYTES;
   if (gathers + copies > INT32_MAX) {
@@ -249,7 +315,7 @@ int dkv_evict(const dkv_evict_args* args, void* stream) {
     return DKV_EINVAL;
   }
   if (gathers + copies)
-    hipLaunchKernelGGL(evict::move_kernel, dim3((unsigned)(gathers + copies)), dim3(256), 0, st, e, (int)gathers, place);
+    hipLaunchKernelGGL(evict::move_kernel, dim3((unsigned)(gathers + copies)), dim3(256), 0, st, e, (int)gathers, w.place);
   return (int)hipGetLastError();
 }
 

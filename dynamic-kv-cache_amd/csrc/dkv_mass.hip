@@ -463,7 +463,8 @@ __global__ __launch_bounds__(256) void add_parts_kernel(dkv_attn_args a, MassArg
 
 constexpr int WORKGROUPS = 1024;  // workgroups of a launch, where there is work for as many
 constexpr int MAX_SPLITS = 32;    // ranges of units that the second launch joins for many rows, at most
-constexpr int MAX_SPLITS_FEW = 128;
+constexpr int WORKGROUPS_FEW = 512;  // (two a CU are resident, and each joins the splits once)
+constexpr int MAX_SPLITS_FEW = 64;
 constexpr int MAX_ROW_PARTS = 8;
 
 struct MassPlan {
@@ -476,7 +477,7 @@ static MassPlan plan_of(const dkv_attn_args& a) {
   const int64_t rows = (int64_t)(a.q_heads / a.heads) * a.nq, units = (int64_t)a.n_tiles + (a.nq + TILE - 1) / TILE;
   m.p.row_groups = (int)((rows + GROUP - 1) / GROUP);
   const bool few = rows <= FEW;
-  int64_t most = WORKGROUPS / ((int64_t)a.heads * m.p.row_groups);
+  int64_t most = (few ? WORKGROUPS_FEW : WORKGROUPS) / ((int64_t)a.heads * m.p.row_groups);
   const int64_t cap = few ? MAX_SPLITS_FEW : MAX_SPLITS;
   most = most < 1 ? 1 : most > cap ? cap : most;
   m.p.splits = split_count((int)most, (int)units, few);
@@ -539,7 +540,7 @@ int dkv_attention_mass(const dkv_attn_args* args, float* mass, int64_t mass_head
                                         : (rows <= 16 ? few_stats_kernel<0, 1> : few_stats_kernel<0, 4>);
     const auto columns = a.precision == 1 ? (rows <= 16 ? few_columns_kernel<1, 1> : few_columns_kernel<1, 4>)
                                           : (rows <= 16 ? few_columns_kernel<0, 1> : few_columns_kernel<0, 4>);
-    const int by_unit = (units + 3) / 4, most = 2 * WORKGROUPS / a.heads;
+    const int by_unit = (units + 3) / 4, most = WORKGROUPS_FEW / a.heads;
     hipLaunchKernelGGL(stats, dim3(p.splits, a.heads), dim3(256), 0, st, a, p);
     hipLaunchKernelGGL(columns, dim3(by_unit < most ? by_unit : most < 1 ? 1 : most, a.heads), dim3(256), 0, st, a, p);
     return (int)hipGetLastError();

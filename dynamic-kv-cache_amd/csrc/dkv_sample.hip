@@ -64,7 +64,7 @@ struct Cut {
 };
 
 struct Scratch {
-  SelectScratch select;
+  SelectScratch<THREADS, 8> select;
   uint64_t mass[256];
   uint64_t sums[THREADS / 64];
   uint32_t counts[THREADS / 64];
@@ -178,9 +178,8 @@ __device__ __forceinline__ void search_row(Scratch& s, const Row<T>& r, const Fi
   Cut ranked{0, vocab};
   if (top_k > 0 && top_k < vocab) {
     int ties;
-    ranked.key = kth_largest<THREADS>(s.select, vocab, (uint32_t)top_k, ties, [&](int i, uint32_t& x) {
-      x = order_key(r.at(i));
-      return true;
+    ranked.key = kth_largest<THREADS, 8>(s.select, (uint32_t)top_k, ties, [&](auto f) {
+      for (int i = threadIdx.x; i < vocab; i += THREADS) f(order_key(r.at(i)));
     });
     ranked.last = nth_of_key(s, r, ranked.key, ties);
   }

@@ -164,34 +164,19 @@ __global__ __launch_bounds__(256) void score_kernel(dkv_attn_args a, dkv_sparse 
   }
 }
 
-// The chosen tiles of a (query, KV head), in order.
-__global__ __launch_bounds__(256) void choose_kernel(dkv_attn_args a, dkv_sparse s, int max_indexed, int max_chosen,
-                                                     const uint32_t* keys, int32_t* lists) {
-  __shared__ SelectScratch scratch;
-  __shared__ uint32_t sums[4];
+// The chosen tiles of a (query, KV head), in order. Up to N * CHOOSERS keys stay in registers.
+constexpr int CHOOSERS = 256;
+template <int N>
+__global__ __launch_bounds__(CHOOSERS) void choose_kernel(dkv_attn_args a, dkv_sparse s, int max_indexed, int max_chosen,
+                                                          const uint32_t* keys, int32_t* lists) {
+  __shared__ SelectScratch<CHOOSERS, 8> scratch;
   const Seen v = seen_of(a, s);
   if (v.chosen == v.n_indexed) return;  // every tile, or none: no list is read
   const int64_t pair = (int64_t)blockIdx.y * a.nq + blockIdx.x;
   keys += pair * max_indexed;
   lists += pair * max_chosen;
-  int ties;
-  const uint32_t at = kth_largest<256>(scratch, v.n_indexed, v.chosen, ties, [&](int i, uint32_t& x) {
-    x = keys[i];
-    return true;
-  });
-  int listed = 0, tied = 0;
-  for (int i0 = 0; i0 < v.n_indexed; i0 += 256) {
-    const int i = i0 + threadIdx.x;
-    const uint32_t x = i < v.n_indexed ? keys[i] : 0u;
-    int n;
-    const bool tie = i < v.n_indexed && x == at;
-    const int rank = tied + block_rank<256>(tie, sums, n);
-    tied += n;
-    const bool take = i < v.n_indexed && (x > at || (tie && rank < ties));
-    const int place = listed + block_rank<256>(take, sums, n);
-    listed += n;
-    if (take) lists[place] = i;
-  }
+  auto key = [&](int i) { return max(keys[i], 1u); };
+  Elements<CHOOSERS, N, decltype(key)>(v.n_indexed, key).largest(scratch, (uint32_t)v.chosen, [&](int to, int i) { lists[to] = i; });
 }
 
 // A wave's running softmax over its units for 16 query rows: row c's maximum (base 2), this lane's share of its sum, of
@@ -359,12 +344,22 @@ __global__ __launch_bounds__(256) void merge_kernel(dkv_attn_args a, dkv_sparse 
   for (int d = 8; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 16));
   float l = 0.f;
   f32x4 x = {0, 0, 0, 0};
-#pragma unroll 4
-  for (int i = 0; i < splits; ++i) {
-    const float2 p = part_ml[first + (int64_t)i * G];
-    const float f = __builtin_amdgcn_exp2f(p.x - top);
-    l += f * p.y;
-    x += f * *reinterpret_cast<const f32x4*>(part_o + (first + (int64_t)i * G) * D + 4 * e4);
+  constexpr int AHEAD = 8;  // splits in flight
+  for (int i0 = 0; i0 < splits; i0 += AHEAD) {
+    float2 p[AHEAD];
+    f32x4 o[AHEAD];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      const int64_t at = first + (int64_t)min(i0 + j, splits - 1) * G;
+      p[j] = part_ml[at];
+      o[j] = *reinterpret_cast<const f32x4*>(part_o + at * D + 4 * e4);
+    }
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      const float f = i0 + j < splits ? __builtin_amdgcn_exp2f(p[j].x - top) : 0.f;
+      l += f * p[j].y;
+      x += f * o[j];
+    }
   }
   store4(a.out, a.out_dtype, m * a.out_tok_stride + (h * G + row) * a.out_head_stride + 4 * e4, x / l);
 }
@@ -494,7 +489,9 @@ int dkv_attend_sparse(const dkv_attn_args* args, const dkv_sparse* sparse, void*
   if (p.max_chosen > 0 && (p.max_chosen < p.max_indexed || a.step)) {
     hipLaunchKernelGGL(score_kernel, dim3((p.max_indexed + BLOCK - 1) / BLOCK, a.heads, (a.nq + SCORE_QUERIES - 1) / SCORE_QUERIES),
                        dim3(256), 0, st, a, s, p.max_indexed, keys);
-    hipLaunchKernelGGL(choose_kernel, dim3(a.nq, a.heads), dim3(256), 0, st, a, s, p.max_indexed, p.max_chosen, keys, lists);
+    const int n = p.max_indexed;
+    const auto choose = n <= 2 * CHOOSERS ? choose_kernel<2> : n <= 8 * CHOOSERS ? choose_kernel<8> : choose_kernel<0>;
+    hipLaunchKernelGGL(choose, dim3(a.nq, a.heads), dim3(CHOOSERS), 0, st, a, s, p.max_indexed, p.max_chosen, keys, lists);
   }
   const dim3 grid(p.splits, a.heads * p.row_blocks, a.nq);
   const auto attend = a.precision == 1 ? (a.out_dtype == 1 ? attend_kernel<1, 3> : attend_kernel<1, 2>)

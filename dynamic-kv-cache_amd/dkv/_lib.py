@@ -72,6 +72,7 @@ class EvictArgs(ctypes.Structure):
                 ('end_tile', ctypes.c_int32), ('end_token', ctypes.c_int32),
                 ('lead_bytes', ctypes.c_int64), ('tail_offset', ctypes.c_int64), ('tail_bytes', ctypes.c_int64),
                 ('n_classes', ctypes.c_int32), ('class_bits', ctypes.c_int32 * 3), ('class_keep', ctypes.c_int32 * 3),
+                ('class_held', ctypes.c_int32 * 3),
                 ('mass', ctypes.c_void_p), ('mass_stride', ctypes.c_int64),
                 ('out_arena', ctypes.c_void_p), ('out_arena_bytes', ctypes.c_int64), ('out_tiles', ctypes.c_void_p),
                 ('out_mass', ctypes.c_void_p), ('out_mass_stride', ctypes.c_int64), ('kept', ctypes.c_void_p),

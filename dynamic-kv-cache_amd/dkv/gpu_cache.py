@@ -884,6 +884,7 @@ class GPUCache(_CacheBase):
             e.n_classes = len(share)
             for i, (w, m) in enumerate(share.items()):
                 e.class_bits[i], e.class_keep[i] = w, m
+                e.class_held[i] = sum(s.rows for s in self.segments[a:b] if s.bits == w)
             e.mass, e.mass_stride = self._mass.data_ptr(), self.capacity
             e.out_arena, e.out_arena_bytes = into.arena.data_ptr(), into.arena_bytes
             e.out_tiles, e.out_mass, e.out_mass_stride = into.tiles.data_ptr(), into._mass.data_ptr(), into.capacity

@@ -430,8 +430,8 @@ int dkv_attention_mass(const dkv_attn_args* args, float* mass, int64_t mass_head
  * tail_offset) are copied whole. Of the tiles between, every layer and KV head
  * keeps the class_keep[c] tokens at class_bits[c] bits of the largest mass (equal
  * ones: the first; NaN last), in token order, as one segment a width in the order
- * of the classes; widths that no class names are dropped. At least class_keep[c]
- * tokens of that width must be there. The new tiles start at byte 0 of out_arena;
+ * of the classes; widths that no class names are dropped. class_held[c] is how
+ * many tokens of that width there are: the kernels trust it, and the tables. The new tiles start at byte 0 of out_arena;
  * out_tiles and out_mass (zeros after the kept tokens) are written to match, and
  * kept [layers, heads, new tokens] gets the old index of every new token. */
 typedef struct dkv_evict_args {
@@ -445,6 +445,7 @@ typedef struct dkv_evict_args {
   int64_t lead_bytes, tail_offset, tail_bytes;
   int32_t n_classes;         /* 0..3 */
   int32_t class_bits[3], class_keep[3];
+  int32_t class_held[3];     /* tokens of that width between */
   const float* mass;         /* [layers * heads] rows of mass_stride */
   int64_t mass_stride;
   void* out_arena;           /* must not overlap arena */
