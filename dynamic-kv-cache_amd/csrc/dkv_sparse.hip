@@ -24,7 +24,16 @@ __device__ __forceinline__ int64_t piece_at(int block, int layer, int layers, in
   return (((int64_t)block * layers + layer) * heads + h) * BLOCK_PIECES * BLOCK;
 }
 
-constexpr int INDEX_TILES = 16;  // tiles of an index workgroup, four a wave
+constexpr int INDEX_TILES = 16;  // tiles of an index workgroup, a wave a tile
+
+// One step of a minimum (and maximum, of the negated) over lanes that halves the elements a lane holds: x keeps the lower
+// half's lanes, y the upper half's. v_permlane swaps x's upper lanes with y's lower ones.
+template <int LANES>
+__device__ __forceinline__ void swap_lanes(float& x, float& y) {
+  const auto r = LANES == 32 ? __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(y), false, false)
+                             : __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(y), false, false);
+  x = __uint_as_float(r[0]), y = __uint_as_float(r[1]);
+}
 
 // The bounds of a tile's keys, dequantized. Lane (row / 4, quarter): 16 elements of every 16th row; then halves of
 // the elements change lanes, so that each lane ends with one element's bounds.
@@ -36,17 +45,25 @@ __device__ __forceinline__ void tile_bounds(const UnitRows& u, int lane, float& 
   for (int j = 0; j < 4; ++j) load_key<BITS>(u, 16 * j + (lane >> 2), lane & 3, p[j]);
 #pragma unroll
   for (int e = 0; e < 16; ++e) {
-    lo[e] = INFINITY, hi[e] = -INFINITY;
+    float x[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float x = BITS == 16 ? (e & 1 ? bf16_hi(p[j].w[e / 2]) : bf16_lo(p[j].w[e / 2]))
-                                 : code_at<BITS>(p[j].w, e) * p[j].as.y + p[j].as.x;
-      lo[e] = fminf(lo[e], x);
-      hi[e] = fmaxf(hi[e], x);
-    }
+    for (int j = 0; j < 4; ++j)
+      x[j] = BITS == 16 ? (e & 1 ? bf16_hi(p[j].w[e / 2]) : bf16_lo(p[j].w[e / 2])) : code_at<BITS>(p[j].w, e) * p[j].as.y + p[j].as.x;
+    lo[e] = fminf(fminf(fminf(x[0], x[1]), x[2]), x[3]);
+    hi[e] = fmaxf(fmaxf(fmaxf(x[0], x[1]), x[2]), x[3]);
   }
 #pragma unroll
-  for (int half = 8, bit = 32; half >= 1; half >>= 1, bit >>= 1) {
+  for (int e = 0; e < 8; ++e) {
+    swap_lanes<32>(lo[e], lo[e + 8]), swap_lanes<32>(hi[e], hi[e + 8]);
+    lo[e] = fminf(lo[e], lo[e + 8]), hi[e] = fmaxf(hi[e], hi[e + 8]);
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    swap_lanes<16>(lo[e], lo[e + 4]), swap_lanes<16>(hi[e], hi[e + 4]);
+    lo[e] = fminf(lo[e], lo[e + 4]), hi[e] = fmaxf(hi[e], hi[e + 4]);
+  }
+#pragma unroll
+  for (int half = 2, bit = 8; half >= 1; half >>= 1, bit >>= 1) {
     const bool upper = lane & bit;
 #pragma unroll
     for (int e = 0; e < half; ++e) {
@@ -59,27 +76,27 @@ __device__ __forceinline__ void tile_bounds(const UnitRows& u, int lane, float& 
   low = lo[0], high = hi[0];
 }
 
-__global__ __launch_bounds__(256) void index_kernel(const uint8_t* arena, const dkv_tile* tiles, int tile0, int tile1,
-                                                    int layers, int heads, u32x4* bounds) {
+__global__ __launch_bounds__(64 * INDEX_TILES) void index_kernel(const uint8_t* arena, const dkv_tile* tiles, int tile0, int tile1,
+                                                                 int layers, int heads, u32x4* bounds) {
   __shared__ u32x4 out[BLOCK_PIECES][INDEX_TILES];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int first = (tile0 / INDEX_TILES + blockIdx.x) * INDEX_TILES;
   const int layer = blockIdx.y / heads, h = blockIdx.y % heads;
-  dkv_attn_args a{};
-  a.arena = arena, a.layer = layer, a.heads = heads;
-  for (int i = wave; i < INDEX_TILES; i += 4) {
-    const int t = first + i;
-    if (t < tile0 || t >= tile1) continue;
+  if (const int t = first + wave; t >= tile0 && t < tile1) {
+    dkv_attn_args a{};
+    a.arena = arena, a.layer = layer, a.heads = heads;
     const UnitRows u = tile_rows(a, tiles[t], INT32_MAX, h);
+    const int bits = __builtin_amdgcn_readfirstlane(u.bits);
     float low, high;
-    if (u.bits == 4) tile_bounds<4>(u, lane, low, high);
-    else if (u.bits == 8) tile_bounds<8>(u, lane, low, high);
+    if (bits == 4) tile_bounds<4>(u, lane, low, high);
+    else if (bits == 8) tile_bounds<8>(u, lane, low, high);
     else tile_bounds<16>(u, lane, low, high);
     const int d = 16 * (lane & 3) + 8 * (lane >> 5) + 4 * (lane >> 4 & 1) + 2 * (lane >> 3 & 1) + (lane >> 2 & 1);
-    reinterpret_cast<uint16_t*>(&out[d / 8][i])[d % 8] = (uint16_t)f32_to_bf16_rne(low);
-    reinterpret_cast<uint16_t*>(&out[8 + d / 8][i])[d % 8] = (uint16_t)f32_to_bf16_rne(high);
+    reinterpret_cast<uint16_t*>(&out[d / 8][wave])[d % 8] = (uint16_t)f32_to_bf16_rne(low);
+    reinterpret_cast<uint16_t*>(&out[8 + d / 8][wave])[d % 8] = (uint16_t)f32_to_bf16_rne(high);
   }
   __syncthreads();
+  if (threadIdx.x >= BLOCK_PIECES * INDEX_TILES) return;
   const int p = threadIdx.x / INDEX_TILES, i = threadIdx.x % INDEX_TILES, t = first + i;
   if (t >= tile0 && t < tile1) bounds[piece_at(t / BLOCK, layer, layers, h, heads) + p * BLOCK + t % BLOCK] = out[p][i];
 }
@@ -127,17 +144,29 @@ __global__ __launch_bounds__(256) void score_kernel(dkv_attn_args a, dkv_sparse 
   if (v.chosen == v.n_indexed || block * BLOCK >= v.n_indexed) return;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, G = a.q_heads / a.heads;
   const int queries = min(SCORE_QUERIES, a.nq - m0);
-  for (int i = threadIdx.x; i < queries * D; i += 256) {
-    const int m = i / D, d = i % D;
-    double plus = 0, minus = 0;
-    for (int g = 0; g < G; ++g) {
-      const uint16_t* q = static_cast<const uint16_t*>(a.q) + (h * G + g) * a.q_head_stride + (m0 + m) * a.q_tok_stride;
-      const float x = bf16_lo(q[d]);
-      plus += x > 0.f ? x : 0.f;
-      minus += x > 0.f ? 0.f : x;
-    }
-    query[m][d] = minus;  // meets low
-    query[m][D + d] = plus;
+  constexpr int EACH = SCORE_QUERIES * D / 256, AHEAD = 4;  // sums a thread; query heads in flight
+  double plus[EACH] = {}, minus[EACH] = {};
+  const int d = threadIdx.x % D;
+  for (int g0 = 0; g0 < G; g0 += AHEAD) {
+    float x[AHEAD][EACH];
+#pragma unroll
+    for (int g = 0; g < AHEAD; ++g)
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) {
+        const int m = min(i * (256 / D) + (int)threadIdx.x / D, queries - 1);
+        x[g][i] = bf16_lo((static_cast<const uint16_t*>(a.q) + (h * G + min(g0 + g, G - 1)) * a.q_head_stride + (m0 + m) * a.q_tok_stride)[d]);
+      }
+#pragma unroll
+    for (int g = 0; g < AHEAD; ++g)
+#pragma unroll
+      for (int i = 0; i < EACH; ++i)
+        if (g0 + g < G) plus[i] += x[g][i] > 0.f ? x[g][i] : 0.f, minus[i] += x[g][i] > 0.f ? 0.f : x[g][i];
+  }
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const int m = i * (256 / D) + (int)threadIdx.x / D;
+    query[m][d] = minus[i];  // meets low
+    query[m][D + d] = plus[i];
   }
   const u32x4* from = static_cast<const u32x4*>(s.bounds) + piece_at(block, a.layer, a.layers, h, a.heads) +
                       4 * wave * BLOCK + lane;
@@ -286,11 +315,18 @@ __global__ __launch_bounds__(256) void attend_kernel(dkv_attn_args a, dkv_sparse
   const int piece0 = start / TILE, units = v.chosen + tail + m / TILE - piece0 + 1;
   const bool listed = v.chosen < v.n_indexed;
   const float scale2 = a.scale * LOG2E;
-  for (int i = blockIdx.x * 4 + wave; i < units; i += 4 * splits) {
+  auto tile_at = [&](int i) {  // unit i's tile (any that can be read where it is a chunk piece)
+    const int j = min(i, v.chosen + tail - 1);
+    return a.tiles[j >= v.chosen ? v.n_indexed + j - v.chosen : listed ? lists[pair * max_chosen + j] : j];
+  };
+  int i = blockIdx.x * 4 + wave;
+  dkv_tile t = {};
+  if (v.chosen + tail > 0) t = tile_at(i);
+  for (; i < units; i += 4 * splits) {
     UnitRows u;
     if (i < v.chosen + tail) {
-      const int t = i >= v.chosen ? v.n_indexed + i - v.chosen : listed ? lists[pair * max_chosen + i] : i;
-      u = tile_rows(a, a.tiles[t], v.past, h);
+      u = tile_rows(a, t, v.past, h);
+      t = tile_at(i + 4 * splits);  // the next unit's, while this one is computed
     } else {
       const int piece = piece0 + i - v.chosen - tail;
       u = chunk_rows(a, piece, h);
@@ -364,7 +400,7 @@ __global__ __launch_bounds__(256) void merge_kernel(dkv_attn_args a, dkv_sparse 
   store4(a.out, a.out_dtype, m * a.out_tok_stride + (h * G + row) * a.out_head_stride + 4 * e4, x / l);
 }
 
-constexpr int WORKGROUPS = 512;  // attention workgroups that a call is split into
+constexpr int WORKGROUPS = 1024;  // attention workgroups that a call is split into
 
 static SparsePlan plan_of(const dkv_attn_args& a, const dkv_sparse& s) {
   SparsePlan p{};
@@ -441,7 +477,7 @@ int dkv_index(const void* arena, const dkv_tile* tiles, int32_t tile0, int32_t n
     return DKV_EINVAL;
   }
   const int groups = (n_tiles + INDEX_TILES - 1) / INDEX_TILES - tile0 / INDEX_TILES;
-  hipLaunchKernelGGL(index_kernel, dim3(groups, layers * heads), dim3(256), 0, (hipStream_t)stream,
+  hipLaunchKernelGGL(index_kernel, dim3(groups, layers * heads), dim3(64 * INDEX_TILES), 0, (hipStream_t)stream,
                      static_cast<const uint8_t*>(arena), tiles, tile0, n_tiles, layers, heads, static_cast<u32x4*>(bounds));
   return (int)hipGetLastError();
 }
