@@ -101,16 +101,21 @@ __global__ __launch_bounds__(64 * INDEX_TILES) void index_kernel(const uint8_t* 
   if (t >= tile0 && t < tile1) bounds[piece_at(t / BLOCK, layer, layers, h, heads) + p * BLOCK + t % BLOCK] = out[p][i];
 }
 
-// The history a launch sees: the arguments' or the device step's {past, n_tiles, n_indexed}.
+// The history a launch sees: the arguments' or the device step's {past, n_tiles, n_indexed, single_rows}. A query attends
+// to the `chosen` tiles of the index, to the `tiles` after it that are units of their own, and to the last single_rows
+// tiles, of one 16-bit row each, 64 a unit: generated tokens, whose rows lie a slab apart.
 struct Seen {
-  int past, n_tiles, n_indexed, chosen;  // chosen: tiles a query chooses of the indexed ones
+  int past, n_tiles, n_indexed, single_rows, chosen, tiles, singles;
 };
 
 __device__ __forceinline__ Seen seen_of(const dkv_attn_args& a, const dkv_sparse& s) {
-  Seen v{a.past, a.n_tiles, s.n_indexed, 0};
-  if (a.step) v = Seen{a.step[0], a.step[1], a.step[2], 0};
+  Seen v{a.past, a.n_tiles, s.n_indexed, s.single_rows};
+  if (a.step) v = Seen{a.step[0], a.step[1], a.step[2], a.step[3]};
   v.n_indexed = min(min(v.n_indexed, s.n_indexed), v.n_tiles);
+  v.single_rows = min(v.single_rows, v.n_tiles - v.n_indexed);
   v.chosen = min(s.blocks, v.n_indexed);
+  v.tiles = v.n_tiles - v.n_indexed - v.single_rows;
+  v.singles = (v.single_rows + TILE - 1) / TILE;
   return v;
 }
 
@@ -128,7 +133,7 @@ __host__ __device__ inline int split_count(int most, int64_t units) {
   return want < 1 ? 1 : want < most ? (int)want : most;
 }
 __device__ __forceinline__ int splits_of(const dkv_attn_args& a, const Seen& v, int most) {
-  return split_count(most, (int64_t)v.chosen + v.n_tiles - v.n_indexed + (a.nq + TILE - 1) / TILE);
+  return split_count(most, (int64_t)v.chosen + v.tiles + v.singles + (a.nq + TILE - 1) / TILE);
 }
 
 constexpr int SCORE_QUERIES = 16;
@@ -311,24 +316,29 @@ __global__ __launch_bounds__(256) void attend_kernel(dkv_attn_args a, dkv_sparse
   r.m = -INFINITY, r.l = r.offset = 0.f;
   const float q_sum = query_sum(q);
   for (int db = 0; db < 4; ++db) r.o[db] = f32x4{0, 0, 0, 0};
-  const int start = chunk_seg_start(a, m), tail = v.n_tiles - v.n_indexed;
-  const int piece0 = start / TILE, units = v.chosen + tail + m / TILE - piece0 + 1;
+  const int start = chunk_seg_start(a, m), own_tile = v.chosen + v.tiles, history = own_tile + v.singles;
+  const int piece0 = start / TILE, units = history + m / TILE - piece0 + 1;
   const bool listed = v.chosen < v.n_indexed;
   const float scale2 = a.scale * LOG2E;
-  auto tile_at = [&](int i) {  // unit i's tile (any that can be read where it is a chunk piece)
-    const int j = min(i, v.chosen + tail - 1);
+  auto tile_at = [&](int i) {  // unit i's (first) tile, any that can be read where it is a chunk piece
+    const int j = min(i, history - 1);
+    if (j >= own_tile) return a.tiles[v.n_tiles - v.single_rows + TILE * (j - own_tile)];
     return a.tiles[j >= v.chosen ? v.n_indexed + j - v.chosen : listed ? lists[pair * max_chosen + j] : j];
   };
   int i = blockIdx.x * 4 + wave;
   dkv_tile t = {};
-  if (v.chosen + tail > 0) t = tile_at(i);
+  if (history > 0) t = tile_at(i);
   for (; i < units; i += 4 * splits) {
     UnitRows u;
-    if (i < v.chosen + tail) {
+    if (i < history) {
       u = tile_rows(a, t, v.past, h);
+      if (i >= own_tile) {
+        u.rows = u.high = min(TILE, v.single_rows - TILE * (i - own_tile));
+        u.k_stride = u.v_stride = slab_bytes(1, 16, a.layers, a.heads);
+      }
       t = tile_at(i + 4 * splits);  // the next unit's, while this one is computed
     } else {
-      const int piece = piece0 + i - v.chosen - tail;
+      const int piece = piece0 + i - history;
       u = chunk_rows(a, piece, h);
       u.low = max(0, start - piece * TILE);
       u.high = min(TILE, m + 1 - piece * TILE);
@@ -409,7 +419,8 @@ static SparsePlan plan_of(const dkv_attn_args& a, const dkv_sparse& s) {
   p.max_indexed = s.n_indexed < a.n_tiles ? s.n_indexed : a.n_tiles;
   p.max_chosen = s.blocks < p.max_indexed ? s.blocks : p.max_indexed;
   const int64_t pairs = (int64_t)a.heads * a.nq;
-  const int64_t units = p.max_chosen + (a.n_tiles - p.max_indexed) + (a.nq + TILE - 1) / TILE;
+  const int tail = a.n_tiles - p.max_indexed, single = a.step ? 0 : s.single_rows < tail ? s.single_rows : tail;
+  const int64_t units = (int64_t)p.max_chosen + tail - single + (single + TILE - 1) / TILE + (a.nq + TILE - 1) / TILE;
   const int64_t most = WORKGROUPS / (pairs * p.row_blocks);
   p.most = most < 1 ? 1 : (int)most;
   p.splits = split_count(p.most, units);
@@ -503,8 +514,9 @@ int dkv_attend_sparse(const dkv_attn_args* args, const dkv_sparse* sparse, void*
     set_error("dkv_attend_sparse: V and out must be 16-byte aligned, strides multiples of 8 and 4 elements, out bf16 (0) or fp32 (1)");
     return DKV_EINVAL;
   }
-  if (s.n_indexed < 0 || s.blocks < 0 || (s.n_indexed > 0 && (!s.bounds || ((uintptr_t)s.bounds & 15)))) {
-    set_error("dkv_attend_sparse: n_indexed %d and blocks %d must not be negative, bounds 16-byte aligned", s.n_indexed, s.blocks);
+  if (s.n_indexed < 0 || s.blocks < 0 || s.single_rows < 0 || (s.n_indexed > 0 && (!s.bounds || ((uintptr_t)s.bounds & 15)))) {
+    set_error("dkv_attend_sparse: n_indexed %d, blocks %d and single_rows %d must not be negative, bounds 16-byte aligned", s.n_indexed,
+              s.blocks, s.single_rows);
     return DKV_EINVAL;
   }
   if (a.nq > 65535) {

@@ -61,7 +61,8 @@ class SegmentIO(ctypes.Structure):
 
 
 class Sparse(ctypes.Structure):
-    _fields_ = [('bounds', ctypes.c_void_p), ('n_indexed', ctypes.c_int32), ('blocks', ctypes.c_int32)]
+    _fields_ = [('bounds', ctypes.c_void_p), ('n_indexed', ctypes.c_int32), ('blocks', ctypes.c_int32),
+                ('single_rows', ctypes.c_int32)]
 
 
 class EvictArgs(ctypes.Structure):

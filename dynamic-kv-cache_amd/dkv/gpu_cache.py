@@ -126,6 +126,7 @@ class GPUCache(_CacheBase):
         self.plan = []  # (start, end, bits, row) per segment, as in the reference
         self.segments = []
         self.tile_starts = []  # first token of every tile, in token order
+        self.tile_singles = []  # of every tile, how many tiles up to it hold one 16-bit row each
         self.host_counts = {4: 0, 8: 0, 16: 0}
         self.arena_used = 0
         planned = []
@@ -185,6 +186,8 @@ class GPUCache(_CacheBase):
         for t in range((n + TILE - 1) // TILE):
             _lib.TILE.pack_into(self._tiles_host_bytes, 16 * (tile0 + t), self.arena_used + t * slab,
                                 start + t * TILE, min(n - t * TILE, TILE), bits, 0)
+            single = bits == 16 and n - t * TILE == 1
+            self.tile_singles.append(1 + (self.tile_singles[-1] if self.tile_singles else 0) if single else 0)
         self.plan.append((start, start + n, bits, self.host_counts[bits]))
         self.host_counts[bits] += n
         self.arena_used += need
@@ -223,6 +226,10 @@ class GPUCache(_CacheBase):
         entries['bits'] = np.repeat(b, counts)
         entries['reserved'] = 0
         self.tile_starts.extend(entries['token_start'].tolist())
+        run = self.tile_singles[-1] if self.tile_singles else 0
+        for single in ((entries['rows'] == 1) & (entries['bits'] == 16)).tolist():
+            run = run + 1 if single else 0
+            self.tile_singles.append(run)
         held = self.host_counts
         for s, w, c, off, t in zip(starts.tolist(), bits, lengths, (ends - need).tolist(), first.tolist()):
             self.segments.append(_Segment(s, c, w, off, t, frame))
@@ -720,6 +727,11 @@ class GPUCache(_CacheBase):
             return self.attend_args(q, k, v, layer, past, out, segments, 0, 0, precision)
         return make.attend_args(q, k, v, layer, out, segments, 0, 0, precision)
 
+    def _single_rows(self, n_tiles):
+        """How many of the first n_tiles' last tiles hold one 16-bit row each (generated tokens) and are not in
+        the index. Tiles that follow each other lie one after the other in the arena."""
+        return min(self.tile_singles[n_tiles - 1], n_tiles - self.n_indexed) if n_tiles > self.n_indexed else 0
+
     def attend_sparse(self, q, k, v, layer, past, blocks, out_dtype=None, segments=None, precision=None):
         """attend() over a part of a long history: each query attends to the `blocks` tiles of the index
         (index()) whose keys can score highest for it, to every token appended after the index, and to its
@@ -737,7 +749,8 @@ class GPUCache(_CacheBase):
         if not n:
             return out
         a = self._chunk_args(q, k, v, layer, past, out, segments, precision)
-        s = _lib.Sparse(0 if self._bounds is None else self._bounds.data_ptr(), self.n_indexed, blocks)
+        s = _lib.Sparse(0 if self._bounds is None else self._bounds.data_ptr(), self.n_indexed, blocks,
+                        0 if self._graph is not None else self._single_rows(a.n_tiles))
         if self._graph is not None:
             s.n_indexed = self._graph.indexed_bound()
         need = _lib.load().dkv_attend_sparse_workspace_bytes(ctypes.byref(a), ctypes.byref(s))
@@ -934,6 +947,7 @@ class GPUCache(_CacheBase):
         other.plan = self.plan.copy()
         other.segments = self.segments.copy()
         other.tile_starts = self.tile_starts.copy()
+        other.tile_singles = self.tile_singles.copy()
         other.host_counts = self.host_counts.copy()
         other._workspace = None
         other._graph = None
@@ -1016,6 +1030,7 @@ class GPUCache(_CacheBase):
         self._clear_mass()
         if self.online:
             self.segments, self.tile_starts, self.plan = [], [], []
+            self.tile_singles = []
             self.host_counts = {4: 0, 8: 0, 16: 0}
             self.arena_used = 0
 
@@ -1140,7 +1155,7 @@ class GraphSteps:
     """Device-side step parameters of one GPUCache for HIP-graph replays.
 
     One device buffer holds a pack job per layer (dkv_pack_batch reads layer l's job) and the
-    {past, n_tiles, n_indexed} that attention launches read (dkv_attn_args.step). step() does the host
+    {past, n_tiles, n_indexed, single_rows} that attention launches read (dkv_attn_args.step). step() does the host
     bookkeeping of one chunk and uploads the buffer through a ring of pinned host copies, so the
     host can prepare step i+1 while the GPU still runs step i. The K/V pointers of the jobs are
     those append() saw while the graph was captured (they are fixed for a captured graph): a
@@ -1230,7 +1245,7 @@ class GraphSteps:
 
     def _view(self, host):
         """(jobs, tail) numpy views of a pinned ring buffer: the per-layer PackJob array, then the
-        int32 values past, n_tiles, n_indexed."""
+        int32 values past, n_tiles, n_indexed, single_rows."""
         raw = host.numpy()
         split = self.cache.layers * self.job_bytes
         return raw[:split].view(self.JOB), raw[split:split + 16].view(np.int32)
@@ -1253,7 +1268,8 @@ class GraphSteps:
             write_job_sources(jobs, self.kv)
             self.slot_kv[self.slot] = self.kv_version
         write_step_jobs(jobs, seg, past, n, write)
-        tail[0], tail[1], tail[2] = past, c._tiles_before(past), c.n_indexed
+        n_tiles = c._tiles_before(past)
+        tail[:] = past, n_tiles, c.n_indexed, c._single_rows(n_tiles)
         if all(kv is not None for kv in self.kv):
             _lib.check(_lib.load().dkv_pack_validate(host.data_ptr(), c.layers, c.arena_bytes, c.layers, c.heads),
                        'dkv_pack_validate')

@@ -399,14 +399,17 @@ typedef struct dkv_sparse {
   const void* bounds; /* the index (may be NULL while n_indexed is 0) */
   int32_t n_indexed;  /* tiles [0, n_indexed) are in the index; those after it are always attended */
   int32_t blocks;     /* tiles that a query attends to of the indexed ones */
+  int32_t single_rows; /* 0, or how many of the last tiles hold one 16-bit row each, in consecutive
+                          slabs (generated tokens): they are attended to 64 at a time */
 } dkv_sparse;
 
 /* dkv_attend over the `blocks` tiles of the index with the largest
  *   sum over the KV head's query heads and d of max(q_d * smallest_d, q_d * largest_d)
  * for each query and KV head (rounded to fp32; equal ones: the first tiles; NaN
  * last), every tile after the index, and the chunk. Of args, path, splits and
- * tiles_host are not read; a step (HIP graph replays) has three elements,
- * {past, n_tiles, n_indexed}, which must stay within the arguments' values.
+ * tiles_host are not read; a step (HIP graph replays) has four elements,
+ * {past, n_tiles, n_indexed, single_rows}, the first three within the arguments'
+ * values.
  * `precision` as in dkv_attend, but p is never rounded below 16 bits. With
  * blocks >= n_indexed the call is dense attention. At most 65535 queries. */
 int64_t dkv_attend_sparse_workspace_bytes(const dkv_attn_args* args, const dkv_sparse* sparse);

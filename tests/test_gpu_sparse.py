@@ -180,6 +180,36 @@ def test_history_after_the_index(cuda, indexed):
     check(cuda, RAGGED + [(1, 16)] * 20, 3, 9, 4, 2, 'bf16', indexed=indexed)
 
 
+@pytest.mark.parametrize('tail', [1, 63, 64, 65, 130])
+def test_generated_tokens_after_the_index(cuda, tail):
+    """Runs of one-row tiles, which are taken 64 at a time, with a frame among them or none."""
+    check(cuda, RAGGED + [(1, 16)] * tail, 2, 6, 2, 3, 'fp32', indexed=10)
+    check(cuda, RAGGED + [(1, 16)] * 5 + [(64, 16)] + [(1, 16)] * tail, 3, 9, 1, 2, 'bf16', indexed=10, layers=2, layer=1)
+    check(cuda, [(65, 16)] + [(1, 16)] * tail, 1, 3, 3, 1, 'bf16', indexed=1)
+
+
+def test_generated_tokens_at_other_widths_and_in_branches(cuda):
+    """Only 16-bit rows lie evenly; a branch counts its own tiles, a reset cache none."""
+    c, dk, dv = build(cuda, RAGGED + [(1, 8)] * 3 + [(1, 16)] * 4, 2)
+    q, kn, vn = chunk_of(2, 6, 1, 7)
+    qc, kc, vc = (t[None].to(cuda) for t in (q, kn, vn))
+    past = dk.shape[2]
+    k = torch.cat((dk[0].to(torch.bfloat16).float(), kn.float()), 1)
+    v = torch.cat((dv[0].to(torch.bfloat16).float(), vn.float()), 1)
+    ref = expected(q, k, v, past, torch.ones(2, 1, past, dtype=torch.bool))
+    for cache in (c, c.fork()):
+        cache.select(16)
+        cache.append(kc, vc, 0)
+        out = cache.attend_sparse(qc, kc, vc, 0, past, 2, out_dtype=torch.float32)
+        assert ((out[0].cpu().double() - ref).abs() <= tolerance(ref, v, torch.float32, 'bf16')).all()
+        assert cache.tile_singles[-5:] == [1, 2, 3, 4, 5]
+    c.reset()
+    c.select(4)
+    for _ in range(3):
+        c.append(kc, vc, 0)
+    assert c.tile_singles == [0, 0, 0] and c._single_rows(3) == 0
+
+
 def test_layers_and_strides(cuda):
     check(cuda, RAGGED, 3, 9, 9, 3, 'bf16', layers=3, layer=2, strided=True)
 
