@@ -1340,7 +1340,12 @@ class GraphSteps:
         a.layer, a.layers, a.heads, a.q_heads, a.nq = 0, self.cache.layers, self.cache.heads, q_heads, self.chunk
         a.precision = PRECISIONS[self.cache.precision]
         a.step = self.dev.data_ptr() + self.cache.layers * self.job_bytes  # launches sized for any history
-        return _lib.load().dkv_attend_workspace_bytes(ctypes.byref(a))
+        lib, c = _lib.load(), self.cache
+        need = lib.dkv_attend_workspace_bytes(ctypes.byref(a))
+        if c.sparse_blocks:
+            s = _lib.Sparse(None, self.indexed_bound(), c.sparse_blocks, 0)
+            need = max(need, lib.dkv_attend_sparse_workspace_bytes(ctypes.byref(a), ctypes.byref(s)))
+        return max(need, lib.dkv_attention_mass_workspace_bytes(ctypes.byref(a))) if c.observing else need
 
 
 class SegmentExport:

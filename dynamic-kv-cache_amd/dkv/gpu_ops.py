@@ -426,7 +426,8 @@ def fused_decoder_layer(layer, hidden_states, cache, position_embeddings):
     if p is None:
         return None
     tiles = _layer_tiles(layer, p)
-    if p.eager_ok and p.kv_heads == cache.heads and cache._graph is None and cache.chunk_segments is None:
+    if (p.eager_ok and p.kv_heads == cache.heads and cache._graph is None and cache.chunk_segments is None
+            and not cache.sparse_blocks and not cache.observing):
         cos, sin = position_embeddings
         if (h.is_contiguous() and h.data_ptr() % 16 == 0 and cos.shape == (1, n, 64) and sin.shape == cos.shape
                 and cos.dtype == torch.bfloat16 and sin.dtype == torch.bfloat16 and cos.is_contiguous()

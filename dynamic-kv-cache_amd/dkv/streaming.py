@@ -7,7 +7,10 @@ place of the vision encoder:
 - ingest(): one decoder forward for a text prefix, then one per 64-token frame.
   The cache's width is selected per frame (cache.select(bits, i),
   src/streaming.py:178), and every LlamaAttention packs its K/V and attends
-  over the packed history (install_packed_attention).
+  over the packed history (install_packed_attention). With a budget the cache counts the
+  frames' attention and evicts the tokens that got least of it, so a stream has no end.
+- generate(): tokens drawn one after the other on a fork from given random numbers, each
+  attending to all of the history or to the part of it that scores highest for it.
 - answer(): the reference's 'candidate' protocol (src/streaming.py:209-225).
   For each candidate, a fork of the cache runs question + candidate tokens, and
   the score is the mean log-likelihood of the candidate tokens. answer_labels()
@@ -24,7 +27,7 @@ workloads are synthetic; see dkv.workloads.decoder_config.
 import torch
 
 from .gpu_cache import GPUCache, install_packed_attention
-from .gpu_ops import install_fused_ops
+from .gpu_ops import install_fused_ops, sample
 
 MFMA_ROWS = 192  # query rows per frame-chunk attention workgroup (MFMA_ROWS of csrc/dkv_attn_common.h)
 
@@ -60,6 +63,7 @@ class StreamingDecoder:
         install_fused_ops(self.text, self.ops_state)
         install_packed_attention(model)
         self._cache = None  # reused across requests when graphs=True (a captured graph records its buffers)
+        self._spare = None  # the cache that _cache evicts into and back, and that cache's captured forwards
         self._graphs = {}  # chunk length -> captured forward of that length on self._cache
         self._group_graphs = {}  # (chunk length, k) -> captured forwards of k consecutive chunks (pipelined)
         self._qa_graphs = {}  # (chunk length, logits, segments) -> captured forward + lm_head on a fork
@@ -93,6 +97,11 @@ class StreamingDecoder:
                         dtype=self.model.dtype, max_tokens=max_tokens, precision=self.precision,
                         device=self.device, **kw)
 
+    @staticmethod
+    def _position(cache, past=None):
+        """Position of the token after `past` held ones (default: all): evicted tokens keep theirs."""
+        return (cache.get_seq_length() if past is None else past) + getattr(cache, 'dropped', 0)
+
     @torch.inference_mode()
     def forward(self, cache, ids=None, embeddings=None, positions=None, logits=0):
         """One decoder forward of a chunk. Returns fp32 logits of the last `logits` positions.
@@ -102,9 +111,9 @@ class StreamingDecoder:
         """
         if embeddings is None:
             embeddings = self.text.get_input_embeddings()(ids.to(self.device))
-        past = cache.get_seq_length()
         n = embeddings.shape[1]
         if positions is None:
+            past = self._position(cache)
             positions = torch.arange(past, past + n, device=self.device)
         before, cache.as_replayed = getattr(cache, 'as_replayed', False), True
         try:
@@ -117,7 +126,7 @@ class StreamingDecoder:
         return self.model.lm_head(out.last_hidden_state[:, -int(logits):]).float()
 
     @torch.inference_mode()
-    def ingest(self, prefix_ids, frames, bits, cache=None, qa_reserve=256):
+    def ingest(self, prefix_ids, frames, bits, cache=None, qa_reserve=256, budget=None):
         """Prefix at 16 bits, then each frame embedding [1, T, hidden] at its width (src/streaming.py:168-187).
 
         With graphs=True the frames after the first run as replays of one captured HIP graph of the
@@ -129,22 +138,61 @@ class StreamingDecoder:
         data are those of one frame after the other; the GPU overlaps them. With pipeline > 1 every
         chunk's attention (eager or replayed) runs group_split_count() history splits, so replays
         still equal eager ingestion bit for bit; question and candidate forwards keep the default.
+
+        With a `budget` the history stays within that many tokens. The attention of the prefix and of every
+        frame is counted, and before a frame that would pass the budget the tokens of the least attention
+        mass are evicted (GPUCache.evict), down to three quarters of the budget or to what the frame needs;
+        the prefix and the last quarter of the budget stay. The cache that is returned holds the history: with
+        a budget it may be another one than the `cache` given.
         """
         if len(frames) != len(bits):
             raise ValueError('one bit width per frame')
-        total = prefix_ids.shape[1] + sum(f.shape[1] for f in frames) + qa_reserve
+        total = prefix_ids.shape[1] + sum(f.shape[1] for f in frames)
+        if budget is not None:
+            if budget < prefix_ids.shape[1]:
+                raise ValueError(f'a budget of {budget} tokens does not hold the prefix of {prefix_ids.shape[1]}')
+            total = min(total, budget)
+        total += qa_reserve
         if cache is None:
             cache = self._reused_cache(total) if self.graphs else self.create_cache(total)
         # pipelined frames share the GPU: their frame-chunk attention takes fewer history splits
-        cache.chunk_splits = (self.group_split_count(max(f.shape[1] for f in frames))
-                              if self.pipeline > 1 and frames else 0)
+        splits = self.group_split_count(max(f.shape[1] for f in frames)) if self.pipeline > 1 and frames else 0
+        if budget is not None:
+            cache.mass()  # (allocated before a capture records it)
+        caches = [cache]
         try:
-            self._ingest_chunks(cache, prefix_ids, frames, bits)
+            cache.chunk_splits, cache.observing = splits, budget is not None
+            return self._ingest_chunks(caches, prefix_ids, frames, bits, budget)
         finally:
-            cache.chunk_splits = 0
-        return cache
+            for c in caches:
+                c.chunk_splits, c.observing = 0, False
 
-    def _ingest_chunks(self, cache, prefix_ids, frames, bits):
+    def _evict_for(self, caches, budget, frame, prefix):
+        """Room for a frame within the budget: the last of `caches` evicts into the one before it (or a new
+        one), which goes to the end of the list and is returned."""
+        cache = caches[-1]
+        keep = min(budget - budget // 4, budget - frame)
+        own = self.graphs and cache is self._cache
+        into = caches[-2] if len(caches) > 1 else None
+        if own:
+            if self._spare is None or self._spare[0].capacity < cache.capacity:
+                self._spare = (self.create_cache(cache.capacity), {}, {}, {}, set())
+            into = self._spare[0]
+        new = cache.evict(keep, sinks=prefix, recent=budget // 4, into=into)
+        new.chunk_splits, new.observing = cache.chunk_splits, cache.observing
+        if own:  # captured forwards stay with the cache whose buffers they recorded
+            (self._cache, self._graphs, self._group_graphs, self._qa_graphs, self._qa_seen), self._spare = \
+                self._spare, (cache, self._graphs, self._group_graphs, self._qa_graphs, self._qa_seen)
+        caches[:] = [cache, new]
+        return new
+
+    @staticmethod
+    def _graph_key(cache, *key):
+        """Key of a captured forward: one that counts attention records other launches."""
+        return key + ('observing',) if cache.observing else key if len(key) > 1 else key[0]
+
+    def _ingest_chunks(self, caches, prefix_ids, frames, bits, budget):
+        cache = caches[-1]
         cache.select(16, -1)
         graphed = self.graphs and cache is self._cache
         # The first request's prefix and first frame run eagerly (they warm up the library paths
@@ -159,8 +207,13 @@ class StreamingDecoder:
         while i < len(frames):
             emb, b = frames[i], bits[i]
             replay = graphed and (i > 0 or warm)
+            n, most = emb.shape[1], self.pipeline
+            if budget is not None:
+                if cache.get_seq_length() + n > budget:
+                    cache = self._evict_for(caches, budget, n, prefix_ids.shape[1])
+                most = min(most, (budget - cache.get_seq_length()) // n)
             k = 1
-            while k < self.pipeline and i + k < len(frames) and frames[i + k].shape[1] == emb.shape[1]:
+            while k < most and i + k < len(frames) and frames[i + k].shape[1] == n:
                 k += 1
             if replay and k > 1:
                 self._graph_group(cache, frames[i:i + k], bits[i:i + k], i)
@@ -175,19 +228,21 @@ class StreamingDecoder:
         cache.select(16, -1)
         if len(set(cache.seen)) != 1:
             raise RuntimeError('Decoder layers disagree about the cache length')
+        return cache
 
     def _reused_cache(self, total):
         if self._cache is None or self._cache.capacity < total:
             self._cache = self.create_cache(max(total, 8192))
             # a captured graph records the old cache's buffers
             self._graphs, self._group_graphs, self._qa_graphs, self._qa_seen = {}, {}, {}, set()
+            self._spare = None
         else:
             self._cache.reset()
         return self._cache
 
     def _graph_chunk(self, cache, emb):
         """One chunk as a replay of the captured forward of its length (captured on first use)."""
-        fg = self._graphs.get(emb.shape[1])
+        fg = self._graphs.get(self._graph_key(cache, emb.shape[1]))
         if fg is None:
             self._capture_chunk(cache, emb)
             return
@@ -195,7 +250,7 @@ class StreamingDecoder:
         try:
             past = cache.graph_step()
             fg['emb'].copy_(emb)
-            torch.add(fg['arange'], past, out=fg['pos'][0])
+            torch.add(fg['arange'], self._position(cache, past), out=fg['pos'][0])
             fg['graph'].replay()
         finally:
             cache.end_graph_steps()
@@ -208,7 +263,7 @@ class StreamingDecoder:
         steps = cache.begin_graph_steps(chunk, q_heads=self.config.num_attention_heads)
         try:
             past = cache.graph_step()
-            torch.add(arange, past, out=pos[0])
+            torch.add(arange, self._position(cache, past), out=pos[0])
             torch.cuda.synchronize()
             graph = torch.cuda.CUDAGraph()
             with torch.cuda.graph(graph):
@@ -218,17 +273,17 @@ class StreamingDecoder:
             graph.replay()
         finally:
             cache.end_graph_steps()
-        self._graphs[chunk] = dict(chunk=chunk, graph=graph, steps=steps, emb=static_emb, pos=pos, arange=arange)
+        self._graphs[self._graph_key(cache, chunk)] = dict(chunk=chunk, graph=graph, steps=steps, emb=static_emb, pos=pos, arange=arange)
 
     def _group_steps(self, cache, chunk, bits, frame, steps):
         """Host bookkeeping of frames frame .. frame + k - 1 (one GraphSteps each, since their
-        forwards run at once); returns their history lengths and the GraphSteps."""
+        forwards run at once); returns their first positions and the GraphSteps."""
         past, out = [], []
         for j, st in enumerate(steps):
             cache.select(bits[j], frame + j)
             cache.begin_graph_steps(chunk, q_heads=None if st else self.config.num_attention_heads, steps=st)
             try:
-                past.append(cache.graph_step())
+                past.append(self._position(cache, cache.graph_step()))
             finally:
                 out.append(cache.end_graph_steps())
         return past, out
@@ -236,7 +291,7 @@ class StreamingDecoder:
     def _graph_group(self, cache, embs, bits, frame):
         """k consecutive frames as one replay of their pipelined forwards (captured on first use)."""
         chunk, k = embs[0].shape[1], len(embs)
-        fg = self._group_graphs.get((chunk, k))
+        fg = self._group_graphs.get(self._graph_key(cache, chunk, k))
         if fg is None:
             self._capture_group(cache, embs, bits, frame)
             return
@@ -291,7 +346,7 @@ class StreamingDecoder:
         for st in steps:
             st.upload()  # the jobs now carry the K/V addresses recorded in the graph
         graph.replay()
-        self._group_graphs[(chunk, k)] = dict(graph=graph, steps=steps, emb=static_emb, pos=pos, arange=arange,
+        self._group_graphs[self._graph_key(cache, chunk, k)] = dict(graph=graph, steps=steps, emb=static_emb, pos=pos, arange=arange,
                                               events=done, streams=streams)
 
     def _fork_forward(self, branch, ids, logits, lengths=None):
@@ -312,11 +367,13 @@ class StreamingDecoder:
         else:
             rel = torch.arange(chunk, device=self.device)
         key = (chunk, int(logits), tuple(lengths) if lengths else None)
+        if branch.sparse_blocks:  # (a captured forward records the index it reads, too)
+            key += (branch.sparse_blocks, id(branch._bounds))
         graphed = self.graphs and self._cache is not None and branch.arena is self._cache.arena
         if not graphed or key not in self._qa_seen:
             if graphed:
                 self._qa_seen.add(key)
-            past = branch.get_seq_length()
+            past = self._position(branch)
             branch.chunk_segments = segments
             try:
                 return self.forward(branch, embeddings=emb, positions=rel + past, logits=logits)
@@ -326,7 +383,7 @@ class StreamingDecoder:
         steps = fg['steps'] if fg else None
         branch.begin_graph_steps(chunk, q_heads=None if fg else self.config.num_attention_heads, steps=steps)
         try:
-            past = branch.graph_step()
+            past = self._position(branch, branch.graph_step())
             if fg is None:
                 static_emb, pos = emb.clone(), torch.empty((1, chunk), dtype=torch.long, device=self.device)
                 torch.add(rel, past, out=pos[0])
@@ -352,6 +409,25 @@ class StreamingDecoder:
     @staticmethod
     def _mean_loglik(logits, targets):
         return logits.log_softmax(-1).gather(1, targets[:, None]).mean()
+
+    @torch.inference_mode()
+    def generate(self, cache, question_ids, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, blocks=0):
+        """Continues the question on a fork: one token for each random number of u [n] (gpu_ops.sample: fp32
+        or fp64, on the decoder's device), int64 [n]. With `blocks` the question and every token attend to the
+        tiles of the history that score highest for them, that many each, and to all that came after the
+        question (GPUCache.attend_sparse; the cache's index is brought up to date first). Nothing waits for
+        the GPU, so a caller that stops at a token looks for it afterwards."""
+        if u.dim() != 1:
+            raise ValueError('generate expects one random number a token, u [n]')
+        if blocks:
+            cache.index()
+        branch, ids, tokens = cache.fork(), question_ids, []
+        branch.sparse_blocks = blocks
+        for i in range(u.shape[0]):
+            logits = self._fork_forward(branch, ids, 1)[0]
+            tokens.append(sample(logits, u[i:i + 1], temperature, top_k, top_p, min_p))
+            ids = tokens[-1][None]
+        return torch.cat(tokens) if tokens else u.new_empty(0, dtype=torch.int64)
 
     @torch.inference_mode()
     def answer(self, cache, question_ids, candidates):
