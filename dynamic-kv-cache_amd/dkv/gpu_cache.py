@@ -814,9 +814,9 @@ class GPUCache(_CacheBase):
         return self._own_mass()[:, :, :self.seen[0]]
 
     def _eviction(self, keep, sinks, recent):
-        """(first segment, one past the last, {width: tokens kept}) of an eviction: the segments between the
-        protected ends, and their `keep` less the ends' tokens shared among the widths they have, in
-        proportion to what each holds (largest remainders, the wider one first)."""
+        """(first segment, one past the last, {width: tokens kept}, {width: tokens held}) of an eviction: the
+        segments between the protected ends, and their `keep` less the ends' tokens shared among the widths
+        they have, in proportion to what each holds (largest remainders, the wider one first)."""
         n, segs = self.seen[0], self.segments
         a, b = 0, len(segs)
         while a < b and segs[a].start < sinks:
@@ -824,10 +824,17 @@ class GPUCache(_CacheBase):
         while b > a and segs[b - 1].end > n - recent:
             b -= 1
         if keep >= n:
-            return len(segs), len(segs), {}
-        held = {}
+            return len(segs), len(segs), {}, {}
+        count = dict(self.host_counts)  # less the ends': what the middle holds
+        for seg in segs[:a] + segs[b:]:
+            count[seg.bits] -= seg.rows
+        widths = []  # as they come
         for seg in segs[a:b]:
-            held[seg.bits] = held.get(seg.bits, 0) + seg.rows
+            if seg.bits not in widths:
+                widths.append(seg.bits)
+                if len(widths) == sum(m > 0 for m in count.values()):
+                    break
+        held = {w: count[w] for w in widths}
         total = sum(held.values())
         left = keep - (n - total)
         if left < 0:
@@ -835,7 +842,7 @@ class GPUCache(_CacheBase):
         share = {w: left * m // total for w, m in held.items()}
         for w in sorted(held, key=lambda w: (-(left * held[w] % total), -w))[:left - sum(share.values())]:
             share[w] += 1
-        return a, b, {w: m for w, m in share.items() if m}
+        return a, b, {w: m for w, m in share.items() if m}, held
 
     def evict(self, keep, sinks=0, recent=0, into=None):
         """The `keep` tokens of this cache that matter, as another cache: `into` (an online cache of the same
@@ -857,7 +864,7 @@ class GPUCache(_CacheBase):
             raise ValueError('evict: keep, sinks and recent must not be negative')
         if self._mass is None:
             raise ValueError('evict: no attention mass has been counted (observe(), observing or mass())')
-        a, b, share = self._eviction(keep, sinks, recent)
+        a, b, share, held = self._eviction(keep, sinks, recent)
         if into is None:
             into = GPUCache(None, self.layers, self.heads, self.dim, self.arena.device, self.dtype, self.backend,
                             self.block_m, self.block_n, self.capacity, precision=self.precision)
@@ -897,7 +904,7 @@ class GPUCache(_CacheBase):
             e.n_classes = len(share)
             for i, (w, m) in enumerate(share.items()):
                 e.class_bits[i], e.class_keep[i] = w, m
-                e.class_held[i] = sum(s.rows for s in self.segments[a:b] if s.bits == w)
+                e.class_held[i] = held[w]
             e.mass, e.mass_stride = self._mass.data_ptr(), self.capacity
             e.out_arena, e.out_arena_bytes = into.arena.data_ptr(), into.arena_bytes
             e.out_tiles, e.out_mass, e.out_mass_stride = into.tiles.data_ptr(), into._mass.data_ptr(), into.capacity

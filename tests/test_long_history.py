@@ -153,13 +153,14 @@ def test_shares_of_an_eviction():
     c = GPUCache(None, layers=1, heads=1, max_tokens=4096, device='cpu')
     c._open_segments(0, [40, 64, 64, 64, 64, 64, 10], [16, 4, 8, 4, 16, 4, 16])
     c.seen = [370]
-    assert c._eviction(200, 0, 0) == (0, 7, {16: 62, 4: 104, 8: 34})
-    assert c._eviction(200, 1, 1) == (1, 6, {4: 90, 8: 30, 16: 30})
-    assert c._eviction(201, 40, 10) == (1, 6, {4: 91, 8: 30, 16: 30})
-    assert c._eviction(202, 40, 10) == (1, 6, {4: 91, 8: 30, 16: 31})
-    assert c._eviction(200, 41, 11) == (2, 5, {8: 7, 4: 7, 16: 8})
-    assert c._eviction(50, 40, 10) == (1, 6, {})
-    assert c._eviction(370, 0, 0) == c._eviction(999, 5, 5) == (7, 7, {})
+    every, middle = {16: 114, 4: 192, 8: 64}, {4: 192, 8: 64, 16: 64}
+    assert c._eviction(200, 0, 0) == (0, 7, {16: 62, 4: 104, 8: 34}, every)
+    assert c._eviction(200, 1, 1) == (1, 6, {4: 90, 8: 30, 16: 30}, middle)
+    assert c._eviction(201, 40, 10) == (1, 6, {4: 91, 8: 30, 16: 30}, middle)
+    assert c._eviction(202, 40, 10) == (1, 6, {4: 91, 8: 30, 16: 31}, middle)
+    assert c._eviction(200, 41, 11) == (2, 5, {8: 7, 4: 7, 16: 8}, {8: 64, 4: 64, 16: 64})
+    assert c._eviction(50, 40, 10) == (1, 6, {}, middle)
+    assert c._eviction(370, 0, 0) == c._eviction(999, 5, 5) == (7, 7, {}, {})
     with pytest.raises(ValueError, match='protected'):
         c._eviction(49, 40, 10)
 
