@@ -213,6 +213,56 @@ __global__ __launch_bounds__(CHOOSERS) void choose_kernel(dkv_attn_args a, dkv_s
   Elements<CHOOSERS, N, decltype(key)>(v.n_indexed, key).largest(scratch, (uint32_t)v.chosen, [&](int to, int i) { lists[to] = i; });
 }
 
+// Scores and choice of a (query, KV head) in one workgroup, a wave 64 tiles: for up to NEAR_TILES indexed tiles. The sums
+// are score_kernel's, term by term.
+constexpr int NEAR_TILES = 512;
+__global__ __launch_bounds__(NEAR_TILES) void near_kernel(dkv_attn_args a, dkv_sparse s, int max_chosen, int32_t* lists) {
+  __shared__ SelectScratch<NEAR_TILES, 8> scratch;
+  __shared__ double query[2 * D];
+  const Seen v = seen_of(a, s);
+  if (v.chosen == v.n_indexed) return;
+  const int m = blockIdx.x, h = blockIdx.y, G = a.q_heads / a.heads, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int tile = threadIdx.x;
+  u32x4 w[BLOCK_PIECES];
+  if (64 * wave < v.n_indexed) {
+    const u32x4* from = static_cast<const u32x4*>(s.bounds) + piece_at(wave, a.layer, a.layers, h, a.heads) + lane;
+#pragma unroll
+    for (int p = 0; p < BLOCK_PIECES; ++p) w[p] = from[p * BLOCK];
+  }
+  if (threadIdx.x < D) {
+    constexpr int AHEAD = 8;  // query heads in flight
+    const uint16_t* q = static_cast<const uint16_t*>(a.q) + (int64_t)h * G * a.q_head_stride + m * a.q_tok_stride + lane;
+    double plus = 0, minus = 0;
+    for (int g0 = 0; g0 < G; g0 += AHEAD) {
+      float x[AHEAD];
+#pragma unroll
+      for (int g = 0; g < AHEAD; ++g) x[g] = bf16_lo(q[min(g0 + g, G - 1) * a.q_head_stride]);
+#pragma unroll
+      for (int g = 0; g < AHEAD; ++g)
+        if (g0 + g < G) plus += x[g] > 0.f ? x[g] : 0.f, minus += x[g] > 0.f ? 0.f : x[g];
+    }
+    query[lane] = minus, query[D + lane] = plus;
+  }
+  __syncthreads();
+  uint32_t mine = 0;
+  if (64 * wave < v.n_indexed) {
+    double part[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      part[k] = 0;
+#pragma unroll
+      for (int e = 0; e < 32; ++e) {
+        const uint32_t x = w[4 * k + e / 8][e % 8 / 2];
+        part[k] = __builtin_fma(query[32 * k + e], (double)(e & 1 ? bf16_hi(x) : bf16_lo(x)), part[k]);
+      }
+    }
+    if (tile < v.n_indexed) mine = max(order_key((float)(part[0] + part[1] + (part[2] + part[3]))), 1u);
+  }
+  lists += ((int64_t)h * a.nq + m) * max_chosen;
+  auto key = [&](int) { return mine; };  // (wave w's elements are the tiles from 64 w on)
+  Elements<NEAR_TILES, 1, decltype(key)>(v.n_indexed, key).largest(scratch, (uint32_t)v.chosen, [&](int to, int i) { lists[to] = i; });
+}
+
 // A wave's running softmax over its units for 16 query rows: row c's maximum (base 2), this lane's share of its sum, of
 // the packed rows' offsets in the output (precision 1), and the lane's 16 output elements.
 struct Running {
@@ -535,11 +585,15 @@ int dkv_attend_sparse(const dkv_attn_args* args, const dkv_sparse* sparse, void*
   float* part_o = reinterpret_cast<float*>(ws + p.part_o);
   float2* part_ml = reinterpret_cast<float2*>(ws + p.part_ml);
   if (p.max_chosen > 0 && (p.max_chosen < p.max_indexed || a.step)) {
-    hipLaunchKernelGGL(score_kernel, dim3((p.max_indexed + BLOCK - 1) / BLOCK, a.heads, (a.nq + SCORE_QUERIES - 1) / SCORE_QUERIES),
-                       dim3(256), 0, st, a, s, p.max_indexed, keys);
     const int n = p.max_indexed;
-    const auto choose = n <= 2 * CHOOSERS ? choose_kernel<2> : n <= 8 * CHOOSERS ? choose_kernel<8> : choose_kernel<0>;
-    hipLaunchKernelGGL(choose, dim3(a.nq, a.heads), dim3(CHOOSERS), 0, st, a, s, p.max_indexed, p.max_chosen, keys, lists);
+    if (n <= NEAR_TILES) {
+      hipLaunchKernelGGL(near_kernel, dim3(a.nq, a.heads), dim3(NEAR_TILES), 0, st, a, s, p.max_chosen, lists);
+    } else {
+      hipLaunchKernelGGL(score_kernel, dim3((n + BLOCK - 1) / BLOCK, a.heads, (a.nq + SCORE_QUERIES - 1) / SCORE_QUERIES), dim3(256), 0, st,
+                         a, s, n, keys);
+      const auto choose = n <= 8 * CHOOSERS ? choose_kernel<8> : choose_kernel<0>;
+      hipLaunchKernelGGL(choose, dim3(a.nq, a.heads), dim3(CHOOSERS), 0, st, a, s, n, p.max_chosen, keys, lists);
+    }
   }
   const dim3 grid(p.splits, a.heads * p.row_blocks, a.nq);
   const auto attend = a.precision == 1 ? (a.out_dtype == 1 ? attend_kernel<1, 3> : attend_kernel<1, 2>)

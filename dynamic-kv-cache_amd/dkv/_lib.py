@@ -62,7 +62,7 @@ class SegmentIO(ctypes.Structure):
 
 class Sparse(ctypes.Structure):
     _fields_ = [('bounds', ctypes.c_void_p), ('n_indexed', ctypes.c_int32), ('blocks', ctypes.c_int32),
-                ('single_rows', ctypes.c_int32)]
+                ('single_rows', ctypes.c_int32), ('reserved', ctypes.c_int32)]
 
 
 class EvictArgs(ctypes.Structure):
@@ -100,14 +100,14 @@ def _layout(structure):
     return out
 
 
-TILE, PACK_JOB, ATTN_ARGS = _layout(Tile), _layout(PackJob), _layout(AttnArgs)
+TILE, PACK_JOB, ATTN_ARGS, SPARSE = _layout(Tile), _layout(PackJob), _layout(AttnArgs), _layout(Sparse)
 
 _lib = None
 _zeroed_workspace = False
 
 # (name, restype, argtypes) of every symbol include/dkv.h declares. The argument blocks of the calls
-# that run once per layer (dkv_pack, dkv_attend) are declared as addresses: a Structure by reference
-# or the bytes PACK_JOB / ATTN_ARGS make in one call, a fifth of the time of setting a Structure's
+# that run once per layer (dkv_pack, dkv_attend and its like) are declared as addresses: a Structure by reference
+# or the bytes PACK_JOB / ATTN_ARGS / SPARSE make in one call, a fifth of the time of setting a Structure's
 # fields one by one.
 SIGNATURES = [
     ('dkv_version', ctypes.c_int, []),
@@ -175,8 +175,8 @@ SIGNATURES = [
     ('dkv_index_bytes', ctypes.c_int64, [ctypes.c_int32, ctypes.c_int32, ctypes.c_int32]),
     ('dkv_index', ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
                                  ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p]),
-    ('dkv_attend_sparse_workspace_bytes', ctypes.c_int64, [ctypes.c_void_p, ctypes.POINTER(Sparse)]),
-    ('dkv_attend_sparse', ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(Sparse), ctypes.c_void_p]),
+    ('dkv_attend_sparse_workspace_bytes', ctypes.c_int64, [ctypes.c_void_p, ctypes.c_void_p]),
+    ('dkv_attend_sparse', ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
     ('dkv_attention_mass_workspace_bytes', ctypes.c_int64, [ctypes.c_void_p]),
     ('dkv_attention_mass', ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32,
                                           ctypes.c_void_p]),

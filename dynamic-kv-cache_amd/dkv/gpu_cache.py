@@ -696,15 +696,15 @@ class GPUCache(_CacheBase):
         return x[0, :n], x[1, :n]
 
     def _chunk(self, what, q, k, layer, past, segments, precision, v=None):
-        """The checks that the calls over a chunk share; (q, k, v) as the kernels read them, segments and
-        precision as the call uses them."""
-        precision = self.precision if precision is None else precision
-        if precision not in PRECISIONS:
+        """The checks that the calls over a chunk share. Returns (segments, precision) as the call uses them."""
+        if precision is None:
+            precision = self.precision
+        elif precision not in PRECISIONS:
             raise ValueError(f'precision must be one of {sorted(PRECISIONS)}')
-        H, d = self.heads, self.dim
-        if q.dim() != 4 or q.shape[0] != 1 or q.shape[3] != d or q.shape[1] % H or not q.shape[1]:
+        H, d, shape = self.heads, self.dim, q.shape
+        if len(shape) != 4 or shape[0] != 1 or shape[3] != d or shape[1] % H or not shape[1]:
             raise ValueError(f'{what} expects q [1, q_heads, n, {d}] with q_heads a multiple of heads')
-        n = q.shape[2]
+        n = shape[2]
         if k.shape != (1, H, n, d) or (v is not None and v.shape != k.shape):
             raise ValueError(f'{what} expects the chunk of shape [1, {H}, {n}, {d}]')
         if not 0 <= layer < self.layers:
@@ -712,20 +712,41 @@ class GPUCache(_CacheBase):
         if past < 0 or past + n > self.capacity or past > self.seen[layer]:
             raise ValueError(f'{what}: history longer than the cache holds')
         index = self.arena.get_device()
-        if not self.arena.is_cuda or any(t is not None and t.get_device() != index for t in (q, k, v)):
+        if index < 0 or q.get_device() != index or k.get_device() != index or (v is not None and v.get_device() != index):
             raise ValueError(f'{what} requires CUDA tensors on the device of the cache')
         if segments is None:
             segments = self.chunk_segments
         if segments is not None and (segments[0] != 0 or segments[-1] != n):
             raise ValueError(f'chunk segments {segments} do not cover the {n}-token chunk')
-        return self._kv_view(q), self._kv_view(k), None if v is None else self._kv_view(v), segments, precision
+        return segments, precision
 
-    def _chunk_args(self, q, k, v, layer, past, out, segments, precision):
-        """attend_args() of a call over a chunk: of the recorded step in graph steps."""
-        make = self if self._graph is None else self._graph
-        if make is self:
-            return self.attend_args(q, k, v, layer, past, out, segments, 0, 0, precision)
-        return make.attend_args(q, k, v, layer, out, segments, 0, 0, precision)
+    def _chunk_args(self, q, k, v, layer, past, out, segments, precision, need):
+        """The argument block of a call over a chunk, with the workspace of need(block) bytes: bytes for an
+        ordinary call (attend_args() field by field), a Structure where there are segments or graph steps.
+        Returns it with what it points into."""
+        q, qp, qs = self._rows(q)
+        k, kp, ks = self._rows(k)
+        v, vp, vs = self._rows(v) if v is not None else (k, kp, ks)
+        if self._graph is None and not segments:
+            n_tiles = self._tiles_before(past)
+            os = out.stride() if out is not None else (0, 0, 0)
+            head = (qp, qs[1], qs[2], kp, ks[1], ks[2], vp, vs[1], vs[2], self.arena.data_ptr(), self.tiles.data_ptr(),
+                    n_tiles, past, layer, self.layers, self.heads, q.shape[1], q.shape[2], 0, *_ONE_SEGMENT,
+                    self.dim ** -0.5, 0 if out is None else out.data_ptr(), os[1], os[2],
+                    out is not None and out.dtype is torch.float32, 0, 0, PRECISIONS[precision])
+            nbytes = need(_lib.ATTN_ARGS.pack(*head, 0, 0, 0, 0))
+            ws = self.arena.new_empty(nbytes) if nbytes else None
+            return _lib.ATTN_ARGS.pack(*head, ws.data_ptr() if nbytes else 0, nbytes, 0, 0), (q, k, v, ws)
+        out = q if out is None else out  # (not written by a call that has none)
+        if self._graph is None:
+            a = self.attend_args(q, k, v, layer, past, out, segments, 0, 0, precision)
+        else:
+            a = self._graph.attend_args(q, k, v, layer, out, segments, 0, 0, precision)
+        nbytes, ws = need(ctypes.byref(a)), None
+        if nbytes:
+            ws = self.arena.new_empty(nbytes) if self._graph is None else self._graph.workspace(nbytes)
+            a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+        return ctypes.byref(a), (a, q, k, v, ws)
 
     def _single_rows(self, n_tiles):
         """How many of the first n_tiles' last tiles hold one 16-bit row each (generated tokens) and are not in
@@ -743,21 +764,18 @@ class GPUCache(_CacheBase):
             raise ValueError(f'attend_sparse: blocks must not be negative, got {blocks}')
         out_dtype = out_dtype or q.dtype
         _check_dtype(out_dtype, 'attend_sparse output dtype')
-        q, k, v, segments, precision = self._chunk('attend_sparse', q, k, layer, past, segments, precision, v)
-        n, q_heads = q.shape[2], q.shape[1]
-        out = q.new_empty((1, n, q_heads, self.dim), dtype=out_dtype)
+        segments, precision = self._chunk('attend_sparse', q, k, layer, past, segments, precision, v)
+        n = q.shape[2]
+        out = q.new_empty((1, n, q.shape[1], self.dim), dtype=out_dtype)
         if not n:
             return out
-        a = self._chunk_args(q, k, v, layer, past, out, segments, precision)
-        s = _lib.Sparse(0 if self._bounds is None else self._bounds.data_ptr(), self.n_indexed, blocks,
-                        0 if self._graph is not None else self._single_rows(a.n_tiles))
-        if self._graph is not None:
-            s.n_indexed = self._graph.indexed_bound()
-        need = _lib.load().dkv_attend_sparse_workspace_bytes(ctypes.byref(a), ctypes.byref(s))
-        if need:
-            ws = self._graph.workspace(need) if self._graph is not None else self.arena.new_empty(need)
-            a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
-        self._call('dkv_attend_sparse', ctypes.byref(a), ctypes.byref(s))
+        graph = self._graph
+        s = _lib.SPARSE.pack(0 if self._bounds is None else self._bounds.data_ptr(),
+                             self.n_indexed if graph is None else graph.indexed_bound(), blocks,
+                             self._single_rows(self._tiles_before(past)) if graph is None else 0, 0)
+        size = _lib.load().dkv_attend_sparse_workspace_bytes
+        a, keep = self._chunk_args(q, k, v, layer, past, out, segments, precision, lambda block: size(block, s))
+        self._call('dkv_attend_sparse', a, s)
         return out
 
     # -- attention mass and eviction by it (no reference counterpart) ----------
@@ -766,7 +784,7 @@ class GPUCache(_CacheBase):
         each KV head of the weights that attend() gives it, [heads, past + n] fp32 (history, then chunk)."""
         if self._graph is not None:
             raise ValueError('attention_mass() cannot run in graph steps, whose length is not the host\'s: observe()')
-        q, k, _, segments, precision = self._chunk('attention_mass', q, k, layer, past, segments, precision)
+        segments, precision = self._chunk('attention_mass', q, k, layer, past, segments, precision)
         n = q.shape[2]
         out = q.new_empty((self.heads, past + n), dtype=torch.float32)
         if not n:
@@ -777,7 +795,7 @@ class GPUCache(_CacheBase):
     def observe(self, q, k, layer, past, segments=None, precision=None):
         """Adds a chunk's attention mass to the cache's (mass()), which evict() goes by. With `observing` set
         every attend() does."""
-        q, k, _, segments, precision = self._chunk('observe', q, k, layer, past, segments, precision)
+        segments, precision = self._chunk('observe', q, k, layer, past, segments, precision)
         mass = self._own_mass()
         if self._graph is not None:
             self._graph.mass = mass
@@ -785,11 +803,9 @@ class GPUCache(_CacheBase):
             self._run_mass(q, k, layer, past, segments, precision, mass[layer].data_ptr(), self.capacity, 1)
 
     def _run_mass(self, q, k, layer, past, segments, precision, out, stride, accumulate):
-        a = self._chunk_args(q, k, k, layer, past, q, segments, precision)  # (no values and no output are read)
-        need = _lib.load().dkv_attention_mass_workspace_bytes(ctypes.byref(a))
-        ws = self._graph.workspace(need) if self._graph is not None else self.arena.new_empty(need)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
-        self._call('dkv_attention_mass', ctypes.byref(a), out, stride, accumulate)
+        a, keep = self._chunk_args(q, k, None, layer, past, None, segments, precision,
+                                   _lib.load().dkv_attention_mass_workspace_bytes)
+        self._call('dkv_attention_mass', a, out, stride, accumulate)
 
     def _own_mass(self):
         if self._mass is None or self._mass_shared:
@@ -1350,7 +1366,7 @@ class GraphSteps:
         lib, c = _lib.load(), self.cache
         need = lib.dkv_attend_workspace_bytes(ctypes.byref(a))
         if c.sparse_blocks:
-            s = _lib.Sparse(None, self.indexed_bound(), c.sparse_blocks, 0)
+            s = _lib.Sparse(None, self.indexed_bound(), c.sparse_blocks, 0, 0)
             need = max(need, lib.dkv_attend_sparse_workspace_bytes(ctypes.byref(a), ctypes.byref(s)))
         return max(need, lib.dkv_attention_mass_workspace_bytes(ctypes.byref(a))) if c.observing else need
 

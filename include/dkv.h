@@ -401,6 +401,7 @@ typedef struct dkv_sparse {
   int32_t blocks;     /* tiles that a query attends to of the indexed ones */
   int32_t single_rows; /* 0, or how many of the last tiles hold one 16-bit row each, in consecutive
                           slabs (generated tokens): they are attended to 64 at a time */
+  int32_t reserved;
 } dkv_sparse;
 
 /* dkv_attend over the `blocks` tiles of the index with the largest
