@@ -1,12 +1,12 @@
 // Attention mass (gfx950): what every token of the history and the chunk receives of the queries' softmax,
 //   mass(h, t) = sum over the query heads of h and the queries m of exp(s_mt - max_m) / sum_m,
-// the weight by which a cache forgets tokens. Two launches over the keys alone: the first gives every query row its
+// the weight by which a cache forgets tokens. Two passes over the keys alone: the first gives every query row its
 // maximum and sum over ranges of units (64 keys), the second joins them and sums each key's column over all rows. No
-// sum is shared between workgroups, so the result does not depend on their order; of long chunks the second launch's
-// workgroups take a part of the rows each, and a third adds the parts up.
+// sum is shared between workgroups, so the result does not depend on their order.
 //   - up to 64 query rows a KV head (generated tokens): a wave a unit, keys and queries in registers, nothing in LDS;
 //   - more: a workgroup a unit, whose waves unpack 16 keys each into MFMA operands in LDS and take the 16-row query
-//     blocks in turn.
+//     blocks in turn. The rows are joined in a launch between the passes, and where a chunk is long the second pass's
+//     workgroups take a part of the rows each and one more launch adds the parts up.
 #include "dkv_rows.h"
 
 namespace dkv {
@@ -21,6 +21,7 @@ constexpr int BLOCKS = GROUP / 64;  // 16-row blocks of a wave
 struct MassArgs {
   int splits, row_groups, row_parts;
   float2* part;      // [heads][splits][rows] maximum (base 2) and sum
+  float2* norm;      // [heads][rows] reference and 1 / sum (many rows)
   float* columns;    // [row_parts][heads][stride] sums of a part of the rows (row_parts > 1)
   int64_t columns_stride;
   float* out;        // [heads] rows of out_stride
@@ -95,7 +96,7 @@ __device__ __forceinline__ void add_weights(const f32x4 (&s)[4], float scale2, f
     }
 }
 
-// Maximum and sum of a row over the splits, as its reference and 1 / sum.
+// A row's reference and sum with those of the splits [from, to).
 constexpr int AHEAD = 16;  // loads in flight
 __device__ __forceinline__ void join(const float2* part, int from, int to, int64_t stride, float& m, float& l) {
   for (int s0 = from; s0 < to; s0 += AHEAD) {
@@ -393,43 +394,72 @@ __global__ __launch_bounds__(256) void stats_kernel(dkv_attn_args a, MassArgs p)
   }
 }
 
-template <int PREC>
+__global__ __launch_bounds__(256) void norm_kernel(dkv_attn_args a, MassArgs p) {
+  const int rows = a.q_heads / a.heads * a.nq, row = blockIdx.x * 256 + threadIdx.x, h = blockIdx.y;
+  if (row >= rows) return;
+  const int splits = split_count(p.splits, history_of(a).units, false);
+  float m = -INFINITY, l = 0.f;
+  join(p.part + (int64_t)h * splits * rows + row, 0, splits, rows, m, l);
+  p.norm[(int64_t)h * rows + row] = make_float2(m, 1.f / l);
+}
+
+// A wave's 16-row blocks come one after the other without a barrier, the next one's queries loading meanwhile.
+struct QueryBlock {
+  Op q[2];
+  float2 norm;
+};
+__device__ __forceinline__ QueryBlock load_query_block(const dkv_attn_args& a, const float2* norm, int h, int block, int rows, int c, int g) {
+  QueryBlock x;
+  const int row = 16 * block + c;
+  query_row(a, h, row, rows, g, x.q);
+  x.norm = norm[min(row, rows - 1)];
+  if (row >= rows) x.norm = make_float2(0.f, 0.f);
+  return x;
+}
+
+// JOIN: at most a row group, whose rows every workgroup joins itself (a launch less: a frame over 8128 22.2 us against
+// 24.5).
+template <int PREC, bool JOIN>
 __global__ __launch_bounds__(256) void columns_kernel(dkv_attn_args a, MassArgs p) {
   __shared__ Keys keys;
-  __shared__ float2 norm[GROUP];  // reference and 1 / sum of the row group's rows
   __shared__ float column[4][TILE];
+  __shared__ float2 joined[JOIN ? GROUP : 1];
   const History v = history_of(a);
   const int unit = blockIdx.x, h = blockIdx.y;
   if (unit >= v.units) return;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
-  const int rows = a.q_heads / a.heads * a.nq, splits = split_count(p.splits, v.units, false);
+  const int rows = a.q_heads / a.heads * a.nq, blocks = (rows + 15) / 16;
+  const int from = (int)((int64_t)blocks * blockIdx.z / p.row_parts), to = (int)((int64_t)blocks * (blockIdx.z + 1) / p.row_parts);
   const float scale2 = a.scale * LOG2E;
   Unit64 x = unit_of(a, v, unit, h);
   x.u.bits = __builtin_amdgcn_readfirstlane(x.u.bits);
   KeyPiece piece;
   load_block<PREC>(x.u, wave, lane, piece);
+  if (JOIN && (int)threadIdx.x < rows) {
+    const int splits = split_count(p.splits, v.units, false);
+    float m = -INFINITY, l = 0.f;
+    join(p.part + (int64_t)h * splits * rows + threadIdx.x, 0, splits, rows, m, l);
+    joined[threadIdx.x % GROUP] = make_float2(m, 1.f / l);
+  }
   stage_block<PREC>(x.u, piece, wave, lane, keys);
+  __syncthreads();
+  const float2* norm = JOIN ? joined : p.norm + (int64_t)h * rows;
+  int block = from + wave;
+  QueryBlock now = load_query_block(a, norm, h, min(block, blocks - 1), rows, c, g);
   float total[4][4] = {};
-  for (int group = blockIdx.z; group < p.row_groups; group += p.row_parts) {
-    __syncthreads();
-    if (const int row = group * GROUP + (int)threadIdx.x; threadIdx.x < GROUP) {
-      float m = -INFINITY, l = 0.f;
-      if (row < rows) join(p.part + (int64_t)h * splits * rows + row, 0, splits, rows, m, l);
-      norm[threadIdx.x] = row < rows ? make_float2(m, 1.f / l) : make_float2(0.f, 0.f);
-    }
-    Op q[BLOCKS][2];
-#pragma unroll
-    for (int k = 0; k < BLOCKS; ++k) query_row(a, h, group * GROUP + (4 * k + wave) * 16 + c, rows, g, q[k]);
-    __syncthreads();
-    float sum[4][4] = {};  // this group's share, so that long sums are sums of short ones
-#pragma unroll
-    for (int k = 0; k < BLOCKS; ++k) {
-      const int i = (4 * k + wave) * 16 + c, m = (group * GROUP + i) % a.nq, start = chunk_seg_start(a, m);
-      if (group * GROUP + (4 * k + wave) * 16 >= rows || !sees(x, m, start)) continue;
-      f32x4 s[4];
-      block_scores<PREC>(keys, x.u.bits, q[k], PREC == 1 ? query_sum(q[k]) : 0.f, lane, s);
-      mask_scores(x, m, start, g, s);
-      add_weights(s, scale2, norm[i], x.first >= 0, sum);
+  constexpr int SHORT = 8;  // blocks whose sums are added up before they join the total, so that long sums are sums of short ones
+  while (block < to) {
+    float sum[4][4] = {};
+    for (int i = 0; i < SHORT && block < to; ++i, block += 4) {
+      const QueryBlock next = load_query_block(a, norm, h, min(block + 4, blocks - 1), rows, c, g);
+      const int m = (16 * block + c) % a.nq, start = chunk_seg_start(a, m);
+      if (sees(x, m, start)) {
+        f32x4 s[4];
+        block_scores<PREC>(keys, x.u.bits, now.q, PREC == 1 ? query_sum(now.q) : 0.f, lane, s);
+        mask_scores(x, m, start, g, s);
+        add_weights(s, scale2, now.norm, x.first >= 0, sum);
+      }
+      now = next;
     }
 #pragma unroll
     for (int b = 0; b < 4; ++b)
@@ -469,7 +499,7 @@ constexpr int MAX_ROW_PARTS = 8;
 
 struct MassPlan {
   MassArgs p;
-  int64_t part_bytes, bytes;
+  int64_t part_bytes, norm_bytes, bytes;
 };
 
 static MassPlan plan_of(const dkv_attn_args& a) {
@@ -487,7 +517,8 @@ static MassPlan plan_of(const dkv_attn_args& a) {
   if (m.p.row_parts < 1) m.p.row_parts = 1;
   m.p.columns_stride = ((int64_t)a.past + a.nq + 63) & ~63;
   m.part_bytes = ((int64_t)a.heads * m.p.splits * rows * sizeof(float2) + 255) & ~(int64_t)255;
-  m.bytes = m.part_bytes + (m.p.row_parts > 1 ? m.p.row_parts * a.heads * m.p.columns_stride * 4 : 0);
+  m.norm_bytes = few ? 0 : ((int64_t)a.heads * rows * sizeof(float2) + 255) & ~(int64_t)255;
+  m.bytes = m.part_bytes + m.norm_bytes + (m.p.row_parts > 1 ? m.p.row_parts * a.heads * m.p.columns_stride * 4 : 0);
   return m;
 }
 
@@ -531,7 +562,8 @@ int dkv_attention_mass(const dkv_attn_args* args, float* mass, int64_t mass_head
     return DKV_EINVAL;
   }
   p.part = static_cast<float2*>(a.workspace);
-  p.columns = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + plan.part_bytes);
+  p.norm = reinterpret_cast<float2*>(static_cast<char*>(a.workspace) + plan.part_bytes);
+  p.columns = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + plan.part_bytes + plan.norm_bytes);
   p.out = mass, p.out_stride = mass_head_stride, p.accumulate = accumulate;
   const hipStream_t st = (hipStream_t)stream;
   const int units = a.n_tiles + (a.nq + TILE - 1) / TILE;
@@ -546,8 +578,11 @@ int dkv_attention_mass(const dkv_attn_args* args, float* mass, int64_t mass_head
     return (int)hipGetLastError();
   }
   const auto stats = a.precision == 1 ? stats_kernel<1> : stats_kernel<0>;
-  const auto columns = a.precision == 1 ? columns_kernel<1> : columns_kernel<0>;
+  const bool joins = p.row_groups == 1;
+  const auto columns = a.precision == 1 ? (joins ? columns_kernel<1, true> : columns_kernel<1, false>)
+                                        : (joins ? columns_kernel<0, true> : columns_kernel<0, false>);
   hipLaunchKernelGGL(stats, dim3(p.splits, a.heads, p.row_groups), dim3(256), 0, st, a, p);
+  if (!joins) hipLaunchKernelGGL(norm_kernel, dim3((unsigned)((rows + 255) / 256), a.heads), dim3(256), 0, st, a, p);
   hipLaunchKernelGGL(columns, dim3(units, a.heads, p.row_parts), dim3(256), 0, st, a, p);
   if (p.row_parts > 1)
     hipLaunchKernelGGL(add_parts_kernel, dim3((a.past + a.nq + 255) / 256, a.heads), dim3(256), 0, st, a, p);

@@ -904,31 +904,26 @@ __global__ __launch_bounds__(THREADS) void draw_kernel(Args a, Work work) {
   const int part = __ffsll((unsigned long long)__ballot(parts_upto > target)) - 1;
   target -= shfl64(parts_upto, part) - s.part_mass[part];
 
-  // the part, in order: each wave a consecutive run, a lane a token
-  const int from = part * a.part_len, to = min(a.vocab, from + a.part_len);
-  const int run = ((to - from + THREADS / 64 - 1) / (THREADS / 64) + 63) & ~63, begin = min(to, from + wave * run), end = min(to, begin + run);
+  // the part, in order: a consecutive run of tokens a thread
+  const int from = part * a.part_len, to = min(a.vocab, from + a.part_len), run = (to - from + THREADS - 1) / THREADS;
+  const int begin = min(to, from + (int)threadIdx.x * run), end = min(to, begin + run);
   auto kept = [&](int i, float x) -> uint64_t {
     const uint32_t key = order_key(x);
     return cut.takes(key, i) ? weigher.weight(x) : 0;
   };
   uint64_t sum = 0, all;
-  r.template each<8, 64>(begin + lane, end, [&](int i, float x) { sum += kept(i, x); });
-  const uint64_t wave_upto = shfl64(wave_scan(sum), 63);
-  uint64_t before = block_scan<THREADS / 64>(s.bins.sums, lane == 0 ? wave_upto : 0, all);
-  before = shfl64(before, 63) - wave_upto;
+  r.template each<8, 1>(begin, end, [&](int i, float x) { sum += kept(i, x); });
+  uint64_t passed = block_scan<THREADS / 64>(s.bins.sums, sum, all);
   // (bins' sums were rounded down once, tokens' one by one: their total may be a few units short)
   if (target >= all) target = all - 1;
-  if (target < before || target >= before + wave_upto) return;
-  for (int i0 = begin; i0 < end; i0 += 64) {
-    const int i = i0 + lane;
-    const uint64_t passed = before + wave_scan(i < end ? kept(i, r.at(i)) : 0);
-    const uint64_t over = __ballot(passed > target);
-    if (over) {
-      if (lane == 0) *out = i0 + __ffsll((unsigned long long)over) - 1;
-      return;
-    }
-    before = shfl64(passed, 63);
-  }
+  if (target >= passed || target < passed - sum) return;
+  passed -= sum;
+  int token = -1;
+  r.template each<8, 1>(begin, end, [&](int i, float x) {
+    passed += kept(i, x);
+    if (token < 0 && passed > target) token = i;
+  });
+  *out = token;
 }
 
 static int parts_of(int rows, int vocab) {
