@@ -84,9 +84,10 @@ __device__ __forceinline__ void add_scores(const f32x4 (&s)[4], float scale2, fl
   top = m, sum = l;
 }
 
-// Adds 16 keys' weights of a row (norm: reference and 1 / sum). A masked key gets nothing, also of a row whose sum is not
-// a number.
+// Adds 16 keys' weights of a row (norm: reference and 1 / sum, 0 for a row that only fills a block up, whose score with an
+// infinite key is not a number). A masked key gets nothing, also of a row whose sum is not a number.
 __device__ __forceinline__ void add_weights(const f32x4 (&s)[4], float scale2, float2 norm, bool chunk, float (&sum)[4][4]) {
+  if (norm.y == 0.f) return;
 #pragma unroll
   for (int b = 0; b < 4; ++b)
 #pragma unroll

@@ -135,7 +135,6 @@ struct Elements {
       }
     }
   }
-  static __host__ __device__ bool holds(int n) { return (n + THREADS / 64 - 1) / (THREADS / 64) <= 64 * N; }
   // f(i, key) for all lanes together, key 0 past the end
   template <class F>
   __device__ __forceinline__ void each(F f) const {

@@ -121,13 +121,13 @@ __device__ __forceinline__ Seen seen_of(const dkv_attn_args& a, const dkv_sparse
 
 struct SparsePlan {
   int row_blocks;          // 16-row blocks of a KV head's query heads
-  int most, splits;        // workgroups of a (query, KV head, row block): the cap, and those launched
+  int splits;              // workgroups of a (query, KV head, row block): as many as any history within the bounds takes
   int max_indexed, max_chosen;  // launch bounds
   int64_t keys, lists, part_o, part_ml, bytes;  // workspace offsets
 };
 
-// Workgroups of a (query, KV head, row block): a unit a wave while the `most` of the launch give room. Replays apply it
-// to the history they find, so they split it as a call over that history does (their launch may hold more).
+// Workgroups of a (query, KV head, row block): a unit a wave while `most` workgroups give room. Replays apply it to the
+// history they find, with the launched workgroups as `most`, so they split it as a call over that history does.
 __host__ __device__ inline int split_count(int most, int64_t units) {
   const int64_t want = (units + 3) / 4;
   return want < 1 ? 1 : want < most ? (int)want : most;
@@ -470,10 +470,10 @@ static SparsePlan plan_of(const dkv_attn_args& a, const dkv_sparse& s) {
   p.max_chosen = s.blocks < p.max_indexed ? s.blocks : p.max_indexed;
   const int64_t pairs = (int64_t)a.heads * a.nq;
   const int tail = a.n_tiles - p.max_indexed, single = a.step ? 0 : s.single_rows < tail ? s.single_rows : tail;
-  const int64_t units = (int64_t)p.max_chosen + tail - single + (single + TILE - 1) / TILE + (a.nq + TILE - 1) / TILE;
+  int64_t units = (int64_t)p.max_chosen + tail - single + (single + TILE - 1) / TILE + (a.nq + TILE - 1) / TILE;
+  if (a.step) units = (int64_t)a.n_tiles + (a.nq + TILE - 1) / TILE;  // a replay may find none of the tiles indexed
   const int64_t most = WORKGROUPS / (pairs * p.row_blocks);
-  p.most = most < 1 ? 1 : (int)most;
-  p.splits = split_count(p.most, units);
+  p.splits = split_count(most < 1 ? 1 : (int)most, units);
   auto up = [](int64_t x) { return (x + 255) & ~(int64_t)255; };
   const int64_t choosing = p.max_chosen < p.max_indexed || a.step;
   p.keys = 0;
@@ -598,9 +598,9 @@ int dkv_attend_sparse(const dkv_attn_args* args, const dkv_sparse* sparse, void*
   const dim3 grid(p.splits, a.heads * p.row_blocks, a.nq);
   const auto attend = a.precision == 1 ? (a.out_dtype == 1 ? attend_kernel<1, 3> : attend_kernel<1, 2>)
                                        : (a.out_dtype == 1 ? attend_kernel<0, 3> : attend_kernel<0, 2>);
-  hipLaunchKernelGGL(attend, grid, dim3(256), 0, st, a, s, p.row_blocks, p.most, p.max_chosen, lists, part_o, part_ml);
+  hipLaunchKernelGGL(attend, grid, dim3(256), 0, st, a, s, p.row_blocks, p.splits, p.max_chosen, lists, part_o, part_ml);
   if (p.splits > 1)
-    hipLaunchKernelGGL(merge_kernel, dim3((a.q_heads / a.heads + 15) / 16, a.heads, a.nq), dim3(256), 0, st, a, s, p.most,
+    hipLaunchKernelGGL(merge_kernel, dim3((a.q_heads / a.heads + 15) / 16, a.heads, a.nq), dim3(256), 0, st, a, s, p.splits,
                        part_o, part_ml);
   return (int)hipGetLastError();
 }
