@@ -29,6 +29,9 @@ struct MassArgs {
   int accumulate;
 };
 
+// Uniform to the compiler too: what a wave loops over stays in scalar registers, tiles come by scalar loads.
+__device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }
+
 struct History {
   int past, n_tiles, units;
 };
@@ -57,9 +60,10 @@ __device__ __forceinline__ Unit64 unit_of(const dkv_attn_args& a, const History&
 }
 
 // A row's scores are masked where the unit's key is not visible: keys [low, high) are. Row m's segment starts at `start`.
-__device__ __forceinline__ void mask_scores(const Unit64& x, int m, int start, int g, f32x4 (&s)[4]) {
+// Returns whether any is.
+__device__ __forceinline__ bool mask_scores(const Unit64& x, int m, int start, int g, f32x4 (&s)[4]) {
   const int low = x.first < 0 ? 0 : start - x.first, high = x.first < 0 ? x.u.high : min(x.u.high, m + 1 - x.first);
-  if (__all(low <= 0 && high >= TILE)) return;
+  if (__all(low <= 0 && high >= TILE)) return false;
 #pragma unroll
   for (int b = 0; b < 4; ++b)
 #pragma unroll
@@ -67,6 +71,7 @@ __device__ __forceinline__ void mask_scores(const Unit64& x, int m, int start, i
       const int row = 16 * b + 4 * g + i;
       if (row < low || row >= high) s[b][i] = -INFINITY;
     }
+  return true;
 }
 
 // A row's maximum (raw) and sum with 16 scores more. The sum is of exp2(s * scale2 - reference), the reference being the
@@ -84,16 +89,17 @@ __device__ __forceinline__ void add_scores(const f32x4 (&s)[4], float scale2, fl
   top = m, sum = l;
 }
 
-// Adds 16 keys' weights of a row (norm: reference and 1 / sum, 0 for a row that only fills a block up, whose score with an
-// infinite key is not a number). A masked key gets nothing, also of a row whose sum is not a number.
-__device__ __forceinline__ void add_weights(const f32x4 (&s)[4], float scale2, float2 norm, bool chunk, float (&sum)[4][4]) {
+// Adds 16 keys' weights of a row (norm: reference and 1 / sum, 0 for a row that only fills a block up). A masked key gets nothing, also of a row whose sum is not a number.
+template <bool MASKED>
+__device__ __forceinline__ void add_weights(const f32x4 (&s)[4], float scale2, float2 norm, float (&sum)[4][4]) {
   if (norm.y == 0.f) return;
 #pragma unroll
   for (int b = 0; b < 4; ++b)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], scale2, -norm.x));
-      if (!chunk || s[b][i] != -INFINITY) sum[b][i] = __builtin_fmaf(p, norm.y, sum[b][i]);
+      const float x = __builtin_fmaf(p, norm.y, sum[b][i]);
+      sum[b][i] = MASKED && s[b][i] == -INFINITY ? sum[b][i] : x;
     }
 }
 
@@ -115,10 +121,26 @@ __device__ __forceinline__ void join(const float2* part, int from, int to, int64
   }
 }
 
-// Query row `row` (query head by query head, q_heads / heads * nq of a KV head).
-__device__ __forceinline__ void query_row(const dkv_attn_args& a, int h, int row, int rows, int g, Op (&q)[2]) {
-  const int r = min(row, rows - 1), G = a.q_heads / a.heads;
-  query_ops(static_cast<const uint16_t*>(a.q) + (h * G + r / a.nq) * a.q_head_stride + r % a.nq * a.q_tok_stride, row < rows, g, q);
+// A KV head's query rows lie query head by query head. The quotient of a row is below q_heads / heads <= 2^20, its product
+// with the rounded 1 / nq off by less than one; put right after (an integer division a lane and block took a quarter of
+// the second pass).
+struct RowAt {
+  int head, m;
+};
+__device__ __forceinline__ RowAt row_at(int row, int nq) {
+  RowAt r;
+  r.head = (int)((float)row * __builtin_amdgcn_rcpf((float)nq));
+  r.m = (int)((uint32_t)row - (uint32_t)r.head * (uint32_t)nq);
+  if (r.m < 0) --r.head, r.m += nq;
+  if (r.m >= nq) ++r.head, r.m -= nq;
+  return r;
+}
+
+// Query row `row`, the last one behind it (whose results are not used). Returns its query.
+__device__ __forceinline__ int query_row(const dkv_attn_args& a, int h, int row, int rows, int g, Op (&q)[2]) {
+  const RowAt r = row_at(min(row, rows - 1), a.nq);
+  query_ops(static_cast<const uint16_t*>(a.q) + (h * (a.q_heads / a.heads) + r.head) * a.q_head_stride + r.m * a.q_tok_stride, true, g, q);
+  return r.m;
 }
 
 // 16 sums a lane, [b][i] of key 16 b + 4 g + i, over the 16 lanes of a group: each lane ends with one key's, which it
@@ -183,12 +205,12 @@ struct FewRows {
   __device__ __forceinline__ void load(const dkv_attn_args& a, int h, int rows, int c, int g) {
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
-      query_row(a, h, 16 * n + c, rows, g, q[n]);
+      at[n] = query_row(a, h, 16 * n + c, rows, g, q[n]);
       q_sum[n] = PREC == 1 ? query_sum(q[n]) : 0.f;
-      at[n] = (16 * n + c) % a.nq, start[n] = chunk_seg_start(a, at[n]);
+      start[n] = chunk_seg_start(a, at[n]);
     }
   }
-  // use(block, scores) of this wave's units unit, unit + step, ...: the next one's keys load meanwhile
+  // use(unit, the unit, scores) of this wave's units unit, unit + step, ...: the next one's keys load meanwhile
   template <class Use>
   __device__ __forceinline__ void each(const dkv_attn_args& a, const History& v, int h, int unit, int step, int c, int g, Use use) {
     if (unit >= v.units) return;
@@ -224,7 +246,7 @@ __global__ __launch_bounds__(256) void few_stats_kernel(dkv_attn_args a, MassArg
   const History v = history_of(a);
   const int splits = split_count(p.splits, v.units, true);
   if ((int)blockIdx.x >= splits) return;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, h = blockIdx.y;
+  const int wave = wave_index(), lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, h = blockIdx.y;
   const int rows = a.q_heads / a.heads * a.nq;
   FewRows<PREC, NB> few;
   few.load(a, h, rows, c, g);
@@ -288,7 +310,7 @@ __global__ __launch_bounds__(256) void few_columns_kernel(dkv_attn_args a, MassA
   few.each(a, v, h, 4 * blockIdx.x + wave, 4 * gridDim.x, c, g, [&](int unit, const Unit64& x, const f32x4 (&s)[NB][4]) {
     float sum[4][4] = {};
 #pragma unroll
-    for (int n = 0; n < NB; ++n) add_weights(s[n], scale2, nm[n], x.first >= 0, sum);
+    for (int n = 0; n < NB; ++n) add_weights<true>(s[n], scale2, nm[n], sum);
     int key;
     const float w = column_sum(sum, c, g, key);
     if (key >= x.u.high) return;
@@ -343,12 +365,12 @@ __device__ __forceinline__ bool sees(const Unit64& x, int m, int start) {
 }
 
 template <int PREC>
-__global__ __launch_bounds__(256) void stats_kernel(dkv_attn_args a, MassArgs p) {
+__global__ __launch_bounds__(256, PREC ? 2 : 4) void stats_kernel(dkv_attn_args a, MassArgs p) {
   __shared__ Keys keys;
   const History v = history_of(a);
   const int splits = split_count(p.splits, v.units, false);
   if ((int)blockIdx.x >= splits) return;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, h = blockIdx.y;
+  const int wave = wave_index(), lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, h = blockIdx.y;
   const int rows = a.q_heads / a.heads * a.nq;
   Op q[BLOCKS][2];
   float top[BLOCKS], sum[BLOCKS], q_sum[BLOCKS];
@@ -356,13 +378,17 @@ __global__ __launch_bounds__(256) void stats_kernel(dkv_attn_args a, MassArgs p)
 #pragma unroll
   for (int k = 0; k < BLOCKS; ++k) {
     const int row = blockIdx.z * GROUP + (4 * k + wave) * 16 + c;
-    query_row(a, h, row, rows, g, q[k]);
+    at[k] = query_row(a, h, row, rows, g, q[k]);
     q_sum[k] = PREC == 1 ? query_sum(q[k]) : 0.f;
-    at[k] = row % a.nq, start[k] = chunk_seg_start(a, row % a.nq);
+    start[k] = chunk_seg_start(a, at[k]);
     top[k] = -INFINITY, sum[k] = 0.f;
   }
   const float scale2 = a.scale * LOG2E;
-  const int from = (int)((int64_t)v.units * blockIdx.x / splits), to = (int)((int64_t)v.units * (blockIdx.x + 1) / splits);
+  // the units that the row group sees: up to its last query's
+  const int first_row = blockIdx.z * GROUP, last_row = min(rows, first_row + GROUP) - 1;
+  const RowAt r0 = row_at(first_row, a.nq), r1 = row_at(last_row, a.nq);
+  const int last = r0.head == r1.head ? r1.m : a.nq - 1, units = v.n_tiles + last / TILE + 1;
+  const int from = (int)((int64_t)units * blockIdx.x / splits), to = (int)((int64_t)units * (blockIdx.x + 1) / splits);
   Unit64 x = unit_of(a, v, from, h);
   x.u.bits = __builtin_amdgcn_readfirstlane(x.u.bits);
   KeyPiece piece;
@@ -408,11 +434,12 @@ __global__ __launch_bounds__(256) void norm_kernel(dkv_attn_args a, MassArgs p) 
 struct QueryBlock {
   Op q[2];
   float2 norm;
+  int m;
 };
 __device__ __forceinline__ QueryBlock load_query_block(const dkv_attn_args& a, const float2* norm, int h, int block, int rows, int c, int g) {
   QueryBlock x;
   const int row = 16 * block + c;
-  query_row(a, h, row, rows, g, x.q);
+  x.m = query_row(a, h, row, rows, g, x.q);
   x.norm = norm[min(row, rows - 1)];
   if (row >= rows) x.norm = make_float2(0.f, 0.f);
   return x;
@@ -421,14 +448,14 @@ __device__ __forceinline__ QueryBlock load_query_block(const dkv_attn_args& a, c
 // JOIN: at most a row group, whose rows every workgroup joins itself (a launch less: a frame over 8128 22.2 us against
 // 24.5).
 template <int PREC, bool JOIN>
-__global__ __launch_bounds__(256) void columns_kernel(dkv_attn_args a, MassArgs p) {
+__global__ __launch_bounds__(256, PREC ? 2 : 4) void columns_kernel(dkv_attn_args a, MassArgs p) {
   __shared__ Keys keys;
   __shared__ float column[4][TILE];
   __shared__ float2 joined[JOIN ? GROUP : 1];
   const History v = history_of(a);
   const int unit = blockIdx.x, h = blockIdx.y;
   if (unit >= v.units) return;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+  const int wave = wave_index(), lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
   const int rows = a.q_heads / a.heads * a.nq, blocks = (rows + 15) / 16;
   const int from = (int)((int64_t)blocks * blockIdx.z / p.row_parts), to = (int)((int64_t)blocks * (blockIdx.z + 1) / p.row_parts);
   const float scale2 = a.scale * LOG2E;
@@ -445,22 +472,29 @@ __global__ __launch_bounds__(256) void columns_kernel(dkv_attn_args a, MassArgs 
   stage_block<PREC>(x.u, piece, wave, lane, keys);
   __syncthreads();
   const float2* norm = JOIN ? joined : p.norm + (int64_t)h * rows;
-  int block = from + wave;
+  // the next block from `b` on of which a row may see the unit: queries come one after the other within a query head
+  auto seeing = [&](int b) {
+    for (; b < to; b += 4)
+      if (const int m = row_at(16 * b, a.nq).m + 15; m >= x.first || m >= a.nq) break;
+    return b;
+  };
+  int block = seeing(from + wave);
   QueryBlock now = load_query_block(a, norm, h, min(block, blocks - 1), rows, c, g);
   float total[4][4] = {};
   constexpr int SHORT = 8;  // blocks whose sums are added up before they join the total, so that long sums are sums of short ones
   while (block < to) {
     float sum[4][4] = {};
-    for (int i = 0; i < SHORT && block < to; ++i, block += 4) {
-      const QueryBlock next = load_query_block(a, norm, h, min(block + 4, blocks - 1), rows, c, g);
-      const int m = (16 * block + c) % a.nq, start = chunk_seg_start(a, m);
-      if (sees(x, m, start)) {
+    for (int i = 0; i < SHORT && block < to; ++i) {
+      const int after = seeing(block + 4);
+      const QueryBlock next = load_query_block(a, norm, h, min(after, blocks - 1), rows, c, g);
+      const int start = chunk_seg_start(a, now.m);
+      if (sees(x, now.m, start)) {
         f32x4 s[4];
         block_scores<PREC>(keys, x.u.bits, now.q, PREC == 1 ? query_sum(now.q) : 0.f, lane, s);
-        mask_scores(x, m, start, g, s);
-        add_weights(s, scale2, now.norm, x.first >= 0, sum);
+        if (mask_scores(x, now.m, start, g, s)) add_weights<true>(s, scale2, now.norm, sum);
+        else add_weights<false>(s, scale2, now.norm, sum);
       }
-      now = next;
+      now = next, block = after;
     }
 #pragma unroll
     for (int b = 0; b < 4; ++b)

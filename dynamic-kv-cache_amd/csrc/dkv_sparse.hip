@@ -356,7 +356,7 @@ __global__ __launch_bounds__(256) void attend_kernel(dkv_attn_args a, dkv_sparse
   const int splits = splits_of(a, v, most);
   if ((int)blockIdx.x >= splits) return;
   const int G = a.q_heads / a.heads, h = blockIdx.y / row_blocks, rb = blockIdx.y % row_blocks, m = blockIdx.z;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
   const int heads_here = min(16, G - 16 * rb);
   const int64_t pair = (int64_t)h * a.nq + m;
   Op q[2];
