@@ -15,14 +15,20 @@ namespace mass {
 using namespace rows;
 
 constexpr int FEW = 64;           // query rows of a KV head that a wave takes alone
-constexpr int GROUP = 192;        // query rows of a row group: 12 blocks, three a wave
+// Query rows of a KV head whose scores the first pass keeps for the second: a key's scores are 4 bytes a row written and
+// read, its packed row 40 to 128 and the arithmetic again. A token over 131007 at fp32, 8 KV heads: 36.7 us with kept scores
+// against 53.5 at 4 rows, 41.4 against 53.3 at 8.
+constexpr int KEEP = 8;
+constexpr int GROUP = 192;               // query rows of a row group: 12 blocks, three a wave
 constexpr int BLOCKS = GROUP / 64;  // 16-row blocks of a wave
 
 struct MassArgs {
   int splits, row_groups, row_parts;
+  int kept;          // the scores stay for the second launch
   float2* part;      // [heads][splits][rows] maximum (base 2) and sum
   float2* norm;      // [heads][rows] reference and 1 / sum (many rows)
-  float* columns;    // [row_parts][heads][stride] sums of a part of the rows (row_parts > 1)
+  float* columns;    // [row_parts][heads][stride] sums of a part of the rows (row_parts > 1); or with kept scores
+                     // [heads][rows][stride] the scores, -infinity where masked
   int64_t columns_stride;
   float* out;        // [heads] rows of out_stride
   int64_t out_stride;
@@ -143,6 +149,24 @@ __device__ __forceinline__ int query_row(const dkv_attn_args& a, int h, int row,
   return r.m;
 }
 
+// load_key of any width without a branch: what a branch loads is waited for where the widths meet, and the loads of a unit
+// would come one after the other. Two pieces of 16 bytes always: at 8 bits the same one twice, at 4 bits one of which the
+// second half lies in the next piece or in the scales (a sub-block has 8 bytes a row behind its codes).
+struct __attribute__((packed, aligned(8))) Bytes16 {
+  u32x4 x;
+};
+__device__ __forceinline__ void load_any(const UnitRows& u, int row, int g, KeyPiece& p) {
+  const int r = row < u.rows ? row : 0;
+  const uint8_t* at = u.k + r * u.k_stride + g * 2 * u.bits;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const u32x4 x = reinterpret_cast<const Bytes16*>(at + (u.bits == 16 ? 16 * i : 0))->x;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) p.w[4 * i + j] = x[j];
+  }
+  p.as = *reinterpret_cast<const float2*>(u.bits == 16 ? u.k : u.k + (int64_t)u.rows * (8 * u.bits) + 8 * r);
+}
+
 // 16 sums a lane, [b][i] of key 16 b + 4 g + i, over the 16 lanes of a group: each lane ends with one key's, which it
 // returns, and that key. Halves change places with the mirrored lane of 16, of 8, of 4 and of 2.
 template <int CONTROL, int HALF>
@@ -174,13 +198,16 @@ struct RawKeys {
 template <int PREC>
 __device__ __forceinline__ void load_unit(const UnitRows& u, int c, int g, RawKeys& k) {
 #pragma unroll
-  for (int b = 0; b < 4; ++b) {
-    if (u.bits == 4) load_key<4>(u, 16 * b + c, g, k.p[b]);
-    else if (u.bits == 8) load_key<8>(u, 16 * b + c, g, k.p[b]);
-    else load_key<16>(u, 16 * b + c, g, k.p[b]);
-  }
-  if (PREC == 1 && u.bits == 4) load_scales<4>(u.k, u.rows, g, k.as);
-  if (PREC == 1 && u.bits == 8) load_scales<8>(u.k, u.rows, g, k.as);
+  for (int b = 0; b < 4; ++b) load_any(u, 16 * b + c, g, k.p[b]);
+  if (PREC == 0) return;
+  const uint8_t* scales = u.bits == 16 ? u.k : u.k + (int64_t)u.rows * (8 * u.bits);
+#pragma unroll
+  for (int b = 0; b < 4; ++b)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int row = 16 * b + 4 * g + 2 * i;
+      k.as[b][i] = *reinterpret_cast<const f32x4*>(scales + (u.bits < 16 && row < u.rows ? 8 * row : 0));
+    }
 }
 
 template <int BITS, int PREC, int NB>
@@ -240,6 +267,10 @@ struct FewRows {
   }
 };
 
+// Kept scores are stored without a branch, lanes that have none behind the buffer's end, so that the next unit's loads,
+// issued before, are waited for without the stores (51.9 us against 30 for a token over 131007 with branches).
+constexpr uint32_t NOWHERE = 0xffffffffu;
+
 template <int PREC, int NB>
 __global__ __launch_bounds__(256) void few_stats_kernel(dkv_attn_args a, MassArgs p) {
   __shared__ float2 ml[4][16 * NB];
@@ -254,9 +285,27 @@ __global__ __launch_bounds__(256) void few_stats_kernel(dkv_attn_args a, MassArg
 #pragma unroll
   for (int n = 0; n < NB; ++n) top[n] = -INFINITY, sum[n] = 0.f;
   const float scale2 = a.scale * LOG2E;
-  few.each(a, v, h, 4 * blockIdx.x + wave, 4 * splits, c, g, [&](int, const Unit64&, const f32x4 (&s)[NB][4]) {
+  const auto kept = __builtin_amdgcn_make_buffer_rsrc(p.columns + (int64_t)h * rows * p.columns_stride, 0,
+                                                      p.kept ? (int)(rows * p.columns_stride * 4) : 0, 0x00027000);
+  few.each(a, v, h, 4 * blockIdx.x + wave, 4 * splits, c, g, [&](int unit, const Unit64& x, const f32x4 (&s)[NB][4]) {
 #pragma unroll
     for (int n = 0; n < NB; ++n) add_scores(s[n], scale2, top[n], sum[n]);
+    if (NB == 1 && p.kept) {
+      const int token = x.first < 0 ? a.tiles[unit].token_start : v.past + x.first;
+      const uint32_t row = 4u * (uint32_t)(c * p.columns_stride + token + 4 * g);
+      if (x.u.high == TILE) {
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, s[0][b]), kept, c < rows ? row + 64 * b : NOWHERE, 0, 0);
+      } else {
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(s[0][b][i]), kept,
+                                                  c < rows && 16 * b + 4 * g + i < x.u.high ? row + 64 * b + 4 * i : NOWHERE, 0, 0);
+      }
+    }
   });
 #pragma unroll
   for (int n = 0; n < NB; ++n) {  // the four lanes of a row join theirs
@@ -276,36 +325,43 @@ __global__ __launch_bounds__(256) void few_stats_kernel(dkv_attn_args a, MassArg
   }
 }
 
+// The rows' references and 1 / sum, joined from the splits by several threads a row; all threads call it.
+template <int R>
+struct Norms {
+  static constexpr int SLICES = 256 / R;
+  float2 ml[SLICES][R], norm[R];
+  __device__ __forceinline__ void join_splits(const float2* part, int splits, int rows) {
+    const int row = threadIdx.x % R, slice = threadIdx.x / R, from = splits * slice / SLICES, to = splits * (slice + 1) / SLICES;
+    float m = -INFINITY, l = 0.f;
+    if (row < rows) join(part + row, from, to, rows, m, l);
+    ml[slice][row] = make_float2(m, l);
+    __syncthreads();
+    if (threadIdx.x < R) {
+      m = -INFINITY, l = 0.f;
+#pragma unroll
+      for (int i = 0; i < SLICES; ++i) m = fmaxf(m, ml[i][threadIdx.x].x);
+      const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+      for (int i = 0; i < SLICES; ++i) l += ml[i][threadIdx.x].y * __builtin_amdgcn_exp2f(ml[i][threadIdx.x].x - ref);
+      norm[threadIdx.x] = (int)threadIdx.x < rows ? make_float2(m, 1.f / l) : make_float2(0.f, 0.f);
+    }
+    __syncthreads();
+  }
+};
+
 template <int PREC, int NB>
 __global__ __launch_bounds__(256) void few_columns_kernel(dkv_attn_args a, MassArgs p) {
-  constexpr int R = 16 * NB, SLICES = 256 / R;  // threads of a row in the join
-  __shared__ float2 ml[SLICES][R], norm[R];
+  __shared__ Norms<16 * NB> norms;
   const History v = history_of(a);
   const int h = blockIdx.y, wave = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
   if (4 * (int)blockIdx.x >= v.units) return;
   const int rows = a.q_heads / a.heads * a.nq, splits = split_count(p.splits, v.units, true);
-  {
-    const int row = threadIdx.x % R, slice = threadIdx.x / R, from = splits * slice / SLICES, to = splits * (slice + 1) / SLICES;
-    float m = -INFINITY, l = 0.f;
-    if (row < rows) join(p.part + (int64_t)h * splits * rows + row, from, to, rows, m, l);
-    ml[slice][row] = make_float2(m, l);
-  }
   FewRows<PREC, NB> few;
   few.load(a, h, rows, c, g);
-  __syncthreads();
-  if (threadIdx.x < R) {
-    float m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int i = 0; i < SLICES; ++i) m = fmaxf(m, ml[i][threadIdx.x].x);
-    const float ref = m == -INFINITY ? 0.f : m;
-#pragma unroll
-    for (int i = 0; i < SLICES; ++i) l += ml[i][threadIdx.x].y * __builtin_amdgcn_exp2f(ml[i][threadIdx.x].x - ref);
-    norm[threadIdx.x] = (int)threadIdx.x < rows ? make_float2(m, 1.f / l) : make_float2(0.f, 0.f);
-  }
-  __syncthreads();
+  norms.join_splits(p.part + (int64_t)h * splits * rows, splits, rows);
   float2 nm[NB];
 #pragma unroll
-  for (int n = 0; n < NB; ++n) nm[n] = norm[16 * n + c];
+  for (int n = 0; n < NB; ++n) nm[n] = norms.norm[16 * n + c];
   const float scale2 = a.scale * LOG2E;
   few.each(a, v, h, 4 * blockIdx.x + wave, 4 * gridDim.x, c, g, [&](int unit, const Unit64& x, const f32x4 (&s)[NB][4]) {
     float sum[4][4] = {};
@@ -319,20 +375,46 @@ __global__ __launch_bounds__(256) void few_columns_kernel(dkv_attn_args a, MassA
   });
 }
 
+// The columns of kept scores: EACH tokens a thread, no key and no tile is read again.
+template <int EACH>
+struct __attribute__((aligned(4 * EACH))) Scores {
+  float x[EACH];
+};
+constexpr int EACH = 4;
+__global__ __launch_bounds__(256) void kept_columns_kernel(dkv_attn_args a, MassArgs p) {
+  __shared__ Norms<16> norms;
+  const History v = history_of(a);
+  const int h = blockIdx.y, tokens = v.past + a.nq, token = (blockIdx.x * 256 + threadIdx.x) * EACH;
+  if ((int)blockIdx.x * 256 * EACH >= tokens) return;
+  const int rows = a.q_heads / a.heads * a.nq, splits = split_count(p.splits, v.units, true);
+  Scores<EACH> s[KEEP];
+  const float* from = p.columns + (int64_t)h * rows * p.columns_stride + min((int64_t)token, p.columns_stride - EACH);
+#pragma unroll
+  for (int r = 0; r < KEEP; ++r) s[r] = *reinterpret_cast<const Scores<EACH>*>(from + min(r, rows - 1) * p.columns_stride);
+  norms.join_splits(p.part + (int64_t)h * splits * rows, splits, rows);
+  const float scale2 = a.scale * LOG2E;
+  float sum[EACH] = {};
+#pragma unroll
+  for (int r = 0; r < KEEP; ++r) {
+    if (r >= rows) break;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r].x[i], scale2, -norms.norm[r].x));
+      sum[i] = s[r].x[i] == -INFINITY ? sum[i] : __builtin_fmaf(w, norms.norm[r].y, sum[i]);
+    }
+  }
+  float* out = p.out + h * p.out_stride + token;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i)
+    if (token + i < tokens) out[i] = p.accumulate ? out[i] + sum[i] : sum[i];
+}
+
 // ---- many rows: a workgroup a unit -----------------------------------------------------------------------------
 // A unit's keys as MFMA operands, a wave a 16-key block, and their (offset, scale) where scores take them.
 struct Keys {
   Op op[4][2][64];
   f32x4 as[32];
 };
-
-template <int PREC>
-__device__ __forceinline__ void load_block(const UnitRows& u, int wave, int lane, KeyPiece& p) {
-  const int row = 16 * wave + (lane & 15), g = lane >> 4;
-  if (u.bits == 4) load_key<4>(u, row, g, p);
-  else if (u.bits == 8) load_key<8>(u, row, g, p);
-  else load_key<16>(u, row, g, p);
-}
 
 template <int PREC>
 __device__ __forceinline__ void stage_block(const UnitRows& u, const KeyPiece& p, int wave, int lane, Keys& keys) {
@@ -392,7 +474,7 @@ __global__ __launch_bounds__(256, PREC ? 2 : 4) void stats_kernel(dkv_attn_args 
   Unit64 x = unit_of(a, v, from, h);
   x.u.bits = __builtin_amdgcn_readfirstlane(x.u.bits);
   KeyPiece piece;
-  load_block<PREC>(x.u, wave, lane, piece);
+  load_any(x.u, 16 * wave + c, g, piece);
   for (int unit = from; unit < to; ++unit) {
     __syncthreads();
     stage_block<PREC>(x.u, piece, wave, lane, keys);
@@ -400,7 +482,7 @@ __global__ __launch_bounds__(256, PREC ? 2 : 4) void stats_kernel(dkv_attn_args 
     if (unit + 1 < to) {  // the next unit's keys load while this one's scores are computed
       x = unit_of(a, v, unit + 1, h);
       x.u.bits = __builtin_amdgcn_readfirstlane(x.u.bits);
-      load_block<PREC>(x.u, wave, lane, piece);
+      load_any(x.u, 16 * wave + c, g, piece);
     }
     __syncthreads();
 #pragma unroll
@@ -462,7 +544,7 @@ __global__ __launch_bounds__(256, PREC ? 2 : 4) void columns_kernel(dkv_attn_arg
   Unit64 x = unit_of(a, v, unit, h);
   x.u.bits = __builtin_amdgcn_readfirstlane(x.u.bits);
   KeyPiece piece;
-  load_block<PREC>(x.u, wave, lane, piece);
+  load_any(x.u, 16 * wave + c, g, piece);
   if (JOIN && (int)threadIdx.x < rows) {
     const int splits = split_count(p.splits, v.units, false);
     float m = -INFINITY, l = 0.f;
@@ -553,7 +635,9 @@ static MassPlan plan_of(const dkv_attn_args& a) {
   m.p.columns_stride = ((int64_t)a.past + a.nq + 63) & ~63;
   m.part_bytes = ((int64_t)a.heads * m.p.splits * rows * sizeof(float2) + 255) & ~(int64_t)255;
   m.norm_bytes = few ? 0 : ((int64_t)a.heads * rows * sizeof(float2) + 255) & ~(int64_t)255;
-  m.bytes = m.part_bytes + m.norm_bytes + (m.p.row_parts > 1 ? m.p.row_parts * a.heads * m.p.columns_stride * 4 : 0);
+  m.p.kept = rows <= KEEP && rows * m.p.columns_stride * 4 <= INT32_MAX;
+  const int64_t columns = m.p.kept ? rows : m.p.row_parts > 1 ? m.p.row_parts : 0;
+  m.bytes = m.part_bytes + m.norm_bytes + columns * a.heads * m.p.columns_stride * 4;
   return m;
 }
 
@@ -609,7 +693,10 @@ int dkv_attention_mass(const dkv_attn_args* args, float* mass, int64_t mass_head
                                           : (rows <= 16 ? few_columns_kernel<0, 1> : few_columns_kernel<0, 4>);
     const int by_unit = (units + 3) / 4, most = WORKGROUPS_FEW / a.heads;
     hipLaunchKernelGGL(stats, dim3(p.splits, a.heads), dim3(256), 0, st, a, p);
-    hipLaunchKernelGGL(columns, dim3(by_unit < most ? by_unit : most < 1 ? 1 : most, a.heads), dim3(256), 0, st, a, p);
+    if (p.kept)
+      hipLaunchKernelGGL(kept_columns_kernel, dim3((a.past + a.nq + 256 * EACH - 1) / (256 * EACH), a.heads), dim3(256), 0, st, a, p);
+    else
+      hipLaunchKernelGGL(columns, dim3(by_unit < most ? by_unit : most < 1 ? 1 : most, a.heads), dim3(256), 0, st, a, p);
     return (int)hipGetLastError();
   }
   const auto stats = a.precision == 1 ? stats_kernel<1> : stats_kernel<0>;
