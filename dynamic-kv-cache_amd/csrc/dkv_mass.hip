@@ -19,7 +19,7 @@ constexpr int FEW = 64;           // query rows of a KV head that a wave takes a
 // read, its packed row 40 to 128 and the arithmetic again. A token over 131007 at fp32, 8 KV heads: 36.7 us with kept scores
 // against 53.5 at 4 rows, 41.4 against 53.3 at 8.
 constexpr int KEEP = 8;
-constexpr int GROUP = 192;               // query rows of a row group: 12 blocks, three a wave
+constexpr int GROUP = 192;        // query rows of a row group: 12 blocks, three a wave
 constexpr int BLOCKS = GROUP / 64;  // 16-row blocks of a wave
 
 struct MassArgs {

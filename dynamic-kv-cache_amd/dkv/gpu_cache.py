@@ -238,6 +238,56 @@ class GPUCache(_CacheBase):
         self.arena_used = int(ends[-1])
         return tile0
 
+    def _open_kept(self, old, a, b, share):
+        """What an eviction leaves of `old`, in this empty cache: its segments [0, a), a segment of share[w] rows for
+        every width w, and its segments from b on. The bookkeeping of _open_segments(), with the ends' taken over."""
+        segs, n_old = old.segments, len(old.tile_starts)
+        tile, token, offset = (segs[a].tile0, segs[a].start, segs[a].offset) if a < len(segs) else (n_old, old.seen[0], old.arena_used)
+        tail = segs[b:]
+        tile1, token1, offset1 = (tail[0].tile0, tail[0].start, tail[0].offset) if tail else (n_old, old.seen[0], old.arena_used)
+        counts = [-(-m // TILE) for m in share.values()]
+        sizes = [segment_bytes(m, w, self.layers, self.heads) for w, m in share.items()]
+        if offset + sum(sizes) + old.arena_used - offset1 > self.arena_bytes:
+            self._grow(offset + sum(sizes) + old.arena_used - offset1)
+        # the table as pairs of words: offset, and token_start | rows << 32 | bits << 48
+        table, before = self.tiles_host.view(np.int64).reshape(-1, 2), old.tiles_host.view(np.int64).reshape(-1, 2)
+        table[:tile] = before[:tile]
+        starts, singles = old.tile_starts[:tile], old.tile_singles[:tile]
+        segments, plan, held = segs[:a], old.plan[:a], {4: 0, 8: 0, 16: 0}
+        for seg in segments:
+            held[seg.bits] += seg.rows
+        for (w, m), tiles, size in zip(share.items(), counts, sizes):
+            segments.append(_Segment(token, m, w, offset, tile))
+            plan.append((token, token + m, w, held[w]))
+            held[w] += m
+            slab, words = slab_bytes(TILE, w, self.layers, self.heads), token | TILE << 32 | w << 48
+            table[tile:tile + tiles, 0] = np.arange(offset, offset + tiles * slab, slab)
+            table[tile:tile + tiles, 1] = np.arange(words, words + tiles * TILE, TILE)
+            table[tile + tiles - 1, 1] -= (tiles * TILE - m) << 32
+            starts.extend(range(token, token + m, TILE))
+            singles += [0] * tiles
+            if w == 16 and m % TILE == 1:
+                singles[-1] = (singles[-2] if tiles == 1 and tile else 0) + 1
+            tile, token, offset = tile + tiles, token + m, offset + size
+        if tail:
+            by, up = token - token1, offset - offset1
+            table[tile:tile + n_old - tile1] = before[tile1:n_old] + (up, by)
+            starts += [t + by for t in old.tile_starts[tile1:]]
+            run = singles[-1] if singles else 0
+            if run == (old.tile_singles[tile1 - 1] if tile1 else 0):
+                singles += old.tile_singles[tile1:]
+            else:
+                for single in old.tile_singles[tile1:]:
+                    run = run + 1 if single else 0
+                    singles.append(run)
+            for s in tail:
+                segments.append(_Segment(s.start + by, s.rows, s.bits, s.offset + up, s.tile0 + tile - tile1, s.frame))
+                plan.append((s.start + by, s.end + by, s.bits, held[s.bits]))
+                held[s.bits] += s.rows
+            offset += old.arena_used - offset1
+        self.segments, self.plan, self.host_counts = segments, plan, held
+        self.tile_starts, self.tile_singles, self.arena_used = starts, singles, offset
+
     def _grow(self, needed):
         """Grows this cache's arena (forks keep theirs), like the reference's reserve()."""
         size = max(needed, ((int(self.arena_bytes * 1.5) + 255) // 256) * 256)
@@ -891,22 +941,20 @@ class GPUCache(_CacheBase):
                              'no branch and outside graph steps')
         if into.arena is self.arena or into.tiles is self.tiles or into._mass is self._mass:
             raise ValueError('evict: into must not be this cache or share its storage')
-        lead, trail = self.segments[:a], self.segments[b:]
-        lengths = [s.rows for s in lead] + list(share.values()) + [s.rows for s in trail]
-        bits = [s.bits for s in lead] + list(share) + [s.bits for s in trail]
-        if sum(lengths) > into.capacity or sum(-(-m // TILE) for m in lengths) > into.tiles.shape[0]:
+        total = n - sum(held.values()) + sum(share.values())
+        tiles = len(self.tile_starts) + sum(-(-m // TILE) for m in share.values())
+        if b > a:
+            tiles -= (self.segments[b].tile0 if b < len(self.segments) else len(self.tile_starts)) - self.segments[a].tile0
+        if total > into.capacity or tiles > into.tiles.shape[0]:
             raise ValueError('GPU context limit exceeded')
         mass, into._mass = into._mass, None  # (written below: reset() need not clear it)
         into.reset()
         with torch.inference_mode(False):
             into._mass = torch.empty((into.layers, into.heads, into.capacity), dtype=torch.float32,
                                      device=into.device) if mass is None else mass
-        kept = self.arena.new_empty((self.layers, self.heads, sum(lengths)), dtype=torch.int32)
-        if lengths:
-            into._open_segments(0, lengths, bits)
-            for new, old in zip(into.segments, lead + [None] * len(share) + trail):
-                if old is not None:
-                    new.frame = old.frame
+        kept = self.arena.new_empty((self.layers, self.heads, total), dtype=torch.int32)
+        if total:
+            into._open_kept(self, a, b, share)
             first = self.segments[a] if a < len(self.segments) else None
             last = self.segments[b] if b < len(self.segments) else None
             e = _lib.EvictArgs()
@@ -930,8 +978,8 @@ class GPUCache(_CacheBase):
             self._call('dkv_evict', ctypes.byref(e))
         else:
             into._mass.zero_()
-        into.seen = [sum(lengths)] * into.layers
-        into.kept, into.dropped = kept, self.dropped + n - sum(lengths)
+        into.seen = [total] * into.layers
+        into.kept, into.dropped = kept, self.dropped + n - total
         into.pending_bits, into.frame_id = self.pending_bits, self.frame_id
         return into
 
