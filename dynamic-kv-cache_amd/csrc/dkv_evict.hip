@@ -149,12 +149,14 @@ __global__ __launch_bounds__(THREADS) void choose_kernel(dkv_evict_args e, Work 
     kept[first + to] = i;
   });
   __syncthreads();
-  constexpr int AHEAD = 8;  // loads in flight
+  // Places become tokens, where they lie. Loads are in flight together; a thread with fewer than AHEAD reads its own first
+  // place again, never another thread's, which may hold a token by then: an index past the class.
+  constexpr int AHEAD = 8;
   for (int i0 = threadIdx.x; i0 < keep; i0 += AHEAD * THREADS) {
     int token[AHEAD];
     float m[AHEAD];
 #pragma unroll
-    for (int j = 0; j < AHEAD; ++j) token[j] = kept[first + min(i0 + j * THREADS, keep - 1)];
+    for (int j = 0; j < AHEAD; ++j) token[j] = kept[first + (i0 + j * THREADS < keep ? i0 + j * THREADS : i0)];
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) token[j] = order[token[j]];
 #pragma unroll

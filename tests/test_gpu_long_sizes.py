@@ -2,6 +2,7 @@
 chunks of many query rows, rows of logits by the hundred, and replays whose bounds lie on one side of such a border and
 whose history on the other."""
 import math
+import random
 
 import pytest
 import torch
@@ -108,6 +109,17 @@ def test_classes_of_many_tokens(cuda, segments):
     n = sum(t for t, _ in segments)
     for keep in (n // 3, n - 1):
         evicting.check(cuda, segments, 1, 1, keep, 0, 0)
+
+
+@pytest.mark.parametrize('seed', [0, 1])
+def test_kept_places_become_tokens_once(cuda, seed):
+    """Most of three classes of some 10000 tokens stay: every place of a kept token is read by its own thread alone
+    before the token takes its place (a place read after it pointed behind the last class's tokens)."""
+    frames = random.Random(seed).choices([4, 8, 16], weights=[.4, .4, .2], k=351)
+    segments = [(63, 16)] + [(78, b) for b in frames] + [(35, 4)]
+    n = sum(t for t, _ in segments)
+    mass = torch.rand(2, 5, n, generator=torch.Generator().manual_seed(seed))
+    evicting.check(cuda, segments, 5, 2, n - 587, 54, 4101, mass=mass, seed=seed)
 
 
 def test_eviction_on_another_stream(cuda):
