@@ -6,6 +6,9 @@
 // Three launches: where each token lies and which tokens each width has, with the new tile table; the choice, a radix
 // search for the smallest kept mass per (layer, head, width); and the move, which is bound by memory (each kept row
 // read and written once).
+// Measured (kernel times): 65531 to 16384 tokens, 4 layers of 8 heads: 9.0 + 31.8 (96 workgroups: three radix steps and
+// their barriers over up to 26000 keys each) + 51.5 us (148 MB read and written, 2.9 TB/s: a row is 32 to 128
+// bytes at an address of its own). 8128 to 4096, 8 layers of 5: 6.2 + 12.2 + 11.1; a call's host part, some 60 us, is longer.
 #include "dkv_select.h"
 
 namespace dkv {
@@ -125,7 +128,8 @@ __global__ __launch_bounds__(THREADS) void map_kernel(dkv_evict_args e, Work w) 
 }
 
 // blockIdx: (layer * heads + head, class). The class's tokens of the largest masses, in token order; equal masses
-// keep the earlier token. Class 0 also lists the protected ends. Up to N * THREADS keys stay in registers.
+// keep the earlier token. Class 0 also lists the protected ends. Up to N * THREADS keys stay in registers: 65531 to 16384
+// tokens, read back, 146 us with N = 32 and 164 with keys loaded again each time (N = 0); 8128 to 4096 124 with N = 4, 128.
 template <int N>
 __global__ __launch_bounds__(THREADS) void choose_kernel(dkv_evict_args e, Work w) {
   __shared__ SelectScratch<THREADS, 11> scratch;

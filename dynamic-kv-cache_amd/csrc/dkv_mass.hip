@@ -3,10 +3,15 @@
 // the weight by which a cache forgets tokens. Two passes over the keys alone: the first gives every query row its
 // maximum and sum over ranges of units (64 keys), the second joins them and sums each key's column over all rows. No
 // sum is shared between workgroups, so the result does not depend on their order.
-//   - up to 64 query rows a KV head (generated tokens): a wave a unit, keys and queries in registers, nothing in LDS;
+//   - up to 64 query rows a KV head (generated tokens): a wave a unit, keys and queries in registers, nothing in LDS. Of up
+//     to 8 rows the first pass keeps the scores, and the second reads these alone;
 //   - more: a workgroup a unit, whose waves unpack 16 keys each into MFMA operands in LDS and take the 16-row query
 //     blocks in turn. The rows are joined in a launch between the passes, and where a chunk is long the second pass's
 //     workgroups take a part of the rows each and one more launch adds the parts up.
+// Measured (kernel times): a token past 131007 at fp32, 8 KV heads of 4: 29.9 us (73 MB of keys, 2.4 TB/s: two waves a SIMD
+// wait for their next unit) + 8.5 (17 MB of scores). A 64-token frame past 8128, 5 KV heads of 3: 11.1 + 11.7, each a
+// few dependent loads, three units a workgroup and the join. A 2048-token prompt past 1000: 29.9 + 4.9 + 42.1 + 4.8; the
+// products alone are 6.7 us; each pass's 62 million exponentials with what surrounds them some 17, by instructions.
 #include "dkv_rows.h"
 
 namespace dkv {
@@ -14,7 +19,9 @@ namespace mass {
 
 using namespace rows;
 
-constexpr int FEW = 64;           // query rows of a KV head that a wave takes alone
+// Query rows of a KV head that a wave takes alone. A chunk of 48 rows past 8128 (5 KV heads) 13.0 us against 14.8 in
+// workgroups, 63 rows 13.4 and 14.9; 64 rows past 131007 at fp32 127 and 200.
+constexpr int FEW = 64;
 // Query rows of a KV head whose scores the first pass keeps for the second: a key's scores are 4 bytes a row written and
 // read, its packed row 40 to 128 and the arithmetic again. A token over 131007 at fp32, 8 KV heads: 36.7 us with kept scores
 // against 53.5 at 4 rows, 41.4 against 53.3 at 8.
@@ -95,7 +102,8 @@ __device__ __forceinline__ void add_scores(const f32x4 (&s)[4], float scale2, fl
   top = m, sum = l;
 }
 
-// Adds 16 keys' weights of a row (norm: reference and 1 / sum, 0 for a row that only fills a block up). A masked key gets nothing, also of a row whose sum is not a number.
+// Adds 16 keys' weights of a row (norm: reference and 1 / sum, 0 for a row that only fills a block up). A masked key gets
+// nothing, also of a row whose sum is not a number.
 template <bool MASKED>
 __device__ __forceinline__ void add_weights(const f32x4 (&s)[4], float scale2, float2 norm, float (&sum)[4][4]) {
   if (norm.y == 0.f) return;
@@ -380,7 +388,7 @@ template <int EACH>
 struct __attribute__((aligned(4 * EACH))) Scores {
   float x[EACH];
 };
-constexpr int EACH = 4;
+constexpr int EACH = 4;  // (a token a thread: 64.4 us against 58.9 for a token past 131007, more joins of the splits)
 __global__ __launch_bounds__(256) void kept_columns_kernel(dkv_attn_args a, MassArgs p) {
   __shared__ Norms<16> norms;
   const History v = history_of(a);
@@ -608,11 +616,15 @@ __global__ __launch_bounds__(256) void add_parts_kernel(dkv_attn_args a, MassArg
   *out = p.accumulate ? *out + x : x;
 }
 
-constexpr int WORKGROUPS = 1024;  // workgroups of a launch, where there is work for as many
-constexpr int MAX_SPLITS = 32;    // ranges of units that the second launch joins for many rows, at most
-constexpr int WORKGROUPS_FEW = 512;  // (two a CU are resident, and each joins the splits once)
+// Workgroups of a launch where there is work for as many, and ranges of units that the second launch joins, at most. Many
+// rows: 2048 and 4096 workgroups took 78.0 and 82.2 us for 2048 tokens past 1000 against 77.9 with 1024. Few rows: 1024
+// workgroups of up to 128 splits 66.6 us for a token past 131007 against 61.2 (two workgroups a CU are resident, and each
+// joins the splits once).
+constexpr int WORKGROUPS = 1024;
+constexpr int MAX_SPLITS = 32;
+constexpr int WORKGROUPS_FEW = 512;
 constexpr int MAX_SPLITS_FEW = 64;
-constexpr int MAX_ROW_PARTS = 8;
+constexpr int MAX_ROW_PARTS = 8;  // 2048 tokens past 1000 74.9 us, with 4 parts 78.3, with 2 85.7, with 16 the same
 
 struct MassPlan {
   MassArgs p;

@@ -5,8 +5,15 @@
 // bounds the sum of a query's scores over the tile's keys. As max(q x, q y) is q+ y + q- x for x <= y, with
 // q+ = max(q, 0) and q- = min(q, 0), the sum over the query heads comes before the product: one dot product of
 // 128 elements for each (query, KV head, tile). A query attends to the `blocks` tiles of the highest scores
-// (equal ones: the first), to every tile after the index and to its chunk, in four launches: scores, choice,
-// attention, and a merge where a query's tiles are split over workgroups.
+// (equal ones: the first), to every tile after the index and to its chunk: scores and choice in one launch where the
+// index is short (near_kernel), in two where it is long, then the attention, and a merge where a query's tiles are split
+// over workgroups. Nothing of the history but the index, the chosen tiles and the tail is read.
+//
+// Measured (kernel times, 5 KV heads of 3 query heads unless said): a token past 8128 near 6.6, attention 7.8, merge
+// 3.1 us, 16.6 us a call; a token past 131007 with 8 KV heads of 4 scores 4.6, choice 5.8, attention 7.8, merge 4.4, 21.6
+// a call: latency, each launch a few dependent loads. 64 queries past 32704: 10.3 + 36.6 + 4.8, 48.4 a call; 513 queries
+// past 20011 at fp32, 3 KV heads of 3: 22.4 + 8.4 + 136, 159 a call: every query walks some 30 tiles of its own, 400 MB
+// through L2 at 3 TB/s, of whose 16 MFMA rows three are its query heads.
 #include "dkv_rows.h"
 #include "dkv_select.h"
 
@@ -24,7 +31,9 @@ __device__ __forceinline__ int64_t piece_at(int block, int layer, int layers, in
   return (((int64_t)block * layers + layer) * heads + h) * BLOCK_PIECES * BLOCK;
 }
 
-constexpr int INDEX_TILES = 16;  // tiles of an index workgroup, a wave a tile
+// Tiles of an index workgroup, a wave a tile: 16 tiles' pieces of 16 bytes are 256 consecutive bytes of the index. Bound by
+// memory: 32 layers of 5 heads past 8128 (97 MB) 36.5 us, 2.7 TB/s; a workgroup a tile took 64.
+constexpr int INDEX_TILES = 16;
 
 // One step of a minimum (and maximum, of the negated) over lanes that halves the elements a lane holds: x keeps the lower
 // half's lanes, y the upper half's. v_permlane swaps x's upper lanes with y's lower ones.
@@ -140,7 +149,8 @@ constexpr int SCORE_QUERIES = 16;
 
 // Scores of 64 tiles for 16 queries of a KV head, as sortable keys. Each wave takes 32 of the 128 elements, a lane
 // a tile; their sums meet in LDS in a fixed order. In 64 bits, rounded to 32 at the end: the products of bf16 values
-// are exact there and their sums as good as exact, so equal scores tie and no order of summation chooses a tile.
+// are exact there and their sums as good as exact, so equal scores tie and no order of summation chooses a tile. Bound by
+// these products: 513 queries by 520 tiles by 3 KV heads 22.4 us.
 __global__ __launch_bounds__(256) void score_kernel(dkv_attn_args a, dkv_sparse s, int max_indexed, uint32_t* keys) {
   __shared__ double query[SCORE_QUERIES][2 * D];  // q+ then q-, as the pieces' high and low
   __shared__ double part[4][SCORE_QUERIES][BLOCK];
@@ -198,7 +208,9 @@ __global__ __launch_bounds__(256) void score_kernel(dkv_attn_args a, dkv_sparse 
   }
 }
 
-// The chosen tiles of a (query, KV head), in order. Up to N * CHOOSERS keys stay in registers.
+// The chosen tiles of a (query, KV head), in order. Up to N * CHOOSERS keys stay in registers: a token past 131007 (2048
+// tiles) 21.6 us a call with N = 8, 23.4 with keys loaded again each time (N = 0), which longer indexes take. Bound by the
+// barriers of a radix step, about three a choice.
 constexpr int CHOOSERS = 256;
 template <int N>
 __global__ __launch_bounds__(CHOOSERS) void choose_kernel(dkv_attn_args a, dkv_sparse s, int max_indexed, int max_chosen,
@@ -214,7 +226,8 @@ __global__ __launch_bounds__(CHOOSERS) void choose_kernel(dkv_attn_args a, dkv_s
 }
 
 // Scores and choice of a (query, KV head) in one workgroup, a wave 64 tiles: for up to NEAR_TILES indexed tiles. The sums
-// are score_kernel's, term by term.
+// are score_kernel's, term by term. Against scores and choice in two launches: a token past 8128 16.6 us a call and 19.3, 64
+// queries past 32704 (511 tiles) 48.4 and 55.1.
 constexpr int NEAR_TILES = 512;
 __global__ __launch_bounds__(NEAR_TILES) void near_kernel(dkv_attn_args a, dkv_sparse s, int max_chosen, int32_t* lists) {
   __shared__ SelectScratch<NEAR_TILES, 8> scratch;
@@ -347,6 +360,9 @@ __device__ __forceinline__ void store4(void* out, int out_dtype, int64_t at, f32
     *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(out) + at) = u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
 }
 
+// A wave a unit of 64 keys, keys and values straight from global memory into MFMA operands: a unit is read by one query
+// alone, so LDS would only add a pass. 220 to 232 registers, two waves a SIMD; held to three they spill (66 us against 54
+// for 64 queries past 32704).
 template <int PREC, int TERMS>
 __global__ __launch_bounds__(256) void attend_kernel(dkv_attn_args a, dkv_sparse s, int row_blocks, int most, int max_chosen,
                                                      const int32_t* lists, float* part_o, float2* part_ml) {
@@ -460,7 +476,8 @@ __global__ __launch_bounds__(256) void merge_kernel(dkv_attn_args a, dkv_sparse 
   store4(a.out, a.out_dtype, m * a.out_tok_stride + (h * G + row) * a.out_head_stride + 4 * e4, x / l);
 }
 
-constexpr int WORKGROUPS = 1024;  // attention workgroups that a call is split into
+// Attention workgroups that a call is split into: 64 queries past 32704 54 us with 1024, 62 with 512, 60 with 2048 (then).
+constexpr int WORKGROUPS = 1024;
 
 static SparsePlan plan_of(const dkv_attn_args& a, const dkv_sparse& s) {
   SparsePlan p{};
