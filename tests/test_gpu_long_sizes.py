@@ -223,6 +223,31 @@ def test_many_kept_of_a_large_vocabulary(cuda, kw, dtype):
     sampling.check(cuda, *sampling.rows_of(2, 49281, dtype, 32), **kw)
 
 
+def test_vocabularies_past_half_a_million(cuda):
+    """Parts too long for the registers of a workgroup, and the longest row there is."""
+    x, u = sampling.rows_of(1, 600011, torch.float32, 50)
+    for kw in (dict(top_k=20), dict(top_p=0.9), dict(temperature=0.0)):
+        sampling.check(cuda, x, u, **kw)
+    x = torch.full((1, 1 << 22), -math.inf, dtype=torch.bfloat16, device=cuda)
+    x[0, 4000000] = x[0, 7] = 1.0
+    for v, want in ((0.25, 7), (0.75, 4000000)):
+        assert sample(x, torch.tensor([v], device=cuda), top_p=0.99).tolist() == [want]
+    with pytest.raises(ValueError, match='vocab'):
+        sample(torch.zeros(1, (1 << 22) + 1, device=cuda), u.to(cuda))
+
+
+def test_keeping_nothing_empties_the_cache(cuda):
+    c, _, _ = build(cuda, RAGGED, 2)
+    c.mass()
+    new = c.evict(0)
+    assert new.seen == [0] and new.kept.shape == (1, 2, 0) and new.dropped == c.seen[0]
+    q, kn, vn = (t[None].to(cuda) for t in chunk_of(2, 6, 3, 8))
+    assert new.append(kn, vn, 0) == 0
+    out = new.attend_sparse(q, kn, vn, 0, 0, 4, out_dtype=torch.float32)
+    ref = sparse.expected(q[0].cpu(), kn[0].float().cpu(), vn[0].float().cpu(), 0, torch.zeros(2, 3, 0, dtype=torch.bool))
+    assert ((out[0].cpu().double() - ref).abs() <= sparse.tolerance(ref, vn.cpu(), torch.float32, 'bf16')).all()
+
+
 def test_two_streams_draw_at_once(cuda):
     rows = [sampling.rows_of(4, 49280, torch.bfloat16, 40 + i) for i in range(4)]
     rows = [(x.to(cuda), u.to(cuda)) for x, u in rows]
