@@ -165,14 +165,14 @@ struct __attribute__((packed, aligned(8))) Bytes16 {
 };
 __device__ __forceinline__ void load_any(const UnitRows& u, int row, int g, KeyPiece& p) {
   const int r = row < u.rows ? row : 0;
-  const uint8_t* at = u.k + r * u.k_stride + g * 2 * u.bits;
+  const uint8_t* at = u.k + (__umul24(r, u.k_stride) + g * 2 * u.bits);
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const u32x4 x = reinterpret_cast<const Bytes16*>(at + (u.bits == 16 ? 16 * i : 0))->x;
 #pragma unroll
     for (int j = 0; j < 4; ++j) p.w[4 * i + j] = x[j];
   }
-  p.as = *reinterpret_cast<const float2*>(u.bits == 16 ? u.k : u.k + (int64_t)u.rows * (8 * u.bits) + 8 * r);
+  p.as = *reinterpret_cast<const float2*>(u.k + (u.bits == 16 ? 0 : u.rows * (8 * u.bits) + 8 * r));
 }
 
 // 16 sums a lane, [b][i] of key 16 b + 4 g + i, over the 16 lanes of a group: each lane ends with one key's, which it

@@ -35,7 +35,7 @@ __device__ __forceinline__ f32x4 mfma(const Op& a, const Op& b, f32x4 c) {
 struct UnitRows {
   const uint8_t* k;
   const uint8_t* v;
-  int64_t k_stride, v_stride;  // bytes from row to row
+  uint32_t k_stride, v_stride;  // bytes from row to row, below 2^24: a row's offset is a 24-bit product (a 64-bit one is four slow ones)
   int bits, rows, low, high;
 };
 
@@ -63,8 +63,8 @@ __device__ __forceinline__ UnitRows chunk_rows(const dkv_attn_args& a, int piece
   u.high = u.rows;
   u.k = static_cast<const uint8_t*>(a.k_new) + 2 * (h * a.kn_head_stride + first * a.kn_tok_stride);
   u.v = static_cast<const uint8_t*>(a.v_new) + 2 * (h * a.vn_head_stride + first * a.vn_tok_stride);
-  u.k_stride = 2 * a.kn_tok_stride;
-  u.v_stride = 2 * a.vn_tok_stride;
+  u.k_stride = (uint32_t)(2 * a.kn_tok_stride);  // (of a single row, whatever it is)
+  u.v_stride = (uint32_t)(2 * a.vn_tok_stride);
   return u;
 }
 
@@ -113,7 +113,7 @@ struct KeyPiece {
 template <int BITS>
 __device__ __forceinline__ void load_key(const UnitRows& u, int row, int g, KeyPiece& p) {
   const int r = row < u.rows ? row : 0;
-  const uint8_t* at = u.k + r * u.k_stride + g * 2 * BITS;
+  const uint8_t* at = u.k + (__umul24(r, u.k_stride) + g * 2 * BITS);
   if (BITS == 4) {
     const u32x2 x = *reinterpret_cast<const u32x2*>(at);
     p.w[0] = x[0], p.w[1] = x[1];
@@ -125,7 +125,7 @@ __device__ __forceinline__ void load_key(const UnitRows& u, int row, int g, KeyP
       for (int j = 0; j < 4; ++j) p.w[4 * i + j] = x[j];
     }
   }
-  if (BITS < 16) p.as = *reinterpret_cast<const float2*>(u.k + (int64_t)u.rows * (8 * BITS) + 8 * r);
+  if (BITS < 16) p.as = *reinterpret_cast<const float2*>(u.k + (u.rows * (8 * BITS) + 8 * r));
 }
 
 // The operands of a key: elements 16 g + 8 half + [0, 8).
@@ -148,7 +148,7 @@ __device__ __forceinline__ void load_scales(const uint8_t* base, int rows, int g
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int row = 16 * b + 4 * g + 2 * i;
-      as[b][i] = *reinterpret_cast<const f32x4*>(base + (int64_t)rows * (8 * BITS) + 8 * (row < rows ? row : 0));
+      as[b][i] = *reinterpret_cast<const f32x4*>(base + (rows * (8 * BITS) + 8 * (row < rows ? row : 0)));
     }
 }
 
@@ -198,7 +198,7 @@ __device__ __forceinline__ void load_values(const UnitRows& u, int c, int g, Val
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int row = 16 * b + 4 * g + i, r = row < u.rows ? row : 0;
-      const uint8_t* at = u.v + r * u.v_stride;
+      const uint8_t* at = u.v + __umul24(r, u.v_stride);
       if (BITS == 4) {
         p.w[b][i][0] = *reinterpret_cast<const uint16_t*>(at + 2 * c);
       } else if (BITS == 8) {
@@ -211,11 +211,9 @@ __device__ __forceinline__ void load_values(const UnitRows& u, int c, int g, Val
     }
 }
 
-// The operands of output block db: keys 16 (2 step + j / 4) + 4 g + j % 4. Rows that are not visible give zeros, so that
-// what they hold (NaN or infinity in a masked row) meets no p of zero.
+// The operands of output block db: keys 16 (2 step + j / 4) + 4 g + j % 4.
 template <int BITS, int PREC>
-__device__ __forceinline__ void value_ops(const UnitRows& u, const ValuePiece<BITS>& p, const f32x4 (&as)[4][2], int g, int db,
-                                          bool whole, Op (&op)[2]) {
+__device__ __forceinline__ void value_ops(const ValuePiece<BITS>& p, const f32x4 (&as)[4][2], int db, Op (&op)[2]) {
 #pragma unroll
   for (int b = 0; b < 4; ++b)
 #pragma unroll
@@ -227,10 +225,6 @@ __device__ __forceinline__ void value_ops(const UnitRows& u, const ValuePiece<BI
       } else {
         const f32x4 m = as[b][i / 2];
         t = unpack_pair<BITS, PREC>(code_at<BITS>(p.w[b][i], db), code_at<BITS>(p.w[b][i + 1], db), m[1], m[0], m[3], m[2]);
-      }
-      if (!whole) {
-        const int row = 16 * b + 4 * g + i;
-        t &= (row >= u.low && row < u.high ? 0xffffu : 0u) | (row + 1 >= u.low && row + 1 < u.high ? 0xffff0000u : 0u);
       }
       op[b / 2].u[2 * (b % 2) + i / 2] = t;
     }

@@ -10,10 +10,10 @@
 // over workgroups. Nothing of the history but the index, the chosen tiles and the tail is read.
 //
 // Measured (kernel times, 5 KV heads of 3 query heads unless said): a token past 8128 near 6.6, attention 7.8, merge
-// 3.1 us, 16.6 us a call; a token past 131007 with 8 KV heads of 4 scores 4.6, choice 5.8, attention 7.8, merge 4.4, 21.6
-// a call: latency, each launch a few dependent loads. 64 queries past 32704: 10.3 + 36.6 + 4.8, 48.4 a call; 513 queries
-// past 20011 at fp32, 3 KV heads of 3: 22.4 + 8.4 + 136, 159 a call: every query walks some 30 tiles of its own, 400 MB
-// through L2 at 3 TB/s, of whose 16 MFMA rows three are its query heads.
+// 3.1 us, 16.6 us a call; a token past 131007 with 8 KV heads of 4 scores 4.6, choice 5.8, attention 6.5, merge 4.4, 19.9
+// a call: latency, each launch a few dependent loads. 64 queries past 32704: 10.3 + 30.4 + 4.1, 42.2 a call; 513 queries
+// past 20011 at fp32, 3 KV heads of 3: 22.4 + 8.4 + 101, 122 a call: every query walks some 30 tiles of its own and unpacks
+// them, for three of 16 MFMA rows; the unpacking and the softmax keep the VALU busy, not the 400 MB from L2.
 #include "dkv_rows.h"
 #include "dkv_select.h"
 
@@ -303,17 +303,27 @@ __device__ __forceinline__ void attend_unit(const UnitRows& u, const Op (&q)[2],
     s[b] = mfma(k[1], q[1], mfma(k[0], q[0], f32x4{0, 0, 0, 0}));
   }
   if constexpr (AFFINE<BITS, PREC>) affine_scores<BITS>(k_as, q_sum, s);
-  const bool whole = u.low == 0 && u.high == TILE;
+  if (!__builtin_amdgcn_readfirstlane(u.low == 0 && u.high == TILE)) {
+    // (A branch: masks of every element beside 64-bit row offsets took 136 us against 101, 513 queries past 20011.) Rows that are not visible: no score, and values of zero, so that what they hold (NaN or infinity) meets no p of zero.
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = 16 * b + 4 * g + i;
+        const bool seen = row >= u.low && row < u.high;
+        s[b][i] = seen ? s[b][i] : -INFINITY;
+#pragma unroll
+        for (int j = 0; j < (BITS == 16 ? 2 : 1); ++j) vp.w[b][i][j] = seen ? vp.w[b][i][j] : 0u;
+        if (BITS < 16)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) v_as[b][i / 2][2 * (i % 2) + j] = seen ? v_as[b][i / 2][2 * (i % 2) + j] : 0.f;
+      }
+  }
   float top = -INFINITY;
 #pragma unroll
   for (int b = 0; b < 4; ++b)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int row = 16 * b + 4 * g + i;
-      if (!whole && !(row >= u.low && row < u.high)) {
-        s[b][i] = -INFINITY;
-        if (AFFINE<BITS, PREC>) v_as[b][i / 2][2 * (i % 2)] = v_as[b][i / 2][2 * (i % 2) + 1] = 0.f;
-      }
       s[b][i] *= scale2;
       top = fmaxf(top, s[b][i]);
     }
@@ -345,7 +355,7 @@ __device__ __forceinline__ void attend_unit(const UnitRows& u, const Op (&q)[2],
 #pragma unroll
   for (int db = 0; db < 4; ++db) {
     Op v[2];
-    value_ops<BITS, PREC>(u, vp, v_as, g, db, whole, v);
+    value_ops<BITS, PREC>(vp, v_as, db, v);
     f32x4 o = r.o[db] * alpha;
 #pragma unroll
     for (int t = TERMS - 1; t >= 0; --t) o = mfma(v[1], p[t][1], mfma(v[0], p[t][0], o));
@@ -400,7 +410,7 @@ __global__ __launch_bounds__(256) void attend_kernel(dkv_attn_args a, dkv_sparse
       u = tile_rows(a, t, v.past, h);
       if (i >= own_tile) {
         u.rows = u.high = min(TILE, v.single_rows - TILE * (i - own_tile));
-        u.k_stride = u.v_stride = slab_bytes(1, 16, a.layers, a.heads);
+        u.k_stride = u.v_stride = (uint32_t)slab_bytes(1, 16, a.layers, a.heads);
       }
       t = tile_at(i + 4 * splits);  // the next unit's, while this one is computed
     } else {
@@ -520,6 +530,8 @@ int check_history_args(const dkv_attn_args& a, const char* what) {
   } else if (!a16(a.q) || !a16(a.k_new) || (a.q_head_stride & 7) || (a.q_tok_stride & 7) || (a.kn_head_stride & 7) ||
              (a.kn_tok_stride & 7)) {
     set_error("%s: Q and K must be 16-byte aligned with strides that are multiples of 8 elements", what);
+  } else if (a.nq > 1 && (a.kn_tok_stride < 0 || a.kn_tok_stride >= 1 << 23)) {
+    set_error("%s: K's token stride must be from 0 to 2^23 - 1 elements", what);
   } else {
     if (a.n_segs <= 1) return 0;
     bool ok = a.seg_bounds[0] == 0 && a.seg_bounds[a.n_segs] == a.nq;
@@ -584,6 +596,10 @@ int dkv_attend_sparse(const dkv_attn_args* args, const dkv_sparse* sparse, void*
   if (s.n_indexed < 0 || s.blocks < 0 || s.single_rows < 0 || (s.n_indexed > 0 && (!s.bounds || ((uintptr_t)s.bounds & 15)))) {
     set_error("dkv_attend_sparse: n_indexed %d, blocks %d and single_rows %d must not be negative, bounds 16-byte aligned", s.n_indexed,
               s.blocks, s.single_rows);
+    return DKV_EINVAL;
+  }
+  if ((a.nq > 1 && (a.vn_tok_stride < 0 || a.vn_tok_stride >= 1 << 23)) || (int64_t)a.layers * a.heads > 65535) {
+    set_error("dkv_attend_sparse: V's token stride must be from 0 to 2^23 - 1 elements, layers * heads at most 65535");
     return DKV_EINVAL;
   }
   if (a.nq > 65535) {

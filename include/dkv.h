@@ -412,7 +412,9 @@ typedef struct dkv_sparse {
  * {past, n_tiles, n_indexed, single_rows}, the first three within the arguments'
  * values.
  * `precision` as in dkv_attend, but p is never rounded below 16 bits. With
- * blocks >= n_indexed the call is dense attention. At most 65535 queries. */
+ * blocks >= n_indexed the call is dense attention. At most 65535 queries; rows
+ * of k_new and v_new are less than 2^23 elements apart (dkv_attention_mass too),
+ * layers * heads is at most 65535. */
 int64_t dkv_attend_sparse_workspace_bytes(const dkv_attn_args* args, const dkv_sparse* sparse);
 int dkv_attend_sparse(const dkv_attn_args* args, const dkv_sparse* sparse, void* stream);
 

@@ -248,6 +248,30 @@ def test_keeping_nothing_empties_the_cache(cuda):
     assert ((out[0].cpu().double() - ref).abs() <= sparse.tolerance(ref, vn.cpu(), torch.float32, 'bf16')).all()
 
 
+def test_token_strides_at_their_border(cuda):
+    """A chunk's rows up to 2^23 - 8 elements apart are read where they lie; a larger stride is refused, but of one row."""
+    c, dk, dv = build(cuda, RAGGED, 1)
+    c.index()
+    past = c.seen[0]
+    q, kn, vn = (t[None].to(cuda) for t in chunk_of(1, 3, 2, 9))
+    want, mass = c.attend_sparse(q, kn, vn, 0, past, 3), c.attention_mass(q, kn, 0, past)
+    for stride in ((1 << 23) - 8, 1 << 23):
+        far = torch.zeros(2 * stride, dtype=torch.bfloat16, device=cuda).as_strided((1, 1, 2, 64), (0, 0, stride, 1))
+        for x in (kn, vn):
+            far.copy_(x)
+            k, v = (far, vn) if x is kn else (kn, far)
+            if stride < 1 << 23:
+                assert torch.equal(c.attend_sparse(q, k, v, 0, past, 3), want)
+                assert torch.equal(c.attention_mass(q, k, 0, past), mass)
+            else:
+                with pytest.raises(ValueError, match='token stride'):
+                    c.attend_sparse(q, k, v, 0, past, 3)
+        one = c.attend_sparse(q[:, :, :1], far[:, :, :1], vn[:, :, :1], 0, past, 3)
+        assert torch.equal(one, c.attend_sparse(q[:, :, :1], vn[:, :, :1], vn[:, :, :1], 0, past, 3))
+    with pytest.raises(ValueError, match='token stride'):
+        c.attention_mass(q, far, 0, past)
+
+
 def test_two_streams_draw_at_once(cuda):
     rows = [sampling.rows_of(4, 49280, torch.bfloat16, 40 + i) for i in range(4)]
     rows = [(x.to(cuda), u.to(cuda)) for x, u in rows]
