@@ -9,8 +9,8 @@
 // index is short (near_kernel), in two where it is long, then the attention, and a merge where a query's tiles are split
 // over workgroups. Nothing of the history but the index, the chosen tiles and the tail is read.
 //
-// Measured (kernel times, 5 KV heads of 3 query heads unless said): a token past 8128 near 6.6, attention 7.8, merge
-// 3.1 us, 16.6 us a call; a token past 131007 with 8 KV heads of 4 scores 4.6, choice 5.8, attention 6.5, merge 4.4, 19.9
+// Measured (kernel times, 5 KV heads of 3 query heads unless said): a token past 8128 near 6.5, attention 6.2, merge
+// 3.0 us, 16.7 us a call; a token past 131007 with 8 KV heads of 4 scores 4.4, choice 5.7, attention 6.2, merge 4.0, 20.3
 // a call: latency, each launch a few dependent loads. 64 queries past 32704: 10.3 + 30.4 + 4.1, 42.2 a call; 513 queries
 // past 20011 at fp32, 3 KV heads of 3: 22.4 + 8.4 + 101, 122 a call: every query walks some 30 tiles of its own and unpacks
 // them, for three of 16 MFMA rows; the unpacking and the softmax keep the VALU busy, not the 400 MB from L2.
