@@ -724,12 +724,13 @@ __device__ __forceinline__ int kept_of(DrawScratch& s, const Row<T>& r, const We
 
 // Where a filter cuts the bin whose n tokens are listed: after the token at which their weight, `sum` before them,
 // reaches `need`, after `rank` of them, or where w < min_p (min_step: the step of that, if it is in this bin). Only the
-// tokens of one step are ranked.
+// tokens of one step are ranked. The cut is never looser than `within`: a step at which min_p cuts may lie below it.
 template <class T>
 __device__ __forceinline__ Cut cut_bin_at(DrawScratch& s, const Row<T>& r, const Weigher& weigher, int bin, int n, const Cut& within,
                                           uint64_t sum, uint64_t need, int64_t rank, double min_p, int min_step) {
   auto sub_of = [&](uint64_t token) { return SUBS - 1 - (weigher.step(logit_of(key_of(token))) & (SUBS - 1)); };
   auto takes = [&](uint64_t token) { return within.takes(key_of(token), index_of(token)); };
+  auto above = [&](uint32_t key) { return key < within.key ? within : Cut{key, -1}; };  // the keys above `key` that `within` takes
   __syncthreads();
   if (threadIdx.x < SUBS) s.sub_mass[threadIdx.x] = 0, s.sub_count[threadIdx.x] = 0;
   if (threadIdx.x == 0) s.n = 0, s.sub = SUBS;
@@ -752,7 +753,7 @@ __device__ __forceinline__ Cut cut_bin_at(DrawScratch& s, const Row<T>& r, const
   }
   __syncthreads();
   const int sub = s.sub;
-  if (sub == SUBS) return Cut{weigher.first_key(weigher.bin_step(bin)) - 1, -1};  // (sums a few units short: all of it)
+  if (sub == SUBS) return above(weigher.first_key(weigher.bin_step(bin)) - 1);  // (sums a few units short: all of it)
   for (int i = threadIdx.x; i < n; i += THREADS) {
     const uint64_t token = s.list[i];
     if (takes(token) && sub_of(token) == sub) s.few[atomicAdd(&s.n, 1)] = token;
@@ -762,7 +763,7 @@ __device__ __forceinline__ Cut cut_bin_at(DrawScratch& s, const Row<T>& r, const
   rank_few(s, few, [](uint64_t x) { return x; });
   const int keep = kept_of(s, r, weigher, few, rank - s.sub_rank, s.sub_before, need, min_p);
   if (keep) return Cut{key_of(s.few[keep - 1]), index_of(s.few[keep - 1])};
-  return Cut{few ? key_of(s.few[0]) : weigher.first_key(weigher.bin_step(bin) + SUBS - sub) - 1, -1};
+  return above(few ? key_of(s.few[0]) : weigher.first_key(weigher.bin_step(bin) + SUBS - sub) - 1);
 }
 
 // A row whose parts listed what the first top_k can be among: all of it from the lists.
