@@ -910,18 +910,24 @@ __global__ __launch_bounds__(THREADS) void draw_kernel(Args a, Work work) {
   const int part = __ffsll((unsigned long long)__ballot(parts_upto > target)) - 1;
   target -= shfl64(parts_upto, part) - s.part_mass[part];
 
-  // the part, in order: a consecutive run of tokens a thread
+  // The part, in order: a consecutive run of tokens a thread. Weights in the part's own unit, in which its bins hold their
+  // sums: tokens lighter than the row's unit, a few of which can make the part's mass, are none there.
   const int from = part * a.part_len, to = min(a.vocab, from + a.part_len), run = (to - from + THREADS - 1) / THREADS;
   const int begin = min(to, from + (int)threadIdx.x * run), end = min(to, begin + run);
+  const int apart = apart_of(t.exponent, s.exponents[part]);  // (at most `shift`, as the part has mass)
+  const Weigher inside(s.table, r.temperature, a.shift, s.exponents[part]);
   auto kept = [&](int i, float x) -> uint64_t {
-    const uint32_t key = order_key(x);
-    return cut.takes(key, i) ? weigher.weight(x) : 0;
+    if (!cut.takes(order_key(x), i)) return 0;
+    int bin;
+    const uint64_t w = inside.weight(x, bin);
+    return bin + OCTAVE * apart <= OCTAVE * a.shift ? w : 0;  // (of the row's bins, as the part's mass)
   };
   uint64_t sum = 0, all;
   r.template each<8, 1>(begin, end, [&](int i, float x) { sum += kept(i, x); });
   uint64_t passed = block_scan<THREADS / 64>(s.bins.sums, sum, all);
-  // (bins' sums were rounded down once, tokens' one by one: their total may be a few units short)
-  if (target >= all) target = all - 1;
+  // The part's mass is each bin's sum rounded down to the row's unit, so `all` is that many units or a few more: they go
+  // to the last one.
+  target = target + 1 == s.part_mass[part] ? all - 1 : target << apart;
   if (target >= passed || target < passed - sum) return;
   passed -= sum;
   int token = -1;

@@ -1,4 +1,5 @@
-"""sample where two filters cut the same bin of weights."""
+"""sample where two filters cut the same bin of weights, and where the target lies among the lightest tokens that a sum
+still counts."""
 import math
 
 import pytest
@@ -9,6 +10,8 @@ from dkv import gpu_ops
 from test_gpu_sample import check, drawn
 
 pytestmark = pytest.mark.gpu
+
+NEAR_ONE = 1 - 2.0 ** -53
 
 
 def close_rows(rows, vocab, step, seed):
@@ -55,3 +58,51 @@ def test_rank_and_min_p_per_row(cuda):
         us = torch.full((6,), u)
         out = gpu_ops.sample(x.to(cuda), us.to(cuda), 1.0, k.to(cuda), p.to(cuda), m.to(cuda)).tolist()
         assert out == [drawn(x[i], us[i].double().item(), 1.0, int(k[i]), p[i].item(), m[i].item()) for i in range(6)]
+
+
+class Marked:
+    """torch, whose empty int64 tensors hold a mark, so that a result nobody wrote shows."""
+    MARK = -7
+
+    def __getattr__(self, name):
+        return getattr(torch, name)
+
+    @staticmethod
+    def empty(*args, **kw):
+        x = torch.empty(*args, **kw)
+        return x.fill_(Marked.MARK) if kw.get('dtype') is torch.int64 else x
+
+
+@pytest.mark.parametrize('vocab,shift', [(8192, 48), (49280, 46), (131071, 45)])
+@pytest.mark.parametrize('below', [-0.0009, 0.0, 0.0009, -0.4])
+def test_target_among_the_lightest_tokens(cuda, vocab, shift, below, monkeypatch):
+    """One logit at the top, the last 2048 at the weight that one unit of the sums has or `below` it, and a random
+    number so near to one that it lies in their weight: the token is one that may be drawn. A sum counts in units of
+    2^-shift of twice the largest weight, a border may lie as many of them off as there are tokens and bins' sums
+    (64 parts of 401); where they are not lighter than a unit or about it, it is the last of them."""
+    announce(f'sample, lightest tokens: vocab={vocab} below={below}')
+    monkeypatch.setattr(gpu_ops, 'torch', Marked())
+    x = torch.full((1, vocab), -math.inf)
+    x[0, 5] = 0.0
+    x[0, -2048:] = (1 - shift + below) * math.log(2)
+    for u in (1.0, NEAR_ONE, 1 - 2.0 ** -40):
+        for kw in (dict(), dict(top_p=1 - 2.0 ** -50), dict(min_p=1e-30), dict(top_k=1000), dict(top_k=3000), dict(top_k=100)):
+            out = gpu_ops.sample(x.to(cuda), torch.tensor([u], dtype=torch.float64, device=cuda), **kw).tolist()
+            if out[0] == Marked.MARK:
+                pytest.fail(f'no token written: u={u} {kw}')
+            assert out[0] == 5 or out[0] >= vocab - 2048, (u, kw)
+            if u == 1 and below >= 0 and not kw:
+                assert out[0] == vocab - 1, (u, kw)
+
+
+@pytest.mark.parametrize('vocab', [8192, 49280, 131071])
+def test_one_is_the_last_token_that_counts(cuda, vocab):
+    """u of one over tokens at every distance from the largest, in parts far apart: the last one with weight."""
+    announce(f'sample, u = 1: vocab={vocab}')
+    x = torch.full((1, vocab), -math.inf)
+    x[0, 0] = 0.0
+    for at, low in ((vocab - 1, -20.0), (vocab // 2, -25.0), (vocab - 3000, -28.0), (vocab - 7, 0.0)):
+        y = x.clone()
+        y[0, at] = low
+        got = gpu_ops.sample(y.to(cuda), torch.ones(1, dtype=torch.float64, device=cuda)).tolist()
+        assert got == [at]
