@@ -4,10 +4,14 @@
 // top_k, of those the shortest run that holds top_p of their weight, of those the ones with w >= min_p; then the
 // first token, in the vocabulary's order, up to which the kept weight exceeds u times its total.
 //
-// Weights are computed in 64 bits and summed as integers, multiples of 2^-SHIFT of a power of two above the largest:
-// such sums are exact and the same in every order, so neither atomics nor the split of a row into parts can move a
-// border between two tokens. SHIFT leaves room for a whole vocabulary's sum (40 for 4 million tokens, 46 for 49280);
-// what is lighter counts as nothing.
+// Weights are computed in 64 bits and summed as integers, multiples of a unit: 2^-SHIFT of a power of two above the row's
+// largest weight, at most twice that weight. Integer sums are the same in every order, so no order of the atomics moves a
+// border between two tokens. SHIFT leaves room for a whole vocabulary's sum (40 for 4 million tokens, 46 for 49280); what
+// is lighter counts as nothing. A weight is rounded to the unit of its part, which may be finer than the row's, and a
+// part's sums by bins (at most 401) to the row's when they are joined, down each time. So a border lies less than
+// vocab + 401 * parts units from where exact sums have it (1.7e-9 of the largest weight at 49280 tokens in 25 parts), and
+// as the parts follow from the number of rows, a row whose random number is as near to a border as that may give the
+// neighbouring token in a batch of another size.
 //
 // weigh_kernel: many workgroups a row, each over a part of the vocabulary, sum its weights by bins, eight an octave, so
 // that a bin's tokens are consecutive in the order of the logits. A workgroup alone gets some 30 GB/s from memory that

@@ -478,8 +478,12 @@ int dkv_evict(const dkv_evict_args* args, void* stream);
  * fp32 (u_dtype 0) or fp64 (1), clamped to [0, 1]. A parameter's *_rows, if not
  * NULL, gives it for each row (device memory, not checked: a top_p below or above
  * its range is clamped, a negative top_k is 0, a negative temperature 0). At most
- * 2^22 tokens. Sums are exact integers: the token does not depend on the order of
- * any sum. No counterpart in the reference, which scores given answers only. */
+ * 2^22 tokens. Sums are integers: calls alike give the same token whatever order
+ * the sums are taken in. Their unit is at most 2^(1 - s) of the row's largest
+ * weight, with s the largest number up to 50 for which vocab < 2^(62 - s); a border
+ * between two tokens lies less than vocab + 25664 units from where the weights have
+ * it, and within that the token may depend on the number of rows of the call. No
+ * counterpart in the reference, which scores given answers only. */
 typedef struct dkv_sampling {
   double temperature, top_p, min_p;
   int32_t top_k;

@@ -106,3 +106,16 @@ def test_one_is_the_last_token_that_counts(cuda, vocab):
         y[0, at] = low
         got = gpu_ops.sample(y.to(cuda), torch.ones(1, dtype=torch.float64, device=cuda)).tolist()
         assert got == [at]
+
+
+@pytest.mark.parametrize('kw', [dict(), dict(top_p=0.9), dict(top_k=500, min_p=1e-4), dict(top_k=50, top_p=0.95)],
+                         ids=lambda kw: '-'.join(kw) or 'none')
+def test_batches_of_other_sizes(cuda, kw):
+    """Rows cut into other parts by the size of their batch: the same tokens, as none of these random numbers is within
+    the sums' rounding of a border."""
+    announce(f'sample, batch sizes: {kw}')
+    g = torch.Generator().manual_seed(21)
+    x, u = (torch.randn(700, 20011, generator=g) * 2.5).to(cuda), torch.rand(700, generator=g).to(cuda)
+    whole = gpu_ops.sample(x, u, **kw)
+    for rows in (1, 3, 40, 300):
+        assert torch.equal(gpu_ops.sample(x[:rows], u[:rows], **kw), whole[:rows])
