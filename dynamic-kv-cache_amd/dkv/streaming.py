@@ -415,8 +415,9 @@ class StreamingDecoder:
         """Continues the question on a fork: one token for each random number of u [n] (gpu_ops.sample: fp32
         or fp64, on the decoder's device), int64 [n]. With `blocks` the question and every token attend to the
         tiles of the history that score highest for them, that many each, and to all that came after the
-        question (GPUCache.attend_sparse; the cache's index is brought up to date first). Nothing waits for
-        the GPU, so a caller that stops at a token looks for it afterwards."""
+        question (GPUCache.attend_sparse; the cache's index is brought up to date first). From a row without a
+        token that can be drawn on the tokens are -1. Nothing waits for the GPU, so a caller that stops at a
+        token looks for it afterwards."""
         if u.dim() != 1:
             raise ValueError('generate expects one random number a token, u [n]')
         if blocks:
@@ -426,8 +427,11 @@ class StreamingDecoder:
         for i in range(u.shape[0]):
             logits = self._fork_forward(branch, ids, 1)[0]
             tokens.append(sample(logits, u[i:i + 1], temperature, top_k, top_p, min_p))
-            ids = tokens[-1][None]
-        return torch.cat(tokens) if tokens else u.new_empty(0, dtype=torch.int64)
+            ids = tokens[-1][None].clamp(min=0)  # (-1 is no index into the embeddings)
+        if not tokens:
+            return u.new_empty(0, dtype=torch.int64)
+        out = torch.cat(tokens)
+        return out.masked_fill((out < 0).cumsum(0) > 0, -1)
 
     @torch.inference_mode()
     def answer(self, cache, question_ids, candidates):
