@@ -143,7 +143,9 @@ class StreamingDecoder:
         frame is counted, and before a frame that would pass the budget the tokens of the least attention
         mass are evicted (GPUCache.evict), down to three quarters of the budget or to what the frame needs;
         the prefix and the last quarter of the budget stay. The cache that is returned holds the history: with
-        a budget it may be another one than the `cache` given.
+        a budget it may be another one than the `cache` given, which then holds what it did before the first
+        eviction, for its forks too. (With graphs=True the decoder's own cache evicts into another one that
+        the decoder keeps, and that one back: as between requests, forks of either end there.)
         """
         if len(frames) != len(bits):
             raise ValueError('one bit width per frame')
@@ -153,6 +155,7 @@ class StreamingDecoder:
                 raise ValueError(f'a budget of {budget} tokens does not hold the prefix of {prefix_ids.shape[1]}')
             total = min(total, budget)
         total += qa_reserve
+        given = cache
         if cache is None:
             cache = self._reused_cache(total) if self.graphs else self.create_cache(total)
         # pipelined frames share the GPU: their frame-chunk attention takes fewer history splits
@@ -162,28 +165,29 @@ class StreamingDecoder:
         caches = [cache]
         try:
             cache.chunk_splits, cache.observing = splits, budget is not None
-            return self._ingest_chunks(caches, prefix_ids, frames, bits, budget)
+            return self._ingest_chunks(caches, given, prefix_ids, frames, bits, budget)
         finally:
             for c in caches:
                 c.chunk_splits, c.observing = 0, False
 
-    def _evict_for(self, caches, budget, frame, prefix):
-        """Room for a frame within the budget: the last of `caches` evicts into the one before it (or a new
-        one), which goes to the end of the list and is returned."""
+    def _evict_for(self, caches, given, budget, frame, prefix):
+        """Room for a frame within the budget: the last of `caches` (those of this ingest) evicts into another of
+        them, never the `given` one, or into a new one. That goes to the end of the list and is returned."""
         cache = caches[-1]
         keep = min(budget - budget // 4, budget - frame)
         own = self.graphs and cache is self._cache
-        into = caches[-2] if len(caches) > 1 else None
         if own:
             if self._spare is None or self._spare[0].capacity < cache.capacity:
                 self._spare = (self.create_cache(cache.capacity), {}, {}, {}, set())
             into = self._spare[0]
+        else:
+            into = next((c for c in caches if c is not cache and c is not given), None)
         new = cache.evict(keep, sinks=prefix, recent=budget // 4, into=into)
         new.chunk_splits, new.observing = cache.chunk_splits, cache.observing
         if own:  # captured forwards stay with the cache whose buffers they recorded
             (self._cache, self._graphs, self._group_graphs, self._qa_graphs, self._qa_seen), self._spare = \
                 self._spare, (cache, self._graphs, self._group_graphs, self._qa_graphs, self._qa_seen)
-        caches[:] = [cache, new]
+        caches[:] = [c for c in caches if c is not new] + [new]
         return new
 
     @staticmethod
@@ -191,7 +195,7 @@ class StreamingDecoder:
         """Key of a captured forward: one that counts attention records other launches."""
         return key + ('observing',) if cache.observing else key if len(key) > 1 else key[0]
 
-    def _ingest_chunks(self, caches, prefix_ids, frames, bits, budget):
+    def _ingest_chunks(self, caches, given, prefix_ids, frames, bits, budget):
         cache = caches[-1]
         cache.select(16, -1)
         graphed = self.graphs and cache is self._cache
@@ -210,7 +214,7 @@ class StreamingDecoder:
             n, most = emb.shape[1], self.pipeline
             if budget is not None:
                 if cache.get_seq_length() + n > budget:
-                    cache = self._evict_for(caches, budget, n, prefix_ids.shape[1])
+                    cache = self._evict_for(caches, given, budget, n, prefix_ids.shape[1])
                 most = min(most, (budget - cache.get_seq_length()) // n)
             k = 1
             while k < most and i + k < len(frames) and frames[i + k].shape[1] == n:

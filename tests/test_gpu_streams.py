@@ -22,3 +22,26 @@ def test_logits_that_are_not_numbers(cuda, graphs):
     assert dec.generate(cache, question, u.cuda(), **SAMPLING).tolist() == [-1] * 12
     norm.data.fill_(1.0)
     assert min(dec.generate(cache, question, u.cuda(), **SAMPLING).tolist()) >= 0
+
+
+def test_forks_of_a_caller_s_cache_keep_their_rows(cuda):
+    """A budgeted ingest on a cache that has a fork, over several evictions; and one on the fork itself."""
+    announce('budgeted ingest on a forked cache')
+    model = build_decoder(**SMALL, seed=11)
+    dec = StreamingDecoder(model)
+    prefix, question, u = inputs(12)
+    frames, bits = frames_for(model, 20, seed=13), [4, 8, 16, 4, 8] * 4
+    cache = dec.create_cache(700)
+    dec.forward(cache, ids=prefix)
+    fork = cache.fork()
+    dec.forward(fork.fork(), ids=question)
+
+    def rows(c):
+        return [x.clone() for l in range(SMALL['layers']) for x in c.materialize(l)]
+    held = rows(fork)
+    out = dec.ingest(prefix[:, :1], frames, bits, cache=cache, budget=300)
+    assert out is not cache and out.get_seq_length() + out.dropped == 16 + 1 + 20 * 64
+    assert all(torch.equal(a, b) for a, b in zip(rows(fork), held))
+    base = rows(cache)
+    again = dec.ingest(prefix[:, :1], frames, bits, cache=cache.fork(), budget=300)
+    assert again.get_seq_length() <= 300 and all(torch.equal(a, b) for a, b in zip(rows(cache), base))
