@@ -141,8 +141,11 @@ class StreamingDecoder:
 
         With a `budget` the history stays within that many tokens. The attention of the prefix and of every
         frame is counted, and before a frame that would pass the budget the tokens of the least attention
-        mass are evicted (GPUCache.evict), down to three quarters of the budget or to what the frame needs;
-        the prefix and the last quarter of the budget stay. The cache that is returned holds the history: with
+        mass are evicted (GPUCache.evict), down to three quarters of the budget (where the prefix fills
+        these, of what it leaves) or to what the frame needs. The prefix stays (where the cache held tokens
+        before, its first ones instead, as many), and of the frames that the last quarter of the budget takes
+        in the newest that leave room for it. A budget that some frame and the prefix use up is refused
+        before any forward. The cache that is returned holds the history: with
         a budget it may be another one than the `cache` given, which then holds what it did before the first
         eviction, for its forks too. (With graphs=True the decoder's own cache evicts into another one that
         the decoder keeps, and that one back: as between requests, forks of either end there.)
@@ -153,6 +156,7 @@ class StreamingDecoder:
         if budget is not None:
             if budget < prefix_ids.shape[1]:
                 raise ValueError(f'a budget of {budget} tokens does not hold the prefix of {prefix_ids.shape[1]}')
+            self._check_budget(budget, prefix_ids.shape[1], [f.shape[1] for f in frames], cache)
             total = min(total, budget)
         total += qa_reserve
         given = cache
@@ -170,11 +174,49 @@ class StreamingDecoder:
             for c in caches:
                 c.chunk_splits, c.observing = 0, False
 
+    @staticmethod
+    def _protected(cache, prefix):
+        """Tokens at the start of a cache that a budgeted ingest keeps: the segments of the first `prefix` ones."""
+        return next((s.end for s in cache.segments if s.end >= prefix), cache.get_seq_length()) if prefix else 0
+
+    @staticmethod
+    def _kept(budget, protected, frame):
+        """Tokens that an eviction before a frame leaves, of which `protected` stay."""
+        keep = budget - budget // 4
+        if keep <= protected:
+            keep = protected + (budget - protected) * 3 // 4
+        return min(keep, budget - frame)
+
+    def _check_budget(self, budget, prefix, frames, cache):
+        """Whether every eviction of an ingest leaves what is protected, and something beside it."""
+        held, protected = 0, prefix
+        if cache is not None:
+            if not cache.online:
+                raise ValueError('a budget needs an online cache (no plan)')
+            held = cache.get_seq_length()
+            protected = self._protected(cache, prefix) if held >= prefix else held + prefix
+        for n in [prefix] + frames:
+            if held + n > budget:
+                held = self._kept(budget, protected, n)
+                if held <= protected:
+                    raise ValueError(f'a budget of {budget} tokens holds no history beside {protected} protected tokens '
+                                     f'(the prefix) and {n} new ones')
+            held += n
+
     def _evict_for(self, caches, given, budget, frame, prefix):
         """Room for a frame within the budget: the last of `caches` (those of this ingest) evicts into another of
         them, never the `given` one, or into a new one. That goes to the end of the list and is returned."""
         cache = caches[-1]
-        keep = min(budget - budget // 4, budget - frame)
+        protected = self._protected(cache, prefix)
+        keep = self._kept(budget, protected, frame)
+        recent, tail = budget // 4, 0
+        for seg in reversed(cache.segments):  # whole segments stay: those that leave room for the protected ones
+            if tail >= recent:
+                break
+            if tail + seg.rows > keep - protected:
+                recent = tail
+                break
+            tail += seg.rows
         own = self.graphs and cache is self._cache
         if own:
             if self._spare is None or self._spare[0].capacity < cache.capacity:
@@ -182,7 +224,7 @@ class StreamingDecoder:
             into = self._spare[0]
         else:
             into = next((c for c in caches if c is not cache and c is not given), None)
-        new = cache.evict(keep, sinks=prefix, recent=budget // 4, into=into)
+        new = cache.evict(keep, sinks=prefix, recent=recent, into=into)
         new.chunk_splits, new.observing = cache.chunk_splits, cache.observing
         if own:  # captured forwards stay with the cache whose buffers they recorded
             (self._cache, self._graphs, self._group_graphs, self._qa_graphs, self._qa_seen), self._spare = \
@@ -197,6 +239,9 @@ class StreamingDecoder:
 
     def _ingest_chunks(self, caches, given, prefix_ids, frames, bits, budget):
         cache = caches[-1]
+        n = prefix_ids.shape[1]
+        if budget is not None and cache.get_seq_length() + n > budget:
+            cache = self._evict_for(caches, given, budget, n, n)
         cache.select(16, -1)
         graphed = self.graphs and cache is self._cache
         # The first request's prefix and first frame run eagerly (they warm up the library paths
@@ -215,7 +260,7 @@ class StreamingDecoder:
             if budget is not None:
                 if cache.get_seq_length() + n > budget:
                     cache = self._evict_for(caches, given, budget, n, prefix_ids.shape[1])
-                most = min(most, (budget - cache.get_seq_length()) // n)
+                most = min(most, (budget - cache.get_seq_length()) // max(n, 1))
             k = 1
             while k < most and i + k < len(frames) and frames[i + k].shape[1] == n:
                 k += 1

@@ -113,3 +113,59 @@ def test_evictions_take_turns_between_two_caches(hosted, monkeypatch):
     made.clear()
     hosted.ingest(prefix_of(16), *frames(*[64] * 30), cache=given, budget=300)
     assert len(made) == 2
+
+
+@pytest.mark.parametrize('budget,prefix,lengths', [
+    (256, 150, [64] * 8), (300, 150, [78] * 9), (464, 16, [64] * 20), (256, 200, [20] * 30), (256, 250, [5] * 9),
+    (256, 20, [100, 3, 90, 64, 1, 120, 78, 78, 200, 10]), (80, 16, [64, 8, 8, 8, 30]), (100, 60, [39] * 4), (1000, 1, [998] * 4)])
+def test_budgets_that_hold_the_prefix_and_a_frame(hosted, budget, prefix, lengths):
+    """Whatever the frames' lengths: the history never passes the budget, the prefix stays, and more than it."""
+    left = []
+    evict = GPUCache.evict
+
+    def spy(self, keep, **kw):
+        out = evict(self, keep, **kw)
+        left.append((out.segments[0].rows, out.seen[0]))
+        return out
+    GPUCache.evict = spy
+    try:
+        out = hosted.ingest(prefix_of(prefix), *frames(*lengths), budget=budget)
+    finally:
+        GPUCache.evict = evict
+    assert hosted.most <= budget and out.get_seq_length() + out.dropped == prefix + sum(lengths)
+    assert left and all(first == prefix and n > prefix for first, n in left)
+
+
+@pytest.mark.parametrize('budget,prefix,lengths', [
+    (80, 16, [64] * 6), (100, 60, [40, 10, 40]), (256, 150, [10, 106, 10]), (300, 150, [20, 151]), (64, 64, [1])])
+def test_budgets_that_do_not_are_refused_before_any_forward(hosted, budget, prefix, lengths):
+    cache = hosted.create_cache(2000)
+    before = state_of(cache)
+    with pytest.raises(ValueError, match='budget.*protected'):
+        hosted.ingest(prefix_of(prefix), *frames(*lengths), cache=cache, budget=budget)
+    assert state_of(cache) == before and not hasattr(hosted, 'most') and cache._mass is None
+    hosted.ingest(prefix_of(prefix), *frames(*lengths), cache=cache, budget=prefix + sum(lengths))  # (nothing is evicted)
+    with pytest.raises(ValueError, match='no plan'):
+        hosted.ingest(prefix_of(16), *frames(64), cache=GPUCache([(16, 300)], layers=2, heads=1, device='cpu'), budget=200)
+
+
+@pytest.mark.parametrize('budget,prefix', [(300, 16), (300, 100), (200, 30)])
+def test_a_stream_that_goes_on_stays_within_its_budget(hosted, budget, prefix):
+    """Ingests into the cache of the one before, whose first tokens stay: also the next prefix passes no budget."""
+    cache, total = None, 0
+    for n in (64, 50, 64):
+        cache = hosted.ingest(prefix_of(prefix), *frames(*[n] * 7), cache=cache, budget=budget, qa_reserve=100)
+        total += prefix + 7 * n
+        assert cache.get_seq_length() + cache.dropped == total and hosted.most <= budget
+        assert cache.segments[0].rows == prefix
+    with pytest.raises(ValueError, match='budget.*protected'):
+        hosted.ingest(prefix_of(prefix), *frames(budget - prefix), cache=cache, budget=budget)
+
+
+def test_the_newest_frames_that_leave_room_stay(hosted):
+    """The last quarter of the budget, whole frames: as many of the newest as fit beside the prefix."""
+    # 190 tokens, 150 of them to keep: 50 beside the prefix, one whole frame of the two in the quarter
+    one = hosted.ingest(prefix_of(100), *frames(30, 30, 30, 30), budget=200)
+    assert [s.rows for s in one.segments] == [100, 20, 30, 30]
+    two = hosted.ingest(prefix_of(10), *frames(30, 30, 30, 30, 30, 30, 30), budget=200)
+    assert [s.rows for s in two.segments] == [10, 80, 30, 30, 30]

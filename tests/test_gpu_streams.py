@@ -45,3 +45,23 @@ def test_forks_of_a_caller_s_cache_keep_their_rows(cuda):
     base = rows(cache)
     again = dec.ingest(prefix[:, :1], frames, bits, cache=cache.fork(), budget=300)
     assert again.get_seq_length() <= 300 and all(torch.equal(a, b) for a, b in zip(rows(cache), base))
+
+
+@pytest.mark.parametrize('graphs', [False, True])
+def test_a_prefix_of_half_the_budget(cuda, graphs):
+    """Frames above a quarter of a budget that the prefix half fills, and a stream that goes on: eager and replayed."""
+    announce(f'budget 300, prefix 150, frames of 78, graphs={graphs}')
+    model = build_decoder(**SMALL, seed=11)
+    frames, bits = frames_for(model, 9, seed=13, tokens=78), [4, 8, 16, 4, 8, 4, 4, 8, 16]
+    g = torch.Generator().manual_seed(1)
+    prefix = torch.randint(0, 512, (1, 150), generator=g)
+    states = []
+    for replay in {False, graphs}:
+        dec = StreamingDecoder(model, graphs=replay, pipeline=1)
+        for _ in range(2):
+            cache = dec.ingest(prefix, frames, bits, budget=300)
+            assert cache.get_seq_length() <= 300 and (cache.kept[:, :, :150] == torch.arange(150, device='cuda')).all()
+            states.append([cache.kept.clone(), cache.mass().clone(), *cache.materialize(1)])
+        cache = dec.ingest(prefix, frames[:4], bits[:4], cache=cache, budget=450)
+        assert cache.get_seq_length() <= 450 and cache.get_seq_length() + cache.dropped == 300 + 13 * 78
+    assert all(torch.equal(a, b) for state in states[1:] for a, b in zip(state, states[0]))
