@@ -30,6 +30,8 @@ BITS = (4, 8, 16)
 # does (src/gpu_kernels.py:93-94,102). 'fp32': fp32-accurate (split bf16 pairs on the MFMA path).
 PRECISIONS = {'bf16': 0, 'fp32': 1}
 PATHS = {'auto': 0, 'vector': 1, 'mfma': 2, 'short': 3}
+# what a cache was told for the calls to come, beside its shape: an eviction hands it on
+SETTINGS = ('pending_bits', 'frame_id', 'chunk_segments', 'chunk_splits', 'as_replayed', 'sparse_blocks', 'observing')
 WORKSPACE_KEPT = 128 << 20  # bytes of attention workspace a cache holds from one call to the next, at most
 _ONE_SEGMENT = (0,) * (_lib.DKV_MAX_CHUNK_SEGS + 1)  # dkv_attn_args.seg_bounds of an unsegmented chunk
 SMALL_ROWS = 32  # query rows per KV head up to which 'auto' runs the decode-step variant (MFMA_SMALL_ROWS there)
@@ -920,7 +922,9 @@ class GPUCache(_CacheBase):
         the segments hold. So layers and heads keep different tokens, `into.kept` says which, and the rows
         are moved as they are packed. This cache, its branches and its graph steps are not touched;
         graph steps of `into` go on over what it holds now. Nothing waits for the GPU. `into.dropped` counts
-        the tokens evicted so far. The index of the new cache is empty."""
+        the tokens evicted so far. The index of the new cache is empty. What this cache was told for the calls
+        to come holds for the new one: select(), sparse_blocks, observing, as_replayed, chunk_splits and
+        chunk_segments."""
         if not self.online or self._graph is not None:
             raise ValueError('evict needs an online cache (no plan) outside graph steps')
         n = self.seen[0]
@@ -980,7 +984,8 @@ class GPUCache(_CacheBase):
             into._mass.zero_()
         into.seen = [total] * into.layers
         into.kept, into.dropped = kept, self.dropped + n - total
-        into.pending_bits, into.frame_id = self.pending_bits, self.frame_id
+        for name in SETTINGS:
+            setattr(into, name, getattr(self, name))
         return into
 
     def materialize(self, layer, out_dtype=None):

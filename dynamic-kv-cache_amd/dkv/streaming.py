@@ -164,15 +164,15 @@ class StreamingDecoder:
             cache = self._reused_cache(total) if self.graphs else self.create_cache(total)
         # pipelined frames share the GPU: their frame-chunk attention takes fewer history splits
         splits = self.group_split_count(max(f.shape[1] for f in frames)) if self.pipeline > 1 and frames else 0
-        if budget is not None:
-            cache.mass()  # (allocated before a capture records it)
-        caches = [cache]
+        caches, observing = [cache], getattr(cache, 'observing', False)
         try:
-            cache.chunk_splits, cache.observing = splits, budget is not None
+            cache.chunk_splits, cache.observing = splits, observing or budget is not None
+            if cache.observing:
+                cache.mass()  # (allocated before a capture records it)
             return self._ingest_chunks(caches, given, prefix_ids, frames, bits, budget)
         finally:
             for c in caches:
-                c.chunk_splits, c.observing = 0, False
+                c.chunk_splits, c.observing = 0, observing
 
     @staticmethod
     def _protected(cache, prefix):
@@ -225,7 +225,6 @@ class StreamingDecoder:
         else:
             into = next((c for c in caches if c is not cache and c is not given), None)
         new = cache.evict(keep, sinks=prefix, recent=recent, into=into)
-        new.chunk_splits, new.observing = cache.chunk_splits, cache.observing
         if own:  # captured forwards stay with the cache whose buffers they recorded
             (self._cache, self._graphs, self._group_graphs, self._qa_graphs, self._qa_seen), self._spare = \
                 self._spare, (cache, self._graphs, self._group_graphs, self._qa_graphs, self._qa_seen)

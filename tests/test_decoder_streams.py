@@ -169,3 +169,38 @@ def test_the_newest_frames_that_leave_room_stay(hosted):
     assert [s.rows for s in one.segments] == [100, 20, 30, 30]
     two = hosted.ingest(prefix_of(10), *frames(30, 30, 30, 30, 30, 30, 30), budget=200)
     assert [s.rows for s in two.segments] == [10, 80, 30, 30, 30]
+
+
+SETTINGS = dict(observing=True, sparse_blocks=7, chunk_splits=3, as_replayed=True, chunk_segments=[0, 4, 9])
+
+
+@pytest.mark.parametrize('given', [False, True])
+def test_settings_go_with_an_eviction(hosted, given):
+    cache, into = hosted.create_cache(300), hosted.create_cache(300) if given else None
+    cache.select(8, 5)
+    hosted.forward(cache, ids=prefix_of(200))
+    cache.mass()
+    cache.__dict__.update(SETTINGS)
+    out = cache.evict(100, into=into)
+    assert {k: getattr(out, k) for k in SETTINGS} == SETTINGS and (out.pending_bits, out.frame_id) == (8, 5)
+    assert into is None or out is into
+    again = cache.evict(300, into=into)  # (nothing leaves)
+    assert again.observing and again.sparse_blocks == 7
+    fork = cache.fork().evict(100)
+    assert not fork.observing and fork.sparse_blocks == 7  # (a fork does not count)
+
+
+@pytest.mark.parametrize('budget', [None, 300])
+@pytest.mark.parametrize('observing', [False, True])
+def test_an_ingest_leaves_the_settings_of_a_cache(hosted, monkeypatch, budget, observing):
+    """A cache that observes goes on observing through an ingest, with and without a budget, and after it; one that
+    does not observes during a budgeted one alone."""
+    cache, during = hosted.create_cache(2000), []
+    forward = type(hosted).forward
+    monkeypatch.setattr(type(hosted), 'forward', lambda self, cache, **kw: (during.append((cache.observing, cache.sparse_blocks)),
+                                                                            forward(self, cache, **kw))[1])
+    cache.observing, cache.sparse_blocks = observing, 5
+    out = hosted.ingest(prefix_of(16), *frames(*[64] * 12), cache=cache, budget=budget)
+    assert (out is cache) == (budget is None)
+    assert set(during) == {(observing or budget is not None, 5)}
+    assert (out.observing, cache.observing, out.sparse_blocks, cache.sparse_blocks) == (observing, observing, 5, 5)

@@ -65,3 +65,33 @@ def test_a_prefix_of_half_the_budget(cuda, graphs):
         cache = dec.ingest(prefix, frames[:4], bits[:4], cache=cache, budget=450)
         assert cache.get_seq_length() <= 450 and cache.get_seq_length() + cache.dropped == 300 + 13 * 78
     assert all(torch.equal(a, b) for state in states[1:] for a, b in zip(state, states[0]))
+
+
+def test_a_cache_that_observes_goes_on_observing(cuda):
+    """Frame by frame as a caller does it, over evictions by hand, and through ingests, eager and replayed."""
+    announce('observing over evictions')
+    model = build_decoder(**SMALL, seed=11)
+    dec = StreamingDecoder(model, pipeline=1)
+    prefix, question, u = inputs(12)
+    frames = frames_for(model, 8, seed=13)
+    cache = dec.create_cache(700)
+    cache.observing = True
+    dec.forward(cache, ids=prefix)
+    for i, f in enumerate(frames):
+        if cache.get_seq_length() > 300:
+            cache = cache.evict(200, sinks=16, recent=64)
+        cache.select(4, i)
+        dec.forward(cache, embeddings=f)
+        assert (cache.mass()[:, :, -64:] > 0).all()  # the frame's own queries were counted
+    masses = []
+    for graphs in (False, True, True):
+        if graphs and not dec.graphs:
+            dec.graphs = True
+            dec.ingest(prefix, frames[:2], [4] * 2)  # (the decoder's own cache, whose captures do not count)
+        own = dec._cache if graphs else dec.create_cache(700)
+        own.reset()
+        own.observing = True
+        out = dec.ingest(prefix, frames, [4] * 8, cache=own)
+        assert out is own and own.observing
+        masses.append(out.mass().clone())
+    assert (masses[0] > 0).all() and all(torch.equal(m, masses[0]) for m in masses[1:])
