@@ -1280,10 +1280,20 @@ class GraphSteps:
         if c.arena is not self.arena or c.tiles is not self.tiles:
             raise ValueError('the cache no longer holds the arena and tile table these graph steps recorded '
                              '(it grew or was rebuilt): capture again')
-        if self.bounds is not False and c._bounds is not self.bounds:
+        if not self._holds_index(c):
             raise ValueError('the cache no longer holds the index these graph steps recorded: capture again')
-        if self.mass is not False and c._mass is not self.mass:
+        if not self._holds_masses(c):
             raise ValueError('the cache no longer holds the masses these graph steps recorded: capture again')
+
+    def _holds_index(self, cache):
+        return self.bounds is False or cache._bounds is self.bounds
+
+    def _holds_masses(self, cache):
+        return self.mass is False or cache._mass is self.mass
+
+    def replays_on(self, cache):
+        """Whether the recorded launches can still run on the cache, as far as its index and masses go."""
+        return self._holds_index(cache) and self._holds_masses(cache)
 
     def indexed_bound(self):
         """Most tiles that the recorded launches can find in the index: what its buffer has room for. The

@@ -233,8 +233,26 @@ class StreamingDecoder:
 
     @staticmethod
     def _graph_key(cache, *key):
-        """Key of a captured forward: one that counts attention records other launches."""
-        return key + ('observing',) if cache.observing else key if len(key) > 1 else key[0]
+        """Key of a captured forward: one that counts attention or attends sparsely records other launches."""
+        if cache.observing:
+            key += ('observing',)
+        if cache.sparse_blocks:
+            key += ('sparse', cache.sparse_blocks)
+        return key if len(key) > 1 else key[0]
+
+    @staticmethod
+    def _captured(graphs, key, cache):
+        """The captured forward under `key`, or None: one whose index or masses the cache no longer holds is dropped,
+        to be captured again."""
+        fg = graphs.get(key)
+        if fg is None:
+            return None
+        steps = fg['steps'] if isinstance(fg['steps'], list) else [fg['steps']]
+        if all(st.replays_on(cache) for st in steps):
+            return fg
+        torch.cuda.synchronize()  # (it may still run)
+        del graphs[key]
+        return None
 
     def _ingest_chunks(self, caches, given, prefix_ids, frames, bits, budget):
         cache = caches[-1]
@@ -290,7 +308,7 @@ class StreamingDecoder:
 
     def _graph_chunk(self, cache, emb):
         """One chunk as a replay of the captured forward of its length (captured on first use)."""
-        fg = self._graphs.get(self._graph_key(cache, emb.shape[1]))
+        fg = self._captured(self._graphs, self._graph_key(cache, emb.shape[1]), cache)
         if fg is None:
             self._capture_chunk(cache, emb)
             return
@@ -339,7 +357,7 @@ class StreamingDecoder:
     def _graph_group(self, cache, embs, bits, frame):
         """k consecutive frames as one replay of their pipelined forwards (captured on first use)."""
         chunk, k = embs[0].shape[1], len(embs)
-        fg = self._group_graphs.get(self._graph_key(cache, chunk, k))
+        fg = self._captured(self._group_graphs, self._graph_key(cache, chunk, k), cache)
         if fg is None:
             self._capture_group(cache, embs, bits, frame)
             return
@@ -415,8 +433,8 @@ class StreamingDecoder:
         else:
             rel = torch.arange(chunk, device=self.device)
         key = (chunk, int(logits), tuple(lengths) if lengths else None)
-        if branch.sparse_blocks:  # (a captured forward records the index it reads, too)
-            key += (branch.sparse_blocks, id(branch._bounds))
+        if branch.sparse_blocks:
+            key += (branch.sparse_blocks,)
         graphed = self.graphs and self._cache is not None and branch.arena is self._cache.arena
         if not graphed or key not in self._qa_seen:
             if graphed:
@@ -427,7 +445,7 @@ class StreamingDecoder:
                 return self.forward(branch, embeddings=emb, positions=rel + past, logits=logits)
             finally:
                 branch.chunk_segments = None
-        fg = self._qa_graphs.get(key)
+        fg = self._captured(self._qa_graphs, key, branch)
         steps = fg['steps'] if fg else None
         branch.begin_graph_steps(chunk, q_heads=None if fg else self.config.num_attention_heads, steps=steps)
         try:

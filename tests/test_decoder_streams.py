@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from dkv import streaming
-from dkv.gpu_cache import GPUCache
+from dkv.gpu_cache import GPUCache, GraphSteps
 from dkv.streaming import StreamingDecoder
 
 
@@ -204,3 +204,31 @@ def test_an_ingest_leaves_the_settings_of_a_cache(hosted, monkeypatch, budget, o
     assert (out is cache) == (budget is None)
     assert set(during) == {(observing or budget is not None, 5)}
     assert (out.observing, cache.observing, out.sparse_blocks, cache.sparse_blocks) == (observing, observing, 5, 5)
+
+
+def test_captured_forwards_are_told_apart(monkeypatch):
+    """By what a forward is captured under, and dropped where the cache holds another index or other masses."""
+    monkeypatch.setattr(torch.cuda, 'synchronize', lambda: None)
+    cache, d = GPUCache(None, layers=1, heads=1, max_tokens=256, device='cpu'), decoder()
+    keys = []
+    for observing in (False, True):
+        for blocks in (0, 3, 4):
+            cache.observing, cache.sparse_blocks = observing, blocks
+            keys += [d._graph_key(cache, 64), d._graph_key(cache, 64, 2)]
+    assert len(set(keys)) == 12 and keys[:2] == [64, (64, 2)]
+
+    def captured():
+        steps = GraphSteps(cache, 1)
+        steps.mass, steps.bounds = cache._own_mass(), cache._bounds
+        return dict(steps=steps), dict(steps=[steps, GraphSteps(cache, 1)])
+    one, group = captured()
+    graphs = {1: one, 2: group}
+    assert d._captured(graphs, 1, cache) is one and d._captured(graphs, 2, cache) is group and d._captured(graphs, 3, cache) is None
+    cache._bounds = torch.zeros(16, dtype=torch.uint8)
+    assert d._captured(graphs, 1, cache) is None and d._captured(graphs, 2, cache) is None and not graphs
+    graphs[1], _ = captured()
+    cache._mass = cache._mass.clone()
+    assert d._captured(graphs, 1, cache) is None and not graphs
+    graphs[1] = dict(steps=GraphSteps(cache, 1))  # (neither recorded)
+    cache._bounds, cache._mass = None, None
+    assert d._captured(graphs, 1, cache) is graphs[1]

@@ -95,3 +95,32 @@ def test_a_cache_that_observes_goes_on_observing(cuda):
         assert out is own and own.observing
         masses.append(out.mass().clone())
     assert (masses[0] > 0).all() and all(torch.equal(m, masses[0]) for m in masses[1:])
+
+
+@pytest.mark.parametrize('pipeline', [1, 4])
+def test_frames_replay_the_attention_that_the_cache_is_set_to(cuda, pipeline):
+    """Streams that go on in the decoder's own cache, dense, then sparse over an index, then over an index that moved:
+    replayed as eager."""
+    announce(f'sparse frames, pipeline={pipeline}')
+    model = build_decoder(**SMALL, seed=11)
+    prefix, question, u = inputs(12)
+    frames, bits = frames_for(model, 12, seed=13), [4, 8, 16, 4, 8, 4] * 2
+    runs = []
+    for graphs in (False, True):
+        dec = StreamingDecoder(model, graphs=graphs, pipeline=pipeline)
+        out = []
+        for _ in range(2):
+            cache = dec.ingest(prefix, frames, bits, qa_reserve=3000)  # (own cache with graphs: dense, captured in the first round)
+            cache.index()
+            cache.sparse_blocks = 2
+            dec.ingest(prefix, frames, bits, cache=cache)
+            cache.index()  # (longer than its buffer has room for: it moves)
+            dec.ingest(prefix, frames, bits, cache=cache)
+            out += [x.clone() for l in range(SMALL['layers']) for x in cache.materialize(l)]
+            out.append(dec.generate(cache, question, u.cuda(), blocks=3, **SAMPLING))
+            cache.sparse_blocks = 0
+        runs.append(out)
+    dense = StreamingDecoder(model).ingest(prefix, frames * 3, bits * 3)
+    assert not torch.equal(dense.materialize(1)[0][:, :, -600:], runs[0][2][:, :, -600:])
+    for i, (a, b) in enumerate(zip(*runs)):
+        assert torch.equal(a, b), i
