@@ -1126,20 +1126,28 @@ class GPUCache(_CacheBase):
         fp32 scales and offsets, 64-byte header) and a 32-byte descriptor
         (layer, frame, start, end, bits). One byte-moving launch for all segments; nothing
         is requantized. `layers` (default all) must be consecutive and at the same length.
-        The tensors stay on the cache's device unless `device` names another.
+        The tensors stay on the cache's device unless `device` names another. The format counts tokens as
+        the cache holds them and has no place for `dropped`, which import_segments() takes beside it, nor
+        for masses.
         """
         return SegmentExport(self, layers).run().segments(device)
 
-    def import_segments(self, segments):
+    def import_segments(self, segments, dropped=0):
         """Appends {layer: [Segment]} (the MixedPrecisionCache layout) to every layer; returns the old length.
 
         Segment i of every layer must describe the same tokens, frame and width, starting at the
         cache's current length, and hold PackedTensors of [1, heads, rows, 64] tensors with group
         size 64 (16-bit ones in bf16). Their payload, offsets and scales are copied into the arena
         unchanged (one launch), so attending over them equals attending over the same tokens
-        packed by append().
+        packed by append(). `dropped`: of a cache that had evicted tokens when it was exported, its `dropped`,
+        so that the next token's position goes on from there (into an empty cache only).
         """
-        return self._import(segments)[0]
+        if dropped < 0 or (dropped and any(self.seen)):
+            raise ValueError(f'import_segments: dropped must not be negative, and 0 unless the cache is empty, got {dropped}')
+        past = self._import(segments)[0]
+        if dropped:
+            self.dropped = dropped
+        return past
 
     def _import(self, segments):
         """import_segments(), also returning the SegmentBatch that ran (None if nothing moved)."""

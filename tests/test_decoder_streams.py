@@ -232,3 +232,14 @@ def test_captured_forwards_are_told_apart(monkeypatch):
     graphs[1] = dict(steps=GraphSteps(cache, 1))  # (neither recorded)
     cache._bounds, cache._mass = None, None
     assert d._captured(graphs, 1, cache) is graphs[1]
+
+
+def test_positions_of_imported_segments_are_checked():
+    c = GPUCache(None, layers=1, heads=1, max_tokens=64, device='cpu')
+    with pytest.raises(ValueError, match='dropped'):
+        c.import_segments({0: []}, dropped=-1)
+    c._open_segment(0, 8, 16)
+    c.seen = [8]
+    with pytest.raises(ValueError, match='dropped'):
+        c.import_segments({0: []}, dropped=5)
+    assert c.import_segments({0: []}) == 8 and c.dropped == 0

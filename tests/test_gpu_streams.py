@@ -124,3 +124,19 @@ def test_frames_replay_the_attention_that_the_cache_is_set_to(cuda, pipeline):
     assert not torch.equal(dense.materialize(1)[0][:, :, -600:], runs[0][2][:, :, -600:])
     for i, (a, b) in enumerate(zip(*runs)):
         assert torch.equal(a, b), i
+
+
+def test_positions_go_on_after_an_export_and_import(cuda):
+    """An evicted cache through segments into another: the next tokens have the positions they had in the stream."""
+    announce('export and import of an evicted cache')
+    model = build_decoder(**SMALL, seed=14)
+    dec = StreamingDecoder(model)
+    prefix, question, _ = inputs(15)
+    cache = dec.ingest(prefix, frames_for(model, 8, seed=16), [4, 8, 16, 4] * 2, budget=300)
+    assert cache.dropped
+    copy = dec.create_cache(600)
+    assert copy.import_segments(cache.export_segments(), dropped=cache.dropped) == 0 and copy.dropped == cache.dropped
+    want = dec.forward(cache.fork(), ids=question, logits=13)
+    assert torch.equal(dec.forward(copy.fork(), ids=question, logits=13), want)
+    copy.reset()
+    assert copy.dropped == 0
