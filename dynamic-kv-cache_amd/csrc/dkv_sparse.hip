@@ -132,6 +132,7 @@ struct SparsePlan {
   int row_blocks;          // 16-row blocks of a KV head's query heads
   int splits;              // workgroups of a (query, KV head, row block): as many as any history within the bounds takes
   int max_indexed, max_chosen;  // launch bounds
+  int queries;             // that are scored at a time
   int64_t keys, lists, part_o, part_ml, bytes;  // workspace offsets
 };
 
@@ -150,12 +151,13 @@ constexpr int SCORE_QUERIES = 16;
 // Scores of 64 tiles for 16 queries of a KV head, as sortable keys. Each wave takes 32 of the 128 elements, a lane
 // a tile; their sums meet in LDS in a fixed order. In 64 bits, rounded to 32 at the end: the products of bf16 values
 // are exact there and their sums as good as exact, so equal scores tie and no order of summation chooses a tile. Bound by
-// these products: 513 queries by 520 tiles by 3 KV heads 22.4 us.
-__global__ __launch_bounds__(256) void score_kernel(dkv_attn_args a, dkv_sparse s, int max_indexed, uint32_t* keys) {
+// these products: 513 queries by 520 tiles by 3 KV heads 22.4 us. Queries [first, first + some): a KV head's have `room`
+// rows of keys.
+__global__ __launch_bounds__(256) void score_kernel(dkv_attn_args a, dkv_sparse s, int max_indexed, int first, int room, uint32_t* keys) {
   __shared__ double query[SCORE_QUERIES][2 * D];  // q+ then q-, as the pieces' high and low
   __shared__ double part[4][SCORE_QUERIES][BLOCK];
   const Seen v = seen_of(a, s);
-  const int block = blockIdx.x, h = blockIdx.y, m0 = blockIdx.z * SCORE_QUERIES;
+  const int block = blockIdx.x, h = blockIdx.y, m0 = first + blockIdx.z * SCORE_QUERIES;
   if (v.chosen == v.n_indexed || block * BLOCK >= v.n_indexed) return;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, G = a.q_heads / a.heads;
   const int queries = min(SCORE_QUERIES, a.nq - m0);
@@ -203,7 +205,7 @@ __global__ __launch_bounds__(256) void score_kernel(dkv_attn_args a, dkv_sparse 
   for (int i = threadIdx.x; i < queries * BLOCK; i += 256) {
     const int m = i / BLOCK, t = i % BLOCK;
     if (block * BLOCK + t < v.n_indexed)
-      keys[((int64_t)h * a.nq + m0 + m) * max_indexed + block * BLOCK + t] =
+      keys[((int64_t)h * room + m0 - first + m) * max_indexed + block * BLOCK + t] =
           order_key((float)(part[0][m][t] + part[1][m][t] + (part[2][m][t] + part[3][m][t])));
   }
 }
@@ -213,14 +215,13 @@ __global__ __launch_bounds__(256) void score_kernel(dkv_attn_args a, dkv_sparse 
 // barriers of a radix step, about three a choice.
 constexpr int CHOOSERS = 256;
 template <int N>
-__global__ __launch_bounds__(CHOOSERS) void choose_kernel(dkv_attn_args a, dkv_sparse s, int max_indexed, int max_chosen,
-                                                          const uint32_t* keys, int32_t* lists) {
+__global__ __launch_bounds__(CHOOSERS) void choose_kernel(dkv_attn_args a, dkv_sparse s, int max_indexed, int max_chosen, int first,
+                                                          int room, const uint32_t* keys, int32_t* lists) {
   __shared__ SelectScratch<CHOOSERS, 8> scratch;
   const Seen v = seen_of(a, s);
   if (v.chosen == v.n_indexed) return;  // every tile, or none: no list is read
-  const int64_t pair = (int64_t)blockIdx.y * a.nq + blockIdx.x;
-  keys += pair * max_indexed;
-  lists += pair * max_chosen;
+  keys += ((int64_t)blockIdx.y * room + blockIdx.x) * max_indexed;
+  lists += ((int64_t)blockIdx.y * a.nq + first + blockIdx.x) * max_chosen;
   auto key = [&](int i) { return max(keys[i], 1u); };
   Elements<CHOOSERS, N, decltype(key)>(v.n_indexed, key).largest(scratch, (uint32_t)v.chosen, [&](int to, int i) { lists[to] = i; });
 }
@@ -486,6 +487,10 @@ __global__ __launch_bounds__(256) void merge_kernel(dkv_attn_args a, dkv_sparse 
   store4(a.out, a.out_dtype, m * a.out_tok_stride + (h * G + row) * a.out_head_stride + 4 * e4, x / l);
 }
 
+// Bytes of scores at a time: a prompt of tens of thousands of queries over a long index would have gigabytes of them. (At
+// least SCORE_QUERIES queries' whatever the index, and a multiple of these.)
+constexpr int64_t KEYS_BYTES = 64 << 20;
+
 // Attention workgroups that a call is split into: 64 queries past 32704 54 us with 1024, 62 with 512, 60 with 2048 (then).
 constexpr int WORKGROUPS = 1024;
 
@@ -504,7 +509,14 @@ static SparsePlan plan_of(const dkv_attn_args& a, const dkv_sparse& s) {
   auto up = [](int64_t x) { return (x + 255) & ~(int64_t)255; };
   const int64_t choosing = p.max_chosen < p.max_indexed || a.step;
   p.keys = 0;
-  p.lists = p.keys + (choosing ? up(4 * pairs * p.max_indexed) : 0);
+  p.queries = a.nq;
+  int64_t scores = 0;  // (near_kernel keeps them in registers)
+  if (choosing && p.max_indexed > NEAR_TILES) {
+    const int64_t row = 4ll * a.heads * p.max_indexed, fit = KEYS_BYTES / row / SCORE_QUERIES * SCORE_QUERIES;
+    if (fit < p.queries) p.queries = fit > SCORE_QUERIES ? (int)fit : SCORE_QUERIES < a.nq ? SCORE_QUERIES : a.nq;
+    scores = row * p.queries;
+  }
+  p.lists = p.keys + up(scores);
   p.part_o = p.lists + (choosing ? up(4 * pairs * p.max_chosen) : 0);
   const int64_t parts = p.splits > 1 ? pairs * p.splits * G : 0;
   p.part_ml = p.part_o + up(4 * D * parts);
@@ -622,10 +634,13 @@ int dkv_attend_sparse(const dkv_attn_args* args, const dkv_sparse* sparse, void*
     if (n <= NEAR_TILES) {
       hipLaunchKernelGGL(near_kernel, dim3(a.nq, a.heads), dim3(NEAR_TILES), 0, st, a, s, p.max_chosen, lists);
     } else {
-      hipLaunchKernelGGL(score_kernel, dim3((n + BLOCK - 1) / BLOCK, a.heads, (a.nq + SCORE_QUERIES - 1) / SCORE_QUERIES), dim3(256), 0, st,
-                         a, s, n, keys);
       const auto choose = n <= 8 * CHOOSERS ? choose_kernel<8> : choose_kernel<0>;
-      hipLaunchKernelGGL(choose, dim3(a.nq, a.heads), dim3(CHOOSERS), 0, st, a, s, n, p.max_chosen, keys, lists);
+      for (int m = 0; m < a.nq; m += p.queries) {
+        const int some = a.nq - m < p.queries ? a.nq - m : p.queries;
+        hipLaunchKernelGGL(score_kernel, dim3((n + BLOCK - 1) / BLOCK, a.heads, (some + SCORE_QUERIES - 1) / SCORE_QUERIES), dim3(256), 0, st,
+                           a, s, n, m, p.queries, keys);
+        hipLaunchKernelGGL(choose, dim3(some, a.heads), dim3(CHOOSERS), 0, st, a, s, n, p.max_chosen, m, p.queries, keys, lists);
+      }
     }
   }
   const dim3 grid(p.splits, a.heads * p.row_blocks, a.nq);
