@@ -32,6 +32,7 @@ PRECISIONS = {'bf16': 0, 'fp32': 1}
 PATHS = {'auto': 0, 'vector': 1, 'mfma': 2, 'short': 3}
 # what a cache was told for the calls to come, beside its shape: an eviction hands it on
 SETTINGS = ('pending_bits', 'frame_id', 'chunk_segments', 'chunk_splits', 'as_replayed', 'sparse_blocks', 'observing')
+MOST_BLOCKS = 2 ** 31 - 1  # that dkv_sparse can ask for: more than any index has
 WORKSPACE_KEPT = 128 << 20  # bytes of attention workspace a cache holds from one call to the next, at most
 _ONE_SEGMENT = (0,) * (_lib.DKV_MAX_CHUNK_SEGS + 1)  # dkv_attn_args.seg_bounds of an unsegmented chunk
 SMALL_ROWS = 32  # query rows per KV head up to which 'auto' runs the decode-step variant (MFMA_SMALL_ROWS there)
@@ -823,7 +824,7 @@ class GPUCache(_CacheBase):
             return out
         graph = self._graph
         s = _lib.SPARSE.pack(0 if self._bounds is None else self._bounds.data_ptr(),
-                             self.n_indexed if graph is None else graph.indexed_bound(), blocks,
+                             self.n_indexed if graph is None else graph.indexed_bound(), min(blocks, MOST_BLOCKS),
                              self._single_rows(self._tiles_before(past)) if graph is None else 0, 0)
         size = _lib.load().dkv_attend_sparse_workspace_bytes
         a, keep = self._chunk_args(q, k, v, layer, past, out, segments, precision, lambda block: size(block, s))
@@ -1437,7 +1438,7 @@ class GraphSteps:
         lib, c = _lib.load(), self.cache
         need = lib.dkv_attend_workspace_bytes(ctypes.byref(a))
         if c.sparse_blocks:
-            s = _lib.Sparse(None, self.indexed_bound(), c.sparse_blocks, 0, 0)
+            s = _lib.Sparse(None, self.indexed_bound(), min(c.sparse_blocks, MOST_BLOCKS), 0, 0)
             need = max(need, lib.dkv_attend_sparse_workspace_bytes(ctypes.byref(a), ctypes.byref(s)))
         return max(need, lib.dkv_attention_mass_workspace_bytes(ctypes.byref(a))) if c.observing else need
 

@@ -235,7 +235,7 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
             keep.append(x)
             setattr(p, name + '_rows', x.data_ptr())
         else:
-            setattr(p, name, min(int(x), vocab) if name == 'top_k' else float(x))
+            setattr(p, name, max(min(int(x), vocab), -1) if name == 'top_k' else float(x))  # (in 32 bits; -1 is refused)
     rows = logits.reshape(-1, vocab)
     if rows.stride(-1) != 1:
         rows = rows.contiguous()

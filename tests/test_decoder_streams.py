@@ -4,7 +4,7 @@ import types
 import pytest
 import torch
 
-from dkv import streaming
+from dkv import _lib, streaming
 from dkv.gpu_cache import GPUCache, GraphSteps
 from dkv.streaming import StreamingDecoder
 
@@ -243,3 +243,17 @@ def test_positions_of_imported_segments_are_checked():
     with pytest.raises(ValueError, match='dropped'):
         c.import_segments({0: []}, dropped=5)
     assert c.import_segments({0: []}) == 8 and c.dropped == 0
+
+
+def test_blocks_past_32_bits_are_all_blocks(monkeypatch):
+    """A number of blocks that no 32-bit argument holds is as many as there are, not what is left of it."""
+    seen = []
+    cache = GPUCache(None, layers=1, heads=1, max_tokens=64, device='cpu')
+    steps = GraphSteps(cache, 1)
+    room = _lib.load().dkv_attend_sparse_workspace_bytes
+    monkeypatch.setattr(_lib.load(), 'dkv_attend_sparse_workspace_bytes',
+                        lambda a, s: (seen.append(s._obj.blocks), room(a, s))[1])
+    for blocks in (7, 1 << 32, (1 << 31) + 5):
+        cache.sparse_blocks = blocks
+        steps.workspace_bytes(2)
+    assert seen == [7, (1 << 31) - 1, (1 << 31) - 1]

@@ -3,6 +3,8 @@ import pytest
 import torch
 
 from conftest import announce
+from dkv.gpu_cache import GPUCache
+from dkv.gpu_ops import sample
 from dkv.streaming import StreamingDecoder, build_decoder
 from test_gpu_generate import SAMPLING, inputs
 from test_gpu_streaming import SMALL, frames_for
@@ -140,3 +142,21 @@ def test_positions_go_on_after_an_export_and_import(cuda):
     assert torch.equal(dec.forward(copy.fork(), ids=question, logits=13), want)
     copy.reset()
     assert copy.dropped == 0
+
+
+def test_numbers_past_32_bits(cuda):
+    """A top_k or a number of blocks of more than 32 bits: refused where it is negative, all of them where not."""
+    announce('top_k and blocks past 32 bits')
+    x, u = torch.randn(3, 100, device=cuda), torch.rand(3, device=cuda)
+    for k in (-1, -(1 << 32), -(1 << 32) + 5, -(1 << 40)):
+        with pytest.raises(ValueError, match='top_k'):
+            sample(x, u, top_k=k)
+    assert sample(x, u, top_k=(1 << 32) + 1).tolist() == sample(x, u).tolist()
+    cache = GPUCache(None, layers=1, heads=1, max_tokens=200)
+    rows = torch.randn(1, 1, 131, 64, device=cuda).to(torch.bfloat16)
+    past = [cache.append(rows[:, :, i:i + 65], rows[:, :, i:i + 65], 0) for i in (0, 65)][1]
+    cache.index()
+    args = (rows[:, :, :1], rows[:, :, :1], rows[:, :, :1], 0, past)
+    want = cache.attend_sparse(*args, 1000)
+    for blocks in (1 << 31, 1 << 32, 10 ** 12):
+        assert torch.equal(cache.attend_sparse(*args, blocks), want)
