@@ -899,7 +899,7 @@ class GPUCache(_CacheBase):
             count[seg.bits] -= seg.rows
         widths = []  # as they come
         for seg in segs[a:b]:
-            if seg.bits not in widths:
+            if seg.rows and seg.bits not in widths:
                 widths.append(seg.bits)
                 if len(widths) == sum(m > 0 for m in count.values()):
                     break

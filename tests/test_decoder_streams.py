@@ -257,3 +257,15 @@ def test_blocks_past_32_bits_are_all_blocks(monkeypatch):
         cache.sparse_blocks = blocks
         steps.workspace_bytes(2)
     assert seen == [7, (1 << 31) - 1, (1 << 31) - 1]
+
+
+def test_an_eviction_passes_over_empty_segments():
+    """An append of no tokens opens a segment of none, whose width counts for nothing."""
+    c = GPUCache(None, layers=1, heads=1, max_tokens=400, device='cpu')
+    at = 0
+    for n, bits in [(0, 8), (64, 4), (0, 16), (64, 16), (0, 8), (64, 4), (0, 4)]:
+        c._open_segment(at, n, bits)
+        at += n
+    c.seen = [at]
+    assert c._eviction(96, 0, 0) == (0, 7, {4: 64, 16: 32}, {4: 128, 16: 64})
+    assert c._eviction(96, 1, 0)[2:] == ({16: 16, 4: 16}, {16: 64, 4: 64})
