@@ -4,11 +4,11 @@
 // each width, as many as the host says, so the tile table is known before the kernels run and nothing waits for the
 // device: history rows carry no mask and no position of their own, so a tile may hold other tokens in every head.
 // Three launches: where each token lies and which tokens each width has, with the new tile table; the choice, a radix
-// search for the smallest kept mass per (layer, head, width); and the move, which is bound by memory (each kept row
-// read and written once).
+// search for the smallest kept mass per (layer, head, width); and the move, each kept row read and written
+// once.
 // Measured (kernel times): 65531 to 16384 tokens, 4 layers of 8 heads: 9.0 + 31.8 (96 workgroups: three radix steps and
-// their barriers over up to 26000 keys each) + 51.5 us (148 MB read and written, 2.9 TB/s: a row is 32 to 128
-// bytes at an address of its own). 8128 to 4096, 8 layers of 5: 6.2 + 12.2 + 11.1; a call's host part, some 60 us, is longer.
+// their barriers over up to 26000 keys each) + 51.5 us (148 MB read and written, 2.9 TB/s where a large copy reaches 5.2: a
+// row is 32 to 128 bytes at an address of its own). 8128 to 4096, 8 layers of 5: 6.2 + 12.2 + 11.1; a call's host part, some 60 us, is longer.
 #include "dkv_select.h"
 
 namespace dkv {

@@ -11,7 +11,11 @@
 // Measured (kernel times): a token past 131007 at fp32, 8 KV heads of 4: 29.9 us (73 MB of keys, 2.4 TB/s: two waves a SIMD
 // wait for their next unit) + 8.5 (17 MB of scores). A 64-token frame past 8128, 5 KV heads of 3: 11.1 + 11.7, each a
 // few dependent loads, three units a workgroup and the join. A 2048-token prompt past 1000: 29.9 + 4.9 + 42.1 + 4.8; the
-// products alone are 6.7 us; each pass's 62 million exponentials with what surrounds them some 17, by instructions.
+// products alone are 6.7 us, each pass's 62 million exponentials with what surrounds them some 17 by counting instructions:
+// no count explains what the passes take above that.
+// Replays launch columns_kernel's workgroups for every tile that the table has room for, and those behind the history leave
+// at once: attention and mass of a frame past 8128 36.7 us as calls, replayed 46.0 in a cache of 9152 tokens, 65.5 of
+// 32768, 168.6 of 131072 (few_columns_kernel's grid is bounded: a token 19.0 to 20.3).
 #include "dkv_rows.h"
 
 namespace dkv {
@@ -19,12 +23,14 @@ namespace mass {
 
 using namespace rows;
 
-// Query rows of a KV head that a wave takes alone. A chunk of 48 rows past 8128 (5 KV heads) 13.0 us against 14.8 in
-// workgroups, 63 rows 13.4 and 14.9; 64 rows past 131007 at fp32 127 and 200.
+// Query rows of a KV head that a wave takes alone: what its registers hold (4 blocks of 16 rows, 255 at fp32), not where the
+// two ways meet. A chunk of 48 rows past 8128 (5 KV heads) 13.0 us against 14.8 in workgroups, 63 rows 13.4 and 14.9; 64
+// rows past 131007 at fp32 127 and 200, so there a 65th row costs more than half again.
 constexpr int FEW = 64;
 // Query rows of a KV head whose scores the first pass keeps for the second: a key's scores are 4 bytes a row written and
-// read, its packed row 40 to 128 and the arithmetic again. A token over 131007 at fp32, 8 KV heads: 36.7 us with kept scores
-// against 53.5 at 4 rows, 41.4 against 53.3 at 8.
+// read, its packed row 40 to 128 and the arithmetic again. A token over 131007 at fp32, 8 KV heads: 36.6 us with kept scores
+// against 53.5 at 4 rows, 41.0 against 53.3 at 8. Room for 16 rows costs registers at every number of them: 52.2 us at 4, 63.4
+// at 8, and 66.5, 74.6 and 86.5 at 9, 12 and 16, where none kept take 53.1 to 53.4.
 constexpr int KEEP = 8;
 constexpr int GROUP = 192;        // query rows of a row group: 12 blocks, three a wave
 constexpr int BLOCKS = GROUP / 64;  // 16-row blocks of a wave

@@ -14,6 +14,10 @@
 // a call: latency, each launch a few dependent loads. 64 queries past 32704: 10.3 + 30.4 + 4.1, 42.2 a call; 513 queries
 // past 20011 at fp32, 3 KV heads of 3: 22.4 + 8.4 + 101, 122 a call: every query walks some 30 tiles of its own and unpacks
 // them, for three of 16 MFMA rows; the unpacking and the softmax keep the VALU busy, not the 400 MB from L2.
+// Attention to all of a history is one launch and a merge, and reads each tile once for many queries: it is the faster one
+// up to some length (a call of it and of this one at 16 blocks, us). One token, 5 KV heads of 3: 12.9 and 16.5 past 8128, 15.2
+// and 17.0 past 32704, 21.6 and 21.2 past 65472, 32.2 and 21.2 past 131008; 8 of 4: 13.4 and 16.7, 16.9 and 16.8, 25.4 and
+// 20.2, 42.2 and 20.2. 64 queries, 5 of 3: 16.1 and 29.3, 30.8 and 32.8, 48.6 and 40.2, 83.9 and 42.1.
 #include "dkv_rows.h"
 #include "dkv_select.h"
 
@@ -32,7 +36,8 @@ __device__ __forceinline__ int64_t piece_at(int block, int layer, int layers, in
 }
 
 // Tiles of an index workgroup, a wave a tile: 16 tiles' pieces of 16 bytes are 256 consecutive bytes of the index. Bound by
-// memory: 32 layers of 5 heads past 8128 (97 MB) 36.5 us, 2.7 TB/s; a workgroup a tile took 64.
+// the loads in flight, a tile's a wave: 32 layers of 5 heads past 8128 (97 MB) 36.5 us, 2.7 TB/s, half of what a large copy
+// reaches; a workgroup a tile took 64.
 constexpr int INDEX_TILES = 16;
 
 // One step of a minimum (and maximum, of the negated) over lanes that halves the elements a lane holds: x keeps the lower
@@ -210,9 +215,9 @@ __global__ __launch_bounds__(256) void score_kernel(dkv_attn_args a, dkv_sparse 
   }
 }
 
-// The chosen tiles of a (query, KV head), in order. Up to N * CHOOSERS keys stay in registers: a token past 131007 (2048
-// tiles) 21.6 us a call with N = 8, 23.4 with keys loaded again each time (N = 0), which longer indexes take. Bound by the
-// barriers of a radix step, about three a choice.
+// The chosen tiles of a (query, KV head), in order. Up to N * CHOOSERS keys stay in registers: a token past 131007 (2047
+// tiles) 20.2 us a call with N = 8, 22.0 with keys loaded again each time (N = 0), which longer indexes take; 64 queries past
+// 131007 50.9 and 52.8. Bound by the barriers of a radix step, about three a choice.
 constexpr int CHOOSERS = 256;
 template <int N>
 __global__ __launch_bounds__(CHOOSERS) void choose_kernel(dkv_attn_args a, dkv_sparse s, int max_indexed, int max_chosen, int first,
@@ -227,8 +232,10 @@ __global__ __launch_bounds__(CHOOSERS) void choose_kernel(dkv_attn_args a, dkv_s
 }
 
 // Scores and choice of a (query, KV head) in one workgroup, a wave 64 tiles: for up to NEAR_TILES indexed tiles. The sums
-// are score_kernel's, term by term. Against scores and choice in two launches: a token past 8128 16.6 us a call and 19.3, 64
-// queries past 32704 (511 tiles) 48.4 and 55.1.
+// are score_kernel's, term by term. Against scores and choice in two launches: a token past 8128 15.8 to 16.7 us a call and
+// 19.6, past 32000 16.5 and 19.1, 64 queries past 32704 (511 tiles) 41.7 and 48.2. With room for 1024 tiles (1024 threads)
+// one launch took longer than two above 512, 20.8 against 19.6 for a token past 65000 and 51.5 against 49.1 for 64 queries
+// past 64000, and 47.1 at the 511.
 constexpr int NEAR_TILES = 512;
 __global__ __launch_bounds__(NEAR_TILES) void near_kernel(dkv_attn_args a, dkv_sparse s, int max_chosen, int32_t* lists) {
   __shared__ SelectScratch<NEAR_TILES, 8> scratch;
@@ -372,8 +379,8 @@ __device__ __forceinline__ void store4(void* out, int out_dtype, int64_t at, f32
 }
 
 // A wave a unit of 64 keys, keys and values straight from global memory into MFMA operands: a unit is read by one query
-// alone, so LDS would only add a pass. 220 to 232 registers, two waves a SIMD; held to three they spill (66 us against 54
-// for 64 queries past 32704).
+// alone, so LDS would only add a pass. 198 to 208 registers, two waves a SIMD; held to three they spilled (66 us against 54
+// for 64 queries past 32704, then).
 template <int PREC, int TERMS>
 __global__ __launch_bounds__(256) void attend_kernel(dkv_attn_args a, dkv_sparse s, int row_blocks, int most, int max_chosen,
                                                      const int32_t* lists, float* part_o, float2* part_ml) {
