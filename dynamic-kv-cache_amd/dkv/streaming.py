@@ -144,9 +144,9 @@ class StreamingDecoder:
         mass are evicted (GPUCache.evict), down to three quarters of the budget (where the prefix fills
         these, of what it leaves) or to what the frame needs. The prefix stays (where the cache held tokens
         before, its first ones instead, as many), and of the frames that the last quarter of the budget takes
-        in the newest that leave room for it. A budget that some frame and the prefix use up is refused
-        before any forward. The cache that is returned holds the history: with
-        a budget it may be another one than the `cache` given, which then holds what it did before the first
+        in the newest that leave room for it. A budget that some frame and the prefix use up, or that the
+        cache cannot hold, is refused before any forward. The cache that is returned holds the history: with a
+        budget it may be another one than the `cache` given, which then holds what it did before the first
         eviction, for its forks too. (With graphs=True the decoder's own cache evicts into another one that
         the decoder keeps, and that one back: as between requests, forks of either end there.)
         """
@@ -195,6 +195,8 @@ class StreamingDecoder:
                 raise ValueError('a budget needs an online cache (no plan)')
             held = cache.get_seq_length()
             protected = self._protected(cache, prefix) if held >= prefix else held + prefix
+            if cache.capacity < min(budget, held + prefix + sum(frames)):
+                raise ValueError(f'a budget of {budget} tokens is more than the {cache.capacity} that the cache holds')
         for n in [prefix] + frames:
             if held + n > budget:
                 held = self._kept(budget, protected, n)

@@ -269,3 +269,12 @@ def test_an_eviction_passes_over_empty_segments():
     c.seen = [at]
     assert c._eviction(96, 0, 0) == (0, 7, {4: 64, 16: 32}, {4: 128, 16: 64})
     assert c._eviction(96, 1, 0)[2:] == ({16: 16, 4: 16}, {16: 64, 4: 64})
+
+
+def test_a_cache_smaller_than_the_budget_is_refused_before_any_forward(hosted):
+    cache = hosted.create_cache(250)
+    with pytest.raises(ValueError, match='budget.*250'):
+        hosted.ingest(prefix_of(16), *frames(*[64] * 5), cache=cache, budget=300)
+    assert not hasattr(hosted, 'most') and cache.seen == [0, 0]
+    assert hosted.ingest(prefix_of(16), *frames(*[64] * 3), cache=cache, budget=300) is cache  # (never as long)
+    assert hosted.ingest(prefix_of(16), *frames(*[64] * 5), cache=cache, budget=250).get_seq_length() <= 250
