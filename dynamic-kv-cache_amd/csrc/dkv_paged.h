@@ -1,0 +1,49 @@
+// Paged caches (dkv_paged.hip: plans, pack, read, move; dkv_paged_attn.hip: attention): the page layout, and what a
+// step's plan holds in device memory.
+#pragma once
+#include "dkv_common.h"
+
+namespace dkv {
+namespace paged {
+
+constexpr int GRAIN_ROW = 512;  // bytes of a sub-block in one grain: 2560, 4608 and 8192 are multiples of it
+
+__host__ __device__ inline int page_bits(uint32_t page) { return 4 << (page & 3); }
+__host__ __device__ inline int page_sub(int bits) { return 512 * bits + (bits < 16 ? 512 : 0); }  // subblock_bytes(64, bits)
+__host__ __device__ inline int64_t grain_bytes(int layers, int heads) { return (int64_t)GRAIN_ROW * 2 * layers * heads; }
+__host__ __device__ inline int page_grains(int bits) { return page_sub(bits) / GRAIN_ROW; }
+
+// The K sub-block of (layer, head) of a page; V's lies heads sub-blocks behind it.
+__device__ __forceinline__ int64_t page_at(uint32_t page, int layer, int layers, int heads, int h) {
+  return (int64_t)(page >> 2) * grain_bytes(layers, heads) + ((int64_t)layer * 2 * heads + h) * page_sub(page_bits(page));
+}
+
+// A plan's first words: how many records of each kind it has.
+enum { N_ITEMS, N_WORK, N_LONG, N_MERGES, HEAD_WORDS = 16 };
+
+// Rows of the step that go into one page: dkv_page_rows. History pages: {page, rows of it that are history}.
+struct Page {
+  uint32_t page;
+  int32_t rows;
+};
+
+// One workgroup's share of a sequence's (or, over pages that several sequences have in common, a group's) attention, for
+// each KV head: units [u0, u1) for block `block` of its query rows. Unit u is page first_page + u of the plan while that
+// is below n_pages, then 64 new tokens each. Query row r is token r / G, query head r % G of the KV head; `count` tokens
+// from token0 of the step on. Rows go to the partial rows from `part` on, or where that is negative to the output.
+struct Work {
+  int32_t first_page, n_pages, token0, count, block, u0, u1, part;
+};
+
+// Query rows [row0, row0 + 16) of a sequence that has `rows` of them from token0 on, joined from its own partials (split
+// s: rows part + s * rows + ...) and those of its group (the row's first at shared + its row here, shared_stride apart).
+struct Merge {
+  int32_t token0, rows, row0, part, splits, shared, shared_splits, shared_stride;
+};
+
+constexpr int SHORT_BLOCK = 16;  // query rows of a block
+
+int check_args(const dkv_paged_args& a, bool attend, const char* what);
+
+}  // namespace paged
+}  // namespace dkv

@@ -1,0 +1,551 @@
+// Paged caches of many sequences (gfx950): a step's plan, the pack of its new rows, pages read back, rows moved.
+//
+// A plan is made on the host once a step and read by every layer's launches, so no kernel searches a table: a workgroup
+// loads one record that names its pages, rows and share of the work.
+#include "dkv_paged.h"
+#include "dkv_rope_pack.h"
+#include <string.h>
+#include <algorithm>
+#include <new>
+#include <vector>
+
+namespace dkv {
+namespace paged {
+
+// ---- the pack ----------------------------------------------------------------------------------------------------
+
+// A row held by 8 lanes (lane c: elements [8 c, 8 c + 8)) into a page, with dkv_pack's arithmetic.
+template <int BITS>
+__device__ __forceinline__ void pack_row(const u32x4& w, bool valid, int c, uint8_t* sub, int row) {
+  if (BITS == 16) {
+    if (valid) __builtin_nontemporal_store(w, reinterpret_cast<u32x4*>(sub + row * 128 + 16 * c));
+    return;
+  }
+  float x[8];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[2 * e] = bf16_lo(w[e]), x[2 * e + 1] = bf16_hi(w[e]);
+  float lo = x[0], hi = x[0];
+  uint32_t nz = 0;  // the row holds a -0 (zero_min_sign)
+#pragma unroll
+  for (int e = 0; e < 8; ++e) lo = fminf(lo, x[e]), hi = fmaxf(hi, x[e]), nz |= __float_as_uint(x[e]) == 0x80000000u;
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) {
+    lo = fminf(lo, __shfl_xor(lo, o));
+    hi = fmaxf(hi, __shfl_xor(hi, o));
+    nz |= __shfl_xor(nz, o);
+  }
+  const float a = lo == 0.0f ? zero_min_sign(nz) : lo;
+  const float span = hi - a;
+  const float s = span > 0.0f ? __fdiv_rn(span, BITS == 4 ? 15.0f : 255.0f) : 1.0f;
+  const float rs = __builtin_amdgcn_rcpf(s);
+  const bool fast = s >= 0x1p-126f && s <= 0x1p125f;
+  uint32_t out[2];
+  quantize8<BITS>(x, a, s, rs, fast, out);
+  if (!valid) return;
+  if (BITS == 4) __builtin_nontemporal_store(out[0], reinterpret_cast<uint32_t*>(sub + row * 32 + 4 * c));
+  else __builtin_nontemporal_store((uint64_t)out[1] << 32 | out[0], reinterpret_cast<uint64_t*>(sub + row * 64 + 8 * c));
+  if (c == 0)
+    __builtin_nontemporal_store((uint64_t)__float_as_uint(s) << 32 | __float_as_uint(a),
+                                reinterpret_cast<uint64_t*>(sub + TILE * 8 * BITS + 8 * row));
+}
+
+// A wave takes the rows of one item (up to 64 tokens of a page) of one K or V head, 8 lanes a row, all loads before the
+// first use.
+__global__ __launch_bounds__(256) void append_kernel(dkv_paged_args a) {
+  const int32_t* plan = static_cast<const int32_t*>(a.plan_words);
+  if (a.bounds && (int)blockIdx.x >= plan[N_ITEMS]) return;
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63, H = a.plan.heads;
+  const int kvh = blockIdx.y * 4 + wave;
+  if (kvh >= 2 * H) return;
+  const dkv_page_rows item = reinterpret_cast<const dkv_page_rows*>(plan + a.plan.at_items)[blockIdx.x];
+  const int kv = kvh >= H, h = kvh - kv * H, c = lane & 7, r0 = lane >> 3;
+  const uint16_t* src = static_cast<const uint16_t*>(kv ? a.v_new : a.k_new) +
+                        (kv ? h * a.vn_head_stride + item.token * a.vn_tok_stride : h * a.kn_head_stride + item.token * a.kn_tok_stride);
+  const int64_t stride = kv ? a.vn_tok_stride : a.kn_tok_stride;
+  const int bits = page_bits(item.page);
+  uint8_t* sub = static_cast<uint8_t*>(a.arena) + page_at(item.page, a.layer, a.plan.layers, H, 0) + (int64_t)kvh * page_sub(bits);
+  u32x4 w[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (8 * i < item.rows)
+      w[i] = *reinterpret_cast<const u32x4*>(src + min(8 * i + r0, item.rows - 1) * stride + 8 * c);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (8 * i >= item.rows) break;
+    const int r = 8 * i + r0;
+    const bool valid = r < item.rows;
+    if (bits == 4) pack_row<4>(w[i], valid, c, sub, item.row0 + r);
+    else if (bits == 8) pack_row<8>(w[i], valid, c, sub, item.row0 + r);
+    else pack_row<16>(w[i], valid, c, sub, item.row0 + r);
+  }
+}
+
+// ---- pages read back ---------------------------------------------------------------------------------------------
+
+constexpr int ARG_ITEMS = 128;  // records of a launch's argument block
+struct Items {
+  dkv_page_rows at[ARG_ITEMS];
+};
+
+// A workgroup: the rows of one item of one (layer, K or V, head), four lanes a row.
+__global__ __launch_bounds__(256) void read_kernel(Items items, const uint8_t* __restrict__ arena, int layer0, int n_layers, int layers,
+                                                   int heads, void* __restrict__ out, int64_t n_tokens, int out_dtype) {
+  const dkv_page_rows item = items.at[blockIdx.x];
+  const int r = threadIdx.x >> 2, c = threadIdx.x & 3;
+  if (r >= item.rows) return;
+  const int kvh = blockIdx.y, kv = kvh >= heads, h = kvh - kv * heads, bits = page_bits(item.page), row = item.row0 + r;
+  for (int l = blockIdx.z; l < n_layers; l += gridDim.z) {
+    const uint8_t* sub = arena + page_at(item.page, layer0 + l, layers, heads, 0) + (int64_t)kvh * page_sub(bits);
+    const uint8_t* p = sub + row * (8 * bits) + c * (2 * bits);
+    float x[16];
+    if (bits == 16) {
+      const u32x4 w0 = reinterpret_cast<const u32x4*>(p)[0], w1 = reinterpret_cast<const u32x4*>(p)[1];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        x[2 * i] = bf16_lo(w0[i]), x[2 * i + 1] = bf16_hi(w0[i]), x[8 + 2 * i] = bf16_lo(w1[i]), x[9 + 2 * i] = bf16_hi(w1[i]);
+    } else {
+      const float2 as = reinterpret_cast<const float2*>(sub + TILE * 8 * bits)[row];
+      uint32_t code[16];
+      if (bits == 4) {
+        const uint2 w = *reinterpret_cast<const uint2*>(p);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) code[i] = (w.x >> (4 * i)) & 15u, code[8 + i] = (w.y >> (4 * i)) & 15u;
+      } else {
+        const u32x4 w = *reinterpret_cast<const u32x4*>(p);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) code[i] = (w[i >> 2] >> (8 * (i & 3))) & 255u;
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = __fadd_rn(__fmul_rn((float)code[i], as.y), as.x);
+    }
+    const int64_t o = ((((int64_t)kv * n_layers + l) * heads + h) * n_tokens + item.token + r) * D + c * 16;
+    if (out_dtype == 1) {
+      float4* dst = reinterpret_cast<float4*>(static_cast<float*>(out) + o);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) dst[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+    } else {
+      u32x4* dst = reinterpret_cast<u32x4*>(static_cast<uint16_t*>(out) + o);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        dst[i] = u32x4{pack_bf16(x[8 * i], x[8 * i + 1]), pack_bf16(x[8 * i + 2], x[8 * i + 3]),
+                       pack_bf16(x[8 * i + 4], x[8 * i + 5]), pack_bf16(x[8 * i + 6], x[8 * i + 7])};
+    }
+  }
+}
+
+// ---- rows moved --------------------------------------------------------------------------------------------------
+
+constexpr int ARG_MOVES = 128;
+struct Moves {
+  dkv_page_move at[ARG_MOVES];
+};
+
+// A wave moves the rows of one (layer, K or V, head) of a move: payload and (offset, scale) pairs, which lie behind as
+// many rows as the tile has room for.
+__global__ __launch_bounds__(256) void move_kernel(Moves moves, const uint8_t* __restrict__ src, uint8_t* __restrict__ dst, int subs) {
+  const dkv_page_move m = moves.at[blockIdx.x];
+  const int sub = blockIdx.y * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (sub >= subs) return;
+  const int row = 8 * m.bits;
+  const uint8_t* from = src + m.src_offset + sub * subblock_bytes(m.src_rows, m.bits);
+  uint8_t* to = dst + m.dst_offset + (int64_t)sub * page_sub(m.bits);
+  const u32x4* f = reinterpret_cast<const u32x4*>(from + m.src_row * row);
+  u32x4* t = reinterpret_cast<u32x4*>(to + m.dst_row * row);
+  const int n = m.rows * row / 16;  // up to 512 pieces
+  u32x4 w[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (64 * i + lane < n) w[i] = f[64 * i + lane];
+  uint2 as = make_uint2(0, 0);
+  const bool scaled = m.bits < 16 && lane < m.rows;
+  if (scaled) as = reinterpret_cast<const uint2*>(from + m.src_rows * row)[m.src_row + lane];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (64 * i + lane < n) t[64 * i + lane] = w[i];
+  if (scaled) reinterpret_cast<uint2*>(to + TILE * row)[m.dst_row + lane] = as;
+}
+
+// ---- plans -------------------------------------------------------------------------------------------------------
+
+// Workgroups of a launch of the short kernel over all KV heads, about (a workgroup has four waves, a unit each at a time).
+constexpr int SHORT_TARGET = 1024;
+constexpr int SHORT_MIN_UNITS = 4;
+constexpr int SHARED_MIN = 4;  // pages that neighbours have in common to be attended to as a group
+
+struct Entity {  // a sequence's own part, or what a group of sequences has in common
+  int first_page, n_pages, token0, count, units, part, splits;
+};
+
+static int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+
+static int check_batch(const dkv_paged_batch& b, const char* what) {
+  if (b.seqs <= 0 || !b.count || !b.past || !b.position || !b.first || b.layers <= 0 || b.heads <= 0 || b.q_heads <= 0 ||
+      b.q_heads % b.heads || b.max_pages < 0) {
+    set_error("%s: bad batch (seqs %d, layers %d, heads %d, q_heads %d) or a null array", what, b.seqs, b.layers, b.heads, b.q_heads);
+    return DKV_EINVAL;
+  }
+  if ((int64_t)b.layers * b.heads > 65535 / 2 || b.heads > 16384 || b.q_heads / b.heads > 4096) {
+    set_error("%s: too many layers or heads (%d layers, %d of %d heads)", what, b.layers, b.heads, b.q_heads);
+    return DKV_EINVAL;
+  }
+  int64_t tokens = 0;
+  for (int i = 0; i < b.seqs; ++i) {
+    if (b.count[i] <= 0 || b.past[i] < 0 || (int64_t)b.past[i] + b.count[i] > INT32_MAX) {
+      set_error("%s: sequence %d has %d new tokens after %d", what, i, b.count[i], b.past[i]);
+      return DKV_EINVAL;
+    }
+    tokens += b.count[i];
+  }
+  if (tokens * (b.q_heads / b.heads) > 1 << 24 || tokens > 1 << 22) {
+    set_error("%s: %lld new tokens are too many for one step", what, (long long)tokens);
+    return DKV_EINVAL;
+  }
+  return 0;
+}
+
+// The places and bounds of a plan of these counts, whatever the history.
+static void layout_of(const dkv_paged_batch& b, dkv_paged_plan& p) {
+  const int G = b.q_heads / b.heads;
+  int64_t tokens = 0, items = 0, blocks = 0;
+  for (int i = 0; i < b.seqs; ++i) {
+    tokens += b.count[i];
+    items += ceil_div(b.count[i], TILE) + 1;
+    blocks += ceil_div((int64_t)b.count[i] * G, SHORT_BLOCK);
+  }
+  const int64_t grouped = ceil_div(tokens * G, SHORT_BLOCK) + b.seqs / 2;  // blocks of what groups have in common
+  p.seqs = b.seqs, p.tokens = (int)tokens, p.layers = b.layers, p.heads = b.heads, p.q_heads = b.q_heads;
+  p.max_items = (int)items;
+  p.max_pages = b.max_pages;
+  p.max_work = (int)(blocks + grouped + ceil_div(SHORT_TARGET, b.heads));
+  p.max_long = 0;
+  p.max_merges = (int)blocks;
+  p.max_rows = p.max_work * SHORT_BLOCK;
+  auto up = [](int64_t x) { return (x + 15) & ~(int64_t)15; };
+  int64_t at = HEAD_WORDS;
+  p.at_items = (int)at, at += up(4 * items);
+  p.at_positions = (int)at, at += up(2 * tokens);
+  p.at_pages = (int)at, at += up(2 * (int64_t)b.max_pages);
+  p.at_work = (int)at, at += up(8ll * p.max_work);
+  p.at_long = (int)at, at += up(8ll * p.max_long);
+  p.at_merges = (int)at, at += up(8ll * p.max_merges);
+  p.words = (int)at;
+}
+
+static bool plan_fits(const dkv_paged_batch& b) {  // (the offsets are 32-bit)
+  int64_t tokens = 0;
+  for (int i = 0; i < b.seqs; ++i) tokens += b.count[i];
+  return 64 * tokens * (b.q_heads / b.heads) + 64ll * b.seqs + 2ll * b.max_pages + (1 << 20) < INT32_MAX;
+}
+
+// Splits of every entity so that about `target` workgroups a KV head share all units, `least` units each at least.
+static void split(std::vector<Entity>& es, int G, int block, int target, int least) {
+  int64_t total = 0;
+  for (const Entity& e : es) total += (int64_t)e.units * ceil_div((int64_t)e.count * G, block);
+  const int64_t len = std::max<int64_t>(least, (total + target - 1) / target);
+  for (Entity& e : es) e.splits = std::max(1, ceil_div(e.units, len));
+}
+
+static int write_plan(const dkv_paged_batch& b, int32_t* w, dkv_paged_plan& p) {
+  const int G = b.q_heads / b.heads;
+  layout_of(b, p);
+  const int64_t grain = grain_bytes(b.layers, b.heads), grains = b.arena_bytes / grain;
+  dkv_page_rows* items = reinterpret_cast<dkv_page_rows*>(w + p.at_items);
+  Page* pages = reinterpret_cast<Page*>(w + p.at_pages);
+  std::vector<Entity> own(b.seqs);
+  std::vector<int> rows_at;  // of the step's new rows
+  int n_items = 0, n_pages = 0, token0 = 0;
+  for (int i = 0; i < b.seqs; ++i) {
+    const int from = b.first[i], to = b.first[i + 1];
+    if (from < 0 || to < from || (to > from && (!b.page || !b.rows))) {
+      set_error("dkv_paged_plan_write: sequence %d has pages [%d, %d)", i, from, to);
+      return DKV_EINVAL;
+    }
+    Entity& e = own[i];
+    e = Entity{n_pages, 0, token0, b.count[i], 0, -1, 1};
+    int64_t held = 0;
+    const int64_t end = (int64_t)b.past[i] + b.count[i];
+    for (int j = from; j < to; ++j) {
+      const int code = b.page[j] & 3, rows = b.rows[j];
+      if (code > 2 || (int64_t)(b.page[j] >> 2) + page_grains(4 << code) > grains) {
+        set_error("dkv_paged_plan_write: page %u of sequence %d lies outside the arena", b.page[j], i);
+        return DKV_EINVAL;
+      }
+      if (rows <= 0 || rows > TILE || held + rows > end) {
+        set_error("dkv_paged_plan_write: a page of sequence %d has %d tokens after %lld of %lld", i, rows, (long long)held, (long long)end);
+        return DKV_EINVAL;
+      }
+      const int old = (int)std::min<int64_t>(std::max<int64_t>(b.past[i] - held, 0), rows);
+      if (old > 0) {
+        if (n_pages >= b.max_pages) {
+          set_error("dkv_paged_plan_write: the histories have more than the %d pages that the plan has room for", b.max_pages);
+          return DKV_EINVAL;
+        }
+        pages[n_pages++] = Page{b.page[j], old};
+        ++e.n_pages;
+      }
+      if (old < rows) {
+        if (n_items >= p.max_items) {
+          set_error("dkv_paged_plan_write: the %d new tokens of sequence %d lie in more pages than they need", b.count[i], i);
+          return DKV_EINVAL;
+        }
+        items[n_items++] = dkv_page_rows{token0 + (int)(held + old - b.past[i]), b.page[j], old, rows - old};
+      }
+      held += rows;
+    }
+    if (held != end) {
+      set_error("dkv_paged_plan_write: the pages of sequence %d hold %lld tokens, not %lld", i, (long long)held, (long long)end);
+      return DKV_EINVAL;
+    }
+    int64_t* positions = reinterpret_cast<int64_t*>(w + p.at_positions) + token0;
+    for (int t = 0; t < b.count[i]; ++t) positions[t] = (int64_t)b.position[i] + t;
+    token0 += b.count[i];
+  }
+  // Neighbours that begin with the same pages attend to these as one entity, whose query rows are all their tokens'.
+  std::vector<Entity> all;
+  std::vector<int> group(b.seqs, -1);
+  for (int i = 0; i < b.seqs;) {
+    int same = 0, j = i + 1;
+    for (; j < b.seqs; ++j) {
+      const int most = std::min(j == i + 1 ? own[i].n_pages : same, own[j].n_pages);
+      int n = 0;
+      while (n < most && pages[own[i].first_page + n].page == pages[own[j].first_page + n].page &&
+             pages[own[i].first_page + n].rows == pages[own[j].first_page + n].rows)
+        ++n;
+      if (n < SHARED_MIN || 2 * n < same) break;
+      same = n;
+    }
+    if (same) {
+      Entity g{own[i].first_page, same, own[i].token0, 0, same, -1, 1};
+      for (int k = i; k < j; ++k) {
+        g.count += own[k].count, group[k] = (int)all.size();
+        own[k].first_page += same, own[k].n_pages -= same;
+      }
+      all.push_back(g);
+    }
+    i = j;
+  }
+  const int groups = (int)all.size();
+  for (Entity& e : own) {
+    e.units = e.n_pages + ceil_div(e.count, TILE);
+    all.push_back(e);
+  }
+  split(all, G, SHORT_BLOCK, ceil_div(SHORT_TARGET, b.heads), SHORT_MIN_UNITS);
+  int64_t rows = 0;
+  for (size_t i = 0; i < all.size(); ++i) {
+    Entity& e = all[i];
+    if ((int)i < groups || e.splits > 1 || group[i - groups] >= 0) {
+      e.part = (int)rows;
+      rows += (int64_t)e.splits * e.count * G;
+    }
+  }
+  Work* work = reinterpret_cast<Work*>(w + p.at_work);
+  int n_work = 0, n_merges = 0;
+  for (size_t i = 0; i < all.size(); ++i) {
+    const Entity& e = all[i];
+    for (int blk = 0; blk < ceil_div((int64_t)e.count * G, SHORT_BLOCK); ++blk) {
+      const int last = (int)std::min<int64_t>(((int64_t)(blk + 1) * SHORT_BLOCK - 1) / G, e.count - 1);
+      const int units = (int)i < groups ? e.units : e.n_pages + last / TILE + 1;  // up to the block's last token
+      for (int s = 0; s < e.splits; ++s)
+        work[n_work++] = Work{e.first_page, e.n_pages, e.token0, e.count, blk, (int)((int64_t)units * s / e.splits),
+                              (int)((int64_t)units * (s + 1) / e.splits), e.part < 0 ? -1 : e.part + s * e.count * G};
+    }
+  }
+  Merge* merges = reinterpret_cast<Merge*>(w + p.at_merges);
+  for (int i = 0; i < b.seqs; ++i) {
+    const Entity& e = all[groups + i];
+    if (e.part < 0) continue;
+    for (int r = 0; r < e.count * G; r += SHORT_BLOCK) {
+      Merge m{e.token0, e.count * G, r, e.part, e.splits, 0, 0, 0};
+      if (group[i] >= 0) {
+        const Entity& g = all[group[i]];
+        m.shared = g.part + (e.token0 - g.token0) * G, m.shared_splits = g.splits, m.shared_stride = g.count * G;
+      }
+      merges[n_merges++] = m;
+    }
+  }
+  p.items = n_items, p.work = n_work, p.long_work = 0, p.merges = n_merges, p.rows = (int)rows;
+  w[N_ITEMS] = n_items, w[N_WORK] = n_work, w[N_LONG] = 0, w[N_MERGES] = n_merges;
+  return 0;
+}
+
+int check_args(const dkv_paged_args& a, bool attend, const char* what) {
+  const dkv_paged_plan& p = a.plan;
+  auto a16 = [](const void* x) { return ((uintptr_t)x & 15) == 0; };
+  if (!a.k_new || !a.v_new || !a.arena || !a.plan_words || (attend && (!a.q || !a.out))) {
+    set_error("%s: null pointer argument", what);
+  } else if (p.seqs <= 0 || p.tokens <= 0 || p.heads <= 0 || p.q_heads <= 0 || p.q_heads % p.heads || a.layer < 0 || a.layer >= p.layers) {
+    set_error("%s: not a plan (seqs %d, heads %d of %d), or layer %d of %d", what, p.seqs, p.heads, p.q_heads, a.layer, p.layers);
+  } else if (!a16(a.k_new) || !a16(a.v_new) || !a16(a.arena) || !a16(a.plan_words) || (a.kn_head_stride & 7) || (a.kn_tok_stride & 7) ||
+             (a.vn_head_stride & 7) || (a.vn_tok_stride & 7)) {
+    set_error("%s: K, V, arena and plan must be 16-byte aligned with strides that are multiples of 8 elements", what);
+  } else if (attend && (!a16(a.q) || !a16(a.out) || (a.q_head_stride & 7) || (a.q_tok_stride & 7) || (a.out_tok_stride & 3) ||
+                        (a.out_head_stride & 3) || a.out_dtype < 0 || a.out_dtype > 1)) {
+    set_error("%s: Q and out must be 16-byte aligned, strides multiples of 8 and 4 elements, out bf16 (0) or fp32 (1)", what);
+  } else if (attend && (a.precision < 0 || a.precision > 1)) {
+    set_error("%s: precision must be 0 (bf16) or 1 (fp32)", what);
+  } else if (attend && p.tokens > 1 && (a.kn_tok_stride < 0 || a.kn_tok_stride >= 1 << 23 || a.vn_tok_stride < 0 || a.vn_tok_stride >= 1 << 23)) {
+    set_error("%s: K's and V's token strides must be from 0 to 2^23 - 1 elements", what);
+  } else {
+    return 0;
+  }
+  return DKV_EINVAL;
+}
+
+}  // namespace paged
+}  // namespace dkv
+
+using namespace dkv;
+using namespace dkv::paged;
+
+extern "C" {
+
+int64_t dkv_page_grain(int32_t layers, int32_t heads) { return layers > 0 && heads > 0 ? grain_bytes(layers, heads) : 0; }
+
+int64_t dkv_paged_plan_bytes(const dkv_paged_batch* batch) {
+  if (!batch || check_batch(*batch, "dkv_paged_plan_bytes") || !plan_fits(*batch)) return 0;
+  dkv_paged_plan p{};
+  layout_of(*batch, p);
+  return 4ll * p.words;
+}
+
+int dkv_paged_plan_write(const dkv_paged_batch* batch, void* buffer, int64_t bytes, dkv_paged_plan* plan) {
+  clear_error();
+  if (!batch || !buffer || !plan || ((uintptr_t)buffer & 15)) {
+    set_error("dkv_paged_plan_write: null or misaligned pointer argument");
+    return DKV_EINVAL;
+  }
+  if (int rc = check_batch(*batch, "dkv_paged_plan_write")) return rc;
+  const int64_t need = dkv_paged_plan_bytes(batch);
+  if (!need || bytes < need) {
+    set_error("dkv_paged_plan_write: a plan of %lld bytes needed, room for %lld", (long long)need, (long long)bytes);
+    return DKV_EINVAL;
+  }
+  try {
+    dkv_paged_plan p{};
+    if (int rc = write_plan(*batch, static_cast<int32_t*>(buffer), p)) return rc;
+    *plan = p;
+    return 0;
+  } catch (const std::exception&) {
+    set_error("dkv_paged_plan_write: out of host memory");
+    return DKV_EINVAL;
+  }
+}
+
+int dkv_paged_append(const dkv_paged_args* args, void* stream) {
+  clear_error();
+  if (!args) {
+    set_error("dkv_paged_append: null args");
+    return DKV_EINVAL;
+  }
+  if (int rc = check_args(*args, false, "dkv_paged_append")) return rc;
+  const dkv_paged_plan& p = args->plan;
+  hipLaunchKernelGGL(append_kernel, dim3(args->bounds ? p.max_items : p.items, (2 * p.heads + 3) / 4), dim3(256), 0, (hipStream_t)stream,
+                     *args);
+  return (int)hipGetLastError();
+}
+
+int dkv_paged_read(const void* arena, int64_t arena_bytes, const dkv_page_rows* items, int32_t n_items, int32_t layer0,
+                   int32_t n_layers, int32_t layers, int32_t heads, void* out, int32_t n_tokens, int32_t out_dtype, void* stream) {
+  clear_error();
+  if (n_items < 0 || n_tokens < 0 || layer0 < 0 || n_layers <= 0 || (int64_t)layer0 + n_layers > layers || heads <= 0 ||
+      (int64_t)layers * heads > 65535 / 2 || out_dtype < 0 || out_dtype > 1) {
+    set_error("dkv_paged_read: bad shape (items %d, tokens %d, layers [%d, %d + %d) of %d, heads %d)", n_items, n_tokens, layer0, layer0,
+              n_layers, layers, heads);
+    return DKV_EINVAL;
+  }
+  if (n_items == 0) return 0;
+  if (!arena || !items || !out || ((uintptr_t)arena & 15) || ((uintptr_t)out & 15)) {
+    set_error("dkv_paged_read: null or misaligned pointer argument");
+    return DKV_EINVAL;
+  }
+  const int64_t grains = arena_bytes / grain_bytes(layers, heads);
+  for (int i = 0; i < n_items; ++i) {
+    const dkv_page_rows& r = items[i];
+    if ((r.page & 3) > 2 || (int64_t)(r.page >> 2) + page_grains(page_bits(r.page)) > grains || r.row0 < 0 || r.rows <= 0 ||
+        r.row0 > TILE - r.rows || r.token < 0 || r.token > n_tokens - r.rows) {
+      set_error("dkv_paged_read: item %d (page %u, rows [%d, %d + %d), token %d) lies outside the arena, its page or the output", i,
+                r.page, r.row0, r.row0, r.rows, r.token);
+      return DKV_EINVAL;
+    }
+  }
+  for (int i = 0; i < n_items; i += ARG_ITEMS) {
+    const int n = std::min(ARG_ITEMS, n_items - i);
+    Items block{};
+    memcpy(block.at, items + i, n * sizeof(dkv_page_rows));
+    hipLaunchKernelGGL(read_kernel, dim3(n, 2 * heads, std::min(n_layers, 32768)), dim3(256), 0, (hipStream_t)stream, block,
+                       static_cast<const uint8_t*>(arena), layer0, n_layers, layers, heads, out, (int64_t)n_tokens, out_dtype);
+    if (const int rc = (int)hipGetLastError()) return rc;
+  }
+  return 0;
+}
+
+int dkv_paged_move(const void* src, int64_t src_bytes, void* dst, int64_t dst_bytes, const dkv_page_move* moves, int32_t n_moves,
+                   int32_t layers, int32_t heads, void* stream) {
+  clear_error();
+  if (n_moves < 0 || layers <= 0 || heads <= 0 || (int64_t)layers * heads > 65535 / 2) {
+    set_error("dkv_paged_move: bad shape (moves %d, layers %d, heads %d)", n_moves, layers, heads);
+    return DKV_EINVAL;
+  }
+  if (n_moves == 0) return 0;
+  if (!src || !dst || !moves || ((uintptr_t)src & 15) || ((uintptr_t)dst & 15)) {
+    set_error("dkv_paged_move: null or misaligned pointer argument");
+    return DKV_EINVAL;
+  }
+  struct Span {  // tiles that are read (or pages that are written) by a move
+    int64_t at, end;
+    int row, rows;
+    bool write;
+  };
+  try {
+    std::vector<Span> spans;
+    for (int i = 0; i < n_moves; ++i) {
+      const dkv_page_move& m = moves[i];
+      const int64_t from = slab_bytes(m.src_rows, m.bits, layers, heads), to = slab_bytes(TILE, m.bits, layers, heads);
+      if ((m.bits != 4 && m.bits != 8 && m.bits != 16) || m.rows < 1 || m.src_rows > TILE || m.src_row + m.rows > m.src_rows ||
+          m.dst_row + m.rows > TILE || m.src_offset < 0 || (m.src_offset & 15) || m.src_offset > src_bytes - from || m.dst_offset < 0 ||
+          (m.dst_offset & 15) || m.dst_offset > dst_bytes - to) {
+        set_error("dkv_paged_move: move %d (%d bits, rows [%d, +%d) of %d at byte %lld to row %d at %lld) lies outside an arena or tile", i,
+                  m.bits, m.src_row, m.rows, m.src_rows, (long long)m.src_offset, m.dst_row, (long long)m.dst_offset);
+        return DKV_EINVAL;
+      }
+      spans.push_back(Span{m.dst_offset, m.dst_offset + to, m.dst_row, m.rows, true});
+      if (src == dst) spans.push_back(Span{m.src_offset, m.src_offset + from, m.src_row, m.rows, false});
+    }
+    // Sorted by place, spans of one page follow each other: two of them may meet only in rows that neither shares, or where both read.
+    std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.at != b.at ? a.at < b.at : a.row < b.row; });
+    int64_t reach = -1, reach_write = -1;  // ends of the spans before, of those that write
+    for (size_t i = 0, j; i < spans.size(); i = j) {
+      bool writes = false, clash = false;
+      int rows_end = 0, write_end = 0;
+      int64_t end = spans[i].end;
+      for (j = i; j < spans.size() && spans[j].at == spans[i].at; ++j) {
+        const Span& s = spans[j];
+        clash = clash || s.end != spans[i].end || s.row < (s.write ? rows_end : write_end);
+        rows_end = std::max(rows_end, s.row + s.rows);
+        if (s.write) writes = true, write_end = std::max(write_end, s.row + s.rows);
+        end = std::max(end, s.end);
+      }
+      if (clash || spans[i].at < (writes ? reach : reach_write)) {
+        set_error("dkv_paged_move: the moves write rows (at byte %lld) that they also read or write elsewhere", (long long)spans[i].at);
+        return DKV_EINVAL;
+      }
+      reach = std::max(reach, end);
+      if (writes) reach_write = std::max(reach_write, end);
+    }
+  } catch (const std::exception&) {
+    set_error("dkv_paged_move: out of host memory");
+    return DKV_EINVAL;
+  }
+  const int subs = 2 * layers * heads;
+  for (int i = 0; i < n_moves; i += ARG_MOVES) {
+    const int n = std::min(ARG_MOVES, n_moves - i);
+    Moves block{};
+    memcpy(block.at, moves + i, n * sizeof(dkv_page_move));
+    hipLaunchKernelGGL(move_kernel, dim3(n, (subs + 3) / 4), dim3(256), 0, (hipStream_t)stream, block, static_cast<const uint8_t*>(src),
+                       static_cast<uint8_t*>(dst), subs);
+    if (const int rc = (int)hipGetLastError()) return rc;
+  }
+  return 0;
+}
+
+}  // extern "C"

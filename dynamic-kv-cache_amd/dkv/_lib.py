@@ -86,6 +86,31 @@ class Sampling(ctypes.Structure):
                 ('min_p_rows', ctypes.c_void_p), ('top_k_rows', ctypes.c_void_p)]
 
 
+class PagedBatch(ctypes.Structure):
+    _fields_ = [('seqs', ctypes.c_int32), ('count', ctypes.c_void_p), ('past', ctypes.c_void_p), ('position', ctypes.c_void_p),
+                ('first', ctypes.c_void_p), ('page', ctypes.c_void_p), ('rows', ctypes.c_void_p),
+                ('layers', ctypes.c_int32), ('heads', ctypes.c_int32), ('q_heads', ctypes.c_int32),
+                ('arena_bytes', ctypes.c_int64), ('max_pages', ctypes.c_int32)]
+
+
+class PagedPlan(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_int32) for name in (
+        'seqs', 'tokens', 'layers', 'heads', 'q_heads', 'words', 'at_items', 'at_positions', 'at_pages', 'at_work', 'at_long',
+        'at_merges', 'items', 'work', 'long_work', 'merges', 'rows', 'max_items', 'max_pages', 'max_work', 'max_long', 'max_merges',
+        'max_rows')]
+
+
+class PagedArgs(ctypes.Structure):
+    _fields_ = [('q', ctypes.c_void_p), ('q_head_stride', ctypes.c_int64), ('q_tok_stride', ctypes.c_int64),
+                ('k_new', ctypes.c_void_p), ('kn_head_stride', ctypes.c_int64), ('kn_tok_stride', ctypes.c_int64),
+                ('v_new', ctypes.c_void_p), ('vn_head_stride', ctypes.c_int64), ('vn_tok_stride', ctypes.c_int64),
+                ('arena', ctypes.c_void_p), ('arena_bytes', ctypes.c_int64), ('plan_words', ctypes.c_void_p),
+                ('plan', PagedPlan), ('layer', ctypes.c_int32), ('bounds', ctypes.c_int32), ('scale', ctypes.c_float),
+                ('out', ctypes.c_void_p), ('out_tok_stride', ctypes.c_int64), ('out_head_stride', ctypes.c_int64),
+                ('out_dtype', ctypes.c_int32), ('precision', ctypes.c_int32),
+                ('workspace', ctypes.c_void_p), ('workspace_bytes', ctypes.c_int64)]
+
+
 assert ctypes.sizeof(Tile) == 16
 
 
@@ -186,6 +211,18 @@ SIGNATURES = [
                                   ctypes.c_void_p, ctypes.c_int32, ctypes.POINTER(Sampling), ctypes.c_void_p,
                                   ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]),
     ('dkv_sample_workspace_bytes', ctypes.c_int64, [ctypes.c_int32, ctypes.c_int32]),
+    ('dkv_page_grain', ctypes.c_int64, [ctypes.c_int32, ctypes.c_int32]),
+    ('dkv_paged_plan_bytes', ctypes.c_int64, [ctypes.POINTER(PagedBatch)]),
+    ('dkv_paged_plan_write', ctypes.c_int, [ctypes.POINTER(PagedBatch), ctypes.c_void_p, ctypes.c_int64,
+                                            ctypes.POINTER(PagedPlan)]),
+    ('dkv_paged_append', ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
+    ('dkv_paged_workspace_bytes', ctypes.c_int64, [ctypes.c_void_p]),
+    ('dkv_paged_attend', ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
+    ('dkv_paged_read', ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32,
+                                      ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p, ctypes.c_int32,
+                                      ctypes.c_int32, ctypes.c_void_p]),
+    ('dkv_paged_move', ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
+                                      ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p]),
 ]
 
 

@@ -497,6 +497,109 @@ int dkv_sample(const void* logits, int32_t dtype, int64_t row_stride, int32_t ro
                void* workspace, int64_t workspace_bytes, void* stream);
 int64_t dkv_sample_workspace_bytes(int32_t rows, int32_t vocab);
 
+/* Paged caches: many sequences in one arena, in pages of 64 tokens that sequences may share. No counterpart in the
+ * reference, whose cache holds one sequence.
+ *
+ * A page is a tile of 64 rows (dkv_subblock_bytes(64, bits) a sub-block) that need not all be filled. Pages lie at
+ * multiples of a grain, dkv_page_grain(layers, heads) bytes; 4-, 8- and 16-bit pages take 5, 9 and 16 grains. A page
+ * is named by its first grain * 4 + its width's code (0, 1, 2 for 4, 8, 16 bits). */
+#define DKV_PAGE_WORD(grain, code) ((uint32_t)(grain) << 2 | (code))
+int64_t dkv_page_grain(int32_t layers, int32_t heads);
+
+/* Rows [row0, row0 + rows) of a page. */
+typedef struct dkv_page_rows {
+  int32_t token; /* where its first row is, or goes to, in a tensor of tokens */
+  uint32_t page;
+  int32_t row0, rows;
+} dkv_page_rows;
+
+/* One step: `count[i]` new tokens of sequence i, one sequence after the other in the step's tensors, after `past[i]`
+ * tokens that it holds. Its pages are page[first[i]..first[i + 1]) in token order with the tokens that each holds
+ * after the step, past[i] + count[i] together. All arrays are HOST memory. */
+typedef struct dkv_paged_batch {
+  int32_t seqs;
+  const int32_t* count;    /* [seqs], from 1 on */
+  const int32_t* past;     /* [seqs] */
+  const int32_t* position; /* [seqs]: of each sequence's first new token */
+  const int32_t* first;    /* [seqs + 1] */
+  const uint32_t* page;
+  const int32_t* rows;
+  int32_t layers, heads, q_heads;
+  int64_t arena_bytes;
+  int32_t max_pages; /* room for this many pages in the plan: replays may have more than the first call */
+} dkv_paged_batch;
+
+/* What a plan holds, in 32-bit words from its start: `at_*` say where, the counts what of it this step uses, `max_*`
+ * what a step of the same counts uses at most, whatever its history. */
+typedef struct dkv_paged_plan {
+  int32_t seqs, tokens, layers, heads, q_heads;
+  int32_t words; /* of the whole plan */
+  int32_t at_items, at_positions, at_pages, at_work, at_long, at_merges;
+  int32_t items, work, long_work, merges, rows;
+  int32_t max_items, max_pages, max_work, max_long, max_merges, max_rows;
+} dkv_paged_plan;
+
+/* Writes a step's plan: what the kernels below read, the same for every layer. buffer (HOST, dkv_paged_plan_bytes()
+ * bytes at least) goes to the device as it is; `plan` describes it. Checked here, since the kernels trust the device
+ * copy: pages inside the arena, rows that sum up, counts. The positions of the new tokens are in it as int64 from
+ * word at_positions on. A plan may be written again over an older one of the same counts and max_pages (steps that
+ * replay a captured graph): the places stay the same. */
+int64_t dkv_paged_plan_bytes(const dkv_paged_batch* batch);
+int dkv_paged_plan_write(const dkv_paged_batch* batch, void* buffer, int64_t bytes, dkv_paged_plan* plan);
+
+/* One layer's launch over a step. */
+typedef struct dkv_paged_args {
+  const void* q;     /* bf16 [q_heads, tokens, 64] */
+  int64_t q_head_stride, q_tok_stride;
+  const void* k_new; /* bf16 [heads, tokens, 64] */
+  int64_t kn_head_stride, kn_tok_stride;
+  const void* v_new;
+  int64_t vn_head_stride, vn_tok_stride;
+  void* arena;
+  int64_t arena_bytes;
+  const void* plan_words; /* DEVICE copy of the plan */
+  dkv_paged_plan plan;
+  int32_t layer;
+  int32_t bounds; /* nonzero: the launch is sized for any plan of these counts (it is captured and will be replayed
+                     over plans written later) */
+  float scale;
+  void* out; /* [tokens, q_heads, 64] with the strides below */
+  int64_t out_tok_stride, out_head_stride;
+  int32_t out_dtype; /* 0 = bf16, 1 = fp32 */
+  int32_t precision; /* 0: packed rows' values are rounded to bf16; 1: taken as they are stored */
+  void* workspace;
+  int64_t workspace_bytes;
+} dkv_paged_args;
+
+/* Packs the step's new rows of a layer into their pages, byte for byte what dkv_pack writes (q and out are not
+ * read). */
+int dkv_paged_append(const dkv_paged_args* args, void* stream);
+
+/* The step's new tokens attend, each to its sequence's history before the step and to the sequence's new tokens up to
+ * itself (these as they are in k_new and v_new). What later tokens hold, NaN and infinities included, does not reach
+ * a query. Q, K and V must be 16-byte aligned with strides in multiples of 8 elements; out 16-byte aligned with
+ * strides in multiples of 4 elements. */
+int64_t dkv_paged_workspace_bytes(const dkv_paged_args* args);
+int dkv_paged_attend(const dkv_paged_args* args, void* stream);
+
+/* Dequantized rows (code * scale + offset in fp32, bf16 or fp32 by out_dtype) of layers [layer0, layer0 + n_layers):
+ * out[2, n_layers, heads, n_tokens, 64], K first; each of the items (a HOST array) writes the tokens from its `token`
+ * on. */
+int dkv_paged_read(const void* arena, int64_t arena_bytes, const dkv_page_rows* items, int32_t n_items,
+                   int32_t layer0, int32_t n_layers, int32_t layers, int32_t heads, void* out, int32_t n_tokens,
+                   int32_t out_dtype, void* stream);
+
+/* Moves packed rows of all layers as they are: rows [src_row, src_row + rows) of a tile of src_rows rows at byte
+ * src_offset of `src` to rows from dst_row on of a page at byte dst_offset of `dst`. moves is a HOST array. No byte
+ * that one of them writes may be one that another of the same call reads or writes (checked where src is dst). */
+typedef struct dkv_page_move {
+  int64_t src_offset, dst_offset;
+  uint8_t src_rows, src_row, dst_row, rows, bits;
+  uint8_t reserved[3];
+} dkv_page_move;
+int dkv_paged_move(const void* src, int64_t src_bytes, void* dst, int64_t dst_bytes, const dkv_page_move* moves,
+                   int32_t n_moves, int32_t layers, int32_t heads, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
