@@ -30,18 +30,48 @@ struct Page {
 // One workgroup's share of a sequence's (or, over pages that several sequences have in common, a group's) attention, for
 // each KV head: units [u0, u1) for block `block` of its query rows. Unit u is page first_page + u of the plan while that
 // is below n_pages, then 64 new tokens each. Query row r is token r / G, query head r % G of the KV head; `count` tokens
-// from token0 of the step on. Rows go to the partial rows from `part` on, or where that is negative to the output.
+// from token0 of the step on. The block's rows go to the partial rows from `part` on, or where that is negative to the
+// output.
 struct Work {
   int32_t first_page, n_pages, token0, count, block, u0, u1, part;
 };
 
-// Query rows [row0, row0 + 16) of a sequence that has `rows` of them from token0 on, joined from its own partials (split
-// s: rows part + s * rows + ...) and those of its group (the row's first at shared + its row here, shared_stride apart).
+// Query rows [row0, row0 + 16) of a sequence that has `rows` of them from token0 on, joined from its own partials (row
+// row0 at part, the splits `stride` rows apart) and those of its group (shared, shared_stride). splits: its own, and the
+// group's in the upper half.
 struct Merge {
-  int32_t token0, rows, row0, part, splits, shared, shared_splits, shared_stride;
+  int32_t token0, rows, row0, part, stride, shared, shared_stride;
+  uint32_t splits;
 };
 
-constexpr int SHORT_BLOCK = 16;  // query rows of a block
+// A record of a plan, or a part of one, by scalar loads: no launch writes the plan that it reads.
+template <class T>
+__device__ __forceinline__ T plan_record(const int32_t* plan, int at, int i) {
+  typedef const __attribute__((address_space(4))) int32_t* scalar_ptr;
+  const scalar_ptr from = (scalar_ptr)(plan + at + i * (int)(sizeof(T) / 4));
+  union {
+    T t;
+    int32_t w[sizeof(T) / 4];
+  } x;
+#pragma unroll
+  for (int j = 0; j < (int)(sizeof(T) / 4); ++j) x.w[j] = from[j];
+  return x.t;
+}
+
+constexpr int SHORT_BLOCK = 16;  // query rows of a block of the kernel for few rows (dkv_paged_attn.hip)
+constexpr int LONG_BLOCK = 256;  // of the one for many (dkv_paged_prompt.hip)
+
+// Four elements of an output row.
+__device__ __forceinline__ void store4(void* out, int out_dtype, int64_t at, float __attribute__((ext_vector_type(4))) x) {
+  if (out_dtype == 1)
+    *reinterpret_cast<float __attribute__((ext_vector_type(4)))*>(static_cast<float*>(out) + at) = x;
+  else
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + at) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
+}
+
+__device__ __forceinline__ bool bad_bf16(uint32_t half) { return (half & 0x7f80u) == 0x7f80u; }  // infinite or NaN
+
+void launch_long(const dkv_paged_args& a, int work, float* part_o, float2* part_ml, hipStream_t s);
 
 int check_args(const dkv_paged_args& a, bool attend, const char* what);
 

@@ -57,7 +57,7 @@ __global__ __launch_bounds__(256) void append_kernel(dkv_paged_args a) {
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63, H = a.plan.heads;
   const int kvh = blockIdx.y * 4 + wave;
   if (kvh >= 2 * H) return;
-  const dkv_page_rows item = reinterpret_cast<const dkv_page_rows*>(plan + a.plan.at_items)[blockIdx.x];
+  const dkv_page_rows item = plan_record<dkv_page_rows>(plan, a.plan.at_items, blockIdx.x);
   const int kv = kvh >= H, h = kvh - kv * H, c = lane & 7, r0 = lane >> 3;
   const uint16_t* src = static_cast<const uint16_t*>(kv ? a.v_new : a.k_new) +
                         (kv ? h * a.vn_head_stride + item.token * a.vn_tok_stride : h * a.kn_head_stride + item.token * a.kn_tok_stride);
@@ -167,16 +167,24 @@ __global__ __launch_bounds__(256) void move_kernel(Moves moves, const uint8_t* _
 
 // ---- plans -------------------------------------------------------------------------------------------------------
 
-// Workgroups of a launch of the short kernel over all KV heads, about (a workgroup has four waves, a unit each at a time).
-constexpr int SHORT_TARGET = 1024;
-constexpr int SHORT_MIN_UNITS = 4;
+// Entities of up to this many query rows of a KV head go to the kernel for few rows.
+constexpr int SHORT_ROWS = 48;
+// Workgroups over all KV heads that a step is split into, about, and the least units of one: for few rows (four waves, a
+// unit each at a time) and for many (eight waves, a unit at a time).
+constexpr int SHORT_TARGET = 1024, SHORT_LEAST = 4;
+constexpr int LONG_TARGET = 512, LONG_LEAST = 2;
 constexpr int SHARED_MIN = 4;  // pages that neighbours have in common to be attended to as a group
 
 struct Entity {  // a sequence's own part, or what a group of sequences has in common
-  int first_page, n_pages, token0, count, units, part, splits;
+  int first_page, n_pages, token0, count;
+  bool group;
+  int64_t part;  // of a group: its first partial row
+  int splits;
 };
 
 static int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+
+static bool is_long(int64_t rows) { return rows > SHORT_ROWS; }
 
 static int check_batch(const dkv_paged_batch& b, const char* what) {
   if (b.seqs <= 0 || !b.count || !b.past || !b.position || !b.first || b.layers <= 0 || b.heads <= 0 || b.q_heads <= 0 ||
@@ -206,20 +214,27 @@ static int check_batch(const dkv_paged_batch& b, const char* what) {
 // The places and bounds of a plan of these counts, whatever the history.
 static void layout_of(const dkv_paged_batch& b, dkv_paged_plan& p) {
   const int G = b.q_heads / b.heads;
-  int64_t tokens = 0, items = 0, blocks = 0;
+  int64_t tokens = 0, items = 0, merges = 0, few = 0, many = 0;  // blocks of few and of many rows
   for (int i = 0; i < b.seqs; ++i) {
+    const int64_t rows = (int64_t)b.count[i] * G;
     tokens += b.count[i];
     items += ceil_div(b.count[i], TILE) + 1;
-    blocks += ceil_div((int64_t)b.count[i] * G, SHORT_BLOCK);
+    merges += ceil_div(rows, SHORT_BLOCK);
+    if (is_long(rows)) many += ceil_div(rows, LONG_BLOCK);
+    else few += ceil_div(rows, SHORT_BLOCK);
   }
-  const int64_t grouped = ceil_div(tokens * G, SHORT_BLOCK) + b.seqs / 2;  // blocks of what groups have in common
+  if (b.seqs > 1) {  // groups: of all tokens together, each of two sequences at least
+    const int64_t rows = tokens * G;
+    few += ceil_div(std::min<int64_t>(rows, (int64_t)b.seqs / 2 * SHORT_ROWS), SHORT_BLOCK) + b.seqs / 2;
+    if (is_long(rows)) many += ceil_div(rows, LONG_BLOCK) + std::min<int64_t>(b.seqs / 2, rows / SHORT_ROWS);
+  }
   p.seqs = b.seqs, p.tokens = (int)tokens, p.layers = b.layers, p.heads = b.heads, p.q_heads = b.q_heads;
   p.max_items = (int)items;
   p.max_pages = b.max_pages;
-  p.max_work = (int)(blocks + grouped + ceil_div(SHORT_TARGET, b.heads));
-  p.max_long = 0;
-  p.max_merges = (int)blocks;
-  p.max_rows = p.max_work * SHORT_BLOCK;
+  p.max_work = few ? (int)(few + ceil_div(SHORT_TARGET, b.heads)) : 0;
+  p.max_long = many ? (int)(many + ceil_div(LONG_TARGET, b.heads)) : 0;
+  p.max_merges = (int)merges;
+  p.max_rows = p.max_work * SHORT_BLOCK + p.max_long * LONG_BLOCK;
   auto up = [](int64_t x) { return (x + 15) & ~(int64_t)15; };
   int64_t at = HEAD_WORDS;
   p.at_items = (int)at, at += up(4 * items);
@@ -237,12 +252,22 @@ static bool plan_fits(const dkv_paged_batch& b) {  // (the offsets are 32-bit)
   return 64 * tokens * (b.q_heads / b.heads) + 64ll * b.seqs + 2ll * b.max_pages + (1 << 20) < INT32_MAX;
 }
 
-// Splits of every entity so that about `target` workgroups a KV head share all units, `least` units each at least.
-static void split(std::vector<Entity>& es, int G, int block, int target, int least) {
+// Units that a block of an entity's query rows sees: a group's pages, or a sequence's and its new tokens up to the
+// block's last one.
+static int units_of(const Entity& e, int G, int block, int blk) {
+  if (e.group) return e.n_pages;
+  const int last = (int)std::min<int64_t>(((int64_t)(blk + 1) * block - 1) / G, e.count - 1);
+  return e.n_pages + last / TILE + 1;
+}
+
+// Units of a workgroup so that about `target` of them a KV head share all entities' units of this kind.
+static int64_t share(const std::vector<Entity>& es, int G, bool many, int64_t target, int least) {
+  const int block = many ? LONG_BLOCK : SHORT_BLOCK;
   int64_t total = 0;
-  for (const Entity& e : es) total += (int64_t)e.units * ceil_div((int64_t)e.count * G, block);
-  const int64_t len = std::max<int64_t>(least, (total + target - 1) / target);
-  for (Entity& e : es) e.splits = std::max(1, ceil_div(e.units, len));
+  for (const Entity& e : es)
+    if (is_long((int64_t)e.count * G) == many)
+      for (int blk = 0, n = ceil_div((int64_t)e.count * G, block); blk < n; ++blk) total += units_of(e, G, block, blk);
+  return std::max<int64_t>(least, (total + target - 1) / target);
 }
 
 static int write_plan(const dkv_paged_batch& b, int32_t* w, dkv_paged_plan& p) {
@@ -252,7 +277,6 @@ static int write_plan(const dkv_paged_batch& b, int32_t* w, dkv_paged_plan& p) {
   dkv_page_rows* items = reinterpret_cast<dkv_page_rows*>(w + p.at_items);
   Page* pages = reinterpret_cast<Page*>(w + p.at_pages);
   std::vector<Entity> own(b.seqs);
-  std::vector<int> rows_at;  // of the step's new rows
   int n_items = 0, n_pages = 0, token0 = 0;
   for (int i = 0; i < b.seqs; ++i) {
     const int from = b.first[i], to = b.first[i + 1];
@@ -261,7 +285,7 @@ static int write_plan(const dkv_paged_batch& b, int32_t* w, dkv_paged_plan& p) {
       return DKV_EINVAL;
     }
     Entity& e = own[i];
-    e = Entity{n_pages, 0, token0, b.count[i], 0, -1, 1};
+    e = Entity{n_pages, 0, token0, b.count[i], false, 0, 1};
     int64_t held = 0;
     const int64_t end = (int64_t)b.past[i] + b.count[i];
     for (int j = from; j < to; ++j) {
@@ -315,7 +339,7 @@ static int write_plan(const dkv_paged_batch& b, int32_t* w, dkv_paged_plan& p) {
       same = n;
     }
     if (same) {
-      Entity g{own[i].first_page, same, own[i].token0, 0, same, -1, 1};
+      Entity g{own[i].first_page, same, own[i].token0, 0, true, 0, 1};
       for (int k = i; k < j; ++k) {
         g.count += own[k].count, group[k] = (int)all.size();
         own[k].first_page += same, own[k].n_pages -= same;
@@ -325,46 +349,46 @@ static int write_plan(const dkv_paged_batch& b, int32_t* w, dkv_paged_plan& p) {
     i = j;
   }
   const int groups = (int)all.size();
-  for (Entity& e : own) {
-    e.units = e.n_pages + ceil_div(e.count, TILE);
-    all.push_back(e);
-  }
-  split(all, G, SHORT_BLOCK, ceil_div(SHORT_TARGET, b.heads), SHORT_MIN_UNITS);
-  int64_t rows = 0;
-  for (size_t i = 0; i < all.size(); ++i) {
-    Entity& e = all[i];
-    if ((int)i < groups || e.splits > 1 || group[i - groups] >= 0) {
-      e.part = (int)rows;
-      rows += (int64_t)e.splits * e.count * G;
-    }
-  }
-  Work* work = reinterpret_cast<Work*>(w + p.at_work);
-  int n_work = 0, n_merges = 0;
-  for (size_t i = 0; i < all.size(); ++i) {
-    const Entity& e = all[i];
-    for (int blk = 0; blk < ceil_div((int64_t)e.count * G, SHORT_BLOCK); ++blk) {
-      const int last = (int)std::min<int64_t>(((int64_t)(blk + 1) * SHORT_BLOCK - 1) / G, e.count - 1);
-      const int units = (int)i < groups ? e.units : e.n_pages + last / TILE + 1;  // up to the block's last token
-      for (int s = 0; s < e.splits; ++s)
-        work[n_work++] = Work{e.first_page, e.n_pages, e.token0, e.count, blk, (int)((int64_t)units * s / e.splits),
-                              (int)((int64_t)units * (s + 1) / e.splits), e.part < 0 ? -1 : e.part + s * e.count * G};
-    }
-  }
+  all.insert(all.end(), own.begin(), own.end());
+  const int64_t few = share(all, G, false, ceil_div(SHORT_TARGET, b.heads), SHORT_LEAST);
+  const int64_t many = share(all, G, true, ceil_div(LONG_TARGET, b.heads), LONG_LEAST);
+  Work* const work = reinterpret_cast<Work*>(w + p.at_work);
+  Work* const long_work = reinterpret_cast<Work*>(w + p.at_long);
   Merge* merges = reinterpret_cast<Merge*>(w + p.at_merges);
-  for (int i = 0; i < b.seqs; ++i) {
-    const Entity& e = all[groups + i];
-    if (e.part < 0) continue;
-    for (int r = 0; r < e.count * G; r += SHORT_BLOCK) {
-      Merge m{e.token0, e.count * G, r, e.part, e.splits, 0, 0, 0};
-      if (group[i] >= 0) {
-        const Entity& g = all[group[i]];
-        m.shared = g.part + (e.token0 - g.token0) * G, m.shared_splits = g.splits, m.shared_stride = g.count * G;
+  int n_work = 0, n_long = 0, n_merges = 0;
+  int64_t rows = 0;  // partial rows so far
+  for (int i = 0; i < (int)all.size(); ++i) {
+    Entity& e = all[i];
+    const int64_t total = (int64_t)e.count * G;
+    const bool is_many = is_long(total), joined = e.group || group[i - groups] >= 0;
+    const int block = is_many ? LONG_BLOCK : SHORT_BLOCK, blocks = ceil_div(total, block);
+    if (e.group) e.part = rows, e.splits = std::max(1, ceil_div(e.n_pages, is_many ? many : few)), rows += e.splits * total;
+    for (int blk = 0; blk < blocks; ++blk) {
+      const int units = units_of(e, G, block, blk), here = (int)std::min<int64_t>(block, total - (int64_t)blk * block);
+      const int splits = e.group ? e.splits : std::max(1, ceil_div(units, is_many ? many : few));
+      // a group's partial rows lie split after split, as its sequences' rows are not cut where its blocks are
+      const int64_t first = e.group ? e.part + (int64_t)blk * block : rows, stride = e.group ? total : here;
+      const bool parts = joined || splits > 1;
+      for (int s = 0; s < splits; ++s)
+        (is_many ? long_work[n_long++] : work[n_work++]) =
+            Work{e.first_page, e.n_pages, e.token0, e.count, blk, (int)((int64_t)units * s / splits), (int)((int64_t)units * (s + 1) / splits),
+                 parts ? (int)(first + s * stride) : -1};
+      if (e.group || !parts) continue;
+      rows += (int64_t)splits * here;
+      for (int r = 0; r < here; r += SHORT_BLOCK) {
+        Merge m{e.token0, (int)total, blk * block + r, (int)first + r, here, 0, 0, (uint32_t)splits};
+        if (group[i - groups] >= 0) {
+          const Entity& g = all[group[i - groups]];
+          m.shared = (int)g.part + (e.token0 - g.token0) * G + m.row0, m.shared_stride = g.count * G, m.splits |= (uint32_t)g.splits << 16;
+        }
+        merges[n_merges++] = m;
       }
-      merges[n_merges++] = m;
     }
   }
-  p.items = n_items, p.work = n_work, p.long_work = 0, p.merges = n_merges, p.rows = (int)rows;
-  w[N_ITEMS] = n_items, w[N_WORK] = n_work, w[N_LONG] = 0, w[N_MERGES] = n_merges;
+  auto longer = [](const Work& x, const Work& y) { return x.u1 - x.u0 > y.u1 - y.u0; };
+  std::stable_sort(long_work, long_work + n_long, longer);  // (the longest first, so that none of them is left for the end)
+  p.items = n_items, p.work = n_work, p.long_work = n_long, p.merges = n_merges, p.rows = (int)rows;
+  w[N_ITEMS] = n_items, w[N_WORK] = n_work, w[N_LONG] = n_long, w[N_MERGES] = n_merges;
   return 0;
 }
 

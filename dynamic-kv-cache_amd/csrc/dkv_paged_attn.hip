@@ -51,8 +51,6 @@ __device__ __forceinline__ void load_page_scales(const uint8_t* base, int rows, 
     }
 }
 
-__device__ __forceinline__ bool bad_bf16(uint32_t half) { return (half & 0x7f80u) == 0x7f80u; }  // infinite or NaN
-
 // New tokens that some rows of a block see and others do not, of which one has a value that is infinite or NaN: the
 // products took zeros for these values, here they are added for the rows that see them. `p` is room for 16 x 64 floats.
 __device__ __forceinline__ void add_bad_values(const Unit& u, int rows, const f32x4 (&e)[4], int c, int g, float* p, Running& r) {
@@ -178,13 +176,6 @@ __device__ __forceinline__ void attend_unit(const Unit& u, int rows, bool mixed,
   if (BITS == 16 && bad) add_bad_values(u, rows, s, c, g, lds, r);
 }
 
-__device__ __forceinline__ void store4(void* out, int out_dtype, int64_t at, f32x4 x) {
-  if (out_dtype == 1)
-    *reinterpret_cast<f32x4*>(static_cast<float*>(out) + at) = x;
-  else
-    *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(out) + at) = u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
-}
-
 template <int PREC, int TERMS>
 __global__ __launch_bounds__(256) void short_kernel(dkv_paged_args a, float* part_o, float2* part_ml) {
   __shared__ float ml[4][16][2];
@@ -192,8 +183,7 @@ __global__ __launch_bounds__(256) void short_kernel(dkv_paged_args a, float* par
   const int32_t* plan = static_cast<const int32_t*>(a.plan_words);
   const int H = a.plan.heads, G = a.plan.q_heads / H, record = blockIdx.x / H, h = blockIdx.x % H;
   if (a.bounds && record >= plan[N_WORK]) return;
-  const Work w = reinterpret_cast<const Work*>(plan + a.plan.at_work)[record];
-  const Page* pages = reinterpret_cast<const Page*>(plan + a.plan.at_pages) + w.first_page;
+  const Work w = plan_record<Work>(plan, a.plan.at_work, record);
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
   const int row0 = w.block * SHORT_BLOCK, rows_here = min(SHORT_BLOCK, w.count * G - row0);
   const int row = row0 + min(c, rows_here - 1), m = row / G;  // this lane's query row, its token of the sequence
@@ -211,7 +201,7 @@ __global__ __launch_bounds__(256) void short_kernel(dkv_paged_args a, float* par
     int rows;
     bool mixed = false;
     if (i < w.n_pages) {
-      const Page pg = pages[i];
+      const Page pg = plan_record<Page>(plan, a.plan.at_pages, w.first_page + i);
       u.bits = page_bits(pg.page);
       u.k = static_cast<const uint8_t*>(a.arena) + page_at(pg.page, a.layer, a.plan.layers, H, h);
       u.v = u.k + (int64_t)H * page_sub(u.bits);
@@ -260,7 +250,7 @@ __global__ __launch_bounds__(256) void short_kernel(dkv_paged_args a, float* par
     store4(a.out, a.out_dtype, (int64_t)(w.token0 + tok) * a.out_tok_stride + (int64_t)(h * G + at - tok * G) * a.out_head_stride + 4 * e4,
            x / l);
   } else {
-    const int64_t at = (int64_t)(w.part + row0 + rr) * H + h;
+    const int64_t at = (int64_t)(w.part + rr) * H + h;
     *reinterpret_cast<f32x4*>(part_o + at * D + 4 * e4) = x;
     if (e4 == 0) part_ml[at] = make_float2(top, l);
   }
@@ -271,12 +261,12 @@ __global__ __launch_bounds__(256) void merge_kernel(dkv_paged_args a, const floa
   const int32_t* plan = static_cast<const int32_t*>(a.plan_words);
   const int H = a.plan.heads, G = a.plan.q_heads / H, record = blockIdx.x / H, h = blockIdx.x % H;
   if (a.bounds && record >= plan[N_MERGES]) return;
-  const Merge w = reinterpret_cast<const Merge*>(plan + a.plan.at_merges)[record];
+  const Merge w = plan_record<Merge>(plan, a.plan.at_merges, record);
   const int row = w.row0 + (threadIdx.x >> 4), e4 = threadIdx.x & 15;
   if (row >= w.rows) return;
-  const int n = w.splits + w.shared_splits;
+  const int own = w.splits & 0xffff, n = own + (w.splits >> 16);
   auto at = [&](int s) {
-    return ((int64_t)row + (s < w.splits ? w.part + s * w.rows : w.shared + (s - w.splits) * w.shared_stride)) * H + h;
+    return ((int64_t)(row - w.row0) + (s < own ? w.part + s * w.stride : w.shared + (s - own) * w.shared_stride)) * H + h;
   };
   float top = -INFINITY;
   for (int i = e4; i < n; i += 16) top = fmaxf(top, part_ml[at(i)].x);
@@ -343,7 +333,8 @@ int dkv_paged_attend(const dkv_paged_args* args, void* stream) {
   const int work = a.bounds ? p.max_work : p.work, merges = a.bounds ? p.max_merges : p.merges;
   const auto attend = a.precision == 1 ? (a.out_dtype == 1 ? short_kernel<1, 3> : short_kernel<1, 2>)
                                        : (a.out_dtype == 1 ? short_kernel<0, 3> : short_kernel<0, 2>);
-  hipLaunchKernelGGL(attend, dim3(p.heads * work), dim3(256), 0, st, a, part_o, part_ml);
+  if (const int n = a.bounds ? p.max_long : p.long_work) launch_long(a, n, part_o, part_ml, st);
+  if (work > 0) hipLaunchKernelGGL(attend, dim3(p.heads * work), dim3(256), 0, st, a, part_o, part_ml);
   if (merges > 0) hipLaunchKernelGGL(merge_kernel, dim3(p.heads * merges), dim3(256), 0, st, a, part_o, part_ml);
   return (int)hipGetLastError();
 }

@@ -185,14 +185,14 @@ def test_a_plan_covers_every_row_and_unit_once():
         # what every (token, query head) attends to: pages and new tokens, each once
         seen = {}
         parts = {}
-        for at, k, block_rows in ((plan.at_work, plan.work, 16), (plan.at_long, plan.long_work, 128)):
+        for at, k, block_rows in ((plan.at_work, plan.work, 16), (plan.at_long, plan.long_work, 256)):
             for f, pg, tok, cnt, blk, u0, u1, part in records(at, k, 8):
                 for r in range(block_rows * blk, min(block_rows * (blk + 1), cnt * G)):
                     row = (tok + r // G, r % G)
                     units = seen.setdefault(row, [])
                     units += [('page', *held[f + u]) for u in range(u0, min(u1, pg))]
                     units += [('new', tok + 64 * (u - pg)) for u in range(max(u0, pg), u1)]
-                    parts.setdefault(row, []).append(part + r if part >= 0 else -1)
+                    parts.setdefault(row, []).append(part + r - block_rows * blk if part >= 0 else -1)
         at = 0
         for i in range(n):
             at_page, have = first[i], 0
@@ -211,10 +211,10 @@ def test_a_plan_covers_every_row_and_unit_once():
             at += count[i]
         assert not seen
         joined = {}
-        for tok, total, r0, part, splits, shared_part, shared_splits, stride in records(plan.at_merges, plan.merges, 8):
+        for tok, total, r0, part, stride, shared_part, shared_stride, splits in records(plan.at_merges, plan.merges, 8):
             for r in range(r0, min(r0 + 16, total)):
-                joined[(tok + r // G, r % G)] = [part + s * total + r for s in range(splits)] + \
-                    [shared_part + s * stride + r for s in range(shared_splits)]
+                joined[(tok + r // G, r % G)] = [part + s * stride + r - r0 for s in range(splits & 0xffff)] + \
+                    [shared_part + s * shared_stride + r - r0 for s in range(splits >> 16)]
         flat = [x for row, some in parts.items() for x in some if x >= 0]
         assert len(set(flat)) == len(flat) and all(x < plan.rows for x in flat)
         for row, some in parts.items():
