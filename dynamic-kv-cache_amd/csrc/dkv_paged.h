@@ -75,5 +75,8 @@ void launch_long(const dkv_paged_args& a, int work, float* part_o, float2* part_
 
 int check_args(const dkv_paged_args& a, bool attend, const char* what);
 
+// The launches of moves that are known to be in place (dkv_paged_move checks its own). A null dst moves nothing.
+int launch_moves(const void* src, void* dst, const dkv_page_move* moves, int n, int layers, int heads, void* stream);
+
 }  // namespace paged
 }  // namespace dkv

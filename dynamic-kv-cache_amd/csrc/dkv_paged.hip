@@ -165,6 +165,20 @@ __global__ __launch_bounds__(256) void move_kernel(Moves moves, const uint8_t* _
   if (scaled) reinterpret_cast<uint2*>(to + TILE * row)[m.dst_row + lane] = as;
 }
 
+int launch_moves(const void* src, void* dst, const dkv_page_move* moves, int n_moves, int layers, int heads, void* stream) {
+  if (!dst) return 0;
+  const int subs = 2 * layers * heads;
+  for (int i = 0; i < n_moves; i += ARG_MOVES) {
+    const int n = std::min(ARG_MOVES, n_moves - i);
+    Moves block{};
+    memcpy(block.at, moves + i, n * sizeof(dkv_page_move));
+    hipLaunchKernelGGL(move_kernel, dim3(n, (subs + 3) / 4), dim3(256), 0, (hipStream_t)stream, block, static_cast<const uint8_t*>(src),
+                       static_cast<uint8_t*>(dst), subs);
+    if (const int rc = (int)hipGetLastError()) return rc;
+  }
+  return 0;
+}
+
 // ---- plans -------------------------------------------------------------------------------------------------------
 
 // Entities of up to this many query rows of a KV head go to the kernel for few rows.
@@ -560,16 +574,7 @@ int dkv_paged_move(const void* src, int64_t src_bytes, void* dst, int64_t dst_by
     set_error("dkv_paged_move: out of host memory");
     return DKV_EINVAL;
   }
-  const int subs = 2 * layers * heads;
-  for (int i = 0; i < n_moves; i += ARG_MOVES) {
-    const int n = std::min(ARG_MOVES, n_moves - i);
-    Moves block{};
-    memcpy(block.at, moves + i, n * sizeof(dkv_page_move));
-    hipLaunchKernelGGL(move_kernel, dim3(n, (subs + 3) / 4), dim3(256), 0, (hipStream_t)stream, block, static_cast<const uint8_t*>(src),
-                       static_cast<uint8_t*>(dst), subs);
-    if (const int rc = (int)hipGetLastError()) return rc;
-  }
-  return 0;
+  return launch_moves(src, dst, moves, n_moves, layers, heads, stream);
 }
 
 }  // extern "C"

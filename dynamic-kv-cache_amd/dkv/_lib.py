@@ -93,6 +93,11 @@ class PagedBatch(ctypes.Structure):
                 ('arena_bytes', ctypes.c_int64), ('max_pages', ctypes.c_int32)]
 
 
+class PoolInfo(ctypes.Structure):
+    _fields_ = [('grain', ctypes.c_int64), ('blocks', ctypes.c_int64), ('free_blocks', ctypes.c_int64), ('sequences', ctypes.c_int64),
+                ('generation', ctypes.c_int64), ('pages', ctypes.c_int64 * 3), ('width_blocks', ctypes.c_int64 * 3)]
+
+
 class PagedPlan(ctypes.Structure):
     _fields_ = [(name, ctypes.c_int32) for name in (
         'seqs', 'tokens', 'layers', 'heads', 'q_heads', 'words', 'at_items', 'at_positions', 'at_pages', 'at_work', 'at_long',
@@ -223,6 +228,28 @@ SIGNATURES = [
                                       ctypes.c_int32, ctypes.c_void_p]),
     ('dkv_paged_move', ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
                                       ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p]),
+    ('dkv_pool_create', ctypes.c_int, [ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p]),
+    ('dkv_pool_destroy', ctypes.c_int, [ctypes.c_void_p]),
+    ('dkv_pool_info_get', ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(PoolInfo)]),
+    ('dkv_pool_generation', ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
+    ('dkv_pool_tokens', ctypes.c_int64, [ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p]),
+    ('dkv_pool_sequence', ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
+    ('dkv_pool_pages', ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p,
+                                      ctypes.c_void_p]),
+    ('dkv_pool_add', ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
+    ('dkv_pool_adopt', ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64,
+                                      ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
+    ('dkv_pool_fork', ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
+    ('dkv_pool_free', ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32]),
+    ('dkv_pool_truncate', ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p]),
+    ('dkv_pool_compact', ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
+    ('dkv_pool_step_bytes', ctypes.c_int64, [ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+                                             ctypes.c_int64, ctypes.c_void_p]),
+    ('dkv_pool_step', ctypes.c_int, [ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32,
+                                     ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.POINTER(PagedPlan),
+                                     ctypes.c_void_p]),
+    ('dkv_pool_read', ctypes.c_int, [ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32,
+                                     ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p]),
 ]
 
 

@@ -600,6 +600,51 @@ typedef struct dkv_page_move {
 int dkv_paged_move(const void* src, int64_t src_bytes, void* dst, int64_t dst_bytes, const dkv_page_move* moves,
                    int32_t n_moves, int32_t layers, int32_t heads, void* stream);
 
+/* The pages of an arena and the sequences that hold them: host bookkeeping for the calls above (each call takes the
+ * pool's lock), with the launches that move rows. Sequences are named by numbers that are not used again. Where a call
+ * takes `arena` and `stream` it may move pages, also to bring them together where a new page finds too little room;
+ * with a null arena nothing is moved (bookkeeping alone). A call that fails changes no sequence. */
+typedef struct dkv_pool dkv_pool;
+typedef struct dkv_pool_info {
+  int64_t grain, blocks, free_blocks; /* bytes of a grain; blocks of 48 grains, which hold 9, 5 or 3 pages of one width */
+  int64_t sequences;
+  int64_t generation;                 /* counts the calls that freed, cut or moved pages */
+  int64_t pages[3], width_blocks[3];  /* by width */
+} dkv_pool_info;
+int dkv_pool_create(int32_t layers, int32_t heads, int32_t q_heads, int64_t arena_bytes, dkv_pool** pool);
+int dkv_pool_destroy(dkv_pool* pool);
+int dkv_pool_info_get(dkv_pool* pool, dkv_pool_info* info);
+/* Where the pool keeps its generation, for as long as it lives. */
+int dkv_pool_generation(dkv_pool* pool, const int64_t** at);
+/* A sequence's tokens, tokens dropped before them (its next position is their sum) and pages; the pages' names, tokens
+ * and numbers of sequences that hold them, into arrays with room for `room`. */
+int dkv_pool_sequence(dkv_pool* pool, int64_t seq, int64_t* length, int64_t* dropped, int32_t* pages);
+int dkv_pool_pages(dkv_pool* pool, int64_t seq, int32_t room, uint32_t* page, int32_t* rows, int32_t* holders);
+/* A new sequence without tokens; with the `tokens` of a cache's tiles (a HOST table, its arena `src`), copied as they
+ * are packed; n branches of one, which share its pages but a last one that is not full. */
+int dkv_pool_add(dkv_pool* pool, int64_t* seq);
+int dkv_pool_adopt(dkv_pool* pool, const void* src, int64_t src_bytes, const dkv_tile* tiles, int32_t n_tiles,
+                   int64_t tokens, int64_t dropped, void* arena, void* stream, int64_t* seq);
+int dkv_pool_fork(dkv_pool* pool, int64_t seq, int32_t n, void* arena, void* stream, int64_t* out);
+int dkv_pool_free(dkv_pool* pool, const int64_t* seqs, int32_t n);
+/* Drops a sequence's tokens from `length` on. */
+int dkv_pool_truncate(dkv_pool* pool, int64_t seq, int64_t length, void* arena, void* stream);
+/* Brings the pages of each width together into as few blocks as hold them. */
+int dkv_pool_compact(dkv_pool* pool, void* arena, void* stream, int64_t* moved);
+/* A step: counts[i] new tokens of sequence seqs[i] at bits[i] get their pages, and the step's plan is written
+ * (dkv_paged_plan_write). dkv_pool_step_bytes gives the plan's size, 0 for an error, and the pages that it has room
+ * for, with `reserve` more tokens of every sequence. generation: the pool's; the plan holds while it stays the same. */
+int64_t dkv_pool_step_bytes(dkv_pool* pool, int32_t n, const int64_t* seqs, const int32_t* counts, const int32_t* bits,
+                            int64_t reserve, int32_t* max_pages);
+int dkv_pool_step(dkv_pool* pool, int32_t n, const int64_t* seqs, const int32_t* counts, const int32_t* bits,
+                  int32_t max_pages, void* arena, void* stream, void* buffer, int64_t bytes, dkv_paged_plan* plan,
+                  int64_t* generation);
+/* dkv_paged_read of the tokens of some sequences, each from from[i] on, n_tokens together (dkv_pool_tokens; -1 for an
+ * error). */
+int64_t dkv_pool_tokens(dkv_pool* pool, int32_t n, const int64_t* seqs, const int64_t* from);
+int dkv_pool_read(dkv_pool* pool, int32_t n, const int64_t* seqs, const int64_t* from, int32_t layer0, int32_t n_layers,
+                  const void* arena, void* out, int32_t n_tokens, int32_t out_dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -15,7 +15,6 @@ import torch
 
 from conftest import announce
 from dkv import GPUCache, PagedCache
-from dkv.paged_cache import PER_BLOCK
 from oracle.attention import dequant_rows
 from oracle.kv_quantization import pack_rows
 
@@ -135,8 +134,7 @@ def test_packed_bytes_are_the_packs(cuda):
             one.append(k[layer][None], v[layer][None], layer)
             cache.append(k[layer][None], v[layer][None], layer, step)
         n = 64 * {4: 40, 8: 72, 16: 128}[bits] * layers * 2 * heads
-        page = int(cache._seqs[seq].pages[0])
-        at = (page >> 2) * cache.grain
+        at = (cache.pages(seq)[0][0] >> 2) * cache._info().grain
         assert torch.equal(cache.arena[at:at + n], one.arena[:n])
 
 
@@ -245,7 +243,7 @@ def test_adopted_history(cuda):
     seq = cache.adopt(one)
     assert cache.length(seq) == cache.position(seq) == sum(lengths)
     # 50 | 78 + 78 at 4 bits in three pages | 64 + 17 in two | 130 in three | 70 in two
-    assert cache._seqs[seq].rows.tolist() == [50, 64, 64, 28, 64, 17, 64, 64, 2, 64, 6]
+    assert [r for _, r, _ in cache.pages(seq)] == [50, 64, 64, 28, 64, 17, 64, 64, 2, 64, 6]
     for layer in range(layers):
         for a, b in zip(cache.materialize(layer, seq), one.materialize(layer)):
             assert torch.equal(a, b)
@@ -297,7 +295,8 @@ def test_fork_truncate_compact_free(cuda):
                 m.k[s], m.v[s] = m.k[s][:, :n], m.v[s][:, :n]
             elif kind == 'compact':
                 moved += m.cache.compact()
-                assert all(m.cache._n_blocks[w] == -(-m.cache._n_pages[w] // n) for w, n in PER_BLOCK.items())
+                info = m.cache.accounting()
+                assert all(info['blocks'][w] == -(-info['pages'][w] // n) for w, n in ((4, 9), (8, 5), (16, 3)))
         except ValueError as e:  # full: nothing has changed
             assert 'full' in str(e)
             m.cache.free(seqs[1:])
@@ -306,9 +305,6 @@ def test_fork_truncate_compact_free(cuda):
             k, v = m.cache.materialize(0, seqs, out_dtype=torch.float32)
             assert torch.equal(k[0].cpu(), torch.cat([m.k[s] for s in seqs], 1))
             assert torch.equal(v[0].cpu(), torch.cat([m.v[s] for s in seqs], 1))
-        held = [p for s in m.cache._seqs.values() for p in s.pages.tolist()]
-        assert sum(m.cache._n_pages.values()) == len(set(held))
-        assert all(m.cache._refs[p >> 2] == held.count(p) for p in set(held))
     assert moved
     m.cache.free(seqs)
-    assert m.cache.accounting()['page_bytes'] == 0 and len(m.cache._empty) == m.cache.blocks
+    assert m.cache.accounting()['page_bytes'] == 0

@@ -6,80 +6,110 @@ import pytest
 import torch
 
 from dkv import GPUCache, PagedCache, _lib
-from dkv.paged_cache import BLOCK, GRAINS, PER_BLOCK
+
+GRAINS, PER_BLOCK = {4: 5, 8: 9, 16: 16}, {4: 9, 8: 5, 16: 3}
 
 
 class Quiet(PagedCache):
-    """Notes the moves that it would launch."""
+    """Bookkeeping alone: what would be launched is not."""
     def __init__(self, *a, **kw):
         super().__init__(*a, device='cpu', **kw)
-        self.moved = []
+        self._arena_ptr = None
 
-    def _move(self, source, moves):
-        self.moved += moves
-
-
-def grow(cache, seqs, counts, bits):
-    cache._grow(seqs, counts, bits)
+    def _launch(self, what, call):
+        _lib.check(call(None), what)
 
 
-def test_pages_do_not_overlap_and_fill_blocks():
-    c = Quiet(2, 3, 3, max_tokens=64 * 30)
-    assert c.blocks == 10 and c.grain == 512 * 2 * 2 * 3 == _lib.load().dkv_page_grain(2, 3)
-    for w in GRAINS:
-        assert GRAINS[w] * c.grain == _lib.slab_bytes(64, w, 2, 3)
-    taken = [c._take(w) for w in (4, 8, 16) * 5]
-    spans = sorted(((p >> 2), (p >> 2) + GRAINS[4 << (p & 3)]) for p in taken)
+def check(c, seqs):
+    """Pages lie in blocks of their width, do not overlap and are held by as many sequences as name them."""
+    held, info = {}, c.accounting()
+    for s in seqs:
+        pages = c.pages(s)
+        assert sum(r for _, r, _ in pages) == c.length(s) and all(1 <= r <= 64 for _, r, _ in pages)
+        assert not pages or pages[-1][1] == 64 or pages[-1][2] == 1
+        for page, _, holders in pages:
+            held.setdefault(page, [holders, 0])[1] += 1
+    assert all(a == b for a, b in held.values())
+    spans = sorted(((p >> 2), (p >> 2) + GRAINS[4 << (p & 3)], 4 << (p & 3)) for p in held)
     assert all(a[1] <= b[0] for a, b in zip(spans, spans[1:]))
-    assert all(a // BLOCK == (b - 1) // BLOCK for a, b in spans)
-    assert c._n_blocks == {4: 1, 8: 1, 16: 2}
-    for p in taken:
-        c._give(p)
-    assert sorted(c._empty) == list(range(10)) and c._n_pages == {4: 0, 8: 0, 16: 0}
+    assert all(a // 48 == (b - 1) // 48 and a % 48 % GRAINS[w] == 0 for a, b, w in spans)
+    widths = {}
+    for a, _, w in spans:
+        assert widths.setdefault(a // 48, w) == w
+    assert info['pages'] == {w: sum(x == w for _, _, x in spans) for w in GRAINS}
+    assert info['blocks'] == {w: sum(x == w for x in widths.values()) for w in GRAINS}
+    assert info['free_blocks'] == info['allocated_bytes'] // (48 * c._info().grain) - len(widths)
+
+
+def rows(c, seq):
+    return [r for _, r, _ in c.pages(seq)]
+
+
+def test_geometry():
+    c = Quiet(2, 3, 3, max_tokens=64 * 30)
+    i = c._info()
+    assert i.blocks == i.free_blocks == 10 and i.grain == 512 * 2 * 2 * 3 == _lib.load().dkv_page_grain(2, 3)
+    for w in GRAINS:
+        assert GRAINS[w] * i.grain == _lib.slab_bytes(64, w, 2, 3)
+    assert c.arena_bytes == 10 * 48 * i.grain
 
 
 def test_growing_fills_the_last_page_of_the_same_width_first():
     c = Quiet(1, 1, 1)
     a, b = c.add(), c.add()
-    grow(c, [a, b], [70, 10], [4, 16])
-    grow(c, [a, b], [60, 200], [4, 16])
-    grow(c, [a], [1], [8])
-    grow(c, [a], [1], [4])
-    assert c._seqs[a].rows.tolist() == [64, 64, 2, 1, 1] and c.length(a) == 132
-    assert c._seqs[b].rows.tolist() == [64, 64, 64, 18]
-    assert [4 << int(p & 3) for p in c._seqs[a].pages] == [4, 4, 4, 8, 4]
+    s = c.step([a, b], [70, 10], [4, 16])
+    assert s.positions.tolist() == list(range(70)) + list(range(10)) and s.tokens == 80
+    c.step([a, b], [60, 200], [4, 16])
+    c.step([a], [1], [8])
+    s = c.step(a, 1, 4)
+    assert s.positions.tolist() == [131]
+    assert rows(c, a) == [64, 64, 2, 1, 1] and c.length(a) == 132
+    assert rows(c, b) == [64, 64, 64, 18]
+    assert [4 << (p & 3) for p, _, _ in c.pages(a)] == [4, 4, 4, 8, 4]
+    check(c, [a, b])
 
 
 def test_a_full_cache_refuses_and_stays_as_it_was():
     c = Quiet(1, 1, 1, max_tokens=64 * 6)  # 2 blocks
-    a = c.add()
-    grow(c, [a], [64 * 5], [16])
-    before = (c._n_pages.copy(), c._n_blocks.copy(), c.length(a))
+    a, b = c.add(), c.add()
+    c.step(a, 64 * 4 + 63)
+    before = (c.accounting(), c.pages(a))
+    for seqs, counts, bits in ((a, 66, 16), (a, 1, 4), ([b, a], [1, 65], [16, 16]), ([a, b], [1, 1], [16, 8])):
+        with pytest.raises(ValueError, match='full'):
+            c.step(seqs, counts, bits)
+        assert (c.accounting(), c.pages(a)) == before and c.length(b) == 0
     with pytest.raises(ValueError, match='full'):
-        grow(c, [a], [65], [16])
+        c.fork(a, 2)
+    with pytest.raises(ValueError, match='1'):
+        c.fork(a, -1)
+    assert (c.accounting(), c.pages(a)) == before
+    (d,) = c.fork(a)
     with pytest.raises(ValueError, match='full'):
-        grow(c, [a], [1], [4])
-    assert (c._n_pages, c._n_blocks, c.length(a)) == before
-    grow(c, [a], [64], [16])
+        c.truncate(d, 10)  # a page that both hold: a copy has no room
+    assert c.length(d) == 64 * 4 + 63
+    check(c, [a, b, d])
 
 
 def test_branches_share_full_pages_and_copy_a_part_one():
     c = Quiet(1, 1, 1)
     a = c.add()
-    grow(c, [a], [130], [8])
+    c.step(a, 130, 8)
     b, d = c.fork(a, 2)
-    assert c._seqs[b].pages[:2].tolist() == c._seqs[a].pages[:2].tolist()
-    assert len({int(c._seqs[s].pages[2]) for s in (a, b, d)}) == 3
-    assert [m[5] for m in c.moved] == [2, 2] and c._n_pages[8] == 5
+    assert c.pages(b)[:2] == c.pages(a)[:2] and c.pages(a)[0][2] == 3
+    assert len({c.pages(s)[2][0] for s in (a, b, d)}) == 3
+    check(c, [a, b, d])
     c.free(a)
-    assert c._n_pages[8] == 4 and c.length(b) == 130
+    check(c, [b, d])
     c.truncate(b, 100)  # into a page that d holds too
-    assert c._seqs[b].rows.tolist() == [64, 36] and c._n_pages[8] == 4
-    assert c.moved[-1][5] == 36 and int(c._seqs[b].pages[1]) != int(c._seqs[d].pages[1])
+    assert rows(c, b) == [64, 36] and rows(c, d) == [64, 64, 2] and c.pages(b)[1][0] != c.pages(d)[1][0]
+    check(c, [b, d])
     c.truncate(b, 64)
     c.truncate(b, 0)
-    assert len(c._seqs[b].pages) == 0 and c._n_pages[8] == 3
-    assert c.fork(b, 1) and c.fork(d, 0) == []
+    assert c.pages(b) == []
+    seqs = [b, d] + c.fork(b, 1) + c.fork(d, 0) + c.fork(d, 5)
+    check(c, seqs)
+    c.free(seqs)
+    assert c.accounting()['page_bytes'] == 0
 
 
 def test_compacting_leaves_as_few_blocks_as_hold_the_pages():
@@ -87,49 +117,133 @@ def test_compacting_leaves_as_few_blocks_as_hold_the_pages():
     seqs = [c.add() for _ in range(40)]
     for i in range(4):
         for j, s in enumerate(seqs):
-            grow(c, [s], [64], [(4, 8, 16)[(i + j) % 3]])
+            c.step(s, 64, (4, 8, 16)[(i + j) % 3])
     c.free(seqs[::2])
-    held = {s: (c._seqs[s].pages.copy(), c._seqs[s].rows.copy()) for s in seqs[1::2]}
-    n = c.compact()
-    assert n == len(c.moved) > 0
-    to = {(m[0], m[6]): m[1] for m in c.moved}
-    assert len(set(m[1] for m in c.moved)) == n and not set(m[0] for m in c.moved) & set(m[1] for m in c.moved)
-    for s, (pages, rows) in held.items():
-        for old, new in zip(pages.tolist(), c._seqs[s].pages.tolist()):
-            w = 4 << (old & 3)
-            assert (new >> 2) * c.grain == to.get(((old >> 2) * c.grain, w), (old >> 2) * c.grain) and old & 3 == new & 3
-        assert c._seqs[s].rows.tolist() == rows.tolist()
-    for w in GRAINS:
-        assert c._n_blocks[w] == -(-c._n_pages[w] // PER_BLOCK[w])
-    assert sum(c._n_blocks.values()) + len(c._empty) == c.blocks
+    left, old = seqs[1::2], {s: c.pages(s) for s in seqs[1::2]}
+    moved = c.compact()
+    assert moved == sum(a != b for s in left for a, b in zip(old[s], c.pages(s))) > 0
+    for s in left:
+        assert [(p & 3, r) for p, r, _ in old[s]] == [(p & 3, r) for p, r, _ in c.pages(s)]
+    info = c.accounting()
+    assert all(info['blocks'][w] == -(-info['pages'][w] // PER_BLOCK[w]) for w in GRAINS)
+    check(c, left)
     assert c.compact() == 0
 
 
 def test_room_in_pieces_is_brought_together():
     c = Quiet(1, 1, 1, max_tokens=64 * 6)  # 2 blocks
     a, b = c.add(), c.add()
-    grow(c, [a], [64 * 9], [4])
-    grow(c, [b], [64], [4])
+    c.step(a, 64 * 9, 4)
+    c.step(b, 64, 4)
     c.truncate(a, 64 * 3)
-    grow(c, [b], [64], [16])  # the second block's page moves to the first
-    assert c.moved and c._n_blocks == {4: 1, 8: 0, 16: 1}
+    step = c.step(a, 1, 4)
+    c.step(b, 64, 16)  # the second block's page moves to the first
+    assert c.accounting()['blocks'] == {4: 1, 8: 0, 16: 1}
+    check(c, [a, b])
+    with pytest.raises(ValueError, match='moved'):
+        c._check('attend', step, 0, ())
+
+
+def test_random_bookkeeping():
+    rng = np.random.default_rng(1)
+    c = Quiet(1, 2, 2, max_tokens=64 * 60)
+    seqs, want = [c.add()], {0: 0}
+    for _ in range(600):
+        kind = rng.choice(['add', 'step', 'step', 'step', 'fork', 'free', 'truncate', 'compact'])
+        some = [seqs[i] for i in rng.permutation(len(seqs))[:rng.integers(1, len(seqs) + 1)]]
+        try:
+            if kind == 'add':
+                seqs.append(c.add())
+                want[seqs[-1]] = 0
+            elif kind == 'step':
+                counts = rng.choice([1, 2, 63, 64, 65, 200], len(some)).tolist()
+                c.step(some, counts, rng.choice([4, 8, 16], len(some)).tolist(), int(rng.integers(0, 100)))
+                for s, n in zip(some, counts):
+                    want[s] += n
+            elif kind == 'fork':
+                made = c.fork(some[0], int(rng.integers(0, 4)))
+                seqs += made
+                want.update((s, want[some[0]]) for s in made)
+            elif kind == 'free' and len(some) < len(seqs):
+                c.free(some)
+                seqs = [s for s in seqs if s not in some]
+            elif kind == 'truncate':
+                n = int(rng.integers(0, want[some[0]] + 1))
+                c.truncate(some[0], n)
+                want[some[0]] = n
+            elif kind == 'compact':
+                c.compact()
+        except ValueError as e:
+            assert 'full' in str(e)
+            c.free(seqs[1:])
+            seqs = seqs[:1]
+        check(c, seqs)
+        assert all(c.length(s) == want[s] for s in seqs)
+
+
+def test_steps_that_go_on():
+    c = Quiet(1, 1, 1)
+    a, b = c.add(), c.add()
+    step = c.step([a, b], [3, 1], [16, 4], reserve=130)
+    dev = step._dev
+    for i in range(1, 44):
+        step.advance()
+        assert step.positions.tolist() == [3 * i, 3 * i + 1, 3 * i + 2, i] and step._dev is dev
+    lengths = (c.length(a), c.length(b))
+    with pytest.raises(ValueError, match='room'):
+        for _ in range(400):
+            step.advance()
+    assert lengths[0] < c.length(a) == 3 * c.length(b)  # whole steps alone
 
 
 def test_refusals():
-    for kw in (dict(dim=128), dict(precision='fp8'), dict(q_heads=4), dict(layers=0), dict(arena_bytes=100)):
+    for kw in (dict(dim=128), dict(precision='fp8'), dict(q_heads=4), dict(layers=0), dict(arena_bytes=100), dict(layers=40000)):
         with pytest.raises(ValueError):
-            PagedCache(**{**dict(layers=1, heads=3, q_heads=3, device='cpu'), **kw})
+            PagedCache(**{**dict(layers=1, heads=3, q_heads=3, device='cpu', arena_bytes=None), **kw})
     c = Quiet(1, 3, 6)
     a, b = c.add(), c.add()
-    for call in (lambda: c.length(7), lambda: c.free([a, a]), lambda: c.free([a, 9]), lambda: c.truncate(a, 1), lambda: c.truncate(a, -1),
-                 lambda: c.fork(a, -1), lambda: c.step([a, a]), lambda: c.step([a], [1, 2]), lambda: c.step([a], 0), lambda: c.step([]),
-                 lambda: c.step([a], 1, 5), lambda: c.step([a], 1, [4, 8]), lambda: c.step([a], 1, 16, -1), lambda: c.step([a]),
+    for call in (lambda: c.length(7), lambda: c.length(-1), lambda: c.length('a'), lambda: c.length(1 << 64), lambda: c.free([a, a]),
+                 lambda: c.free([a, 9]), lambda: c.truncate(a, 1), lambda: c.truncate(a, -1), lambda: c.truncate(a, 1 << 64), lambda: c.fork(9),
+                 lambda: c.fork(a, -1), lambda: c.fork(a, 1 << 32), lambda: c.step([a, a]), lambda: c.step([a], [1, 2]), lambda: c.step([a], 0),
+                 lambda: c.step([]), lambda: c.step([a], 1, 5), lambda: c.step([a], 1, [4, 8]), lambda: c.step([a], 1, 16, -1),
+                 lambda: c.step([a], (1 << 32) + 1), lambda: c.step([a, 5]), lambda: c.pages(5),
                  lambda: c.adopt(c), lambda: c.adopt(GPUCache(None, layers=2, heads=3, device='cpu')),
-                 lambda: c.materialize(1, [a]), lambda: c.materialize(0, [a], 1), lambda: c.materialize(0, [a], [0, 0]),
+                 lambda: c.materialize(1, [a]), lambda: c.materialize(0, [a], 1), lambda: c.materialize(0, [a], -1),
+                 lambda: c.materialize(0, [a], [0, 0]), lambda: c.materialize(0, [a, a]),
                  lambda: c.materialize(0, [a], out_dtype=torch.float16), lambda: c.append(None, None, 0, None)):
         with pytest.raises(ValueError):
             call()
-    assert c.length(a) == c.length(b) == 0 and len(c._seqs) == 2
+    assert c.length(a) == c.length(b) == 0 and c.accounting()['sequences'] == 2
+    x = torch.zeros(1, 3, 1, 64)
+    step = c.step([a])
+    for call in (lambda: c.append(x, x, 0, step), lambda: c.append(x, x, 1, step), lambda: c.append(x[:, :2], x, 0, step),
+                 lambda: c.attend(x, x, x, 0, step), lambda: c.attend(x.repeat(1, 2, 1, 1), x, x, 0, step),
+                 lambda: c.attend(x, x, x, 0, step, precision='half'), lambda: Quiet(1, 3, 6).append(x, x, 0, step)):
+        with pytest.raises(ValueError):
+            call()
+    with pytest.raises(ValueError, match='CUDA'):
+        c = PagedCache(1, 1, 1, device='cpu')
+        c.step(c.add())
+
+
+def test_pools_refuse_null_and_foreign_tables():
+    lib = _lib.load()
+    assert lib.dkv_pool_add(None, None) == _lib.DKV_EINVAL
+    assert lib.dkv_pool_create(1, 1, 1, 1 << 20, None) == _lib.DKV_EINVAL
+    c = Quiet(1, 1, 1)
+    tile = np.zeros(2, dtype=[('offset', '<i8'), ('start', '<i4'), ('rows', '<u2'), ('bits', 'u1'), ('pad', 'u1')])
+    seq = ctypes.c_int64()
+    def adopt(tokens, size=1 << 20, **kw):
+        tile['offset'], tile['start'], tile['rows'], tile['bits'] = (0, 4096), (0, 10), 10, 16
+        for name, x in kw.items():
+            tile[name] = x
+        return lib.dkv_pool_adopt(c._pool, 4096, size, tile.ctypes.data, 2, tokens, 0, None, None, ctypes.byref(seq))
+    for bad in (dict(tokens=21), dict(tokens=10), dict(tokens=-1), dict(tokens=20, start=(0, 11)), dict(tokens=20, bits=(16, 5)),
+                dict(tokens=20, offset=(0, 1 << 20)), dict(tokens=20, offset=(-16, 4096)), dict(tokens=20, offset=(8, 4096)),
+                dict(tokens=20, rows=(10, 65)), dict(tokens=20, rows=(0, 10)), dict(tokens=20, size=4096)):
+        assert adopt(**bad) == _lib.DKV_EINVAL, bad
+    assert c.accounting()['sequences'] == 0
+    assert adopt(15) == 0 and c.length(seq.value) == 15 and rows(c, seq.value) == [15]
 
 
 def batch(count, past, pages, rows, first, heads=2, q_heads=6, layers=1, arena=1 << 20, max_pages=64, position=None):
@@ -284,11 +398,12 @@ def test_reads_refuse_rows_outside():
 
 
 def test_moves_refuse_what_meets():
-    from dkv.paged_cache import MOVE_DTYPE
+    dtype = np.dtype([('src', '<i8'), ('dst', '<i8'), ('src_rows', 'u1'), ('src_row', 'u1'), ('dst_row', 'u1'), ('rows', 'u1'),
+                      ('bits', 'u1'), ('reserved', 'u1', 3)])
     lib = _lib.load()
     grain = 512 * 2 * 2 * 2
     def move(*moves, src=4096, dst=4096, size=40 * grain):
-        m = np.array([x + (0,) * 0 + ((0, 0, 0),) for x in moves], dtype=MOVE_DTYPE)
+        m = np.array([x + ((0, 0, 0),) for x in moves], dtype=dtype)
         return lib.dkv_paged_move(src, size, dst, size, m.ctypes.data, len(m), 2, 2, None)
     ok = (0, 5 * grain, 64, 0, 0, 64, 4)
     for bad in ([(0, 36 * grain, 64, 0, 0, 64, 4)], [(-16, 0, 64, 0, 0, 1, 4)], [(8, 5 * grain, 64, 0, 0, 1, 4)], [(0, 5 * grain, 64, 0, 1, 64, 4)],
