@@ -49,8 +49,24 @@ __device__ __forceinline__ void pack_row(const u32x4& w, bool valid, int c, uint
                                 reinterpret_cast<uint64_t*>(sub + TILE * 8 * BITS + 8 * row));
 }
 
-// A wave takes the rows of one item (up to 64 tokens of a page) of one K or V head, 8 lanes a row, all loads before the
-// first use.
+// Rows r0 + 8 i of an item, 8 lanes a row, AHEAD of them loaded before the first is packed. (All 8 at once take 230
+// registers and leave two waves a SIMD: 7900 tokens of 8 heads 13.6 us instead of 10.5.)
+template <int BITS>
+__device__ __forceinline__ void pack_rows(const uint16_t* src, int64_t stride, int rows, int r0, int c, uint8_t* sub, int row0) {
+  constexpr int AHEAD = 4;
+  for (int i0 = 0; i0 < rows; i0 += 8 * AHEAD) {
+    u32x4 w[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) w[i] = *reinterpret_cast<const u32x4*>(src + min(i0 + 8 * i + r0, rows - 1) * stride + 8 * c);
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      if (i0 + 8 * i >= rows) break;
+      pack_row<BITS>(w[i], i0 + 8 * i + r0 < rows, c, sub, row0 + i0 + 8 * i + r0);
+    }
+  }
+}
+
+// A wave takes the rows of one item (up to 64 tokens of a page) of one K or V head.
 __global__ __launch_bounds__(256) void append_kernel(dkv_paged_args a) {
   const int32_t* plan = static_cast<const int32_t*>(a.plan_words);
   if (a.bounds && (int)blockIdx.x >= plan[N_ITEMS]) return;
@@ -64,20 +80,9 @@ __global__ __launch_bounds__(256) void append_kernel(dkv_paged_args a) {
   const int64_t stride = kv ? a.vn_tok_stride : a.kn_tok_stride;
   const int bits = page_bits(item.page);
   uint8_t* sub = static_cast<uint8_t*>(a.arena) + page_at(item.page, a.layer, a.plan.layers, H, 0) + (int64_t)kvh * page_sub(bits);
-  u32x4 w[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (8 * i < item.rows)
-      w[i] = *reinterpret_cast<const u32x4*>(src + min(8 * i + r0, item.rows - 1) * stride + 8 * c);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if (8 * i >= item.rows) break;
-    const int r = 8 * i + r0;
-    const bool valid = r < item.rows;
-    if (bits == 4) pack_row<4>(w[i], valid, c, sub, item.row0 + r);
-    else if (bits == 8) pack_row<8>(w[i], valid, c, sub, item.row0 + r);
-    else pack_row<16>(w[i], valid, c, sub, item.row0 + r);
-  }
+  if (bits == 4) pack_rows<4>(src, stride, item.rows, r0, c, sub, item.row0);
+  else if (bits == 8) pack_rows<8>(src, stride, item.rows, r0, c, sub, item.row0);
+  else pack_rows<16>(src, stride, item.rows, r0, c, sub, item.row0);
 }
 
 // ---- pages read back ---------------------------------------------------------------------------------------------
@@ -87,50 +92,60 @@ struct Items {
   dkv_page_rows at[ARG_ITEMS];
 };
 
-// A workgroup: the rows of one item of one (layer, K or V, head), four lanes a row.
+// Rows of a page as values, 8 lanes a row (lane c: elements [8 c, 8 c + 8)): every store of bf16 writes whole lines.
+template <int BITS>
+__device__ __forceinline__ void read_rows(const uint8_t* sub, int row0, int rows, int r0, int c, void* out, int64_t at, int out_dtype) {
+  constexpr int AHEAD = 4;
+  for (int i0 = 0; i0 < rows; i0 += 8 * AHEAD) {
+    u32x4 w[AHEAD];
+    float2 as[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int row = row0 + min(i0 + 8 * i + r0, rows - 1);
+      const uint8_t* p = sub + row * (8 * BITS) + c * BITS;
+      if (BITS == 4) w[i][0] = *reinterpret_cast<const uint32_t*>(p);
+      else if (BITS == 16) w[i] = *reinterpret_cast<const u32x4*>(p);
+      else {
+        const uint2 x = *reinterpret_cast<const uint2*>(p);
+        w[i][0] = x.x, w[i][1] = x.y;
+      }
+      if (BITS < 16) as[i] = reinterpret_cast<const float2*>(sub + TILE * 8 * BITS)[row];
+    }
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int r = i0 + 8 * i + r0;
+      if (r >= rows) break;
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if (BITS == 16) x[e] = e & 1 ? bf16_hi(w[i][e / 2]) : bf16_lo(w[i][e / 2]);
+        else x[e] = __fadd_rn(__fmul_rn((float)(BITS == 4 ? (w[i][0] >> (4 * e)) & 15u : (w[i][e / 4] >> (8 * (e % 4))) & 255u), as[i].y), as[i].x);
+      }
+      const int64_t o = at + (int64_t)r * D + 8 * c;
+      if (out_dtype == 1) {
+        float4* dst = reinterpret_cast<float4*>(static_cast<float*>(out) + o);
+        dst[0] = make_float4(x[0], x[1], x[2], x[3]), dst[1] = make_float4(x[4], x[5], x[6], x[7]);
+      } else {
+        *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(out) + o) =
+            u32x4{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])};
+      }
+    }
+  }
+}
+
+// A wave: the rows of one item of one (layer, K or V, head).
 __global__ __launch_bounds__(256) void read_kernel(Items items, const uint8_t* __restrict__ arena, int layer0, int n_layers, int layers,
                                                    int heads, void* __restrict__ out, int64_t n_tokens, int out_dtype) {
   const dkv_page_rows item = items.at[blockIdx.x];
-  const int r = threadIdx.x >> 2, c = threadIdx.x & 3;
-  if (r >= item.rows) return;
-  const int kvh = blockIdx.y, kv = kvh >= heads, h = kvh - kv * heads, bits = page_bits(item.page), row = item.row0 + r;
-  for (int l = blockIdx.z; l < n_layers; l += gridDim.z) {
-    const uint8_t* sub = arena + page_at(item.page, layer0 + l, layers, heads, 0) + (int64_t)kvh * page_sub(bits);
-    const uint8_t* p = sub + row * (8 * bits) + c * (2 * bits);
-    float x[16];
-    if (bits == 16) {
-      const u32x4 w0 = reinterpret_cast<const u32x4*>(p)[0], w1 = reinterpret_cast<const u32x4*>(p)[1];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        x[2 * i] = bf16_lo(w0[i]), x[2 * i + 1] = bf16_hi(w0[i]), x[8 + 2 * i] = bf16_lo(w1[i]), x[9 + 2 * i] = bf16_hi(w1[i]);
-    } else {
-      const float2 as = reinterpret_cast<const float2*>(sub + TILE * 8 * bits)[row];
-      uint32_t code[16];
-      if (bits == 4) {
-        const uint2 w = *reinterpret_cast<const uint2*>(p);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) code[i] = (w.x >> (4 * i)) & 15u, code[8 + i] = (w.y >> (4 * i)) & 15u;
-      } else {
-        const u32x4 w = *reinterpret_cast<const u32x4*>(p);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) code[i] = (w[i >> 2] >> (8 * (i & 3))) & 255u;
-      }
-#pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] = __fadd_rn(__fmul_rn((float)code[i], as.y), as.x);
-    }
-    const int64_t o = ((((int64_t)kv * n_layers + l) * heads + h) * n_tokens + item.token + r) * D + c * 16;
-    if (out_dtype == 1) {
-      float4* dst = reinterpret_cast<float4*>(static_cast<float*>(out) + o);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) dst[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
-    } else {
-      u32x4* dst = reinterpret_cast<u32x4*>(static_cast<uint16_t*>(out) + o);
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        dst[i] = u32x4{pack_bf16(x[8 * i], x[8 * i + 1]), pack_bf16(x[8 * i + 2], x[8 * i + 3]),
-                       pack_bf16(x[8 * i + 4], x[8 * i + 5]), pack_bf16(x[8 * i + 6], x[8 * i + 7])};
-    }
-  }
+  const int sub_index = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63;
+  if (sub_index >= 2 * heads * n_layers) return;
+  const int l = sub_index / (2 * heads), kvh = sub_index - l * 2 * heads, kv = kvh >= heads, h = kvh - kv * heads;
+  const int bits = page_bits(item.page);
+  const uint8_t* sub = arena + page_at(item.page, layer0 + l, layers, heads, 0) + (int64_t)kvh * page_sub(bits);
+  const int64_t at = ((((int64_t)kv * n_layers + l) * heads + h) * n_tokens + item.token) * D;
+  if (bits == 4) read_rows<4>(sub, item.row0, item.rows, lane >> 3, lane & 7, out, at, out_dtype);
+  else if (bits == 8) read_rows<8>(sub, item.row0, item.rows, lane >> 3, lane & 7, out, at, out_dtype);
+  else read_rows<16>(sub, item.row0, item.rows, lane >> 3, lane & 7, out, at, out_dtype);
 }
 
 // ---- rows moved --------------------------------------------------------------------------------------------------
@@ -140,29 +155,35 @@ struct Moves {
   dkv_page_move at[ARG_MOVES];
 };
 
-// A wave moves the rows of one (layer, K or V, head) of a move: payload and (offset, scale) pairs, which lie behind as
-// many rows as the tile has room for.
+// One sub-block's rows: the payload in 16-byte pieces, then the (offset, scale) pairs, which lie behind as many rows as
+// the tile has room for. All loads before the first store.
+template <int BITS>
+__device__ __forceinline__ void move_rows(const dkv_page_move& m, const uint8_t* from, uint8_t* to, int lane) {
+  constexpr int ROW = 8 * BITS, PIECES = BITS / 2;  // bytes; of 64 rows, a lane's pieces
+  const u32x4* f = reinterpret_cast<const u32x4*>(from + m.src_row * ROW);
+  u32x4* t = reinterpret_cast<u32x4*>(to + m.dst_row * ROW);
+  const int n = m.rows * (ROW / 16);
+  u32x4 w[PIECES];
+#pragma unroll
+  for (int i = 0; i < PIECES; ++i) w[i] = f[min(64 * i + lane, n - 1)];
+  uint2 as = make_uint2(0, 0);
+  if (BITS < 16) as = reinterpret_cast<const uint2*>(from + m.src_rows * ROW)[m.src_row + min(lane, m.rows - 1)];
+#pragma unroll
+  for (int i = 0; i < PIECES; ++i)
+    if (64 * i + lane < n) __builtin_nontemporal_store(w[i], t + 64 * i + lane);
+  if (BITS < 16 && lane < m.rows) reinterpret_cast<uint2*>(to + TILE * ROW)[m.dst_row + lane] = as;
+}
+
+// A wave moves the rows of one (layer, K or V, head) of a move.
 __global__ __launch_bounds__(256) void move_kernel(Moves moves, const uint8_t* __restrict__ src, uint8_t* __restrict__ dst, int subs) {
   const dkv_page_move m = moves.at[blockIdx.x];
-  const int sub = blockIdx.y * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int sub = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63;
   if (sub >= subs) return;
-  const int row = 8 * m.bits;
   const uint8_t* from = src + m.src_offset + sub * subblock_bytes(m.src_rows, m.bits);
   uint8_t* to = dst + m.dst_offset + (int64_t)sub * page_sub(m.bits);
-  const u32x4* f = reinterpret_cast<const u32x4*>(from + m.src_row * row);
-  u32x4* t = reinterpret_cast<u32x4*>(to + m.dst_row * row);
-  const int n = m.rows * row / 16;  // up to 512 pieces
-  u32x4 w[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (64 * i + lane < n) w[i] = f[64 * i + lane];
-  uint2 as = make_uint2(0, 0);
-  const bool scaled = m.bits < 16 && lane < m.rows;
-  if (scaled) as = reinterpret_cast<const uint2*>(from + m.src_rows * row)[m.src_row + lane];
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (64 * i + lane < n) t[64 * i + lane] = w[i];
-  if (scaled) reinterpret_cast<uint2*>(to + TILE * row)[m.dst_row + lane] = as;
+  if (m.bits == 4) move_rows<4>(m, from, to, lane);
+  else if (m.bits == 8) move_rows<8>(m, from, to, lane);
+  else move_rows<16>(m, from, to, lane);
 }
 
 int launch_moves(const void* src, void* dst, const dkv_page_move* moves, int n_moves, int layers, int heads, void* stream) {
@@ -185,12 +206,13 @@ int launch_moves(const void* src, void* dst, const dkv_page_move* moves, int n_m
 constexpr int SHORT_ROWS = 48;
 // Workgroups over all KV heads that a step is split into, about, and the least units of one: for few rows (four waves, a
 // unit each at a time) and for many (eight waves, a unit at a time).
-constexpr int SHORT_TARGET = 1024, SHORT_LEAST = 4;
+constexpr int SHORT_TARGET = 2048, SHORT_LEAST = 8;
 constexpr int LONG_TARGET = 512, LONG_LEAST = 2;
 constexpr int SHARED_MIN = 4;  // pages that neighbours have in common to be attended to as a group
 
 struct Entity {  // a sequence's own part, or what a group of sequences has in common
   int first_page, n_pages, token0, count;
+  int n4, n8;  // pages up to which they have 4 bits, 8 at most
   bool group;
   int64_t part;  // of a group: its first partial row
   int splits;
@@ -254,8 +276,8 @@ static void layout_of(const dkv_paged_batch& b, dkv_paged_plan& p) {
   p.at_items = (int)at, at += up(4 * items);
   p.at_positions = (int)at, at += up(2 * tokens);
   p.at_pages = (int)at, at += up(2 * (int64_t)b.max_pages);
-  p.at_work = (int)at, at += up(8ll * p.max_work);
-  p.at_long = (int)at, at += up(8ll * p.max_long);
+  p.at_work = (int)at, at += up((int64_t)(sizeof(Work) / 4) * p.max_work);
+  p.at_long = (int)at, at += up((int64_t)(sizeof(Work) / 4) * p.max_long);
   p.at_merges = (int)at, at += up(8ll * p.max_merges);
   p.words = (int)at;
 }
@@ -299,7 +321,7 @@ static int write_plan(const dkv_paged_batch& b, int32_t* w, dkv_paged_plan& p) {
       return DKV_EINVAL;
     }
     Entity& e = own[i];
-    e = Entity{n_pages, 0, token0, b.count[i], false, 0, 1};
+    e = Entity{n_pages, 0, token0, b.count[i], 0, 0, false, 0, 1};
     int64_t held = 0;
     const int64_t end = (int64_t)b.past[i] + b.count[i];
     for (int j = from; j < to; ++j) {
@@ -353,7 +375,7 @@ static int write_plan(const dkv_paged_batch& b, int32_t* w, dkv_paged_plan& p) {
       same = n;
     }
     if (same) {
-      Entity g{own[i].first_page, same, own[i].token0, 0, true, 0, 1};
+      Entity g{own[i].first_page, same, own[i].token0, 0, 0, 0, true, 0, 1};
       for (int k = i; k < j; ++k) {
         g.count += own[k].count, group[k] = (int)all.size();
         own[k].first_page += same, own[k].n_pages -= same;
@@ -364,6 +386,11 @@ static int write_plan(const dkv_paged_batch& b, int32_t* w, dkv_paged_plan& p) {
   }
   const int groups = (int)all.size();
   all.insert(all.end(), own.begin(), own.end());
+  for (Entity& e : all) {  // by width (of pages that several sequences have in common, the first one's are read)
+    Page* const from = pages + e.first_page;
+    std::stable_sort(from, from + e.n_pages, [](const Page& x, const Page& y) { return (x.page & 3) < (y.page & 3); });
+    for (int i = 0; i < e.n_pages; ++i) e.n4 += (from[i].page & 3) == 0, e.n8 += (from[i].page & 3) <= 1;
+  }
   const int64_t few = share(all, G, false, ceil_div(SHORT_TARGET, b.heads), SHORT_LEAST);
   const int64_t many = share(all, G, true, ceil_div(LONG_TARGET, b.heads), LONG_LEAST);
   Work* const work = reinterpret_cast<Work*>(w + p.at_work);
@@ -385,8 +412,8 @@ static int write_plan(const dkv_paged_batch& b, int32_t* w, dkv_paged_plan& p) {
       const bool parts = joined || splits > 1;
       for (int s = 0; s < splits; ++s)
         (is_many ? long_work[n_long++] : work[n_work++]) =
-            Work{e.first_page, e.n_pages, e.token0, e.count, blk, (int)((int64_t)units * s / splits), (int)((int64_t)units * (s + 1) / splits),
-                 parts ? (int)(first + s * stride) : -1};
+            Work{e.first_page, e.n4, e.n8, e.n_pages, e.token0, e.count, blk, (int)((int64_t)units * s / splits),
+                 (int)((int64_t)units * (s + 1) / splits), parts ? (int)(first + s * stride) : -1, {}};
       if (e.group || !parts) continue;
       rows += (int64_t)splits * here;
       for (int r = 0; r < here; r += SHORT_BLOCK) {
@@ -419,8 +446,8 @@ int check_args(const dkv_paged_args& a, bool attend, const char* what) {
   } else if (attend && (!a16(a.q) || !a16(a.out) || (a.q_head_stride & 7) || (a.q_tok_stride & 7) || (a.out_tok_stride & 3) ||
                         (a.out_head_stride & 3) || a.out_dtype < 0 || a.out_dtype > 1)) {
     set_error("%s: Q and out must be 16-byte aligned, strides multiples of 8 and 4 elements, out bf16 (0) or fp32 (1)", what);
-  } else if (attend && (a.precision < 0 || a.precision > 1)) {
-    set_error("%s: precision must be 0 (bf16) or 1 (fp32)", what);
+  } else if (attend && (a.precision < 0 || a.precision > 1 || !(a.scale > 0.f) || a.scale > 3e38f)) {
+    set_error("%s: precision must be 0 (bf16) or 1 (fp32), scale positive", what);
   } else if (attend && p.tokens > 1 && (a.kn_tok_stride < 0 || a.kn_tok_stride >= 1 << 23 || a.vn_tok_stride < 0 || a.vn_tok_stride >= 1 << 23)) {
     set_error("%s: K's and V's token strides must be from 0 to 2^23 - 1 elements", what);
   } else {
@@ -510,7 +537,7 @@ int dkv_paged_read(const void* arena, int64_t arena_bytes, const dkv_page_rows* 
     const int n = std::min(ARG_ITEMS, n_items - i);
     Items block{};
     memcpy(block.at, items + i, n * sizeof(dkv_page_rows));
-    hipLaunchKernelGGL(read_kernel, dim3(n, 2 * heads, std::min(n_layers, 32768)), dim3(256), 0, (hipStream_t)stream, block,
+    hipLaunchKernelGGL(read_kernel, dim3(n, (2 * heads * n_layers + 3) / 4), dim3(256), 0, (hipStream_t)stream, block,
                        static_cast<const uint8_t*>(arena), layer0, n_layers, layers, heads, out, (int64_t)n_tokens, out_dtype);
     if (const int rc = (int)hipGetLastError()) return rc;
   }

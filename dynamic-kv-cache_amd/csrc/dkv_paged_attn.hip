@@ -7,179 +7,265 @@ namespace paged {
 
 using namespace rows;
 
-// A unit's rows: a page's, or 64 new tokens' from `k` and `v` on. Rows [0, rows) are there.
-struct Unit {
+constexpr int HALF = 32;  // keys at a time
+
+// Half a unit's rows: a page's, or new tokens', from `k` and `v` on. Rows [0, rows) are there.
+struct Half {
   const uint8_t* k;
   const uint8_t* v;
-  uint32_t k_stride, v_stride;  // bytes from row to row, below 2^24
-  int bits, rows;
-  int high;  // rows that this lane's query row sees
+  const uint8_t* scales;        // a packed page's: lane l's (offset, scale) pair, of key l or value l - 32
+  uint32_t k_stride, v_stride;  // of new tokens: bytes from row to row, below 2^24
+  int rows;
 };
+
+// What a lane has loaded: of keys 16 b + c the elements [16 g, 16 g + 16), of values 16 b + 4 g + i the elements
+// [4 c, 4 c + 4), and one (offset, scale) pair, which goes to the lanes that need it through LDS (each lane's own copies
+// of them would be 20 to 32 registers).
+template <int BITS>
+struct Loaded {
+  uint32_t k[2][BITS / 2], v[2][4][BITS == 16 ? 2 : 1];
+  float2 pair;
+};
+
+// Rows that a half page does not hold are read too (what is there meets no score and no weight): without a test a lane's
+// rows are one address and constant distances. Of new tokens (NEW) the row past the last one is its first again.
+template <int BITS, bool NEW = false>
+__device__ __forceinline__ void load_keys(const Half& u, int c, int g, Loaded<BITS>& x) {
+#pragma unroll
+  for (int b = 0; b < 2; ++b) {
+    const int row = 16 * b + c;
+    const uint8_t* at = NEW ? u.k + (__umul24(row < u.rows ? row : 0, u.k_stride) + g * 2 * BITS)
+                            : u.k + (uint32_t)(c * 8 * BITS + g * 2 * BITS) + 16 * b * 8 * BITS;
+    if (BITS == 4) {
+      const u32x2 w = *reinterpret_cast<const u32x2*>(at);
+      x.k[b][0] = w[0], x.k[b][1] = w[1];
+    } else {
+#pragma unroll
+      for (int i = 0; i < BITS / 8; ++i) {
+        const u32x4 w = *reinterpret_cast<const u32x4*>(at + 16 * i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x.k[b][4 * i + j] = w[j];
+      }
+    }
+  }
+  if (BITS < 16) x.pair = *reinterpret_cast<const float2*>(u.scales);
+}
+
+template <int BITS, bool NEW = false>
+__device__ __forceinline__ void load_vals(const Half& u, int c, int g, Loaded<BITS>& x) {
+#pragma unroll
+  for (int b = 0; b < 2; ++b)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = 16 * b + 4 * g + i;
+      const uint8_t* at = NEW ? u.v + (__umul24(row < u.rows ? row : 0, u.v_stride) + c * BITS / 2)
+                              : u.v + (uint32_t)(4 * g * 8 * BITS + c * BITS / 2) + (16 * b + i) * 8 * BITS;
+      if (BITS == 4) {
+        x.v[b][i][0] = *reinterpret_cast<const uint16_t*>(at);
+      } else if (BITS == 8) {
+        x.v[b][i][0] = *reinterpret_cast<const uint32_t*>(at);
+      } else {
+        const u32x2 w = *reinterpret_cast<const u32x2*>(at);
+        x.v[b][i][0] = w[0], x.v[b][i][1 % (BITS == 16 ? 2 : 1)] = w[1];
+      }
+    }
+}
+
+// Codes e and e + 1 of packed words as a bf16 pair: their values (c * scale + offset, each step rounded) at PREC 0, else the
+// codes, which bf16 holds exactly; scale and offset come later. Nibbles are bytes of two words first, so that a code is one
+// conversion.
+template <int BITS>
+struct Codes {
+  uint32_t w[BITS == 4 ? 2 : 1];
+};
+template <int BITS>
+__device__ __forceinline__ Codes<BITS> codes_of(uint32_t w) {
+  Codes<BITS> x;
+  if (BITS == 4) x.w[0] = w & 0x0f0f0f0fu, x.w[BITS == 4 ? 1 : 0] = (w >> 4) & 0x0f0f0f0fu;
+  else x.w[0] = w;
+  return x;
+}
+template <int BITS>
+__device__ __forceinline__ float code(const Codes<BITS>& x, int e) {
+  return (float)(BITS == 4 ? (x.w[e % (BITS == 4 ? 2 : 1)] >> (8 * (e / 2))) & 255u : (x.w[0] >> (8 * e)) & 255u);
+}
+template <int PREC>
+__device__ __forceinline__ uint32_t values(float c0, float c1, float scale0, float offset0, float scale1, float offset1) {
+  return PREC ? pack_bf16(c0, c1) : pack_bf16(c0 * scale0 + offset0, c1 * scale1 + offset1);
+}
+
+// A wave's 32 pairs of keys, then of values, to be read by any of its lanes.
+__device__ __forceinline__ void share_scales(float2* lds, int lane, const float2& mine, int rows) {
+  lds[lane] = (lane & (HALF - 1)) < rows ? mine : make_float2(0.f, 0.f);
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+template <int BITS, int PREC>
+__device__ __forceinline__ void scores(const Loaded<BITS>& x, const float2* scales, int c, int g, const Op (&q)[2], float q_sum, f32x4 (&s)[2]) {
+#pragma unroll
+  for (int b = 0; b < 2; ++b) {
+    Op k[2];
+    if (BITS == 16) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) k[j / 4].u[j % 4] = x.k[b][j % (BITS / 2)];
+    } else {
+      float2 as = make_float2(0.f, 0.f);
+      if (!PREC) as = scales[16 * b + c];
+      constexpr int PER = 32 / BITS;  // codes of a word
+#pragma unroll
+      for (int i = 0; i < BITS / 2; ++i) {
+        const auto w = codes_of<BITS == 16 ? 8 : BITS>(x.k[b][i]);
+#pragma unroll
+        for (int e = 0; e < PER; e += 2) {
+          const int j = (PER * i + e) / 2;
+          k[j / 4].u[j % 4] = values<PREC>(code(w, e), code(w, e + 1), as.y, as.x, as.y, as.x);
+        }
+      }
+    }
+    s[b] = mfma(k[1], q[1], mfma(k[0], q[0], f32x4{0, 0, 0, 0}));
+  }
+  if constexpr (PREC == 1 && BITS < 16)
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < 4; i += 2) {  // scale * product + offset * (sum of the query)
+        const f32x4 as = *reinterpret_cast<const f32x4*>(&scales[16 * b + 4 * g + i]);
+        s[b][i] = __builtin_fmaf(as[1], s[b][i], as[0] * q_sum);
+        s[b][i + 1] = __builtin_fmaf(as[3], s[b][i + 1], as[2] * q_sum);
+      }
+}
 
 struct Running {
   float m, l, offset;
   f32x4 o[4];
 };
 
-template <int BITS>
-__device__ __forceinline__ void load_page_key(const Unit& u, int row, int g, KeyPiece& p) {
-  const int r = row < u.rows ? row : 0;
-  const uint8_t* at = u.k + (__umul24(r, u.k_stride) + g * 2 * BITS);
-  if (BITS == 4) {
-    const u32x2 w = *reinterpret_cast<const u32x2*>(at);
-    p.w[0] = w[0], p.w[1] = w[1];
-  } else {
+// Scores in s to weights. The sums so far are moved to a new maximum only where some lane's scores pass the old one.
+__device__ __forceinline__ void soften(f32x4 (&s)[2], float scale2, Running& r) {
+  const float top = max_nn(max_nn(max_nn(s[0][0], s[0][1]), max_nn(s[0][2], s[0][3])), max_nn(max_nn(s[1][0], s[1][1]), max_nn(s[1][2], s[1][3])));
+  if (__builtin_amdgcn_ballot_w64(top * scale2 > r.m)) {
+    const float m = max_nn(row_max(top) * scale2, r.m);
+    const float alpha = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(r.m - m);
+    r.m = m;
+    r.l *= alpha, r.offset *= alpha;
 #pragma unroll
-    for (int i = 0; i < BITS / 8; ++i) {
-      const u32x4 w = *reinterpret_cast<const u32x4*>(at + 16 * i);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) p.w[4 * i + j] = w[j];
-    }
+    for (int db = 0; db < 4; ++db) r.o[db] *= alpha;
   }
-  if (BITS < 16) p.as = *reinterpret_cast<const float2*>(u.k + (TILE * 8 * BITS + 8 * r));
-}
-
-// (offset, scale) of the lane's rows 16 b + 4 g + i, two rows a load.
-template <int BITS>
-__device__ __forceinline__ void load_page_scales(const uint8_t* base, int rows, int g, f32x4 (&as)[4][2]) {
+  const float ref = r.m == -INFINITY ? 0.f : r.m;  // nothing visible yet: keep the empty state
+  float sum = 0;
 #pragma unroll
-  for (int b = 0; b < 4; ++b)
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int row = 16 * b + 4 * g + 2 * i;
-      as[b][i] = *reinterpret_cast<const f32x4*>(base + (TILE * 8 * BITS + 8 * (row < rows ? row : 0)));
-    }
-}
-
-// New tokens that some rows of a block see and others do not, of which one has a value that is infinite or NaN: the
-// products took zeros for these values, here they are added for the rows that see them. `p` is room for 16 x 64 floats.
-__device__ __forceinline__ void add_bad_values(const Unit& u, int rows, const f32x4 (&e)[4], int c, int g, float* p, Running& r) {
-#pragma unroll
-  for (int b = 0; b < 4; ++b)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) p[c * TILE + 16 * b + 4 * g + i] = e[b][i];
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-  for (int j = 0; j < rows; ++j) {
-    const uint32_t* v = reinterpret_cast<const uint32_t*>(u.v + __umul24(j, u.v_stride) + 32 * g);
-    if (j >= u.high) continue;
-    const float pj = p[c * TILE + j];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const uint32_t w = v[k];
-      if (bad_bf16(w)) r.o[(2 * k) % 4][k / 2] += pj * bf16_lo(w);
-      if (bad_bf16(w >> 16)) r.o[(2 * k + 1) % 4][k / 2] += pj * bf16_hi(w);
-    }
-  }
-  __builtin_amdgcn_wave_barrier();
-}
-
-// `rows`: rows of the unit that some query row of the block sees; `mixed`: they do not all see the same ones.
-template <int BITS, int PREC, int TERMS>
-__device__ __forceinline__ void attend_unit(const Unit& u, int rows, bool mixed, const Op (&q)[2], float q_sum, float scale2, int c, int g,
-                                            float* lds, Running& r) {
-  KeyPiece kp[4];
-  ValuePiece<BITS> vp;
-  f32x4 k_as[4][2], v_as[4][2];
-#pragma unroll
-  for (int b = 0; b < 4; ++b) load_page_key<BITS>(u, 16 * b + c, g, kp[b]);
-  if (AFFINE<BITS, PREC>) load_page_scales<BITS>(u.k, u.rows, g, k_as);
-  load_values<BITS>(UnitRows{u.k, u.v, u.k_stride, u.v_stride, BITS, u.rows, 0, u.rows}, c, g, vp);
-  if (BITS < 16) load_page_scales<BITS>(u.v, u.rows, g, v_as);
-  f32x4 s[4];
-#pragma unroll
-  for (int b = 0; b < 4; ++b) {
-    Op k[2];
-    key_ops<BITS, PREC>(kp[b], k);
-    s[b] = mfma(k[1], q[1], mfma(k[0], q[0], f32x4{0, 0, 0, 0}));
-  }
-  if constexpr (AFFINE<BITS, PREC>) affine_scores<BITS>(k_as, q_sum, s);
-  bool bad = false;
-  if (rows < TILE || mixed) {
-    // Rows that are not visible: no score, and values of zero, so that what they hold (NaN or infinity) meets no p of zero.
-#pragma unroll
-    for (int b = 0; b < 4; ++b)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = 16 * b + 4 * g + i;
-        s[b][i] = row < u.high ? s[b][i] : -INFINITY;
-#pragma unroll
-        for (int j = 0; j < (BITS == 16 ? 2 : 1); ++j) vp.w[b][i][j] = row < rows ? vp.w[b][i][j] : 0u;
-        if (BITS < 16)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) v_as[b][i / 2][2 * (i % 2) + j] = row < rows ? v_as[b][i / 2][2 * (i % 2) + j] : 0.f;
-      }
-    if (BITS == 16 && mixed) {
-#pragma unroll
-      for (int b = 0; b < 4; ++b)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) bad = bad || bad_bf16(vp.w[b][i][j % (BITS == 16 ? 2 : 1)]) || bad_bf16(vp.w[b][i][j % (BITS == 16 ? 2 : 1)] >> 16);
-      bad = __builtin_amdgcn_ballot_w64(bad) != 0;
-      if (bad)
-#pragma unroll
-        for (int b = 0; b < 4; ++b)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              uint32_t& w = vp.w[b][i][j % (BITS == 16 ? 2 : 1)];
-              w &= (bad_bf16(w) ? 0u : 0xffffu) | (bad_bf16(w >> 16) ? 0u : 0xffff0000u);
-            }
-    }
-  }
-  float top = -INFINITY;
-#pragma unroll
-  for (int b = 0; b < 4; ++b)
+  for (int b = 0; b < 2; ++b)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      s[b][i] *= scale2;
-      top = fmaxf(top, s[b][i]);
+      s[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], scale2, -ref));
+      sum += s[b][i];
     }
-  top = fmaxf(row_max(top), r.m);
-  const float ref = top == -INFINITY ? 0.f : top;  // nothing visible yet: keep the empty state
-  const float alpha = __builtin_amdgcn_exp2f(r.m - ref);
-  r.m = top;
-  float sum = 0, offset = 0;
-  Op p[TERMS][2];
+  r.l += sum;
+}
+
+// The values by their weights (in s), which enter the product as the sum of TERMS bf16 values.
+template <int BITS, int PREC, int TERMS>
+__device__ __forceinline__ void weigh(const Loaded<BITS>& x, const float2* scales, int g, const f32x4 (&s)[2], Running& r) {
+  Op p[TERMS];
+  f32x4 as[2][2];
 #pragma unroll
-  for (int b = 0; b < 4; ++b)
+  for (int b = 0; b < 2; ++b)
 #pragma unroll
     for (int i = 0; i < 4; i += 2) {
-      float p0 = __builtin_amdgcn_exp2f(s[b][i] - ref), p1 = __builtin_amdgcn_exp2f(s[b][i + 1] - ref);
-      s[b][i] = p0, s[b][i + 1] = p1;
-      sum += p0 + p1;
-      if constexpr (AFFINE<BITS, PREC>) {
-        const f32x4 m = v_as[b][i / 2];
-        offset = __builtin_fmaf(p0, __builtin_fmaf(m[1], CENTRE<BITS>, m[0]), offset);
-        offset = __builtin_fmaf(p1, __builtin_fmaf(m[3], CENTRE<BITS>, m[2]), offset);
+      float p0 = s[b][i], p1 = s[b][i + 1];
+      if (BITS < 16) as[b][i / 2] = *reinterpret_cast<const f32x4*>(&scales[HALF + 16 * b + 4 * g + i]);
+      if constexpr (PREC == 1 && BITS < 16) {
+        const f32x4 m = as[b][i / 2];
+        r.offset = __builtin_fmaf(p0, m[0], r.offset);
+        r.offset = __builtin_fmaf(p1, m[2], r.offset);
         p0 *= m[1], p1 *= m[3];
       }
       uint32_t t[TERMS];
       split_pair<TERMS>(p0, p1, t);
 #pragma unroll
-      for (int k = 0; k < TERMS; ++k) p[k][b / 2].u[2 * (b % 2) + i / 2] = t[k];
+      for (int k = 0; k < TERMS; ++k) p[k].u[2 * b + i / 2] = t[k];
     }
-  r.l = r.l * alpha + sum;
-  if (PREC == 1) r.offset = r.offset * alpha + offset;
+  Codes<BITS == 16 ? 8 : BITS> w[2][4];
+  if (BITS < 16)
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[b][i] = codes_of<BITS == 16 ? 8 : BITS>(x.v[b][i][0]);
 #pragma unroll
   for (int db = 0; db < 4; ++db) {
-    Op v[2];
-    value_ops<BITS, PREC>(vp, v_as, db, v);
-    f32x4 o = r.o[db] * alpha;
+    Op v;
 #pragma unroll
-    for (int t = TERMS - 1; t >= 0; --t) o = mfma(v[1], p[t][1], mfma(v[0], p[t][0], o));
-    r.o[db] = o;
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < 4; i += 2) {
+        uint32_t y;
+        if (BITS == 16) {
+          const uint32_t x0 = x.v[b][i][(db >> 1) % (BITS == 16 ? 2 : 1)], x1 = x.v[b][i + 1][(db >> 1) % (BITS == 16 ? 2 : 1)];
+          y = db & 1 ? (x0 >> 16) | (x1 & 0xffff0000u) : (x0 & 0xffffu) | (x1 << 16);
+        } else {
+          const f32x4 m = as[b][i / 2];
+          y = values<PREC>(code(w[b][i], db), code(w[b][i + 1], db), m[1], m[0], m[3], m[2]);
+        }
+        v.u[2 * b + i / 2] = y;
+      }
+#pragma unroll
+    for (int t = TERMS - 1; t >= 0; --t) r.o[db] = mfma(v, p[t], r.o[db]);
   }
-  if (BITS == 16 && bad) add_bad_values(u, rows, s, c, g, lds, r);
+}
+
+// A wave's query rows and what it needs of them everywhere.
+struct Rows {
+  Op q[2];
+  float q_sum, scale2;
+  int c, g, lane;
+  float2* scales;  // LDS
+};
+
+// Half pages [at, end) of one width (2 u and 2 u + 1: unit u). The next one's keys are loaded when this one's are
+// multiplied, its values when these are. (A loop over pages of any width has to move what was loaded to the registers
+// that its branches share, and waits for it there. Whole pages at a time take 200 registers, two waves a SIMD.)
+template <int BITS, int PREC, int TERMS, class PAGE>
+__device__ __forceinline__ void attend_pages(int& at, int end, PAGE page, const Rows& w, Running& r) {
+  if (at >= end) return;
+  Loaded<BITS> x;
+  Half u = page(at);
+  load_keys<BITS>(u, w.c, w.g, x);
+  load_vals<BITS>(u, w.c, w.g, x);
+  for (;;) {
+    const int rows = u.rows;
+    const bool more = ++at < end;
+    f32x4 s[2];
+    if (BITS < 16) share_scales(w.scales, w.lane, x.pair, rows);
+    scores<BITS, PREC>(x, w.scales, w.c, w.g, w.q, w.q_sum, s);
+    if (more) {
+      u = page(at);
+      load_keys<BITS>(u, w.c, w.g, x);
+    }
+    if (rows < HALF) {  // rows that are not there: no score, and values of zero, so that what they hold meets no p of zero
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool there = 16 * b + 4 * w.g + i < rows;
+          s[b][i] = there ? s[b][i] : -INFINITY;
+#pragma unroll
+          for (int j = 0; j < (BITS == 16 ? 2 : 1); ++j) x.v[b][i][j] = there ? x.v[b][i][j] : 0u;
+        }
+    }
+    soften(s, w.scale2, r);
+    weigh<BITS, PREC, TERMS>(x, w.scales, w.g, s, r);
+    if (!more) break;
+    load_vals<BITS>(u, w.c, w.g, x);
+  }
 }
 
 template <int PREC, int TERMS>
-__global__ __launch_bounds__(256) void short_kernel(dkv_paged_args a, float* part_o, float2* part_ml) {
+__global__ __launch_bounds__(256, 4) void short_kernel(dkv_paged_args a, float* part_o, float2* part_ml) {
   __shared__ float ml[4][16][2];
   __shared__ f32x4 o[4][16][17];  // [wave][row][element / 4], padded
+  __shared__ __attribute__((aligned(16))) float2 scales[4][2 * HALF];
   const int32_t* plan = static_cast<const int32_t*>(a.plan_words);
   const int H = a.plan.heads, G = a.plan.q_heads / H, record = blockIdx.x / H, h = blockIdx.x % H;
   if (a.bounds && record >= plan[N_WORK]) return;
@@ -188,42 +274,99 @@ __global__ __launch_bounds__(256) void short_kernel(dkv_paged_args a, float* par
   const int row0 = w.block * SHORT_BLOCK, rows_here = min(SHORT_BLOCK, w.count * G - row0);
   const int row = row0 + min(c, rows_here - 1), m = row / G;  // this lane's query row, its token of the sequence
   const int m_first = row0 / G, m_last = (row0 + rows_here - 1) / G;
-  Op q[2];
+  Rows rw;
   query_ops(static_cast<const uint16_t*>(a.q) + (int64_t)(h * G + row - m * G) * a.q_head_stride + (int64_t)(w.token0 + m) * a.q_tok_stride,
-            c < rows_here, g, q);
+            c < rows_here, g, rw.q);
+  rw.q_sum = query_sum(rw.q);
+  rw.scale2 = a.scale * LOG2E;
+  rw.c = c, rw.g = g, rw.lane = lane;
+  rw.scales = scales[wave];
+  const Op (&q)[2] = rw.q;
+  const float scale2 = rw.scale2;
   Running r;
   r.m = -INFINITY, r.l = r.offset = 0.f;
-  const float q_sum = query_sum(q);
   for (int db = 0; db < 4; ++db) r.o[db] = f32x4{0, 0, 0, 0};
-  const float scale2 = a.scale * LOG2E;
-  for (int i = w.u0 + wave; i < w.u1; i += 4) {
-    Unit u;
-    int rows;
-    bool mixed = false;
-    if (i < w.n_pages) {
-      const Page pg = plan_record<Page>(plan, a.plan.at_pages, w.first_page + i);
-      u.bits = page_bits(pg.page);
-      u.k = static_cast<const uint8_t*>(a.arena) + page_at(pg.page, a.layer, a.plan.layers, H, h);
-      u.v = u.k + (int64_t)H * page_sub(u.bits);
-      u.k_stride = u.v_stride = 8 * u.bits;
-      u.rows = u.high = rows = pg.rows;
-    } else {
-      const int first = (i - w.n_pages) * TILE;
-      u.bits = 16;
-      u.k = static_cast<const uint8_t*>(a.k_new) + 2 * (h * a.kn_head_stride + (int64_t)(w.token0 + first) * a.kn_tok_stride);
-      u.v = static_cast<const uint8_t*>(a.v_new) + 2 * (h * a.vn_head_stride + (int64_t)(w.token0 + first) * a.vn_tok_stride);
-      u.k_stride = (uint32_t)(2 * a.kn_tok_stride);  // (of a single row, whatever it is)
-      u.v_stride = (uint32_t)(2 * a.vn_tok_stride);
-      u.rows = min(TILE, w.count - first);
-      u.high = min(TILE, m + 1 - first);
-      rows = min(TILE, m_last + 1 - first);
-      mixed = m_first + 1 - first < rows;
+  const uint8_t* const base = static_cast<const uint8_t*>(a.arena);
+  const int64_t grain = grain_bytes(a.plan.layers, H), sub = (int64_t)a.layer * 2 * H + h;
+  auto page = [&](int i) {
+    const Page pg = plan_record<Page>(plan, a.plan.at_pages, w.first_page + i / 2);
+    const int bits = page_bits(pg.page), first = i % 2 * HALF;
+    const uint8_t *k = base + (pg.page >> 2) * grain + sub * page_sub(bits), *v = k + (int64_t)H * page_sub(bits);
+    Half u;
+    u.rows = min(HALF, pg.rows - first);  // (none: a page of up to 32 tokens)
+    u.k = k + first * 8 * bits, u.v = v + first * 8 * bits;
+    u.scales = (lane < HALF ? k : v) + (TILE * 8 * bits + 8 * first + 8 * (lane & (HALF - 1)));
+    return u;
+  };
+  // A wave takes a fourth of the units that follow each other, so that it meets few widths.
+  const int u0 = w.u0 + (w.u1 - w.u0) * wave / 4, u1 = w.u0 + (w.u1 - w.u0) * (wave + 1) / 4;
+  int at = 2 * u0;
+  attend_pages<4, PREC, TERMS>(at, 2 * min(w.n4, u1), page, rw, r);
+  attend_pages<8, PREC, TERMS>(at, 2 * min(w.n8, u1), page, rw, r);
+  attend_pages<16, PREC, TERMS>(at, 2 * min(w.n_pages, u1), page, rw, r);
+  bool bad = false;  // some new value that is infinite or NaN was taken for zero
+  for (; at < 2 * u1; ++at) {  // new tokens, as they are, up to each query row's own
+    const int first = (at - 2 * w.n_pages) * HALF, seen = min(HALF, m_last + 1 - first), high = min(seen, m + 1 - first);
+    if (seen <= 0) break;
+    const bool mixed = m_first + 1 - first < seen;
+    Half u;
+    u.k = static_cast<const uint8_t*>(a.k_new) + 2 * (h * a.kn_head_stride + (int64_t)(w.token0 + first) * a.kn_tok_stride);
+    u.v = static_cast<const uint8_t*>(a.v_new) + 2 * (h * a.vn_head_stride + (int64_t)(w.token0 + first) * a.vn_tok_stride);
+    u.k_stride = (uint32_t)(2 * a.kn_tok_stride), u.v_stride = (uint32_t)(2 * a.vn_tok_stride);  // (of a single row, whatever it is)
+    u.rows = min(HALF, w.count - first);
+    Loaded<16> x;
+    load_keys<16, true>(u, c, g, x);
+    load_vals<16, true>(u, c, g, x);
+    f32x4 s[2];
+    scores<16, PREC>(x, rw.scales, c, g, q, rw.q_sum, s);
+    // Values that not every query row of the block sees are zero where they are infinite or NaN (a p of zero makes NaN of
+    // them) and are added after all units; those that none sees are zero.
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = 16 * b + 4 * g + i;
+        s[b][i] = key < high ? s[b][i] : -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          uint32_t& y = x.v[b][i][j];
+          y = key < seen ? y : 0u;
+          const uint32_t keep = mixed ? (bad_bf16(y) ? 0u : 0xffffu) | (bad_bf16(y >> 16) ? 0u : 0xffff0000u) : 0xffffffffu;
+          bad = bad || keep != 0xffffffffu;
+          y &= keep;
+        }
+      }
+    soften(s, scale2, r);
+    weigh<16, PREC, TERMS>(x, rw.scales, g, s, r);
+  }
+  if (__builtin_amdgcn_ballot_w64(bad)) {  // (rare) with their weights computed again
+    for (int j = 0; j <= m_last; ++j) {
+      const int piece = w.n_pages + j / TILE;
+      const int first = j / HALF * HALF;
+      if (piece < u0 || piece >= u1 || m_first + 1 - first >= min(HALF, m_last + 1 - first)) continue;  // not this wave's, or seen by every row
+      const int64_t tok = w.token0 + j;
+      const u32x4* k = reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.k_new) + h * a.kn_head_stride + tok * a.kn_tok_stride + 16 * g);
+      const u32x4* v = reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.v_new) + h * a.vn_head_stride + tok * a.vn_tok_stride + 16 * g);
+      float dot = 0;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const u32x4 y = k[i];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          dot = __builtin_fmaf(bf16_lo(q[i].u[e]), bf16_lo(y[e]), __builtin_fmaf(bf16_hi(q[i].u[e]), bf16_hi(y[e]), dot));
+      }
+      const float p = __builtin_amdgcn_exp2f(row_sum(dot) * scale2 - r.m);
+      if (j > m) continue;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const u32x4 y = v[i];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {  // elements 16 g + 8 i + 2 e + ... = 16 g + 4 (2 i + e / 2) + 2 (e % 2) + ...
+          if (bad_bf16(y[e])) r.o[2 * (e % 2)][2 * i + e / 2] += p * bf16_lo(y[e]);
+          if (bad_bf16(y[e] >> 16)) r.o[2 * (e % 2) + 1][2 * i + e / 2] += p * bf16_hi(y[e]);
+        }
+      }
     }
-    const int bits = __builtin_amdgcn_readfirstlane(u.bits);
-    float* lds = reinterpret_cast<float*>(&o[wave][0][0]);
-    if (bits == 4) attend_unit<4, PREC, TERMS>(u, rows, mixed, q, q_sum, scale2, c, g, lds, r);
-    else if (bits == 8) attend_unit<8, PREC, TERMS>(u, rows, mixed, q, q_sum, scale2, c, g, lds, r);
-    else attend_unit<16, PREC, TERMS>(u, rows, mixed, q, q_sum, scale2, c, g, lds, r);
   }
   r.l = row_sum(r.l);
   r.offset = PREC == 1 ? row_sum(r.offset) : 0.f;
@@ -238,62 +381,74 @@ __global__ __launch_bounds__(256) void short_kernel(dkv_paged_args a, float* par
   for (int k = 0; k < 4; ++k) top = fmaxf(top, ml[k][rr][0]);
   const float ref = top == -INFINITY ? 0.f : top;
   float l = 0.f;
-  f32x4 x = {0, 0, 0, 0};
+  f32x4 y = {0, 0, 0, 0};
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const float f = __builtin_amdgcn_exp2f(ml[k][rr][0] - ref);
     l += f * ml[k][rr][1];
-    x += f * o[k][rr][e4];
+    y += f * o[k][rr][e4];
   }
   if (w.part < 0) {
-    const int at = row0 + rr, tok = at / G;
-    store4(a.out, a.out_dtype, (int64_t)(w.token0 + tok) * a.out_tok_stride + (int64_t)(h * G + at - tok * G) * a.out_head_stride + 4 * e4,
-           x / l);
+    const int out_row = row0 + rr, tok = out_row / G;
+    store4(a.out, a.out_dtype, (int64_t)(w.token0 + tok) * a.out_tok_stride + (int64_t)(h * G + out_row - tok * G) * a.out_head_stride + 4 * e4,
+           y / l);
   } else {
-    const int64_t at = (int64_t)(w.part + rr) * H + h;
-    *reinterpret_cast<f32x4*>(part_o + at * D + 4 * e4) = x;
-    if (e4 == 0) part_ml[at] = make_float2(top, l);
+    const int64_t to = (int64_t)(w.part + rr) * H + h;
+    *reinterpret_cast<f32x4*>(part_o + to * D + 4 * e4) = y;
+    if (e4 == 0) part_ml[to] = make_float2(top, l);
   }
 }
 
-// Joins the partials of 16 query rows: 16 lanes a row, four elements a lane.
+// Joins the partials of 16 query rows: a wave a row, 16 lanes a split with four elements each, four splits at a time and
+// AHEAD of these in flight. (16 lanes a row: 48 branches, whose 127 pages in common are split 64 ways, 13.9 us.)
 __global__ __launch_bounds__(256) void merge_kernel(dkv_paged_args a, const float* part_o, const float2* part_ml) {
   const int32_t* plan = static_cast<const int32_t*>(a.plan_words);
-  const int H = a.plan.heads, G = a.plan.q_heads / H, record = blockIdx.x / H, h = blockIdx.x % H;
+  const int H = a.plan.heads, G = a.plan.q_heads / H, h = blockIdx.x % H, four = blockIdx.x / H, record = four / (SHORT_BLOCK / 4);
   if (a.bounds && record >= plan[N_MERGES]) return;
   const Merge w = plan_record<Merge>(plan, a.plan.at_merges, record);
-  const int row = w.row0 + (threadIdx.x >> 4), e4 = threadIdx.x & 15;
+  const int lane = threadIdx.x & 63, e4 = lane & 15, s0 = lane >> 4;
+  const int row = w.row0 + four % (SHORT_BLOCK / 4) * 4 + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   if (row >= w.rows) return;
   const int own = w.splits & 0xffff, n = own + (w.splits >> 16);
   auto at = [&](int s) {
     return ((int64_t)(row - w.row0) + (s < own ? w.part + s * w.stride : w.shared + (s - own) * w.shared_stride)) * H + h;
   };
-  float top = -INFINITY;
-  for (int i = e4; i < n; i += 16) top = fmaxf(top, part_ml[at(i)].x);
-#pragma unroll
-  for (int d = 8; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 16));
-  const float ref = top == -INFINITY ? 0.f : top;
-  float l = 0.f;
+  float top = -INFINITY, l = 0.f;
   f32x4 x = {0, 0, 0, 0};
-  constexpr int AHEAD = 8;  // splits in flight
-  for (int i0 = 0; i0 < n; i0 += AHEAD) {
+  constexpr int AHEAD = 4;
+  for (int i0 = 0; i0 < n; i0 += 4 * AHEAD) {
     float2 p[AHEAD];
     f32x4 o[AHEAD];
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
-      const int64_t i = at(min(i0 + j, n - 1));
+      const int64_t i = at(min(i0 + 4 * j + s0, n - 1));
       p[j] = part_ml[i];
       o[j] = *reinterpret_cast<const f32x4*>(part_o + i * D + 4 * e4);
     }
+    float here = top;
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
-      const float f = i0 + j < n ? __builtin_amdgcn_exp2f(p[j].x - ref) : 0.f;
-      if (i0 + j < n) l += f * p[j].y, x += f * o[j];
+      if (i0 + 4 * j + s0 >= n) p[j] = make_float2(-INFINITY, 0.f), o[j] = f32x4{0, 0, 0, 0};
+      here = fmaxf(here, p[j].x);
+    }
+    const float ref = here == -INFINITY ? 0.f : here, alpha = __builtin_amdgcn_exp2f(top - ref);
+    l *= alpha, x *= alpha;
+    top = here;
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      const float f = __builtin_amdgcn_exp2f(p[j].x - ref);
+      l += f * p[j].y;
+      x += f * o[j];
     }
   }
+  const float all = rows::row_max(top), ref = all == -INFINITY ? 0.f : all, f = __builtin_amdgcn_exp2f(top - ref);
+  l = rows::row_sum(l * f);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] = rows::row_sum(x[e] * f);
   const int tok = row / G;
-  store4(a.out, a.out_dtype, (int64_t)(w.token0 + tok) * a.out_tok_stride + (int64_t)(h * G + row - tok * G) * a.out_head_stride + 4 * e4,
-         x / l);
+  if (s0 == 0)
+    store4(a.out, a.out_dtype, (int64_t)(w.token0 + tok) * a.out_tok_stride + (int64_t)(h * G + row - tok * G) * a.out_head_stride + 4 * e4,
+           x / l);
 }
 
 static int64_t up256(int64_t x) { return (x + 255) & ~(int64_t)255; }
@@ -331,11 +486,12 @@ int dkv_paged_attend(const dkv_paged_args* args, void* stream) {
   float* part_o = static_cast<float*>(a.workspace);
   float2* part_ml = reinterpret_cast<float2*>(static_cast<char*>(a.workspace) + up256(4 * D * rows));
   const int work = a.bounds ? p.max_work : p.work, merges = a.bounds ? p.max_merges : p.merges;
-  const auto attend = a.precision == 1 ? (a.out_dtype == 1 ? short_kernel<1, 3> : short_kernel<1, 2>)
-                                       : (a.out_dtype == 1 ? short_kernel<0, 3> : short_kernel<0, 2>);
+  // (At precision 1 a weight meets codes of up to 255 whose offset comes apart: two terms would be off by 2^-17 of a row's
+  // range.)
+  const auto attend = a.precision == 1 ? short_kernel<1, 3> : a.out_dtype == 1 ? short_kernel<0, 3> : short_kernel<0, 2>;
   if (const int n = a.bounds ? p.max_long : p.long_work) launch_long(a, n, part_o, part_ml, st);
   if (work > 0) hipLaunchKernelGGL(attend, dim3(p.heads * work), dim3(256), 0, st, a, part_o, part_ml);
-  if (merges > 0) hipLaunchKernelGGL(merge_kernel, dim3(p.heads * merges), dim3(256), 0, st, a, part_o, part_ml);
+  if (merges > 0) hipLaunchKernelGGL(merge_kernel, dim3(p.heads * merges * (SHORT_BLOCK / 4)), dim3(256), 0, st, a, part_o, part_ml);
   return (int)hipGetLastError();
 }
 

@@ -272,7 +272,7 @@ def test_a_plan_covers_every_row_and_unit_once():
         pages, rows, first, past, shared = [], [], [0], [], rng.integers(0, 12)
         for i in range(n):
             old = int(rng.integers(0, 20)) if rng.random() < .8 else 0
-            mine = [(int(x) * 16 << 2 | 2) for x in ((list(range(shared)) if old else []) + (100 + 40 * i + np.arange(40)).tolist())]
+            mine = [(int(x) * 16 << 2 | int(x) % 3) for x in ((list(range(shared)) if old else []) + (100 + 40 * i + np.arange(40)).tolist())]
             held = [64] * int(shared if old else 0)
             held += [int(x) for x in rng.integers(1, 65, old)]
             past.append(sum(held))
@@ -300,7 +300,8 @@ def test_a_plan_covers_every_row_and_unit_once():
         seen = {}
         parts = {}
         for at, k, block_rows in ((plan.at_work, plan.work, 16), (plan.at_long, plan.long_work, 256)):
-            for f, pg, tok, cnt, blk, u0, u1, part in records(at, k, 8):
+            for f, n4, n8, pg, tok, cnt, blk, u0, u1, part, _, _ in records(at, k, 12):
+                assert [held[f + u][0] & 3 for u in range(pg)] == [0] * n4 + [1] * (n8 - n4) + [2] * (pg - n8)
                 for r in range(block_rows * blk, min(block_rows * (blk + 1), cnt * G)):
                     row = (tok + r // G, r % G)
                     units = seen.setdefault(row, [])
@@ -371,7 +372,7 @@ def test_append_and_attend_refuse(kw):
 
 
 @pytest.mark.parametrize('kw', [dict(q=0), dict(q=4104), dict(q_tok_stride=4), dict(out=None), dict(out=4100), dict(out_tok_stride=2),
-                                dict(out_dtype=2), dict(precision=2), dict(kn_tok_stride=1 << 23), dict(vn_tok_stride=-64)])
+                                dict(out_dtype=2), dict(precision=2), dict(scale=0.0), dict(scale=-1.0), dict(scale=float('nan')), dict(scale=float('inf')), dict(kn_tok_stride=1 << 23), dict(vn_tok_stride=-64)])
 def test_attend_refuses(kw):
     assert _lib.load().dkv_paged_attend(ctypes.byref(args(**kw)), None) == _lib.DKV_EINVAL
 
