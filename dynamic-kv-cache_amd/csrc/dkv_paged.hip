@@ -6,6 +6,7 @@
 #include "dkv_rope_pack.h"
 #include <string.h>
 #include <algorithm>
+#include <functional>
 #include <new>
 #include <vector>
 
@@ -202,12 +203,16 @@ int launch_moves(const void* src, void* dst, const dkv_page_move* moves, int n_m
 
 // ---- plans -------------------------------------------------------------------------------------------------------
 
-// Entities of up to this many query rows of a KV head go to the kernel for few rows.
-constexpr int SHORT_ROWS = 48;
-// Workgroups over all KV heads that a step is split into, about, and the least units of one: for few rows (four waves, a
-// unit each at a time) and for many (eight waves, a unit at a time).
+// Entities of up to this many query rows of a KV head go to the kernel for few rows. (144 rows over 127 pages, 5 heads: 18.5 us
+// there, 29.0 in the kernel for many, which has few workgroups for them; 180 rows and more over 96 pages 46.1 and 44.7.)
+constexpr int SHORT_ROWS = 160;
+// Few rows (four waves, a unit each at a time): about SHORT_TARGET workgroups over all KV heads share a step's units, four
+// resident a CU, of SHORT_LEAST units at least (three short histories 8.0 us with 8, 11.6 with 4 and a join). A token of 64
+// streams / of 6 long ones: 1024 workgroups 34.3 / 110.6 us, 2048 31.8 / 105.9.
 constexpr int SHORT_TARGET = 2048, SHORT_LEAST = 8;
-constexpr int LONG_TARGET = 512, LONG_LEAST = 2;
+// Many rows (eight waves, a unit at a time): a step is split into LONG_TARGET workgroups at most (two a CU) beside those that
+// its blocks need, of LONG_LEAST units at least, by ranges of such a length that the last workgroup ends first (long_share).
+constexpr int LONG_TARGET = 512, LONG_LEAST = 2, CUS = 256;
 constexpr int SHARED_MIN = 4;  // pages that neighbours have in common to be attended to as a group
 
 struct Entity {  // a sequence's own part, or what a group of sequences has in common
@@ -296,14 +301,57 @@ static int units_of(const Entity& e, int G, int block, int blk) {
   return e.n_pages + last / TILE + 1;
 }
 
-// Units of a workgroup so that about `target` of them a KV head share all entities' units of this kind.
-static int64_t share(const std::vector<Entity>& es, int G, bool many, int64_t target, int least) {
+static int64_t total_units(const std::vector<Entity>& es, int G, bool many) {
   const int block = many ? LONG_BLOCK : SHORT_BLOCK;
   int64_t total = 0;
   for (const Entity& e : es)
     if (is_long((int64_t)e.count * G) == many)
       for (int blk = 0, n = ceil_div((int64_t)e.count * G, block); blk < n; ++blk) total += units_of(e, G, block, blk);
-  return std::max<int64_t>(least, (total + target - 1) / target);
+  return total;
+}
+
+// Units of a workgroup so that about `target` of them a KV head share all entities' units of this kind.
+static int64_t share(int64_t total, int64_t target, int least) { return std::max<int64_t>(least, (total + target - 1) / target); }
+
+// The same for many rows: of ranges from that length on, the one whose workgroups are done first when each free CU takes the
+// longest that is left (one workgroup keeps its vector units busy: two on a CU take twice as long). In units: a workgroup
+// costs its units and what its start takes, one that is joined its partial rows beside, and the join reads them. (Equal
+// shares for 512 workgroups and for 256: 12500 tokens of prompts 267 and 239 us, 12 prompts 82 and 68, 8 frames 131 and 172.)
+static int64_t long_share(const std::vector<Entity>& es, int G, int heads, int groups, const std::vector<int>& group) {
+  const int slots = std::max(1, CUS / heads);
+  const int64_t least = share(total_units(es, G, true), ceil_div(LONG_TARGET, heads), LONG_LEAST);
+  int64_t most = 0, best = least;
+  for (const Entity& e : es)
+    if (is_long((int64_t)e.count * G)) most = std::max<int64_t>(most, units_of(e, G, LONG_BLOCK, ceil_div((int64_t)e.count * G, LONG_BLOCK) - 1));
+  constexpr float START = 2.5f, PARTIAL = 2.f, JOIN = 3e-5f;  // of a workgroup; of its 256 rows; of a partial row and head
+  float best_time = 0.f;
+  std::vector<float> costs, ends;
+  for (int64_t len = least;; len += std::max<int64_t>(1, len / 4)) {
+    costs.clear();
+    int64_t rows = 0;
+    for (size_t i = 0; i < es.size(); ++i) {
+      const Entity& e = es[i];
+      const int64_t total = (int64_t)e.count * G;
+      if (!is_long(total)) continue;
+      for (int blk = 0; blk < ceil_div(total, LONG_BLOCK); ++blk) {
+        const int units = units_of(e, G, LONG_BLOCK, blk), splits = std::max(1, ceil_div(units, len));
+        const bool parts = splits > 1 || e.group || group[i - groups] >= 0;
+        if (parts) rows += (int64_t)splits * std::min<int64_t>(LONG_BLOCK, total - (int64_t)blk * LONG_BLOCK);
+        for (int s = 0; s < splits; ++s) costs.push_back((float)units / splits + START + (parts ? PARTIAL : 0.f));
+      }
+    }
+    std::sort(costs.begin(), costs.end(), std::greater<float>());
+    ends.assign(slots, 0.f);  // a heap of when each place is free
+    float last = 0.f;
+    for (float c : costs) {
+      std::pop_heap(ends.begin(), ends.end(), std::greater<float>());
+      last = std::max(last, ends.back() += c);
+      std::push_heap(ends.begin(), ends.end(), std::greater<float>());
+    }
+    const float time = last + JOIN * (float)rows * heads;
+    if (best_time == 0.f || time < best_time) best_time = time, best = len;
+    if (len >= most) return best;
+  }
 }
 
 static int write_plan(const dkv_paged_batch& b, int32_t* w, dkv_paged_plan& p) {
@@ -391,8 +439,8 @@ static int write_plan(const dkv_paged_batch& b, int32_t* w, dkv_paged_plan& p) {
     std::stable_sort(from, from + e.n_pages, [](const Page& x, const Page& y) { return (x.page & 3) < (y.page & 3); });
     for (int i = 0; i < e.n_pages; ++i) e.n4 += (from[i].page & 3) == 0, e.n8 += (from[i].page & 3) <= 1;
   }
-  const int64_t few = share(all, G, false, ceil_div(SHORT_TARGET, b.heads), SHORT_LEAST);
-  const int64_t many = share(all, G, true, ceil_div(LONG_TARGET, b.heads), LONG_LEAST);
+  const int64_t few = share(total_units(all, G, false), ceil_div(SHORT_TARGET, b.heads), SHORT_LEAST);
+  const int64_t many = long_share(all, G, b.heads, groups, group);
   Work* const work = reinterpret_cast<Work*>(w + p.at_work);
   Work* const long_work = reinterpret_cast<Work*>(w + p.at_long);
   Merge* merges = reinterpret_cast<Merge*>(w + p.at_merges);

@@ -20,6 +20,7 @@ using rows::split_pair;
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
 union Op8 {
   bf16x8 v;
@@ -28,37 +29,43 @@ union Op8 {
 };
 
 constexpr int WAVES = LONG_BLOCK / 32;
-constexpr int RING = 3;          // units in LDS: one is read, one arrives, one is written
-constexpr int TILE_BYTES = 8192;  // K or V of a unit: row r's 16-byte piece p lies at r * 128 + (p ^ r % 8) * 16
+constexpr int RING = 3;           // units' tiles in LDS (one is read, one is written or has arrived, one arrives), and packed units
+constexpr int TILE_BYTES = 8192;  // K or V of a unit: row r's 16-byte piece p lies at r * 128 + (p ^ place(r)) * 16
+constexpr int RAW_V = 4096, RAW_SCALES = 8192, RAW_BYTES = 9216;  // a packed unit as it is stored: K, V, (offset, scale) of K and V
 
-// A unit that comes through registers: a page's rows, or new ones that not all of the workgroup's query rows see.
-struct Source {
-  const uint8_t* k;
-  const uint8_t* v;
-  uint32_t k_stride, v_stride;  // bytes from row to row
-  int bits, rows;               // rows that are there
-  bool page;
-};
+// Rows of equal parity share banks. This order keeps apart the equal pieces of rows {0-3, 12-15, 20-23, 24-27} (and these
+// + 4, + 8, + 16), which one step of a 16-byte read takes, and the four neighbouring pieces of rows 4 n + {0, 2}, which the
+// transposing reads do.
+__device__ __forceinline__ int place(int row) { return (row >> 1 & 1) << 2 | (row >> 3 & 1) << 1 | (row >> 2 & 1); }
 
-struct Raw {  // a thread's 8 elements of a row of K and of V
-  u32x4 k, v;
-  float2 ka, va;
-};
+// load_piece (dkv_common.h) from an address that a wave shares and an offset of each lane.
+__device__ __forceinline__ void load_piece_at(const uint8_t* from, uint32_t offset, uint32_t to) {
+  uint32_t m0;
+  asm volatile("s_mov_b32 %0, m0\n s_mov_b32 m0, %3\n s_nop 0\n global_load_lds_dwordx4 %1, %2\n s_mov_b32 m0, %0"
+               : "=&s"(m0) : "v"(offset), "s"(from), "s"(to) : "memory");
+}
 
 // 8 elements of a packed row as bf16: their values (PREC 0), or the centred codes, whose scale and offset come later.
 template <int PREC>
-__device__ __forceinline__ u32x4 unpack8(int bits, const u32x4& w, const float2& as) {
-  if (bits == 16) return w;
+__device__ __forceinline__ u32x4 unpack8(int bits, const uint2& w, const float2& as) {
   float x[8];
+  const uint32_t even = bits == 4 ? w.x & 0x0f0f0f0fu : w.x, odd = bits == 4 ? (w.x >> 4) & 0x0f0f0f0fu : w.y;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = (float)(bits == 4 ? (w[0] >> (4 * e)) & 15u : (w[e >> 2] >> (8 * (e & 3))) & 255u);
-  u32x4 out;
+  for (int e = 0; e < 4; ++e) x[e] = (float)((even >> (8 * e)) & 255u), x[4 + e] = (float)((odd >> (8 * e)) & 255u);
+  const float c = bits == 4 ? CENTRE<4> : CENTRE<8>;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float c = bits == 4 ? CENTRE<4> : CENTRE<8>;
-    out[i] = PREC ? pack_bf16(x[2 * i] - c, x[2 * i + 1] - c) : pack_bf16(x[2 * i] * as.y + as.x, x[2 * i + 1] * as.y + as.x);
-  }
-  return out;
+  for (int e = 0; e < 8; ++e) x[e] = PREC ? x[e] - c : x[e] * as.y + as.x;
+  if (bits == 4)  // (bytes of `even` and `odd` are every other element)
+    return u32x4{pack_bf16(x[0], x[4]), pack_bf16(x[1], x[5]), pack_bf16(x[2], x[6]), pack_bf16(x[3], x[7])};
+  return u32x4{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])};
+}
+
+// At most n loads straight to LDS of this wave are under way.
+__device__ __forceinline__ void wait_loads(int n) {
+  if (n == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  else if (n == 1) asm volatile("s_waitcnt vmcnt(1)" ::: "memory");
+  else if (n == 2) asm volatile("s_waitcnt vmcnt(2)" ::: "memory");
+  else asm volatile("s_waitcnt vmcnt(3)" ::: "memory");
 }
 
 // max(a, b, c) of values that are never NaN (see max_nn).
@@ -71,87 +78,110 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 template <int PREC, int TERMS>
 __global__ __launch_bounds__(64 * WAVES, PREC ? 2 : 4) void long_kernel(dkv_paged_args a, float* part_o, float2* part_ml) {
   __shared__ __attribute__((aligned(1024))) uint8_t tiles[RING][2][TILE_BYTES];
-  __shared__ int bad;  // a new value that is infinite or NaN was taken for zero
+  __shared__ __attribute__((aligned(1024))) uint8_t packed_rows[RING][RAW_BYTES];
   __shared__ __attribute__((aligned(16))) float2 scales[PREC ? RING : 1][2][PREC ? TILE : 1];  // {offset + scale * centre, scale}
+  __shared__ int bad;  // a new value that is infinite or NaN was taken for zero
   const int32_t* plan = static_cast<const int32_t*>(a.plan_words);
   const int H = a.plan.heads, G = a.plan.q_heads / H, record = blockIdx.x / H, h = blockIdx.x % H;
   if (a.bounds && record >= plan[N_LONG]) return;
   const Work w = plan_record<Work>(plan, a.plan.at_long, record);
-  auto page = [&](int u) { return plan_record<Page>(plan, a.plan.at_pages, w.first_page + u); };
   const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, c = lane & 31, half = lane >> 5;
   const int total = w.count * G, wave0 = w.block * LONG_BLOCK + 32 * wave;  // the wave's first query row
   const bool on = wave0 < total;
   const int row = min(wave0 + c, total - 1), m = row / G;  // this lane's query row and its token
+  const int first_token = w.block * LONG_BLOCK / G;  // of the workgroup's query rows
   const int m_first = min(wave0, total - 1) / G, m_last = min(wave0 + 31, total - 1) / G;
-  const int srow = t >> 3, piece = (t & 7) ^ (srow & 7);  // of the tiles' rows, this thread's 8 elements 8 * piece
+  const int srow = t >> 3, piece = (t & 7) ^ place(srow);  // of the tiles' rows, this thread's 8 elements 8 * piece
 
-  // Units from here on come straight to LDS while every query row of the workgroup sees all of their keys.
-  const int seen_by_all = w.n_pages + (min(w.block * LONG_BLOCK, total - 1) / G + 1) / TILE;
-  auto straight = [&](int u) { return u >= w.n_pages && u < seen_by_all; };
-  auto source = [&](int u) {
-    Source s;
-    s.page = u < w.n_pages;
-    if (s.page) {
-      const Page p = page(u);
-      s.bits = page_bits(p.page), s.rows = p.rows;
-      s.k = static_cast<const uint8_t*>(a.arena) + page_at(p.page, a.layer, a.plan.layers, H, h);
-      s.v = s.k + (int64_t)H * page_sub(s.bits);
-      s.k_stride = s.v_stride = 8 * s.bits;
-    } else {
-      const int first = (u - w.n_pages) * TILE;
-      s.bits = 16, s.rows = min(TILE, w.count - first);
-      s.k = static_cast<const uint8_t*>(a.k_new) + 2 * (h * a.kn_head_stride + (int64_t)(w.token0 + first) * a.kn_tok_stride);
-      s.v = static_cast<const uint8_t*>(a.v_new) + 2 * (h * a.vn_head_stride + (int64_t)(w.token0 + first) * a.vn_tok_stride);
-      s.k_stride = (uint32_t)(2 * a.kn_tok_stride), s.v_stride = (uint32_t)(2 * a.vn_tok_stride);
-    }
-    return s;
+  // A unit: 64 rows (`rows` of them there) of a page or of the new tokens, and how many loads of it this wave issues.
+  struct Unit {
+    int bits, rows, loads;
+    uint32_t page;
   };
-  auto load_raw = [&](const Source& s, Raw& r) {
-    const int at = srow < s.rows ? srow : 0;
-    const uint8_t* k = s.k + (__umul24(at, s.k_stride) + s.bits * piece);
-    const uint8_t* v = s.v + (__umul24(at, s.v_stride) + s.bits * piece);
-    if (s.bits == 4) {
-      r.k[0] = *reinterpret_cast<const uint32_t*>(k);
-      r.v[0] = *reinterpret_cast<const uint32_t*>(v);
-    } else if (s.bits == 8) {
-      const uint2 x = *reinterpret_cast<const uint2*>(k), y = *reinterpret_cast<const uint2*>(v);
-      r.k[0] = x.x, r.k[1] = x.y, r.v[0] = y.x, r.v[1] = y.y;
+  auto unit_at = [&](int u) {
+    Unit x{16, 0, 0, 0};
+    if (u >= w.u1) return x;
+    if (u < w.n_pages) {
+      const Page p = plan_record<Page>(plan, a.plan.at_pages, w.first_page + u);
+      x.bits = page_bits(p.page), x.rows = p.rows, x.page = p.page;
     } else {
-      r.k = *reinterpret_cast<const u32x4*>(k);
-      r.v = *reinterpret_cast<const u32x4*>(v);
+      x.rows = min(TILE, w.count - (u - w.n_pages) * TILE);
     }
-    if (s.bits < 16) {
-      r.ka = *reinterpret_cast<const float2*>(s.k + TILE * 8 * s.bits + 8 * at);
-      r.va = *reinterpret_cast<const float2*>(s.v + TILE * 8 * s.bits + 8 * at);
-    }
+    x.loads = x.bits == 16 ? 2 : x.bits == 8 ? 1 + (wave == 0) : (wave & 3) < 2 || wave == 2;
+    return x;
   };
-  auto write_raw = [&](const Source& s, const Raw& r, int buf) {
-    const bool there = srow < s.rows;  // (rows that are not there: zeros, which meet a p of zero)
-    const u32x4 k = unpack8<PREC>(s.bits, r.k, r.ka);
-    u32x4 v = unpack8<PREC>(s.bits, r.v, r.va);
-    if (!s.page) {  // an infinite or NaN value meets a p of zero where it is not seen: zero, and added after all units
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint32_t keep = (bad_bf16(v[e]) ? 0u : 0xffffu) | (bad_bf16(v[e] >> 16) ? 0u : 0xffff0000u);
-        if (there && keep != 0xffffffffu) bad = 1;
-        v[e] &= keep;
-      }
+  const uint32_t tile0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)&tiles[0][0][0];
+  const uint32_t raw0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)&packed_rows[0][0];
+  const uint8_t* const base = static_cast<const uint8_t*>(a.arena);
+  const int64_t grain = grain_bytes(a.plan.layers, H), sub = (int64_t)a.layer * 2 * H + h;
+  // Rows of 16 bits go straight to their tile: a wave 8 rows of K and of V. New rows past the last one repeat it; rows of a
+  // page that are not there are read as they are (zero_values).
+  auto load_tile = [&](int u, const Unit& x, int buf) {
+    const uint8_t *k, *v;
+    uint32_t k_off = 16 * piece, v_off = 16 * piece;
+    if (u < w.n_pages) {
+      k = base + (x.page >> 2) * grain + sub * page_sub(16);
+      v = k + (int64_t)H * page_sub(16);
+      k_off += srow * 128, v_off += srow * 128;
+    } else {
+      const int64_t tok = w.token0 + (u - w.n_pages) * TILE;
+      const int r = min(srow, x.rows - 1);
+      k = static_cast<const uint8_t*>(a.k_new) + 2 * (h * a.kn_head_stride + tok * a.kn_tok_stride);
+      v = static_cast<const uint8_t*>(a.v_new) + 2 * (h * a.vn_head_stride + tok * a.vn_tok_stride);
+      k_off += __umul24(r, (uint32_t)(2 * a.kn_tok_stride)), v_off += __umul24(r, (uint32_t)(2 * a.vn_tok_stride));
     }
-    *reinterpret_cast<u32x4*>(&tiles[buf][0][16 * t]) = there ? k : u32x4{0, 0, 0, 0};
-    *reinterpret_cast<u32x4*>(&tiles[buf][1][16 * t]) = there ? v : u32x4{0, 0, 0, 0};
+    const uint32_t to = tile0 + buf * (2 * TILE_BYTES) + 1024 * wave;
+    load_piece_at(k, k_off, to);
+    load_piece_at(v, v_off, to + TILE_BYTES);
+  };
+  // Packed rows come as they are: at 8 bits a wave 1 KB of K (waves 0 to 3) or V, at 4 bits every other wave, and one wave
+  // the (offset, scale) pairs.
+  auto load_raw = [&](const Unit& x, int buf) {
+    const uint8_t* k = base + (x.page >> 2) * grain + sub * page_sub(x.bits);
+    const uint32_t to = raw0 + buf * RAW_BYTES, kv = H * page_sub(x.bits);  // (a page's V lies that far behind its K)
+    if (x.bits == 8 || (wave & 3) < 2)
+      load_piece_at(k + (wave < 4 ? 0 : kv) + 1024 * (wave & 3), 16 * lane, to + (wave < 4 ? 0 : RAW_V) + 1024 * (wave & 3));
+    if (wave == (x.bits == 8 ? 0 : 2)) load_piece_at(k, TILE * 8 * x.bits + 16 * (lane & 31) + (lane < 32 ? 0 : kv), to + RAW_SCALES);
+  };
+  auto unpack = [&](const Unit& x, int raw_buf, int buf) {
+    const uint8_t* from = packed_rows[raw_buf];
+    const float2 ka = reinterpret_cast<const float2*>(from + RAW_SCALES)[srow], va = reinterpret_cast<const float2*>(from + RAW_SCALES)[TILE + srow];
+    uint2 k, v;
+    if (x.bits == 4) {
+      k.x = *reinterpret_cast<const uint32_t*>(from + srow * 32 + 4 * piece);
+      v.x = *reinterpret_cast<const uint32_t*>(from + RAW_V + srow * 32 + 4 * piece);
+    } else {
+      k = *reinterpret_cast<const uint2*>(from + srow * 64 + 8 * piece);
+      v = *reinterpret_cast<const uint2*>(from + RAW_V + srow * 64 + 8 * piece);
+    }
+    const bool there = srow < x.rows;  // (rows that are not there: zeros, which meet a p of zero)
+    const u32x4 ku = unpack8<PREC>(x.bits, k, ka), vu = unpack8<PREC>(x.bits, v, va);
+    *reinterpret_cast<u32x4*>(&tiles[buf][0][16 * t]) = there ? ku : u32x4{0, 0, 0, 0};
+    *reinterpret_cast<u32x4*>(&tiles[buf][1][16 * t]) = there ? vu : u32x4{0, 0, 0, 0};
     if (PREC && (t & 7) == 0) {
-      const float centre = s.bits == 4 ? CENTRE<4> : CENTRE<8>;
-      const bool scaled = there && s.bits < 16;
-      scales[buf][0][srow] = scaled ? make_float2(__builtin_fmaf(r.ka.y, centre, r.ka.x), r.ka.y) : make_float2(0.f, 1.f);
-      scales[buf][1][srow] = scaled ? make_float2(__builtin_fmaf(r.va.y, centre, r.va.x), r.va.y) : make_float2(0.f, there ? 1.f : 0.f);
+      const float centre = x.bits == 4 ? CENTRE<4> : CENTRE<8>;
+      scales[buf][0][srow] = there ? make_float2(__builtin_fmaf(ka.y, centre, ka.x), ka.y) : make_float2(0.f, 0.f);
+      scales[buf][1][srow] = there ? make_float2(__builtin_fmaf(va.y, centre, va.x), va.y) : make_float2(0.f, 0.f);
     }
   };
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)&tiles[0][0][0];
-  auto load_new = [&](int u, int buf) {  // 64 new tokens, all there
-    const int tok = w.token0 + (u - w.n_pages) * TILE + srow;
-    const uint32_t to = lds0 + buf * (2 * TILE_BYTES) + 1024 * wave;
-    load_piece(static_cast<const uint16_t*>(a.k_new) + h * a.kn_head_stride + tok * a.kn_tok_stride + 8 * piece, to);
-    load_piece(static_cast<const uint16_t*>(a.v_new) + h * a.vn_head_stride + tok * a.vn_tok_stride + 8 * piece, to + TILE_BYTES);
+  // Values of a tile that would make NaN of a weight of zero become zeros: of rows that are not there, and infinite or NaN
+  // ones of new rows (added after all units). Each thread looks at its own 16 bytes.
+  auto zero_values = [&](const Unit& x, uint8_t* vt, bool fresh) {
+    u32x4* at = reinterpret_cast<u32x4*>(vt + 16 * t);
+    const bool there = srow < x.rows;
+    u32x4 y = *at;
+    bool changed = !there;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t keep = !there ? 0u : !fresh ? 0xffffffffu : (bad_bf16(y[e]) ? 0u : 0xffffu) | (bad_bf16(y[e] >> 16) ? 0u : 0xffff0000u);
+      changed = changed || keep != 0xffffffffu;
+      y[e] &= keep;
+    }
+    if (changed) *at = y;
+    if (changed && there) bad = 1;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
   };
 
   Op8 q[4];
@@ -161,28 +191,14 @@ __global__ __launch_bounds__(64 * WAVES, PREC ? 2 : 4) void long_kernel(dkv_page
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) q[ks].u = *reinterpret_cast<const u32x4*>(src + 16 * ks);
   }
-  Raw raw;
-  Source ahead{};  // the unit in `raw`
   if (t == 0) bad = 0;
-  __syncthreads();
-  // the first unit to LDS, the second on its way
-  if (w.u0 < w.u1) {
-    if (straight(w.u0)) {
-      load_new(w.u0, 0);
-    } else {
-      ahead = source(w.u0);
-      load_raw(ahead, raw);
-      write_raw(ahead, raw, 0);
-    }
-    if (w.u0 + 1 < w.u1) {
-      if (straight(w.u0 + 1)) {
-        load_new(w.u0 + 1, 1);
-      } else {
-        ahead = source(w.u0 + 1);
-        load_raw(ahead, raw);
-      }
-    }
-  }
+  // Units u, u + 1, u + 2 and u + 3. Packed ones are asked for three units ahead, unpacked one ahead; the others two ahead.
+  Unit x0 = unit_at(w.u0), x1 = unit_at(w.u0 + 1), x2 = unit_at(w.u0 + 2), x3 = unit_at(w.u0 + 3);
+  if (x0.bits < 16) load_raw(x0, 0);
+  else if (x0.rows) load_tile(w.u0, x0, 0);
+  if (x1.bits < 16) load_raw(x1, 1);
+  else if (x1.rows) load_tile(w.u0 + 1, x1, 1);
+  if (x2.bits < 16) load_raw(x2, 2);
   float q_sum = 0.f;  // of the query row's elements
   if (PREC) {
 #pragma unroll
@@ -199,123 +215,145 @@ __global__ __launch_bounds__(64 * WAVES, PREC ? 2 : 4) void long_kernel(dkv_page
   const float xs = a.scale * LOG2E;
   // This lane's LDS places: pieces of key c for the K operands, and the 4 elements it reads for the V^T operands.
   // (Piece 2 ks + half of a row lies 32 ks further on but for the carry, the same bits in the other order: ^.)
-  const uint32_t k_at = c * 128 + ((half ^ (c & 7)) << 4);
+  const uint32_t k_at = c * 128 + ((half ^ place(c)) << 4);
   uint32_t v_at;
   {
     const int i = lane & 15, vr = 4 * half + (i >> 2), sub = (lane >> 4) & 1;
-    v_at = vr * 128 + (((2 * sub + ((i & 3) >> 1)) ^ (vr & 7)) << 4) + 8 * (i & 1);
+    v_at = vr * 128 + (((2 * sub + ((i & 3) >> 1)) ^ place(vr)) << 4) + 8 * (i & 1);
   }
+  // (The query operands have arrived: a wait for them inside the loop would drain the loads under way in every iteration.)
+  asm volatile("" ::"v"(q[0].u), "v"(q[1].u), "v"(q[2].u), "v"(q[3].u));
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
   __builtin_amdgcn_s_barrier();
-
-  int buf = 0;
-  for (int u = w.u0; u < w.u1; ++u) {
-    const int next = buf + 1 == RING ? 0 : buf + 1, after = next + 1 == RING ? 0 : next + 1;
-    int rows_here = TILE;
-    if (u < w.n_pages) rows_here = page(u).rows;
-    const bool packed = PREC && u < w.n_pages;
-    if (u + 1 < w.u1 && !straight(u + 1)) write_raw(ahead, raw, next);
-    bool direct = false;  // rows were asked for straight to LDS in this iteration
-    if (u + 2 < w.u1) {
-      if (straight(u + 2)) {
-        load_new(u + 2, after);
-        direct = true;
-      } else {
-        ahead = source(u + 2);
-        load_raw(ahead, raw);
-      }
-    }
-    const int first = (u - w.n_pages) * TILE;
-    if (on && (u < w.n_pages || first <= m_last)) {
-      const uint8_t* kt = &tiles[buf][0][0];
-      const uint8_t* vt = &tiles[buf][1][0];
-      const int high = u < w.n_pages ? rows_here : m + 1 - first;  // keys below are visible to this lane's row
-      const bool masked = u < w.n_pages ? rows_here < TILE : first + TILE - 1 > m_first;
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {  // 32 keys at a time
-        f32x16 s;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = 0.f;
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-          Op8 k;
-          k.u = *reinterpret_cast<const u32x4*>(kt + (k_at ^ (32 * ks)) + 4096 * kb);
-          s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k.v, q[ks].v, s, 0, 0, 0);
-        }
-        // max3 below is a statement of its own, before which the compiler does not wait for a matrix product's result: 19
-        // states after one of 16 passes.
-        asm volatile("s_nop 15\n s_nop 7" : "+v"(s));
-        if (packed) {
-#pragma unroll
-          for (int i = 0; i < 16; i += 2) {
-            const f32x4 as = *reinterpret_cast<const f32x4*>(&scales[buf][0][32 * kb + 8 * (i / 4) + 4 * half + i % 4]);
-            s[i] = __builtin_fmaf(as[1], s[i], as[0] * q_sum);
-            s[i + 1] = __builtin_fmaf(as[3], s[i + 1], as[2] * q_sum);
-          }
-        }
-        if (masked)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s[i] = 32 * kb + 8 * (i / 4) + 4 * half + i % 4 < high ? s[i] : -INFINITY;
-        float top = max3(s[0], s[1], s[2]);
-#pragma unroll
-        for (int i = 3; i < 15; i += 2) top = max3(top, s[i], s[i + 1]);
-        top = max_nn(top, s[15]);
-        // The running maximum moves when some lane's scores pass it; only then do a row's two lanes exchange theirs.
-        if (__builtin_amdgcn_ballot_w64(top * xs > m_run)) {
-          const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-          const float mnew = max_nn(m_run, max_nn(__uint_as_float(x[0]), __uint_as_float(x[1])) * xs);
-          const float alpha = mnew == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - mnew);
-          m_run = mnew;
-          l_part *= alpha;
-          if (PREC) offset *= alpha;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) acc[0][i] *= alpha, acc[1][i] *= alpha;
-        }
-        const float mref = m_run == -INFINITY ? 0.f : m_run;
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], xs, -mref));
-          sum += s[i];
-        }
-        l_part += sum;
-#pragma unroll
-        for (int st = 0; st < 2; ++st) {  // 16 keys
-          Op8 p[TERMS];
-#pragma unroll
-          for (int j = 0; j < 8; j += 2) {
-            float p0 = s[8 * st + j], p1 = s[8 * st + j + 1];
-            if (packed) {
-              const f32x4 as = *reinterpret_cast<const f32x4*>(&scales[buf][1][32 * kb + 16 * st + 8 * (j / 4) + 4 * half + j % 4]);
-              offset = __builtin_fmaf(p0, as[0], offset);
-              offset = __builtin_fmaf(p1, as[2], offset);
-              p0 *= as[1], p1 *= as[3];
-            }
-            uint32_t x[TERMS];
-            split_pair<TERMS>(p0, p1, x);
-#pragma unroll
-            for (int k = 0; k < TERMS; ++k) p[k].u[j / 2] = x[k];
-          }
-#pragma unroll
-          for (int db = 0; db < 2; ++db) {
-            Op8 v;
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-              v.h[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                  (__attribute__((address_space(3))) s16x4*)(vt + (v_at ^ (64 * db)) + (32 * kb + 16 * st + 8 * j) * 128));
-#pragma unroll
-            for (int k = TERMS - 1; k >= 0; --k) acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v.v, p[k].v, acc[db], 0, 0, 0);
-          }
-        }
-      }
-    }
-    // The next unit has landed (its direct loads were issued an iteration ago: at most this one's two are under way)
-    // and is written, by every wave, and no wave reads this one any more.
-    if (direct) asm volatile("s_waitcnt vmcnt(2)" ::: "memory");
-    else if (straight(u + 1)) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  asm volatile("" ::: "memory");
+  if (x0.bits < 16) {
+    unpack(x0, 0, 0);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
+  }
+
+  // A unit's keys from its tiles. packed: their scales and offsets are to come (PREC 1). Keys from `high` on are not visible
+  // to this lane's row, none from 32 on to any row of the wave where there is one half.
+  auto attend = [&](int buf, bool packed, bool masked, int high, bool one_half) {
+    const uint8_t* kt = &tiles[buf][0][0];
+    const uint8_t* vt = &tiles[buf][1][0];
+    f32x16 s[2];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[kb][i] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        Op8 k;
+        k.u = *reinterpret_cast<const u32x4*>(kt + (k_at ^ (32 * ks)) + 4096 * kb);
+        s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k.v, q[ks].v, s[kb], 0, 0, 0);
+      }
+    // max3 below is a statement of its own, before which the compiler does not wait for a matrix product's result: 19
+    // states after one of 16 passes.
+    asm volatile("s_nop 15\n s_nop 7" : "+v"(s[0]), "+v"(s[1]));
+    if (packed) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          const f32x4 as = *reinterpret_cast<const f32x4*>(&scales[buf][0][32 * kb + 8 * (i / 4) + 4 * half + i % 4]);
+          s[kb][i] = __builtin_fmaf(as[1], s[kb][i], as[0] * q_sum);
+          s[kb][i + 1] = __builtin_fmaf(as[3], s[kb][i + 1], as[2] * q_sum);
+        }
+    }
+    if (masked)
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[kb][i] = 32 * kb + 8 * (i / 4) + 4 * half + i % 4 < high ? s[kb][i] : -INFINITY;
+    float top = max3(s[0][0], s[0][1], s[0][2]), top1 = max3(s[1][0], s[1][1], s[1][2]);
+#pragma unroll
+    for (int i = 3; i < 15; i += 2) top = max3(top, s[0][i], s[0][i + 1]), top1 = max3(top1, s[1][i], s[1][i + 1]);
+    top = max_nn(max3(top, s[0][15], s[1][15]), top1);
+    // The running maximum moves when some lane's scores pass it; only then do a row's two lanes exchange theirs.
+    if (__builtin_amdgcn_ballot_w64(top * xs > m_run)) {
+      const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+      const float mnew = max_nn(m_run, max_nn(__uint_as_float(x[0]), __uint_as_float(x[1])) * xs);
+      const float alpha = mnew == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - mnew);
+      m_run = mnew;
+      l_part *= alpha;
+      if (PREC) offset *= alpha;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[0][i] *= alpha, acc[1][i] *= alpha;
+    }
+    const float mref = m_run == -INFINITY ? 0.f : m_run;
+    float sum = 0.f;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      if (kb == 1 && one_half) break;
+#pragma unroll
+      for (int st = 0; st < 2; ++st) {  // 16 keys
+        Op8 p[TERMS];
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+          float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][8 * st + j], xs, -mref));
+          float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][8 * st + j + 1], xs, -mref));
+          if (TERMS > 1) sum += p0 + p1;
+          if (packed) {
+            const f32x4 as = *reinterpret_cast<const f32x4*>(&scales[buf][1][32 * kb + 16 * st + 8 * (j / 4) + 4 * half + j % 4]);
+            offset = __builtin_fmaf(p0, as[0], offset);
+            offset = __builtin_fmaf(p1, as[2], offset);
+            p0 *= as[1], p1 *= as[3];
+          }
+          uint32_t x[TERMS];
+          split_pair<TERMS>(p0, p1, x);
+#pragma unroll
+          for (int k = 0; k < TERMS; ++k) p[k].u[j / 2] = x[k];
+          // (Weights of one bf16 value are summed as they are multiplied.)
+          if (TERMS == 1) sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, x[0]), __builtin_bit_cast(bf16x2, 0x3f803f80u), sum, false);
+        }
+#pragma unroll
+        for (int db = 0; db < 2; ++db) {
+          Op8 v;
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            v.h[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (__attribute__((address_space(3))) s16x4*)(vt + (v_at ^ (64 * db) ^ (32 * j)) + (32 * kb + 16 * st + 8 * j) * 128));
+#pragma unroll
+          for (int k = TERMS - 1; k >= 0; --k) acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v.v, p[k].v, acc[db], 0, 0, 0);
+        }
+      }
+    }
+    l_part += sum;
+  };
+  // What was asked for before this iteration has landed (this wave's part; the barrier: every wave's), the next unit is
+  // unpacked, and no wave reads this one any more.
+  auto step = [&](int asked) {
+    wait_loads(asked);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  int buf = 0, u = w.u0;
+  for (; u < min(w.u1, w.n_pages); ++u) {
+    const int next = buf + 1 == RING ? 0 : buf + 1, after = next + 1 == RING ? 0 : next + 1;
+    int asked = 0;  // loads of this wave in this iteration
+    if (x3.bits < 16) load_raw(x3, buf), asked = x3.loads;  // (unit u's packed rows were unpacked in the iteration before)
+    if (x2.bits == 16 && x2.rows) load_tile(u + 2, x2, after), asked += x2.loads;
+    if (x1.bits < 16) unpack(x1, next, next);
+    const Unit x4 = unit_at(u + 4);
+    if (x0.rows < TILE && x0.bits == 16) zero_values(x0, tiles[buf][1], false);
+    if (on) attend(buf, PREC && x0.bits < 16, x0.rows < TILE, x0.rows, x0.rows <= 32);
+    step(asked);
+    x0 = x1, x1 = x2, x2 = x3, x3 = x4;
+    buf = next;
+  }
+  for (; u < w.u1; ++u) {  // new tokens: nothing to be unpacked
+    const int next = buf + 1 == RING ? 0 : buf + 1, after = next + 1 == RING ? 0 : next + 1;
+    const int first = (u - w.n_pages) * TILE;
+    const bool more = u + 2 < w.u1;
+    if (more) load_tile(u + 2, Unit{16, min(TILE, w.count - first - 2 * TILE), 2, 0}, after);
+    if (first + TILE - 1 > first_token) zero_values(Unit{16, min(TILE, w.count - first), 0, 0}, tiles[buf][1], true);
+    if (on && first <= m_last) attend(buf, false, first + TILE - 1 > m_first, m + 1 - first, m_last - first < 32);
+    step(more ? 2 : 0);
     buf = next;
   }
   if (!on) return;
@@ -325,8 +363,9 @@ __global__ __launch_bounds__(64 * WAVES, PREC ? 2 : 4) void long_kernel(dkv_page
   };
   const float l = both(l_part), off = PREC ? both(offset) : 0.f;
   if (bad) {  // (rare) new values that the products took for zero, with their weights computed again
-    for (int u = max(w.u0, seen_by_all); u < w.u1; ++u) {
+    for (int u = max(w.u0, w.n_pages); u < w.u1; ++u) {
       const int first = (u - w.n_pages) * TILE;
+      if (first + TILE - 1 <= first_token) continue;
       for (int j = 0; j < min(TILE, w.count - first); ++j) {
         const int64_t tok = w.token0 + first + j;
         const uint2* v = reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(a.v_new) + h * a.vn_head_stride + tok * a.vn_tok_stride);

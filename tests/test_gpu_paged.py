@@ -5,7 +5,7 @@ the attention: a query's weights are off by a relative e, its output by at most 
 (numerator and denominator), and by its own rounding (bf16 2^-8, fp32 2^-24). e: the score's products are exact and
 their sums of 64 terms, with the scaling, are off by at most 66 roundings of 2^-24 of sum |q k| / 8, which enters the
 exponent; exp2 and the sums of weights and products add 2^-20 at the lengths here; weights are kept in 16 bits (bf16
-output) or 24 (fp32): 2^-16 and 2^-24, or, where a KV head has more than 48 query rows (tokens times query heads of a
+output) or 24 (fp32): 2^-16 and 2^-24, or, where a KV head has more than 160 query rows (tokens times query heads of a
 sequence, or of branches over the pages that they share) at precision and output bf16, in one bf16 value: 2^-8.
 """
 import math
@@ -81,7 +81,7 @@ class Model:
                 later = torch.arange(hist + n)[None] > hist + torch.arange(n)[:, None]
                 p = torch.softmax(scores.masked_fill(later, -math.inf), -1)
                 size = (torch.matmul(x.abs(), keys.abs().t()) / 8).masked_fill(later, 0).amax(-1, keepdim=True)
-                e = 66 * 2 ** -24 * size + 2 ** -20 + (2 ** -24 if fp32 else 2 ** -8 if one and (n * G > 48 or s in long) else 2 ** -16)
+                e = 66 * 2 ** -24 * size + 2 ** -20 + (2 ** -24 if fp32 else 2 ** -8 if one and (n * G > 160 or s in long) else 2 ** -16)
                 ref = torch.matmul(p, values)
                 tol = 2 * e * torch.matmul(p, values.abs()) + (2 ** -24 if fp32 else 2 ** -8) * ref.abs() + 1e-30
                 got = out[at:at + n, h * G:(h + 1) * G].transpose(0, 1).double()
