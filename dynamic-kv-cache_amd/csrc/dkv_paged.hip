@@ -323,7 +323,7 @@ static int64_t long_share(const std::vector<Entity>& es, int G, int heads, int g
   int64_t most = 0, best = least;
   for (const Entity& e : es)
     if (is_long((int64_t)e.count * G)) most = std::max<int64_t>(most, units_of(e, G, LONG_BLOCK, ceil_div((int64_t)e.count * G, LONG_BLOCK) - 1));
-  constexpr float START = 2.5f, PARTIAL = 2.f, JOIN = 3e-5f;  // of a workgroup; of its 256 rows; of a partial row and head
+  constexpr float START = 1.f, PARTIAL = 2.f, JOIN = 3e-5f;  // of a workgroup; of its 256 rows; of a partial row and head
   float best_time = 0.f;
   std::vector<float> costs, ends;
   for (int64_t len = least;; len += std::max<int64_t>(1, len / 4)) {

@@ -293,6 +293,17 @@ int dkv_pool_sequence(dkv_pool* pool, int64_t seq, int64_t* length, int64_t* dro
   });
 }
 
+int64_t dkv_pool_length(dkv_pool* pool, int64_t seq) {
+  int64_t length = -1;
+  guarded(pool, "dkv_pool_length", [&](dkv_pool& p) {
+    const Sequence* s = p.find(seq, "dkv_pool_length");
+    if (!s) return DKV_EINVAL;
+    length = s->length;
+    return 0;
+  });
+  return length;
+}
+
 int dkv_pool_pages(dkv_pool* pool, int64_t seq, int32_t room, uint32_t* page, int32_t* rows, int32_t* holders) {
   return guarded(pool, "dkv_pool_pages", [&](dkv_pool& p) {
     const Sequence* s = p.find(seq, "dkv_pool_pages");

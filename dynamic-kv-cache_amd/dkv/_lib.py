@@ -233,6 +233,7 @@ SIGNATURES = [
     ('dkv_pool_info_get', ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(PoolInfo)]),
     ('dkv_pool_generation', ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
     ('dkv_pool_tokens', ctypes.c_int64, [ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p]),
+    ('dkv_pool_length', ctypes.c_int64, [ctypes.c_void_p, ctypes.c_int64]),
     ('dkv_pool_sequence', ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
     ('dkv_pool_pages', ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p,
                                       ctypes.c_void_p]),

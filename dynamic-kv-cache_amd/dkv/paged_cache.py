@@ -106,7 +106,7 @@ class PagedCache:
         return x
 
     def _sequence(self, seq):
-        (seq,), _ = self._ids(seq)
+        (seq,), _ = self._ids([seq])
         out = (ctypes.c_int64 * 3)()
         at = ctypes.addressof(out)
         rc = _lib.load().dkv_pool_sequence(self._pool, seq, at, at + 8, at + 16)
@@ -122,7 +122,12 @@ class PagedCache:
 
     def length(self, seq):
         """Tokens that a sequence holds, those of steps that were planned among them."""
-        return self._sequence(seq)[0]
+        if not isinstance(seq, (int, np.integer)) or not 0 <= seq < 1 << 62:
+            self._ids([seq])
+        n = _lib.load().dkv_pool_length(self._pool, seq)
+        if n < 0:
+            _lib.check(_lib.DKV_EINVAL, 'dkv_pool_length')
+        return n
 
     def position(self, seq):
         """Position of a sequence's next token: its length and what an evicted GPUCache that it was adopted from had
@@ -158,7 +163,7 @@ class PagedCache:
     def fork(self, seq, n=1):
         """n new sequences that go on from this one. They share its pages but a last one that is not full, of which
         each gets a copy."""
-        (seq,), _ = self._ids(seq)
+        (seq,), _ = self._ids([seq])
         if not 0 <= n <= 1 << 20:
             raise ValueError(f'fork: cannot make {n} branches')
         self._not_captured('fork')
@@ -174,7 +179,7 @@ class PagedCache:
 
     def truncate(self, seq, length):
         """Drops a sequence's tokens from `length` on."""
-        (seq,), _ = self._ids(seq)
+        (seq,), _ = self._ids([seq])
         if not 0 <= length < 1 << 62:
             raise ValueError(f'truncate: a sequence cannot hold {length} tokens')
         self._not_captured('truncate')

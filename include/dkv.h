@@ -616,8 +616,9 @@ int dkv_pool_destroy(dkv_pool* pool);
 int dkv_pool_info_get(dkv_pool* pool, dkv_pool_info* info);
 /* Where the pool keeps its generation, for as long as it lives. */
 int dkv_pool_generation(dkv_pool* pool, const int64_t** at);
-/* A sequence's tokens, tokens dropped before them (its next position is their sum) and pages; the pages' names, tokens
+/* A sequence's tokens (-1 for an error); these, tokens dropped before them (its next position is their sum) and pages; the pages' names, tokens
  * and numbers of sequences that hold them, into arrays with room for `room`. */
+int64_t dkv_pool_length(dkv_pool* pool, int64_t seq);
 int dkv_pool_sequence(dkv_pool* pool, int64_t seq, int64_t* length, int64_t* dropped, int32_t* pages);
 int dkv_pool_pages(dkv_pool* pool, int64_t seq, int32_t room, uint32_t* page, int32_t* rows, int32_t* holders);
 /* A new sequence without tokens; with the `tokens` of a cache's tiles (a HOST table, its arena `src`), copied as they
