@@ -1594,17 +1594,20 @@ def attend_projection(module, cache, qkv, position_embeddings):
 
 
 def install_packed_attention(model):
-    """Routes LlamaAttention through the packed cache when given a GPUCache (src/gpu_cache.py:151-183).
+    """Routes LlamaAttention through the packed cache when given a GPUCache (src/gpu_cache.py:151-183) or a step of a
+    PagedCache.
 
     All other caches keep the upstream forward. Accepts both the `past_key_value` keyword of
     transformers 4.x and the `past_key_values` keyword of 5.x.
     """
     from transformers.models.llama.modeling_llama import apply_rotary_pos_emb
 
+    from .paged_cache import PagedStep
+
     def forward(module, hidden_states, position_embeddings=None, attention_mask=None, past_key_value=None,
                 cache_position=None, **kwargs):
         cache = past_key_value if past_key_value is not None else kwargs.get('past_key_values')
-        fused = isinstance(cache, GPUCache) and cache.backend == 'fused'
+        fused = isinstance(cache, (GPUCache, PagedStep)) and cache.backend == 'fused'
         fast_gqa = getattr(cache, 'fast_gqa', False)
         if not fused and not fast_gqa:
             if past_key_value is not None:

@@ -408,16 +408,18 @@ def _fused_layer_eager(p, tiles, h, n, cache, cos, sin):
 
 
 def fused_decoder_layer(layer, hidden_states, cache, position_embeddings):
-    """One LlamaDecoderLayer forward on a packed GPUCache; None when the layer, the inputs or the cache
+    """One LlamaDecoderLayer forward on a packed GPUCache or a step of a PagedCache; None when the layer, the inputs or the cache
     are outside what the kernels cover. Launches beside the attention's (one to three): four, up to six
     where the norms run apart (many rows), one more in graph steps of so many rows that the norm before
     Q/K/V is apart, which rotate and pack in a launch of their own. What depends only on the layer and
     the chunk length is checked once (_layer_plan); eager launches on contiguous inputs then take
     _fused_layer_eager, and graph captures the general path below."""
     from .gpu_cache import GPUCache, attend_projection
+    from .paged_cache import PagedStep
     attn, mlp = layer._modules['self_attn'], layer._modules['mlp']
     h = hidden_states
-    if not (isinstance(cache, GPUCache) and cache.backend == 'fused' and position_embeddings is not None
+    single = isinstance(cache, GPUCache)
+    if not ((single or isinstance(cache, PagedStep)) and cache.backend == 'fused' and position_embeddings is not None
             and hasattr(attn, '_qkv_weight') and hasattr(mlp, '_gate_up_weight') and h.dim() == 3
             and h.shape[0] == 1 and _fused(h)):
         return None
@@ -426,7 +428,7 @@ def fused_decoder_layer(layer, hidden_states, cache, position_embeddings):
     if p is None:
         return None
     tiles = _layer_tiles(layer, p)
-    if (p.eager_ok and p.kv_heads == cache.heads and cache._graph is None and cache.chunk_segments is None
+    if (single and p.eager_ok and p.kv_heads == cache.heads and cache._graph is None and cache.chunk_segments is None
             and not cache.sparse_blocks and not cache.observing):
         cos, sin = position_embeddings
         if (h.is_contiguous() and h.data_ptr() % 16 == 0 and cos.shape == (1, n, 64) and sin.shape == cos.shape
@@ -438,7 +440,7 @@ def fused_decoder_layer(layer, hidden_states, cache, position_embeddings):
     x = h.reshape(n, width)
     qt, ot, gt, dt = tiles if tiles is not None else (None,) * 4
     packed = None
-    if p.eager_ok and not p.norm1_apart and p.kv_heads == cache.heads and cache._graph is not None:
+    if single and p.eager_ok and not p.norm1_apart and p.kv_heads == cache.heads and cache._graph is not None:
         cos, sin = position_embeddings
         if (x.stride(-1) == 1 and x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0 and cos.shape == (1, n, 64)
                 and sin.shape == cos.shape and all(t.is_cuda and t.dtype == torch.bfloat16 and t.stride(-1) == 1

@@ -11,6 +11,8 @@ place of the vision encoder:
   frames' attention and evicts the tokens that got least of it, so a stream has no end.
 - generate(): tokens drawn one after the other on a fork from given random numbers, each
   attending to all of the history or to the part of it that scores highest for it.
+- generate_batch(): the same for many questions at once, about one stream or several, on branches in
+  the shared pages of a PagedCache: a forward of all questions, then one forward a token for all.
 - answer(): the reference's 'candidate' protocol (src/streaming.py:209-225).
   For each candidate, a fork of the cache runs question + candidate tokens, and
   the score is the mean log-likelihood of the candidate tokens. answer_labels()
@@ -28,6 +30,7 @@ import torch
 
 from .gpu_cache import GPUCache, install_packed_attention
 from .gpu_ops import install_fused_ops, sample
+from .paged_cache import PagedCache
 
 MFMA_ROWS = 192  # query rows per frame-chunk attention workgroup (MFMA_ROWS of csrc/dkv_attn_common.h)
 
@@ -96,6 +99,12 @@ class StreamingDecoder:
         return GPUCache(None, layers=c.num_hidden_layers, heads=c.num_key_value_heads, dim=c.head_dim,
                         dtype=self.model.dtype, max_tokens=max_tokens, precision=self.precision,
                         device=self.device, **kw)
+
+    def create_paged_cache(self, max_tokens, **kw):
+        """A PagedCache of the decoder's shape, which adopts the histories that ingest() returned."""
+        c = self.config
+        return PagedCache(c.num_hidden_layers, c.num_key_value_heads, c.num_attention_heads, max_tokens=max_tokens,
+                          dim=c.head_dim, precision=self.precision, device=self.device, **kw)
 
     @staticmethod
     def _position(cache, past=None):
@@ -500,6 +509,65 @@ class StreamingDecoder:
             return u.new_empty(0, dtype=torch.int64)
         out = torch.cat(tokens)
         return out.masked_fill((out < 0).cumsum(0) > 0, -1)
+
+    def _paged_forward(self, step, ids, last):
+        """fp32 logits [sequences, vocabulary] of a step's tokens ids [1, tokens] at the places `last` of them."""
+        out = self.text(inputs_embeds=self.text.get_input_embeddings()(ids), past_key_values=step, use_cache=True,
+                        position_ids=step.positions[None], attention_mask=None, return_dict=True)
+        return self.model.lm_head(out.last_hidden_state[0, last]).float()
+
+    @torch.inference_mode()
+    def generate_batch(self, pages, seqs, questions, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        """Continues each question [1, n] (of any lengths) on a branch of its sequence of the PagedCache `pages` (one
+        of seqs each, or one for all; questions about one sequence attend to it together where they stand next to
+        each other): tokens int64 [questions, n] for the random numbers u [questions, n], each row as generate() draws
+        it. The branches take pages for a question and its tokens, and end with the call. With graphs=True the third
+        token's forward on is captured and replayed, and the call waits for the GPU."""
+        seqs, questions = [seqs] * len(questions) if isinstance(seqs, int) else list(seqs), list(questions)
+        if len(seqs) != len(questions) or u.dim() != 2 or u.shape[0] != len(questions):
+            raise ValueError(f'generate_batch expects a sequence and random numbers u [questions, n] for each question, got '
+                             f'{len(seqs)} and {list(u.shape)} for {len(questions)}')
+        if any(x.dim() != 2 or x.shape[0] != 1 or not x.shape[1] for x in questions):
+            raise ValueError('generate_batch expects questions of one token or more, [1, n]')
+        if not u.numel():
+            return u.new_empty(u.shape, dtype=torch.int64)
+        branches, tokens, graph = [], [], None
+        try:
+            i = 0
+            while i < len(seqs):  # branches of one sequence with one call
+                n = next((j for j in range(i, len(seqs)) if seqs[j] != seqs[i]), len(seqs)) - i
+                branches += pages.fork(seqs[i], n)
+                i += n
+            counts = [x.shape[1] for x in questions]
+            last = torch.tensor(counts).cumsum(0).sub(1).to(self.device)
+            ids = torch.cat([x.to(self.device) for x in questions], dim=1)
+            step = pages.step(branches, counts)
+            logits = self._paged_forward(step, ids, last)
+            n, last = u.shape[1], slice(None)
+            for i in range(n):
+                tokens.append(sample(logits, u[:, i], temperature, top_k, top_p, min_p))
+                if i + 1 == n:
+                    break
+                ids = tokens[-1][None].clamp(min=0)  # (-1 is no index into the embeddings)
+                step = step.advance() if i else pages.step(branches, reserve=n)
+                if graph is not None:
+                    held.copy_(ids)
+                    graph.replay()
+                elif not (self.graphs and i):  # (the first of these forwards warms the library paths that a capture records)
+                    logits = self._paged_forward(step, ids, last)
+                else:
+                    held, graph = ids.clone(), torch.cuda.CUDAGraph()
+                    torch.cuda.synchronize()
+                    with torch.cuda.graph(graph):
+                        logits = self._paged_forward(step, held, last)
+                    graph.replay()
+        finally:
+            if graph is not None:
+                torch.cuda.synchronize(self.device)  # (it may still run, and ends here)
+            if branches:
+                pages.free(branches)
+        out = torch.stack(tokens, dim=1)
+        return out.masked_fill((out < 0).cumsum(1) > 0, -1)
 
     @torch.inference_mode()
     def answer(self, cache, question_ids, candidates):
