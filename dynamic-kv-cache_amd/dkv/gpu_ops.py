@@ -413,7 +413,7 @@ def fused_decoder_layer(layer, hidden_states, cache, position_embeddings):
     where the norms run apart (many rows), one more in graph steps of so many rows that the norm before
     Q/K/V is apart, which rotate and pack in a launch of their own. What depends only on the layer and
     the chunk length is checked once (_layer_plan); eager launches on contiguous inputs then take
-    _fused_layer_eager, and graph captures the general path below."""
+    _fused_layer_eager (a PagedStep's captured ones too), and graph captures the general path below."""
     from .gpu_cache import GPUCache, attend_projection
     from .paged_cache import PagedStep
     attn, mlp = layer._modules['self_attn'], layer._modules['mlp']
@@ -428,8 +428,11 @@ def fused_decoder_layer(layer, hidden_states, cache, position_embeddings):
     if p is None:
         return None
     tiles = _layer_tiles(layer, p)
-    if (single and p.eager_ok and p.kv_heads == cache.heads and cache._graph is None and cache.chunk_segments is None
-            and not cache.sparse_blocks and not cache.observing):
+    if single:
+        direct = cache._graph is None and cache.chunk_segments is None and not cache.sparse_blocks and not cache.observing
+    else:
+        direct = h.get_device() == cache.cache._index
+    if direct and p.eager_ok and p.kv_heads == cache.heads:
         cos, sin = position_embeddings
         if (h.is_contiguous() and h.data_ptr() % 16 == 0 and cos.shape == (1, n, 64) and sin.shape == cos.shape
                 and cos.dtype == torch.bfloat16 and sin.dtype == torch.bfloat16 and cos.is_contiguous()

@@ -375,6 +375,30 @@ class PagedStep(_CacheBase):
     def append_projection(self, qkv, cos, sin, q_heads, layer):
         return None  # (no launch of its own: split and RoPE, then append())
 
+    def _fused_attention(self, n, q_heads, layer, project, cos, sin, cs_stride, qkv_out, out, stream):
+        """The joined Q/K/V projection, its split and RoPE, append() and attend() for the fused decoder layer's eager
+        launches, with the arguments and promises of GPUCache._fused_attention: the same bytes and outputs as the
+        general entry points', which cost more host time than the GPU spends on a token of each sequence."""
+        c, d = self.cache, self.cache.dim
+        if self.generation != c._generation.value:
+            raise ValueError('attend: pages were freed, cut or moved since this step was planned')
+        if n != self.tokens or q_heads != c.q_heads or layer >= c.layers:
+            raise ValueError(f'a step of {self.tokens} tokens and {c.q_heads} query heads in {c.layers} layers got {n} and {q_heads} in layer {layer}')
+        H, lib, bounds = c.heads, _lib.load(), self.captured()
+        x, x_stride, weight, w_stride, _, k, norm, eps, layout = project
+        width = (q_heads + 2 * H) * d
+        need = self.workspace_bytes(bounds)
+        ws = c.arena.new_empty(max(need, 2 * n * width))  # (the projection's rows are done with before the attention starts)
+        at, kp = ws.data_ptr(), qkv_out + q_heads * n * d * 2
+        vp, head = kp + H * n * d * 2, n * d
+        args = _ARGS.pack(qkv_out, head, d, kp, head, d, vp, head, d, c._arena_ptr, c.arena_bytes, self.device_plan(), self.plan_bytes,
+                          layer, bounds, d ** -0.5, out, q_heads * d, d, 0, PRECISIONS[c.precision], at if need else 0, need)
+        rc = (lib.dkv_linear_tiled(x, x_stride, weight, w_stride, n, width, k, norm, eps, 0, None, 0, at, width, layout, stream)
+              or lib.dkv_rope_qkv(at, width, cos, sin, cs_stride, n, q_heads, H, qkv_out, kp, vp, stream)
+              or lib.dkv_paged_append(args, stream) or lib.dkv_paged_attend(args, stream))
+        if rc:
+            _lib.check(rc, 'the launches of a fused decoder layer')
+
     def append(self, k, v, layer):
         self.cache.append(k, v, layer, self)
         return 0

@@ -32,6 +32,9 @@ from .gpu_cache import GPUCache, install_packed_attention
 from .gpu_ops import install_fused_ops, sample
 from .paged_cache import PagedCache
 
+# generate_batch() captures more tokens than these: a replayed forward of a token of each sequence takes 1.35 ms and an eager one,
+# which waits for the host, 1.74 (32 layers, 1 to 16 questions; at 64 both take 1.85), a capture 3 to 5 ms.
+GRAPH_TOKENS = 16
 MFMA_ROWS = 192  # query rows per frame-chunk attention workgroup (MFMA_ROWS of csrc/dkv_attn_common.h)
 
 
@@ -521,8 +524,9 @@ class StreamingDecoder:
         """Continues each question [1, n] (of any lengths) on a branch of its sequence of the PagedCache `pages` (one
         of seqs each, or one for all; questions about one sequence attend to it together where they stand next to
         each other): tokens int64 [questions, n] for the random numbers u [questions, n], each row as generate() draws
-        it. The branches take pages for a question and its tokens, and end with the call. With graphs=True the third
-        token's forward on is captured and replayed, and the call waits for the GPU."""
+        it. The branches take pages for a question and its tokens, and end with the call. With graphs=True the
+        forwards of more than GRAPH_TOKENS tokens are replays of a captured one from the third token's on, and the call
+        waits for the GPU."""
         seqs, questions = [seqs] * len(questions) if isinstance(seqs, int) else list(seqs), list(questions)
         if len(seqs) != len(questions) or u.dim() != 2 or u.shape[0] != len(questions):
             raise ValueError(f'generate_batch expects a sequence and random numbers u [questions, n] for each question, got '
@@ -553,7 +557,7 @@ class StreamingDecoder:
                 if graph is not None:
                     held.copy_(ids)
                     graph.replay()
-                elif not (self.graphs and i):  # (the first of these forwards warms the library paths that a capture records)
+                elif not (self.graphs and i and n > GRAPH_TOKENS):  # (the first of these forwards warms the library paths that a capture records)
                     logits = self._paged_forward(step, ids, last)
                 else:
                     held, graph = ids.clone(), torch.cuda.CUDAGraph()
