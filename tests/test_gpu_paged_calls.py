@@ -1,0 +1,249 @@
+"""PagedCache's calls on the GPU in other circumstances: captured and replayed steps, other streams, strides, types and threads,
+arenas and histories past 32 bits. Attention's bounds are those of test_gpu_paged."""
+import threading
+
+import pytest
+import torch
+
+from conftest import announce
+from dkv import PagedCache
+from test_gpu_paged import Model, rows_like
+
+pytestmark = pytest.mark.gpu
+
+
+def history(cache, layers, heads, gen):
+    """Four sequences of which two share 300 tokens, every layer packed."""
+    base, other, empty = cache.add(), cache.add(), cache.add()
+    for counts, bits in (([200, 64], [8, 4]), ([100, 33], [4, 16])):
+        step = cache.step([base, other], counts, bits)
+        for layer in range(layers):
+            cache.append(rows_like(gen, 1, heads, sum(counts)).cuda(), rows_like(gen, 1, heads, sum(counts)).cuda(), layer, step)
+    return [base, *cache.fork(base), other, empty]
+
+
+@pytest.mark.parametrize('counts', [1, [1, 3, 2, 1], [70, 9, 1, 130]])
+def test_replayed_steps_are_eager_ones(cuda, counts):
+    """Ten steps captured once and replayed after advance(), beside a second captured step over the same cache, with eager work
+    and waits between, against eager steps of an equal cache: the same bits."""
+    announce(f'replays {counts}')
+    layers, heads, q_heads = 2, 2, 6
+    caches, seqs = [], []
+    for _ in range(2):
+        caches.append(PagedCache(layers, heads, q_heads, max_tokens=1 << 14))
+        seqs.append(history(caches[-1], layers, heads, torch.Generator().manual_seed(3)))
+    mine, theirs = caches
+    gen = torch.Generator().manual_seed(4)
+    late = [mine.add(), theirs.add()]
+    step = mine.step(seqs[0], counts, [16, 8, 4, 16], reserve=3000)
+    second = mine.step(late[0], 5, 8, reserve=100)
+    n = step.tokens
+
+    def inputs(n):
+        return [rows_like(gen, 1, h, n).cuda() for h in (q_heads, heads, heads)]
+    q, k, v = inputs(n)
+    q2, k2, v2 = inputs(5)
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    outs = [[], []]
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graphs[0]):
+        for layer in range(layers):
+            mine.append(k, v, layer, step)
+            outs[0].append(mine.attend(q, k, v, layer, step))
+    with torch.cuda.graph(graphs[1]):
+        for layer in range(layers):
+            outs[1].append(mine.attend(q2, k2, v2, layer, second, out_dtype=torch.float32))
+            mine.append(k2, v2, layer, second)
+    for turn in range(10):
+        if turn:
+            step.advance()
+            second.advance()
+            for x, y in zip((q, k, v, q2, k2, v2), inputs(n) + inputs(5)):
+                x.copy_(y)
+        for g in graphs if turn % 2 else graphs[::-1]:
+            g.replay()
+        own = theirs.step(seqs[1], counts, [16, 8, 4, 16])
+        own2 = theirs.step(late[1], 5, 8)
+        assert torch.equal(own.positions, step.positions) and torch.equal(own2.positions, second.positions)
+        for layer in range(layers):
+            want = theirs.attend(q, k, v, layer, own)
+            want2 = theirs.attend(q2, k2, v2, layer, own2, out_dtype=torch.float32)
+            theirs.append(k, v, layer, own)
+            theirs.append(k2, v2, layer, own2)
+            assert torch.equal(outs[0][layer], want) and torch.equal(outs[1][layer], want2), (turn, layer)
+        if turn % 3 == 0:
+            torch.cuda.synchronize()
+            for layer in range(layers):
+                for a, b in zip(mine.materialize(layer, seqs[0] + late[:1]), theirs.materialize(layer, seqs[1] + late[1:])):
+                    assert torch.equal(a, b)
+
+
+def test_nothing_of_the_host_is_captured(cuda):
+    cache = PagedCache(1, 1, 1, max_tokens=1024)
+    seq = cache.add()
+    step = cache.step(seq, 4)
+    x = torch.zeros(1, 1, 4, 64, dtype=torch.bfloat16, device='cuda')
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        cache.append(x, x, 0, step)
+        for call in (lambda: cache.step(seq), step.advance, lambda: cache.fork(seq), lambda: cache.free(seq), lambda: cache.compact(),
+                     lambda: cache.truncate(seq, 0), lambda: cache.materialize(0, seq)):
+            with pytest.raises(ValueError, match='captured'):
+                call()
+    graph.replay()
+    assert cache.length(seq) == 4
+    cache.truncate(seq, 2)
+    with pytest.raises(ValueError, match='since this step was planned'):
+        cache.append(x, x, 0, step)
+    with pytest.raises(ValueError, match='since this step was planned'):
+        cache.attend(x, x, x, 0, step)
+
+
+def test_other_streams(cuda):
+    """Steps whose launches run on a stream of their own, which waits for the one before and which the next one waits for."""
+    announce('streams')
+    m = Model(2, 6, seed=9)
+    seqs = [m.add() for _ in range(3)]
+    side = torch.cuda.Stream()
+    for i in range(6):
+        stream = side if i % 2 else torch.cuda.current_stream()
+        stream.wait_stream(torch.cuda.current_stream() if i % 2 else side)
+        with torch.cuda.stream(stream):
+            m.attend(seqs, [1, 40, 120], (4, 8, 16)[i % 3])
+    torch.cuda.current_stream().wait_stream(side)
+    step, k, v = m.step(seqs, 1, 16)  # planned here, launched there
+    q = (torch.randn(6, 3, 64, generator=m.gen) * 0.5).bfloat16()
+    args = [x[None].cuda() for x in (q, k, v)]
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        out = m.cache.attend(*args, 0, step)
+    side.synchronize()
+    m.check(step, q, k, v, out[0].cpu())
+
+
+def test_strides_alignment_and_types(cuda):
+    """The same values as token-major rows, rows of a wider tensor, misaligned ones, fp32 and one row that all heads and tokens
+    share: the same bits."""
+    announce('strides')
+    heads, q_heads, counts = 2, 6, [1, 5, 100]
+    gen = torch.Generator().manual_seed(2)
+    n = sum(counts)
+    q, k, v = (rows_like(gen, 1, h, n).cuda() for h in (q_heads, heads, heads))
+
+    def wide(x, pad, at):
+        y = torch.full((*x.shape[:3], 64 + pad), float('nan'), dtype=x.dtype, device='cuda')
+        y[..., at:at + 64] = x
+        return y[..., at:at + 64]
+    forms = [lambda x: x, lambda x: x.transpose(1, 2).contiguous().transpose(1, 2), lambda x: wide(x, 64, 8), lambda x: wide(x, 64, 3),
+             lambda x: wide(x, 5, 2), lambda x: x.float(), lambda x: x.transpose(2, 3).contiguous().transpose(2, 3)]
+    outs = []
+    for form in forms:
+        cache = PagedCache(1, heads, q_heads, max_tokens=4096)
+        seqs = [cache.add() for _ in counts]
+        first = cache.step(seqs, counts, [4, 8, 16])
+        cache.append(form(k), form(v), 0, first)
+        step = cache.step(seqs, counts, 16)
+        out = cache.attend(form(q), form(k), form(v), 0, step, out_dtype=torch.bfloat16)
+        outs.append((out, *cache.materialize(0, seqs, first=0, out_dtype=torch.float32)))
+        cache.append(form(k), form(v), 0, step)
+    for other in outs[1:]:
+        assert torch.equal(other[0], outs[0][0])
+    cache = PagedCache(1, heads, q_heads, max_tokens=4096)
+    seqs = [cache.add() for _ in counts]
+    one = rows_like(gen, 1, 1, 1).cuda()
+    step = cache.step(seqs, counts, 8)
+    cache.append(one.expand(1, heads, n, 64), one.expand(1, heads, n, 64), 0, step)
+    same = one.expand(1, heads, n, 64).contiguous()
+    out = cache.attend(one.expand(1, q_heads, n, 64), one.expand(1, heads, n, 64), same, 0, step)
+    assert torch.equal(out, cache.attend(one.expand(1, q_heads, n, 64).contiguous(), same, same, 0, step))
+    got = cache.materialize(0, step, out_dtype=torch.float32)[0]
+    assert torch.equal(got, got[:, :1, :1].expand_as(got))
+
+
+def test_offsets_past_32_bits(cuda):
+    """An arena of 12 GiB: pages of 8 MiB whose last layer and head lie past 2^32 bytes from its start, read in short and long
+    steps, from branches, and moved."""
+    announce('12 GiB arena')
+    layers, heads, q_heads = 64, 8, 16
+    cache = PagedCache(layers, heads, q_heads, max_tokens=64 * 1440)
+    assert cache.arena_bytes > 11 << 30
+    m = Model(heads, q_heads, seed=4)
+    low, seq, between = cache.add(), cache.add(), cache.add()
+    cache.step(low, 64 * 900, 16)  # 7 GiB of pages in front
+    m.cache = _Last(cache, layers - 1)
+    m.k[seq] = m.v[seq] = torch.zeros(heads, 0, 64)
+    for n, bits in ((3000, 16), (500, 4), (700, 8)):
+        m.step([seq], [n], bits)
+    for _ in range(6):  # pages that leave gaps
+        m.step([seq], [64], 16)
+        cache.step(between, 128, 16)
+    assert min(p >> 2 for p, _, _ in cache.pages(seq)) * cache._info().grain > 7 << 30
+    m.attend([seq], 1)
+    m.attend([seq], 90)
+    branch = cache.fork(seq)[0]
+    m.k[branch], m.v[branch] = m.k[seq], m.v[seq]
+    m.attend([seq, branch], [3, 120], long=[seq, branch])
+    cache.free([low, between])
+    assert cache.compact() > 0
+    k, v = cache.materialize(layers - 1, [seq, branch], out_dtype=torch.float32)
+    for i, have in enumerate((m.k, m.v)):
+        assert torch.equal((k, v)[i][0].cpu(), torch.cat((have[seq], have[branch]), 1))
+    m.attend([branch, seq], 1)
+
+
+class _Last:
+    """A cache whose layer 0 is another one's `layer`."""
+
+    def __init__(self, cache, layer):
+        self.cache, self.layer = cache, layer
+        self.step = cache.step
+
+    def append(self, k, v, _, step):
+        self.cache.append(k, v, self.layer, step)
+
+    def attend(self, q, k, v, _, step, **kw):
+        return self.cache.attend(q, k, v, self.layer, step, **kw)
+
+
+def test_threads_of_one_process(cuda):
+    """Caches of two threads, each on a stream of its own: what each gives alone."""
+    announce('threads')
+
+    def work(seed, out):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            m = Model(2, 6, seed=seed)
+            seqs = [m.add() for _ in range(3)]
+            for i in range(15):
+                out.append(m.attend(seqs, [1, 2 + i, 60], (4, 8, 16)[i % 3]))
+            torch.cuda.current_stream().synchronize()
+    results = [[], []]
+    threads = [threading.Thread(target=work, args=(s, results[s])) for s in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert [len(r) for r in results] == [15, 15]
+
+
+def test_tokens_behind_the_last_sequence_stay(cuda):
+    """Outputs and pages beyond a step's tokens are left as they were."""
+    announce('rows behind')
+    cache = PagedCache(1, 1, 3, max_tokens=1024)
+    seqs = [cache.add(), cache.add()]
+    cache.arena.fill_(0xA5)
+    step = cache.step(seqs, [70, 3], 8)
+    x = torch.randn(1, 1, 73, 64, device='cuda').bfloat16()
+    cache.append(x, x, 0, step)
+    grain = cache._info().grain
+    page, rows = cache.pages(seqs[0])[1][:2]
+    at = (page >> 2) * grain
+    assert rows == 6
+    codes, scales = cache.arena[at:at + 4096].view(64, 64), cache.arena[at + 4096:at + 4608].view(64, 8)
+    assert (codes[6:] == 0xA5).all() and (scales[6:] == 0xA5).all()
+    held = {p >> 2 for s in seqs for p, _, _ in cache.pages(s)}
+    for block in range(cache.arena_bytes // grain // 48):
+        for slot in range(5):
+            g = 48 * block + 9 * slot
+            if g not in held:
+                assert (cache.arena[g * grain:(g + 9) * grain] == 0xA5).all()

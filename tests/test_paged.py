@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from dkv import GPUCache, PagedCache, _lib
+from test_long_history import test_struct_layout_matches_header as check_layout
 
 GRAINS, PER_BLOCK = {4: 5, 8: 9, 16: 16}, {4: 9, 8: 5, 16: 3}
 
@@ -43,6 +44,12 @@ def check(c, seqs):
 
 def rows(c, seq):
     return [r for _, r, _ in c.pages(seq)]
+
+
+@pytest.mark.parametrize('cls,cname', [(_lib.PagedBatch, 'dkv_paged_batch'), (_lib.PagedPlan, 'dkv_paged_plan'),
+                                       (_lib.PagedArgs, 'dkv_paged_args'), (_lib.PoolInfo, 'dkv_pool_info')])
+def test_struct_layout_matches_header(tmp_path, cls, cname):
+    check_layout(tmp_path, cls, cname)
 
 
 def test_geometry():
