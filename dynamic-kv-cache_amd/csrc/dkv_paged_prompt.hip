@@ -7,6 +7,8 @@
 // in the places that the second product reads P^T from: P never leaves its registers, and a row's maximum and sum take
 // one exchange between the two halves of a wave. V^T comes from V's rows in LDS by transposing reads (ds_read_b64_tr_b16:
 // of 16 lanes that read 4 elements of 4 rows each, lane i gets element i of the rows).
+#include <type_traits>
+
 #include "dkv_rows.h"
 #include "dkv_paged.h"
 
@@ -233,9 +235,11 @@ __global__ __launch_bounds__(64 * WAVES, PREC ? 2 : 4) void long_kernel(dkv_page
     asm volatile("" ::: "memory");
   }
 
-  // A unit's keys from its tiles. packed: their scales and offsets are to come (PREC 1). Keys from `high` on are not visible
+  // A unit's keys from its tiles. PACKED: their scales and offsets are to come (PREC 1; a constant, since a branch at every
+  // pair of keys waits for each of their reads). Keys from `high` on are not visible
   // to this lane's row, none from 32 on to any row of the wave where there is one half.
-  auto attend = [&](int buf, bool packed, bool masked, int high, bool one_half) {
+  auto attend = [&](auto packed_keys, int buf, bool masked, int high, bool one_half) {
+    constexpr bool PACKED = decltype(packed_keys)::value;
     const uint8_t* kt = &tiles[buf][0][0];
     const uint8_t* vt = &tiles[buf][1][0];
     f32x16 s[2];
@@ -256,7 +260,7 @@ __global__ __launch_bounds__(64 * WAVES, PREC ? 2 : 4) void long_kernel(dkv_page
     // max3 below is a statement of its own, before which the compiler does not wait for a matrix product's result: 19
     // states after one of 16 passes.
     asm volatile("s_nop 15\n s_nop 7" : "+v"(s[0]), "+v"(s[1]));
-    if (packed) {
+    if constexpr (PACKED) {
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -290,7 +294,7 @@ __global__ __launch_bounds__(64 * WAVES, PREC ? 2 : 4) void long_kernel(dkv_page
     float sum = 0.f;
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
-      if (kb == 1 && one_half) break;
+      if (TERMS > 1 && kb == 1 && one_half) break;  // (8 frames of 78 tokens, 3 terms: 102 us, 110 without; at 1 term 2 % slower)
 #pragma unroll
       for (int st = 0; st < 2; ++st) {  // 16 keys
         Op8 p[TERMS];
@@ -299,7 +303,7 @@ __global__ __launch_bounds__(64 * WAVES, PREC ? 2 : 4) void long_kernel(dkv_page
           float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][8 * st + j], xs, -mref));
           float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][8 * st + j + 1], xs, -mref));
           if (TERMS > 1) sum += p0 + p1;
-          if (packed) {
+          if constexpr (PACKED) {
             const f32x4 as = *reinterpret_cast<const f32x4*>(&scales[buf][1][32 * kb + 16 * st + 8 * (j / 4) + 4 * half + j % 4]);
             offset = __builtin_fmaf(p0, as[0], offset);
             offset = __builtin_fmaf(p1, as[2], offset);
@@ -343,7 +347,10 @@ __global__ __launch_bounds__(64 * WAVES, PREC ? 2 : 4) void long_kernel(dkv_page
     if (x1.bits < 16) unpack(x1, next, next);
     const Unit x4 = unit_at(u + 4);
     if (x0.rows < TILE && x0.bits == 16) zero_values(x0, tiles[buf][1], false);
-    if (on) attend(buf, PREC && x0.bits < 16, x0.rows < TILE, x0.rows, x0.rows <= 32);
+    if (on) {
+      if (PREC && x0.bits < 16) attend(std::integral_constant<bool, PREC == 1>(), buf, x0.rows < TILE, x0.rows, x0.rows <= 32);
+      else attend(std::false_type(), buf, x0.rows < TILE, x0.rows, x0.rows <= 32);
+    }
     step(asked);
     x0 = x1, x1 = x2, x2 = x3, x3 = x4;
     buf = next;
@@ -354,7 +361,7 @@ __global__ __launch_bounds__(64 * WAVES, PREC ? 2 : 4) void long_kernel(dkv_page
     const bool more = u + 2 < w.u1;
     if (more) load_tile(u + 2, Unit{16, min(TILE, w.count - first - 2 * TILE), 2, 0}, after);
     if (first + TILE - 1 > first_token) zero_values(Unit{16, min(TILE, w.count - first), 0, 0}, tiles[buf][1], true);
-    if (on && first <= m_last) attend(buf, false, first + TILE - 1 > m_first, m + 1 - first, m_last - first < 32);
+    if (on && first <= m_last) attend(std::false_type(), buf, first + TILE - 1 > m_first, m + 1 - first, m_last - first < 32);
     step(more ? 2 : 0);
     buf = next;
   }
