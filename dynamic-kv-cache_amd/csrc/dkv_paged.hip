@@ -270,6 +270,7 @@ static void layout_of(const dkv_paged_batch& b, dkv_paged_plan& p) {
     if (is_long(rows)) many += ceil_div(rows, LONG_BLOCK) + std::min<int64_t>(b.seqs / 2, rows / SHORT_ROWS);
   }
   p.seqs = b.seqs, p.tokens = (int)tokens, p.layers = b.layers, p.heads = b.heads, p.q_heads = b.q_heads;
+  p.grains = (int)std::min<int64_t>(std::max<int64_t>(b.arena_bytes, 0) / grain_bytes(b.layers, b.heads), 1 << 30);
   p.max_items = (int)items;
   p.max_pages = b.max_pages;
   p.max_work = few ? (int)(few + ceil_div(SHORT_TARGET, b.heads)) : 0;
@@ -287,10 +288,22 @@ static void layout_of(const dkv_paged_batch& b, dkv_paged_plan& p) {
   p.words = (int)at;
 }
 
-static bool plan_fits(const dkv_paged_batch& b) {  // (the offsets are 32-bit)
+// A batch whose plan's offsets fit into 32 bits, and its launches' threads.
+static int check_plan(const dkv_paged_batch& b, const char* what) {
+  if (int rc = check_batch(b, what)) return rc;
   int64_t tokens = 0;
   for (int i = 0; i < b.seqs; ++i) tokens += b.count[i];
-  return 64 * tokens * (b.q_heads / b.heads) + 64ll * b.seqs + 2ll * b.max_pages + (1 << 20) < INT32_MAX;
+  bool fits = 64 * tokens * (b.q_heads / b.heads) + 64ll * b.seqs + 2ll * b.max_pages + (1 << 20) < INT32_MAX;
+  if (fits) {
+    dkv_paged_plan p{};
+    layout_of(b, p);
+    const int64_t threads = std::max<int64_t>({p.max_items, (int64_t)p.max_work * b.heads, 2ll * p.max_long * b.heads,
+                                      (int64_t)p.max_merges * (SHORT_BLOCK / 4) * b.heads}) * 256;
+    fits = threads <= UINT32_MAX;
+  }
+  if (fits) return 0;
+  set_error("%s: %lld new tokens, %d query heads and %d pages are too many for one step", what, (long long)tokens, b.q_heads, b.max_pages);
+  return DKV_EINVAL;
 }
 
 // Units that a block of an entity's query rows sees: a group's pages, or a sequence's and its new tokens up to the
@@ -357,7 +370,6 @@ static int64_t long_share(const std::vector<Entity>& es, int G, int heads, int g
 static int write_plan(const dkv_paged_batch& b, int32_t* w, dkv_paged_plan& p) {
   const int G = b.q_heads / b.heads;
   layout_of(b, p);
-  const int64_t grain = grain_bytes(b.layers, b.heads), grains = b.arena_bytes / grain;
   dkv_page_rows* items = reinterpret_cast<dkv_page_rows*>(w + p.at_items);
   Page* pages = reinterpret_cast<Page*>(w + p.at_pages);
   std::vector<Entity> own(b.seqs);
@@ -374,7 +386,7 @@ static int write_plan(const dkv_paged_batch& b, int32_t* w, dkv_paged_plan& p) {
     const int64_t end = (int64_t)b.past[i] + b.count[i];
     for (int j = from; j < to; ++j) {
       const int code = b.page[j] & 3, rows = b.rows[j];
-      if (code > 2 || (int64_t)(b.page[j] >> 2) + page_grains(4 << code) > grains) {
+      if (code > 2 || (int64_t)(b.page[j] >> 2) + page_grains(4 << code) > p.grains) {
         set_error("dkv_paged_plan_write: page %u of sequence %d lies outside the arena", b.page[j], i);
         return DKV_EINVAL;
       }
@@ -488,6 +500,8 @@ int check_args(const dkv_paged_args& a, bool attend, const char* what) {
     set_error("%s: null pointer argument", what);
   } else if (p.seqs <= 0 || p.tokens <= 0 || p.heads <= 0 || p.q_heads <= 0 || p.q_heads % p.heads || a.layer < 0 || a.layer >= p.layers) {
     set_error("%s: not a plan (seqs %d, heads %d of %d), or layer %d of %d", what, p.seqs, p.heads, p.q_heads, a.layer, p.layers);
+  } else if (p.layers <= 0 || a.arena_bytes / grain_bytes(p.layers, p.heads) < p.grains) {
+    set_error("%s: an arena of %lld bytes is smaller than the plan's of %d grains", what, (long long)a.arena_bytes, p.grains);
   } else if (!a16(a.k_new) || !a16(a.v_new) || !a16(a.arena) || !a16(a.plan_words) || (a.kn_head_stride & 7) || (a.kn_tok_stride & 7) ||
              (a.vn_head_stride & 7) || (a.vn_tok_stride & 7)) {
     set_error("%s: K, V, arena and plan must be 16-byte aligned with strides that are multiples of 8 elements", what);
@@ -515,7 +529,9 @@ extern "C" {
 int64_t dkv_page_grain(int32_t layers, int32_t heads) { return layers > 0 && heads > 0 ? grain_bytes(layers, heads) : 0; }
 
 int64_t dkv_paged_plan_bytes(const dkv_paged_batch* batch) {
-  if (!batch || check_batch(*batch, "dkv_paged_plan_bytes") || !plan_fits(*batch)) return 0;
+  clear_error();
+  if (!batch) set_error("dkv_paged_plan_bytes: null batch");
+  if (!batch || check_plan(*batch, "dkv_paged_plan_bytes")) return 0;
   dkv_paged_plan p{};
   layout_of(*batch, p);
   return 4ll * p.words;
@@ -527,9 +543,9 @@ int dkv_paged_plan_write(const dkv_paged_batch* batch, void* buffer, int64_t byt
     set_error("dkv_paged_plan_write: null or misaligned pointer argument");
     return DKV_EINVAL;
   }
-  if (int rc = check_batch(*batch, "dkv_paged_plan_write")) return rc;
+  if (int rc = check_plan(*batch, "dkv_paged_plan_write")) return rc;
   const int64_t need = dkv_paged_plan_bytes(batch);
-  if (!need || bytes < need) {
+  if (bytes < need) {
     set_error("dkv_paged_plan_write: a plan of %lld bytes needed, room for %lld", (long long)need, (long long)bytes);
     return DKV_EINVAL;
   }

@@ -7,6 +7,7 @@
 // sequence alone; the others may be held by several.
 #include "dkv_paged.h"
 #include <algorithm>
+#include <initializer_list>
 #include <map>
 #include <mutex>
 #include <new>
@@ -32,6 +33,47 @@ struct Sequence {
   }
 };
 
+// Some of the blocks, of which it gives the lowest: bits, of every 64 words whether any has one, and so on up to one word.
+// (No call allocates after the start, so none of them can fail between two changes.)
+class BlockSet {
+  std::vector<std::vector<uint64_t>> level;
+
+ public:
+  int64_t size = 0;
+
+  explicit BlockSet(int64_t n = 0) {
+    do {
+      n = (n + 63) / 64;
+      level.emplace_back(std::max<int64_t>(n, 1), 0);
+    } while (n > 1);
+  }
+  bool has(int64_t b) const { return level[0][b >> 6] >> (b & 63) & 1; }
+  int first() const {
+    int64_t b = 0;
+    for (size_t i = level.size(); i-- > 0;) b = b << 6 | __builtin_ctzll(level[i][b]);
+    return (int)b;
+  }
+  void insert(int64_t b) {
+    if (has(b)) return;
+    ++size;
+    for (auto& words : level) {
+      const bool some = words[b >> 6] != 0;
+      words[b >> 6] |= 1ull << (b & 63);
+      if (some) return;
+      b >>= 6;
+    }
+  }
+  void erase(int64_t b) {
+    if (!has(b)) return;
+    --size;
+    for (auto& words : level) {
+      words[b >> 6] &= ~(1ull << (b & 63));
+      if (words[b >> 6]) return;
+      b >>= 6;
+    }
+  }
+};
+
 }  // namespace paged
 }  // namespace dkv
 
@@ -44,7 +86,7 @@ struct dkv_pool {
   std::mutex lock;
   std::vector<int8_t> code;    // of a block's pages, -1: it holds none
   std::vector<uint16_t> used;  // which of its places hold one
-  std::set<int> empty, part[3];  // blocks without pages; with some and room for more
+  BlockSet empty, part[3];  // blocks without pages; with some and room for more
   int64_t n_pages[3] = {}, n_blocks[3] = {};
   std::vector<int32_t> refs;  // sequences that hold the page at a grain
   std::map<int64_t, Sequence> seqs;
@@ -54,16 +96,16 @@ struct dkv_pool {
   static uint16_t full(int c) { return (uint16_t)((1 << PER_BLOCK[c]) - 1); }
 
   uint32_t take(int c) {
-    if (part[c].empty()) {
-      const int b = *empty.begin();
-      part[c].insert(b);  // (before anything changes: it may throw)
-      empty.erase(empty.begin());
+    if (!part[c].size) {
+      const int b = empty.first();
+      part[c].insert(b);
+      empty.erase(b);
       code[b] = (int8_t)c;
       ++n_blocks[c];
     }
-    const int b = *part[c].begin(), slot = __builtin_ctz(~(unsigned)used[b]);
+    const int b = part[c].first(), slot = __builtin_ctz(~(unsigned)used[b]);
     used[b] |= (uint16_t)(1 << slot);
-    if (used[b] == full(c)) part[c].erase(part[c].begin());
+    if (used[b] == full(c)) part[c].erase(b);
     ++n_pages[c];
     const uint32_t g = (uint32_t)b * BLOCK + slot * page_grains(4 << c);
     refs[g] = 1;
@@ -187,12 +229,12 @@ struct dkv_pool {
 
 namespace {
 
-// A call on a pool: its lock, and an error where it throws.
+// A call on a pool that needs some pointers beside: its lock, and an error where it throws.
 template <class F>
-int guarded(dkv_pool* pool, const char* what, F&& f) {
+int guarded(dkv_pool* pool, const char* what, std::initializer_list<const void*> needed, F&& f) {
   clear_error();
-  if (!pool) {
-    set_error("%s: null pool", what);
+  if (!pool || std::count(needed.begin(), needed.end(), nullptr)) {
+    set_error("%s: null %s", what, pool ? "pointer argument" : "pool");
     return DKV_EINVAL;
   }
   try {
@@ -254,7 +296,9 @@ int dkv_pool_create(int32_t layers, int32_t heads, int32_t q_heads, int64_t aren
     p = new dkv_pool;
     p->layers = layers, p->heads = heads, p->q_heads = q_heads, p->grain = grain, p->blocks = blocks;
     p->code.assign(blocks, -1), p->used.assign(blocks, 0), p->refs.assign(blocks * BLOCK, 0);
-    for (int b = 0; b < blocks; ++b) p->empty.insert(p->empty.end(), b);
+    p->empty = BlockSet(blocks);
+    for (auto& some : p->part) some = BlockSet(blocks);
+    for (int b = 0; b < blocks; ++b) p->empty.insert(b);
     *pool = p;
     return 0;
   } catch (const std::exception&) {
@@ -270,22 +314,22 @@ int dkv_pool_destroy(dkv_pool* pool) {
 }
 
 int dkv_pool_info_get(dkv_pool* pool, dkv_pool_info* info) {
-  return guarded(pool, "dkv_pool_info_get", [&](dkv_pool& p) {
-    *info = dkv_pool_info{p.grain, p.blocks, (int64_t)p.empty.size(), (int64_t)p.seqs.size(), p.generation,
+  return guarded(pool, "dkv_pool_info_get", {info}, [&](dkv_pool& p) {
+    *info = dkv_pool_info{p.grain, p.blocks, p.empty.size, (int64_t)p.seqs.size(), p.generation,
                           {p.n_pages[0], p.n_pages[1], p.n_pages[2]}, {p.n_blocks[0], p.n_blocks[1], p.n_blocks[2]}};
     return 0;
   });
 }
 
 int dkv_pool_generation(dkv_pool* pool, const int64_t** at) {
-  return guarded(pool, "dkv_pool_generation", [&](dkv_pool& p) {
+  return guarded(pool, "dkv_pool_generation", {at}, [&](dkv_pool& p) {
     *at = &p.generation;
     return 0;
   });
 }
 
 int dkv_pool_sequence(dkv_pool* pool, int64_t seq, int64_t* length, int64_t* dropped, int32_t* pages) {
-  return guarded(pool, "dkv_pool_sequence", [&](dkv_pool& p) {
+  return guarded(pool, "dkv_pool_sequence", {length, dropped, pages}, [&](dkv_pool& p) {
     const Sequence* s = p.find(seq, "dkv_pool_sequence");
     if (!s) return DKV_EINVAL;
     *length = s->length, *dropped = s->dropped, *pages = (int32_t)s->pages.size();
@@ -295,7 +339,7 @@ int dkv_pool_sequence(dkv_pool* pool, int64_t seq, int64_t* length, int64_t* dro
 
 int64_t dkv_pool_length(dkv_pool* pool, int64_t seq) {
   int64_t length = -1;
-  guarded(pool, "dkv_pool_length", [&](dkv_pool& p) {
+  guarded(pool, "dkv_pool_length", {}, [&](dkv_pool& p) {
     const Sequence* s = p.find(seq, "dkv_pool_length");
     if (!s) return DKV_EINVAL;
     length = s->length;
@@ -305,7 +349,7 @@ int64_t dkv_pool_length(dkv_pool* pool, int64_t seq) {
 }
 
 int dkv_pool_pages(dkv_pool* pool, int64_t seq, int32_t room, uint32_t* page, int32_t* rows, int32_t* holders) {
-  return guarded(pool, "dkv_pool_pages", [&](dkv_pool& p) {
+  return guarded(pool, "dkv_pool_pages", {room > 0 ? (const void*)page : pool, room > 0 ? (const void*)rows : pool, room > 0 ? (const void*)holders : pool}, [&](dkv_pool& p) {
     const Sequence* s = p.find(seq, "dkv_pool_pages");
     if (!s) return DKV_EINVAL;
     if ((size_t)std::max(room, 0) < s->pages.size()) {
@@ -318,7 +362,7 @@ int dkv_pool_pages(dkv_pool* pool, int64_t seq, int32_t room, uint32_t* page, in
 }
 
 int dkv_pool_add(dkv_pool* pool, int64_t* seq) {
-  return guarded(pool, "dkv_pool_add", [&](dkv_pool& p) {
+  return guarded(pool, "dkv_pool_add", {seq}, [&](dkv_pool& p) {
     p.seqs.emplace(p.next, Sequence());
     *seq = p.next++;
     return 0;
@@ -327,7 +371,7 @@ int dkv_pool_add(dkv_pool* pool, int64_t* seq) {
 
 int dkv_pool_adopt(dkv_pool* pool, const void* src, int64_t src_bytes, const dkv_tile* tiles, int32_t n_tiles, int64_t tokens,
                    int64_t dropped, void* arena, void* stream, int64_t* seq) {
-  return guarded(pool, "dkv_pool_adopt", [&](dkv_pool& p) {
+  return guarded(pool, "dkv_pool_adopt", {seq}, [&](dkv_pool& p) {
     const char* what = "dkv_pool_adopt";
     if (n_tiles < 0 || tokens < 0 || dropped < 0 || tokens > INT32_MAX || dropped > INT32_MAX || (n_tiles > 0 && (!tiles || !src))) {
       set_error("%s: bad arguments (tiles %d, tokens %lld, dropped %lld) or a null pointer", what, n_tiles, (long long)tokens, (long long)dropped);
@@ -378,7 +422,7 @@ int dkv_pool_adopt(dkv_pool* pool, const void* src, int64_t src_bytes, const dkv
 }
 
 int dkv_pool_fork(dkv_pool* pool, int64_t seq, int32_t n, void* arena, void* stream, int64_t* out) {
-  return guarded(pool, "dkv_pool_fork", [&](dkv_pool& p) {
+  return guarded(pool, "dkv_pool_fork", {n > 0 ? (const void*)out : pool}, [&](dkv_pool& p) {
     const char* what = "dkv_pool_fork";
     Sequence* s = p.find(seq, what);
     if (!s) return DKV_EINVAL;
@@ -426,7 +470,7 @@ int dkv_pool_fork(dkv_pool* pool, int64_t seq, int32_t n, void* arena, void* str
 }
 
 int dkv_pool_free(dkv_pool* pool, const int64_t* seqs, int32_t n) {
-  return guarded(pool, "dkv_pool_free", [&](dkv_pool& p) {
+  return guarded(pool, "dkv_pool_free", {}, [&](dkv_pool& p) {
     std::vector<Sequence*> s;
     if (int rc = p.named(seqs, n, s, "dkv_pool_free")) return rc;
     for (int i = 0; i < n; ++i) {
@@ -439,7 +483,7 @@ int dkv_pool_free(dkv_pool* pool, const int64_t* seqs, int32_t n) {
 }
 
 int dkv_pool_truncate(dkv_pool* pool, int64_t seq, int64_t length, void* arena, void* stream) {
-  return guarded(pool, "dkv_pool_truncate", [&](dkv_pool& p) {
+  return guarded(pool, "dkv_pool_truncate", {}, [&](dkv_pool& p) {
     const char* what = "dkv_pool_truncate";
     Sequence* s = p.find(seq, what);
     if (!s) return DKV_EINVAL;
@@ -476,13 +520,13 @@ int dkv_pool_truncate(dkv_pool* pool, int64_t seq, int64_t length, void* arena, 
 }
 
 int dkv_pool_compact(dkv_pool* pool, void* arena, void* stream, int64_t* moved) {
-  return guarded(pool, "dkv_pool_compact", [&](dkv_pool& p) { return p.compact(arena, stream, *moved); });
+  return guarded(pool, "dkv_pool_compact", {moved}, [&](dkv_pool& p) { return p.compact(arena, stream, *moved); });
 }
 
 int64_t dkv_pool_step_bytes(dkv_pool* pool, int32_t n, const int64_t* seqs, const int32_t* counts, const int32_t* bits, int64_t reserve,
                             int32_t* max_pages) {
   int64_t bytes = 0;
-  const int rc = guarded(pool, "dkv_pool_step_bytes", [&](dkv_pool& p) {
+  const int rc = guarded(pool, "dkv_pool_step_bytes", {max_pages}, [&](dkv_pool& p) {
     Ask a;
     if (int rc = read_ask(p, n, seqs, counts, bits, a, "dkv_pool_step_bytes")) return rc;
     // a page that is begun and those that the reserve fills, of every sequence
@@ -502,7 +546,7 @@ int64_t dkv_pool_step_bytes(dkv_pool* pool, int32_t n, const int64_t* seqs, cons
 
 int dkv_pool_step(dkv_pool* pool, int32_t n, const int64_t* seqs, const int32_t* counts, const int32_t* bits, int32_t max_pages, void* arena,
                   void* stream, void* buffer, int64_t bytes, dkv_paged_plan* plan, int64_t* generation) {
-  return guarded(pool, "dkv_pool_step", [&](dkv_pool& p) {
+  return guarded(pool, "dkv_pool_step", {plan, generation}, [&](dkv_pool& p) {
     const char* what = "dkv_pool_step";
     Ask a;
     if (int rc = read_ask(p, n, seqs, counts, bits, a, what)) return rc;
@@ -560,7 +604,7 @@ int dkv_pool_step(dkv_pool* pool, int32_t n, const int64_t* seqs, const int32_t*
 
 int64_t dkv_pool_tokens(dkv_pool* pool, int32_t n, const int64_t* seqs, const int64_t* from) {
   int64_t total = 0;
-  const int rc = guarded(pool, "dkv_pool_tokens", [&](dkv_pool& p) {
+  const int rc = guarded(pool, "dkv_pool_tokens", {n > 0 ? (const void*)from : pool}, [&](dkv_pool& p) {
     std::vector<Sequence*> s;
     if (int rc = p.named(seqs, n, s, "dkv_pool_tokens")) return rc;
     for (int i = 0; i < n; ++i) {
@@ -584,7 +628,7 @@ int dkv_pool_read(dkv_pool* pool, int32_t n, const int64_t* seqs, const int64_t*
   std::vector<dkv_page_rows> items;
   int64_t arena_bytes = 0;
   int32_t layers = 0, heads = 0;
-  const int rc = guarded(pool, "dkv_pool_read", [&](dkv_pool& p) {
+  const int rc = guarded(pool, "dkv_pool_read", {n > 0 ? (const void*)from : pool}, [&](dkv_pool& p) {
     const char* what = "dkv_pool_read";
     std::vector<Sequence*> s;
     if (int rc = p.named(seqs, n, s, what)) return rc;

@@ -533,7 +533,8 @@ typedef struct dkv_paged_batch {
  * what a step of the same counts uses at most, whatever its history. */
 typedef struct dkv_paged_plan {
   int32_t seqs, tokens, layers, heads, q_heads;
-  int32_t words; /* of the whole plan */
+  int32_t grains; /* of the arena that the pages lie in */
+  int32_t words;  /* of the whole plan */
   int32_t at_items, at_positions, at_pages, at_work, at_long, at_merges;
   int32_t items, work, long_work, merges, rows;
   int32_t max_items, max_pages, max_work, max_long, max_merges, max_rows;

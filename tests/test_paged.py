@@ -236,6 +236,15 @@ def test_refusals():
 def test_pools_refuse_null_and_foreign_tables():
     lib = _lib.load()
     assert lib.dkv_pool_add(None, None) == _lib.DKV_EINVAL
+    pool, one = Quiet(1, 1, 1), (ctypes.c_int64 * 1)(0)
+    one[0] = pool.add()
+    null = dict(add=(None,), info_get=(None,), generation=(None,), sequence=(0, None, None, None), compact=(None, None, None),
+                fork=(one[0], 1, None, None, None), free=(None, 1), adopt=(None, 0, None, 0, 0, 0, None, None, None),
+                read=(1, one, None, 0, 1, None, None, 0, 0, None), pages=(one[0], 1, None, None, None))
+    for name, rest in null.items():
+        assert getattr(lib, f'dkv_pool_{name}')(pool._pool, *rest) == _lib.DKV_EINVAL and b'null' in lib.dkv_last_error(), name
+    assert lib.dkv_pool_tokens(pool._pool, 1, one, None) == lib.dkv_pool_length(pool._pool, 77) == -1
+    assert lib.dkv_pool_step_bytes(pool._pool, 1, one, None, None, 0, None) == 0 and pool.accounting()['sequences'] == 1
     assert lib.dkv_pool_create(1, 1, 1, 1 << 20, None) == _lib.DKV_EINVAL
     c = Quiet(1, 1, 1)
     tile = np.zeros(2, dtype=[('offset', '<i8'), ('start', '<i4'), ('rows', '<u2'), ('bits', 'u1'), ('pad', 'u1')])
@@ -353,6 +362,11 @@ def test_plans_refuse_what_the_kernels_would_trust():
                dict(pages=[2 | 2047 << 2]), dict(q_heads=5), dict(heads=0), dict(layers=0), dict(count=[1 << 23], rows=[64])):
         with pytest.raises(ValueError):
             write(batch(**{**ok, **kw}))
+    # a launch has fewer than 2^32 threads: a wave for each query row and head that is joined
+    for heads, tokens, fits in ((1, 1 << 22, True), (16, 1 << 21, True), (64, 1 << 20, False), (16, 1 << 22, False)):
+        b = batch([tokens], [0], [], [], [0, 0], heads=heads, q_heads=heads)
+        assert (_lib.load().dkv_paged_plan_bytes(ctypes.byref(b)) > 0) == fits
+        assert fits or b'too many for one step' in _lib.load().dkv_last_error()
     lib = _lib.load()
     b = batch(**ok)
     assert lib.dkv_paged_plan_write(ctypes.byref(b), None, 1 << 20, ctypes.byref(plan)) == _lib.DKV_EINVAL
@@ -371,7 +385,7 @@ def args(**kw):
 
 
 @pytest.mark.parametrize('kw', [dict(k_new=0), dict(v_new=8), dict(kn_tok_stride=63), dict(vn_head_stride=4), dict(arena=None),
-                                dict(plan_words=None), dict(layer=1), dict(layer=-1), dict(plan=_lib.PagedPlan())])
+                                dict(plan_words=None), dict(layer=1), dict(layer=-1), dict(plan=_lib.PagedPlan()), dict(arena_bytes=(1 << 20) - 1)])
 def test_append_and_attend_refuse(kw):
     lib = _lib.load()
     for call in (lib.dkv_paged_append, lib.dkv_paged_attend):
