@@ -221,6 +221,8 @@ SIGNATURES = [
     ('dkv_paged_plan_write', ctypes.c_int, [ctypes.POINTER(PagedBatch), ctypes.c_void_p, ctypes.c_int64,
                                             ctypes.POINTER(PagedPlan)]),
     ('dkv_paged_append', ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
+    ('dkv_paged_rope_append', ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p,
+                                             ctypes.c_int64, ctypes.c_void_p]),
     ('dkv_paged_workspace_bytes', ctypes.c_int64, [ctypes.c_void_p]),
     ('dkv_paged_attend', ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
     ('dkv_paged_read', ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32,

@@ -373,7 +373,25 @@ class PagedStep(_CacheBase):
 
     # -- as the cache of a patched decoder (install_packed_attention) ------------
     def append_projection(self, qkv, cos, sin, q_heads, layer):
-        return None  # (no launch of its own: split and RoPE, then append())
+        """The joined Q/K/V projection [1, tokens, (q_heads + 2 heads) * 64] of one layer -> (q, k, v, 0), split, with RoPE
+        from cos and sin [1, tokens, 64] and packed in one launch: what rope_qkv() and append() give, bit for bit. None
+        where the inputs are not bf16 rows that the launch takes (GPUCache.append_projection)."""
+        c, n = self.cache, self.tokens
+        c._check('append', self, layer, ())
+        if (qkv.dim() != 3 or qkv.shape[:2] != (1, n) or qkv.shape[2] != (q_heads + 2 * c.heads) * c.dim or q_heads != c.q_heads
+                or cos.shape[-2:] != (n, 64) or cos.numel() != n * 64 or sin.shape != cos.shape
+                or not all(t.get_device() == c._index >= 0 and t.dtype == torch.bfloat16 for t in (qkv, cos, sin))):
+            return None
+        qkv, cos, sin = qkv.reshape(n, -1), cos.reshape(n, 64), sin.reshape(n, 64)
+        if cos.stride() != sin.stride() or any(t.stride(-1) != 1 or t.stride(0) % 8 or t.data_ptr() % 16 for t in (qkv, cos, sin)):
+            return None
+        q, k, v = (qkv.new_empty((1, heads, n, c.dim)) for heads in (q_heads, c.heads, c.heads))
+        head = n * c.dim
+        args = _ARGS.pack(q.data_ptr(), head, c.dim, k.data_ptr(), head, c.dim, v.data_ptr(), head, c.dim, c._arena_ptr, c.arena_bytes,
+                          self.device_plan(), self.plan_bytes, layer, self.captured(), 0.0, 0, 0, 0, 0, 0, 0, 0)
+        c._launch('dkv_paged_rope_append', lambda stream: _lib.load().dkv_paged_rope_append(
+            args, qkv.data_ptr(), qkv.stride(0), cos.data_ptr(), sin.data_ptr(), cos.stride(0), stream))
+        return q, k, v, 0
 
     def _fused_attention(self, n, q_heads, layer, project, cos, sin, cs_stride, qkv_out, out, stream):
         """The joined Q/K/V projection, its split and RoPE, append() and attend() for the fused decoder layer's eager
@@ -394,8 +412,7 @@ class PagedStep(_CacheBase):
         args = _ARGS.pack(qkv_out, head, d, kp, head, d, vp, head, d, c._arena_ptr, c.arena_bytes, self.device_plan(), self.plan_bytes,
                           layer, bounds, d ** -0.5, out, q_heads * d, d, 0, PRECISIONS[c.precision], at if need else 0, need)
         rc = (lib.dkv_linear_tiled(x, x_stride, weight, w_stride, n, width, k, norm, eps, 0, None, 0, at, width, layout, stream)
-              or lib.dkv_rope_qkv(at, width, cos, sin, cs_stride, n, q_heads, H, qkv_out, kp, vp, stream)
-              or lib.dkv_paged_append(args, stream) or lib.dkv_paged_attend(args, stream))
+              or lib.dkv_paged_rope_append(args, at, width, cos, sin, cs_stride, stream) or lib.dkv_paged_attend(args, stream))
         if rc:
             _lib.check(rc, 'the launches of a fused decoder layer')
 

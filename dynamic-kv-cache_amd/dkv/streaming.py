@@ -32,8 +32,8 @@ from .gpu_cache import GPUCache, install_packed_attention
 from .gpu_ops import install_fused_ops, sample
 from .paged_cache import PagedCache
 
-# generate_batch() captures more tokens than these: a replayed forward of a token of each sequence takes 1.35 ms and an eager one,
-# which waits for the host, 1.74 (32 layers, 1 to 16 questions; at 64 both take 1.85), a capture 3 to 5 ms.
+# generate_batch() captures more tokens than these: a replayed forward of a token of each sequence takes 1.3 ms and an eager one,
+# which waits for the host, 1.6 (32 layers, 1 to 16 questions; at 64 both take 1.8), a capture 3 to 5 ms.
 GRAPH_TOKENS = 16
 MFMA_ROWS = 192  # query rows per frame-chunk attention workgroup (MFMA_ROWS of csrc/dkv_attn_common.h)
 

@@ -575,6 +575,12 @@ typedef struct dkv_paged_args {
 /* Packs the step's new rows of a layer into their pages, byte for byte what dkv_pack writes (q and out are not
  * read). */
 int dkv_paged_append(const dkv_paged_args* args, void* stream);
+/* The joined Q/K/V projection [tokens, (q_heads + 2 heads) * 64] of a step's tokens, split and with RoPE from cos / sin rows
+ * [tokens, 64] as dkv_rope_qkv computes it, into q, k_new and v_new, which here are written, with their strides (no two of their
+ * rows may share memory), and K and V packed as dkv_paged_append packs them. All bf16, 16-byte aligned, strides in multiples of 8
+ * elements. No counterpart in the reference (src/gpu_cache.py:164-172 is the same of one sequence). */
+int dkv_paged_rope_append(const dkv_paged_args* args, const void* qkv, int64_t qkv_row_stride, const void* cos, const void* sin,
+                          int64_t cs_row_stride, void* stream);
 
 /* The step's new tokens attend, each to its sequence's history before the step and to the sequence's new tokens up to
  * itself (these as they are in k_new and v_new). What later tokens hold, NaN and infinities included, does not reach

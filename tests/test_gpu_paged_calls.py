@@ -247,3 +247,45 @@ def test_tokens_behind_the_last_sequence_stay(cuda):
             g = 48 * block + 9 * slot
             if g not in held:
                 assert (cache.arena[g * grain:(g + 9) * grain] == 0xA5).all()
+
+
+@pytest.mark.parametrize('heads,group,counts', [(1, 1, [1]), (5, 3, [1] * 9), (2, 4, [70, 1, 64, 200, 3])])
+def test_joined_projections(cuda, heads, group, counts):
+    """Split, RoPE and pack in one launch: the rows of rope_qkv() and the bytes of append(), also replayed."""
+    from dkv.gpu_ops import rope_qkv
+    gen = torch.Generator().manual_seed(len(counts))
+    n, q_heads = sum(counts), heads * group
+    qkv = torch.randn(1, n, (q_heads + 2 * heads) * 64 + 64, generator=gen).bfloat16().cuda()[..., 64:]
+    qkv[0, 0, -64:] = 0.0  # a row of one value, with a zero of each sign
+    qkv[0, 0, -1] = -0.0
+    angle = torch.rand(1, n, 32, generator=gen).repeat(1, 1, 2) * 50
+    cos, sin = angle.cos().bfloat16().cuda(), angle.sin().bfloat16().cuda()
+    for bits in (4, 8, 16):
+        announce(f'joined projection {heads} x {group} {counts} {bits}')
+        a, b = (PagedCache(3, heads, q_heads, max_tokens=4096) for _ in range(2))
+        steps = []
+        for cache in (a, b):
+            cache.arena.zero_()
+            seqs = [cache.add() for _ in counts]
+            cache.step(seqs, 10, bits)
+            steps.append(cache.step(seqs, counts, bits))
+        q, k, v = rope_qkv(qkv, cos, sin, q_heads, heads)
+        a.append(k, v, 1, steps[0])
+        got = steps[1].append_projection(qkv, cos, sin, q_heads, 1)
+        assert got[3] == 0 and all(torch.equal(x, y) for x, y in zip((q, k, v), got))
+        assert torch.equal(a.arena, b.arena)
+        b.arena.zero_()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = steps[1].append_projection(qkv, cos, sin, q_heads, 1)
+        for _ in range(2):
+            b.arena.zero_()
+            graph.replay()
+            assert torch.equal(a.arena, b.arena) and all(torch.equal(x, y) for x, y in zip((q, k, v), got))
+    step = steps[1]
+    for args in ((qkv[:, :, :64], cos, sin, q_heads, 1), (qkv.float(), cos, sin, q_heads, 1), (qkv, cos[..., :32], sin, q_heads, 1),
+                 (qkv.cpu(), cos, sin, q_heads, 1), (qkv, cos, sin, q_heads + 1, 1)):
+        assert step.append_projection(*args) is None
+    with pytest.raises(ValueError, match='layer 3 of 3'):
+        step.append_projection(qkv, cos, sin, q_heads, 3)

@@ -398,6 +398,16 @@ def test_attend_refuses(kw):
     assert _lib.load().dkv_paged_attend(ctypes.byref(args(**kw)), None) == _lib.DKV_EINVAL
 
 
+def test_rope_append_refuses():
+    lib = _lib.load()
+    for kw, qkv, row, cos, sin, cs in ((dict(layer=1), 4096, 640, 4096, 4096, 64), (dict(q=0), 4096, 640, 4096, 4096, 64),
+                                       (dict(q=4104), 4096, 640, 4096, 4096, 64), (dict(q_tok_stride=4), 4096, 640, 4096, 4096, 64),
+                                       ({}, None, 640, 4096, 4096, 64), ({}, 4098, 640, 4096, 4096, 64), ({}, 4096, 644, 4096, 4096, 64),
+                                       ({}, 4096, 640, None, 4096, 64), ({}, 4096, 640, 4096, 4104, 64), ({}, 4096, 640, 4096, 4096, 66)):
+        assert lib.dkv_paged_rope_append(ctypes.byref(args(**kw)), qkv, row, cos, sin, cs, None) == _lib.DKV_EINVAL and lib.dkv_last_error()
+    assert lib.dkv_paged_rope_append(None, 4096, 640, 4096, 4096, 64, None) == _lib.DKV_EINVAL
+
+
 def test_attend_wants_its_workspace():
     pages = [16 * i << 2 | 2 for i in range(400)]
     _, plan = write(batch([1], [64 * 399], pages, [64] * 399 + [1], [0, 400], arena=1 << 26, max_pages=400))
