@@ -29,9 +29,9 @@ struct Page {
 
 // One workgroup's share of a sequence's (or, over pages that several sequences have in common, a group's) attention, for
 // each KV head: units [u0, u1) for block `block` of its query rows. Unit u is page first_page + u of the plan while u is
-// below n_pages (at 4 bits below n4, 8 below n8, else 16: attention takes keys in any order), then 64 new tokens each. Query row r is token r / G, query head r % G of the KV head; `count` tokens
-// from token0 of the step on. The block's rows go to the partial rows from `part` on, or where that is negative to the
-// output.
+// below n_pages (at 4 bits below n4, 8 below n8, else 16: attention takes keys in any order), then 64 new tokens each. Query
+// row r is token r / G, query head r % G of the KV head; `count` tokens from token0 of the step on. The block's rows go to the
+// partial rows from `part` on, or where that is negative to the output.
 struct Work {
   int32_t first_page, n4, n8, n_pages, token0, count, block, u0, u1, part, reserved[2];
 };

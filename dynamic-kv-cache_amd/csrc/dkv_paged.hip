@@ -50,31 +50,34 @@ __device__ __forceinline__ void pack_row(const u32x4& w, bool valid, int c, uint
                                 reinterpret_cast<uint64_t*>(sub + TILE * 8 * BITS + 8 * row));
 }
 
-// Rows r0 + 8 i of an item, 8 lanes a row, AHEAD of them loaded before the first is packed. (All 8 at once take 230
-// registers and leave two waves a SIMD: 7900 tokens of 8 heads 13.6 us instead of 10.5.)
+// Rows r0 + 8 i of at most HALF_ITEM, 8 lanes a row, all loaded before the first is packed.
+constexpr int HALF_ITEM = 32;
 template <int BITS>
 __device__ __forceinline__ void pack_rows(const uint16_t* src, int64_t stride, int rows, int r0, int c, uint8_t* sub, int row0) {
-  constexpr int AHEAD = 4;
-  for (int i0 = 0; i0 < rows; i0 += 8 * AHEAD) {
-    u32x4 w[AHEAD];
+  u32x4 w[HALF_ITEM / 8];
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) w[i] = *reinterpret_cast<const u32x4*>(src + min(i0 + 8 * i + r0, rows - 1) * stride + 8 * c);
+  for (int i = 0; i < HALF_ITEM / 8; ++i) w[i] = *reinterpret_cast<const u32x4*>(src + min(8 * i + r0, rows - 1) * stride + 8 * c);
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) {
-      if (i0 + 8 * i >= rows) break;
-      pack_row<BITS>(w[i], i0 + 8 * i + r0 < rows, c, sub, row0 + i0 + 8 * i + r0);
-    }
+  for (int i = 0; i < HALF_ITEM / 8; ++i) {
+    if (8 * i >= rows) break;
+    pack_row<BITS>(w[i], 8 * i + r0 < rows, c, sub, row0 + 8 * i + r0);
   }
 }
 
-// A wave takes the rows of one item (up to 64 tokens of a page) of one K or V head.
+// Packs a step's rows: a = min, s = (max - min) / (2^b - 1), q = rint((x - a) / s), dkv_pack's bytes. Bound by the bytes of a long
+// prompt (128 read and 40 to 136 written a row) and the launch of a short one. A wave takes half of the rows of one item (up to 64
+// tokens of a page) of one K or V head, whose loads are one group: 5833 tokens of 8 heads, 21.9 MB, 8.2 us (2.7 TB/s; whole items in
+// two groups 10.5, in one, which takes 230 registers, 13.6), a token of each of 32 sequences of 5 heads 2.8 us.
 __global__ __launch_bounds__(256) void append_kernel(dkv_paged_args a) {
   const int32_t* plan = static_cast<const int32_t*>(a.plan_words);
-  if (a.bounds && (int)blockIdx.x >= plan[N_ITEMS]) return;
+  if (a.bounds && (int)(blockIdx.x >> 1) >= plan[N_ITEMS]) return;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63, H = a.plan.heads;
   const int kvh = blockIdx.y * 4 + wave;
   if (kvh >= 2 * H) return;
-  const dkv_page_rows item = plan_record<dkv_page_rows>(plan, a.plan.at_items, blockIdx.x);
+  dkv_page_rows item = plan_record<dkv_page_rows>(plan, a.plan.at_items, blockIdx.x >> 1);
+  const int skip = HALF_ITEM * (blockIdx.x & 1);
+  if (skip >= item.rows) return;
+  item.token += skip, item.row0 += skip, item.rows = min(HALF_ITEM, item.rows - skip);
   const int kv = kvh >= H, h = kvh - kv * H, c = lane & 7, r0 = lane >> 3;
   const uint16_t* src = static_cast<const uint16_t*>(kv ? a.v_new : a.k_new) +
                         (kv ? h * a.vn_head_stride + item.token * a.vn_tok_stride : h * a.kn_head_stride + item.token * a.kn_tok_stride);
@@ -148,7 +151,8 @@ struct Items {
   dkv_page_rows at[ARG_ITEMS];
 };
 
-// Rows of a page as values, 8 lanes a row (lane c: elements [8 c, 8 c + 8)): every store of bf16 writes whole lines.
+// Rows of a page as values code * s + a, 8 lanes a row (lane c: elements [8 c, 8 c + 8)): every store of bf16 writes whole lines.
+// Bound by its bytes: 8138 tokens of 8 layers of 5 heads, 131 MB read and written, 31 us in two launches (4.2 TB/s).
 template <int BITS>
 __device__ __forceinline__ void read_rows(const uint8_t* sub, int row0, int rows, int r0, int c, void* out, int64_t at, int out_dtype) {
   constexpr int AHEAD = 4;
@@ -212,7 +216,8 @@ struct Moves {
 };
 
 // One sub-block's rows: the payload in 16-byte pieces, then the (offset, scale) pairs, which lie behind as many rows as
-// the tile has room for. All loads before the first store.
+// the tile has room for. All loads before the first store. Bound by its bytes: the same history gathered into pages, 96 MB, 18 us in
+// two launches (5.3 TB/s, a large copy's rate).
 template <int BITS>
 __device__ __forceinline__ void move_rows(const dkv_page_move& m, const uint8_t* from, uint8_t* to, int lane) {
   constexpr int ROW = 8 * BITS, PIECES = BITS / 2;  // bytes; of 64 rows, a lane's pieces
@@ -352,7 +357,7 @@ static int check_plan(const dkv_paged_batch& b, const char* what) {
   if (fits) {
     dkv_paged_plan p{};
     layout_of(b, p);
-    const int64_t threads = std::max<int64_t>({p.max_items, (int64_t)p.max_work * b.heads, 2ll * p.max_long * b.heads,
+    const int64_t threads = std::max<int64_t>({2ll * p.max_items, (int64_t)p.max_work * b.heads, 2ll * p.max_long * b.heads,
                                       (int64_t)p.max_merges * (SHORT_BLOCK / 4) * b.heads}) * 256;
     fits = threads <= UINT32_MAX;
   }
@@ -623,7 +628,7 @@ int dkv_paged_append(const dkv_paged_args* args, void* stream) {
   }
   if (int rc = check_args(*args, false, "dkv_paged_append")) return rc;
   const dkv_paged_plan& p = args->plan;
-  hipLaunchKernelGGL(append_kernel, dim3(args->bounds ? p.max_items : p.items, (2 * p.heads + 3) / 4), dim3(256), 0, (hipStream_t)stream,
+  hipLaunchKernelGGL(append_kernel, dim3(2 * (args->bounds ? p.max_items : p.items), (2 * p.heads + 3) / 4), dim3(256), 0, (hipStream_t)stream,
                      *args);
   return (int)hipGetLastError();
 }

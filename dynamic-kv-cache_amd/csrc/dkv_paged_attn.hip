@@ -1,4 +1,18 @@
-// Attention of a step's new tokens over pages (gfx950).
+// Attention of a step's new tokens over pages, sequences (and groups that share pages) of few query rows; the join (gfx950).
+//
+// o = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m), s_j = q k_j / 8, over the history's rows and the new ones up to a query's own, in
+// one pass with a running maximum m. A workgroup takes 16 query rows (tokens times query heads) of a KV head over a range of units
+// of 64 keys, each of its four waves a fourth of these; a step's ranges are cut so that about 2048 workgroups share its units
+// whatever the lengths (dkv_paged.hip), and partial rows are joined by merge_kernel. Per half page and wave: keys straight from
+// global memory into the operands of S^T = K Q^T (16x16x32 bf16), whose result lies where O^T = V^T P^T reads P^T, values into V^T's.
+// No LDS but for scales and the waves' join.
+// Weights: sums and statistics in 32 bits; P is the sum of two bf16 values (2^-16) for a bf16 output, of three (2^-24) for fp32.
+// At precision bf16 a packed value is rounded to bf16, GPUCache's rounding; at fp32 its code is multiplied and its scale and offset
+// come apart.
+// What bounds it: long histories their bytes, six of 30k to 131k tokens of 8 heads at fp32 506 MB in 100 us (5.0 TB/s, of a large
+// copy's 5.2), a token of each of 64 streams of 300 to 8128 tokens 107 MB in 27 us; short ones the chain of loads of one launch
+// (three of up to 333 tokens 7.5 us); branches the unpacking of shared pages once for each 16 of their rows (48 of 8128 shared
+// tokens 15.5 us).
 #include "dkv_rows.h"
 #include "dkv_paged.h"
 
@@ -406,8 +420,9 @@ __global__ __launch_bounds__(256, 4) void short_kernel(dkv_paged_args a, float* 
   }
 }
 
-// Joins the partials of 16 query rows: a wave a row, 16 lanes a split with four elements each, four splits at a time and
-// AHEAD of these in flight. (16 lanes a row: 48 branches, whose 127 pages in common are split 64 ways, 13.9 us.)
+// Joins the partials of 16 query rows: o = sum_s exp(m_s - m) o_s / sum_s exp(m_s - m) l_s. A wave a row, 16 lanes a split with
+// four elements each, four splits at a time and AHEAD of these in flight: 4 to 7 us, a launch and its chain of loads. (16 lanes a
+// row: 48 branches, whose 127 pages in common were split 64 ways, 13.9 us.)
 __global__ __launch_bounds__(256) void merge_kernel(dkv_paged_args a, const float* part_o, const float2* part_ml) {
   const int32_t* plan = static_cast<const int32_t*>(a.plan_words);
   const int H = a.plan.heads, G = a.plan.q_heads / H, h = blockIdx.x % H, four = blockIdx.x / H, record = four / (SHORT_BLOCK / 4);

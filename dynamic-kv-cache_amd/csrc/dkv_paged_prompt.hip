@@ -7,6 +7,15 @@
 // in the places that the second product reads P^T from: P never leaves its registers, and a row's maximum and sum take
 // one exchange between the two halves of a wave. V^T comes from V's rows in LDS by transposing reads (ds_read_b64_tr_b16:
 // of 16 lanes that read 4 elements of 4 rows each, lane i gets element i of the rows).
+//
+// Packed rows of unit u + 3 are asked for, and those of u + 1 unpacked, while u is multiplied; new and 16-bit rows come two units
+// ahead; one barrier a unit. Scores, statistics and sums are fp32. P is one bf16 value at precision and output bf16 (a relative 2^-8
+// of each weight, averaged over the keys; a sequence of few rows keeps two, see dkv_paged_attn.hip), else the sum of two or three.
+// What bounds it: the vector units, 187 instructions a unit and wave beside its 16 matrix products of 32 cycles, of them 32
+// exponentials of four times the cost: 12.5k tokens of prompts of 5 heads of 3 214 us (773 TFLOP/s, 59 % of a large product's), 12
+// prompts of up to 2048 tokens of 8 heads of 4 65 us (534); with few units a workgroup the chain from the plan to the first tile, 16
+// questions about 6144 shared tokens 32 us. At fp32 the split into three values and the scales apart, 527 instructions, and two
+// waves a SIMD, of whose time 38 % waits: 8 frames of 78 tokens over 92k 97 us.
 #include <type_traits>
 
 #include "dkv_rows.h"
