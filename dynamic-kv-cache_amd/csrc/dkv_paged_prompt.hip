@@ -12,10 +12,10 @@
 // ahead; one barrier a unit. Scores, statistics and sums are fp32. P is one bf16 value at precision and output bf16 (a relative 2^-8
 // of each weight, averaged over the keys; a sequence of few rows keeps two, see dkv_paged_attn.hip), else the sum of two or three.
 // What bounds it: the vector units, 187 instructions a unit and wave beside its 16 matrix products of 32 cycles, of them 32
-// exponentials of four times the cost: 12.5k tokens of prompts of 5 heads of 3 214 us (773 TFLOP/s, 59 % of a large product's), 12
-// prompts of up to 2048 tokens of 8 heads of 4 65 us (534); with few units a workgroup the chain from the plan to the first tile, 16
+// exponentials of four times the cost: 12.5k tokens of prompts of 5 heads of 3 217 us (762 TFLOP/s, 58 % of a large product's), 12
+// prompts of up to 2048 tokens of 8 heads of 4 63 us (546); with few units a workgroup the chain from the plan to the first tile, 16
 // questions about 6144 shared tokens 32 us. At fp32 the split into three values and the scales apart, 527 instructions, and two
-// waves a SIMD, of whose time 38 % waits: 8 frames of 78 tokens over 92k 97 us.
+// waves a SIMD, of whose time 38 % waits: 8 frames of 78 tokens over 92k 99 us.
 #include <type_traits>
 
 #include "dkv_rows.h"
@@ -86,6 +86,13 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
+// x as a value of its own: what is computed from it is not kept in registers from before. (These are full: addresses that are used
+// once a unit or less would be kept in scratch memory.)
+__device__ __forceinline__ int anew(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
 template <int PREC, int TERMS>
 __global__ __launch_bounds__(64 * WAVES, PREC ? 2 : 4) void long_kernel(dkv_paged_args a, float* part_o, float2* part_ml) {
   __shared__ __attribute__((aligned(1024))) uint8_t tiles[RING][2][TILE_BYTES];
@@ -128,6 +135,7 @@ __global__ __launch_bounds__(64 * WAVES, PREC ? 2 : 4) void long_kernel(dkv_page
   // Rows of 16 bits go straight to their tile: a wave 8 rows of K and of V. New rows past the last one repeat it; rows of a
   // page that are not there are read as they are (zero_values).
   auto load_tile = [&](int u, const Unit& x, int buf) {
+    const int thread = anew(t), srow = thread >> 3, piece = (thread & 7) ^ place(srow);
     const uint8_t *k, *v;
     uint32_t k_off = 16 * piece, v_off = 16 * piece;
     if (u < w.n_pages) {
@@ -303,7 +311,7 @@ __global__ __launch_bounds__(64 * WAVES, PREC ? 2 : 4) void long_kernel(dkv_page
     float sum = 0.f;
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
-      if (TERMS > 1 && kb == 1 && one_half) break;  // (8 frames of 78 tokens, 3 terms: 102 us, 110 without; at 1 term 2 % slower)
+      if (TERMS > 1 && kb == 1 && one_half) break;  // (8 frames of 78 tokens, 3 terms: 102 us with it, 110 without; at 1 term 2 % slower)
 #pragma unroll
       for (int st = 0; st < 2; ++st) {  // 16 keys
         Op8 p[TERMS];
@@ -364,17 +372,19 @@ __global__ __launch_bounds__(64 * WAVES, PREC ? 2 : 4) void long_kernel(dkv_page
     x0 = x1, x1 = x2, x2 = x3, x3 = x4;
     buf = next;
   }
+  const int m_new = min(wave0 + (anew(t) & 31), total - 1) / G;  // this lane's token again
   for (; u < w.u1; ++u) {  // new tokens: nothing to be unpacked
     const int next = buf + 1 == RING ? 0 : buf + 1, after = next + 1 == RING ? 0 : next + 1;
     const int first = (u - w.n_pages) * TILE;
     const bool more = u + 2 < w.u1;
     if (more) load_tile(u + 2, Unit{16, min(TILE, w.count - first - 2 * TILE), 2, 0}, after);
     if (first + TILE - 1 > first_token) zero_values(Unit{16, min(TILE, w.count - first), 0, 0}, tiles[buf][1], true);
-    if (on && first <= m_last) attend(std::false_type(), buf, first + TILE - 1 > m_first, m + 1 - first, m_last - first < 32);
+    if (on && first <= m_last) attend(std::false_type(), buf, first + TILE - 1 > m_first, m_new + 1 - first, m_last - first < 32);
     step(more ? 2 : 0);
     buf = next;
   }
   if (!on) return;
+  const int last = anew(t), c_last = last & 31, half_last = last >> 5 & 1, row_last = min(wave0 + c_last, total - 1), m_out = row_last / G;
   auto both = [](float x) {
     const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return __uint_as_float(y[0]) + __uint_as_float(y[1]);
@@ -390,8 +400,8 @@ __global__ __launch_bounds__(64 * WAVES, PREC ? 2 : 4) void long_kernel(dkv_page
         uint2 x[8];
         bool some = false;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {  // elements 8 i + 4 half + ...
-          x[i] = v[2 * i + half];
+        for (int i = 0; i < 8; ++i) {  // elements 8 i + 4 half_last + ...
+          x[i] = v[2 * i + half_last];
           some = some || bad_bf16(x[i].x) || bad_bf16(x[i].x >> 16) || bad_bf16(x[i].y) || bad_bf16(x[i].y >> 16);
         }
         if (!__builtin_amdgcn_ballot_w64(some)) continue;
@@ -399,13 +409,13 @@ __global__ __launch_bounds__(64 * WAVES, PREC ? 2 : 4) void long_kernel(dkv_page
         float dot = 0.f;
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) {
-          const u32x4 y = k[2 * ks + half];
+          const u32x4 y = k[2 * ks + half_last];
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             dot = __builtin_fmaf(bf16_lo(q[ks].u[e]), bf16_lo(y[e]), __builtin_fmaf(bf16_hi(q[ks].u[e]), bf16_hi(y[e]), dot));
         }
         const float p = __builtin_amdgcn_exp2f(both(dot) * xs - m_run);
-        if (first + j > m) continue;
+        if (first + j > m_out) continue;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const int db = i / 4, at = 4 * (i % 4);
@@ -417,22 +427,22 @@ __global__ __launch_bounds__(64 * WAVES, PREC ? 2 : 4) void long_kernel(dkv_page
       }
     }
   }
-  if (wave0 + c >= total) return;
+  if (wave0 + c_last >= total) return;
   if (w.part < 0) {
     const float inv = 1.f / l;
-    const int64_t at = (int64_t)(w.token0 + m) * a.out_tok_stride + (int64_t)(h * G + row - m * G) * a.out_head_stride + 4 * half;
+    const int64_t at = (int64_t)(w.token0 + m_out) * a.out_tok_stride + (int64_t)(h * G + row_last - m_out * G) * a.out_head_stride + 4 * half_last;
 #pragma unroll
     for (int i = 0; i < 32; i += 4) {
       const f32x4 x = f32x4{acc[i / 16][i % 16] + off, acc[i / 16][i % 16 + 1] + off, acc[i / 16][i % 16 + 2] + off, acc[i / 16][i % 16 + 3] + off} * inv;
       store4(a.out, a.out_dtype, at + 32 * (i / 16) + 8 * (i % 16 / 4), x);
     }
   } else {
-    const int64_t at = (int64_t)(w.part + 32 * wave + c) * H + h;
+    const int64_t at = (int64_t)(w.part + 32 * wave + c_last) * H + h;
 #pragma unroll
     for (int i = 0; i < 32; i += 4)
-      *reinterpret_cast<f32x4*>(part_o + at * D + 32 * (i / 16) + 8 * (i % 16 / 4) + 4 * half) =
+      *reinterpret_cast<f32x4*>(part_o + at * D + 32 * (i / 16) + 8 * (i % 16 / 4) + 4 * half_last) =
           f32x4{acc[i / 16][i % 16] + off, acc[i / 16][i % 16 + 1] + off, acc[i / 16][i % 16 + 2] + off, acc[i / 16][i % 16 + 3] + off};
-    if (half == 0) part_ml[at] = make_float2(m_run, l);
+    if (half_last == 0) part_ml[at] = make_float2(m_run, l);
   }
 }
 
