@@ -213,7 +213,7 @@ class PagedCache:
     def step(self, seqs, counts=1, bits=16, reserve=0):
         """The next tokens of some sequences: `counts` of each (one number or one a sequence), at width `bits` (too).
         Opens their pages and plans what every layer's append() and attend() do; the sequences are as long from here
-        on. The step's tensors hold the sequences' tokens one after the other, in this order. `reserve`: room in the
+        on, and what other calls read or copy of the new tokens is what append() has packed by then. The step's tensors hold the sequences' tokens one after the other, in this order. `reserve`: room in the
         plan for as many more tokens of every sequence, for steps that go on with advance(). Sequences that share
         pages attend to these together where they stand next to each other."""
         return PagedStep(self, seqs, counts, bits, reserve)
@@ -298,7 +298,8 @@ class PagedStep(_CacheBase):
     positions: [tokens] int64 on the device, of every new token. A step can be the `past_key_values` of a decoder that
     install_packed_attention() patched: its attention then packs and attends for all the sequences. A step that a graph
     capture records can go on: advance() plans the sequences' next tokens into the same device memory, and a replay of
-    the graph runs over them.
+    the graph runs over them. (Nothing looks at a replay: once pages were freed, cut or moved, the graph is replayed after
+    an advance() alone.)
     """
 
     backend = 'fused'
@@ -341,6 +342,8 @@ class PagedStep(_CacheBase):
         at = 4 * plan.at_positions
         self.positions = self._dev[at:at + 8 * self.tokens].view(torch.int64)
         self._needs = {}
+        if self._stream is not None:
+            self.device_plan()  # (it was copied on the stream of now)
 
     def advance(self):
         """Plans the same sequences' next tokens, as many of each and at the same widths, in place of this step's. The

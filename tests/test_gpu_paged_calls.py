@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from conftest import announce
-from dkv import PagedCache
+from dkv import GPUCache, PagedCache
 from test_gpu_paged import Model, rows_like
 
 pytestmark = pytest.mark.gpu
@@ -289,3 +289,54 @@ def test_joined_projections(cuda, heads, group, counts):
         assert step.append_projection(*args) is None
     with pytest.raises(ValueError, match='layer 3 of 3'):
         step.append_projection(qkv, cos, sin, q_heads, 3)
+
+
+@pytest.mark.parametrize('q_heads,counts', [(200, [1, 2]), (300, [1, 1, 3]), (161, [1]), (64, [3, 1, 2])])
+def test_many_query_heads_of_one(cuda, q_heads, counts):
+    """One KV head with more query heads than a block has rows: a token's rows go over several blocks."""
+    announce(f'{q_heads} query heads {counts}')
+    m = Model(1, q_heads, seed=q_heads)
+    seqs = [m.add() for _ in counts]
+    for bits, n in ((4, 100), (16, 30), (8, 70)):
+        m.step(seqs, n, bits)
+    m.attend(seqs, counts)
+    m.attend(seqs, counts, 8, torch.float32)
+
+
+def test_adopted_branches_and_plans(cuda):
+    """A fork's history with the tokens after it, and a planned cache that is filled up to the middle of a tile."""
+    announce('adopted branches and plans')
+    gen = torch.Generator().manual_seed(6)
+    layers, heads = 2, 3
+    rows = [rows_like(gen, 1, heads, n).cuda() for n in (100, 30, 1, 1)]
+    base = GPUCache(None, layers=layers, heads=heads, max_tokens=1024)
+    plan = GPUCache([(4, 100), (8, 90), (16, 30)], layers=layers, heads=heads)
+    for cache, some in ((base, rows[:1]), (plan, rows)):
+        for i, x in enumerate(some):
+            cache.select(8 if i else 4)
+            for layer in range(layers):
+                cache.append(x, x, layer)
+    fork = base.fork()
+    for x in rows[1:]:
+        fork.select(8)
+        for layer in range(layers):
+            fork.append(x, x, layer)
+    pages = PagedCache(layers, heads, heads, max_tokens=2048)
+    for cache, n in ((base, 100), (fork, 132), (plan, 132)):
+        seq = pages.adopt(cache)
+        assert pages.length(seq) == n
+        for layer in range(layers):
+            for x, y in zip(pages.materialize(layer, seq), cache.materialize(layer)):
+                assert torch.equal(x, y)
+
+
+def test_nothing_to_read(cuda):
+    pages = PagedCache(2, 1, 1, max_tokens=256)
+    seq = pages.add()
+    for layer, shape in ((0, (1, 1, 0, 64)), (None, (2, 1, 0, 64))):
+        assert [x.shape for x in pages.materialize(layer, [seq])] == [shape] * 2
+    assert pages.fork(seq, 0) == [] and pages.compact() == 0
+    assert pages.adopt(GPUCache(None, layers=2, heads=1, max_tokens=64)) != seq
+    pages.free([])
+    step = pages.step(seq, 3)
+    assert pages.materialize(0, seq, first=3)[0].shape == (1, 1, 0, 64) and step.positions.tolist() == [0, 1, 2]
