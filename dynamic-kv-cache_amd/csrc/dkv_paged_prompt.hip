@@ -287,11 +287,13 @@ __global__ __launch_bounds__(64 * WAVES, PREC ? 2 : 4) void long_kernel(dkv_page
           s[kb][i + 1] = __builtin_fmaf(as[3], s[kb][i + 1], as[2] * q_sum);
         }
     }
-    if (masked)
+    if (masked) {
+      const int below = high - 4 * half;  // (compared with constants: the lanes' keys are not kept in registers)
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[kb][i] = 32 * kb + 8 * (i / 4) + 4 * half + i % 4 < high ? s[kb][i] : -INFINITY;
+        for (int i = 0; i < 16; ++i) s[kb][i] = 32 * kb + 8 * (i / 4) + i % 4 < below ? s[kb][i] : -INFINITY;
+    }
     float top = max3(s[0][0], s[0][1], s[0][2]), top1 = max3(s[1][0], s[1][1], s[1][2]);
 #pragma unroll
     for (int i = 3; i < 15; i += 2) top = max3(top, s[0][i], s[0][i + 1]), top1 = max3(top1, s[1][i], s[1][i + 1]);
