@@ -134,24 +134,24 @@ __global__ __launch_bounds__(64 * WAVES, PREC ? 2 : 4) void long_kernel(dkv_page
   const int64_t grain = grain_bytes(a.plan.layers, H), sub = (int64_t)a.layer * 2 * H + h;
   // Rows of 16 bits go straight to their tile: a wave 8 rows of K and of V. New rows past the last one repeat it; rows of a
   // page that are not there are read as they are (zero_values).
-  auto load_tile = [&](int u, const Unit& x, int buf) {
-    const int thread = anew(t), srow = thread >> 3, piece = (thread & 7) ^ place(srow);
-    const uint8_t *k, *v;
-    uint32_t k_off = 16 * piece, v_off = 16 * piece;
-    if (u < w.n_pages) {
-      k = base + (x.page >> 2) * grain + sub * page_sub(16);
-      v = k + (int64_t)H * page_sub(16);
-      k_off += srow * 128, v_off += srow * 128;
-    } else {
-      const int64_t tok = w.token0 + (u - w.n_pages) * TILE;
-      const int r = min(srow, x.rows - 1);
-      k = static_cast<const uint8_t*>(a.k_new) + 2 * (h * a.kn_head_stride + tok * a.kn_tok_stride);
-      v = static_cast<const uint8_t*>(a.v_new) + 2 * (h * a.vn_head_stride + tok * a.vn_tok_stride);
-      k_off += __umul24(r, (uint32_t)(2 * a.kn_tok_stride)), v_off += __umul24(r, (uint32_t)(2 * a.vn_tok_stride));
-    }
+  auto load_rows = [&](const uint8_t* k, const uint8_t* v, int rows, uint32_t k_stride, uint32_t v_stride, int buf) {
+    const int thread = anew(t), srow = thread >> 3, piece = (thread & 7) ^ place(srow), r = min(srow, rows - 1);
     const uint32_t to = tile0 + buf * (2 * TILE_BYTES) + 1024 * wave;
-    load_piece_at(k, k_off, to);
-    load_piece_at(v, v_off, to + TILE_BYTES);
+    load_piece_at(k, 16 * piece + __umul24(r, k_stride), to);
+    load_piece_at(v, 16 * piece + __umul24(r, v_stride), to + TILE_BYTES);
+  };
+  const uint32_t kn_stride = (uint32_t)(2 * a.kn_tok_stride), vn_stride = (uint32_t)(2 * a.vn_tok_stride);  // (of a single row, whatever it is)
+  auto new_rows = [&](const void* x, int64_t head_stride, int64_t tok_stride, int u) {
+    return static_cast<const uint8_t*>(x) + 2 * (h * head_stride + ((int64_t)w.token0 + (u - w.n_pages) * TILE) * tok_stride);
+  };
+  auto load_tile = [&](int u, const Unit& x, int buf) {
+    if (u < w.n_pages) {
+      const uint8_t* k = base + (x.page >> 2) * grain + sub * page_sub(16);
+      load_rows(k, k + (int64_t)H * page_sub(16), TILE, 128, 128, buf);
+    } else {
+      load_rows(new_rows(a.k_new, a.kn_head_stride, a.kn_tok_stride, u), new_rows(a.v_new, a.vn_head_stride, a.vn_tok_stride, u), x.rows,
+                kn_stride, vn_stride, buf);
+    }
   };
   // Packed rows come as they are: at 8 bits a wave 1 KB of K (waves 0 to 3) or V, at 4 bits every other wave, and one wave
   // the (offset, scale) pairs.
@@ -257,6 +257,7 @@ __global__ __launch_bounds__(64 * WAVES, PREC ? 2 : 4) void long_kernel(dkv_page
   // to this lane's row, none from 32 on to any row of the wave where there is one half.
   auto attend = [&](auto packed_keys, int buf, bool masked, int high, bool one_half) {
     constexpr bool PACKED = decltype(packed_keys)::value;
+    constexpr int AHEAD = 4;  // operands of K under way
     const uint8_t* kt = &tiles[buf][0][0];
     const uint8_t* vt = &tiles[buf][1][0];
     f32x16 s[2];
@@ -265,14 +266,17 @@ __global__ __launch_bounds__(64 * WAVES, PREC ? 2 : 4) void long_kernel(dkv_page
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[kb][i] = 0.f;
     __builtin_amdgcn_s_setprio(1);  // (products before the other waves' exponentials: 0.7 %)
+    Op8 k[AHEAD];
+    auto load_k = [&](int i) { k[i % AHEAD].u = *reinterpret_cast<const u32x4*>(kt + (k_at ^ (32 * (i / 2))) + 4096 * (i % 2)); };
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks)
+    for (int i = 0; i < AHEAD; ++i) load_k(i);
+    __builtin_amdgcn_sched_barrier(0);  // (the compiler would read each operand right before its product)
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
-        Op8 k;
-        k.u = *reinterpret_cast<const u32x4*>(kt + (k_at ^ (32 * ks)) + 4096 * kb);
-        s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k.v, q[ks].v, s[kb], 0, 0, 0);
-      }
+    for (int i = 0; i < 8; ++i) {
+      s[i % 2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[i % AHEAD].v, q[i / 2].v, s[i % 2], 0, 0, 0);
+      if (i + AHEAD < 8) load_k(i + AHEAD);
+      __builtin_amdgcn_sched_barrier(0);
+    }
     __builtin_amdgcn_s_setprio(0);
     // max3 below is a statement of its own, before which the compiler does not wait for a matrix product's result: 19
     // states after one of 16 passes.
@@ -316,7 +320,13 @@ __global__ __launch_bounds__(64 * WAVES, PREC ? 2 : 4) void long_kernel(dkv_page
       if (TERMS > 1 && kb == 1 && one_half) break;  // (8 frames of 78 tokens, 3 terms: 102 us with it, 110 without; at 1 term 2 % slower)
 #pragma unroll
       for (int st = 0; st < 2; ++st) {  // 16 keys
-        Op8 p[TERMS];
+        Op8 p[TERMS], v[2];
+#pragma unroll
+        for (int db = 0; db < 2; ++db)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            v[db].h[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (__attribute__((address_space(3))) s16x4*)(vt + (v_at ^ (64 * db) ^ (32 * j)) + (32 * kb + 16 * st + 8 * j) * 128));
 #pragma unroll
         for (int j = 0; j < 8; j += 2) {
           float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][8 * st + j], xs, -mref));
@@ -336,15 +346,9 @@ __global__ __launch_bounds__(64 * WAVES, PREC ? 2 : 4) void long_kernel(dkv_page
           if (TERMS == 1) sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, x[0]), __builtin_bit_cast(bf16x2, 0x3f803f80u), sum, false);
         }
 #pragma unroll
-        for (int db = 0; db < 2; ++db) {
-          Op8 v;
+        for (int db = 0; db < 2; ++db)
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
-            v.h[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) s16x4*)(vt + (v_at ^ (64 * db) ^ (32 * j)) + (32 * kb + 16 * st + 8 * j) * 128));
-#pragma unroll
-          for (int k = TERMS - 1; k >= 0; --k) acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v.v, p[k].v, acc[db], 0, 0, 0);
-        }
+          for (int k = TERMS - 1; k >= 0; --k) acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[db].v, p[k].v, acc[db], 0, 0, 0);
       }
     }
     l_part += sum;
@@ -375,11 +379,14 @@ __global__ __launch_bounds__(64 * WAVES, PREC ? 2 : 4) void long_kernel(dkv_page
     buf = next;
   }
   const int m_new = min(wave0 + (anew(t) & 31), total - 1) / G;  // this lane's token again
+  const uint8_t* kn = new_rows(a.k_new, a.kn_head_stride, a.kn_tok_stride, u + 2);
+  const uint8_t* vn = new_rows(a.v_new, a.vn_head_stride, a.vn_tok_stride, u + 2);
   for (; u < w.u1; ++u) {  // new tokens: nothing to be unpacked
     const int next = buf + 1 == RING ? 0 : buf + 1, after = next + 1 == RING ? 0 : next + 1;
     const int first = (u - w.n_pages) * TILE;
     const bool more = u + 2 < w.u1;
-    if (more) load_tile(u + 2, Unit{16, min(TILE, w.count - first - 2 * TILE), 2, 0}, after);
+    if (more) load_rows(kn, vn, w.count - first - 2 * TILE, kn_stride, vn_stride, after);
+    kn += 2 * TILE * a.kn_tok_stride, vn += 2 * TILE * a.vn_tok_stride;
     if (first + TILE - 1 > first_token) zero_values(Unit{16, min(TILE, w.count - first), 0, 0}, tiles[buf][1], true);
     if (on && first <= m_last) attend(std::false_type(), buf, first + TILE - 1 > m_first, m_new + 1 - first, m_last - first < 32);
     step(more ? 2 : 0);
