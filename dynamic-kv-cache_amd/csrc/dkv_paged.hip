@@ -264,11 +264,12 @@ int launch_moves(const void* src, void* dst, const dkv_page_move* moves, int n_m
 // ---- plans -------------------------------------------------------------------------------------------------------
 
 // Entities of up to this many query rows of a KV head go to the kernel for few rows. (144 rows over 127 pages, 5 heads: 18.5 us
-// there, 29.0 in the kernel for many, which has few workgroups for them; 180 rows and more over 96 pages 46.1 and 44.7.)
+// there, 24.2 in the kernel for many, which has few workgroups for them; 16 questions of 15 to 180 rows about 96 pages 40.6 us by this
+// rule, 43.5 from 100 rows on, 40.9 from 200.)
 constexpr int SHORT_ROWS = 160;
 // Few rows (four waves, a unit each at a time): about SHORT_TARGET workgroups over all KV heads share a step's units, four
-// resident a CU, of SHORT_LEAST units at least (three short histories 8.0 us with 8, 11.6 with 4 and a join). A token of 64
-// streams / of 6 long ones: 1024 workgroups 34.3 / 110.6 us, 2048 31.8 / 105.9.
+// resident a CU, of SHORT_LEAST units at least (three short histories 8.4 us with 8, 12.1 with 4 and a join). A token of 64
+// streams / of 6 long ones: 1024 workgroups 34.3 / 113 us, 2048 31.7 / 106.
 constexpr int SHORT_TARGET = 2048, SHORT_LEAST = 8;
 // Many rows (eight waves, a unit at a time): a step is split into LONG_TARGET workgroups at most (two a CU) beside those that
 // its blocks need, of LONG_LEAST units at least, by ranges of such a length that the last workgroup ends first (long_share).
@@ -389,7 +390,8 @@ static int64_t share(int64_t total, int64_t target, int least) { return std::max
 // The same for many rows: of ranges from that length on, the one whose workgroups are done first when each free CU takes the
 // longest that is left (one workgroup keeps its vector units busy: two on a CU take twice as long). In units: a workgroup
 // costs its units and what its start takes, one that is joined its partial rows beside, and the join reads them. (Equal
-// shares for 512 workgroups and for 256: 12500 tokens of prompts 267 and 239 us, 12 prompts 82 and 68, 8 frames 131 and 172.)
+// shares for 512 workgroups and for 256: 12500 tokens of prompts 228 and 204 us, 12 prompts 73.8 and 59.4, 8 frames 99.5 and 108,
+// 16 questions 42.6 and 40.6; these 204, 59.4, 101 and 40.7.)
 static int64_t long_share(const std::vector<Entity>& es, int G, int heads, int groups, const std::vector<int>& group) {
   const int slots = std::max(1, CUS / heads);
   const int64_t least = share(total_units(es, G, true), ceil_div(LONG_TARGET, heads), LONG_LEAST);

@@ -11,11 +11,11 @@
 // Packed rows of unit u + 3 are asked for, and those of u + 1 unpacked, while u is multiplied; new and 16-bit rows come two units
 // ahead; one barrier a unit. Scores, statistics and sums are fp32. P is one bf16 value at precision and output bf16 (a relative 2^-8
 // of each weight, averaged over the keys; a sequence of few rows keeps two, see dkv_paged_attn.hip), else the sum of two or three.
-// What bounds it: the vector units, 187 instructions a unit and wave beside its 16 matrix products of 32 cycles, of them 32
-// exponentials of four times the cost: 12.5k tokens of prompts of 5 heads of 3 217 us (762 TFLOP/s, 58 % of a large product's), 12
-// prompts of up to 2048 tokens of 8 heads of 4 63 us (546); with few units a workgroup the chain from the plan to the first tile, 16
-// questions about 6144 shared tokens 32 us. At fp32 the split into three values and the scales apart, 527 instructions, and two
-// waves a SIMD, of whose time 38 % waits: 8 frames of 78 tokens over 92k 99 us.
+// What bounds it: the vector units, some 150 instructions a unit and wave beside its 16 matrix products of 32 cycles, of them 32
+// exponentials of twice the cost or more: 12.5k tokens of prompts of 5 heads of 3 205 us (806 TFLOP/s, 61 % of a large product's), 12
+// prompts of up to 2048 tokens of 8 heads of 4 59 us (580); with few units a workgroup the chain from the plan to the first tile, 16
+// questions about 6144 shared tokens 30 us. At fp32 the split into three values and the scales apart, 527 instructions, and two
+// waves a SIMD, of whose time 38 % waits: 8 frames of 78 tokens over 92k 95 us.
 #include <type_traits>
 
 #include "dkv_rows.h"
@@ -257,7 +257,7 @@ __global__ __launch_bounds__(64 * WAVES, PREC ? 2 : 4) void long_kernel(dkv_page
   // to this lane's row, none from 32 on to any row of the wave where there is one half.
   auto attend = [&](auto packed_keys, int buf, bool masked, int high, bool one_half) {
     constexpr bool PACKED = decltype(packed_keys)::value;
-    constexpr int AHEAD = 4;  // operands of K under way
+    constexpr int AHEAD = 4;  // operands of K under way (12.5k tokens of prompts 2: 224.4 us, 4: 223.5, 6: 225.2; 8 frames at fp32 101.1, 101.0, 104.4)
     const uint8_t* kt = &tiles[buf][0][0];
     const uint8_t* vt = &tiles[buf][1][0];
     f32x16 s[2];
@@ -317,7 +317,7 @@ __global__ __launch_bounds__(64 * WAVES, PREC ? 2 : 4) void long_kernel(dkv_page
     float sum = 0.f;
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
-      if (TERMS > 1 && kb == 1 && one_half) break;  // (8 frames of 78 tokens, 3 terms: 102 us with it, 110 without; at 1 term 2 % slower)
+      if (TERMS > 1 && kb == 1 && one_half) break;  // (8 frames of 78 tokens, 3 terms: 101 us with it, 109 without; at 1 term 2 % slower)
 #pragma unroll
       for (int st = 0; st < 2; ++st) {  // 16 keys
         Op8 p[TERMS], v[2];
