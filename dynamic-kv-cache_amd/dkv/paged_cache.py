@@ -70,6 +70,9 @@ class PagedCache:
         self._index = self.arena.get_device()
         self._arena_ptr = self.arena.data_ptr()
 
+    def __reduce_ex__(self, protocol):
+        raise TypeError('a PagedCache cannot be copied or pickled: fork its sequences')
+
     def _launch(self, what, call):
         """call(stream) on this cache's device and torch's current stream there."""
         index = self._index

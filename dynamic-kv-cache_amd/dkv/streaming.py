@@ -527,7 +527,8 @@ class StreamingDecoder:
         it. The branches take pages for a question and its tokens, and end with the call. With graphs=True the
         forwards of more than GRAPH_TOKENS tokens are replays of a captured one from the third token's on, and the call
         waits for the GPU."""
-        seqs, questions = [seqs] * len(questions) if isinstance(seqs, int) else list(seqs), list(questions)
+        questions = list(questions)
+        seqs = list(seqs) if hasattr(seqs, '__len__') else [seqs] * len(questions)
         if len(seqs) != len(questions) or u.dim() != 2 or u.shape[0] != len(questions):
             raise ValueError(f'generate_batch expects a sequence and random numbers u [questions, n] for each question, got '
                              f'{len(seqs)} and {list(u.shape)} for {len(questions)}')

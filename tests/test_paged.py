@@ -1,5 +1,7 @@
 """PagedCache bookkeeping, plans and refusals on the CPU (device='cpu' arenas; no kernel runs)."""
+import copy
 import ctypes
+import pickle
 
 import numpy as np
 import pytest
@@ -231,6 +233,14 @@ def test_refusals():
     with pytest.raises(ValueError, match='CUDA'):
         c = PagedCache(1, 1, 1, device='cpu')
         c.step(c.add())
+
+
+def test_caches_are_not_copied():
+    c = Quiet(1, 1, 1)
+    step = c.step(c.add())
+    for call, x in ((copy.copy, c), (copy.deepcopy, c), (pickle.dumps, c), (copy.deepcopy, step), (pickle.dumps, step)):
+        with pytest.raises(TypeError, match='copied'):
+            call(x)
 
 
 def test_pools_refuse_null_and_foreign_tables():
