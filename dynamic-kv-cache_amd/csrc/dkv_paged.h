@@ -1,5 +1,5 @@
-// Paged caches (dkv_paged.hip: plans, pack, read, move; dkv_paged_attn.hip: attention): the page layout, and what a
-// step's plan holds in device memory.
+// Paged caches (dkv_paged.hip: plans, pack, read, move; dkv_paged_attn.hip, dkv_paged_short.h, dkv_paged_prompt.hip: attention): the
+// page layout, and what a step's plan holds in device memory.
 #pragma once
 #include "dkv_common.h"
 
@@ -58,7 +58,7 @@ __device__ __forceinline__ T plan_record(const int32_t* plan, int at, int i) {
   return x.t;
 }
 
-constexpr int SHORT_BLOCK = 16;  // query rows of a block of the kernel for few rows (dkv_paged_attn.hip)
+constexpr int SHORT_BLOCK = 16;  // query rows of a block of the kernel for few rows (dkv_paged_short.h)
 constexpr int LONG_BLOCK = 256;  // of the one for many (dkv_paged_prompt.hip)
 
 // Four elements of an output row.
@@ -71,7 +71,8 @@ __device__ __forceinline__ void store4(void* out, int out_dtype, int64_t at, flo
 
 __device__ __forceinline__ bool bad_bf16(uint32_t half) { return (half & 0x7f80u) == 0x7f80u; }  // infinite or NaN
 
-void launch_long(const dkv_paged_args& a, int work, float* part_o, float2* part_ml, hipStream_t s);
+// The launch of many query rows, with workgroups of few ones behind it.
+void launch_long(const dkv_paged_args& a, int n_long, int n_short, float* part_o, float2* part_ml, hipStream_t s);
 
 int check_args(const dkv_paged_args& a, bool attend, const char* what);
 

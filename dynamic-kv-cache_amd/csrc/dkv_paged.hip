@@ -264,8 +264,8 @@ int launch_moves(const void* src, void* dst, const dkv_page_move* moves, int n_m
 // ---- plans -------------------------------------------------------------------------------------------------------
 
 // Entities of up to this many query rows of a KV head go to the kernel for few rows. (144 rows over 127 pages, 5 heads: 18.5 us
-// there, 24.2 in the kernel for many, which has few workgroups for them; 16 questions of 15 to 180 rows about 96 pages 40.6 us by this
-// rule, 43.5 from 100 rows on, 40.9 from 200.)
+// there, 24.2 in the kernel for many, which has few workgroups for them; 16 questions of 15 to 180 rows about 96 pages, few rows in a
+// launch of their own, 40.6 us by this rule, 43.5 from 100 rows on, 40.9 from 200.)
 constexpr int SHORT_ROWS = 160;
 // Few rows (four waves, a unit each at a time): about SHORT_TARGET workgroups over all KV heads share a step's units, four
 // resident a CU, of SHORT_LEAST units at least (three short histories 8.4 us with 8, 12.1 with 4 and a join). A token of 64
@@ -358,7 +358,7 @@ static int check_plan(const dkv_paged_batch& b, const char* what) {
   if (fits) {
     dkv_paged_plan p{};
     layout_of(b, p);
-    const int64_t threads = std::max<int64_t>({2ll * p.max_items, (int64_t)p.max_work * b.heads, 2ll * p.max_long * b.heads,
+    const int64_t threads = std::max<int64_t>({2ll * p.max_items, (int64_t)p.max_work * b.heads, 2ll * (p.max_long + p.max_work) * b.heads,
                                       (int64_t)p.max_merges * (SHORT_BLOCK / 4) * b.heads}) * 256;
     fits = threads <= UINT32_MAX;
   }
@@ -391,7 +391,7 @@ static int64_t share(int64_t total, int64_t target, int least) { return std::max
 // longest that is left (one workgroup keeps its vector units busy: two on a CU take twice as long). In units: a workgroup
 // costs its units and what its start takes, one that is joined its partial rows beside, and the join reads them. (Equal
 // shares for 512 workgroups and for 256: 12500 tokens of prompts 228 and 204 us, 12 prompts 73.8 and 59.4, 8 frames 99.5 and 108,
-// 16 questions 42.6 and 40.6; these 204, 59.4, 101 and 40.7.)
+// 16 questions 42.6 and 40.6; these 204, 59.4, 101 and 40.7, all with few rows in a launch of their own.)
 static int64_t long_share(const std::vector<Entity>& es, int G, int heads, int groups, const std::vector<int>& group) {
   const int slots = std::max(1, CUS / heads);
   const int64_t least = share(total_units(es, G, true), ceil_div(LONG_TARGET, heads), LONG_LEAST);
@@ -519,7 +519,7 @@ static int write_plan(const dkv_paged_batch& b, int32_t* w, dkv_paged_plan& p) {
   Work* const long_work = reinterpret_cast<Work*>(w + p.at_long);
   Merge* merges = reinterpret_cast<Merge*>(w + p.at_merges);
   int n_work = 0, n_long = 0, n_merges = 0;
-  int64_t rows = 0;  // partial rows so far
+  int64_t rows = 0, few_units = 0;  // partial rows so far; units of few query rows
   for (int i = 0; i < (int)all.size(); ++i) {
     Entity& e = all[i];
     const int64_t total = (int64_t)e.count * G;
@@ -532,6 +532,7 @@ static int write_plan(const dkv_paged_batch& b, int32_t* w, dkv_paged_plan& p) {
       // a group's partial rows lie split after split, as its sequences' rows are not cut where its blocks are
       const int64_t first = e.group ? e.part + (int64_t)blk * block : rows, stride = e.group ? total : here;
       const bool parts = joined || splits > 1;
+      if (!is_many) few_units += units;
       for (int s = 0; s < splits; ++s)
         (is_many ? long_work[n_long++] : work[n_work++]) =
             Work{e.first_page, e.n4, e.n8, e.n_pages, e.token0, e.count, blk, (int)((int64_t)units * s / splits),
@@ -551,6 +552,7 @@ static int write_plan(const dkv_paged_batch& b, int32_t* w, dkv_paged_plan& p) {
   auto longer = [](const Work& x, const Work& y) { return x.u1 - x.u0 > y.u1 - y.u0; };
   std::stable_sort(long_work, long_work + n_long, longer);  // (the longest first, so that none of them is left for the end)
   p.items = n_items, p.work = n_work, p.long_work = n_long, p.merges = n_merges, p.rows = (int)rows;
+  p.units = (int)std::min<int64_t>(few_units, INT32_MAX);
   w[N_ITEMS] = n_items, w[N_WORK] = n_work, w[N_LONG] = n_long, w[N_MERGES] = n_merges;
   return 0;
 }

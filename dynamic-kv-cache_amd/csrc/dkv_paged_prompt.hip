@@ -10,16 +10,15 @@
 //
 // Packed rows of unit u + 3 are asked for, and those of u + 1 unpacked, while u is multiplied; new and 16-bit rows come two units
 // ahead; one barrier a unit. Scores, statistics and sums are fp32. P is one bf16 value at precision and output bf16 (a relative 2^-8
-// of each weight, averaged over the keys; a sequence of few rows keeps two, see dkv_paged_attn.hip), else the sum of two or three.
+// of each weight, averaged over the keys; a sequence of few rows keeps two, dkv_paged_short.h), else the sum of two or three.
 // What bounds it: the vector units, some 150 instructions a unit and wave beside its 16 matrix products of 32 cycles, of them 32
 // exponentials of twice the cost or more: 12.5k tokens of prompts of 5 heads of 3 205 us (806 TFLOP/s, 61 % of a large product's), 12
-// prompts of up to 2048 tokens of 8 heads of 4 59 us (580); with few units a workgroup the chain from the plan to the first tile, 16
-// questions about 6144 shared tokens 30 us. At fp32 the split into three values and the scales apart, 527 instructions, and two
+// prompts of up to 2048 tokens of 8 heads of 4 55 us (631); with few units a workgroup the chain from the plan to the first tile, 16
+// questions about 6144 shared tokens 27 us. At fp32 the split into three values and the scales apart, 527 instructions, and two
 // waves a SIMD, of whose time 38 % waits: 8 frames of 78 tokens over 92k 95 us.
 #include <type_traits>
 
-#include "dkv_rows.h"
-#include "dkv_paged.h"
+#include "dkv_paged_short.h"
 
 namespace dkv {
 namespace paged {
@@ -93,14 +92,20 @@ __device__ __forceinline__ int anew(int x) {
   return x;
 }
 
-template <int PREC, int TERMS>
-__global__ __launch_bounds__(64 * WAVES, PREC ? 2 : 4) void long_kernel(dkv_paged_args a, float* part_o, float2* part_ml) {
+// Workgroups behind the first n_long records' take those of few query rows, in the first half of their threads.
+template <int PREC, int TERMS, int FEW_TERMS>
+__global__ __launch_bounds__(64 * WAVES, PREC ? 2 : 4) void long_kernel(dkv_paged_args a, int n_long, float* part_o, float2* part_ml) {
   __shared__ __attribute__((aligned(1024))) uint8_t tiles[RING][2][TILE_BYTES];
   __shared__ __attribute__((aligned(1024))) uint8_t packed_rows[RING][RAW_BYTES];
   __shared__ __attribute__((aligned(16))) float2 scales[PREC ? RING : 1][2][PREC ? TILE : 1];  // {offset + scale * centre, scale}
   __shared__ int bad;  // a new value that is infinite or NaN was taken for zero
   const int32_t* plan = static_cast<const int32_t*>(a.plan_words);
   const int H = a.plan.heads, G = a.plan.q_heads / H, record = blockIdx.x / H, h = blockIdx.x % H;
+  if (record >= n_long) {
+    static_assert(sizeof(few::ShortShared) <= sizeof(tiles), "in the tiles' place");
+    if (threadIdx.x < 256) few::short_rows<PREC, FEW_TERMS>(a, part_o, part_ml, blockIdx.x - n_long * H, *reinterpret_cast<few::ShortShared*>(&tiles[0][0][0]));
+    return;
+  }
   if (a.bounds && record >= plan[N_LONG]) return;
   const Work w = plan_record<Work>(plan, a.plan.at_long, record);
   const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, c = lane & 31, half = lane >> 5;
@@ -455,10 +460,10 @@ __global__ __launch_bounds__(64 * WAVES, PREC ? 2 : 4) void long_kernel(dkv_page
   }
 }
 
-void launch_long(const dkv_paged_args& a, int work, float* part_o, float2* part_ml, hipStream_t s) {
-  const auto kernel = a.precision == 1 ? (a.out_dtype == 1 ? long_kernel<1, 3> : long_kernel<1, 2>)
-                                       : (a.out_dtype == 1 ? long_kernel<0, 3> : long_kernel<0, 1>);
-  hipLaunchKernelGGL(kernel, dim3(work * a.plan.heads), dim3(64 * WAVES), 0, s, a, part_o, part_ml);
+void launch_long(const dkv_paged_args& a, int n_long, int n_short, float* part_o, float2* part_ml, hipStream_t s) {
+  const auto kernel = a.precision == 1 ? (a.out_dtype == 1 ? long_kernel<1, 3, 3> : long_kernel<1, 2, 3>)
+                                       : (a.out_dtype == 1 ? long_kernel<0, 3, 3> : long_kernel<0, 1, 2>);
+  hipLaunchKernelGGL(kernel, dim3((n_long + n_short) * a.plan.heads), dim3(64 * WAVES), 0, s, a, n_long, part_o, part_ml);
 }
 
 }  // namespace paged

@@ -101,7 +101,7 @@ class PoolInfo(ctypes.Structure):
 class PagedPlan(ctypes.Structure):
     _fields_ = [(name, ctypes.c_int32) for name in (
         'seqs', 'tokens', 'layers', 'heads', 'q_heads', 'grains', 'words', 'at_items', 'at_positions', 'at_pages', 'at_work', 'at_long',
-        'at_merges', 'items', 'work', 'long_work', 'merges', 'rows', 'max_items', 'max_pages', 'max_work', 'max_long', 'max_merges',
+        'at_merges', 'items', 'work', 'long_work', 'merges', 'rows', 'units', 'max_items', 'max_pages', 'max_work', 'max_long', 'max_merges',
         'max_rows')]
 
 

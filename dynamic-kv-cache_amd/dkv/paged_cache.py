@@ -67,6 +67,7 @@ class PagedCache:
         weakref.finalize(self, _lib.load().dkv_pool_destroy, self._pool)
         with torch.inference_mode(False):
             self.arena = torch.empty(self.arena_bytes, dtype=torch.uint8, device=self.device)
+        self.device = self.arena.device  # (with its index, whatever the current device is later)
         self._index = self.arena.get_device()
         self._arena_ptr = self.arena.data_ptr()
 
@@ -86,8 +87,15 @@ class PagedCache:
         if rc:
             _lib.check(rc, what)
 
+    def _captured(self):
+        """Whether the current stream of this cache's device records a graph."""
+        if self._index < 0 or torch.cuda.current_device() == self._index:
+            return self._index >= 0 and torch.cuda.is_current_stream_capturing()
+        with torch.cuda.device(self._index):
+            return torch.cuda.is_current_stream_capturing()
+
     def _not_captured(self, what):
-        if self._index >= 0 and torch.cuda.is_current_stream_capturing():
+        if self._captured():
             raise ValueError(f'{what} cannot run while a graph is captured')
 
     # -- sequences -------------------------------------------------------------
@@ -368,7 +376,7 @@ class PagedStep(_CacheBase):
 
     def captured(self):
         """Whether launches are being recorded, which then are sized for every plan that advance() may write."""
-        return int(torch.cuda.is_current_stream_capturing())
+        return int(self.cache._captured())
 
     def workspace_bytes(self, bounds):
         need = self._needs.get(bounds)

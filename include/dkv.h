@@ -537,6 +537,7 @@ typedef struct dkv_paged_plan {
   int32_t words;  /* of the whole plan */
   int32_t at_items, at_positions, at_pages, at_work, at_long, at_merges;
   int32_t items, work, long_work, merges, rows;
+  int32_t units; /* of 64 keys that `work` takes */
   int32_t max_items, max_pages, max_work, max_long, max_merges, max_rows;
 } dkv_paged_plan;
 

@@ -340,3 +340,16 @@ def test_nothing_to_read(cuda):
     pages.free([])
     step = pages.step(seq, 3)
     assert pages.materialize(0, seq, first=3)[0].shape == (1, 1, 0, 64) and step.positions.tolist() == [0, 1, 2]
+
+
+@pytest.mark.parametrize('precision,out', [('bf16', torch.bfloat16), ('fp32', torch.float32), ('fp32', torch.bfloat16), ('bf16', torch.float32)])
+def test_prompts_beside_long_histories(cuda, precision, out):
+    """Single tokens of long and short histories beside prompts: at fp32 too many units for one launch, at bf16 not, and few of them at
+    both."""
+    announce(f'prompts beside long histories {precision} {out}')
+    m = Model(2, 6, precision, max_tokens=1 << 17, seed=11)
+    seqs = [m.add() for _ in range(6)]
+    m.step(seqs[:3], [40000, 30000, 20000], [4, 8, 4])
+    m.step(seqs[3:5], [70, 200], 16)
+    m.attend(seqs, [1, 2, 1, 100, 3, 300], 16, out)
+    m.attend(seqs[3:], [90, 1, 2], 4, out)
