@@ -578,7 +578,7 @@ typedef struct dkv_paged_args {
 int dkv_paged_append(const dkv_paged_args* args, void* stream);
 /* The joined Q/K/V projection [tokens, (q_heads + 2 heads) * 64] of a step's tokens, split and with RoPE from cos / sin rows
  * [tokens, 64] as dkv_rope_qkv computes it, into q, k_new and v_new, which here are written, with their strides (no two of their
- * rows may share memory), and K and V packed as dkv_paged_append packs them. All bf16, 16-byte aligned, strides in multiples of 8
+ * rows may share memory, nor any with the inputs), and K and V packed as dkv_paged_append packs them. All bf16, 16-byte aligned, strides in multiples of 8
  * elements. No counterpart in the reference (src/gpu_cache.py:164-172 is the same of one sequence). */
 int dkv_paged_rope_append(const dkv_paged_args* args, const void* qkv, int64_t qkv_row_stride, const void* cos, const void* sin,
                           int64_t cs_row_stride, void* stream);
@@ -586,7 +586,7 @@ int dkv_paged_rope_append(const dkv_paged_args* args, const void* qkv, int64_t q
 /* The step's new tokens attend, each to its sequence's history before the step and to the sequence's new tokens up to
  * itself (these as they are in k_new and v_new). What later tokens hold, NaN and infinities included, does not reach
  * a query. Q, K and V must be 16-byte aligned with strides in multiples of 8 elements; out 16-byte aligned with
- * strides in multiples of 4 elements. */
+ * strides in multiples of 4 elements, in memory of its own. */
 int64_t dkv_paged_workspace_bytes(const dkv_paged_args* args);
 int dkv_paged_attend(const dkv_paged_args* args, void* stream);
 
@@ -624,8 +624,8 @@ int dkv_pool_destroy(dkv_pool* pool);
 int dkv_pool_info_get(dkv_pool* pool, dkv_pool_info* info);
 /* Where the pool keeps its generation, for as long as it lives. */
 int dkv_pool_generation(dkv_pool* pool, const int64_t** at);
-/* A sequence's tokens (-1 for an error); these, tokens dropped before them (its next position is their sum) and pages; the pages' names, tokens
- * and numbers of sequences that hold them, into arrays with room for `room`. */
+/* A sequence's tokens (-1 for an error); these, tokens dropped before them (its next position is their sum) and pages; the
+ * pages' names, tokens and numbers of sequences that hold them, into arrays with room for `room`. */
 int64_t dkv_pool_length(dkv_pool* pool, int64_t seq);
 int dkv_pool_sequence(dkv_pool* pool, int64_t seq, int64_t* length, int64_t* dropped, int32_t* pages);
 int dkv_pool_pages(dkv_pool* pool, int64_t seq, int32_t room, uint32_t* page, int32_t* rows, int32_t* holders);
