@@ -146,13 +146,14 @@ __global__ __launch_bounds__(256) void rope_append_kernel(dkv_paged_args a, cons
 
 // ---- pages read back ---------------------------------------------------------------------------------------------
 
-constexpr int ARG_ITEMS = 128;  // records of a launch's argument block
+constexpr int ARG_ITEMS = 224;  // records of a launch's argument block, of less than 4 KB
 struct Items {
   dkv_page_rows at[ARG_ITEMS];
 };
 
 // Rows of a page as values code * s + a, 8 lanes a row (lane c: elements [8 c, 8 c + 8)): every store of bf16 writes whole lines.
-// Bound by its bytes: 8138 tokens of 8 layers of 5 heads, 131 MB read and written, 31 us in two launches (4.2 TB/s).
+// Bound by its bytes: 8138 tokens of 8 layers of 5 heads, 131 MB read and written, 25.5 us (5.1 TB/s; in launches of 128 records
+// 31).
 template <int BITS>
 __device__ __forceinline__ void read_rows(const uint8_t* sub, int row0, int rows, int r0, int c, void* out, int64_t at, int out_dtype) {
   constexpr int AHEAD = 4;
@@ -210,14 +211,14 @@ __global__ __launch_bounds__(256) void read_kernel(Items items, const uint8_t* _
 
 // ---- rows moved --------------------------------------------------------------------------------------------------
 
-constexpr int ARG_MOVES = 128;
+constexpr int ARG_MOVES = 160;
 struct Moves {
   dkv_page_move at[ARG_MOVES];
 };
 
 // One sub-block's rows: the payload in 16-byte pieces, then the (offset, scale) pairs, which lie behind as many rows as
-// the tile has room for. All loads before the first store. Bound by its bytes: the same history gathered into pages, 96 MB, 18 us in
-// two launches (5.3 TB/s, a large copy's rate).
+// the tile has room for. All loads before the first store. Bound by its bytes: the same history gathered into pages, 96 MB, some 25 us
+// in two launches, of 160 and 100 moves (3.9 TB/s).
 template <int BITS>
 __device__ __forceinline__ void move_rows(const dkv_page_move& m, const uint8_t* from, uint8_t* to, int lane) {
   constexpr int ROW = 8 * BITS, PIECES = BITS / 2;  // bytes; of 64 rows, a lane's pieces

@@ -30,6 +30,7 @@ except Exception:
     _CacheBase = object
 
 BLOCK, BLOCK_TOKENS = 48, 3 * TILE  # grains of a block of pages; tokens that it holds at 16 bits
+IDS = 1 << 62  # sequences' names are below
 _PLAN_BYTES = ctypes.sizeof(_lib.PagedPlan)
 _ARGS = struct.Struct(f'PqqPqqPqqPqP{_PLAN_BYTES}siifPqqiiPq')  # dkv_paged_args, with the plan as bytes
 assert _ARGS.size == ctypes.sizeof(_lib.PagedArgs)
@@ -64,6 +65,7 @@ class PagedCache:
         at = ctypes.c_void_p()
         _lib.check(_lib.load().dkv_pool_generation(self._pool, ctypes.byref(at)), 'dkv_pool_generation')
         self._generation = ctypes.c_int64.from_address(at.value)  # counts the calls that freed, cut or moved pages
+        self._length = _lib.load().dkv_pool_length
         weakref.finalize(self, _lib.load().dkv_pool_destroy, self._pool)
         with torch.inference_mode(False):
             self.arena = torch.empty(self.arena_bytes, dtype=torch.uint8, device=self.device)
@@ -103,13 +105,19 @@ class PagedCache:
     def _ids(seqs):
         """(array, number) of the ids of one or several sequences."""
         seqs = [seqs] if isinstance(seqs, (int, np.integer)) else list(seqs)
-        if not all(isinstance(s, (int, np.integer)) and 0 <= s < 1 << 62 for s in seqs):
+        ints = set(map(type, seqs)) <= {int} or all(isinstance(s, (int, np.integer)) for s in seqs)
+        if not ints or seqs and not 0 <= min(seqs) <= max(seqs) < IDS:
             raise ValueError(f'sequences are named by the ints of add(), adopt() and fork(), got {seqs!r}')
         return (ctypes.c_int64 * len(seqs))(*seqs), len(seqs)
 
     @staticmethod
     def _each(x, n, what):
-        x = [x] * n if isinstance(x, (int, np.integer)) else [int(v) for v in x]
+        if isinstance(x, (int, np.integer)):
+            x = [int(x)] * n
+        else:
+            x = list(x)
+            if not set(map(type, x)) <= {int}:
+                x = [int(v) for v in x]
         if len(x) != n:
             raise ValueError(f'one {what} a sequence: {len(x)} for {n}')
         if x and not -1 << 31 <= min(x) <= max(x) < 1 << 31:
@@ -133,9 +141,9 @@ class PagedCache:
 
     def length(self, seq):
         """Tokens that a sequence holds, those of steps that were planned among them."""
-        if not isinstance(seq, (int, np.integer)) or not 0 <= seq < 1 << 62:
+        if type(seq) is not int or not 0 <= seq < IDS:
             self._ids([seq])
-        n = _lib.load().dkv_pool_length(self._pool, seq)
+        n = self._length(self._pool, seq)
         if n < 0:
             _lib.check(_lib.DKV_EINVAL, 'dkv_pool_length')
         return n
@@ -191,7 +199,7 @@ class PagedCache:
     def truncate(self, seq, length):
         """Drops a sequence's tokens from `length` on."""
         (seq,), _ = self._ids([seq])
-        if not 0 <= length < 1 << 62:
+        if not 0 <= length < IDS:
             raise ValueError(f'truncate: a sequence cannot hold {length} tokens')
         self._not_captured('truncate')
         self._launch('dkv_pool_truncate', lambda stream: _lib.load().dkv_pool_truncate(self._pool, seq, length, self._arena_ptr, stream))
