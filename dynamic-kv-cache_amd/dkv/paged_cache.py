@@ -76,28 +76,36 @@ class PagedCache:
     def __reduce_ex__(self, protocol):
         raise TypeError('a PagedCache cannot be copied or pickled: fork its sequences')
 
-    def _launch(self, what, call):
+    def _stream(self):
+        """Torch's current stream on this cache's device."""
+        return _lib.raw_stream(self._index) if self._index >= 0 else 0
+
+    def _launch(self, what, call, stream=None):
         """call(stream) on this cache's device and torch's current stream there."""
         index = self._index
         if index < 0:
             raise ValueError(f'{what}: PagedCache requires a CUDA device')
+        if stream is None:
+            stream = _lib.raw_stream(index)
         if torch.cuda.current_device() == index:
-            rc = call(_lib.raw_stream(index))
+            rc = call(stream)
         else:
             with torch.cuda.device(index):
-                rc = call(_lib.raw_stream(index))
+                rc = call(stream)
         if rc:
             _lib.check(rc, what)
 
-    def _captured(self):
-        """Whether the current stream of this cache's device records a graph."""
-        if self._index < 0 or torch.cuda.current_device() == self._index:
-            return self._index >= 0 and torch.cuda.is_current_stream_capturing()
+    def _captured(self, stream):
+        """Whether the current stream of this cache's device records a graph (the default one, 0, never does)."""
+        if not stream:
+            return 0
+        if torch.cuda.current_device() == self._index:
+            return int(torch.cuda.is_current_stream_capturing())
         with torch.cuda.device(self._index):
-            return torch.cuda.is_current_stream_capturing()
+            return int(torch.cuda.is_current_stream_capturing())
 
     def _not_captured(self, what):
-        if self._captured():
+        if self._captured(self._stream()):
             raise ValueError(f'{what} cannot run while a graph is captured')
 
     # -- sequences -------------------------------------------------------------
@@ -255,9 +263,10 @@ class PagedCache:
         self._check('append', step, layer, ((k, self.heads), (v, self.heads)))
         k, kp, ks = GPUCache._rows(k)
         v, vp, vs = GPUCache._rows(v)
-        args = _ARGS.pack(0, 0, 0, kp, ks[1], ks[2], vp, vs[1], vs[2], self._arena_ptr, self.arena_bytes, step.device_plan(),
-                          step.plan_bytes, layer, step.captured(), 0.0, 0, 0, 0, 0, 0, 0, 0)
-        self._launch('dkv_paged_append', lambda stream: _lib.load().dkv_paged_append(args, stream))
+        stream = self._stream()
+        args = _ARGS.pack(0, 0, 0, kp, ks[1], ks[2], vp, vs[1], vs[2], self._arena_ptr, self.arena_bytes, step.device_plan(stream),
+                          step.plan_bytes, layer, self._captured(stream), 0.0, 0, 0, 0, 0, 0, 0, 0)
+        self._launch('dkv_paged_append', lambda stream: _lib.load().dkv_paged_append(args, stream), stream)
 
     def attend(self, q, k, v, layer, step, out_dtype=None, precision=None):
         """Causal attention of the step's tokens, q [1, q_heads, tokens, 64], each over its sequence's history and the
@@ -274,13 +283,14 @@ class PagedCache:
         k, kp, ks = GPUCache._rows(k)
         v, vp, vs = GPUCache._rows(v)
         out = q.new_empty((1, step.tokens, self.q_heads, self.dim), dtype=out_dtype)
-        bounds = step.captured()
+        stream = self._stream()
+        bounds = self._captured(stream)
         need = step.workspace_bytes(bounds)
         ws = self.arena.new_empty(need) if need else None
-        args = _ARGS.pack(qp, qs[1], qs[2], kp, ks[1], ks[2], vp, vs[1], vs[2], self._arena_ptr, self.arena_bytes, step.device_plan(),
+        args = _ARGS.pack(qp, qs[1], qs[2], kp, ks[1], ks[2], vp, vs[1], vs[2], self._arena_ptr, self.arena_bytes, step.device_plan(stream),
                           step.plan_bytes, layer, bounds, self.dim ** -0.5, out.data_ptr(), self.q_heads * self.dim, self.dim,
                           out_dtype is torch.float32, PRECISIONS[precision], ws.data_ptr() if need else 0, need)
-        self._launch('dkv_paged_attend', lambda stream: _lib.load().dkv_paged_attend(args, stream))
+        self._launch('dkv_paged_attend', lambda stream: _lib.load().dkv_paged_attend(args, stream), stream)
         return out
 
     def materialize(self, layer, seqs, first=0, out_dtype=torch.bfloat16):
@@ -362,7 +372,7 @@ class PagedStep(_CacheBase):
         self.positions = self._dev[at:at + 8 * self.tokens].view(torch.int64)
         self._needs = {}
         if self._stream is not None:
-            self.device_plan()  # (it was copied on the stream of now)
+            self.device_plan(cache._stream())  # (it was copied on the stream of now)
 
     def advance(self):
         """Plans the same sequences' next tokens, as many of each and at the same widths, in place of this step's. The
@@ -376,15 +386,11 @@ class PagedStep(_CacheBase):
         """The step's rows and the pages they go to (dkv_page_rows), on the host: (address, number)."""
         return self._host.data_ptr() + 4 * self.plan.at_items, self.plan.items
 
-    def device_plan(self):
-        stream = _lib.raw_stream(self.cache.device)
+    def device_plan(self, stream):
+        """The plan's address, for launches on `stream`, the current one."""
         if stream != self._stream:  # (its memory is not given out again before that stream is done with it)
             self._dev.record_stream(torch.cuda.current_stream(self.cache.device))
         return self._dev.data_ptr()
-
-    def captured(self):
-        """Whether launches are being recorded, which then are sized for every plan that advance() may write."""
-        return int(self.cache._captured())
 
     def workspace_bytes(self, bounds):
         need = self._needs.get(bounds)
@@ -408,11 +414,11 @@ class PagedStep(_CacheBase):
         if cos.stride() != sin.stride() or any(t.stride(-1) != 1 or t.stride(0) % 8 or t.data_ptr() % 16 for t in (qkv, cos, sin)):
             return None
         q, k, v = (qkv.new_empty((1, heads, n, c.dim)) for heads in (q_heads, c.heads, c.heads))
-        head = n * c.dim
+        head, stream = n * c.dim, c._stream()
         args = _ARGS.pack(q.data_ptr(), head, c.dim, k.data_ptr(), head, c.dim, v.data_ptr(), head, c.dim, c._arena_ptr, c.arena_bytes,
-                          self.device_plan(), self.plan_bytes, layer, self.captured(), 0.0, 0, 0, 0, 0, 0, 0, 0)
+                          self.device_plan(stream), self.plan_bytes, layer, c._captured(stream), 0.0, 0, 0, 0, 0, 0, 0, 0)
         c._launch('dkv_paged_rope_append', lambda stream: _lib.load().dkv_paged_rope_append(
-            args, qkv.data_ptr(), qkv.stride(0), cos.data_ptr(), sin.data_ptr(), cos.stride(0), stream))
+            args, qkv.data_ptr(), qkv.stride(0), cos.data_ptr(), sin.data_ptr(), cos.stride(0), stream), stream)
         return q, k, v, 0
 
     def _fused_attention(self, n, q_heads, layer, project, cos, sin, cs_stride, qkv_out, out, stream):
@@ -424,14 +430,15 @@ class PagedStep(_CacheBase):
             raise ValueError('attend: pages were freed, cut or moved since this step was planned')
         if n != self.tokens or q_heads != c.q_heads or layer >= c.layers:
             raise ValueError(f'a step of {self.tokens} tokens and {c.q_heads} query heads in {c.layers} layers got {n} and {q_heads} in layer {layer}')
-        H, lib, bounds = c.heads, _lib.load(), self.captured()
+        H, lib, here = c.heads, _lib.load(), c._stream()
+        bounds = c._captured(here)
         x, x_stride, weight, w_stride, _, k, norm, eps, layout = project
         width = (q_heads + 2 * H) * d
         need = self.workspace_bytes(bounds)
         ws = c.arena.new_empty(max(need, 2 * n * width))  # (the projection's rows are done with before the attention starts)
         at, kp = ws.data_ptr(), qkv_out + q_heads * n * d * 2
         vp, head = kp + H * n * d * 2, n * d
-        args = _ARGS.pack(qkv_out, head, d, kp, head, d, vp, head, d, c._arena_ptr, c.arena_bytes, self.device_plan(), self.plan_bytes,
+        args = _ARGS.pack(qkv_out, head, d, kp, head, d, vp, head, d, c._arena_ptr, c.arena_bytes, self.device_plan(here), self.plan_bytes,
                           layer, bounds, d ** -0.5, out, q_heads * d, d, 0, PRECISIONS[c.precision], at if need else 0, need)
         rc = (lib.dkv_linear_tiled(x, x_stride, weight, w_stride, n, width, k, norm, eps, 0, None, 0, at, width, layout, stream)
               or lib.dkv_paged_rope_append(args, at, width, cos, sin, cs_stride, stream) or lib.dkv_paged_attend(args, stream))

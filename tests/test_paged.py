@@ -19,7 +19,7 @@ class Quiet(PagedCache):
         super().__init__(*a, device='cpu', **kw)
         self._arena_ptr = None
 
-    def _launch(self, what, call):
+    def _launch(self, what, call, stream=None):
         _lib.check(call(None), what)
 
 
