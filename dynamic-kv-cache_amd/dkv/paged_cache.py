@@ -318,7 +318,7 @@ class PagedCache:
         else:
             self._launch('dkv_pool_read', lambda stream: _lib.load().dkv_pool_read(
                 self._pool, count, ids, first, layer0, layers, self._arena_ptr, out.data_ptr(), n, fp32, stream))
-        return out[0], out[1]
+        return out.unbind(0)
 
 
 class PagedStep(_CacheBase):
