@@ -107,8 +107,7 @@ int dkv_paged_attend(const dkv_paged_args* args, void* stream) {
   float* part_o = static_cast<float*>(a.workspace);
   float2* part_ml = reinterpret_cast<float2*>(static_cast<char*>(a.workspace) + up256(4 * D * rows));
   const int work = a.bounds ? p.max_work : p.work, merges = a.bounds ? p.max_merges : p.merges;
-  // (At precision 1 a weight meets codes of up to 255 whose offset comes apart: two terms would be off by 2^-17 of a row's
-  // range.)
+  // (At precision 1 a weight meets codes whose offset comes apart: two terms would be off by 2^-18 of a row's range.)
   const auto attend = a.precision == 1 ? short_kernel<1, 3> : a.out_dtype == 1 ? short_kernel<0, 3> : short_kernel<0, 2>;
   const int n_long = a.bounds ? p.max_long : p.long_work;
   const bool together = n_long > 0 && !a.bounds && (int64_t)p.units * p.heads <= TOGETHER[a.precision] * CUS;

@@ -10,7 +10,9 @@
 //
 // Packed rows of unit u + 3 are asked for, and those of u + 1 unpacked, while u is multiplied; new and 16-bit rows come two units
 // ahead; one barrier a unit. Scores, statistics and sums are fp32. P is one bf16 value at precision and output bf16 (a relative 2^-8
-// of each weight, averaged over the keys; a sequence of few rows keeps two, dkv_paged_short.h), else the sum of two or three.
+// of each weight, averaged over the keys; a sequence of few rows keeps two, dkv_paged_short.h), else the sum of three
+// (at precision fp32 for either output: a weight meets a code that is up to half a row's range from its offset, whatever is left of
+// the two).
 // What bounds it: the vector units, some 150 instructions a unit and wave beside its 16 matrix products of 32 cycles, of them 32
 // exponentials of twice the cost or more: 12.5k tokens of prompts of 5 heads of 3 205 us (806 TFLOP/s, 61 % of a large product's), 12
 // prompts of up to 2048 tokens of 8 heads of 4 55 us (631); with few units a workgroup the chain from the plan to the first tile, 16
@@ -461,8 +463,7 @@ __global__ __launch_bounds__(64 * WAVES, PREC ? 2 : 4) void long_kernel(dkv_page
 }
 
 void launch_long(const dkv_paged_args& a, int n_long, int n_short, float* part_o, float2* part_ml, hipStream_t s) {
-  const auto kernel = a.precision == 1 ? (a.out_dtype == 1 ? long_kernel<1, 3, 3> : long_kernel<1, 2, 3>)
-                                       : (a.out_dtype == 1 ? long_kernel<0, 3, 3> : long_kernel<0, 1, 2>);
+  const auto kernel = a.precision == 1 ? long_kernel<1, 3, 3> : a.out_dtype == 1 ? long_kernel<0, 3, 3> : long_kernel<0, 1, 2>;
   hipLaunchKernelGGL(kernel, dim3((n_long + n_short) * a.plan.heads), dim3(64 * WAVES), 0, s, a, n_long, part_o, part_ml);
 }
 

@@ -353,3 +353,39 @@ def test_prompts_beside_long_histories(cuda, precision, out):
     m.step(seqs[3:5], [70, 200], 16)
     m.attend(seqs, [1, 2, 1, 100, 3, 300], 16, out)
     m.attend(seqs[3:], [90, 1, 2], 4, out)
+
+
+@pytest.mark.parametrize('out', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('bits', [4, 8])
+@pytest.mark.parametrize('counts', [[1, 3], [70, 1, 200]])
+def test_values_far_from_their_rows_middle(cuda, counts, bits, out):
+    """One loud element a row puts the others at its edge. At precision fp32 a row is its middle plus scale * code, so what is summed
+    is up to R = 2 max |v| of each row beside its values: products p * scale are off by 2^-24, weights kept in 24 bits by 2^-24, and a
+    lane adds the middles of 32 keys a unit, the products of 16 keys in 3 terms each, which is 12 sums a unit of 16 products (their
+    own sum taken as exact to 2^-23): 32 + 2 * 12 roundings of 2^-24 a unit of 64 keys, and 16 for the joins."""
+    announce(f'values far from the middle {counts} {bits} {out}')
+    m = Model(1, 3, 'fp32', seed=bits)
+    seqs = [m.add() for _ in counts]
+    n = 400 * len(counts)
+    k, v = rows_like(m.gen, 1, n), (torch.rand(1, n, 64, generator=m.gen) * 2 - 1).bfloat16()
+    v[..., 5] = -30
+    v[..., 7::8] = 0.01
+    m.step(seqs, 400, bits, k, v)
+    step, k, v = m.step(seqs, counts, 16)
+    q = (torch.randn(3, step.tokens, 64, generator=m.gen) * 0.5).bfloat16()
+    got = m.cache.attend(q[None].cuda(), k[None].cuda(), v[None].cuda(), 0, step, out_dtype=out)[0].cpu().double()
+    at = 0
+    for s, c in zip(seqs, counts):
+        keys, values = m.k[s][0].double(), m.v[s][0].double()
+        later = torch.arange(400 + c)[None] > 400 + torch.arange(c)[:, None]
+        x = q[:, at:at + c].double()
+        p = torch.softmax((torch.matmul(x, keys.t()) / 8).masked_fill(later, float('-inf')), -1)
+        size = (torch.matmul(x.abs(), keys.abs().t()) / 8).masked_fill(later, 0).amax(-1, keepdim=True)
+        units = -(-400 // 64) + -(-c // 64)
+        e = 66 * 2 ** -24 * size + 2 ** -20 + 2 ** -24
+        ref = torch.matmul(p, values)
+        spread = torch.matmul(p, 2 * values.abs().amax(-1, keepdim=True))
+        tol = 2 * e * torch.matmul(p, values.abs()) + (2 + 56 * units + 16) * 2 ** -24 * spread + (2 ** -24 if out == torch.float32 else 2 ** -8) * ref.abs()
+        ratio = ((got[at:at + c].transpose(0, 1) - ref).abs() / tol).max().item()
+        assert ratio <= 1, (s, ratio)
+        at += c
