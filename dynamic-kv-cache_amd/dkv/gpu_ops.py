@@ -408,17 +408,18 @@ def _fused_layer_eager(p, tiles, h, n, cache, cos, sin):
 
 
 def fused_decoder_layer(layer, hidden_states, cache, position_embeddings):
-    """One LlamaDecoderLayer forward on a packed GPUCache or a step of a PagedCache; None when the layer, the inputs or the cache
-    are outside what the kernels cover. Launches beside the attention's (one to three): four, up to six
+    """One LlamaDecoderLayer forward on a packed GPUCache or a step of a PagedCache; None when the layer, the
+    inputs or the cache are outside what the kernels cover. Launches beside the attention's (one to three): four, up to six
     where the norms run apart (many rows), one more in graph steps of so many rows that the norm before
     Q/K/V is apart, which rotate and pack in a launch of their own. What depends only on the layer and
     the chunk length is checked once (_layer_plan); eager launches on contiguous inputs then take
     _fused_layer_eager (a PagedStep's captured ones too), and graph captures the general path below."""
     from .gpu_cache import GPUCache, attend_projection
-    from .paged_cache import PagedStep
     attn, mlp = layer._modules['self_attn'], layer._modules['mlp']
     h = hidden_states
     single = isinstance(cache, GPUCache)
+    if not single:
+        from .paged_cache import PagedStep
     if not ((single or isinstance(cache, PagedStep)) and cache.backend == 'fused' and position_embeddings is not None
             and hasattr(attn, '_qkv_weight') and hasattr(mlp, '_gate_up_weight') and h.dim() == 3
             and h.shape[0] == 1 and _fused(h)):
