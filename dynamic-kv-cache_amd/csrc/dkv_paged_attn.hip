@@ -30,7 +30,7 @@ __global__ __launch_bounds__(256) void merge_kernel(dkv_paged_args a, const floa
   };
   float top = -INFINITY, l = 0.f;
   f32x4 x = {0, 0, 0, 0};
-  constexpr int AHEAD = 4;
+  constexpr int AHEAD = 5;  // (a token of 48 branches / of 64 streams / 16 questions: 4 18.3 / 31.7 / 33.7 us, 5 17.8 / 31.4 / 33.6, 8 18.5 / 32.2 / 35.7)
   for (int i0 = 0; i0 < n; i0 += 4 * AHEAD) {
     float2 p[AHEAD];
     f32x4 o[AHEAD];
