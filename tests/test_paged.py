@@ -2,6 +2,8 @@
 import copy
 import ctypes
 import pickle
+import random
+import threading
 
 import numpy as np
 import pytest
@@ -188,6 +190,49 @@ def test_random_bookkeeping():
             seqs = seqs[:1]
         check(c, seqs)
         assert all(c.length(s) == want[s] for s in seqs)
+
+
+def test_calls_of_several_threads():
+    """Threads that add, grow, fork, cut and end sequences of their own in one cache, and bring pages together."""
+    c, errors, kept = Quiet(1, 1, 1, max_tokens=64 * 400), [], []
+
+    def work(seed):
+        try:
+            rng = random.Random(seed)
+            mine = [c.add()]
+            for _ in range(200):
+                kind, s = rng.choice(['step', 'step', 'fork', 'free', 'cut', 'compact']), rng.choice(mine)
+                if kind == 'step':
+                    n = c.length(s)
+                    c.step(s, rng.randint(1, 100), rng.choice([4, 8, 16]))
+                    assert c.length(s) > n
+                elif kind == 'fork' and len(mine) < 6:
+                    mine += c.fork(s, 2)
+                    assert c.length(mine[-1]) == c.length(s)
+                elif kind == 'free' and len(mine) > 1:
+                    mine.remove(s)
+                    c.free(s)
+                elif kind == 'cut':
+                    c.truncate(s, rng.randint(0, c.length(s)))
+                elif kind == 'compact':
+                    c.compact()
+                if c.length(mine[0]) > 1500:
+                    c.truncate(mine[0], 10)
+                for x in mine[1:]:
+                    if c.length(x) > 1500:
+                        c.truncate(x, 20)
+            kept.append(mine)
+        except Exception as e:  # (an assertion too)
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    check(c, [s for mine in kept for s in mine])
+    c.free([s for mine in kept for s in mine])
+    assert c.accounting()['page_bytes'] == 0
 
 
 def test_steps_that_go_on():
