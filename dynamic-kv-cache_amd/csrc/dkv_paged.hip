@@ -274,7 +274,7 @@ constexpr int SHORT_ROWS = 160;
 constexpr int SHORT_TARGET = 2048, SHORT_LEAST = 8;
 // Many rows (eight waves, a unit at a time): a step is split into LONG_TARGET workgroups at most (two a CU) beside those that
 // its blocks need, of LONG_LEAST units at least, by ranges of such a length that the last workgroup ends first (long_share).
-constexpr int LONG_TARGET = 512, LONG_LEAST = 2, CUS = 256;
+constexpr int LONG_TARGET = 512, LONG_LEAST = 2, SLOTS[2] = {256, 512};
 constexpr int SHARED_MIN = 4;  // pages that neighbours have in common to be attended to as a group
 
 struct Entity {  // a sequence's own part, or what a group of sequences has in common
@@ -291,7 +291,7 @@ static bool is_long(int64_t rows) { return rows > SHORT_ROWS; }
 
 static int check_batch(const dkv_paged_batch& b, const char* what) {
   if (b.seqs <= 0 || !b.count || !b.past || !b.position || !b.first || b.layers <= 0 || b.heads <= 0 || b.q_heads <= 0 ||
-      b.q_heads % b.heads || b.max_pages < 0) {
+      b.q_heads % b.heads || b.max_pages < 0 || b.precision < 0 || b.precision > 1) {
     set_error("%s: bad batch (seqs %d, layers %d, heads %d, q_heads %d) or a null array", what, b.seqs, b.layers, b.heads, b.q_heads);
     return DKV_EINVAL;
   }
@@ -388,13 +388,13 @@ static int64_t total_units(const std::vector<Entity>& es, int G, bool many) {
 // Units of a workgroup so that about `target` of them a KV head share all entities' units of this kind.
 static int64_t share(int64_t total, int64_t target, int least) { return std::max<int64_t>(least, (total + target - 1) / target); }
 
-// The same for many rows: of ranges from that length on, the one whose workgroups are done first when each free CU takes the
-// longest that is left (one workgroup keeps its vector units busy: two on a CU take twice as long). In units: a workgroup
-// costs its units and what its start takes, one that is joined its partial rows beside, and the join reads them. (Equal
-// shares for 512 workgroups and for 256: 12500 tokens of prompts 228 and 204 us, 12 prompts 73.8 and 59.4, 8 frames 99.5 and 108,
-// 16 questions 42.6 and 40.6; these 204, 59.4, 101 and 40.7, all with few rows in a launch of their own.)
-static int64_t long_share(const std::vector<Entity>& es, int G, int heads, int groups, const std::vector<int>& group) {
-  const int slots = std::max(1, CUS / heads);
+// The same for many rows: of ranges from that length on, the one whose workgroups are done first when each free place takes the
+// longest that is left. A CU is one place, since one workgroup keeps its vector units busy; at precision 1 it is two (8 frames 83 us,
+// 104 with one). In units: a workgroup costs its units and what its start takes, one that is joined its partial rows beside, and the
+// join reads them. (Equal shares for 512 workgroups and for 256: 12500 tokens of prompts 228 and 204 us, 12 prompts 73.8 and 59.4, 16
+// questions 42.6 and 40.6; these 204, 59.4 and 40.7, all with few rows in a launch of their own.)
+static int64_t long_share(const std::vector<Entity>& es, int G, int heads, int precision, int groups, const std::vector<int>& group) {
+  const int slots = std::max(1, SLOTS[precision] / heads);
   const int64_t least = share(total_units(es, G, true), ceil_div(LONG_TARGET, heads), LONG_LEAST);
   int64_t most = 0, best = least;
   for (const Entity& e : es)
@@ -515,7 +515,7 @@ static int write_plan(const dkv_paged_batch& b, int32_t* w, dkv_paged_plan& p) {
     for (int i = 0; i < e.n_pages; ++i) e.n4 += (from[i].page & 3) == 0, e.n8 += (from[i].page & 3) <= 1;
   }
   const int64_t few = share(total_units(all, G, false), ceil_div(SHORT_TARGET, b.heads), SHORT_LEAST);
-  const int64_t many = long_share(all, G, b.heads, groups, group);
+  const int64_t many = long_share(all, G, b.heads, b.precision, groups, group);
   Work* const work = reinterpret_cast<Work*>(w + p.at_work);
   Work* const long_work = reinterpret_cast<Work*>(w + p.at_long);
   Merge* merges = reinterpret_cast<Merge*>(w + p.at_merges);

@@ -67,10 +67,10 @@ __global__ __launch_bounds__(256) void merge_kernel(dkv_paged_args a, const floa
 }
 
 // Up to so many units of few query rows a CU (over all heads) go behind the workgroups of many in one launch, which has half as many
-// waves for them, at precision 1 a fourth. One launch / two, us: 16 questions, 260 workgroups, 33.5 / 40.6; a prompt of 200 tokens
-// beside a token of each of 8 sequences of 2000 tokens (6 units a CU) 14.4 / 21.3, 24 of 8000 (60) 43.7 / 48.1, 64 of 2000 (41) 35.0 /
-// 39.3, 64 of 8000 (160) 86 / 82, 6 of 100k (185) 101 / 94; at precision 1 15.0 / 22.5 (6), 56 / 40 (41).
-constexpr int64_t TOGETHER[2] = {64, 8}, CUS = 256;
+// waves for them. One launch / two, us: 16 questions, 260 workgroups, 33.5 / 40.6; a prompt of 200 tokens beside a token of each of 8
+// sequences of 2000 tokens (6 units a CU) 14.4 / 21.3, 24 of 8000 (60) 43.7 / 48.1, 64 of 2000 (41) 35.0 / 39.3 and at precision 1
+// 36.7 / 42.6, 64 of 8000 (160) 86 / 82, 6 of 100k (185) 101 / 94.
+constexpr int64_t TOGETHER = 64, CUS = 256;
 
 static int64_t up256(int64_t x) { return (x + 255) & ~(int64_t)255; }
 
@@ -110,7 +110,7 @@ int dkv_paged_attend(const dkv_paged_args* args, void* stream) {
   // (At precision 1 a weight meets codes whose offset comes apart: two terms would be off by 2^-18 of a row's range.)
   const auto attend = a.precision == 1 ? short_kernel<1, 3> : a.out_dtype == 1 ? short_kernel<0, 3> : short_kernel<0, 2>;
   const int n_long = a.bounds ? p.max_long : p.long_work;
-  const bool together = n_long > 0 && !a.bounds && (int64_t)p.units * p.heads <= TOGETHER[a.precision] * CUS;
+  const bool together = n_long > 0 && !a.bounds && (int64_t)p.units * p.heads <= TOGETHER * CUS;
   if (n_long > 0) launch_long(a, n_long, together ? work : 0, part_o, part_ml, st);
   if (work > 0 && !together) hipLaunchKernelGGL(attend, dim3(p.heads * work), dim3(256), 0, st, a, part_o, part_ml);
   if (merges > 0) hipLaunchKernelGGL(merge_kernel, dim3(p.heads * merges * (SHORT_BLOCK / 4)), dim3(256), 0, st, a, part_o, part_ml);

@@ -16,9 +16,8 @@
 // What bounds it: the vector units, some 150 instructions a unit and wave beside its 16 matrix products of 32 cycles, of them 32
 // exponentials of twice the cost or more: 12.5k tokens of prompts of 5 heads of 3 205 us (806 TFLOP/s, 61 % of a large product's), 12
 // prompts of up to 2048 tokens of 8 heads of 4 55 us (631); with few units a workgroup the chain from the plan to the first tile, 16
-// questions about 6144 shared tokens 27 us. At fp32 the split into three values and the scales apart, 527 instructions, and two
-// waves a SIMD, of whose time 38 % waits: 8 frames of 78 tokens over 92k 95 us.
-#include <type_traits>
+// questions about 6144 shared tokens 27 us. At fp32 the split into three values and the scales apart, some 500 instructions a unit
+// and wave: 8 frames of 78 tokens over 92k 71 us.
 
 #include "dkv_paged_short.h"
 
@@ -96,7 +95,7 @@ __device__ __forceinline__ int anew(int x) {
 
 // Workgroups behind the first n_long records' take those of few query rows, in the first half of their threads.
 template <int PREC, int TERMS, int FEW_TERMS>
-__global__ __launch_bounds__(64 * WAVES, PREC ? 2 : 4) void long_kernel(dkv_paged_args a, int n_long, float* part_o, float2* part_ml) {
+__global__ __launch_bounds__(64 * WAVES, 4) void long_kernel(dkv_paged_args a, int n_long, float* part_o, float2* part_ml) {
   __shared__ __attribute__((aligned(1024))) uint8_t tiles[RING][2][TILE_BYTES];
   __shared__ __attribute__((aligned(1024))) uint8_t packed_rows[RING][RAW_BYTES];
   __shared__ __attribute__((aligned(16))) float2 scales[PREC ? RING : 1][2][PREC ? TILE : 1];  // {offset + scale * centre, scale}
@@ -146,6 +145,7 @@ __global__ __launch_bounds__(64 * WAVES, PREC ? 2 : 4) void long_kernel(dkv_page
     const uint32_t to = tile0 + buf * (2 * TILE_BYTES) + 1024 * wave;
     load_piece_at(k, 16 * piece + __umul24(r, k_stride), to);
     load_piece_at(v, 16 * piece + __umul24(r, v_stride), to + TILE_BYTES);
+    if (PREC && (thread & 7) == 0) scales[buf][0][srow] = scales[buf][1][srow] = make_float2(0.f, 1.f);
   };
   const uint32_t kn_stride = (uint32_t)(2 * a.kn_tok_stride), vn_stride = (uint32_t)(2 * a.vn_tok_stride);  // (of a single row, whatever it is)
   auto new_rows = [&](const void* x, int64_t head_stride, int64_t tok_stride, int u) {
@@ -163,6 +163,7 @@ __global__ __launch_bounds__(64 * WAVES, PREC ? 2 : 4) void long_kernel(dkv_page
   // Packed rows come as they are: at 8 bits a wave 1 KB of K (waves 0 to 3) or V, at 4 bits every other wave, and one wave
   // the (offset, scale) pairs.
   auto load_raw = [&](const Unit& x, int buf) {
+    const int lane = anew(t) & 63;
     const uint8_t* k = base + (x.page >> 2) * grain + sub * page_sub(x.bits);
     const uint32_t to = raw0 + buf * RAW_BYTES, kv = H * page_sub(x.bits);  // (a page's V lies that far behind its K)
     if (x.bits == 8 || (wave & 3) < 2)
@@ -259,12 +260,11 @@ __global__ __launch_bounds__(64 * WAVES, PREC ? 2 : 4) void long_kernel(dkv_page
     asm volatile("" ::: "memory");
   }
 
-  // A unit's keys from its tiles. PACKED: their scales and offsets are to come (PREC 1; a constant, since a branch at every
-  // pair of keys waits for each of their reads). Keys from `high` on are not visible
-  // to this lane's row, none from 32 on to any row of the wave where there is one half.
-  auto attend = [&](auto packed_keys, int buf, bool masked, int high, bool one_half) {
-    constexpr bool PACKED = decltype(packed_keys)::value;
-    constexpr int AHEAD = 4;  // operands of K under way (12.5k tokens of prompts 2: 224.4 us, 4: 223.5, 6: 225.2; 8 frames at fp32 101.1, 101.0, 104.4)
+  // A unit's keys from its tiles, at PREC 1 with their scales and offsets to come (16-bit rows' are 1 and 0: a second path for these
+  // takes 221 registers, one workgroup a CU, 8 frames 101 us instead of 77). Keys from `high` on are not visible to this lane's
+  // row, none from 32 on to any row of the wave where there is one half.
+  auto attend = [&](int buf, bool masked, int high, bool one_half) {
+    constexpr int AHEAD = 4;  // operands of K under way (12.5k tokens of prompts 2: 224.4 us, 4: 223.5, 6: 225.2)
     const uint8_t* kt = &tiles[buf][0][0];
     const uint8_t* vt = &tiles[buf][1][0];
     f32x16 s[2];
@@ -288,7 +288,7 @@ __global__ __launch_bounds__(64 * WAVES, PREC ? 2 : 4) void long_kernel(dkv_page
     // max3 below is a statement of its own, before which the compiler does not wait for a matrix product's result: 19
     // states after one of 16 passes.
     asm volatile("s_nop 15\n s_nop 7" : "+v"(s[0]), "+v"(s[1]));
-    if constexpr (PACKED) {
+    if constexpr (PREC == 1) {
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -324,10 +324,11 @@ __global__ __launch_bounds__(64 * WAVES, PREC ? 2 : 4) void long_kernel(dkv_page
     float sum = 0.f;
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
-      if (TERMS > 1 && kb == 1 && one_half) break;  // (8 frames of 78 tokens, 3 terms: 101 us with it, 109 without; at 1 term 2 % slower)
+      if (kb == 1 && one_half) break;  // (8 frames of 78 tokens, 3 terms: 80 us with it, 86 without; full units 1 % either way)
 #pragma unroll
       for (int st = 0; st < 2; ++st) {  // 16 keys
         Op8 p[TERMS], v[2];
+        if (PREC) __builtin_amdgcn_sched_barrier(0);  // (8 frames 80 us with it, 82 without: the scales of all keys are read first)
 #pragma unroll
         for (int db = 0; db < 2; ++db)
 #pragma unroll
@@ -339,7 +340,7 @@ __global__ __launch_bounds__(64 * WAVES, PREC ? 2 : 4) void long_kernel(dkv_page
           float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][8 * st + j], xs, -mref));
           float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][8 * st + j + 1], xs, -mref));
           if (TERMS > 1) sum += p0 + p1;
-          if constexpr (PACKED) {
+          if constexpr (PREC == 1) {
             const f32x4 as = *reinterpret_cast<const f32x4*>(&scales[buf][1][32 * kb + 16 * st + 8 * (j / 4) + 4 * half + j % 4]);
             offset = __builtin_fmaf(p0, as[0], offset);
             offset = __builtin_fmaf(p1, as[2], offset);
@@ -377,10 +378,7 @@ __global__ __launch_bounds__(64 * WAVES, PREC ? 2 : 4) void long_kernel(dkv_page
     if (x1.bits < 16) unpack(x1, next, next);
     const Unit x4 = unit_at(u + 4);
     if (x0.rows < TILE && x0.bits == 16) zero_values(x0, tiles[buf][1], false);
-    if (on) {
-      if (PREC && x0.bits < 16) attend(std::integral_constant<bool, PREC == 1>(), buf, x0.rows < TILE, x0.rows, x0.rows <= 32);
-      else attend(std::false_type(), buf, x0.rows < TILE, x0.rows, x0.rows <= 32);
-    }
+    if (on) attend(buf, x0.rows < TILE, x0.rows, x0.rows <= 32);
     step(asked);
     x0 = x1, x1 = x2, x2 = x3, x3 = x4;
     buf = next;
@@ -395,7 +393,7 @@ __global__ __launch_bounds__(64 * WAVES, PREC ? 2 : 4) void long_kernel(dkv_page
     if (more) load_rows(kn, vn, w.count - first - 2 * TILE, kn_stride, vn_stride, after);
     kn += 2 * TILE * a.kn_tok_stride, vn += 2 * TILE * a.vn_tok_stride;
     if (first + TILE - 1 > first_token) zero_values(Unit{16, min(TILE, w.count - first), 0, 0}, tiles[buf][1], true);
-    if (on && first <= m_last) attend(std::false_type(), buf, first + TILE - 1 > m_first, m_new + 1 - first, m_last - first < 32);
+    if (on && first <= m_last) attend(buf, first + TILE - 1 > m_first, m_new + 1 - first, m_last - first < 32);
     step(more ? 2 : 0);
     buf = next;
   }
@@ -407,6 +405,7 @@ __global__ __launch_bounds__(64 * WAVES, PREC ? 2 : 4) void long_kernel(dkv_page
   };
   const float l = both(l_part), off = PREC ? both(offset) : 0.f;
   if (bad) {  // (rare) new values that the products took for zero, with their weights computed again
+    asm volatile("" : "+v"(q[0].u), "+v"(q[1].u), "+v"(q[2].u), "+v"(q[3].u));  // (as values of their own, as in anew)
     for (int u = max(w.u0, w.n_pages); u < w.u1; ++u) {
       const int first = (u - w.n_pages) * TILE;
       if (first + TILE - 1 <= first_token) continue;

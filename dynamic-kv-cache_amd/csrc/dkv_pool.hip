@@ -81,7 +81,7 @@ using namespace dkv;
 using namespace dkv::paged;
 
 struct dkv_pool {
-  int layers, heads, q_heads;
+  int layers, heads, q_heads, precision;
   int64_t grain, blocks;
   std::mutex lock;
   std::vector<int8_t> code;    // of a block's pages, -1: it holds none
@@ -279,10 +279,11 @@ int read_ask(dkv_pool& p, int32_t n, const int64_t* seqs, const int32_t* counts,
 
 extern "C" {
 
-int dkv_pool_create(int32_t layers, int32_t heads, int32_t q_heads, int64_t arena_bytes, dkv_pool** pool) {
+int dkv_pool_create(int32_t layers, int32_t heads, int32_t q_heads, int32_t precision, int64_t arena_bytes, dkv_pool** pool) {
   clear_error();
-  if (!pool || layers <= 0 || heads <= 0 || q_heads <= 0 || q_heads % heads || (int64_t)layers * heads > 65535 / 2) {
-    set_error("dkv_pool_create: bad shape (%d layers, %d of %d heads)", layers, heads, q_heads);
+  if (!pool || layers <= 0 || heads <= 0 || q_heads <= 0 || q_heads % heads || (int64_t)layers * heads > 65535 / 2 || precision < 0 ||
+      precision > 1) {
+    set_error("dkv_pool_create: bad shape (%d layers, %d of %d heads) or precision %d", layers, heads, q_heads, precision);
     return DKV_EINVAL;
   }
   const int64_t grain = grain_bytes(layers, heads), blocks = arena_bytes / (grain * BLOCK);
@@ -294,7 +295,7 @@ int dkv_pool_create(int32_t layers, int32_t heads, int32_t q_heads, int64_t aren
   dkv_pool* p = nullptr;
   try {
     p = new dkv_pool;
-    p->layers = layers, p->heads = heads, p->q_heads = q_heads, p->grain = grain, p->blocks = blocks;
+    p->layers = layers, p->heads = heads, p->q_heads = q_heads, p->precision = precision, p->grain = grain, p->blocks = blocks;
     p->code.assign(blocks, -1), p->used.assign(blocks, 0), p->refs.assign(blocks * BLOCK, 0);
     p->empty = BlockSet(blocks);
     for (auto& some : p->part) some = BlockSet(blocks);
@@ -536,7 +537,8 @@ int64_t dkv_pool_step_bytes(dkv_pool* pool, int32_t n, const int64_t* seqs, cons
       return DKV_EINVAL;
     }
     const std::vector<int32_t> zero(n + 1, 0);
-    const dkv_paged_batch b{n, counts, zero.data(), zero.data(), zero.data(), nullptr, nullptr, p.layers, p.heads, p.q_heads, 0, (int32_t)most};
+    const dkv_paged_batch b{n, counts, zero.data(), zero.data(), zero.data(), nullptr, nullptr, p.layers, p.heads, p.q_heads, 0, (int32_t)most,
+                            p.precision};
     bytes = dkv_paged_plan_bytes(&b);
     *max_pages = (int32_t)most;
     return bytes ? 0 : DKV_EINVAL;
@@ -589,7 +591,7 @@ int dkv_pool_step(dkv_pool* pool, int32_t n, const int64_t* seqs, const int32_t*
         first[grown + 1] = (int32_t)pages.size();
       }
       const dkv_paged_batch b{n, counts, past.data(), position.data(), first.data(), pages.data(), rows.data(), p.layers, p.heads, p.q_heads,
-                              p.blocks * BLOCK * p.grain, max_pages};
+                              p.blocks * BLOCK * p.grain, max_pages, p.precision};
       rc = dkv_paged_plan_write(&b, buffer, bytes, plan);
     } catch (...) {
       grown = std::min(grown + 1, n);  // (the one that was growing among them)

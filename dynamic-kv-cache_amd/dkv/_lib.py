@@ -90,7 +90,7 @@ class PagedBatch(ctypes.Structure):
     _fields_ = [('seqs', ctypes.c_int32), ('count', ctypes.c_void_p), ('past', ctypes.c_void_p), ('position', ctypes.c_void_p),
                 ('first', ctypes.c_void_p), ('page', ctypes.c_void_p), ('rows', ctypes.c_void_p),
                 ('layers', ctypes.c_int32), ('heads', ctypes.c_int32), ('q_heads', ctypes.c_int32),
-                ('arena_bytes', ctypes.c_int64), ('max_pages', ctypes.c_int32)]
+                ('arena_bytes', ctypes.c_int64), ('max_pages', ctypes.c_int32), ('precision', ctypes.c_int32)]
 
 
 class PoolInfo(ctypes.Structure):
@@ -230,7 +230,7 @@ SIGNATURES = [
                                       ctypes.c_int32, ctypes.c_void_p]),
     ('dkv_paged_move', ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
                                       ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p]),
-    ('dkv_pool_create', ctypes.c_int, [ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p]),
+    ('dkv_pool_create', ctypes.c_int, [ctypes.c_int32] * 4 + [ctypes.c_int64, ctypes.c_void_p]),
     ('dkv_pool_destroy', ctypes.c_int, [ctypes.c_void_p]),
     ('dkv_pool_info_get', ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(PoolInfo)]),
     ('dkv_pool_generation', ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),

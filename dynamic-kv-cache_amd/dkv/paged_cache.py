@@ -60,7 +60,8 @@ class PagedCache:
             arena_bytes = -(-max(max_tokens, 1) // BLOCK_TOKENS) * block
         self.arena_bytes = int(arena_bytes) // block * block
         pool = ctypes.c_void_p()
-        _lib.check(_lib.load().dkv_pool_create(layers, heads, q_heads, self.arena_bytes, ctypes.byref(pool)), 'dkv_pool_create')
+        _lib.check(_lib.load().dkv_pool_create(layers, heads, q_heads, PRECISIONS[precision], self.arena_bytes, ctypes.byref(pool)),
+                   'dkv_pool_create')
         self._pool = pool.value
         at = ctypes.c_void_p()
         _lib.check(_lib.load().dkv_pool_generation(self._pool, ctypes.byref(at)), 'dkv_pool_generation')

@@ -527,6 +527,7 @@ typedef struct dkv_paged_batch {
   int32_t layers, heads, q_heads;
   int64_t arena_bytes;
   int32_t max_pages; /* room for this many pages in the plan: replays may have more than the first call */
+  int32_t precision; /* of attention (dkv_paged_args), whose workgroups' shares are planned for it: 0 or 1 */
 } dkv_paged_batch;
 
 /* What a plan holds, in 32-bit words from its start: `at_*` say where, the counts what of it this step uses, `max_*`
@@ -619,7 +620,7 @@ typedef struct dkv_pool_info {
   int64_t generation;                 /* counts the calls that freed, cut or moved pages */
   int64_t pages[3], width_blocks[3];  /* by width */
 } dkv_pool_info;
-int dkv_pool_create(int32_t layers, int32_t heads, int32_t q_heads, int64_t arena_bytes, dkv_pool** pool);
+int dkv_pool_create(int32_t layers, int32_t heads, int32_t q_heads, int32_t precision, int64_t arena_bytes, dkv_pool** pool);
 int dkv_pool_destroy(dkv_pool* pool);
 int dkv_pool_info_get(dkv_pool* pool, dkv_pool_info* info);
 /* Where the pool keeps its generation, for as long as it lives. */

@@ -300,7 +300,7 @@ def test_pools_refuse_null_and_foreign_tables():
         assert getattr(lib, f'dkv_pool_{name}')(pool._pool, *rest) == _lib.DKV_EINVAL and b'null' in lib.dkv_last_error(), name
     assert lib.dkv_pool_tokens(pool._pool, 1, one, None) == lib.dkv_pool_length(pool._pool, 77) == -1
     assert lib.dkv_pool_step_bytes(pool._pool, 1, one, None, None, 0, None) == 0 and pool.accounting()['sequences'] == 1
-    assert lib.dkv_pool_create(1, 1, 1, 1 << 20, None) == _lib.DKV_EINVAL
+    assert lib.dkv_pool_create(1, 1, 1, 0, 1 << 20, None) == _lib.DKV_EINVAL
     c = Quiet(1, 1, 1)
     tile = np.zeros(2, dtype=[('offset', '<i8'), ('start', '<i4'), ('rows', '<u2'), ('bits', 'u1'), ('pad', 'u1')])
     seq = ctypes.c_int64()
@@ -317,10 +317,10 @@ def test_pools_refuse_null_and_foreign_tables():
     assert adopt(15) == 0 and c.length(seq.value) == 15 and rows(c, seq.value) == [15]
 
 
-def batch(count, past, pages, rows, first, heads=2, q_heads=6, layers=1, arena=1 << 20, max_pages=64, position=None):
+def batch(count, past, pages, rows, first, heads=2, q_heads=6, layers=1, arena=1 << 20, max_pages=64, position=None, precision=0):
     arrays = [np.array(x, dtype=t) for x, t in ((count, np.int32), (past, np.int32), (position or past, np.int32), (first, np.int32),
                                                 (pages, np.uint32), (rows, np.int32))]
-    b = _lib.PagedBatch(len(count), *[x.ctypes.data for x in arrays], layers, heads, q_heads, arena, max_pages)
+    b = _lib.PagedBatch(len(count), *[x.ctypes.data for x in arrays], layers, heads, q_heads, arena, max_pages, precision)
     b.keep = arrays
     return b
 
@@ -358,7 +358,7 @@ def test_a_plan_covers_every_row_and_unit_once():
             pages += mine[:len(held)]
             rows += held
             first.append(len(pages))
-        words, plan = write(batch(count, past, pages, rows, first, q_heads=2 * G, arena=1 << 26, max_pages=len(pages)))
+        words, plan = write(batch(count, past, pages, rows, first, q_heads=2 * G, arena=1 << 26, max_pages=len(pages), precision=trial % 2))
         assert plan.tokens == sum(count) and plan.work <= plan.max_work and plan.merges <= plan.max_merges
         assert plan.rows <= plan.max_rows and plan.items <= plan.max_items and plan.long_work <= plan.max_long
         def records(at, k, width):
@@ -414,7 +414,7 @@ def test_plans_refuse_what_the_kernels_would_trust():
     grain = 512 * 2 * 2
     for kw in (dict(count=[0]), dict(past=[-1]), dict(rows=[4]), dict(rows=[6]), dict(rows=[65]), dict(pages=[3]), dict(first=[0, 0]),
                dict(first=[1, 0]), dict(max_pages=0), dict(arena=4 * grain), dict(pages=[(1 << 20) // grain << 2]),
-               dict(pages=[2 | 2047 << 2]), dict(q_heads=5), dict(heads=0), dict(layers=0), dict(count=[1 << 23], rows=[64])):
+               dict(pages=[2 | 2047 << 2]), dict(q_heads=5), dict(precision=2), dict(heads=0), dict(layers=0), dict(count=[1 << 23], rows=[64])):
         with pytest.raises(ValueError):
             write(batch(**{**ok, **kw}))
     # a launch has fewer than 2^32 threads: a wave for each query row and head that is joined
