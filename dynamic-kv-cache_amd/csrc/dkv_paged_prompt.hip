@@ -19,6 +19,8 @@
 // questions about 6144 shared tokens 27 us. At fp32 the split into three values and the scales apart, some 500 instructions a unit
 // and wave: 8 frames of 78 tokens over 92k 71 us.
 
+#include <type_traits>
+
 #include "dkv_paged_short.h"
 
 namespace dkv {
@@ -178,8 +180,9 @@ __global__ __launch_bounds__(64 * WAVES, 4) void long_kernel(dkv_paged_args a, i
       k.x = *reinterpret_cast<const uint32_t*>(from + srow * 32 + 4 * piece);
       v.x = *reinterpret_cast<const uint32_t*>(from + RAW_V + srow * 32 + 4 * piece);
     } else {
-      k = *reinterpret_cast<const uint2*>(from + srow * 64 + 8 * piece);
-      v = *reinterpret_cast<const uint2*>(from + RAW_V + srow * 64 + 8 * piece);
+      const int at = srow * 64 + 8 * anew(piece);
+      k = *reinterpret_cast<const uint2*>(from + at);
+      v = *reinterpret_cast<const uint2*>(from + RAW_V + at);
     }
     const bool there = srow < x.rows;  // (rows that are not there: zeros, which meet a p of zero)
     const u32x4 ku = unpack8<PREC>(x.bits, k, ka), vu = unpack8<PREC>(x.bits, v, va);
@@ -260,10 +263,12 @@ __global__ __launch_bounds__(64 * WAVES, 4) void long_kernel(dkv_paged_args a, i
     asm volatile("" ::: "memory");
   }
 
-  // A unit's keys from its tiles, at PREC 1 with their scales and offsets to come (16-bit rows' are 1 and 0: a second path for these
-  // takes 221 registers, one workgroup a CU, 8 frames 101 us instead of 77). Keys from `high` on are not visible to this lane's
+  // A unit's keys from its tiles; SCALED: their scales and offsets are to come (PREC 1, pages; those of 16-bit ones are 1 and 0: a
+  // path of their own in that loop takes 221 registers, one workgroup a CU, 8 frames 101 us instead of 77; new tokens' loop has one,
+  // 15 prompts of 645 tokens 97 us, 108 without). Keys from `high` on are not visible to this lane's
   // row, none from 32 on to any row of the wave where there is one half.
-  auto attend = [&](int buf, bool masked, int high, bool one_half) {
+  auto attend = [&](auto scaled, int buf, bool masked, int high, bool one_half) {
+    constexpr bool SCALED = decltype(scaled)::value;
     constexpr int AHEAD = 4;  // operands of K under way (12.5k tokens of prompts 2: 224.4 us, 4: 223.5, 6: 225.2)
     const uint8_t* kt = &tiles[buf][0][0];
     const uint8_t* vt = &tiles[buf][1][0];
@@ -288,7 +293,7 @@ __global__ __launch_bounds__(64 * WAVES, 4) void long_kernel(dkv_paged_args a, i
     // max3 below is a statement of its own, before which the compiler does not wait for a matrix product's result: 19
     // states after one of 16 passes.
     asm volatile("s_nop 15\n s_nop 7" : "+v"(s[0]), "+v"(s[1]));
-    if constexpr (PREC == 1) {
+    if constexpr (SCALED) {
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -340,7 +345,7 @@ __global__ __launch_bounds__(64 * WAVES, 4) void long_kernel(dkv_paged_args a, i
           float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][8 * st + j], xs, -mref));
           float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][8 * st + j + 1], xs, -mref));
           if (TERMS > 1) sum += p0 + p1;
-          if constexpr (PREC == 1) {
+          if constexpr (SCALED) {
             const f32x4 as = *reinterpret_cast<const f32x4*>(&scales[buf][1][32 * kb + 16 * st + 8 * (j / 4) + 4 * half + j % 4]);
             offset = __builtin_fmaf(p0, as[0], offset);
             offset = __builtin_fmaf(p1, as[2], offset);
@@ -378,7 +383,7 @@ __global__ __launch_bounds__(64 * WAVES, 4) void long_kernel(dkv_paged_args a, i
     if (x1.bits < 16) unpack(x1, next, next);
     const Unit x4 = unit_at(u + 4);
     if (x0.rows < TILE && x0.bits == 16) zero_values(x0, tiles[buf][1], false);
-    if (on) attend(buf, x0.rows < TILE, x0.rows, x0.rows <= 32);
+    if (on) attend(std::integral_constant<bool, PREC == 1>(), buf, x0.rows < TILE, x0.rows, x0.rows <= 32);
     step(asked);
     x0 = x1, x1 = x2, x2 = x3, x3 = x4;
     buf = next;
@@ -393,7 +398,7 @@ __global__ __launch_bounds__(64 * WAVES, 4) void long_kernel(dkv_paged_args a, i
     if (more) load_rows(kn, vn, w.count - first - 2 * TILE, kn_stride, vn_stride, after);
     kn += 2 * TILE * a.kn_tok_stride, vn += 2 * TILE * a.vn_tok_stride;
     if (first + TILE - 1 > first_token) zero_values(Unit{16, min(TILE, w.count - first), 0, 0}, tiles[buf][1], true);
-    if (on && first <= m_last) attend(buf, first + TILE - 1 > m_first, m_new + 1 - first, m_last - first < 32);
+    if (on && first <= m_last) attend(std::false_type(), buf, first + TILE - 1 > m_first, m_new + 1 - first, m_last - first < 32);
     step(more ? 2 : 0);
     buf = next;
   }
