@@ -409,33 +409,57 @@ __global__ __launch_bounds__(64 * WAVES, 4) void long_kernel(dkv_paged_args a, i
     return __uint_as_float(y[0]) + __uint_as_float(y[1]);
   };
   const float l = both(l_part), off = PREC ? both(offset) : 0.f;
-  if (bad) {  // (rare) new values that the products took for zero, with their weights computed again
+  // (rare) New values that the products took for zero, with their weights computed again; where an element of this wave became NaN,
+  // which an infinite value's products with a weight's lower terms also make, all infinite and NaN values that it sees.
+  uint32_t lost = 0;  // such elements, of rows whose scores are no NaN: bit 16 db + i
+  if (TERMS > 1)
+#pragma unroll
+    for (int i = 0; i < 32; ++i) lost |= acc[i / 16][i % 16] != acc[i / 16][i % 16] && l == l ? 1u << i : 0u;
+  const bool again = TERMS > 1 && __builtin_amdgcn_ballot_w64(lost != 0);
+  if (bad || again) {
     asm volatile("" : "+v"(q[0].u), "+v"(q[1].u), "+v"(q[2].u), "+v"(q[3].u));  // (as values of their own, as in anew)
-    for (int u = max(w.u0, w.n_pages); u < w.u1; ++u) {
+    if (TERMS > 1)
+#pragma unroll
+      for (int i = 0; i < 32; ++i) acc[i / 16][i % 16] = lost >> i & 1 ? 0.f : acc[i / 16][i % 16];
+    bool packed = false;  // a packed row of values is infinite or NaN: its elements stay NaN
+    for (int u = again ? w.u0 : max(w.u0, w.n_pages); u < w.u1; ++u) {
       const int first = (u - w.n_pages) * TILE;
-      if (first + TILE - 1 <= first_token) continue;
-      for (int j = 0; j < min(TILE, w.count - first); ++j) {
-        const int64_t tok = w.token0 + first + j;
-        const uint2* v = reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(a.v_new) + h * a.vn_head_stride + tok * a.vn_tok_stride);
+      const uint8_t *k, *v;
+      int64_t k_stride = 128, v_stride = 128;
+      int rows;
+      if (u < w.n_pages) {
+        const Page pg = plan_record<Page>(plan, a.plan.at_pages, w.first_page + u);
+        const int bits = page_bits(pg.page);
+        k = base + (pg.page >> 2) * grain + sub * page_sub(bits), v = k + (int64_t)H * page_sub(bits), rows = pg.rows;
+        if (bits < 16) {
+          const float2 as = reinterpret_cast<const float2*>(v + TILE * 8 * bits)[last & 63];
+          packed = packed || ((last & 63) < rows && !(fabsf(as.x) < INFINITY && fabsf(as.y) < INFINITY));
+          continue;
+        }
+      } else {
+        if (!again && first + TILE - 1 <= first_token) continue;
+        k = new_rows(a.k_new, a.kn_head_stride, a.kn_tok_stride, u), v = new_rows(a.v_new, a.vn_head_stride, a.vn_tok_stride, u);
+        k_stride = 2 * a.kn_tok_stride, v_stride = 2 * a.vn_tok_stride, rows = min(TILE, w.count - first);
+      }
+      for (int j = 0; j < rows; ++j, k += k_stride, v += v_stride) {
         uint2 x[8];
         bool some = false;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {  // elements 8 i + 4 half_last + ...
-          x[i] = v[2 * i + half_last];
+          x[i] = reinterpret_cast<const uint2*>(v)[2 * i + half_last];
           some = some || bad_bf16(x[i].x) || bad_bf16(x[i].x >> 16) || bad_bf16(x[i].y) || bad_bf16(x[i].y >> 16);
         }
         if (!__builtin_amdgcn_ballot_w64(some)) continue;
-        const u32x4* k = reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.k_new) + h * a.kn_head_stride + tok * a.kn_tok_stride);
         float dot = 0.f;
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) {
-          const u32x4 y = k[2 * ks + half_last];
+          const u32x4 y = reinterpret_cast<const u32x4*>(k)[2 * ks + half_last];
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             dot = __builtin_fmaf(bf16_lo(q[ks].u[e]), bf16_lo(y[e]), __builtin_fmaf(bf16_hi(q[ks].u[e]), bf16_hi(y[e]), dot));
         }
         const float p = __builtin_amdgcn_exp2f(both(dot) * xs - m_run);
-        if (first + j > m_out) continue;
+        if (first + j > m_out) continue;  // (of pages: negative)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const int db = i / 4, at = 4 * (i % 4);
@@ -445,6 +469,12 @@ __global__ __launch_bounds__(64 * WAVES, 4) void long_kernel(dkv_paged_args a, i
           if (bad_bf16(x[i].y >> 16)) acc[db][at + 3] += p * bf16_hi(x[i].y);
         }
       }
+    }
+    if (TERMS > 1) {
+      const bool keep = __builtin_amdgcn_ballot_w64(packed);
+#pragma unroll
+      for (int i = 0; i < 32; ++i)  // (no such value was found: the NaN comes from a score)
+        if (lost >> i & 1 && (keep || acc[i / 16][i % 16] == 0.f)) acc[i / 16][i % 16] = NAN;
     }
   }
   if (wave0 + c_last >= total) return;

@@ -370,37 +370,71 @@ __device__ __forceinline__ void short_rows(const dkv_paged_args& a, float* part_
     soften(s, scale2, r);
     weigh<16, PREC, TERMS>(x, rw.scales, g, s, r);
   }
-  if (__builtin_amdgcn_ballot_w64(bad)) {  // (rare) with their weights computed again
-    for (int j = 0; j <= m_last; ++j) {
-      const int piece = w.n_pages + j / TILE;
-      const int first = j / HALF * HALF;
-      if (piece < u0 || piece >= u1 || m_first + 1 - first >= min(HALF, m_last + 1 - first)) continue;  // not this wave's, or seen by every row
-      const int64_t tok = w.token0 + j;
-      const u32x4* k = reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.k_new) + h * a.kn_head_stride + tok * a.kn_tok_stride + 16 * g);
-      const u32x4* v = reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.v_new) + h * a.vn_head_stride + tok * a.vn_tok_stride + 16 * g);
-      float dot = 0;
+  r.l = row_sum(r.l);
+  r.offset = PREC == 1 ? row_sum(r.offset) : 0.f;
+  // (rare) Infinite and NaN values with their weights computed again: those that were taken for zero, and in elements that became NaN all
+  // that is seen, since an infinite value's product with a weight's lower terms, which may be zero or negative, makes NaN of infinity.
+  uint32_t lost = 0;  // such elements, of rows whose scores are no NaN: bit 4 db + i
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const u32x4 y = k[i];
+  for (int db = 0; db < 4; ++db)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          dot = __builtin_fmaf(bf16_lo(q[i].u[e]), bf16_lo(y[e]), __builtin_fmaf(bf16_hi(q[i].u[e]), bf16_hi(y[e]), dot));
+    for (int i = 0; i < 4; ++i) lost |= r.o[db][i] != r.o[db][i] && r.l == r.l ? 1u << (4 * db + i) : 0u;
+  const bool again = __builtin_amdgcn_ballot_w64(lost != 0);
+  if (__builtin_amdgcn_ballot_w64(bad) || again) {
+#pragma unroll
+    for (int db = 0; db < 4; ++db)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r.o[db][i] = lost >> (4 * db + i) & 1 ? 0.f : r.o[db][i];
+    bool packed = false;  // a packed row of values is infinite or NaN: its elements stay NaN
+    for (int at = again ? 2 * u0 : max(2 * u0, 2 * w.n_pages); at < 2 * u1; ++at) {
+      const int first = (at - 2 * w.n_pages) * HALF;
+      const uint8_t *key, *value;  // a row's, from its elements 16 g on
+      int64_t k_stride = 128, v_stride = 128;
+      int rows;
+      if (first < 0) {
+        const Half u = page(at);
+        key = u.k + 32 * g, value = u.v + 32 * g, rows = u.rows;
+        if (at < 2 * w.n8) {
+          const float2 as = *reinterpret_cast<const float2*>(u.scales);
+          packed = packed || (lane >= HALF && lane - HALF < rows && !(fabsf(as.x) < INFINITY && fabsf(as.y) < INFINITY));
+          continue;
+        }
+      } else {
+        rows = min(HALF, m_last + 1 - first);
+        if (!again && m_first + 1 - first >= rows) continue;  // seen by every row
+        key = static_cast<const uint8_t*>(a.k_new) + 2 * (h * a.kn_head_stride + (int64_t)(w.token0 + first) * a.kn_tok_stride) + 32 * g;
+        value = static_cast<const uint8_t*>(a.v_new) + 2 * (h * a.vn_head_stride + (int64_t)(w.token0 + first) * a.vn_tok_stride) + 32 * g;
+        k_stride = 2 * a.kn_tok_stride, v_stride = 2 * a.vn_tok_stride;
       }
-      const float p = __builtin_amdgcn_exp2f(row_sum(dot) * scale2 - r.m);
-      if (j > m) continue;
+      for (int j = 0; j < rows; ++j, key += k_stride, value += v_stride) {
+        float dot = 0;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const u32x4 y = v[i];
+        for (int i = 0; i < 2; ++i) {
+          const u32x4 y = reinterpret_cast<const u32x4*>(key)[i];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {  // elements 16 g + 8 i + 2 e + ... = 16 g + 4 (2 i + e / 2) + 2 (e % 2) + ...
-          if (bad_bf16(y[e])) r.o[2 * (e % 2)][2 * i + e / 2] += p * bf16_lo(y[e]);
-          if (bad_bf16(y[e] >> 16)) r.o[2 * (e % 2) + 1][2 * i + e / 2] += p * bf16_hi(y[e]);
+          for (int e = 0; e < 4; ++e)
+            dot = __builtin_fmaf(bf16_lo(q[i].u[e]), bf16_lo(y[e]), __builtin_fmaf(bf16_hi(q[i].u[e]), bf16_hi(y[e]), dot));
+        }
+        const float p = __builtin_amdgcn_exp2f(row_sum(dot) * scale2 - r.m);
+        if (first + j > m) continue;  // (of pages: negative)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const u32x4 y = reinterpret_cast<const u32x4*>(value)[i];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {  // elements 16 g + 8 i + 2 e + ... = 16 g + 4 (2 i + e / 2) + 2 (e % 2) + ...
+            if (bad_bf16(y[e])) r.o[2 * (e % 2)][2 * i + e / 2] += p * bf16_lo(y[e]);
+            if (bad_bf16(y[e] >> 16)) r.o[2 * (e % 2) + 1][2 * i + e / 2] += p * bf16_hi(y[e]);
+          }
         }
       }
     }
+    const bool keep = __builtin_amdgcn_ballot_w64(packed);
+#pragma unroll
+    for (int db = 0; db < 4; ++db)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)  // (no such value was found: the NaN comes from a score)
+        if (lost >> (4 * db + i) & 1 && (keep || r.o[db][i] == 0.f)) r.o[db][i] = NAN;
   }
-  r.l = row_sum(r.l);
-  r.offset = PREC == 1 ? row_sum(r.offset) : 0.f;
   if (g == 0) ml[wave][c][0] = r.m, ml[wave][c][1] = r.l;
 #pragma unroll
   for (int i = 0; i < 4; ++i) o[wave][c][4 * g + i] = f32x4{r.o[0][i], r.o[1][i], r.o[2][i], r.o[3][i]} + r.offset;

@@ -586,7 +586,7 @@ int dkv_paged_rope_append(const dkv_paged_args* args, const void* qkv, int64_t q
 
 /* The step's new tokens attend, each to its sequence's history before the step and to the sequence's new tokens up to
  * itself (these as they are in k_new and v_new). What later tokens hold, NaN and infinities included, does not reach
- * a query. Q, K and V must be 16-byte aligned with strides in multiples of 8 elements; out 16-byte aligned with
+ * a query; an infinite value that it sees gives the formula's infinity or NaN. Q, K and V must be 16-byte aligned with strides in multiples of 8 elements; out 16-byte aligned with
  * strides in multiples of 4 elements, in memory of its own. */
 int64_t dkv_paged_workspace_bytes(const dkv_paged_args* args);
 int dkv_paged_attend(const dkv_paged_args* args, void* stream);
