@@ -627,11 +627,10 @@ int64_t dkv_pool_tokens(dkv_pool* pool, int32_t n, const int64_t* seqs, const in
 
 int dkv_pool_read(dkv_pool* pool, int32_t n, const int64_t* seqs, const int64_t* from, int32_t layer0, int32_t n_layers, const void* arena,
                   void* out, int32_t n_tokens, int32_t out_dtype, void* stream) {
-  std::vector<dkv_page_rows> items;
-  int64_t arena_bytes = 0;
-  int32_t layers = 0, heads = 0;
-  const int rc = guarded(pool, "dkv_pool_read", {n > 0 ? (const void*)from : pool}, [&](dkv_pool& p) {
+  // (Launched under the lock: a call that moves or frees the pages is enqueued before they are looked up or behind the reads.)
+  return guarded(pool, "dkv_pool_read", {n > 0 ? (const void*)from : pool}, [&](dkv_pool& p) {
     const char* what = "dkv_pool_read";
+    std::vector<dkv_page_rows> items;
     std::vector<Sequence*> s;
     if (int rc = p.named(seqs, n, s, what)) return rc;
     int64_t to = 0;
@@ -650,11 +649,9 @@ int dkv_pool_read(dkv_pool* pool, int32_t n, const int64_t* seqs, const int64_t*
       set_error("%s: room for %d tokens, not %lld", what, n_tokens, (long long)to);
       return DKV_EINVAL;
     }
-    arena_bytes = p.blocks * BLOCK * p.grain, layers = p.layers, heads = p.heads;
-    return 0;
+    return dkv_paged_read(arena, p.blocks * BLOCK * p.grain, items.data(), (int32_t)items.size(), layer0, n_layers, p.layers, p.heads, out,
+                          n_tokens, out_dtype, stream);
   });
-  if (rc) return rc;
-  return dkv_paged_read(arena, arena_bytes, items.data(), (int32_t)items.size(), layer0, n_layers, layers, heads, out, n_tokens, out_dtype, stream);
 }
 
 }  // extern "C"

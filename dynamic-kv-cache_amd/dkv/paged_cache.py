@@ -16,6 +16,7 @@ GPUCache's, byte for byte (include/dkv.h). No counterpart in the reference, whos
 """
 import ctypes
 import struct
+import threading
 import weakref
 
 import numpy as np
@@ -43,7 +44,8 @@ class PagedCache:
     max_tokens: room for that many tokens at 16 bits in full pages (some more at 8, three times as many at 4); a
     sequence's last page, and one after which the width changes, may be part full. precision as in GPUCache.
     The calls on one cache belong on one stream, or on streams that wait for each other: pages that a call frees are
-    written again by later ones.
+    written again by later ones. Threads may call at once; what one of them frees, cuts or moves makes the others' planned
+    steps refuse, as it does its own, so each holds `lock` from a step() or advance() to the last launch or replay over it.
     """
 
     def __init__(self, layers, heads, q_heads, max_tokens=8192, dim=64, device='cuda', precision='bf16', arena_bytes=None):
@@ -63,6 +65,8 @@ class PagedCache:
         _lib.check(_lib.load().dkv_pool_create(layers, heads, q_heads, PRECISIONS[precision], self.arena_bytes, ctypes.byref(pool)),
                    'dkv_pool_create')
         self._pool = pool.value
+        # (every call holds it from its look at the pages, or at a step's generation, to its launch)
+        self.lock = threading.RLock()
         at = ctypes.c_void_p()
         _lib.check(_lib.load().dkv_pool_generation(self._pool, ctypes.byref(at)), 'dkv_pool_generation')
         self._generation = ctypes.c_int64.from_address(at.value)  # counts the calls that freed, cut or moved pages
@@ -81,18 +85,25 @@ class PagedCache:
         """Torch's current stream on this cache's device."""
         return _lib.raw_stream(self._index) if self._index >= 0 else 0
 
-    def _launch(self, what, call, stream=None):
-        """call(stream) on this cache's device and torch's current stream there."""
+    def _planned(self, what, step):
+        if step.generation != self._generation.value:
+            raise ValueError(f'{what}: pages were freed, cut or moved since this step was planned')
+
+    def _launch(self, what, call, stream=None, step=None):
+        """call(stream) on this cache's device and torch's current stream there, over `step` if that is given."""
         index = self._index
         if index < 0:
             raise ValueError(f'{what}: PagedCache requires a CUDA device')
         if stream is None:
             stream = _lib.raw_stream(index)
-        if torch.cuda.current_device() == index:
-            rc = call(stream)
-        else:
-            with torch.cuda.device(index):
+        with self.lock:
+            if step is not None:
+                self._planned(what, step)
+            if torch.cuda.current_device() == index:
                 rc = call(stream)
+            else:
+                with torch.cuda.device(index):
+                    rc = call(stream)
         if rc:
             _lib.check(rc, what)
 
@@ -203,7 +214,10 @@ class PagedCache:
         """Ends sequences; pages that no other one holds are free again."""
         ids, n = self._ids(seqs)
         self._not_captured('free')
-        _lib.check(_lib.load().dkv_pool_free(self._pool, ids, n), 'dkv_pool_free')
+        with self.lock:
+            rc = _lib.load().dkv_pool_free(self._pool, ids, n)
+        if rc:
+            _lib.check(rc, 'dkv_pool_free')
 
     def truncate(self, seq, length):
         """Drops a sequence's tokens from `length` on."""
@@ -249,8 +263,7 @@ class PagedCache:
     def _check(self, what, step, layer, tensors):
         if not isinstance(step, PagedStep) or step.cache is not self:
             raise ValueError(f'{what} expects a step of this cache')
-        if step.generation != self._generation.value:
-            raise ValueError(f'{what}: pages were freed, cut or moved since this step was planned')
+        self._planned(what, step)
         if not 0 <= layer < self.layers:
             raise ValueError(f'{what}: layer {layer} of {self.layers}')
         for x, heads in tensors:
@@ -267,7 +280,7 @@ class PagedCache:
         stream = self._stream()
         args = _ARGS.pack(0, 0, 0, kp, ks[1], ks[2], vp, vs[1], vs[2], self._arena_ptr, self.arena_bytes, step.device_plan(stream),
                           step.plan_bytes, layer, self._captured(stream), 0.0, 0, 0, 0, 0, 0, 0, 0)
-        self._launch('dkv_paged_append', lambda stream: _lib.load().dkv_paged_append(args, stream), stream)
+        self._launch('dkv_paged_append', lambda stream: _lib.load().dkv_paged_append(args, stream), stream, step)
 
     def attend(self, q, k, v, layer, step, out_dtype=None, precision=None):
         """Causal attention of the step's tokens, q [1, q_heads, tokens, 64], each over its sequence's history and the
@@ -291,7 +304,7 @@ class PagedCache:
         args = _ARGS.pack(qp, qs[1], qs[2], kp, ks[1], ks[2], vp, vs[1], vs[2], self._arena_ptr, self.arena_bytes, step.device_plan(stream),
                           step.plan_bytes, layer, bounds, self.dim ** -0.5, out.data_ptr(), self.q_heads * self.dim, self.dim,
                           out_dtype is torch.float32, PRECISIONS[precision], ws.data_ptr() if need else 0, need)
-        self._launch('dkv_paged_attend', lambda stream: _lib.load().dkv_paged_attend(args, stream), stream)
+        self._launch('dkv_paged_attend', lambda stream: _lib.load().dkv_paged_attend(args, stream), stream, step)
         return out
 
     def materialize(self, layer, seqs, first=0, out_dtype=torch.bfloat16):
@@ -315,7 +328,8 @@ class PagedCache:
         out = self.arena.new_empty((2, layers, self.heads, n, self.dim), dtype=out_dtype)
         if isinstance(seqs, PagedStep):
             self._launch('dkv_paged_read', lambda stream: _lib.load().dkv_paged_read(
-                self._arena_ptr, self.arena_bytes, items, n_items, layer0, layers, self.layers, self.heads, out.data_ptr(), n, fp32, stream))
+                self._arena_ptr, self.arena_bytes, items, n_items, layer0, layers, self.layers, self.heads, out.data_ptr(), n, fp32, stream),
+                step=seqs)
         else:
             self._launch('dkv_pool_read', lambda stream: _lib.load().dkv_pool_read(
                 self._pool, count, ids, first, layer0, layers, self._arena_ptr, out.data_ptr(), n, fp32, stream))
@@ -419,7 +433,7 @@ class PagedStep(_CacheBase):
         args = _ARGS.pack(q.data_ptr(), head, c.dim, k.data_ptr(), head, c.dim, v.data_ptr(), head, c.dim, c._arena_ptr, c.arena_bytes,
                           self.device_plan(stream), self.plan_bytes, layer, c._captured(stream), 0.0, 0, 0, 0, 0, 0, 0, 0)
         c._launch('dkv_paged_rope_append', lambda stream: _lib.load().dkv_paged_rope_append(
-            args, qkv.data_ptr(), qkv.stride(0), cos.data_ptr(), sin.data_ptr(), cos.stride(0), stream), stream)
+            args, qkv.data_ptr(), qkv.stride(0), cos.data_ptr(), sin.data_ptr(), cos.stride(0), stream), stream, self)
         return q, k, v, 0
 
     def _fused_attention(self, n, q_heads, layer, project, cos, sin, cs_stride, qkv_out, out, stream):
@@ -427,8 +441,6 @@ class PagedStep(_CacheBase):
         launches, with the arguments and promises of GPUCache._fused_attention: the same bytes and outputs as the
         general entry points', which cost more host time than the GPU spends on a token of each sequence."""
         c, d = self.cache, self.cache.dim
-        if self.generation != c._generation.value:
-            raise ValueError('attend: pages were freed, cut or moved since this step was planned')
         if n != self.tokens or q_heads != c.q_heads or layer >= c.layers:
             raise ValueError(f'a step of {self.tokens} tokens and {c.q_heads} query heads in {c.layers} layers got {n} and {q_heads} in layer {layer}')
         H, lib, here = c.heads, _lib.load(), c._stream()
@@ -441,8 +453,10 @@ class PagedStep(_CacheBase):
         vp, head = kp + H * n * d * 2, n * d
         args = _ARGS.pack(qkv_out, head, d, kp, head, d, vp, head, d, c._arena_ptr, c.arena_bytes, self.device_plan(here), self.plan_bytes,
                           layer, bounds, d ** -0.5, out, q_heads * d, d, 0, PRECISIONS[c.precision], at if need else 0, need)
-        rc = (lib.dkv_linear_tiled(x, x_stride, weight, w_stride, n, width, k, norm, eps, 0, None, 0, at, width, layout, stream)
-              or lib.dkv_paged_rope_append(args, at, width, cos, sin, cs_stride, stream) or lib.dkv_paged_attend(args, stream))
+        with c.lock:
+            c._planned('attend', self)
+            rc = (lib.dkv_linear_tiled(x, x_stride, weight, w_stride, n, width, k, norm, eps, 0, None, 0, at, width, layout, stream)
+                  or lib.dkv_paged_rope_append(args, at, width, cos, sin, cs_stride, stream) or lib.dkv_paged_attend(args, stream))
         if rc:
             _lib.check(rc, 'the launches of a fused decoder layer')
 

@@ -524,9 +524,9 @@ class StreamingDecoder:
         """Continues each question [1, n] (of any lengths) on a branch of its sequence of the PagedCache `pages` (one
         of seqs each, or one for all; questions about one sequence attend to it together where they stand next to
         each other): tokens int64 [questions, n] for the random numbers u [questions, n], each row as generate() draws
-        it. The branches take pages for a question and its tokens, and end with the call. With graphs=True the
-        forwards of more than GRAPH_TOKENS tokens are replays of a captured one from the third token's on, and the call
-        waits for the GPU."""
+        it. The branches take pages for a question and its tokens, and end with the call. Threads may call at once with one
+        `pages` on one stream. With graphs=True the forwards of more than GRAPH_TOKENS tokens are replays of a captured one from
+        the third token's on, the call waits for the GPU, and a capture allows no other thread's work on the device."""
         questions = list(questions)
         seqs = list(seqs) if hasattr(seqs, '__len__') else [seqs] * len(questions)
         if len(seqs) != len(questions) or u.dim() != 2 or u.shape[0] != len(questions):
@@ -546,26 +546,28 @@ class StreamingDecoder:
             counts = [x.shape[1] for x in questions]
             last = torch.tensor(counts).cumsum(0).sub(1).to(self.device)
             ids = torch.cat([x.to(self.device) for x in questions], dim=1)
-            step = pages.step(branches, counts)
-            logits = self._paged_forward(step, ids, last)
+            with pages.lock:  # (a plan and the launches over it: another thread's call frees or moves no pages between the two)
+                step = pages.step(branches, counts)
+                logits = self._paged_forward(step, ids, last)
             n, last = u.shape[1], slice(None)
             for i in range(n):
                 tokens.append(sample(logits, u[:, i], temperature, top_k, top_p, min_p))
                 if i + 1 == n:
                     break
                 ids = tokens[-1][None].clamp(min=0)  # (-1 is no index into the embeddings)
-                step = step.advance() if i else pages.step(branches, reserve=n)
-                if graph is not None:
-                    held.copy_(ids)
-                    graph.replay()
-                elif not (self.graphs and i and n > GRAPH_TOKENS):  # (the first of these forwards warms the library paths that a capture records)
-                    logits = self._paged_forward(step, ids, last)
-                else:
-                    held, graph = ids.clone(), torch.cuda.CUDAGraph()
-                    torch.cuda.synchronize()
-                    with torch.cuda.graph(graph):
-                        logits = self._paged_forward(step, held, last)
-                    graph.replay()
+                with pages.lock:
+                    step = step.advance() if i else pages.step(branches, reserve=n)
+                    if graph is not None:
+                        held.copy_(ids)
+                        graph.replay()
+                    elif not (self.graphs and i and n > GRAPH_TOKENS):  # (the first of these forwards warms the library paths that a capture records)
+                        logits = self._paged_forward(step, ids, last)
+                    else:
+                        held, graph = ids.clone(), torch.cuda.CUDAGraph()
+                        torch.cuda.synchronize()
+                        with torch.cuda.graph(graph):
+                            logits = self._paged_forward(step, held, last)
+                        graph.replay()
         finally:
             if graph is not None:
                 torch.cuda.synchronize(self.device)  # (it may still run, and ends here)

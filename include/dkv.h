@@ -609,8 +609,10 @@ typedef struct dkv_page_move {
 int dkv_paged_move(const void* src, int64_t src_bytes, void* dst, int64_t dst_bytes, const dkv_page_move* moves,
                    int32_t n_moves, int32_t layers, int32_t heads, void* stream);
 
-/* The pages of an arena and the sequences that hold them: host bookkeeping for the calls above (each call takes the
- * pool's lock), with the launches that move rows. Sequences are named by numbers that are not used again. Where a call
+/* The pages of an arena and the sequences that hold them: host bookkeeping for the calls above, with the launches that
+ * move or read rows. Each call takes the pool's lock, its launches too, so threads that share a stream may call at once. The
+ * launches over a plan know no pool: with several threads the caller holds a lock of its own over the look at the generation
+ * and the launch, and over the calls that change it (dkv_pool_step, adopt and fork too, where they make room). Sequences are named by numbers that are not used again. Where a call
  * takes `arena` and `stream` it may move pages, also to bring them together where a new page finds too little room;
  * with a null arena nothing is moved (bookkeeping alone). A call that fails changes no sequence. */
 typedef struct dkv_pool dkv_pool;
