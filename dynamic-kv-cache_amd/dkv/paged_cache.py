@@ -15,6 +15,7 @@ GPUCache's, byte for byte (include/dkv.h). No counterpart in the reference, whos
     step = cache.step(seqs)                     # the next token of each
 """
 import ctypes
+import operator
 import struct
 import threading
 import weakref
@@ -131,17 +132,27 @@ class PagedCache:
         return (ctypes.c_int64 * len(seqs))(*seqs), len(seqs)
 
     @staticmethod
+    def _whole(x, what):
+        try:
+            return operator.index(x)
+        except TypeError:
+            raise ValueError(f'{what}: {x!r} is no whole number') from None
+
+    @staticmethod
     def _each(x, n, what):
-        if isinstance(x, (int, np.integer)):
-            x = [int(x)] * n
+        if isinstance(x, int):
+            x = [x] * n
+        elif not getattr(x, 'ndim', 1) or not hasattr(x, '__iter__'):
+            x = [PagedCache._whole(x, what)] * n
         else:
             x = list(x)
             if not set(map(type, x)) <= {int}:
-                x = [int(v) for v in x]
+                x = [PagedCache._whole(v, what) for v in x]
         if len(x) != n:
             raise ValueError(f'one {what} a sequence: {len(x)} for {n}')
-        if x and not -1 << 31 <= min(x) <= max(x) < 1 << 31:
-            raise ValueError(f'{what}: {max(x)} is out of range')
+        for v in (min(x), max(x)) if x else ():
+            if not -1 << 31 <= v < 1 << 31:
+                raise ValueError(f'{what}: {v} is out of range')
         return x
 
     def _sequence(self, seq):
@@ -203,6 +214,7 @@ class PagedCache:
         """n new sequences that go on from this one. They share its pages but a last one that is not full, of which
         each gets a copy."""
         (seq,), _ = self._ids([seq])
+        n = self._whole(n, 'fork')
         if not 0 <= n <= 1 << 20:
             raise ValueError(f'fork: cannot make {n} branches')
         self._not_captured('fork')
@@ -222,6 +234,7 @@ class PagedCache:
     def truncate(self, seq, length):
         """Drops a sequence's tokens from `length` on."""
         (seq,), _ = self._ids([seq])
+        length = self._whole(length, 'truncate')
         if not 0 <= length < IDS:
             raise ValueError(f'truncate: a sequence cannot hold {length} tokens')
         self._not_captured('truncate')
@@ -357,6 +370,7 @@ class PagedStep(_CacheBase):
         ids, n = cache._ids(seqs)
         self.seqs = list(ids)
         self.counts, self.bits = cache._each(counts, n, 'count'), cache._each(bits, n, 'width')
+        reserve = cache._whole(reserve, 'reserve')
         if not 0 <= reserve < 1 << 31:
             raise ValueError(f'step: a reserve of {reserve} tokens')
         self._ask = (n, ids, (ctypes.c_int32 * n)(*self.counts), (ctypes.c_int32 * n)(*self.bits))
