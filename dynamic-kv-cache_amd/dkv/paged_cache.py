@@ -481,6 +481,18 @@ class PagedStep(_CacheBase):
     def attend(self, q, k, v, layer, past=0, **kw):
         return self.cache.attend(q, k, v, layer, self, **kw)
 
+    def update(self, key_states, value_states, layer_idx, *args, **kw):
+        raise ValueError('a PagedStep has no update(): its rows are read by the attention of install_packed_attention() alone')
+
+    def _none(name):
+        def refuse(self, *args, **kw):
+            raise ValueError(f'a PagedStep has no {name}(): what it holds are sequences of a PagedCache')
+        return refuse
+
+    crop, reorder_cache, batch_repeat_interleave, batch_select_indices, reset = map(
+        _none, ('crop', 'reorder_cache', 'batch_repeat_interleave', 'batch_select_indices', 'reset'))
+    del _none
+
     def get_seq_length(self, layer_idx=0):
         return 0
 
