@@ -6,6 +6,7 @@
 // a block that is emptied to a free place of one that stays. A sequence's last page, unless it is full, is held by that
 // sequence alone; the others may be held by several.
 #include "dkv_paged.h"
+#include <stdio.h>
 #include <algorithm>
 #include <initializer_list>
 #include <map>
@@ -501,7 +502,13 @@ int dkv_pool_truncate(dkv_pool* pool, int64_t seq, int64_t length, void* arena, 
       const int c = s->pages[keep - 1] & 3;
       int64_t need[3] = {};
       need[c] = 1;
-      if (int rc = p.make_room(need, arena, stream, what)) return rc;
+      // (The copy is made before anything is freed, so that a launch that fails has changed nothing.)
+      int64_t first = held;  // the least length whose cut needs no copy
+      for (size_t j = keep - 1; s->rows[j] < TILE && p.refs[s->pages[j] >> 2] > 1;) first += s->rows[++j];
+      char why[160];
+      snprintf(why, sizeof why, first < s->length ? "%s (copies a page that others hold, then frees; cut to %lld first)" : "%s (copies a page that others hold)",
+               what, (long long)first);
+      if (int rc = p.make_room(need, arena, stream, why)) return rc;
       const uint32_t old = s->pages[keep - 1], page = p.take(c);
       const dkv_page_move move{p.offset(old), p.offset(page), TILE, 0, 0, (uint8_t)last, (uint8_t)(4 << c), {}};
       if (int rc = launch_moves(arena, arena, &move, 1, p.layers, p.heads, stream)) {

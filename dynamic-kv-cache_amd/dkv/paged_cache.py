@@ -232,7 +232,8 @@ class PagedCache:
             _lib.check(rc, 'dkv_pool_free')
 
     def truncate(self, seq, length):
-        """Drops a sequence's tokens from `length` on."""
+        """Drops a sequence's tokens from `length` on. A cut within a page that other sequences hold copies what stays of it
+        before it frees the pages behind; a cache without room for the copy refuses it, and says which cut comes first."""
         (seq,), _ = self._ids([seq])
         length = self._whole(length, 'truncate')
         if not 0 <= length < IDS:

@@ -639,7 +639,8 @@ int dkv_pool_adopt(dkv_pool* pool, const void* src, int64_t src_bytes, const dkv
                    int64_t tokens, int64_t dropped, void* arena, void* stream, int64_t* seq);
 int dkv_pool_fork(dkv_pool* pool, int64_t seq, int32_t n, void* arena, void* stream, int64_t* out);
 int dkv_pool_free(dkv_pool* pool, const int64_t* seqs, int32_t n);
-/* Drops a sequence's tokens from `length` on. */
+/* Drops a sequence's tokens from `length` on. A cut within a page that other sequences hold copies what stays of it before it frees the
+ * pages behind: without room for the copy it is refused, and the error names the length to cut to first, which frees without one. */
 int dkv_pool_truncate(dkv_pool* pool, int64_t seq, int64_t length, void* arena, void* stream);
 /* Brings the pages of each width together into as few blocks as hold them. */
 int dkv_pool_compact(dkv_pool* pool, void* arena, void* stream, int64_t* moved);
