@@ -6,8 +6,8 @@
 // whatever the lengths (dkv_paged.hip), and partial rows are joined by merge_kernel. Per half page and wave: keys straight from
 // global memory into the operands of S^T = K Q^T (16x16x32 bf16), whose result lies where O^T = V^T P^T reads P^T, values into V^T's.
 // No LDS but for scales and the waves' join.
-// Weights: sums and statistics in 32 bits; P is the sum of two bf16 values (2^-16) for a bf16 output, of three (2^-24) for fp32.
-// At precision bf16 a packed value is rounded to bf16, GPUCache's rounding; at fp32 its code is multiplied and its scale and offset
+// Weights: sums and statistics in 32 bits; P is the sum of two bf16 values (2^-16) at precision and output bf16, of three (2^-24) at
+// fp32 of either. At precision bf16 a packed value is rounded to bf16, GPUCache's rounding; at fp32 its code is multiplied and its scale and offset
 // come apart.
 // What bounds it: long histories their bytes, six of 30k to 131k tokens of 8 heads at fp32 506 MB in 100 us (5.0 TB/s, of a large
 // copy's 5.2), a token of each of 64 streams of 300 to 8128 tokens 107 MB in 27 us; short ones the chain of loads of one launch

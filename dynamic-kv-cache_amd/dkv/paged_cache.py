@@ -299,7 +299,9 @@ class PagedCache:
     def attend(self, q, k, v, layer, step, out_dtype=None, precision=None):
         """Causal attention of the step's tokens, q [1, q_heads, tokens, 64], each over its sequence's history and the
         sequence's new tokens k, v [1, heads, tokens, 64] up to itself (these as they are, not as they are packed;
-        append() may come before or after). Returns [1, tokens, q_heads, 64] in out_dtype (default q's)."""
+        append() may come before or after). Returns [1, tokens, q_heads, 64] in out_dtype (default q's). At precision and output
+        bf16 weights have 16 bits, and are rounded to bf16 where more than 160 query rows of a KV head attend together (a prompt, or
+        tokens of branches that stand next to each other, over the pages that these share); at fp32 of either 24."""
         precision = precision or self.precision
         if precision not in PRECISIONS:
             raise ValueError(f'precision must be one of {sorted(PRECISIONS)}')

@@ -569,7 +569,11 @@ typedef struct dkv_paged_args {
   void* out; /* [tokens, q_heads, 64] with the strides below */
   int64_t out_tok_stride, out_head_stride;
   int32_t out_dtype; /* 0 = bf16, 1 = fp32 */
-  int32_t precision; /* 0: packed rows' values are rounded to bf16; 1: taken as they are stored */
+  int32_t precision; /* 0: packed rows' values are rounded to bf16; 1: taken as they are stored. A weight is kept in 24 bits
+                        at precision 1 or fp32 output, else in 16, but rounded to bf16 (dkv_attn_args' precision 0) for a
+                        sequence of more than 160 query rows (tokens times query heads) of a KV head, and for the pages
+                        that neighbours in the step share where these have as many together: a token's weights of shared
+                        pages depend on how many branches attend with it. */
   void* workspace;
   int64_t workspace_bytes;
 } dkv_paged_args;
