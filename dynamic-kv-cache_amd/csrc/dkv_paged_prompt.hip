@@ -141,13 +141,13 @@ __global__ __launch_bounds__(64 * WAVES, 4) void long_kernel(dkv_paged_args a, i
   const uint8_t* const base = static_cast<const uint8_t*>(a.arena);
   const int64_t grain = grain_bytes(a.plan.layers, H), sub = (int64_t)a.layer * 2 * H + h;
   // Rows of 16 bits go straight to their tile: a wave 8 rows of K and of V. New rows past the last one repeat it; rows of a
-  // page that are not there are read as they are (zero_values).
-  auto load_rows = [&](const uint8_t* k, const uint8_t* v, int rows, uint32_t k_stride, uint32_t v_stride, int buf) {
+  // page that are not there are read as they are (zero_values). New rows are attended to without scales.
+  auto load_rows = [&](auto of_page, const uint8_t* k, const uint8_t* v, int rows, uint32_t k_stride, uint32_t v_stride, int buf) {
     const int thread = anew(t), srow = thread >> 3, piece = (thread & 7) ^ place(srow), r = min(srow, rows - 1);
     const uint32_t to = tile0 + buf * (2 * TILE_BYTES) + 1024 * wave;
     load_piece_at(k, 16 * piece + __umul24(r, k_stride), to);
     load_piece_at(v, 16 * piece + __umul24(r, v_stride), to + TILE_BYTES);
-    if (PREC && (thread & 7) == 0) scales[buf][0][srow] = scales[buf][1][srow] = make_float2(0.f, 1.f);
+    if (PREC && of_page && (thread & 7) == 0) scales[buf][0][srow] = scales[buf][1][srow] = make_float2(0.f, 1.f);
   };
   const uint32_t kn_stride = (uint32_t)(2 * a.kn_tok_stride), vn_stride = (uint32_t)(2 * a.vn_tok_stride);  // (of a single row, whatever it is)
   auto new_rows = [&](const void* x, int64_t head_stride, int64_t tok_stride, int u) {
@@ -156,10 +156,10 @@ __global__ __launch_bounds__(64 * WAVES, 4) void long_kernel(dkv_paged_args a, i
   auto load_tile = [&](int u, const Unit& x, int buf) {
     if (u < w.n_pages) {
       const uint8_t* k = base + (x.page >> 2) * grain + sub * page_sub(16);
-      load_rows(k, k + (int64_t)H * page_sub(16), TILE, 128, 128, buf);
+      load_rows(std::true_type(), k, k + (int64_t)H * page_sub(16), TILE, 128, 128, buf);
     } else {
-      load_rows(new_rows(a.k_new, a.kn_head_stride, a.kn_tok_stride, u), new_rows(a.v_new, a.vn_head_stride, a.vn_tok_stride, u), x.rows,
-                kn_stride, vn_stride, buf);
+      load_rows(std::false_type(), new_rows(a.k_new, a.kn_head_stride, a.kn_tok_stride, u),
+                new_rows(a.v_new, a.vn_head_stride, a.vn_tok_stride, u), x.rows, kn_stride, vn_stride, buf);
     }
   };
   // Packed rows come as they are: at 8 bits a wave 1 KB of K (waves 0 to 3) or V, at 4 bits every other wave, and one wave
@@ -395,7 +395,7 @@ __global__ __launch_bounds__(64 * WAVES, 4) void long_kernel(dkv_paged_args a, i
     const int next = buf + 1 == RING ? 0 : buf + 1, after = next + 1 == RING ? 0 : next + 1;
     const int first = (u - w.n_pages) * TILE;
     const bool more = u + 2 < w.u1;
-    if (more) load_rows(kn, vn, w.count - first - 2 * TILE, kn_stride, vn_stride, after);
+    if (more) load_rows(std::false_type(), kn, vn, w.count - first - 2 * TILE, kn_stride, vn_stride, after);
     kn += 2 * TILE * a.kn_tok_stride, vn += 2 * TILE * a.vn_tok_stride;
     if (first + TILE - 1 > first_token) zero_values(Unit{16, min(TILE, w.count - first), 0, 0}, tiles[buf][1], true);
     if (on && first <= m_last) attend(std::false_type(), buf, first + TILE - 1 > m_first, m_new + 1 - first, m_last - first < 32);
