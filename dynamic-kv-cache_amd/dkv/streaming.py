@@ -26,6 +26,8 @@ place of the vision encoder:
 The model is a random-init LlamaForCausalLM. There is no checkpoint, and the
 workloads are synthetic; see dkv.workloads.decoder_config.
 """
+import contextlib
+
 import torch
 
 from .gpu_cache import GPUCache, install_packed_attention
@@ -513,6 +515,10 @@ class StreamingDecoder:
         out = torch.cat(tokens)
         return out.masked_fill((out < 0).cumsum(0) > 0, -1)
 
+    def _current(self):
+        """The decoder's device as the current one: where a capture records and the fused layers launch."""
+        return torch.cuda.device(self.device) if self.device.type == 'cuda' else contextlib.nullcontext()
+
     def _paged_forward(self, step, ids, last):
         """fp32 logits [sequences, vocabulary] of a step's tokens ids [1, tokens] at the places `last` of them."""
         out = self.text(inputs_embeds=self.text.get_input_embeddings()(ids), past_key_values=step, use_cache=True,
@@ -546,7 +552,8 @@ class StreamingDecoder:
             counts = [x.shape[1] for x in questions]
             last = torch.tensor(counts).cumsum(0).sub(1).to(self.device)
             ids = torch.cat([x.to(self.device) for x in questions], dim=1)
-            with pages.lock:  # (a plan and the launches over it: another thread's call frees or moves no pages between the two)
+            # (a plan and the launches over it: another thread's call frees or moves no pages between the two)
+            with pages.lock, self._current():
                 step = pages.step(branches, counts)
                 logits = self._paged_forward(step, ids, last)
             n, last = u.shape[1], slice(None)
@@ -555,7 +562,7 @@ class StreamingDecoder:
                 if i + 1 == n:
                     break
                 ids = tokens[-1][None].clamp(min=0)  # (-1 is no index into the embeddings)
-                with pages.lock:
+                with pages.lock, self._current():
                     step = step.advance() if i else pages.step(branches, reserve=n)
                     if graph is not None:
                         held.copy_(ids)
