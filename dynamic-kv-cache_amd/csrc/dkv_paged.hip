@@ -91,7 +91,8 @@ __global__ __launch_bounds__(256) void append_kernel(dkv_paged_args a) {
 
 // The joined projection's rows [q | k | v] of one item and head: rotated (Q and K heads; V rows keep their input), stored,
 // and for K and V heads packed. 8 lanes a row as above; rotate_half pairs lane c with lane c ^ 4. (A token of each of 4 / 48
-// sequences, 15 + 2 * 5 heads: one launch of 3.6 / 3.8 us in place of RoPE's 2.8 / 3.2 and the pack's 2.5 / 3.2.)
+// sequences, 15 + 2 * 5 heads: one launch of 3.6 / 3.8 us in place of RoPE's 2.8 / 3.2 and the pack's 2.5 / 3.2; 24 prompts of 6503 tokens
+// together 18.4 us, 48 MB at 2.6 TB/s, in place of 21.2 for both.)
 template <int BITS>
 __device__ __forceinline__ void rope_rows(const uint16_t* src, int64_t src_stride, const uint16_t* cosv, const uint16_t* sinv, int64_t cs_stride,
                                           int rows, int r0, int c, bool is_v, uint16_t* dst, int64_t dst_stride, uint8_t* sub, int row0) {
@@ -264,9 +265,11 @@ int launch_moves(const void* src, void* dst, const dkv_page_move* moves, int n_m
 
 // ---- plans -------------------------------------------------------------------------------------------------------
 
-// Entities of up to this many query rows of a KV head go to the kernel for few rows. (144 rows over 127 pages, 5 heads: 18.5 us
-// there, 24.2 in the kernel for many, which has few workgroups for them; 16 questions of 15 to 180 rows about 96 pages, few rows in a
-// launch of their own, 40.6 us by this rule, 43.5 from 100 rows on, 40.9 from 200.)
+// Entities of up to this many query rows of a KV head go to the kernel for few rows. In us there / in the kernel for many, single tokens
+// of branches: 5 heads of 3 over 127 pages in common, bf16, 96 rows 15.5 / 16.8, 144 19.1 / 19.4, 162 21.3 / 20.0, 258 28.0 / 25.3; 8 heads of
+// 4 over 32 pages 96 rows 12.6 / 12.7, 164 16.3 / 14.8, 320 22.0 / 22.2; over 625 pages 96 rows 41.2 / 33.6, 162 61.7 / 39.7. At precision 1,
+// whose kernel for many splits weights in three, few rows stay ahead for longer: 162 rows over the 127 pages 20.5 / 28.1, 321 30.6 / 35.1.
+// 16 questions of 15 to 180 rows about 96 pages, few rows in a launch of their own: 40.6 us by this rule, 43.5 from 100 rows on, 40.9 from 200.
 constexpr int SHORT_ROWS = 160;
 // Few rows (four waves, a unit each at a time): about SHORT_TARGET workgroups over all KV heads share a step's units, four
 // resident a CU, of SHORT_LEAST units at least (three short histories 8.4 us with 8, 12.1 with 4 and a join). A token of 64

@@ -13,11 +13,11 @@
 // of each weight, averaged over the keys; a sequence of few rows keeps two, dkv_paged_short.h), else the sum of three
 // (at precision fp32 for either output: a weight meets a code that is up to half a row's range from its offset, whatever is left of
 // the two).
-// What bounds it: the vector units, some 150 instructions a unit and wave beside its 16 matrix products of 32 cycles, of them 32
-// exponentials of twice the cost or more: 12.5k tokens of prompts of 5 heads of 3 205 us (806 TFLOP/s, 61 % of a large product's), 12
-// prompts of up to 2048 tokens of 8 heads of 4 55 us (631); with few units a workgroup the chain from the plan to the first tile, 16
+// What bounds it: the vector units, some 180 instructions a unit and wave beside its 16 matrix products of 32 cycles, of them 32
+// exponentials of twice the cost or more: 12.5k tokens of prompts of 5 heads of 3 209 us (791 TFLOP/s, 60 % of a large product's; vector units busy 62 % of the time, matrix units 35), 12
+// prompts of up to 2048 tokens of 8 heads of 4 56 us (615); with few units a workgroup the chain from the plan to the first tile, 16
 // questions about 6144 shared tokens 27 us. At fp32 the split into three values and the scales apart, some 500 instructions a unit
-// and wave: 8 frames of 78 tokens over 92k 71 us.
+// and wave: 8 frames of 78 tokens over 92k 71 us (62 and 23 %).
 
 #include <type_traits>
 

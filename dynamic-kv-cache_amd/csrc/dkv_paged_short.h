@@ -12,7 +12,7 @@
 // What bounds it: long histories their bytes, six of 30k to 131k tokens of 8 heads at fp32 506 MB in 100 us (5.0 TB/s, of a large
 // copy's 5.2), a token of each of 64 streams of 300 to 8128 tokens 107 MB in 27 us; short ones the chain of loads of one launch
 // (three of up to 333 tokens 7.5 us); branches the unpacking of shared pages once for each 16 of their rows (48 of 8128 shared
-// tokens 15.5 us).
+// tokens 15.8 us).
 #pragma once
 #include "dkv_rows.h"
 #include "dkv_paged.h"

@@ -34,8 +34,9 @@ from .gpu_cache import GPUCache, install_packed_attention
 from .gpu_ops import install_fused_ops, sample
 from .paged_cache import PagedCache
 
-# generate_batch() captures more tokens than these: a replayed forward of a token of each sequence takes 1.3 ms and an eager one,
-# which waits for the host, 1.6 (32 layers, 1 to 16 questions; at 64 both take 1.8), a capture 3 to 5 ms.
+# generate_batch() captures more tokens than these: a replayed forward of a token of each sequence takes 1.30 to 1.37 ms and an eager
+# one, which waits for the host, 1.6 (32 layers, 1 to 16 questions; at 64 1.81 and 1.66, its launches are sized for any step), a capture 3
+# to 8 ms.
 GRAPH_TOKENS = 16
 MFMA_ROWS = 192  # query rows per frame-chunk attention workgroup (MFMA_ROWS of csrc/dkv_attn_common.h)
 
