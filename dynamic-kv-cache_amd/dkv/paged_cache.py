@@ -86,9 +86,9 @@ class PagedCache:
         """Torch's current stream on this cache's device."""
         return _lib.raw_stream(self._index) if self._index >= 0 else 0
 
-    def _planned(self, what, step):
-        if step.generation != self._generation.value:
-            raise ValueError(f'{what}: pages were freed, cut or moved since this step was planned')
+    @staticmethod
+    def _over(what):
+        raise ValueError(f'{what}: pages were freed, cut or moved since this step was planned')
 
     def _launch(self, what, call, stream=None, step=None):
         """call(stream) on this cache's device and torch's current stream there, over `step` if that is given."""
@@ -98,8 +98,8 @@ class PagedCache:
         if stream is None:
             stream = _lib.raw_stream(index)
         with self.lock:
-            if step is not None:
-                self._planned(what, step)
+            if step is not None and step.generation != self._generation.value:
+                self._over(what)
             if torch.cuda.current_device() == index:
                 rc = call(stream)
             else:
@@ -277,7 +277,8 @@ class PagedCache:
     def _check(self, what, step, layer, tensors):
         if not isinstance(step, PagedStep) or step.cache is not self:
             raise ValueError(f'{what} expects a step of this cache')
-        self._planned(what, step)
+        if step.generation != self._generation.value:
+            self._over(what)
         if not 0 <= layer < self.layers:
             raise ValueError(f'{what}: layer {layer} of {self.layers}')
         for x, heads in tensors:
@@ -471,7 +472,8 @@ class PagedStep(_CacheBase):
         args = _ARGS.pack(qkv_out, head, d, kp, head, d, vp, head, d, c._arena_ptr, c.arena_bytes, self.device_plan(here), self.plan_bytes,
                           layer, bounds, d ** -0.5, out, q_heads * d, d, 0, PRECISIONS[c.precision], at if need else 0, need)
         with c.lock:
-            c._planned('attend', self)
+            if self.generation != c._generation.value:
+                c._over('attend')
             rc = (lib.dkv_linear_tiled(x, x_stride, weight, w_stride, n, width, k, norm, eps, 0, None, 0, at, width, layout, stream)
                   or lib.dkv_paged_rope_append(args, at, width, cos, sin, cs_stride, stream) or lib.dkv_paged_attend(args, stream))
         if rc:
