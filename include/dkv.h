@@ -588,10 +588,12 @@ int dkv_paged_append(const dkv_paged_args* args, void* stream);
 int dkv_paged_rope_append(const dkv_paged_args* args, const void* qkv, int64_t qkv_row_stride, const void* cos, const void* sin,
                           int64_t cs_row_stride, void* stream);
 
-/* The step's new tokens attend, each to its sequence's history before the step and to the sequence's new tokens up to
- * itself (these as they are in k_new and v_new). What later tokens hold, NaN and infinities included, does not reach
- * a query; an infinite value that it sees gives the formula's infinity or NaN. Q, K and V must be 16-byte aligned with strides in multiples of 8 elements; out 16-byte aligned with
- * strides in multiples of 4 elements, in memory of its own. */
+/* The step's new tokens attend, each to its sequence's history before the step and to the sequence's new tokens up
+ * to itself (these as they are in k_new and v_new). What later tokens hold, NaN and infinities included, does not
+ * reach a query; an infinite value that it sees gives the formula's infinity or NaN. Scores times scale are below
+ * 2^30 in magnitude: past that their exponents' rounding leaves fp32's range. Q, K and V must be 16-byte aligned
+ * with strides in multiples of 8 elements; out 16-byte aligned with strides in multiples of 4 elements, in memory
+ * of its own. */
 int64_t dkv_paged_workspace_bytes(const dkv_paged_args* args);
 int dkv_paged_attend(const dkv_paged_args* args, void* stream);
 
@@ -613,12 +615,13 @@ typedef struct dkv_page_move {
 int dkv_paged_move(const void* src, int64_t src_bytes, void* dst, int64_t dst_bytes, const dkv_page_move* moves,
                    int32_t n_moves, int32_t layers, int32_t heads, void* stream);
 
-/* The pages of an arena and the sequences that hold them: host bookkeeping for the calls above, with the launches that
- * move or read rows. Each call takes the pool's lock, its launches too, so threads that share a stream may call at once. The
- * launches over a plan know no pool: with several threads the caller holds a lock of its own over the look at the generation
- * and the launch, and over the calls that change it (dkv_pool_step, adopt and fork too, where they make room). Sequences are named by numbers that are not used again. Where a call
- * takes `arena` and `stream` it may move pages, also to bring them together where a new page finds too little room;
- * with a null arena nothing is moved (bookkeeping alone). A call that fails changes no sequence. */
+/* The pages of an arena and the sequences that hold them: host bookkeeping for the calls above, with the launches
+ * that move or read rows. Each call takes the pool's lock, its launches too, so threads that share a stream may
+ * call at once. The launches over a plan know no pool: with several threads the caller holds a lock of its own
+ * over the look at the generation and the launch, and over the calls that change it (dkv_pool_step, adopt and fork
+ * too, where they make room). Sequences are named by numbers that are not used again. Where a call takes `arena`
+ * and `stream` it may move pages, also to bring them together where a new page finds too little room; with a null
+ * arena nothing is moved (bookkeeping alone). A call that fails changes no sequence. */
 typedef struct dkv_pool dkv_pool;
 typedef struct dkv_pool_info {
   int64_t grain, blocks, free_blocks; /* bytes of a grain; blocks of 48 grains, which hold 9, 5 or 3 pages of one width */
@@ -643,8 +646,9 @@ int dkv_pool_adopt(dkv_pool* pool, const void* src, int64_t src_bytes, const dkv
                    int64_t tokens, int64_t dropped, void* arena, void* stream, int64_t* seq);
 int dkv_pool_fork(dkv_pool* pool, int64_t seq, int32_t n, void* arena, void* stream, int64_t* out);
 int dkv_pool_free(dkv_pool* pool, const int64_t* seqs, int32_t n);
-/* Drops a sequence's tokens from `length` on. A cut within a page that other sequences hold copies what stays of it before it frees the
- * pages behind: without room for the copy it is refused, and the error names the length to cut to first, which frees without one. */
+/* Drops a sequence's tokens from `length` on. A cut within a page that other sequences hold copies what stays of
+ * it before it frees the pages behind: without room for the copy it is refused, and the error names the length to
+ * cut to first, which frees without one. */
 int dkv_pool_truncate(dkv_pool* pool, int64_t seq, int64_t length, void* arena, void* stream);
 /* Brings the pages of each width together into as few blocks as hold them. */
 int dkv_pool_compact(dkv_pool* pool, void* arena, void* stream, int64_t* moved);
